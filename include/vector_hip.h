@@ -393,6 +393,62 @@ int vhip_ivfpq_file_info(const char *path, vhip_ivfpq_config *cfg, size_t *dim, 
 int vhip_ivfpq_file_load(const char *path, float *coarse, float *codebooks, uint32_t *list_sizes, uint32_t *ids,
                          uint8_t *codes);
 
+/* ---- training operators (no reference counterpart) -------------------------------------
+ * What trains the vectors that the engines above search: layer norm, softmax cross entropy against a whole
+ * table of vectors, and the orthogonalisation of an update.  They differ from the engines in three ways.
+ *  * Inputs and outputs are device memory of GPU `ordinal`; rows are `ld` elements apart, and an output
+ *    overlaps no other argument.
+ *  * Work is enqueued on `stream` (a hipStream_t, NULL the default stream) and the call returns without
+ *    waiting for it.  Nothing is allocated: working memory is the caller's (`workspace`, of at least the
+ *    bytes the ..._workspace function gives for the same sizes, aligned to 16 bytes), in use until the
+ *    enqueued work has run.  A call may be captured into a graph.
+ *  * The calling thread's current device is left as it was.
+ * Sums, statistics and softmax are in 32 bits or more, and no result depends on timing. */
+#define VHIP_DTYPE_F32  0
+#define VHIP_DTYPE_F16  1
+#define VHIP_DTYPE_BF16 2
+
+/* y = (x - mean) rstd weight + bias over the rows of x, rstd = 1 / sqrt(variance + eps).  weight, bias (dim
+ * values of param_dtype, which is dtype or f32), mean and rstd (`rows` floats) may be NULL. */
+int vhip_layer_norm(int ordinal, int dtype, int param_dtype, const void *x, size_t rows, size_t dim, size_t ldx,
+                    const void *weight, const void *bias, float eps, void *y, size_t ldy, float *mean, float *rstd,
+                    void *stream);
+/* Gradients from that of y and the statistics of the forward call: dx, dweight and dbias (param_dtype); each
+ * may be NULL, and without dweight and dbias so may the workspace. */
+size_t vhip_layer_norm_backward_workspace(size_t rows, size_t dim);
+int vhip_layer_norm_backward(int ordinal, int dtype, int param_dtype, const void *dy, size_t lddy, const void *x,
+                             size_t ldx, const void *weight, const float *mean, const float *rstd, size_t rows,
+                             size_t dim, void *dx, size_t lddx, void *dweight, void *dbias, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of `rows` rows h against all table_rows rows of a table:
+ *   z_tv = scale <h_t, table_v> + bias_v,  lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_{t, target_t}.
+ * bias (table_rows floats, may be NULL) is a constant, such as the log of the rate at which an entry is drawn
+ * taken off; -inf leaves an entry out, whatever its values.  A row with a negative target has loss 0; one
+ * whose target is left out, or with every entry left out, +inf; one whose target is past the table NaN.
+ * loss and lse may be NULL.  dim <= 65536, table_rows <= 2^23 - 64.  The logits are not kept. */
+size_t vhip_softmax_xent_workspace(int dtype, size_t rows, size_t table_rows, size_t dim, int gradients);
+int vhip_softmax_xent(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table, size_t table_rows,
+                      size_t ldt, size_t dim, const int64_t *target, const float *bias, float scale, float *loss,
+                      float *lse, void *workspace, size_t workspace_bytes, void *stream);
+/* The same with the gradients of sum_t row_weight_t loss_t (row_weight NULL: all 1) for h and for the table
+ * (either may be NULL).  A row with a negative target has no part in them, whatever h holds there, and
+ * neither has one whose loss is +inf as above.  Rows are taken in pieces that keep the working memory for the
+ * logits' gradient below 4 GiB; the environment variable VHIP_XENT_PIECE_BYTES sets another limit. */
+int vhip_softmax_xent_grad(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table,
+                           size_t table_rows, size_t ldt, size_t dim, const int64_t *target, const float *bias,
+                           const float *row_weight, float scale, float *loss, float *lse, void *dh, size_t lddh,
+                           void *dtable, size_t lddt, void *workspace, size_t workspace_bytes, void *stream);
+
+/* `steps` Newton-Schulz steps on each of `count` matrices (stride elements apart):
+ *   X = M / (|M|_F + eps);  A = X X^T, X <- a X + (b A + c A A) X   (on M^T where rows > cols),
+ * which moves the singular values towards one.  The coefficients have to keep X bounded (singular values
+ * below 32). */
+size_t vhip_orthogonalize_workspace(size_t count, size_t rows, size_t cols);
+int vhip_orthogonalize(int ordinal, int dtype, const void *in, size_t count, size_t rows, size_t cols, size_t ld_in,
+                       size_t stride_in, int steps, float a, float b, float c, float eps, void *out, size_t ld_out,
+                       size_t stride_out, void *workspace, size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -1,0 +1,729 @@
+// softmax_xent.hip -- softmax cross entropy of rows against every row of a table, and its gradients.
+//
+//   z_tv = scale <h_t, w_v> + b_v,  lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_{t, y_t}
+//   G_tv = c_t scale (exp(z_tv - lse_t) - [v = y_t]),  dh = G W,  dW = G^T h      (c: weights of the rows)
+//
+// The logits are never kept.  A first product (mm16.h) ends each 128-entry piece of a row's logits in its
+// largest value and the sum of exp about it; a small kernel joins the pieces.  For the gradients a second
+// product makes the same logits again and ends in G, which two more products multiply with the table and
+// with the rows.  Rows are taken in pieces so that G stays below kPieceBytes; from the second piece on the
+// table's gradient is added up in 32 bits.  Every sum has a fixed order: results do not depend on timing.
+//
+// Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as two float16 planes
+// (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
+// plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
+// operands), which is as far as the gradients that are returned are rounded too.  In float16 it is held
+// times 2^14 / 2^e, where 2^e is the power of two above the largest weight times scale: |G| is then at most
+// 2^14 and small probabilities keep their bits; the products' epilogues take the factor out again.
+//
+// What does not count: a row whose target is negative has loss 0 and no part in the gradients, whatever its
+// values (its h is replaced by zeros where sums over rows are made).  An entry whose bias is -inf is out of
+// the softmax whatever its values.  A row whose target is out, or that has nothing left in, has loss +inf
+// and no part in the gradients.  A target past the table gives NaN.
+#include "mm16.h"
+
+#include <cmath>
+#include <cstdlib>
+
+namespace vh {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G in both orders
+constexpr int kGBits = 14;
+
+// State of a call on the device.
+struct Scalars {
+    uint32_t amax_h, amax_w;  // bits of the largest finite |value|
+    uint32_t cmax;            // bits of the largest |weight x scale| of a row that counts
+};
+
+// 2^(14 - e) with 2^e > x >= 2^(e-1), so that x times it is in [2^13, 2^14); 1 for 0.
+__device__ __forceinline__ float unit_scale(uint32_t bits) {
+    const int e = (int)(bits >> 23) - 126;  // x < 2^e
+    if (bits == 0) return 1.f;
+    int k = kGBits - e;
+    k = k > 120 ? 120 : (k < -120 ? -120 : k);
+    return ldexpf(1.f, k);
+}
+
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// exp to 32-bit accuracy: what x log2(e) loses in rounding is put back to first order
+__device__ __forceinline__ float exp_fine(float x) {
+    const float t = x * kLog2e;
+    const float r = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t > -150.f && t < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
+}
+
+__global__ void k_xent_init(Scalars *s) {
+    if (threadIdx.x == 0) *s = Scalars{0, 0, 0};
+}
+
+__global__ __launch_bounds__(256) void k_amax(const float *x, size_t rows, int dim, size_t ld, uint32_t *out) {
+    uint32_t m = 0;
+    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        for (int c = threadIdx.x; c < dim; c += 256) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, x[r * ld + c]) & 0x7fffffffu;
+            if (u < 0x7f800000u && u > m) m = u;
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_xor(m, o, 64);
+        m = v > m ? v : m;
+    }
+    if ((threadIdx.x & 63) == 0) atomicMax(out, m);
+}
+
+// Planes of an operand: T itself, or hi and lo of a float times its scale.
+template <class T>
+struct Planes {
+    typedef T type;
+    static constexpr int count = 1;
+};
+template <>
+struct Planes<float> {
+    typedef half_t type;
+    static constexpr int count = 2;
+};
+
+// rows x dim -> planes of rows x kp, zeros past dim.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
+                                              size_t plane, int kp, const uint32_t *amax) {
+    const size_t n = rows * (kp / 8);
+    float sc = 1.f;
+    if constexpr (Planes<T>::count == 2) sc = unit_scale(*amax);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / (kp / 8);
+        const int c = (int)(i % (kp / 8)) * 8;
+        Pack<typename Planes<T>::type, 8> hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const T v = c + e < dim ? x[r * ld + c + e] : (T)0.f;
+            if constexpr (Planes<T>::count == 2) {
+                const float f = v * sc;
+                hi.v[e] = (half_t)f;
+                lo.v[e] = (half_t)(f - (float)hi.v[e]);
+            } else {
+                hi.v[e] = v;
+            }
+        }
+        *reinterpret_cast<Pack<typename Planes<T>::type, 8> *>(out + r * kp + c) = hi;
+        if constexpr (Planes<T>::count == 2)
+            *reinterpret_cast<Pack<typename Planes<T>::type, 8> *>(out + plane + r * kp + c) = lo;
+    }
+}
+
+// rows x dim -> planes of dim x rp, zeros past rows.  Rows that do not count are zeros: those with a
+// negative target (`target`) or a bias of -inf (`bias`).
+template <class T>
+__global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim, size_t ld,
+                                                typename Planes<T>::type *out, size_t plane, size_t rp,
+                                                const uint32_t *amax, const int64_t *target, const float *bias) {
+    __shared__ T tile[64][65];
+    const size_t r0 = (size_t)blockIdx.x * 64;
+    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const size_t r = r0 + ty + 4 * i;
+        const int c = c0 + tx;
+        T v = (T)0.f;
+        if (r < rows && c < dim && !(target && target[r] < 0) && !(bias && bias[r] == -INFINITY)) v = x[r * ld + c];
+        tile[ty + 4 * i][tx] = v;
+    }
+    __syncthreads();
+    float sc = 1.f;
+    if constexpr (Planes<T>::count == 2) sc = unit_scale(*amax);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int c = c0 + ty + 4 * i;
+        const size_t r = r0 + tx;
+        if (c < dim && r < rp) {
+            const T v = tile[tx][ty + 4 * i];
+            if constexpr (Planes<T>::count == 2) {
+                const float f = v * sc;
+                const half_t h = (half_t)f;
+                out[c * rp + r] = h;
+                out[plane + c * rp + r] = (half_t)(f - (float)h);
+            } else {
+                out[c * rp + r] = v;
+            }
+        }
+    }
+}
+
+// What turns a product's sum into a logit.
+struct Logits {
+    const float *bias;
+    const Scalars *sc;
+    float scale;
+    bool split;
+    __device__ __forceinline__ float factor() const {
+        return split ? scale / unit_scale(sc->amax_h) / unit_scale(sc->amax_w) : scale;
+    }
+};
+__device__ __forceinline__ float logit(float acc, float f, float b) {
+    return b == -INFINITY ? -INFINITY : fmaf(acc, f, b);
+}
+
+// Epilogue of the first product (A: table, B: rows): a wave's 16 MB entries of each row end in one piece.
+struct StatEpi {
+    Logits lg;
+    float2 *part;  // [piece][rows]: largest logit, sum of exp about it
+    float *zt;     // the target's logit
+    const int64_t *target;
+    int rows, table;
+    template <int MB, int NB>
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &) const {
+        if (m >= table) return;
+        const int l = threadIdx.x & 63, q = l >> 4;
+        const float f = lg.factor();
+        const int piece = m / (16 * MB);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int t = n + 16 * j + (l & 15);
+            const bool in = t < rows;
+            const int64_t y = in ? target[t] : -1;
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = m + 16 * i + 4 * q + e;
+                    float z = -INFINITY;
+                    if (v < table) {
+                        z = logit(acc[i][j][e], f, lg.bias ? lg.bias[v] : 0.f);
+                        if (v == y) zt[t] = z;
+                    }
+                    acc[i][j][e] = z;
+                    top = fmaxf(top, z);
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float about = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += exp_neg(acc[i][j][e] - about);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
+        }
+    }
+};
+
+// Joins the pieces: 16 rows a workgroup, 16 lanes of a row each taking every sixteenth piece.
+__global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float *zt,
+                                                   const int64_t *target, int64_t table, const float *weight,
+                                                   float scale, float *loss, float *lse, float2 *stat,
+                                                   float *rowfac, Scalars *sc) {
+    __shared__ float s_top[16][17], s_sum[16][17];
+    const int k = threadIdx.x & 15, g = threadIdx.x >> 4, t = blockIdx.x * 16 + k;
+    float top = -INFINITY, sum = 0.f;
+    if (t < rows) {
+        for (int p = g; p < pieces; p += 16) {
+            const float2 v = part[(size_t)p * rows + t];
+            const float m = fmaxf(top, v.x), about = m == -INFINITY ? 0.f : m;
+            sum = sum * exp_neg(top - about) + v.y * exp_neg(v.x - about);
+            top = m;
+        }
+    }
+    s_top[g][k] = top;
+    s_sum[g][k] = sum;
+    __syncthreads();
+    if (g != 0) return;
+    for (int p = 1; p < 16; ++p) top = fmaxf(top, s_top[p][k]);
+    const float about = top == -INFINITY ? 0.f : top;
+    sum = 0.f;
+    for (int p = 0; p < 16; ++p) sum += s_sum[p][k] * exp_neg(s_top[p][k] - about);
+    const float L = sum == 0.f ? -INFINITY : about + logf(sum);
+    const int64_t y = t < rows ? target[t] : -1;
+    float ls = 0.f, fac = 0.f;
+    if (y >= table) {
+        ls = fac = NAN;
+    } else if (y >= 0) {
+        const float z = zt[t];
+        const bool out = L == -INFINITY || z == -INFINITY;
+        ls = out ? INFINITY : about - z + logf(sum);  // not lse - z, which cancels where the loss is small
+        if (!out) fac = (weight ? weight[t] : 1.f) * scale;
+    }
+    if (t < rows) {
+        if (loss) loss[t] = ls;
+        if (lse) lse[t] = L;
+        if (rowfac) {
+            stat[t] = make_float2(about, 1.f / sum);
+            rowfac[t] = fac;
+        }
+    }
+    if (rowfac) {
+        uint32_t u = __builtin_bit_cast(uint32_t, fac) & 0x7fffffffu;
+        if (u >= 0x7f800000u) u = 0;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const uint32_t v = __shfl_xor(u, o, 16);
+            u = v > u ? v : u;
+        }
+        if (k == 0 && u) atomicMax(&sc->cmax, u);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_zero_rows(char *p, size_t rows, size_t row_bytes, size_t ld_bytes) {
+    for (size_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (size_t i = threadIdx.x; i < row_bytes; i += 256) p[r * ld_bytes + i] = 0;
+}
+
+// Epilogue of the second product: G in both orders.
+template <class G>  // element type of G's planes
+struct GradEpi {
+    Logits lg;
+    const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
+    const float *rowfac;
+    const int64_t *target;
+    G *g, *gt;  // [rows][vp], [table][tp]
+    size_t g_plane, gt_plane;
+    size_t vp, tp;
+    int rows, table;
+    bool split;
+    template <int MB, int NB>
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &) const {
+        const int l = threadIdx.x & 63, q = l >> 4;
+        const float f = lg.factor(), unit = unit_scale(lg.sc->cmax);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int t = n + 16 * j + (l & 15);
+            const bool in = t < rows;
+            const int64_t y = in ? target[t] : -1;
+            const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
+            const float c = in ? rowfac[t] * unit : 0.f;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int v0 = m + 16 * i + 4 * q;
+                Pack<G, 4> hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = v0 + e;
+                    float x = 0.f;
+                    if (v < table && c != 0.f) {
+                        const float z = logit(acc[i][j][e], f, lg.bias ? lg.bias[v] : 0.f);
+                        x = c * fmaf(split ? exp_fine(z - st.x) : exp_neg(z - st.x), st.y, v == y ? -1.f : 0.f);
+                    }
+                    hi.v[e] = (G)x;
+                    lo.v[e] = (G)(x - (float)hi.v[e]);
+                }
+                if (in && (size_t)v0 < vp) {
+                    *reinterpret_cast<Pack<G, 4> *>(g + (size_t)t * vp + v0) = hi;
+                    if (split) *reinterpret_cast<Pack<G, 4> *>(g + g_plane + (size_t)t * vp + v0) = lo;
+                }
+                if ((size_t)t < tp) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (v0 + e < table) {
+                            gt[(size_t)(v0 + e) * tp + t] = hi.v[e];
+                            if (split) gt[gt_plane + (size_t)(v0 + e) * tp + t] = lo.v[e];
+                        }
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Factor that a gradient's product still has to be multiplied with.
+struct OutScale {
+    const Scalars *sc;
+    bool split;
+    bool of_table;  // the product with the rows (the table's gradient), else with the table
+    __device__ __forceinline__ float operator()() const {
+        float f = 1.f / unit_scale(sc->cmax);
+        if (split) f /= unit_scale(of_table ? sc->amax_h : sc->amax_w);
+        return f;
+    }
+};
+
+// Epilogue of the gradients' products (A: columns, B: rows of the result): out, a part of a split K loop,
+// or the 32-bit sum over pieces.
+template <class O>
+struct OutEpi {
+    OutScale sc;
+    O *out;
+    size_t ld;
+    float *part;  // [part][rows][cols4], or null
+    float *sum;   // [rows][cols4], or null
+    int cols, rows, cols4;
+    bool first, last, vec;
+    template <int MB, int NB>
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl) const {
+        const int l = threadIdx.x & 63, q = l >> 4;
+        const float f = sc();
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int r = n + 16 * j + (l & 15);
+            if (r >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int c = m + 16 * i + 4 * q;
+                if (c >= cols) continue;
+                if (part) {
+                    *reinterpret_cast<floatx4_t *>(part + ((size_t)pl.part * rows + r) * cols4 + c) = acc[i][j];
+                    continue;
+                }
+                floatx4_t v = acc[i][j] * f;
+                if (sum) {
+                    floatx4_t *s = reinterpret_cast<floatx4_t *>(sum + (size_t)r * cols4 + c);
+                    if (!first) v += *s;
+                    if (!last) {
+                        *s = v;
+                        continue;
+                    }
+                }
+                O *o = out + (size_t)r * ld + c;
+                if (vec && c + 4 <= cols) {
+                    Pack<O, 4> p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p.v[e] = (O)v[e];
+                    *reinterpret_cast<Pack<O, 4> *>(o) = p;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < cols) o[e] = (O)v[e];
+                }
+            }
+        }
+    }
+};
+
+// Adds the parts of a split K loop.
+template <class O>
+__global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts, int rows, int cols, int cols4,
+                                                    OutScale sc, O *out, size_t ld) {
+    const float f = sc();
+    const size_t n = (size_t)rows * (cols4 / 4);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const int r = (int)(i / (cols4 / 4)), c = (int)(i % (cols4 / 4)) * 4;
+        floatx4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < parts; ++p) v += *reinterpret_cast<const floatx4_t *>(part + ((size_t)p * rows + r) * cols4 + c);
+        v *= f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) out[(size_t)r * ld + c + e] = (O)v[e];
+    }
+}
+
+// Tile of a product.  256 x 256 tiles (8 waves) reach 1.2 PFLOP/s where they fill the chip, 128 x 128 ones
+// (4 waves, two workgroups a CU) 0.85, so the estimate is whole rounds of workgroups times a tile's work.
+inline bool big_tiles(size_t M, size_t N, size_t batch) {
+    const size_t b = (size_t)ceil_div(M, 256) * ceil_div(N, 256) * batch, s = (size_t)ceil_div(M, 128) * ceil_div(N, 128) * batch;
+    return ((b + 255) / 256) * 4 * 10 <= ((s + 511) / 512) * 2 * 14;
+}
+
+template <class P, class Epi>
+int product(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
+    return big ? mm_launch<P, 2, 4, 8, 4>(g, epi, s) : mm_launch<P, 2, 2, 4, 4>(g, epi, s);
+}
+
+struct Sizes {
+    int dtype;
+    size_t rows, table, dim;
+    bool grad;
+    size_t kp, vp, piece_rows, tp, cols4;
+    bool stat_big;
+    int pieces;       // of a row's logits
+    bool dh_big, dw_big;
+    int ksplit;
+};
+
+inline size_t piece_bytes() {
+    const char *e = std::getenv("VHIP_XENT_PIECE_BYTES");
+    const unsigned long long v = e ? std::strtoull(e, nullptr, 10) : 0;
+    return v ? (size_t)v : kPieceBytes;
+}
+
+inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool grad) {
+    Sizes z{};
+    rows = rows ? rows : 1;  // an empty call gets the smallest workspace
+    table = table ? table : 1;
+    dim = dim ? dim : 1;
+    z.dtype = dtype;
+    z.rows = rows;
+    z.table = table;
+    z.dim = dim;
+    z.grad = grad;
+    z.kp = round_up(dim, kMmK);
+    z.vp = round_up(table, kMmK);
+    const size_t per = z.vp * (dtype == VHIP_DTYPE_F32 ? 8 : 4);
+    size_t fit = piece_bytes() / per / 256 * 256;
+    if (fit < 256) fit = 256;
+    z.piece_rows = !grad || rows <= fit ? rows : fit;
+    z.tp = round_up(z.piece_rows, kMmK);
+    z.cols4 = round_up(dim, 4);
+    z.stat_big = big_tiles(table, z.piece_rows, 1);
+    z.pieces = ceil_div(table, z.stat_big ? 128 : 64);
+    z.dh_big = dim > 128 && z.piece_rows > 128;
+    const size_t bs = z.dh_big ? 256 : 128, tiles = (size_t)ceil_div(dim, bs) * ceil_div(z.piece_rows, bs);
+    const size_t want = z.dh_big ? 256 : 512, ks = z.vp / kMmK;
+    size_t k = want / tiles;
+    if (k > ks / 8) k = ks / 8;
+    z.ksplit = (int)(k < 1 ? 1 : k);
+    z.dw_big = big_tiles(dim, table, 1);
+    return z;
+}
+
+struct Parts {
+    Scalars *sc;
+    float2 *part;
+    float2 *stat;
+    float *zt, *rowfac, *split, *sum;
+    void *hp, *wp, *ht, *wt, *g, *gt;
+};
+
+inline Parts carve(Carver &c, const Sizes &z) {
+    const size_t planes = z.dtype == VHIP_DTYPE_F32 ? 2 : 1;
+    Parts p{};
+    p.sc = c.take<Scalars>(1);
+    p.part = c.take<float2>((size_t)z.pieces * z.piece_rows);
+    p.zt = c.take<float>(z.piece_rows);
+    p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
+    p.wp = c.take<uint16_t>(planes * z.table * z.kp);
+    if (z.grad) {
+        p.stat = c.take<float2>(z.piece_rows);
+        p.rowfac = c.take<float>(z.piece_rows);
+        p.ht = c.take<uint16_t>(planes * z.dim * z.tp);
+        p.wt = c.take<uint16_t>(planes * z.dim * z.vp);
+        p.g = c.take<uint16_t>(planes * z.piece_rows * z.vp);
+        p.gt = c.take<uint16_t>(planes * z.table * z.tp);
+        if (z.ksplit > 1) p.split = c.take<float>((size_t)z.ksplit * z.piece_rows * z.cols4);
+        if (z.piece_rows < z.rows) p.sum = c.take<float>(z.table * z.cols4);
+    }
+    return p;
+}
+
+inline uint32_t wide_grid(size_t items) {
+    const size_t b = (items + 255) / 256;
+    return (uint32_t)(b < 4096 ? (b ? b : 1) : 4096);
+}
+
+struct Call {
+    const void *h, *table, *bias;
+    size_t ldh, ldt;
+    float scale;
+    const int64_t *target;
+    const float *row_weight;
+    float *loss, *lse;
+    void *dh, *dtable;
+    size_t lddh, lddt;
+};
+
+// Whether rows can be multiplied where they lie.
+template <class T>
+bool direct(const void *p, size_t ld, size_t dim) {
+    return Planes<T>::count == 1 && dim % kMmK == 0 && ld % 8 == 0 && aligned16(p) && ld <= kMmMaxLd;
+}
+
+template <class T>
+int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
+    typedef typename Planes<T>::type P;
+    constexpr bool kSplit = Planes<T>::count == 2;
+    const int dim = (int)z.dim, table = (int)z.table;
+    const T *h = (const T *)c.h, *w = (const T *)c.table;
+
+    k_xent_init<<<1, 64, 0, s>>>(p.sc);
+    if constexpr (kSplit) {
+        k_amax<<<(uint32_t)(z.rows < 1024 ? z.rows : 1024), 256, 0, s>>>((const float *)c.h, z.rows, dim, c.ldh, &p.sc->amax_h);
+        k_amax<<<(uint32_t)(z.table < 1024 ? z.table : 1024), 256, 0, s>>>((const float *)c.table, z.table, dim, c.ldt, &p.sc->amax_w);
+    }
+    const P *wp = (const P *)c.table;
+    size_t ldw = c.ldt;
+    if (!direct<T>(c.table, c.ldt, z.dim)) {
+        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, z.table * z.kp, (int)z.kp, &p.sc->amax_w);
+        wp = (const P *)p.wp;
+        ldw = z.kp;
+    }
+    if (z.grad)
+        k_pack_t<T><<<dim3((uint32_t)(z.vp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
+            w, z.table, dim, c.ldt, (P *)p.wt, z.dim * z.vp, z.vp, &p.sc->amax_w, nullptr, (const float *)c.bias);
+
+    for (size_t r0 = 0; r0 < z.rows; r0 += z.piece_rows) {
+        const size_t rows = z.rows - r0 < z.piece_rows ? z.rows - r0 : z.piece_rows;
+        const T *hr = h + r0 * c.ldh;
+        const int64_t *target = c.target + r0;
+        const P *hp = (const P *)(const void *)hr;
+        size_t ldh = c.ldh;
+        if (!direct<T>(hr, c.ldh, z.dim)) {
+            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, z.piece_rows * z.kp, (int)z.kp, &p.sc->amax_h);
+            hp = (const P *)p.hp;
+            ldh = z.kp;
+        }
+        MmArgs g{};
+        g.a[0] = wp;
+        g.a[1] = kSplit ? wp + z.table * z.kp : wp;
+        g.b[0] = hp;
+        g.b[1] = kSplit ? hp + z.piece_rows * z.kp : hp;
+        g.lda = ldw;
+        g.ldb = ldh;
+        g.M = table;
+        g.N = (int)rows;
+        g.ktiles = (int)(z.kp / kMmK);
+        g.nseg = kSplit ? 3 : 1;
+        g.ksplit = g.batch = 1;
+        const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
+        VH_CHECK(product<P>(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
+        k_xent_join<<<(uint32_t)ceil_div(rows, 16), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table,
+                                                                c.row_weight ? c.row_weight + r0 : nullptr, c.scale,
+                                                                c.loss ? c.loss + r0 : nullptr, c.lse ? c.lse + r0 : nullptr,
+                                                                p.stat, p.rowfac, p.sc);
+        VH_CHECK(launch_status("softmax launch"));
+        if (!z.grad) continue;
+        const size_t tp = round_up(rows, kMmK);
+        k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
+            hr, rows, dim, c.ldh, (P *)p.ht, z.dim * z.tp, tp, &p.sc->amax_h, target, nullptr);
+        GradEpi<P> ge{};
+        ge.lg = lg;
+        ge.stat = p.stat;
+        ge.rowfac = p.rowfac;
+        ge.target = target;
+        ge.g = (P *)p.g;
+        ge.gt = (P *)p.gt;
+        ge.g_plane = z.piece_rows * z.vp;
+        ge.gt_plane = z.table * z.tp;
+        ge.vp = z.vp;
+        ge.tp = tp;
+        ge.rows = (int)rows;
+        ge.table = table;
+        ge.split = kSplit;
+        VH_CHECK(product<P>(g, z.stat_big, ge, s));
+        if (c.dh) {
+            MmArgs d = g;
+            const P *wt = (const P *)p.wt, *gg = (const P *)p.g;
+            d.a[0] = wt;
+            d.a[1] = wt + (kSplit ? z.dim * z.vp : 0);
+            d.b[0] = gg;
+            d.b[1] = gg + (kSplit ? z.piece_rows * z.vp : 0);
+            d.lda = d.ldb = z.vp;
+            d.M = dim;
+            d.N = (int)rows;
+            d.ktiles = (int)(z.vp / kMmK);
+            d.ksplit = z.ksplit;
+            const OutScale os{p.sc, kSplit, false};
+            T *out = (T *)c.dh + r0 * c.lddh;
+            OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
+                         true, true, c.lddh % 4 == 0 && aligned16(out)};
+            VH_CHECK(product<P>(d, z.dh_big, oe, s));
+            if (z.ksplit > 1)
+                k_join_parts<T><<<wide_grid(rows * z.cols4 / 4), 256, 0, s>>>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh);
+        }
+        if (c.dtable) {
+            MmArgs d = g;
+            const P *ht = (const P *)p.ht, *gt = (const P *)p.gt;
+            d.a[0] = ht;
+            d.a[1] = ht + (kSplit ? z.dim * z.tp : 0);
+            d.b[0] = gt;
+            d.b[1] = gt + (kSplit ? z.table * z.tp : 0);
+            d.lda = d.ldb = tp;
+            d.M = dim;
+            d.N = table;
+            d.ktiles = (int)(tp / kMmK);
+            const bool many = z.piece_rows < z.rows;
+            OutEpi<T> oe{OutScale{p.sc, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
+                         (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % 4 == 0 && aligned16(c.dtable)};
+            VH_CHECK(product<P>(d, z.dw_big, oe, s));
+        }
+        VH_CHECK(launch_status("gradient launch"));
+    }
+    return VHIP_OK;
+}
+
+int check_call(int dtype, const Call &c, size_t rows, size_t table, size_t dim, bool grad) {
+    if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
+    if (dim == 0 || dim > 65536) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 65536]");
+    if (table == 0 || table > kMmMaxLd - kMmK) return set_error(VHIP_ERR_INVALID_CONFIG, "the table must have 1 to 2^23 - 64 rows");
+    if (rows > 0x3fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows");
+    if ((rows && (!c.h || !c.target)) || !c.table) return set_error(VHIP_ERR_INVALID_CONFIG, "an input is null");
+    if (c.ldh < dim || c.ldt < dim || (c.dh && c.lddh < dim) || (c.dtable && c.lddt < dim))
+        return set_error(VHIP_ERR_INVALID_CONFIG, "rows are closer than dim");
+    if (!std::isfinite(c.scale)) return set_error(VHIP_ERR_INVALID_CONFIG, "scale must be finite");
+    if (grad && !c.dh && !c.dtable) return set_error(VHIP_ERR_INVALID_CONFIG, "no gradient is asked for");
+    return VHIP_OK;
+}
+
+int run(int ordinal, int dtype, const Call &c, size_t rows, size_t table, size_t dim, bool grad, void *ws, size_t ws_bytes,
+        void *stream) {
+    clear_error();
+    VH_CHECK(check_call(dtype, c, rows, table, dim, grad));
+    const Sizes z = sizes_of(dtype, rows, table, dim, grad);
+    Carver cv{(char *)ws, 0};
+    const Parts p = carve(cv, z);
+    if (!ws || !aligned16(ws) || ws_bytes < cv.used)
+        return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_softmax_xent_workspace() (" +
+                                                      std::to_string(cv.used) + " bytes) or not aligned to 16 bytes");
+    CallDevice dev;
+    VH_CHECK(dev.enter(ordinal));
+    hipStream_t s = (hipStream_t)stream;
+    if (rows == 0) {
+        if (!grad || !c.dtable) return VHIP_OK;
+        const size_t es = dtype_size(dtype);
+        k_zero_rows<<<(uint32_t)(table < 4096 ? table : 4096), 256, 0, s>>>((char *)c.dtable, table, dim * es, c.lddt * es);
+        return launch_status("gradient launch");
+    }
+    switch (dtype) {
+        case VHIP_DTYPE_F32: return xent<float>(c, z, p, s);
+        case VHIP_DTYPE_F16: return xent<half_t>(c, z, p, s);
+        default: return xent<bf16_t>(c, z, p, s);
+    }
+}
+
+}  // namespace
+}  // namespace vh
+
+using namespace vh;
+
+extern "C" {
+
+size_t vhip_softmax_xent_workspace(int dtype, size_t rows, size_t table_rows, size_t dim, int gradients) {
+    Carver cv;
+    carve(cv, sizes_of(dtype, rows, table_rows, dim, gradients != 0));
+    return cv.used;
+}
+
+int vhip_softmax_xent(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table, size_t table_rows,
+                      size_t ldt, size_t dim, const int64_t *target, const float *bias, float scale, float *loss,
+                      float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    Call c{};
+    c.h = h;
+    c.table = table;
+    c.bias = bias;
+    c.ldh = ldh;
+    c.ldt = ldt;
+    c.scale = scale;
+    c.target = target;
+    c.loss = loss;
+    c.lse = lse;
+    return run(ordinal, dtype, c, rows, table_rows, dim, false, workspace, workspace_bytes, stream);
+}
+
+int vhip_softmax_xent_grad(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table,
+                           size_t table_rows, size_t ldt, size_t dim, const int64_t *target, const float *bias,
+                           const float *row_weight, float scale, float *loss, float *lse, void *dh, size_t lddh,
+                           void *dtable, size_t lddt, void *workspace, size_t workspace_bytes, void *stream) {
+    Call c{};
+    c.h = h;
+    c.table = table;
+    c.bias = bias;
+    c.ldh = ldh;
+    c.ldt = ldt;
+    c.scale = scale;
+    c.target = target;
+    c.row_weight = row_weight;
+    c.loss = loss;
+    c.lse = lse;
+    c.dh = dh;
+    c.dtable = dtable;
+    c.lddh = lddh;
+    c.lddt = lddt;
+    return run(ordinal, dtype, c, rows, table_rows, dim, true, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

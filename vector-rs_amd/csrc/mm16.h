@@ -1,17 +1,23 @@
 // mm16.h -- tile product C = A B^T of 16-bit operands on the matrix cores, shared by the training operators.
 //
-// A is M x K, B is N x K, both row-major with K contiguous ("planes"): rows 16-byte aligned, K a multiple of
-// 64.  Sums are held in 32 bits.  A 32-bit operand is carried as two float16 planes, x ~ hi + lo with
+// A is M x K and B is N x K, each either with K contiguous, or ("across", a template flag) stored as K rows
+// of its M or N values.  Rows are 16-byte aligned; K is a multiple of 64 where it is contiguous, and an
+// operand across may have fewer rows: the missing ones are read as its last, for the other operand to
+// multiply with zeros.  Sums are held in 32 bits.  A 32-bit operand is carried as two float16 planes, x ~ hi + lo with
 // hi = f16(x) and lo = f16(x - hi) (22 bits), and the product as three segments of one long K loop,
 // hi hi + hi lo + lo hi; the dropped lo lo term is 2^-22 of the product.
 //
 // A workgroup computes a BM x BN tile, its waves MB x NB blocks of 16 x 16.  Operand tiles of 64 k come in
-// by 16-byte global->LDS DMA into two buffers; a row's 128 bytes lie as eight 16-byte slots, slot s of row r
-// holding chunk s ^ (r & 7), so the 16 rows that one fragment read touches spread over all banks (the DMA
-// writes LDS in lane order, so the swizzle is in the addresses that the lanes read from).  The two halves of
-// a tile's k are two sets of fragments: while one set is multiplied the other is read, and the next tile's
-// DMA has the time of a whole tile's products to land.  Rows past M or N are clamped to the last row: what
-// they give is in accumulators that the epilogue does not use.
+// by 16-byte global->LDS DMA into two buffers; the two halves of a tile's k are two sets of fragments: while
+// one set is multiplied the other is read, and the next tile's DMA has the time of a whole tile's products to
+// land.  Rows past M or N are clamped to the last row: what they give is in accumulators that the epilogue
+// does not use.  The DMA writes LDS in lane order, so a tile is swizzled by the addresses that lanes read:
+//  * K contiguous: a row's 128 bytes are eight 16-byte slots, slot s of row r holding chunk s ^ (r & 7), so
+//    the 16 rows of a fragment read spread over all banks;
+//  * across: a row of k is BM / 8 slots, chunk s ^ 2 f(k), f from the bits of k that differ between the 16
+//    rows of a read (two 4 x 16 blocks of the transposing LDS read make a lane's 8 values of k).
+// Measured on 8192^3 in bfloat16: 256 x 256 tiles of 8 waves 1,222 TFLOP/s, 128 x 128 of 4 waves 831, the
+// library's product 1,326.
 #pragma once
 
 #include "train_common.h"
@@ -20,10 +26,11 @@ namespace vh {
 
 struct MmArgs {
     const void *a[2], *b[2];  // planes; [1] the low halves where nseg is 3
-    size_t lda, ldb;          // elements; 2^23 at most
+    size_t lda, ldb;          // elements; 2^23 at most where K is contiguous
     size_t sa, sb;            // from one product of a batch to the next, elements
     int M, N;
-    int ktiles;               // K / 64
+    int ktiles;               // K / 64, rounded up
+    int ka, kb;               // rows of an operand that is stored across
     int nseg;                 // 1, or 3 for split operands
     int mt, nt;               // tiles along M and N
     int ksplit;               // parts of the K loop, each a workgroup of its own
@@ -39,6 +46,7 @@ template <class T>
 struct MmVec;
 template <>
 struct MmVec<half_t> {
+    typedef _Float16 v4 __attribute__((ext_vector_type(4)));
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ floatx4_t mfma(v8 a, v8 b, floatx4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -46,6 +54,7 @@ struct MmVec<half_t> {
 };
 template <>
 struct MmVec<bf16_t> {
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ floatx4_t mfma(v8 a, v8 b, floatx4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -93,15 +102,148 @@ __device__ __forceinline__ MmPlace mm_place(const MmArgs &g, uint32_t id, uint32
     return p;
 }
 
-// Epi: void operator()(acc, m, n, place): the wave's MB x NB blocks, block (i, j) lane l element e being
-// C[m + 16 i + 4 (l >> 4) + e][n + 16 j + (l & 15)].
-template <class T, int WM, int WN, int MB, int NB, class Epi>
-__global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
-    constexpr int NW = WM * WN, BM = WM * MB * 16, BN = WN * NB * 16;
-    constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;  // DMAs of a wave: 8 rows each
-    static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN, "whole DMAs");
+// One operand's tile of BR rows (of M or N) by 64 k in LDS: its DMAs and its fragments.
+template <class T, bool ACROSS, int BR, int NW>
+struct MmTile {
+    static constexpr int I = BR / 8 / NW;           // DMAs of a wave
+    static constexpr int CH = BR / 8;               // chunks of a k row where stored across
+    static constexpr int kBytes = BR * 128;
+    static_assert(I * 8 * NW == BR, "whole DMAs");
+    typedef typename MmVec<T>::v4 v4;
     typedef typename MmVec<T>::v8 v8;
-    __shared__ __align__(1024) char lds[2 * (BM + BN) * 128];
+    uint32_t off[I];
+    const char *base[2];
+    size_t step;    // bytes from one tile of k to the next
+    size_t ld2;
+    int c_last, wave, lane;
+
+    static __device__ __forceinline__ int swizzle(int k) {
+        return 2 * ((k & 3) | (((k >> 3) & (CH >= 32 ? 3 : 1)) << 2));
+    }
+    // the chunk and row of DMA i, across
+    __device__ __forceinline__ void spot(int i, int &k, int &c) const {
+        const int n = (wave * I + i) * 64 + lane;
+        k = n / CH;
+        c = min((n % CH) ^ swizzle(k), c_last);
+    }
+    __device__ __forceinline__ void init(const void *const (&p)[2], size_t ld, int r0, int rows, size_t batch_off, int w, int l) {
+        wave = w;
+        lane = l;
+        ld2 = ld * 2;
+        if constexpr (ACROSS) {
+            c_last = (rows - 1 - r0) / 8;
+            step = ld2 * kMmK;
+            base[0] = (const char *)p[0] + (batch_off + r0) * 2;
+            base[1] = (const char *)p[1] + (batch_off + r0) * 2;
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                int k, c;
+                spot(i, k, c);
+                off[i] = (uint32_t)(k * ld2 + c * 16);
+            }
+        } else {
+            step = kMmK * 2;
+            base[0] = (const char *)p[0] + (batch_off + (size_t)r0 * ld) * 2;
+            base[1] = (const char *)p[1] + (batch_off + (size_t)r0 * ld) * 2;
+            const int r = l >> 3, c = (l & 7) ^ r;
+#pragma unroll
+            for (int i = 0; i < I; ++i) off[i] = (uint32_t)((size_t)(min(r0 + (w * I + i) * 8 + r, rows - 1) - r0) * ld2 + c * 16);
+        }
+    }
+    // DMA of tile kt of a plane to LDS address `to`; krows: rows of k from this tile on
+    __device__ __forceinline__ void issue(int plane, int kt, int krows, uint32_t to) const {
+        const char *g = base[plane] + kt * step;
+        to += wave * I * 1024;
+        if (ACROSS && krows < kMmK) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                int k, c;
+                spot(i, k, c);
+                dma_lds16_at(g, (uint32_t)(min(k, krows - 1) * ld2 + c * 16), to + i * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) dma_lds16_at(g, off[i], to + i * 1024);
+        }
+    }
+    // Fragments of N blocks from row r0 of the tile, half h of its k.
+    template <int N>
+    static __device__ __forceinline__ void read(v8 (&f)[N], const char *tile, int r0, int h, int l) {
+        const int i = l & 15, q = l >> 4;
+        if constexpr (ACROSS) {
+            typedef __attribute__((address_space(3))) v4 lds_v4;
+            const int k = h * 32 + q * 8 + (i >> 2);
+            const char *p = tile + k * (BR * 2) + (i & 1) * 8;
+            const int s = swizzle(k);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int c = (((r0 >> 3) + 2 * n + ((i >> 1) & 1)) ^ s) * 16;
+                const v4 x = read_tr((lds_v4 *)(p + c)), y = read_tr((lds_v4 *)(p + c + 4 * BR * 2));
+                f[n] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        } else {
+            const char *p = tile + (r0 + i) * 128 + ((q + 4 * h) ^ (i & 7)) * 16;
+#pragma unroll
+            for (int n = 0; n < N; ++n) f[n] = *(const v8 *)(p + n * 2048);
+        }
+    }
+    static __device__ __forceinline__ v4 read_tr(__attribute__((address_space(3))) v4 *p) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p));
+    }
+};
+
+// LDS of a wave for its epilogue, 16 KB.
+constexpr int kEpiBytes = 16384;
+
+// Values of a wave's blocks as whole rows: value(i, j, e) is element e of block (i, j) (see Epi), given once
+// each; emit(n, m, pack) gets 16 bytes of row n (of N, within the wave's) from column m.  What 16 lanes hold
+// of 16 rows goes through LDS, so that rows leave in pieces of up to 256 bytes.
+template <class O, int MB, int NB, class Value, class Emit>
+__device__ __forceinline__ void rows_through_lds(char *w, const Value &value, const Emit &emit) {
+    constexpr int PER = 16 / (int)sizeof(O);                                   // values of a chunk
+    constexpr int BP = MB * 16 * (int)sizeof(O) <= 256 ? MB : 256 / 16 / (int)sizeof(O);  // blocks of a pass
+    constexpr int PITCH = BP * 16 * (int)sizeof(O), NC = PITCH / 16;
+    static_assert(NB * 16 * PITCH <= kEpiBytes && MB % BP == 0, "fits");
+    const int l = threadIdx.x & 63, q = l >> 4;
+#pragma unroll
+    for (int p = 0; p < MB / BP; ++p) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = 16 * j + (l & 15);
+#pragma unroll
+            for (int i = 0; i < BP; ++i) {
+                Pack<O, 4> v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.v[e] = value(p * BP + i, j, e);
+                const int at = (16 * i + 4 * q) * (int)sizeof(O);
+                *reinterpret_cast<Pack<O, 4> *>(w + n * PITCH + (((at >> 4) ^ (n & (NC - 1))) << 4) + (at & 15)) = v;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int k = 0; k < NB * 16 * NC / 64; ++k) {
+            const int n = k * (64 / NC) + l / NC, c = l % NC;
+            emit(n, p * BP * 16 + c * PER, *reinterpret_cast<const Pack<O, PER> *>(w + n * PITCH + ((c ^ (n & (NC - 1))) << 4)));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// Epi: void operator()(acc, m, n, place, lds): the wave's MB x NB blocks, block (i, j) lane l element e being
+// C[m + 16 i + 4 (l >> 4) + e][n + 16 j + (l & 15)]; lds: kEpiBytes of the wave's own.
+template <class T, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
+__global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
+    constexpr int NW = WM * WN, BM = WM * MB * 16, BN = WN * NB * 16, BUF = (BM + BN) * 128;
+    typedef MmTile<T, TA, BM, NW> TileA;
+    typedef MmTile<T, TB, BN, NW> TileB;
+    typedef typename MmVec<T>::v8 v8;
+    static_assert(2 * BUF >= NW * kEpiBytes, "the epilogue's LDS");
+    __shared__ __align__(1024) char lds[2 * BUF];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -113,42 +255,19 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
     const int s0 = (int)((long)all * pl.part / g.ksplit), s1 = (int)((long)all * (pl.part + 1) / g.ksplit);
     int seg = s0 / g.ktiles, kt = s0 % g.ktiles;
 
-    uint32_t offa[IA], offb[IB];
-    {
-        const int r = lane >> 3, c = (lane & 7) ^ r;
-#pragma unroll
-        for (int i = 0; i < IA; ++i) {
-            const int row = min(m0 + (wave * IA + i) * 8 + r, g.M - 1) - m0;
-            offa[i] = (uint32_t)((size_t)row * g.lda * 2 + c * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < IB; ++i) {
-            const int row = min(n0 + (wave * IB + i) * 8 + r, g.N - 1) - n0;
-            offb[i] = (uint32_t)((size_t)row * g.ldb * 2 + c * 16);
-        }
-    }
-    const size_t pa = ((size_t)m0 * g.lda + pl.batch * g.sa) * 2, pb = ((size_t)n0 * g.ldb + pl.batch * g.sb) * 2;
+    TileA ta;
+    TileB tb;
+    ta.init(g.a, g.lda, m0, g.M, pl.batch * g.sa, wave, lane);
+    tb.init(g.b, g.ldb, n0, g.N, pl.batch * g.sb, wave, lane);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-
     auto issue = [&](int buf) {
-        const char *ga = (const char *)g.a[seg == 2] + pa + (size_t)kt * (kMmK * 2);
-        const char *gb = (const char *)g.b[seg == 1] + pb + (size_t)kt * (kMmK * 2);
-        const uint32_t la = lds0 + buf * (BM + BN) * 128 + wave * IA * 1024;
-        const uint32_t lb = lds0 + buf * (BM + BN) * 128 + BM * 128 + wave * IB * 1024;
-#pragma unroll
-        for (int i = 0; i < IA; ++i) dma_lds16_at(ga, offa[i], la + i * 1024);
-#pragma unroll
-        for (int i = 0; i < IB; ++i) dma_lds16_at(gb, offb[i], lb + i * 1024);
+        ta.issue(seg == 2, kt, g.ka - kt * kMmK, lds0 + buf * BUF);
+        tb.issue(seg == 1, kt, g.kb - kt * kMmK, lds0 + buf * BUF + TileA::kBytes);
         if (++kt == g.ktiles) {
             kt = 0;
             ++seg;
         }
     };
-
-    // fragment addresses: row l & 15 of a block, chunk (l >> 4) of its half
-    const int fr = lane & 15, fc = lane >> 4;
-    const int sw0 = ((fc) ^ (fr & 7)) * 16, sw1 = ((fc + 4) ^ (fr & 7)) * 16;
-    const char *fa = lds + (wm * MB * 16 + fr) * 128, *fb = lds + (BM + wn * NB * 16 + fr) * 128;
 
     floatx4_t acc[MB][NB];
 #pragma unroll
@@ -157,11 +276,9 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
         for (int j = 0; j < NB; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
     v8 a0[MB], b0[NB], a1[MB], b1[NB];
-    auto read = [&](v8(&a)[MB], v8(&b)[NB], int buf, int sw) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) b[j] = *(const v8 *)(fb + buf * (BM + BN) * 128 + j * 2048 + sw);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) a[i] = *(const v8 *)(fa + buf * (BM + BN) * 128 + i * 2048 + sw);
+    auto read = [&](v8(&a)[MB], v8(&b)[NB], int buf, int h) {
+        TileB::template read<NB>(b, lds + buf * BUF + TileA::kBytes, wn * NB * 16, h, lane);
+        TileA::template read<MB>(a, lds + buf * BUF, wm * MB * 16, h, lane);
     };
     auto multiply = [&](const v8(&a)[MB], const v8(&b)[NB]) {
 #pragma unroll
@@ -175,15 +292,15 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
         issue(0);
         if (n > 1) {
             issue(1);
-            __builtin_amdgcn_s_waitcnt(VH_VMCNT(IA + IB));
+            __builtin_amdgcn_s_waitcnt(VH_VMCNT(TileA::I + TileB::I));
         } else {
             __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
         }
         lds_barrier();
-        read(a0, b0, 0, sw0);
+        read(a0, b0, 0, 0);
         for (int s = 0; s < n; ++s) {
             const int buf = s & 1;
-            read(a1, b1, buf, sw1);
+            read(a1, b1, buf, 1);
             multiply(a0, b0);
             if (s + 1 < n) {
                 // this wave's reads of the buffer are done (lds_barrier waits for them) and the next
@@ -191,24 +308,40 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
                 __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
                 lds_barrier();
                 if (s + 2 < n) issue(buf);
-                read(a0, b0, buf ^ 1, sw0);
+                read(a0, b0, buf ^ 1, 0);
             }
             multiply(a1, b1);
         }
     }
-    epi(acc, m0 + wm * MB * 16, n0 + wn * NB * 16, pl);
+    lds_barrier();  // every wave's fragments are read: the buffers are the epilogue's
+    epi(acc, m0 + wm * MB * 16, n0 + wn * NB * 16, pl, lds + wave * kEpiBytes);
 }
 
-template <class T, int WM, int WN, int MB, int NB, class Epi>
-int mm_launch(MmArgs g, const Epi &epi, hipStream_t s) {
+template <class T, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
+int mm_launch_tile(MmArgs g, const Epi &epi, hipStream_t s) {
     g.mt = ceil_div(g.M, WM * MB * 16);
     g.nt = ceil_div(g.N, WN * NB * 16);
     const size_t tiles = g.upper ? (size_t)g.mt * (g.mt + 1) / 2 : (size_t)g.mt * g.nt;
     const size_t total = tiles * g.ksplit * g.batch;
-    if (total > 0x7fffffff || g.lda > kMmMaxLd || g.ldb > kMmMaxLd)
+    if (total > 0x7fffffff || (!TA && g.lda > kMmMaxLd) || (!TB && g.ldb > kMmMaxLd))
         return set_error(VHIP_ERR_INVALID_CONFIG, "a product of the call has too many tiles");
-    k_mm<T, WM, WN, MB, NB, Epi><<<dim3((uint32_t)total), dim3(WM * WN * 64), 0, s>>>(g, epi);
+    k_mm<T, TA, TB, WM, WN, MB, NB, Epi><<<dim3((uint32_t)total), dim3(WM * WN * 64), 0, s>>>(g, epi);
     return launch_status("product launch");
+}
+
+// Whether 256 x 256 tiles (8 waves, one workgroup a CU) beat 128 x 128 ones (4 waves, two a CU): whole rounds
+// of workgroups times a tile's work at the rates above.
+inline bool mm_big_tiles(size_t M, size_t N, size_t batch, bool upper = false) {
+    auto tiles = [&](size_t b) {
+        const size_t m = (M + b - 1) / b, n = (N + b - 1) / b;
+        return (upper ? m * (m + 1) / 2 : m * n) * batch;
+    };
+    return ((tiles(256) + 255) / 256) * 4 * 10 <= ((tiles(128) + 511) / 512) * 2 * 14;
+}
+
+template <class T, bool TA, bool TB, class Epi>
+int mm_launch(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
+    return big ? mm_launch_tile<T, TA, TB, 2, 4, 8, 4>(g, epi, s) : mm_launch_tile<T, TA, TB, 2, 2, 4, 4>(g, epi, s);
 }
 
 }  // namespace vh

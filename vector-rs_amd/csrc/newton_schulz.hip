@@ -10,7 +10,7 @@
 // singular values stay below 2 for any useful coefficients, so neither leaves float16's range.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.  a X is part
-// of B's diagonal.  The products want K contiguous in both operands, so X is kept in both orders.
+// of B's diagonal.
 #include "mm16.h"
 
 #include <cmath>
@@ -51,10 +51,10 @@ struct Planes2 {
     size_t ld, stride;
 };
 
-// The scaled matrix in both orders: x [m][np], xt [n][mp], zeros past n and m.
+// The scaled matrix x [m][np], zeros past n.
 template <class T>
 __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int cols, size_t ld, size_t stride, bool tall,
-                                                  const double *part, float eps, Planes2 x, Planes2 xt) {
+                                                  const double *part, float eps, Planes2 x) {
     __shared__ float tile[64][65];
     __shared__ float s_inv;
     if (threadIdx.x < 64) {
@@ -70,32 +70,36 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int r = r0 + ty + 4 * i, c = c0 + tx;
-        tile[ty + 4 * i][tx] = r < rows && c < cols ? (float)p[(size_t)r * ld + c] * inv : 0.f;
+        const float v = r < rows && c < cols ? (float)p[(size_t)r * ld + c] * inv : 0.f;
+        tile[tall ? tx : ty + 4 * i][tall ? ty + 4 * i : tx] = v;
     }
     __syncthreads();
-    // `by_row` is indexed [r][c] and `by_col` [c][r]
-    const Planes2 by_row = tall ? xt : x, by_col = tall ? x : xt;
-    half_t *o1 = by_row.p + blockIdx.z * by_row.stride, *o2 = by_col.p + blockIdx.z * by_col.stride;
+    const int m0 = tall ? c0 : r0, n0 = tall ? r0 : c0, m = tall ? cols : rows;
+    half_t *o = x.p + blockIdx.z * x.stride;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        half_t hi, lo;
-        {
-            const int r = r0 + ty + 4 * i, c = c0 + tx;
-            if (r < rows && (size_t)c < by_row.ld) {
-                split(tile[ty + 4 * i][tx], hi, lo);
-                o1[(size_t)r * by_row.ld + c] = hi;
-                o1[by_row.plane + (size_t)r * by_row.ld + c] = lo;
-            }
-        }
-        {
-            const int c = c0 + ty + 4 * i, r = r0 + tx;
-            if (c < cols && (size_t)r < by_col.ld) {
-                split(tile[tx][ty + 4 * i], hi, lo);
-                o2[(size_t)c * by_col.ld + r] = hi;
-                o2[by_col.plane + (size_t)c * by_col.ld + r] = lo;
-            }
+        const int r = m0 + ty + 4 * i, c = n0 + tx;
+        if (r < m && (size_t)c < x.ld) {
+            half_t hi, lo;
+            split(tile[ty + 4 * i][tx], hi, lo);
+            o[(size_t)r * x.ld + c] = hi;
+            o[x.plane + (size_t)r * x.ld + c] = lo;
         }
     }
+}
+
+// A wave's blocks as both planes of rows [r0, rows) and columns [c0, ld).
+template <int MB, int NB>
+__device__ __forceinline__ void store_planes(const floatx4_t (&acc)[MB][NB], char *lds, half_t *p, size_t plane, size_t ld,
+                                             int r0, int rows, int c0) {
+    auto store = [=](half_t *to) {
+        return [=](int r, int c, const Pack<half_t, 8> &v) {
+            if (r0 + r < rows && (size_t)(c0 + c) < ld) *reinterpret_cast<Pack<half_t, 8> *>(to + (size_t)(r0 + r) * ld + c0 + c) = v;
+        };
+    };
+    rows_through_lds<half_t, MB, NB>(lds, [&](int i, int j, int e) { return (half_t)acc[i][j][e]; }, store(p));
+    rows_through_lds<half_t, MB, NB>(
+        lds, [&](int i, int j, int e) { return (half_t)(acc[i][j][e] - (float)(half_t)acc[i][j][e]); }, store(p + plane));
 }
 
 // Epilogue of the symmetric products: out = alpha acc + beta add + diag I, stored at both places.
@@ -104,7 +108,7 @@ struct SymEpi {
     float alpha, beta, diag;
     int m;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl) const {
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl, char *lds) const {
         const int l = threadIdx.x & 63, q = l >> 4;
         half_t *o = out.p + pl.batch * out.stride;
         const half_t *ad = add.p ? add.p + pl.batch * add.stride : nullptr;
@@ -112,14 +116,11 @@ struct SymEpi {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int c = nw + 16 * j + (l & 15);
-            if ((size_t)c >= out.ld) continue;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 const int r = mw + 16 * i + 4 * q;
-                if ((size_t)r >= out.ld) continue;
-                Pack<half_t, 4> hi, lo;
                 floatx4_t v = acc[i][j] * alpha;
-                if (ad && c < m) {
+                if (ad && c < m && (size_t)r < add.ld) {
                     const Pack<half_t, 4> h = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + r);
                     const Pack<half_t, 4> w = *reinterpret_cast<const Pack<half_t, 4> *>(ad + add.plane + (size_t)c * add.ld + r);
 #pragma unroll
@@ -129,78 +130,64 @@ struct SymEpi {
                 for (int e = 0; e < 4; ++e) {
                     float x = v[e] + (r + e == c ? diag : 0.f);
                     if (r + e >= m || c >= m) x = 0.f;
-                    split(x, hi.v[e], lo.v[e]);
-                }
-                if (c < m) {
-                    *reinterpret_cast<Pack<half_t, 4> *>(o + (size_t)c * out.ld + r) = hi;
-                    *reinterpret_cast<Pack<half_t, 4> *>(o + out.plane + (size_t)c * out.ld + r) = lo;
-                }
-                if (mirror) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (r + e < m) {
-                            o[(size_t)(r + e) * out.ld + c] = hi.v[e];
-                            o[out.plane + (size_t)(r + e) * out.ld + c] = lo.v[e];
-                        }
+                    acc[i][j][e] = x;
+                    if (mirror && r + e < m && (size_t)c < out.ld) {
+                        half_t hi, lo;
+                        split(x, hi, lo);
+                        o[(size_t)(r + e) * out.ld + c] = hi;
+                        o[out.plane + (size_t)(r + e) * out.ld + c] = lo;
                     }
                 }
             }
         }
+        store_planes(acc, lds, o, out.plane, out.ld, nw, m, mw);
     }
 };
 
-// Epilogue of B X (A operand X^T, B operand B): the next X in both orders, or the result.
+// Epilogue of B X: the next X (A operand X across, B operand B), or the result in the order that the A
+// operand's rows have (B where the matrix is tall).
 template <class T>
 struct StepEpi {
-    Planes2 x, xt;
+    Planes2 x;
     float alpha;
-    int m, n;
-    T *out;  // null: not the last step
+    int cols, rows;  // of what is stored
+    T *out;          // null: not the last step
     size_t ldo, so;
-    bool tall;
+    bool vec;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl) const {
-        const int l = threadIdx.x & 63, q = l >> 4;
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl, char *lds) const {
+        if (!out) {
+            const int l = threadIdx.x & 63, q = l >> 4;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int r = nw + 16 * j + (l & 15);  // row of X
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const int c = mw + 16 * i + 4 * q;  // column of X
-                if (out) {
-                    T *o = out + pl.batch * so;
-                    if (r < m) {
+                for (int j = 0; j < NB; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (c + e < n) o[tall ? (size_t)(c + e) * ldo + r : (size_t)r * ldo + c + e] = (T)(acc[i][j][e] * alpha);
-                    }
-                    continue;
-                }
-                half_t *ox = x.p + pl.batch * x.stride, *ot = xt.p + pl.batch * xt.stride;
-                Pack<half_t, 4> hi, lo;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) split(r < m && c + e < n ? acc[i][j][e] * alpha : 0.f, hi.v[e], lo.v[e]);
-                if (r < m && (size_t)c < x.ld) {
-                    *reinterpret_cast<Pack<half_t, 4> *>(ox + (size_t)r * x.ld + c) = hi;
-                    *reinterpret_cast<Pack<half_t, 4> *>(ox + x.plane + (size_t)r * x.ld + c) = lo;
-                }
-                if ((size_t)r < xt.ld) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (c + e < n) {
-                            ot[(size_t)(c + e) * xt.ld + r] = hi.v[e];
-                            ot[xt.plane + (size_t)(c + e) * xt.ld + r] = lo.v[e];
-                        }
-                    }
-                }
-            }
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = mw + 16 * i + 4 * q + e < cols ? acc[i][j][e] * alpha : 0.f;
+            store_planes(acc, lds, x.p + pl.batch * x.stride, x.plane, x.ld, nw, rows, mw);
+            return;
         }
+        constexpr int PER = 16 / (int)sizeof(T);
+        T *o = out + pl.batch * so;
+        rows_through_lds<T, MB, NB>(
+            lds, [&](int i, int j, int e) { return (T)(acc[i][j][e] * alpha); },
+            [&](int r, int c, const Pack<T, PER> &v) {
+                if (nw + r >= rows || mw + c >= cols) return;
+                T *p = o + (size_t)(nw + r) * ldo + mw + c;
+                if (vec && mw + c + PER <= cols) {
+                    *reinterpret_cast<Pack<T, PER> *>(p) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (mw + c + e < cols) p[e] = v.v[e];
+                }
+            });
     }
 };
 
 struct NsParts {
     double *norm;
-    Planes2 x, xt[2], a, b;
+    Planes2 x[2], a, b;
 };
 
 inline Planes2 planes(Carver &c, size_t count, size_t rows, size_t ld) {
@@ -216,9 +203,8 @@ inline NsParts carve(Carver &c, size_t count, size_t m, size_t n) {
     NsParts p{};
     const size_t mp = round_up(m, kMmK), np = round_up(n, kMmK);
     p.norm = c.take<double>(count * kNormParts);
-    p.x = planes(c, count, m, np);
-    p.xt[0] = planes(c, count, n, mp);
-    p.xt[1] = planes(c, count, n, mp);
+    p.x[0] = planes(c, count, m, np);
+    p.x[1] = planes(c, count, m, np);
     p.a = planes(c, count, m, mp);
     p.b = planes(c, count, m, mp);
     return p;
@@ -231,30 +217,21 @@ inline void operand(const Planes2 &p, const void *(&pl)[2], size_t &ld, size_t &
     stride = p.stride;
 }
 
-inline bool ns_big(size_t M, size_t N, size_t batch, bool upper) {
-    size_t b = (size_t)ceil_div(M, 256) * ceil_div(N, 256), s = (size_t)ceil_div(M, 128) * ceil_div(N, 128);
-    if (upper) {
-        b = (size_t)ceil_div(M, 256) * (ceil_div(M, 256) + 1) / 2;
-        s = (size_t)ceil_div(M, 128) * (ceil_div(M, 128) + 1) / 2;
-    }
-    b *= batch;
-    s *= batch;
-    return ((b + 255) / 256) * 4 * 10 <= ((s + 511) / 512) * 2 * 14;
-}
-
-template <class Epi>
-int multiply(const Planes2 &a, int M, const Planes2 &b, int N, size_t count, bool upper, const Epi &epi, hipStream_t s) {
+// K rows of an operand across, or 0 where K is contiguous.
+template <bool TA, bool TB, class Epi>
+int multiply(const Planes2 &a, int M, const Planes2 &b, int N, int K, size_t count, bool upper, const Epi &epi, hipStream_t s) {
     MmArgs g{};
     operand(a, g.a, g.lda, g.sa);
     operand(b, g.b, g.ldb, g.sb);
     g.M = M;
     g.N = N;
-    g.ktiles = (int)(a.ld / kMmK);
+    g.ktiles = ceil_div(K, kMmK);
+    g.ka = g.kb = K;
     g.nseg = 3;
     g.ksplit = 1;
     g.batch = (int)count;
     g.upper = upper;
-    return ns_big(M, N, count, upper) ? mm_launch<half_t, 2, 4, 8, 4>(g, epi, s) : mm_launch<half_t, 2, 2, 4, 4>(g, epi, s);
+    return mm_launch<half_t, TA, TB>(g, mm_big_tiles(M, N, count, upper), epi, s);
 }
 
 struct NsCall {
@@ -273,17 +250,31 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
     const T *in = (const T *)k.in;
     k_ns_norm<T><<<dim3(kNormParts, (uint32_t)k.count), 256, 0, s>>>(in, k.rows, k.cols, k.ldi, k.si, p.norm);
     k_ns_start<T><<<dim3((uint32_t)ceil_div(k.rows, 64), (uint32_t)ceil_div(k.cols, 64), (uint32_t)k.count), 256, 0, s>>>(
-        in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x, p.xt[0]);
+        in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0]);
     VH_CHECK(launch_status("orthogonalize launch"));
     for (int i = 0; i < k.steps; ++i) {
-        const bool last = i + 1 == k.steps;
-        const Planes2 &from = p.xt[i & 1], &to = p.xt[(i & 1) ^ 1];
+        const Planes2 &from = p.x[i & 1], &to = p.x[(i & 1) ^ 1];
         SymEpi ea{p.a, Planes2{}, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
-        VH_CHECK(multiply(p.x, m, p.x, m, k.count, true, ea, s));
+        VH_CHECK((multiply<false, false>)(from, m, from, m, n, k.count, true, ea, s));
         SymEpi eb{p.b, p.a, k.c / kAScale, k.b, k.a * kAScale, m};
-        VH_CHECK(multiply(p.a, m, p.a, m, k.count, true, eb, s));
-        StepEpi<T> es{p.x, to, last ? 1.f / (kAScale * kXScale) : 1.f / kAScale, m, n, last ? (T *)k.out : nullptr, k.ldo, k.so, tall};
-        VH_CHECK(multiply(from, n, p.b, m, k.count, false, es, s));
+        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, k.count, true, eb, s));
+        StepEpi<T> es{to, 1.f / kAScale, n, m, nullptr, 0, 0, false};
+        if (i + 1 < k.steps) {
+            VH_CHECK((multiply<true, false>)(from, n, p.b, m, m, k.count, false, es, s));
+            continue;
+        }
+        es.alpha /= kXScale;
+        es.out = (T *)k.out;
+        es.ldo = k.ldo;
+        es.so = k.so;
+        es.vec = k.ldo % (16 / sizeof(T)) == 0 && (k.count == 1 || k.so % (16 / sizeof(T)) == 0) && aligned16(k.out);
+        if (tall) {
+            es.cols = m;
+            es.rows = n;
+            VH_CHECK((multiply<false, true>)(p.b, m, from, n, m, k.count, false, es, s));
+        } else {
+            VH_CHECK((multiply<true, false>)(from, n, p.b, m, m, k.count, false, es, s));
+        }
     }
     return VHIP_OK;
 }

@@ -29,7 +29,7 @@ namespace vh {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G in both orders
+constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G
 constexpr int kGBits = 14;
 
 // State of a call on the device.
@@ -88,20 +88,21 @@ struct Planes<float> {
     static constexpr int count = 2;
 };
 
-// rows x dim -> planes of rows x kp, zeros past dim.
+// rows x dim -> planes of rows x kp, zeros past dim and in rows whose bias is -inf.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              size_t plane, int kp, const uint32_t *amax) {
+                                              size_t plane, int kp, const uint32_t *amax, const float *bias) {
     const size_t n = rows * (kp / 8);
     float sc = 1.f;
     if constexpr (Planes<T>::count == 2) sc = unit_scale(*amax);
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
         const size_t r = i / (kp / 8);
         const int c = (int)(i % (kp / 8)) * 8;
+        const bool keep = !bias || bias[r] != -INFINITY;
         Pack<typename Planes<T>::type, 8> hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const T v = c + e < dim ? x[r * ld + c + e] : (T)0.f;
+            const T v = keep && c + e < dim ? x[r * ld + c + e] : (T)0.f;
             if constexpr (Planes<T>::count == 2) {
                 const float f = v * sc;
                 hi.v[e] = (half_t)f;
@@ -116,12 +117,11 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
     }
 }
 
-// rows x dim -> planes of dim x rp, zeros past rows.  Rows that do not count are zeros: those with a
-// negative target (`target`) or a bias of -inf (`bias`).
+// rows x dim -> planes of dim x rp, zeros past rows and for rows with a negative target.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim, size_t ld,
                                                 typename Planes<T>::type *out, size_t plane, size_t rp,
-                                                const uint32_t *amax, const int64_t *target, const float *bias) {
+                                                const uint32_t *amax, const int64_t *target) {
     __shared__ T tile[64][65];
     const size_t r0 = (size_t)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim
         const size_t r = r0 + ty + 4 * i;
         const int c = c0 + tx;
         T v = (T)0.f;
-        if (r < rows && c < dim && !(target && target[r] < 0) && !(bias && bias[r] == -INFINITY)) v = x[r * ld + c];
+        if (r < rows && c < dim && target[r] >= 0) v = x[r * ld + c];
         tile[ty + 4 * i][tx] = v;
     }
     __syncthreads();
@@ -164,60 +164,85 @@ struct Logits {
         return split ? scale / unit_scale(sc->amax_h) / unit_scale(sc->amax_w) : scale;
     }
 };
-__device__ __forceinline__ float logit(float acc, float f, float b) {
-    return b == -INFINITY ? -INFINITY : fmaf(acc, f, b);
+// A wave's sums to f times them being the logits: where there is a bias, or entries past the table, the
+// logits themselves (-inf where an entry is out) and f = 1.
+template <int MB, int NB>
+__device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logits &lg, int m, int table) {
+    const float f = lg.factor();
+    if (!lg.bias && m + 16 * MB <= table) return f;
+    const int q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        float b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int v = m + 16 * i + 4 * q + e;
+            b[e] = v < table ? (lg.bias ? lg.bias[v] : 0.f) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = b[e] == -INFINITY ? -INFINITY : fmaf(acc[i][j][e], f, b[e]);
+    }
+    return 1.f;
 }
 
 // Epilogue of the first product (A: table, B: rows): a wave's 16 MB entries of each row end in one piece.
 struct StatEpi {
     Logits lg;
     float2 *part;  // [piece][rows]: largest logit, sum of exp about it
-    float *zt;     // the target's logit
+    float2 *zt;    // the target's logit less its piece's largest, and that
     const int64_t *target;
     int rows, table;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &) const {
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *) const {
         if (m >= table) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = lg.factor();
+        float f = to_logits(acc, lg, m, table);
+        if (f < 0.f) {
+            f = -f;
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = -acc[i][j];
+        }
         const int piece = m / (16 * MB);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
             const bool in = t < rows;
-            const int64_t y = in ? target[t] : -1;
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = m + 16 * i + 4 * q + e;
-                    float z = -INFINITY;
-                    if (v < table) {
-                        z = logit(acc[i][j][e], f, lg.bias ? lg.bias[v] : 0.f);
-                        if (v == y) zt[t] = z;
-                    }
-                    acc[i][j][e] = z;
-                    top = fmaxf(top, z);
-                }
+                const floatx4_t a = acc[i][j];
+                top = fmaxf(fmaxf(fmaxf(top, a[0]), fmaxf(a[1], a[2])), a[3]);
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * f;
             const float about = top == -INFINITY ? 0.f : top;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += exp_neg(acc[i][j][e] - about);
+                for (int e = 0; e < 4; ++e) sum += exp_neg(fmaf(acc[i][j][e], f, -about));
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
+            const int64_t y = in ? target[t] : -1;
+            if (y >= m && y < m + 16 * MB && y < table) {
+                const int d = (int)(y - m) - 4 * q;
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d == 16 * i + e) zt[t] = make_float2(fmaf(acc[i][j][e], f, -about), about);
+            }
         }
     }
 };
 
 // Joins the pieces: 16 rows a workgroup, 16 lanes of a row each taking every sixteenth piece.
-__global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float *zt,
+__global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float2 *zt,
                                                    const int64_t *target, int64_t table, const float *weight,
                                                    float scale, float *loss, float *lse, float2 *stat,
                                                    float *rowfac, Scalars *sc) {
@@ -246,9 +271,9 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int piece
     if (y >= table) {
         ls = fac = NAN;
     } else if (y >= 0) {
-        const float z = zt[t];
-        const bool out = L == -INFINITY || z == -INFINITY;
-        ls = out ? INFINITY : about - z + logf(sum);  // not lse - z, which cancels where the loss is small
+        const float2 z = zt[t];
+        const bool out = L == -INFINITY || z.x == -INFINITY;
+        ls = out ? INFINITY : (about - z.y) - z.x + logf(sum);  // not lse - z, which cancels where the loss is small
         if (!out) fac = (weight ? weight[t] : 1.f) * scale;
     }
     if (t < rows) {
@@ -276,59 +301,65 @@ __global__ __launch_bounds__(256) void k_zero_rows(char *p, size_t rows, size_t 
         for (size_t i = threadIdx.x; i < row_bytes; i += 256) p[r * ld_bytes + i] = 0;
 }
 
-// Epilogue of the second product: G in both orders.
+// Epilogue of the second product: G.
 template <class G>  // element type of G's planes
 struct GradEpi {
     Logits lg;
     const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
     const float *rowfac;
     const int64_t *target;
-    G *g, *gt;  // [rows][vp], [table][tp]
-    size_t g_plane, gt_plane;
-    size_t vp, tp;
-    int rows, table;
+    G *g;  // [tp][vp]
+    size_t plane, vp;
+    int rows, tp, table;
     bool split;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &) const {
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
+        if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = lg.factor(), unit = unit_scale(lg.sc->cmax);
+        const float f = to_logits(acc, lg, m, table), unit = unit_scale(lg.sc->cmax);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
             const bool in = t < rows;
-            const int64_t y = in ? target[t] : -1;
             const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
-            const float c = in ? rowfac[t] * unit : 0.f;
+            const float c = in ? rowfac[t] * unit : 0.f, cs = c * st.y;
+            if (split) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const int v0 = m + 16 * i + 4 * q;
-                Pack<G, 4> hi, lo;
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = v0 + e;
-                    float x = 0.f;
-                    if (v < table && c != 0.f) {
-                        const float z = logit(acc[i][j][e], f, lg.bias ? lg.bias[v] : 0.f);
-                        x = c * fmaf(split ? exp_fine(z - st.x) : exp_neg(z - st.x), st.y, v == y ? -1.f : 0.f);
-                    }
-                    hi.v[e] = (G)x;
-                    lo.v[e] = (G)(x - (float)hi.v[e]);
-                }
-                if (in && (size_t)v0 < vp) {
-                    *reinterpret_cast<Pack<G, 4> *>(g + (size_t)t * vp + v0) = hi;
-                    if (split) *reinterpret_cast<Pack<G, 4> *>(g + g_plane + (size_t)t * vp + v0) = lo;
-                }
-                if ((size_t)t < tp) {
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = cs * exp_fine(fmaf(acc[i][j][e], f, -st.x));
+            } else {
+                const float f2 = f * kLog2e, a2 = st.x * kLog2e;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (v0 + e < table) {
-                            gt[(size_t)(v0 + e) * tp + t] = hi.v[e];
-                            if (split) gt[gt_plane + (size_t)(v0 + e) * tp + t] = lo.v[e];
-                        }
-                    }
-                }
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = cs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], f2, -a2));
+            }
+            const int64_t y = in ? target[t] : -1;
+            if (y >= m && y < m + 16 * MB) {
+                const int d = (int)(y - m) - 4 * q;
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d == 16 * i + e) acc[i][j][e] -= c;
+            }
+            if (__any(c == 0.f)) {  // whatever such a row's logits are
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = c == 0.f ? 0.f : acc[i][j][e];
             }
         }
+        auto store = [&](G *p) {
+            return [=, *this](int r, int c, const Pack<G, 8> &v) {
+                if (n + r < tp && (size_t)(m + c) < vp) *reinterpret_cast<Pack<G, 8> *>(p + (size_t)(n + r) * vp + m + c) = v;
+            };
+        };
+        rows_through_lds<G, MB, NB>(lds, [&](int i, int j, int e) { return (G)acc[i][j][e]; }, store(g));
+        if (split)
+            rows_through_lds<G, MB, NB>(
+                lds, [&](int i, int j, int e) { return (G)(acc[i][j][e] - (float)(G)acc[i][j][e]); }, store(g + plane));
     }
 };
 
@@ -356,43 +387,47 @@ struct OutEpi {
     int cols, rows, cols4;
     bool first, last, vec;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl) const {
-        const int l = threadIdx.x & 63, q = l >> 4;
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
         const float f = sc();
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int r = n + 16 * j + (l & 15);
-            if (r >= rows) continue;
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const int c = m + 16 * i + 4 * q;
-                if (c >= cols) continue;
-                if (part) {
-                    *reinterpret_cast<floatx4_t *>(part + ((size_t)pl.part * rows + r) * cols4 + c) = acc[i][j];
-                    continue;
-                }
-                floatx4_t v = acc[i][j] * f;
-                if (sum) {
-                    floatx4_t *s = reinterpret_cast<floatx4_t *>(sum + (size_t)r * cols4 + c);
-                    if (!first) v += *s;
-                    if (!last) {
+        if (part || sum) {
+            float *to = part ? part + (size_t)pl.part * rows * cols4 : sum;
+            rows_through_lds<float, MB, NB>(
+                lds, [&](int i, int j, int e) { return part ? acc[i][j][e] : acc[i][j][e] * f; },
+                [&](int r, int c, const Pack<float, 4> &v) {
+                    if (n + r >= rows || m + c >= cols) return;
+                    Pack<float, 4> *s = reinterpret_cast<Pack<float, 4> *>(to + (size_t)(n + r) * cols4 + m + c);
+                    if (part || (first && !last)) {
                         *s = v;
-                        continue;
+                        return;
                     }
-                }
-                O *o = out + (size_t)r * ld + c;
-                if (vec && c + 4 <= cols) {
-                    Pack<O, 4> p;
+                    Pack<float, 4> u = *s;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p.v[e] = (O)v[e];
-                    *reinterpret_cast<Pack<O, 4> *>(o) = p;
-                } else {
+                    for (int e = 0; e < 4; ++e) u.v[e] += v.v[e];
+                    if (!last) {
+                        *s = u;
+                        return;
+                    }
+                    O *o = out + (size_t)(n + r) * ld + m + c;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (c + e < cols) o[e] = (O)v[e];
-                }
-            }
+                        if (m + c + e < cols) o[e] = (O)u.v[e];
+                });
+            return;
         }
+        constexpr int PER = 16 / (int)sizeof(O);
+        rows_through_lds<O, MB, NB>(
+            lds, [&](int i, int j, int e) { return (O)(acc[i][j][e] * f); },
+            [&](int r, int c, const Pack<O, PER> &v) {
+                if (n + r >= rows || m + c >= cols) return;
+                O *o = out + (size_t)(n + r) * ld + m + c;
+                if (vec && m + c + PER <= cols) {
+                    *reinterpret_cast<Pack<O, PER> *>(o) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (m + c + e < cols) o[e] = v.v[e];
+                }
+            });
     }
 };
 
@@ -411,18 +446,6 @@ __global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts
         for (int e = 0; e < 4; ++e)
             if (c + e < cols) out[(size_t)r * ld + c + e] = (O)v[e];
     }
-}
-
-// Tile of a product.  256 x 256 tiles (8 waves) reach 1.2 PFLOP/s where they fill the chip, 128 x 128 ones
-// (4 waves, two workgroups a CU) 0.85, so the estimate is whole rounds of workgroups times a tile's work.
-inline bool big_tiles(size_t M, size_t N, size_t batch) {
-    const size_t b = (size_t)ceil_div(M, 256) * ceil_div(N, 256) * batch, s = (size_t)ceil_div(M, 128) * ceil_div(N, 128) * batch;
-    return ((b + 255) / 256) * 4 * 10 <= ((s + 511) / 512) * 2 * 14;
-}
-
-template <class P, class Epi>
-int product(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
-    return big ? mm_launch<P, 2, 4, 8, 4>(g, epi, s) : mm_launch<P, 2, 2, 4, 4>(g, epi, s);
 }
 
 struct Sizes {
@@ -454,13 +477,13 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.grad = grad;
     z.kp = round_up(dim, kMmK);
     z.vp = round_up(table, kMmK);
-    const size_t per = z.vp * (dtype == VHIP_DTYPE_F32 ? 8 : 4);
+    const size_t per = z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2);
     size_t fit = piece_bytes() / per / 256 * 256;
     if (fit < 256) fit = 256;
     z.piece_rows = !grad || rows <= fit ? rows : fit;
     z.tp = round_up(z.piece_rows, kMmK);
     z.cols4 = round_up(dim, 4);
-    z.stat_big = big_tiles(table, z.piece_rows, 1);
+    z.stat_big = mm_big_tiles(table, z.piece_rows, 1);
     z.pieces = ceil_div(table, z.stat_big ? 128 : 64);
     z.dh_big = dim > 128 && z.piece_rows > 128;
     const size_t bs = z.dh_big ? 256 : 128, tiles = (size_t)ceil_div(dim, bs) * ceil_div(z.piece_rows, bs);
@@ -468,16 +491,16 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     size_t k = want / tiles;
     if (k > ks / 8) k = ks / 8;
     z.ksplit = (int)(k < 1 ? 1 : k);
-    z.dw_big = big_tiles(dim, table, 1);
+    z.dw_big = mm_big_tiles(dim, table, 1);
     return z;
 }
 
 struct Parts {
     Scalars *sc;
     float2 *part;
-    float2 *stat;
-    float *zt, *rowfac, *split, *sum;
-    void *hp, *wp, *ht, *wt, *g, *gt;
+    float2 *stat, *zt;
+    float *rowfac, *split, *sum;
+    void *hp, *wp, *ht, *g;
 };
 
 inline Parts carve(Carver &c, const Sizes &z) {
@@ -485,16 +508,14 @@ inline Parts carve(Carver &c, const Sizes &z) {
     Parts p{};
     p.sc = c.take<Scalars>(1);
     p.part = c.take<float2>((size_t)z.pieces * z.piece_rows);
-    p.zt = c.take<float>(z.piece_rows);
+    p.zt = c.take<float2>(z.piece_rows);
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
         p.stat = c.take<float2>(z.piece_rows);
         p.rowfac = c.take<float>(z.piece_rows);
         p.ht = c.take<uint16_t>(planes * z.dim * z.tp);
-        p.wt = c.take<uint16_t>(planes * z.dim * z.vp);
-        p.g = c.take<uint16_t>(planes * z.piece_rows * z.vp);
-        p.gt = c.take<uint16_t>(planes * z.table * z.tp);
+        p.g = c.take<uint16_t>(planes * z.tp * z.vp);
         if (z.ksplit > 1) p.split = c.take<float>((size_t)z.ksplit * z.piece_rows * z.cols4);
         if (z.piece_rows < z.rows) p.sum = c.take<float>(z.table * z.cols4);
     }
@@ -537,14 +558,13 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
-    if (!direct<T>(c.table, c.ldt, z.dim)) {
-        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, z.table * z.kp, (int)z.kp, &p.sc->amax_w);
+    if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
+        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, z.table * z.kp, (int)z.kp,
+                                                                  &p.sc->amax_w, (const float *)c.bias);
         wp = (const P *)p.wp;
         ldw = z.kp;
     }
-    if (z.grad)
-        k_pack_t<T><<<dim3((uint32_t)(z.vp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
-            w, z.table, dim, c.ldt, (P *)p.wt, z.dim * z.vp, z.vp, &p.sc->amax_w, nullptr, (const float *)c.bias);
+    const size_t w_plane = kSplit ? z.table * z.kp : 0;
 
     for (size_t r0 = 0; r0 < z.rows; r0 += z.piece_rows) {
         const size_t rows = z.rows - r0 < z.piece_rows ? z.rows - r0 : z.piece_rows;
@@ -553,13 +573,14 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, z.piece_rows * z.kp, (int)z.kp, &p.sc->amax_h);
+            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, z.piece_rows * z.kp, (int)z.kp,
+                                                                &p.sc->amax_h, nullptr);
             hp = (const P *)p.hp;
             ldh = z.kp;
         }
         MmArgs g{};
         g.a[0] = wp;
-        g.a[1] = kSplit ? wp + z.table * z.kp : wp;
+        g.a[1] = wp + w_plane;
         g.b[0] = hp;
         g.b[1] = kSplit ? hp + z.piece_rows * z.kp : hp;
         g.lda = ldw;
@@ -570,7 +591,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.nseg = kSplit ? 3 : 1;
         g.ksplit = g.batch = 1;
         const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
-        VH_CHECK(product<P>(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
+        VH_CHECK((mm_launch<P, false, false>)(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
         k_xent_join<<<(uint32_t)ceil_div(rows, 16), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table,
                                                                 c.row_weight ? c.row_weight + r0 : nullptr, c.scale,
                                                                 c.loss ? c.loss + r0 : nullptr, c.lse ? c.lse + r0 : nullptr,
@@ -578,58 +599,61 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         VH_CHECK(launch_status("softmax launch"));
         if (!z.grad) continue;
         const size_t tp = round_up(rows, kMmK);
-        k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
-            hr, rows, dim, c.ldh, (P *)p.ht, z.dim * z.tp, tp, &p.sc->amax_h, target, nullptr);
         GradEpi<P> ge{};
         ge.lg = lg;
         ge.stat = p.stat;
         ge.rowfac = p.rowfac;
         ge.target = target;
         ge.g = (P *)p.g;
-        ge.gt = (P *)p.gt;
-        ge.g_plane = z.piece_rows * z.vp;
-        ge.gt_plane = z.table * z.tp;
+        ge.plane = kSplit ? z.tp * z.vp : 0;
         ge.vp = z.vp;
-        ge.tp = tp;
         ge.rows = (int)rows;
+        ge.tp = (int)tp;
         ge.table = table;
         ge.split = kSplit;
-        VH_CHECK(product<P>(g, z.stat_big, ge, s));
+        VH_CHECK((mm_launch<P, false, false>)(g, z.stat_big, ge, s));
+        const P *gg = (const P *)p.g;
         if (c.dh) {
+            // columns of the table, K its rows: G's columns past the table are zeros
             MmArgs d = g;
-            const P *wt = (const P *)p.wt, *gg = (const P *)p.g;
-            d.a[0] = wt;
-            d.a[1] = wt + (kSplit ? z.dim * z.vp : 0);
             d.b[0] = gg;
-            d.b[1] = gg + (kSplit ? z.piece_rows * z.vp : 0);
-            d.lda = d.ldb = z.vp;
+            d.b[1] = gg + ge.plane;
+            d.ldb = z.vp;
             d.M = dim;
             d.N = (int)rows;
             d.ktiles = (int)(z.vp / kMmK);
+            d.ka = table;
             d.ksplit = z.ksplit;
             const OutScale os{p.sc, kSplit, false};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
-                         true, true, c.lddh % 4 == 0 && aligned16(out)};
-            VH_CHECK(product<P>(d, z.dh_big, oe, s));
+                         true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
+            VH_CHECK((mm_launch<P, true, false>)(d, z.dh_big, oe, s));
             if (z.ksplit > 1)
                 k_join_parts<T><<<wide_grid(rows * z.cols4 / 4), 256, 0, s>>>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh);
         }
         if (c.dtable) {
-            MmArgs d = g;
-            const P *ht = (const P *)p.ht, *gt = (const P *)p.gt;
+            // K the rows: those past the last are zeros in both operands, those that do not count in the first
+            k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
+                hr, rows, dim, c.ldh, (P *)p.ht, z.dim * z.tp, tp, &p.sc->amax_h, target);
+            MmArgs d{};
+            const P *ht = (const P *)p.ht;
             d.a[0] = ht;
             d.a[1] = ht + (kSplit ? z.dim * z.tp : 0);
-            d.b[0] = gt;
-            d.b[1] = gt + (kSplit ? z.table * z.tp : 0);
-            d.lda = d.ldb = tp;
+            d.b[0] = gg;
+            d.b[1] = gg + ge.plane;
+            d.lda = tp;
+            d.ldb = z.vp;
             d.M = dim;
             d.N = table;
             d.ktiles = (int)(tp / kMmK);
+            d.kb = (int)tp;
+            d.nseg = g.nseg;
+            d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
             OutEpi<T> oe{OutScale{p.sc, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
-                         (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % 4 == 0 && aligned16(c.dtable)};
-            VH_CHECK(product<P>(d, z.dw_big, oe, s));
+                         (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % (16 / sizeof(T)) == 0 && aligned16(c.dtable)};
+            VH_CHECK((mm_launch<P, false, true>)(d, z.dw_big, oe, s));
         }
         VH_CHECK(launch_status("gradient launch"));
     }

@@ -5,8 +5,8 @@
 * ``orthogonalize``                              Newton-Schulz steps on update matrices
 
 They have no counterpart in the reference.  Arguments are arrays in the memory of one GPU: objects with the
-tensor interface ``data_ptr() / dtype / shape / stride() / device / new_empty()`` (torch's, which this module
-does not need itself: outputs and working memory come from the arguments' own ``new_empty``).  Element types
+tensor interface of torch (``data_ptr()``, ``stride()``, ``new_empty()`` and so on), which this module does not
+load itself: outputs and working memory come from the arguments' own ``new_empty``.  Element types
 are float32, float16 and bfloat16.  The last dimension is contiguous; rows may be any distance apart.
 
 A call enqueues its work on the current stream of its arguments' device and returns without waiting, as
@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import ctypes
 import sys
-from typing import Optional, Tuple
 
 from . import InvalidConfig, _check, _lib, _sig, _sz
 
@@ -38,107 +37,102 @@ _sig("vhip_orthogonalize_workspace", _sz, _sz, _sz, _sz)
 _sig("vhip_orthogonalize", _int, _int, _int, _p, _sz, _sz, _sz, _sz, _sz, _int, _f, _f, _f, _f, _p, _sz, _sz, _p, _sz,
      _p)
 
-_codes = {}   # dtype object -> code
-_tensors = {}  # dtype class -> (library, its float32, uint8 and int64)
+class _Types(dict):
+    """dtype object -> code"""
 
-
-def _code(dtype) -> int:
-    c = _codes.get(dtype)
-    if c is None:
-        c = _NAMES.get(str(dtype))
-        if c is None:
+    def __missing__(self, dtype):
+        code = _NAMES.get(str(dtype))
+        if code is None:
             raise InvalidConfig(f"element type {dtype} is not float32, float16 or bfloat16")
-        _codes[dtype] = c
-    return c
+        self[dtype] = code
+        return code
 
 
-def _library(a):
-    """The library that the caller's arrays come from, with the types that calls make outputs of."""
-    kind = type(a.dtype)
-    got = _tensors.get(kind)
-    if got is None:
-        lib = sys.modules[kind.__module__]
-        got = _tensors[kind] = (lib, lib.float32, lib.uint8, lib.int64)
-    return got
+_code = _Types()
+
+
+class _Library:
+    """What calls need of the library that the caller's arrays come from: the types that they make outputs
+    of, and the current stream of a device (by the quicker of the two ways where it has both)."""
+
+    def __init__(self, lib):
+        self.f32, self.u8, self.i64 = lib.float32, lib.uint8, lib.int64
+        current = lib.cuda.current_stream
+        self.stream = getattr(lib._C, "_cuda_getCurrentRawStream", lambda index: current(index).cuda_stream)
+
+
+class _Libraries(dict):
+    """dtype class -> _Library"""
+
+    def __missing__(self, kind):
+        got = self[kind] = _Library(sys.modules[kind.__module__])
+        return got
+
+
+_library = _Libraries()
 
 
 def _on_gpu(name, a):
-    if not hasattr(a, "data_ptr") or not hasattr(a, "new_empty"):
-        raise InvalidConfig(f"{name} is not a GPU array")
-    if a.device.type != "cuda":
-        raise InvalidConfig(f"{name} is not in GPU memory")
+    if not getattr(a, "is_cuda", False):
+        raise InvalidConfig(f"{name} is not an array in GPU memory")
 
 
 def _rows2(name, a, like=None) -> int:
     """Checks a matrix of contiguous rows; its distance between rows."""
-    _on_gpu(name, a)
-    if a.dim() != 2:
+    if not getattr(a, "is_cuda", False):
+        _on_gpu(name, a)
+    st = a.stride()
+    if len(st) != 2:
         raise InvalidConfig(f"{name} must have two dimensions")
-    if like is not None and (a.dtype != like.dtype or a.device != like.device):
+    if like is not None and (a.dtype != like.dtype or a.get_device() != like.get_device()):
         raise InvalidConfig(f"{name} must have the type and the device of the other rows")
-    ld, one = a.stride()
     n, d = a.shape
-    if one != 1 and d > 1:
+    if st[1] != 1 and d > 1:
         raise InvalidConfig(f"the values of a row of {name} must be contiguous")
     if n <= 1:
         return d
-    if ld < d:
+    if st[0] < d:
         raise InvalidConfig(f"rows of {name} overlap")
-    return ld
+    return st[0]
 
 
-def _vector(name, a, n, like, dtype=None):
-    _on_gpu(name, a)
-    if a.dim() != 1 or a.shape[0] != n or (n > 1 and a.stride(0) != 1):
+def _vector(name, a, n, device, dtype=None) -> int:
+    """Checks n contiguous values; their address."""
+    if not getattr(a, "is_cuda", False):
+        _on_gpu(name, a)
+    if a.shape != (n,) or not a.is_contiguous():
         raise InvalidConfig(f"{name} must hold {n} contiguous values")
-    if a.device != like.device:
+    if a.get_device() != device:
         raise InvalidConfig(f"{name} is on another device")
     if dtype is not None and a.dtype != dtype:
         raise InvalidConfig(f"{name} must be of {dtype}")
+    return a.data_ptr()
 
 
-def _ptr(a) -> Optional[int]:
-    return None if a is None else a.data_ptr()
-
-
-def _place(lib, a) -> Tuple[int, int]:
-    s = lib.cuda.current_stream(a.device)
-    return s.device_index, s.cuda_stream
-
-
-def _params(x, weight, bias):
-    """Checks a layer norm's parameters; the code of their type."""
-    code = None
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        _vector(name, p, x.shape[1], x)
-        c = _code(p.dtype)
-        if code is not None and c != code:
-            raise InvalidConfig("weight and bias must have the same type")
-        code = c
-    return _param_code(code, x)
-
-
-def _param_code(code, x) -> int:
-    if code is None:
-        return _code(x.dtype)
-    if code not in (F32, _code(x.dtype)):
+def _param_code(dtype, code) -> int:
+    c = _code[dtype]
+    if c != F32 and c != code:
         raise InvalidConfig("parameters must have the rows' type or float32")
-    return code
+    return c
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """(y, mean, rstd): y = (x - mean) rstd weight + bias over the last dimension of x [rows, dim], with
     rstd = 1 / sqrt(variance + eps).  y has x's type; the statistics are float32."""
     ldx = _rows2("x", x)
-    lib, f32, _, _ = _library(x)
     rows, dim = x.shape
-    params = _params(x, weight, bias)
-    y, mean, rstd = x.new_empty((rows, dim)), x.new_empty((rows,), dtype=f32), x.new_empty((rows,), dtype=f32)
-    ordinal, stream = _place(lib, x)
-    _check(_lib.vhip_layer_norm(ordinal, _code(x.dtype), params, x.data_ptr(), rows, dim, ldx, _ptr(weight), _ptr(bias),
-                                eps, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr(), stream))
+    device, code, lib = x.get_device(), _code[x.dtype], _library[type(x.dtype)]
+    params, w, b = code, None, None
+    if weight is not None:
+        w, params = _vector("weight", weight, dim, device), _param_code(weight.dtype, code)
+    if bias is not None:
+        b, params = _vector("bias", bias, dim, device), _param_code(bias.dtype, code)
+        if weight is not None and bias.dtype != weight.dtype:
+            raise InvalidConfig("weight and bias must have the same type")
+    y = x.new_empty((rows, dim))
+    mean, rstd = x.new_empty((2, rows), dtype=lib.f32).unbind()
+    _check(_lib.vhip_layer_norm(device, code, params, x.data_ptr(), rows, dim, ldx, w, b, eps, y.data_ptr(), dim,
+                                mean.data_ptr(), rstd.data_ptr(), lib.stream(device)))
     return y, mean, rstd
 
 
@@ -146,74 +140,66 @@ def layer_norm_backward(dy, x, weight, mean, rstd, param_dtype=None):
     """(dx, dweight, dbias) from the gradient of layer_norm's y, its x and weight (or None) and its statistics.
     The parameters' gradients have the weight's type; without a weight `param_dtype` (x's type by default)."""
     ldx, lddy = _rows2("x", x), _rows2("dy", dy, x)
-    lib, f32, u8, _ = _library(x)
     rows, dim = x.shape
-    if tuple(dy.shape) != (rows, dim):
+    if dy.shape != x.shape:
         raise InvalidConfig("dy must have the shape of x")
-    _vector("mean", mean, rows, x, f32)
-    _vector("rstd", rstd, rows, x, f32)
-    params = _params(x, weight, None)
-    ptype = weight.dtype if weight is not None else x.dtype
-    if weight is None and param_dtype is not None:
-        ptype, params = param_dtype, _param_code(_code(param_dtype), x)
-    dx, dweight, dbias = x.new_empty((rows, dim)), x.new_empty((dim,), dtype=ptype), x.new_empty((dim,), dtype=ptype)
+    device, code, lib = x.get_device(), _code[x.dtype], _library[type(x.dtype)]
+    m, r = _vector("mean", mean, rows, device, lib.f32), _vector("rstd", rstd, rows, device, lib.f32)
+    w = None
+    if weight is not None:
+        w, param_dtype = _vector("weight", weight, dim, device), weight.dtype
+    elif param_dtype is None:
+        param_dtype = x.dtype
+    params = _param_code(param_dtype, code)
+    dx = x.new_empty((rows, dim))
+    dweight, dbias = x.new_empty((2, dim), dtype=param_dtype).unbind()
     need = _lib.vhip_layer_norm_backward_workspace(rows, dim)
-    ws = x.new_empty((need,), dtype=u8)
-    ordinal, stream = _place(lib, x)
-    _check(_lib.vhip_layer_norm_backward(ordinal, _code(x.dtype), params, dy.data_ptr(), lddy, x.data_ptr(), ldx,
-                                         _ptr(weight), mean.data_ptr(), rstd.data_ptr(), rows, dim, dx.data_ptr(), dim,
-                                         dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), need, stream))
+    ws = x.new_empty(need, dtype=lib.u8)
+    _check(_lib.vhip_layer_norm_backward(device, code, params, dy.data_ptr(), lddy, x.data_ptr(), ldx, w, m, r, rows, dim,
+                                         dx.data_ptr(), dim, dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), need,
+                                         lib.stream(device)))
     return dx, dweight, dbias
 
 
-def _xent_args(h, table, target, bias, row_weight):
+def _xent_args(h, table, target, bias):
     ldh, ldt = _rows2("h", h), _rows2("table", table, h)
-    lib, f32, u8, i64 = _library(h)
     rows, dim = h.shape
-    if table.shape[1] != dim:
-        raise InvalidConfig(f"rows have {dim} elements, the table's have {table.shape[1]}")
-    if table.shape[0] == 0:
+    n, d = table.shape
+    if d != dim:
+        raise InvalidConfig(f"rows have {dim} elements, the table's have {d}")
+    if n == 0:
         raise InvalidConfig("the table is empty")
-    _vector("target", target, rows, h, i64)
-    if bias is not None:
-        _vector("bias", bias, table.shape[0], h, f32)
-    if row_weight is not None:
-        _vector("row_weight", row_weight, rows, h, f32)
-    return ldh, ldt, lib, f32, u8
+    device, lib = h.get_device(), _library[type(h.dtype)]
+    y = _vector("target", target, rows, device, lib.i64)
+    b = None if bias is None else _vector("bias", bias, n, device, lib.f32)
+    return rows, n, dim, ldh, ldt, device, _code[h.dtype], lib, y, b
 
 
 def softmax_xent(h, table, target, scale: float = 1.0, bias=None):
     """(loss, lse) of the rows of h [rows, dim] against every row of table [n, dim], float32 each:
     z = scale h table^T + bias, lse = log sum exp z, loss = lse - z[target].  target is int64; a negative one
     has loss 0.  bias (float32, constant) may hold -inf, which leaves an entry out."""
-    ldh, ldt, lib, f32, u8 = _xent_args(h, table, target, bias, None)
-    rows, dim = h.shape
-    n, code = table.shape[0], _code(h.dtype)
-    loss, lse = h.new_empty((rows,), dtype=f32), h.new_empty((rows,), dtype=f32)
+    rows, n, dim, ldh, ldt, device, code, lib, y, b = _xent_args(h, table, target, bias)
+    loss, lse = h.new_empty((2, rows), dtype=lib.f32).unbind()
     need = _lib.vhip_softmax_xent_workspace(code, rows, n, dim, 0)
-    ws = h.new_empty((need,), dtype=u8)
-    ordinal, stream = _place(lib, h)
-    _check(_lib.vhip_softmax_xent(ordinal, code, h.data_ptr(), rows, ldh, table.data_ptr(), n, ldt, dim,
-                                  target.data_ptr(), _ptr(bias), scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
-                                  need, stream))
+    ws = h.new_empty(need, dtype=lib.u8)
+    _check(_lib.vhip_softmax_xent(device, code, h.data_ptr(), rows, ldh, table.data_ptr(), n, ldt, dim, y, b, scale,
+                                  loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
     return loss, lse
 
 
 def softmax_xent_grad(h, table, target, row_weight=None, scale: float = 1.0, bias=None):
     """(loss, lse, dh, dtable): softmax_xent with the gradients of sum(row_weight * loss) for h and the table,
     in their type.  row_weight (float32) is 1 everywhere by default; 1 / (number of targets) gives the mean."""
-    ldh, ldt, lib, f32, u8 = _xent_args(h, table, target, bias, row_weight)
-    rows, dim = h.shape
-    n, code = table.shape[0], _code(h.dtype)
-    loss, lse = h.new_empty((rows,), dtype=f32), h.new_empty((rows,), dtype=f32)
+    rows, n, dim, ldh, ldt, device, code, lib, y, b = _xent_args(h, table, target, bias)
+    c = None if row_weight is None else _vector("row_weight", row_weight, rows, device, lib.f32)
+    loss, lse = h.new_empty((2, rows), dtype=lib.f32).unbind()
     dh, dtable = h.new_empty((rows, dim)), h.new_empty((n, dim))
     need = _lib.vhip_softmax_xent_workspace(code, rows, n, dim, 1)
-    ws = h.new_empty((need,), dtype=u8)
-    ordinal, stream = _place(lib, h)
-    _check(_lib.vhip_softmax_xent_grad(ordinal, code, h.data_ptr(), rows, ldh, table.data_ptr(), n, ldt, dim,
-                                       target.data_ptr(), _ptr(bias), _ptr(row_weight), scale, loss.data_ptr(),
-                                       lse.data_ptr(), dh.data_ptr(), dim, dtable.data_ptr(), dim, ws.data_ptr(), need,
-                                       stream))
+    ws = h.new_empty(need, dtype=lib.u8)
+    _check(_lib.vhip_softmax_xent_grad(device, code, h.data_ptr(), rows, ldh, table.data_ptr(), n, ldt, dim, y, b, c, scale,
+                                       loss.data_ptr(), lse.data_ptr(), dh.data_ptr(), dim, dtable.data_ptr(), dim,
+                                       ws.data_ptr(), need, lib.stream(device)))
     return loss, lse, dh, dtable
 
 
@@ -232,12 +218,11 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
     if ld < cols:
         raise InvalidConfig("rows of update overlap")
     a, b, c = coefficients
-    lib, _, u8, _ = _library(update)
-    out = update.new_empty(tuple(update.shape))
+    device, code, lib = update.get_device(), _code[update.dtype], _library[type(update.dtype)]
+    out = update.new_empty(update.shape)
     need = _lib.vhip_orthogonalize_workspace(count, rows, cols)
-    ws = update.new_empty((need,), dtype=u8)
-    ordinal, stream = _place(lib, update)
-    _check(_lib.vhip_orthogonalize(ordinal, _code(update.dtype), update.data_ptr(), count, rows, cols, ld,
+    ws = update.new_empty(need, dtype=lib.u8)
+    _check(_lib.vhip_orthogonalize(device, code, update.data_ptr(), count, rows, cols, ld,
                                    st[0] if update.dim() == 3 else 0, steps, a, b, c, eps, out.data_ptr(), cols,
-                                   rows * cols, ws.data_ptr(), need, stream))
+                                   rows * cols, ws.data_ptr(), need, lib.stream(device)))
     return out

@@ -20,7 +20,7 @@
 // values (its h is replaced by zeros where sums over rows are made).  An entry whose bias is -inf is out of
 // the softmax whatever its values.  A row whose target is out, or that has nothing left in, has loss +inf
 // and no part in the gradients.  A target past the table gives NaN.
-#include "mm16.h"
+#include "xent_small.h"
 
 #include <cmath>
 #include <cstdlib>
@@ -28,7 +28,6 @@
 namespace vh {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G
 constexpr int kGBits = 14;
 
@@ -45,15 +44,6 @@ __device__ __forceinline__ float unit_scale(uint32_t bits) {
     int k = kGBits - e;
     k = k > 120 ? 120 : (k < -120 ? -120 : k);
     return ldexpf(1.f, k);
-}
-
-__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-// exp to 32-bit accuracy: what x log2(e) loses in rounding is put back to first order
-__device__ __forceinline__ float exp_fine(float x) {
-    const float t = x * kLog2e;
-    const float r = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return t > -150.f && t < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
 }
 
 __global__ void k_xent_init(Scalars *s) {
@@ -241,16 +231,18 @@ struct StatEpi {
     }
 };
 
-// Joins the pieces: 16 rows a workgroup, 16 lanes of a row each taking every sixteenth piece.
+// Joins the pieces: R rows a workgroup, 256 / R lanes of a row each taking every (256 / R)th piece.
+template <int R>
 __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float2 *zt,
                                                    const int64_t *target, int64_t table, const float *weight,
                                                    float scale, float *loss, float *lse, float2 *stat,
                                                    float *rowfac, Scalars *sc) {
-    __shared__ float s_top[16][17], s_sum[16][17];
-    const int k = threadIdx.x & 15, g = threadIdx.x >> 4, t = blockIdx.x * 16 + k;
+    constexpr int L0 = 256 / R;
+    __shared__ float s_top[L0][R + 1], s_sum[L0][R + 1];
+    const int k = threadIdx.x % R, g = threadIdx.x / R, t = blockIdx.x * R + k;
     float top = -INFINITY, sum = 0.f;
     if (t < rows) {
-        for (int p = g; p < pieces; p += 16) {
+        for (int p = g; p < pieces; p += L0) {
             const float2 v = part[(size_t)p * rows + t];
             const float m = fmaxf(top, v.x), about = m == -INFINITY ? 0.f : m;
             sum = sum * exp_neg(top - about) + v.y * exp_neg(v.x - about);
@@ -259,12 +251,18 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int piece
     }
     s_top[g][k] = top;
     s_sum[g][k] = sum;
-    __syncthreads();
+    for (int h = L0 / 2; h > 0; h /= 2) {
+        __syncthreads();
+        if (g < h) {
+            const float m2 = s_top[g + h][k], m = fmaxf(top, m2), about = m == -INFINITY ? 0.f : m;
+            sum = sum * exp_neg(top - about) + s_sum[g + h][k] * exp_neg(m2 - about);
+            top = m;
+            s_top[g][k] = top;
+            s_sum[g][k] = sum;
+        }
+    }
     if (g != 0) return;
-    for (int p = 1; p < 16; ++p) top = fmaxf(top, s_top[p][k]);
     const float about = top == -INFINITY ? 0.f : top;
-    sum = 0.f;
-    for (int p = 0; p < 16; ++p) sum += s_sum[p][k] * exp_neg(s_top[p][k] - about);
     const float L = sum == 0.f ? -INFINITY : about + logf(sum);
     const int64_t y = t < rows ? target[t] : -1;
     float ls = 0.f, fac = 0.f;
@@ -284,12 +282,12 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int piece
             rowfac[t] = fac;
         }
     }
-    if (rowfac) {
+    if (sc) {
         uint32_t u = __builtin_bit_cast(uint32_t, fac) & 0x7fffffffu;
         if (u >= 0x7f800000u) u = 0;
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            const uint32_t v = __shfl_xor(u, o, 16);
+        for (int o = 1; o < R; o <<= 1) {
+            const uint32_t v = __shfl_xor(u, o, 64);
             u = v > u ? v : u;
         }
         if (k == 0 && u) atomicMax(&sc->cmax, u);
@@ -431,21 +429,34 @@ struct OutEpi {
     }
 };
 
-// Adds the parts of a split K loop.
+// Adds the parts of a split K loop: 32 vectors of four values a workgroup, its 8 groups of lanes every
+// eighth part.
 template <class O>
 __global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts, int rows, int cols, int cols4,
                                                     OutScale sc, O *out, size_t ld) {
-    const float f = sc();
-    const size_t n = (size_t)rows * (cols4 / 4);
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const int r = (int)(i / (cols4 / 4)), c = (int)(i % (cols4 / 4)) * 4;
-        floatx4_t v = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < parts; ++p) v += *reinterpret_cast<const floatx4_t *>(part + ((size_t)p * rows + r) * cols4 + c);
-        v *= f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < cols) out[(size_t)r * ld + c + e] = (O)v[e];
+    __shared__ floatx4_t sums[8][32];
+    const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const size_t at = (size_t)blockIdx.x * 32 + l, n = (size_t)rows * (cols4 / 4);
+    floatx4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (at < n) {
+#pragma unroll 4
+        for (int p = g; p < parts; p += 8) v += *reinterpret_cast<const floatx4_t *>(part + (p * n + at) * 4);
     }
+    sums[g][l] = v;
+    __syncthreads();
+    if (g != 0 || at >= n) return;
+#pragma unroll
+    for (int p = 1; p < 8; ++p) v += sums[p][l];
+    v *= sc.sc ? sc() : 1.f;
+    const int r = (int)(at / (cols4 / 4)), c = (int)(at % (cols4 / 4)) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c + e < cols) out[(size_t)r * ld + c + e] = (O)v[e];
+}
+template <class O>
+void join_parts(const float *part, int parts, int rows, int cols, int cols4, OutScale sc, O *out, size_t ld, hipStream_t s) {
+    const size_t n = (size_t)rows * (cols4 / 4);
+    k_join_parts<O><<<(uint32_t)((n + 31) / 32), 256, 0, s>>>(part, parts, rows, cols, cols4, sc, out, ld);
 }
 
 struct Sizes {
@@ -453,6 +464,7 @@ struct Sizes {
     size_t rows, table, dim;
     bool grad;
     size_t kp, vp, piece_rows, tp, cols4;
+    bool small;       // few rows: xent_small.h
     bool stat_big;
     int pieces;       // of a row's logits
     bool dh_big, dw_big;
@@ -477,12 +489,22 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.grad = grad;
     z.kp = round_up(dim, kMmK);
     z.vp = round_up(table, kMmK);
+    z.cols4 = round_up(dim, 4);
+    z.small = rows <= (size_t)kSmallRows;
+    if (z.small) {
+        z.piece_rows = rows;
+        const size_t groups = (table + 15) / 16, tiles = (table + 63) / 64, ny = ceil_div(dim, vh::kSmallCols);
+        z.pieces = (int)(groups < 2048 ? groups : 2048);
+        size_t gx = 1024 / ny;
+        if (gx < 64) gx = 64;
+        z.ksplit = (int)(tiles < gx ? tiles : gx);
+        return z;
+    }
     const size_t per = z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2);
     size_t fit = piece_bytes() / per / 256 * 256;
     if (fit < 256) fit = 256;
     z.piece_rows = !grad || rows <= fit ? rows : fit;
     z.tp = round_up(z.piece_rows, kMmK);
-    z.cols4 = round_up(dim, 4);
     z.stat_big = mm_big_tiles(table, z.piece_rows, 1);
     z.pieces = ceil_div(table, z.stat_big ? 128 : 64);
     z.dh_big = dim > 128 && z.piece_rows > 128;
@@ -500,6 +522,7 @@ struct Parts {
     float2 *part;
     float2 *stat, *zt;
     float *rowfac, *split, *sum;
+    float *z;  // few rows: the logits
     void *hp, *wp, *ht, *g;
 };
 
@@ -509,6 +532,15 @@ inline Parts carve(Carver &c, const Sizes &z) {
     p.sc = c.take<Scalars>(1);
     p.part = c.take<float2>((size_t)z.pieces * z.piece_rows);
     p.zt = c.take<float2>(z.piece_rows);
+    if (z.small) {
+        if (z.grad) {
+            p.stat = c.take<float2>(z.rows);
+            p.rowfac = c.take<float>(z.rows);
+            p.z = c.take<float>(z.rows * z.vp);
+            p.split = c.take<float>((size_t)z.ksplit * z.rows * z.cols4);
+        }
+        return p;
+    }
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
@@ -538,6 +570,38 @@ struct Call {
     size_t lddh, lddt;
 };
 
+// The pieces' join: as many rows a workgroup as still fill the chip.
+inline void join_pieces(const Parts &p, const Sizes &z, size_t rows, const int64_t *target, const float *weight, float scale,
+                        float *loss, float *lse, hipStream_t s) {
+    Scalars *sc = z.grad && !z.small ? p.sc : nullptr;
+#define JOIN(R)                                                                                                       \
+    k_xent_join<R><<<(uint32_t)ceil_div(rows, R), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table, \
+                                                               weight, scale, loss, lse, p.stat, p.rowfac, sc)
+    if (rows <= 512)
+        JOIN(1);
+    else if (rows <= 8192)
+        JOIN(4);
+    else
+        JOIN(16);
+#undef JOIN
+}
+
+template <class T>
+int xent_small(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
+    const int dim = (int)z.dim, table = (int)z.table, rows = (int)z.rows;
+    small_stat<T>(SmallStat{c.h, c.table, (const float *)c.bias, c.target, p.part, p.zt, p.z, c.ldh, c.ldt, z.vp, rows, table, dim, c.scale},
+                  (uint32_t)z.pieces, s);
+    join_pieces(p, z, z.rows, c.target, c.row_weight, c.scale, c.loss, c.lse, s);
+    if (z.grad) {
+        const bool vec = c.lddt % 4 == 0 && ((uintptr_t)c.dtable & (4 * sizeof(T) - 1)) == 0;
+        small_grad<T>(SmallGrad{c.h, c.table, (const float *)c.bias, p.z, p.rowfac, p.stat, c.target, c.dtable, c.dh ? p.split : nullptr,
+                                c.ldh, c.ldt, c.lddt, z.vp, rows, table, dim, (int)z.cols4, vec},
+                      (uint32_t)z.ksplit, s);
+        if (c.dh) join_parts<T>(p.split, z.ksplit, rows, dim, (int)z.cols4, OutScale{}, (T *)c.dh, c.lddh, s);
+    }
+    return launch_status("softmax launch");
+}
+
 // Whether rows can be multiplied where they lie.
 template <class T>
 bool direct(const void *p, size_t ld, size_t dim) {
@@ -551,7 +615,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
-    k_xent_init<<<1, 64, 0, s>>>(p.sc);
+    if (kSplit || z.grad) k_xent_init<<<1, 64, 0, s>>>(p.sc);
     if constexpr (kSplit) {
         k_amax<<<(uint32_t)(z.rows < 1024 ? z.rows : 1024), 256, 0, s>>>((const float *)c.h, z.rows, dim, c.ldh, &p.sc->amax_h);
         k_amax<<<(uint32_t)(z.table < 1024 ? z.table : 1024), 256, 0, s>>>((const float *)c.table, z.table, dim, c.ldt, &p.sc->amax_w);
@@ -592,10 +656,8 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.ksplit = g.batch = 1;
         const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
         VH_CHECK((mm_launch<P, false, false>)(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
-        k_xent_join<<<(uint32_t)ceil_div(rows, 16), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table,
-                                                                c.row_weight ? c.row_weight + r0 : nullptr, c.scale,
-                                                                c.loss ? c.loss + r0 : nullptr, c.lse ? c.lse + r0 : nullptr,
-                                                                p.stat, p.rowfac, p.sc);
+        join_pieces(p, z, rows, target, c.row_weight ? c.row_weight + r0 : nullptr, c.scale, c.loss ? c.loss + r0 : nullptr,
+                    c.lse ? c.lse + r0 : nullptr, s);
         VH_CHECK(launch_status("softmax launch"));
         if (!z.grad) continue;
         const size_t tp = round_up(rows, kMmK);
@@ -630,7 +692,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
                          true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
             VH_CHECK((mm_launch<P, true, false>)(d, z.dh_big, oe, s));
             if (z.ksplit > 1)
-                k_join_parts<T><<<wide_grid(rows * z.cols4 / 4), 256, 0, s>>>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh);
+                join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
         }
         if (c.dtable) {
             // K the rows: those past the last are zeros in both operands, those that do not count in the first
@@ -691,6 +753,13 @@ int run(int ordinal, int dtype, const Call &c, size_t rows, size_t table, size_t
         const size_t es = dtype_size(dtype);
         k_zero_rows<<<(uint32_t)(table < 4096 ? table : 4096), 256, 0, s>>>((char *)c.dtable, table, dim * es, c.lddt * es);
         return launch_status("gradient launch");
+    }
+    if (z.small) {
+        switch (dtype) {
+            case VHIP_DTYPE_F32: return xent_small<float>(c, z, p, s);
+            case VHIP_DTYPE_F16: return xent_small<half_t>(c, z, p, s);
+            default: return xent_small<bf16_t>(c, z, p, s);
+        }
     }
     switch (dtype) {
         case VHIP_DTYPE_F32: return xent<float>(c, z, p, s);

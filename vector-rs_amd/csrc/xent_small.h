@@ -1,0 +1,333 @@
+// xent_small.h -- softmax cross entropy of up to 64 rows (included by softmax_xent.hip).
+//
+// With few rows the table is what costs: the products of softmax_xent.hip would run tiles that are mostly
+// clamped rows, and 32-bit tables would first be turned into planes.  Here the table is read from memory
+// straight into matrix operands, twice in all for the gradients:
+//  * k_small_stat makes the logits, and keeps them where gradients follow (64 rows of them are less than a
+//    table of 64 columns).  A workgroup takes 16 entries at a time; its four waves share the K loop, so a CU
+//    has enough loads in flight for short tables too.  32-bit operands are multiplied as they are, in the
+//    32-bit matrix instruction (157 TFLOP/s: above the memory's rate up to 48 rows).
+//  * k_small_grad turns 64 entries' logits into G in LDS, writes these entries' rows of the table's gradient
+//    and adds the rows' gradient up in registers; the workgroups' sums are joined afterwards.  G is not
+//    rounded here, and 16-bit operands are widened.
+#pragma once
+
+#include "mm16.h"
+
+namespace vh {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// exp to 32-bit accuracy: what x log2(e) loses in rounding is put back to first order
+__device__ __forceinline__ float exp_fine(float x) {
+    const float t = x * kLog2e;
+    const float r = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t > -150.f && t < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
+}
+
+constexpr int kSmallRows = 64;
+
+// Values of one lane in a K step of the logits.
+template <class T>
+struct SmallStep {
+    typedef typename MmVec<T>::v8 vec;
+    static constexpr int E = 8, K = 32;
+    static __device__ __forceinline__ floatx4_t mfma(vec a, vec b, floatx4_t c) { return MmVec<T>::mfma(a, b, c); }
+};
+template <>
+struct SmallStep<float> {
+    typedef floatx4_t vec;
+    static constexpr int E = 4, K = 16;
+    static __device__ __forceinline__ floatx4_t mfma(vec a, vec b, floatx4_t c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// E values of a row from column c on, zeros past dim.
+template <class T, bool VEC>
+__device__ __forceinline__ typename SmallStep<T>::vec small_load(const T *row, int c, int dim) {
+    typedef typename SmallStep<T>::vec vec;
+    vec v;
+    if constexpr (VEC) {
+        if (c < dim) return *reinterpret_cast<const vec *>(row + c);
+#pragma unroll
+        for (int e = 0; e < SmallStep<T>::E; ++e) v[e] = (T)0.f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < SmallStep<T>::E; ++e) v[e] = c + e < dim ? row[c + e] : (T)0.f;
+    }
+    return v;
+}
+
+struct SmallStat {
+    const void *h, *w;
+    const float *bias;
+    const int64_t *target;
+    float2 *part, *zt;
+    float *z;  // [rows][vp], null: not kept
+    size_t ldh, ldw, vp;
+    int rows, table, dim;
+    float scale;
+};
+
+template <class T, int NB, bool VEC>
+__global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
+    typedef SmallStep<T> S;
+    __shared__ floatx4_t s_acc[2][4][NB][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+    const T *hr[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) hr[j] = (const T *)a.h + (size_t)min(16 * j + i, a.rows - 1) * a.ldh;
+    const int steps = (a.dim + S::K - 1) / S::K;
+    // wave w ends rows 16 w .. 16 w + 15
+    const int t = 16 * wave + i;
+    const bool mine = wave < NB && t < a.rows;
+    const int64_t y = mine ? a.target[t] : -1;
+    float top = -INFINITY, sum = 0.f;
+    int buf = 0;
+    const int groups = (a.table + 15) / 16;
+    for (int g = blockIdx.x; g < groups; g += gridDim.x, buf ^= 1) {
+        const T *wr = (const T *)a.w + (size_t)min(16 * g + i, a.table - 1) * a.ldw;
+        floatx4_t acc[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = wave; s < steps; s += 4) {
+            const int c = s * S::K + q * S::E;
+            const typename S::vec x = small_load<T, VEC>(wr, c, a.dim);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, VEC>(hr[j], c, a.dim), acc[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) s_acc[buf][wave][j][lane] = acc[j];
+        __syncthreads();  // the other buffer is written next: one barrier a group is enough
+        if (wave >= NB) continue;
+        const floatx4_t v = (s_acc[buf][0][wave][lane] + s_acc[buf][1][wave][lane]) +
+                            (s_acc[buf][2][wave][lane] + s_acc[buf][3][wave][lane]);
+        const int e0 = 16 * g + 4 * q;
+        floatx4_t z;
+        float m = top;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float b = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
+            z[e] = b == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b);
+            m = fmaxf(m, z[e]);
+        }
+        const float about = m == -INFINITY ? 0.f : m;
+        sum *= exp_neg(top - about);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += exp_neg(z[e] - about);
+        top = m;
+        if (mine) {
+            if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e0 + e == y && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
+        }
+    }
+    if (wave >= NB) return;
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(sum, o, 64), m = fmaxf(top, m2);
+        const float about = m == -INFINITY ? 0.f : m;
+        sum = sum * exp_neg(top - about) + s2 * exp_neg(m2 - about);
+        top = m;
+    }
+    if (mine && q == 0) a.part[(size_t)blockIdx.x * a.rows + t] = make_float2(top, sum);
+}
+
+struct SmallGrad {
+    const void *h, *w;
+    const float *bias, *z, *rowfac;
+    const float2 *stat;
+    const int64_t *target;
+    void *dtable;  // null: not wanted
+    float *part;   // [gridDim.x][rows][cols4], null: the rows' gradient is not wanted
+    size_t ldh, ldw, ldo, vp;
+    int rows, table, dim, cols4;
+    bool vec;  // of dtable
+};
+
+constexpr int kSmallCols = 128;  // columns of a workgroup
+
+template <class T, int TB, bool VEC>
+__global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
+    constexpr int R = 16 * TB, GP = 68, HP = kSmallCols + 4;
+    __shared__ __align__(16) float s_g[R * GP], s_h[R * HP];
+    __shared__ float s_cs[R], s_c[R], s_about[R];
+    __shared__ int s_y[R];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
+    const int d0 = blockIdx.y * kSmallCols;
+    for (int t = tid; t < R; t += 256) {
+        const float c = t < a.rows ? a.rowfac[t] : 0.f;
+        const float2 st = t < a.rows ? a.stat[t] : make_float2(0.f, 0.f);
+        const int64_t y = t < a.rows ? a.target[t] : -1;
+        s_c[t] = c;
+        s_cs[t] = c * st.y;
+        s_about[t] = st.x;
+        s_y[t] = y < a.table ? (int)y : -1;
+    }
+    for (int k = tid; k < R * kSmallCols; k += 256) {
+        const int t = k / kSmallCols, c = k % kSmallCols;
+        float v = 0.f;
+        if (t < a.rows && d0 + c < a.dim && a.target[t] >= 0) v = (float)((const T *)a.h)[(size_t)t * a.ldh + d0 + c];
+        s_h[t * HP + c] = v;
+    }
+    floatx4_t dh[2][TB][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < TB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dh[c][j][e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+
+    // 64 columns are four MFMA blocks: block e's row r is column 4 r + e, so that operands and results are
+    // four neighbouring columns a lane
+    for (int v0 = blockIdx.x * 64; v0 < a.table; v0 += gridDim.x * 64) {
+        __syncthreads();  // s_h (first turn), the last turn's s_g
+#pragma unroll 4
+        for (int k = tid; k < R * 64; k += 256) {
+            const int t = k >> 6, v = v0 + (k & 63);
+            const float c = s_c[t];
+            float g = 0.f;
+            if (c != 0.f && t < a.rows && v < a.table)
+                g = fmaf(s_cs[t], exp_fine(a.z[(size_t)t * a.vp + v] - s_about[t]), v == s_y[t] ? -c : 0.f);
+            s_g[t * GP + (k & 63)] = g;
+        }
+        __syncthreads();
+        const int vw = v0 + 16 * wave;
+        if (vw >= a.table) continue;  // a whole wave; the barriers are at the loop's head
+        if (a.part) {
+            floatx4_t g[TB];  // rows 16 j + i, entries vw + 4 q ..
+#pragma unroll
+            for (int j = 0; j < TB; ++j) g[j] = *reinterpret_cast<const floatx4_t *>(s_g + (16 * j + i) * GP + 16 * wave + 4 * q);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int v = vw + 4 * q + k;
+                const bool on = v < a.table && !(a.bias && a.bias[v] == -INFINITY);
+                const T *wr = (const T *)a.w + (size_t)(on ? v : 0) * a.ldw;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = d0 + 64 * c + 4 * i;
+                    float x[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (VEC) {
+                        if (on && col < a.dim) {
+                            const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4> *>(wr + col);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = (float)p.v[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (on && col + e < a.dim) x[e] = (float)wr[col + e];
+                    }
+#pragma unroll
+                    for (int j = 0; j < TB; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            dh[c][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], g[j][k], dh[c][j][e], 0, 0, 0);
+                }
+            }
+        }
+        if (!a.dtable) continue;
+        const int v = vw + i;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            if (d0 + 64 * c >= a.dim) break;
+            floatx4_t dw[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dw[e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4 * TB; ++k) {
+                const floatx4_t x = *reinterpret_cast<const floatx4_t *>(s_h + (4 * k + q) * HP + 64 * c + 4 * i);
+                const float g = s_g[(4 * k + q) * GP + 16 * wave + i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dw[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], g, dw[e], 0, 0, 0);
+            }
+            if (v >= a.table) continue;
+            T *o = (T *)a.dtable + (size_t)v * a.ldo;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int col = d0 + 64 * c + 16 * q + 4 * x;
+                if (a.vec && col + 4 <= a.dim) {
+                    Pack<T, 4> p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p.v[e] = (T)dw[e][x];
+                    *reinterpret_cast<Pack<T, 4> *>(o + col) = p;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (col + e < a.dim) o[col + e] = (T)dw[e][x];
+                }
+            }
+        }
+    }
+    if (!a.part) return;
+    // the four waves' sums, one wave after the other
+    for (int w = 0; w < 4; ++w) {
+        __syncthreads();
+        if (wave != w) continue;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < TB; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    floatx4_t *p = reinterpret_cast<floatx4_t *>(s_h + (16 * j + i) * HP + 64 * c + 16 * q + 4 * x);
+                    const floatx4_t v = {dh[c][j][0][x], dh[c][j][1][x], dh[c][j][2][x], dh[c][j][3][x]};
+                    *p = w == 0 ? v : *p + v;
+                }
+    }
+    __syncthreads();
+    for (int k = tid; k < a.rows * (kSmallCols / 4); k += 256) {
+        const int t = k / (kSmallCols / 4), c = k % (kSmallCols / 4) * 4;
+        if (d0 + c < a.cols4)
+            *reinterpret_cast<floatx4_t *>(a.part + ((size_t)blockIdx.x * a.rows + t) * a.cols4 + d0 + c) =
+                *reinterpret_cast<const floatx4_t *>(s_h + t * HP + c);
+    }
+}
+
+template <class T>
+void small_stat(const SmallStat &a, uint32_t grid, hipStream_t s) {
+    constexpr int E = SmallStep<T>::E;
+    const bool vec = a.dim % E == 0 && a.ldh % E == 0 && a.ldw % E == 0 && aligned16(a.h) && aligned16(a.w);
+#define SMALL_STAT(NB)                                             \
+    if (vec)                                                       \
+        k_small_stat<T, NB, true><<<grid, 256, 0, s>>>(a);         \
+    else                                                           \
+        k_small_stat<T, NB, false><<<grid, 256, 0, s>>>(a);
+    if (a.rows <= 16) {
+        SMALL_STAT(1)
+    } else if (a.rows <= 32) {
+        SMALL_STAT(2)
+    } else {
+        SMALL_STAT(4)
+    }
+#undef SMALL_STAT
+}
+
+template <class T>
+void small_grad(const SmallGrad &a, uint32_t gx, hipStream_t s) {
+    const dim3 grid(gx, (uint32_t)ceil_div(a.dim, kSmallCols));
+    const bool vec = a.dim % 4 == 0 && a.ldw % 4 == 0 && ((uintptr_t)a.w & (4 * sizeof(T) - 1)) == 0;
+#define SMALL_GRAD(TB)                                             \
+    if (vec)                                                       \
+        k_small_grad<T, TB, true><<<grid, 256, 0, s>>>(a);         \
+    else                                                           \
+        k_small_grad<T, TB, false><<<grid, 256, 0, s>>>(a);
+    if (a.rows <= 16) {
+        SMALL_GRAD(1)
+    } else if (a.rows <= 32) {
+        SMALL_GRAD(2)
+    } else {
+        SMALL_GRAD(4)
+    }
+#undef SMALL_GRAD
+}
+
+}  // namespace
+}  // namespace vh

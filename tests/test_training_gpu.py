@@ -398,6 +398,26 @@ def test_orthogonalize_a_stack(tr, dtype):
         assert torch.equal(got[i], tr.orthogonalize(stack[i].contiguous()))
 
 
+@pytest.mark.parametrize("count,rows,cols", [(60, 130, 300), (60, 300, 130), (12, 400, 390), (1, 1500, 1600), (1, 1700, 1410)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("steps", [1, 2, 5])
+def test_orthogonalize_many_tiles(tr, count, rows, cols, dtype, steps):
+    """Stacks and matrices that take the tiled products."""
+    m = (0.01 * normal(rows + cols, count, rows, cols)).to(TYPES[dtype])
+    got = tr.orthogonalize(m, steps=steps)
+    for i in (0, count - 1):
+        want = ns_reference(m[i], steps, 1e-7)
+        assert float((got[i].double() - want).norm()) <= ns_tolerance(want, steps, min(rows, cols), 2 * UNIT[m.dtype])
+
+
+def test_orthogonalize_against_a_large_eps(tr):
+    """eps takes part in the scale: a matrix of a thousandth of eps is hardly moved towards one."""
+    m = normal(8, 30, 50)
+    eps = 1000 * float(m.norm())
+    got, want = tr.orthogonalize(m, eps=eps), ns_reference(m, 5, eps)
+    assert float((got.double() - want).norm()) <= ns_tolerance(want, 5, 30, 2 * E)
+
+
 def test_orthogonalize_brings_singular_values_to_one(tr):
     s = torch.linalg.svdvals(tr.orthogonalize(normal(2, 96, 300)).double())
     assert 0.6 < float(s.min()) and float(s.max()) < 1.3

@@ -298,20 +298,24 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
         }
         lds_barrier();
         read(a0, b0, 0, 0);
-        for (int s = 0; s < n; ++s) {
+        // The last stage stands by itself: with a way round the barrier inside the loop the compiler would
+        // have the second half's products wait for fragments that are read for the next stage.
+        int s = 0;
+        for (; s + 1 < n; ++s) {
             const int buf = s & 1;
             read(a1, b1, buf, 1);
             multiply(a0, b0);
-            if (s + 1 < n) {
-                // this wave's reads of the buffer are done (lds_barrier waits for them) and the next
-                // tile has landed; after the barrier that holds for every wave
-                __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
-                lds_barrier();
-                if (s + 2 < n) issue(buf);
-                read(a0, b0, buf ^ 1, 0);
-            }
+            // this wave's reads of the buffer are done (lds_barrier waits for them) and the next tile has
+            // landed; after the barrier that holds for every wave
+            __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
+            lds_barrier();
+            if (s + 2 < n) issue(buf);
+            read(a0, b0, buf ^ 1, 0);
             multiply(a1, b1);
         }
+        read(a1, b1, s & 1, 1);
+        multiply(a0, b0);
+        multiply(a1, b1);
     }
     lds_barrier();  // every wave's fragments are read: the buffers are the epilogue's
     epi(acc, m0 + wm * MB * 16, n0 + wn * NB * 16, pl, lds + wave * kEpiBytes);

@@ -8,12 +8,18 @@
 // as two float16 planes each (22 bits, mm16.h) and multiplied as three products with 32-bit sums: as exact as
 // 32-bit products, at a third of the 16-bit matrix rate.  X is held times 2^10 and A and B times 2^8: the
 // singular values stay below 2 for any useful coefficients, so neither leaves float16's range.
+// The first X is the matrix times the power of two that brings |M|_F to [2^12, 2^13); what is left of the
+// norm goes into the first step's epilogues, so 16-bit matrices are exact in one plane and their first
+// products have no low plane to multiply.  Where the result is rounded to bfloat16 (2^-9), the last step
+// multiplies high planes alone: its rounding of 2^-12 is not amplified by any later step.
+// X's planes reach down to 2^-34: a matrix whose norm is below 2^-34 of eps comes out as zero.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.  a X is part
 // of B's diagonal.
 #include "mm16.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace vh {
 namespace {
@@ -51,17 +57,26 @@ struct Planes2 {
     size_t ld, stride;
 };
 
-// The scaled matrix x [m][np], zeros past n.
-template <class T>
+// The matrix times a power of two as x [m][np], zeros past n; BOTH: and its transpose xt [n][mp].
+// gain: what is left to multiply for M / (|M| + eps) times kXScale.
+template <class T, bool BOTH>
 __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int cols, size_t ld, size_t stride, bool tall,
-                                                  const double *part, float eps, Planes2 x) {
+                                                  const double *part, float eps, Planes2 x, Planes2 xt, float *gain) {
     __shared__ float tile[64][65];
     __shared__ float s_inv;
     if (threadIdx.x < 64) {
         double s = part[blockIdx.z * kNormParts + threadIdx.x];
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
-        if (threadIdx.x == 0) s_inv = (float)((double)kXScale / (sqrt(s) + (double)eps));
+        if (threadIdx.x == 0) {
+            const double norm = sqrt(s);
+            int e = 0;
+            (void)frexp(norm, &e);  // norm < 2^e
+            const double up = norm > 0.0 && norm <= 1e300 ? ldexp(1.0, 13 - e) : 1.0;
+            // a power of two that a float holds: what is past its range goes into the gain as well
+            s_inv = (float)fmin(fmax(up, 0x1p-126), 0x1p126);
+            if (blockIdx.x == 0 && blockIdx.y == 0) gain[blockIdx.z] = (float)((double)kXScale / ((norm + (double)eps) * (double)s_inv));
+        }
     }
     __syncthreads();
     const float inv = s_inv;
@@ -74,7 +89,7 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
         tile[tall ? tx : ty + 4 * i][tall ? ty + 4 * i : tx] = v;
     }
     __syncthreads();
-    const int m0 = tall ? c0 : r0, n0 = tall ? r0 : c0, m = tall ? cols : rows;
+    const int m0 = tall ? c0 : r0, n0 = tall ? r0 : c0, m = tall ? cols : rows, n = tall ? rows : cols;
     half_t *o = x.p + blockIdx.z * x.stride;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -84,6 +99,19 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
             split(tile[ty + 4 * i][tx], hi, lo);
             o[(size_t)r * x.ld + c] = hi;
             o[x.plane + (size_t)r * x.ld + c] = lo;
+        }
+    }
+    if constexpr (BOTH) {
+        o = xt.p + blockIdx.z * xt.stride;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = n0 + ty + 4 * i, c = m0 + tx;
+            if (r < n && (size_t)c < xt.ld) {
+                half_t hi, lo;
+                split(tile[tx][ty + 4 * i], hi, lo);
+                o[(size_t)r * xt.ld + c] = hi;
+                o[xt.plane + (size_t)r * xt.ld + c] = lo;
+            }
         }
     }
 }
@@ -104,7 +132,8 @@ __device__ __forceinline__ void store_planes(const floatx4_t (&acc)[MB][NB], cha
 
 // Epilogue of the symmetric products: out = alpha acc + beta add + diag I, stored at both places.
 struct SymEpi {
-    Planes2 out, add;  // add.p null: none
+    Planes2 out, add;   // add.p null: none
+    const float *gain;  // null: 1
     float alpha, beta, diag;
     int m;
     template <int MB, int NB>
@@ -113,13 +142,14 @@ struct SymEpi {
         half_t *o = out.p + pl.batch * out.stride;
         const half_t *ad = add.p ? add.p + pl.batch * add.stride : nullptr;
         const bool mirror = pl.tm != pl.tn;
+        const float al = gain ? gain[pl.batch] * gain[pl.batch] * alpha : alpha;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int c = nw + 16 * j + (l & 15);
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 const int r = mw + 16 * i + 4 * q;
-                floatx4_t v = acc[i][j] * alpha;
+                floatx4_t v = acc[i][j] * al;
                 if (ad && c < m && (size_t)r < add.ld) {
                     const Pack<half_t, 4> h = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + r);
                     const Pack<half_t, 4> w = *reinterpret_cast<const Pack<half_t, 4> *>(ad + add.plane + (size_t)c * add.ld + r);
@@ -149,6 +179,7 @@ struct SymEpi {
 template <class T>
 struct StepEpi {
     Planes2 x;
+    const float *gain;  // null: 1
     float alpha;
     int cols, rows;  // of what is stored
     T *out;          // null: not the last step
@@ -156,6 +187,7 @@ struct StepEpi {
     bool vec;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl, char *lds) const {
+        const float al = gain ? gain[pl.batch] * alpha : alpha;
         if (!out) {
             const int l = threadIdx.x & 63, q = l >> 4;
 #pragma unroll
@@ -163,14 +195,14 @@ struct StepEpi {
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = mw + 16 * i + 4 * q + e < cols ? acc[i][j][e] * alpha : 0.f;
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = mw + 16 * i + 4 * q + e < cols ? acc[i][j][e] * al : 0.f;
             store_planes(acc, lds, x.p + pl.batch * x.stride, x.plane, x.ld, nw, rows, mw);
             return;
         }
         constexpr int PER = 16 / (int)sizeof(T);
         T *o = out + pl.batch * so;
         rows_through_lds<T, MB, NB>(
-            lds, [&](int i, int j, int e) { return (T)(acc[i][j][e] * alpha); },
+            lds, [&](int i, int j, int e) { return (T)(acc[i][j][e] * al); },
             [&](int r, int c, const Pack<T, PER> &v) {
                 if (nw + r >= rows || mw + c >= cols) return;
                 T *p = o + (size_t)(nw + r) * ldo + mw + c;
@@ -185,9 +217,139 @@ struct StepEpi {
     }
 };
 
+// ---- small matrices ------------------------------------------------------------------------------
+// With few tiles a product is bound by how long one workgroup takes for its K loop.  Here a workgroup of
+// 8 waves computes a 64 x 64 tile, each wave all of it over every eighth 32 of K, from operands that it loads
+// straight into registers (K contiguous in both: X is kept in both orders); the waves' sums meet in LDS.
+struct SmallArgs {
+    Planes2 a, b;  // tile rows m of a, n of b
+    int M, N, K;
+    bool alo, blo;  // whether their low planes count
+    bool upper;
+    // out[n][m..] = alpha acc + beta add[n][m..] + diag I
+    Planes2 out, add, out_t;  // out_t: and the transpose; add.p, out_t.p null: none
+    const float *gain;
+    int gains;      // powers of the gain in alpha
+    float alpha, beta, diag;
+    void *result;   // in T instead of out
+    size_t ldr, sr;
+    bool result_t;  // result[m][n]
+};
+
+template <class T>
+__global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
+    typedef MmVec<half_t>::v8 v8;
+    constexpr int PITCH = 68;
+    __shared__ __align__(16) float s_part[8][64][PITCH];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
+    int tm = blockIdx.x, tn = blockIdx.y;
+    if (g.upper) {
+        tn = 0;
+        while ((tn + 1) * (tn + 2) / 2 <= (int)blockIdx.x) ++tn;
+        tm = blockIdx.x - tn * (tn + 1) / 2;
+    }
+    const int m0 = tm * 64, n0 = tn * 64;
+    const half_t *pa = g.a.p + blockIdx.z * g.a.stride + q * 8, *pb = g.b.p + blockIdx.z * g.b.stride + q * 8;
+    size_t ra[4], rb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ra[i] = (size_t)min(m0 + 16 * i + i16, g.M - 1) * g.a.ld;
+        rb[i] = (size_t)min(n0 + 16 * i + i16, g.N - 1) * g.b.ld;
+    }
+    floatx4_t acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    const int steps = (g.K + 31) / 32;  // planes are zero from K to the next multiple of 64
+#pragma unroll 2
+    for (int s = wave; s < steps; s += 8) {
+        v8 ah[4], al[4], bh[4], bl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ah[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 32);
+            bh[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 32);
+            if (g.alo) al[i] = *reinterpret_cast<const v8 *>(pa + g.a.plane + ra[i] + s * 32);
+            if (g.blo) bl[i] = *reinterpret_cast<const v8 *>(pb + g.b.plane + rb[i] + s * 32);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[i][j] = MmVec<half_t>::mfma(ah[i], bh[j], acc[i][j]);
+                if (g.blo) acc[i][j] = MmVec<half_t>::mfma(ah[i], bl[j], acc[i][j]);
+                if (g.alo) acc[i][j] = MmVec<half_t>::mfma(al[i], bh[j], acc[i][j]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<floatx4_t *>(&s_part[wave][16 * j + i16][16 * i + 4 * q]) = acc[i][j];
+    __syncthreads();
+    // 8 values of m of one n a lane
+    const int ln = wave * 8 + (lane >> 3), lm = (lane & 7) * 8, n = n0 + ln, m = m0 + lm;
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        floatx4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w) x += *reinterpret_cast<const floatx4_t *>(&s_part[w][ln][lm + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = x[e];
+    }
+    float alpha = g.alpha;
+    for (int k = 0; k < g.gains; ++k) alpha *= g.gain[blockIdx.z];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= alpha;
+    if (g.result) {
+        T *o = (T *)g.result + blockIdx.z * g.sr;
+        if (n < g.N)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (m + e < g.M) o[g.result_t ? (size_t)(m + e) * g.ldr + n : (size_t)n * g.ldr + m + e] = (T)v[e];
+        return;
+    }
+    if (g.add.p && n < g.N && m < g.M) {
+        const half_t *ad = g.add.p + blockIdx.z * g.add.stride + (size_t)n * g.add.ld + m;
+        const v8 h = *reinterpret_cast<const v8 *>(ad), l = *reinterpret_cast<const v8 *>(ad + g.add.plane);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(g.beta, (float)h[e] + (float)l[e], v[e]);
+    }
+    Pack<half_t, 8> hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (m + e == n) v[e] += g.diag;
+        split(n < g.N && m + e < g.M ? v[e] : 0.f, hi.v[e], lo.v[e]);
+    }
+    if (n < g.N && (size_t)m < g.out.ld) {
+        half_t *o = g.out.p + blockIdx.z * g.out.stride + (size_t)n * g.out.ld + m;
+        *reinterpret_cast<Pack<half_t, 8> *>(o) = hi;
+        *reinterpret_cast<Pack<half_t, 8> *>(o + g.out.plane) = lo;
+    }
+    // the other order: X^T, or the mirror image of a symmetric product's tile
+    const Planes2 &t = g.upper ? g.out : g.out_t;
+    if ((g.upper && tm != tn) || (!g.upper && t.p)) {
+        half_t *o = t.p + blockIdx.z * t.stride;
+        if ((size_t)n < t.ld)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (m + e < g.M) {
+                    o[(size_t)(m + e) * t.ld + n] = hi.v[e];
+                    o[t.plane + (size_t)(m + e) * t.ld + n] = lo.v[e];
+                }
+    }
+}
+
+// Where 64 x 64 tiles of the products between all matrices are at most two rounds of workgroups.
+inline bool ns_small(size_t count, size_t m, size_t n) {
+    const size_t tm = (m + 63) / 64, tn = (n + 63) / 64;
+    return count * tm * tn <= 512;
+}
+
 struct NsParts {
     double *norm;
-    Planes2 x[2], a, b;
+    float *gain;
+    Planes2 x[2], xt[2], a, b;  // xt for small matrices alone
 };
 
 inline Planes2 planes(Carver &c, size_t count, size_t rows, size_t ld) {
@@ -203,8 +365,10 @@ inline NsParts carve(Carver &c, size_t count, size_t m, size_t n) {
     NsParts p{};
     const size_t mp = round_up(m, kMmK), np = round_up(n, kMmK);
     p.norm = c.take<double>(count * kNormParts);
-    p.x[0] = planes(c, count, m, np);
-    p.x[1] = planes(c, count, m, np);
+    p.gain = c.take<float>(count);
+    for (Planes2 &x : p.x) x = planes(c, count, m, np);
+    if (ns_small(count, m, n))
+        for (Planes2 &x : p.xt) x = planes(c, count, n, mp);
     p.a = planes(c, count, m, mp);
     p.b = planes(c, count, m, mp);
     return p;
@@ -217,9 +381,10 @@ inline void operand(const Planes2 &p, const void *(&pl)[2], size_t &ld, size_t &
     stride = p.stride;
 }
 
-// K rows of an operand across, or 0 where K is contiguous.
+// nseg: 3 products of planes, 2 without A's low plane, 1 without either.
 template <bool TA, bool TB, class Epi>
-int multiply(const Planes2 &a, int M, const Planes2 &b, int N, int K, size_t count, bool upper, const Epi &epi, hipStream_t s) {
+int multiply(const Planes2 &a, int M, const Planes2 &b, int N, int K, int nseg, size_t count, bool upper, const Epi &epi,
+             hipStream_t s) {
     MmArgs g{};
     operand(a, g.a, g.lda, g.sa);
     operand(b, g.b, g.ldb, g.sb);
@@ -227,7 +392,7 @@ int multiply(const Planes2 &a, int M, const Planes2 &b, int N, int K, size_t cou
     g.N = N;
     g.ktiles = ceil_div(K, kMmK);
     g.ka = g.kb = K;
-    g.nseg = 3;
+    g.nseg = nseg;
     g.ksplit = 1;
     g.batch = (int)count;
     g.upper = upper;
@@ -245,35 +410,87 @@ struct NsCall {
 
 template <class T>
 int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
-    const bool tall = k.rows > k.cols;
+    const bool tall = k.rows > k.cols, small = p.xt[0].p != nullptr;
     const int m = (int)(tall ? k.cols : k.rows), n = (int)(tall ? k.rows : k.cols);
+    const uint32_t count = (uint32_t)k.count;
     const T *in = (const T *)k.in;
-    k_ns_norm<T><<<dim3(kNormParts, (uint32_t)k.count), 256, 0, s>>>(in, k.rows, k.cols, k.ldi, k.si, p.norm);
-    k_ns_start<T><<<dim3((uint32_t)ceil_div(k.rows, 64), (uint32_t)ceil_div(k.cols, 64), (uint32_t)k.count), 256, 0, s>>>(
-        in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0]);
+    k_ns_norm<T><<<dim3(kNormParts, count), 256, 0, s>>>(in, k.rows, k.cols, k.ldi, k.si, p.norm);
+    const dim3 tiles((uint32_t)ceil_div(k.rows, 64), (uint32_t)ceil_div(k.cols, 64), count);
+    if (small)
+        k_ns_start<T, true><<<tiles, 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0], p.xt[0], p.gain);
+    else
+        k_ns_start<T, false><<<tiles, 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0], p.x[0], p.gain);
     VH_CHECK(launch_status("orthogonalize launch"));
+    const int tm = ceil_div(m, 64), tn = ceil_div(n, 64);
     for (int i = 0; i < k.steps; ++i) {
-        const Planes2 &from = p.x[i & 1], &to = p.x[(i & 1) ^ 1];
-        SymEpi ea{p.a, Planes2{}, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
-        VH_CHECK((multiply<false, false>)(from, m, from, m, n, k.count, true, ea, s));
-        SymEpi eb{p.b, p.a, k.c / kAScale, k.b, k.a * kAScale, m};
-        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, k.count, true, eb, s));
-        StepEpi<T> es{to, 1.f / kAScale, n, m, nullptr, 0, 0, false};
-        if (i + 1 < k.steps) {
-            VH_CHECK((multiply<true, false>)(from, n, p.b, m, m, k.count, false, es, s));
+        const bool first = i == 0, last = i + 1 == k.steps;
+        const float *gain = first ? p.gain : nullptr;
+        // which low planes count: X's is empty at first where the matrix has 16 bits
+        const bool low = !(last && !first && std::is_same_v<T, bf16_t>);
+        const bool xlow = low && !(first && sizeof(T) == 2);
+        const Planes2 &x = p.x[i & 1], &xn = p.x[(i & 1) ^ 1], &xt = p.xt[i & 1], &xtn = p.xt[(i & 1) ^ 1];
+        if (small) {
+            SmallArgs g{};
+            g.gain = p.gain;
+            g.a = g.b = x;
+            g.M = g.N = m;
+            g.K = n;
+            g.alo = g.blo = xlow;
+            g.upper = true;
+            g.out = p.a;
+            g.alpha = kAScale / (kXScale * kXScale);
+            g.gains = first ? 2 : 0;
+            k_ns_small<T><<<dim3(tm * (tm + 1) / 2, 1, count), 512, 0, s>>>(g);
+            g.a = g.b = g.add = p.a;
+            g.K = m;
+            g.alo = g.blo = low;
+            g.out = p.b;
+            g.alpha = k.c / kAScale;
+            g.beta = k.b;
+            g.diag = k.a * kAScale;
+            g.gains = 0;
+            k_ns_small<T><<<dim3(tm * (tm + 1) / 2, 1, count), 512, 0, s>>>(g);
+            SmallArgs h{};
+            h.gain = p.gain;
+            h.a = xt;
+            h.b = p.b;
+            h.M = n;
+            h.N = h.K = m;
+            h.alo = xlow;
+            h.blo = low;
+            h.out = xn;
+            h.out_t = xtn;
+            h.alpha = 1.f / kAScale;
+            h.gains = first ? 1 : 0;
+            if (last) {
+                h.alpha /= kXScale;
+                h.result = k.out;
+                h.ldr = k.ldo;
+                h.sr = k.so;
+                h.result_t = tall;
+            }
+            k_ns_small<T><<<dim3(tn, tm, count), 512, 0, s>>>(h);
+            VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }
-        es.alpha /= kXScale;
-        es.out = (T *)k.out;
-        es.ldo = k.ldo;
-        es.so = k.so;
-        es.vec = k.ldo % (16 / sizeof(T)) == 0 && (k.count == 1 || k.so % (16 / sizeof(T)) == 0) && aligned16(k.out);
-        if (tall) {
+        SymEpi ea{p.a, Planes2{}, gain, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
+        VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow ? 3 : 1, k.count, true, ea, s));
+        SymEpi eb{p.b, p.a, nullptr, k.c / kAScale, k.b, k.a * kAScale, m};
+        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low ? 3 : 1, k.count, true, eb, s));
+        StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0, false};
+        if (last) {
+            es.alpha /= kXScale;
+            es.out = (T *)k.out;
+            es.ldo = k.ldo;
+            es.so = k.so;
+            es.vec = k.ldo % (16 / sizeof(T)) == 0 && (k.count == 1 || k.so % (16 / sizeof(T)) == 0) && aligned16(k.out);
+        }
+        if (last && tall) {
             es.cols = m;
             es.rows = n;
-            VH_CHECK((multiply<false, true>)(p.b, m, from, n, m, k.count, false, es, s));
+            VH_CHECK((multiply<false, true>)(p.b, m, x, n, m, low ? 3 : 1, k.count, false, es, s));
         } else {
-            VH_CHECK((multiply<true, false>)(from, n, p.b, m, m, k.count, false, es, s));
+            VH_CHECK((multiply<true, false>)(x, n, p.b, m, m, xlow ? 3 : (low ? 2 : 1), k.count, false, es, s));
         }
     }
     return VHIP_OK;

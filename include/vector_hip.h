@@ -426,7 +426,7 @@ int vhip_layer_norm_backward(int ordinal, int dtype, int param_dtype, const void
  * bias (table_rows floats, may be NULL) is a constant, such as the log of the rate at which an entry is drawn
  * taken off; -inf leaves an entry out, whatever its values.  A row with a negative target has loss 0; one
  * whose target is left out, or with every entry left out, +inf; one whose target is past the table NaN.
- * loss and lse may be NULL.  dim <= 65536, table_rows <= 2^23 - 64.  The logits are not kept. */
+ * loss and lse may be NULL.  dim <= 65536, table_rows <= 2^22 - 64.  The logits are not kept. */
 size_t vhip_softmax_xent_workspace(int dtype, size_t rows, size_t table_rows, size_t dim, int gradients);
 int vhip_softmax_xent(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table, size_t table_rows,
                       size_t ldt, size_t dim, const int64_t *target, const float *bias, float scale, float *loss,

@@ -57,7 +57,7 @@ def ortho(lib, **k):
     (ln_back, dict(mean=None)), (ln_back, dict(rstd=None)), (ln_back, dict(dy=None)), (ln_back, dict(lddx=7)),
     (ln_back, dict(ws=None)), (ln_back, dict(bytes=255)), (ln_back, dict(ws=P + 2)),
     (grad, dict(dtype=9)), (grad, dict(h=None)), (grad, dict(target=None)), (grad, dict(table=None)), (grad, dict(n=0)),
-    (grad, dict(n=1 << 23)), (grad, dict(dim=0)), (grad, dict(dim=65537, ldh=65537, ldt=65537, lddh=65537, lddt=65537)),
+    (grad, dict(n=1 << 22)), (grad, dict(dim=0)), (grad, dict(dim=65537, ldh=65537, ldt=65537, lddh=65537, lddt=65537)),
     (grad, dict(ldh=7)), (grad, dict(ldt=7)), (grad, dict(lddh=7)), (grad, dict(lddt=7)), (grad, dict(dh=None, dt=None)),
     (grad, dict(scale=float("inf"))), (grad, dict(scale=float("nan"))), (grad, dict(bytes=100)), (grad, dict(ws=None)),
     (grad, dict(ws=P + 8)), (xent, dict(bytes=100)), (xent, dict(ws=None)), (xent, dict(rows=1 << 30)),

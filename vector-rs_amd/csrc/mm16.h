@@ -3,9 +3,11 @@
 // A is M x K and B is N x K, each either with K contiguous, or ("across", a template flag) stored as K rows
 // of its M or N values.  Rows are 16-byte aligned; K is a multiple of 64 where it is contiguous, and an
 // operand across may have fewer rows: the missing ones are read as its last, for the other operand to
-// multiply with zeros.  Sums are held in 32 bits.  A 32-bit operand is carried as two float16 planes, x ~ hi + lo with
-// hi = f16(x) and lo = f16(x - hi) (22 bits), and the product as three segments of one long K loop,
-// hi hi + hi lo + lo hi; the dropped lo lo term is 2^-22 of the product.
+// multiply with zeros.  Sums are held in 32 bits.
+// A 32-bit operand is carried in pairs of float16, x ~ hi + lo with hi = f16(x) and lo = f16(x - hi) (22 bits),
+// and its product is hi hi + hi lo + lo hi; the dropped lo lo term is 2^-22 of the product.  A row of pairs
+// lies as blocks of 32 hi and 32 lo, so that a stage of 64 halves holds both of 32 k and its fragments serve
+// three products where a plain stage's serve two.
 //
 // A workgroup computes a BM x BN tile, its waves MB x NB blocks of 16 x 16.  Operand tiles of 64 k come in
 // by 16-byte global->LDS DMA into two buffers; the two halves of a tile's k are two sets of fragments: while
@@ -24,14 +26,21 @@
 
 namespace vh {
 
+// How the operands are stored, and what of them is multiplied.
+enum MmMode {
+    kPlain,  // 16-bit values
+    kPairs,  // pairs: all three products, or (MmArgs::alo, blo) those of the low halves that are not empty
+    kHigh,   // pairs: the high halves alone
+};
+// Where value c of a row of pairs has its high half, in halves; the low one is 32 further.
+__host__ __device__ inline size_t pair_at(size_t c) { return (c >> 5) * 64 + (c & 31); }
+
 struct MmArgs {
-    const void *a[2], *b[2];  // planes; [1] the low halves where nseg is 3
-    size_t lda, ldb;          // elements; 2^23 at most where K is contiguous
-    size_t sa, sb;            // from one product of a batch to the next, elements
-    int M, N;
-    int ktiles;               // K / 64, rounded up
-    int ka, kb;               // rows of an operand that is stored across
-    int nseg;                 // 1, or 3 for split operands
+    const void *a, *b;
+    size_t lda, ldb;          // 16-bit elements; 2^23 at most where K is contiguous
+    size_t sa, sb;            // from one product of a batch to the next, 16-bit elements
+    int M, N, K;              // K: rows where an operand is stored across
+    bool alo, blo;            // kPairs: whether the low halves count
     int mt, nt;               // tiles along M and N
     int ksplit;               // parts of the K loop, each a workgroup of its own
     int batch;
@@ -102,71 +111,77 @@ __device__ __forceinline__ MmPlace mm_place(const MmArgs &g, uint32_t id, uint32
     return p;
 }
 
-// One operand's tile of BR rows (of M or N) by 64 k in LDS: its DMAs and its fragments.
-template <class T, bool ACROSS, int BR, int NW>
+// One operand's tile of BR rows (of M or N) by 64 halves of k in LDS: its DMAs and its fragments.
+template <class T, MmMode MODE, bool ACROSS, int BR, int NW>
 struct MmTile {
     static constexpr int I = BR / 8 / NW;           // DMAs of a wave
     static constexpr int CH = BR / 8;               // chunks of a k row where stored across
     static constexpr int kBytes = BR * 128;
+    static constexpr int KS = MODE == kPairs ? 32 : 64;  // k of a stage
     static_assert(I * 8 * NW == BR, "whole DMAs");
     typedef typename MmVec<T>::v4 v4;
     typedef typename MmVec<T>::v8 v8;
     uint32_t off[I];
-    const char *base[2];
-    size_t step;    // bytes from one tile of k to the next
+    const char *base;
+    size_t step;    // bytes from one stage to the next
     size_t ld2;
     int c_last, wave, lane;
 
+    // byte of a row's chunk of 8 (high) values
+    static __device__ __forceinline__ int chunk(int c) { return MODE == kPlain ? c * 16 : (c >> 2) * 128 + (c & 3) * 16; }
     static __device__ __forceinline__ int swizzle(int k) {
         return 2 * ((k & 3) | (((k >> 3) & (CH >= 32 ? 3 : 1)) << 2));
     }
-    // the chunk and row of DMA i, across
-    __device__ __forceinline__ void spot(int i, int &k, int &c) const {
+    // DMA i, across: its row of k, and the byte in that row.  In pairs the tile's rows from 32 on are low halves.
+    __device__ __forceinline__ void spot(int i, int &k, int &at) const {
         const int n = (wave * I + i) * 64 + lane;
         k = n / CH;
-        c = min((n % CH) ^ swizzle(k), c_last);
+        at = chunk(min((n % CH) ^ swizzle(k), c_last));
+        if constexpr (MODE == kPairs) {
+            at += k >= 32 ? 64 : 0;
+            k &= 31;
+        }
     }
-    __device__ __forceinline__ void init(const void *const (&p)[2], size_t ld, int r0, int rows, size_t batch_off, int w, int l) {
+    __device__ __forceinline__ void init(const void *p, size_t ld, int r0, int rows, size_t batch_off, int w, int l) {
         wave = w;
         lane = l;
         ld2 = ld * 2;
         if constexpr (ACROSS) {
             c_last = (rows - 1 - r0) / 8;
-            step = ld2 * kMmK;
-            base[0] = (const char *)p[0] + (batch_off + r0) * 2;
-            base[1] = (const char *)p[1] + (batch_off + r0) * 2;
+            step = ld2 * KS;
+            base = (const char *)p + (batch_off + (size_t)r0 * (MODE == kPlain ? 1 : 2)) * 2;  // r0: a multiple of 32
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                int k, c;
-                spot(i, k, c);
-                off[i] = (uint32_t)(k * ld2 + c * 16);
+                int k, at;
+                spot(i, k, at);
+                off[i] = (uint32_t)(k * ld2 + at);
             }
         } else {
-            step = kMmK * 2;
-            base[0] = (const char *)p[0] + (batch_off + (size_t)r0 * ld) * 2;
-            base[1] = (const char *)p[1] + (batch_off + (size_t)r0 * ld) * 2;
+            step = MODE == kHigh ? 256 : 128;
+            base = (const char *)p + (batch_off + (size_t)r0 * ld) * 2;
             const int r = l >> 3, c = (l & 7) ^ r;
+            const int at = MODE == kHigh ? chunk(c) : c * 16;
 #pragma unroll
-            for (int i = 0; i < I; ++i) off[i] = (uint32_t)((size_t)(min(r0 + (w * I + i) * 8 + r, rows - 1) - r0) * ld2 + c * 16);
+            for (int i = 0; i < I; ++i) off[i] = (uint32_t)((size_t)(min(r0 + (w * I + i) * 8 + r, rows - 1) - r0) * ld2 + at);
         }
     }
-    // DMA of tile kt of a plane to LDS address `to`; krows: rows of k from this tile on
-    __device__ __forceinline__ void issue(int plane, int kt, int krows, uint32_t to) const {
-        const char *g = base[plane] + kt * step;
+    // DMA of stage kt to LDS address `to`; krows: rows of k from this stage on
+    __device__ __forceinline__ void issue(int kt, int krows, uint32_t to) const {
+        const char *g = base + kt * step;
         to += wave * I * 1024;
-        if (ACROSS && krows < kMmK) {
+        if (ACROSS && krows < KS) {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                int k, c;
-                spot(i, k, c);
-                dma_lds16_at(g, (uint32_t)(min(k, krows - 1) * ld2 + c * 16), to + i * 1024);
+                int k, at;
+                spot(i, k, at);
+                dma_lds16_at(g, (uint32_t)(min(k, krows - 1) * ld2 + at), to + i * 1024);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < I; ++i) dma_lds16_at(g, off[i], to + i * 1024);
         }
     }
-    // Fragments of N blocks from row r0 of the tile, half h of its k.
+    // Fragments of N blocks from row r0 of the tile, half h of its k (in pairs: the high or the low halves).
     template <int N>
     static __device__ __forceinline__ void read(v8 (&f)[N], const char *tile, int r0, int h, int l) {
         const int i = l & 15, q = l >> 4;
@@ -236,11 +251,11 @@ __device__ __forceinline__ void rows_through_lds(char *w, const Value &value, co
 
 // Epi: void operator()(acc, m, n, place, lds): the wave's MB x NB blocks, block (i, j) lane l element e being
 // C[m + 16 i + 4 (l >> 4) + e][n + 16 j + (l & 15)]; lds: kEpiBytes of the wave's own.
-template <class T, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
+template <class T, MmMode MODE, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
 __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
     constexpr int NW = WM * WN, BM = WM * MB * 16, BN = WN * NB * 16, BUF = (BM + BN) * 128;
-    typedef MmTile<T, TA, BM, NW> TileA;
-    typedef MmTile<T, TB, BN, NW> TileB;
+    typedef MmTile<T, MODE, TA, BM, NW> TileA;
+    typedef MmTile<T, MODE, TB, BN, NW> TileB;
     typedef typename MmVec<T>::v8 v8;
     static_assert(2 * BUF >= NW * kEpiBytes, "the epilogue's LDS");
     __shared__ __align__(1024) char lds[2 * BUF];
@@ -250,23 +265,19 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
     const MmPlace pl = mm_place(g, blockIdx.x, gridDim.x);
     const int m0 = pl.tm * BM, n0 = pl.tn * BN;
 
-    // this part's stages: [s0, s1) of nseg * ktiles
-    const int all = g.nseg * g.ktiles;
-    const int s0 = (int)((long)all * pl.part / g.ksplit), s1 = (int)((long)all * (pl.part + 1) / g.ksplit);
-    int seg = s0 / g.ktiles, kt = s0 % g.ktiles;
+    // this part's stages
+    const int all = (g.K + TileA::KS - 1) / TileA::KS;
+    const int s0 = (int)((long)all * pl.part / g.ksplit), n = (int)((long)all * (pl.part + 1) / g.ksplit) - s0;
 
     TileA ta;
     TileB tb;
     ta.init(g.a, g.lda, m0, g.M, pl.batch * g.sa, wave, lane);
     tb.init(g.b, g.ldb, n0, g.N, pl.batch * g.sb, wave, lane);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    auto issue = [&](int buf) {
-        ta.issue(seg == 2, kt, g.ka - kt * kMmK, lds0 + buf * BUF);
-        tb.issue(seg == 1, kt, g.kb - kt * kMmK, lds0 + buf * BUF + TileA::kBytes);
-        if (++kt == g.ktiles) {
-            kt = 0;
-            ++seg;
-        }
+    auto issue = [&](int s) {
+        const int kt = s0 + s, krows = g.K - kt * TileA::KS, buf = s & 1;
+        ta.issue(kt, krows, lds0 + buf * BUF);
+        tb.issue(kt, krows, lds0 + buf * BUF + TileA::kBytes);
     };
 
     floatx4_t acc[MB][NB];
@@ -276,9 +287,11 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
         for (int j = 0; j < NB; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
     v8 a0[MB], b0[NB], a1[MB], b1[NB];
-    auto read = [&](v8(&a)[MB], v8(&b)[NB], int buf, int h) {
-        TileB::template read<NB>(b, lds + buf * BUF + TileA::kBytes, wn * NB * 16, h, lane);
+    auto read_a = [&](v8(&a)[MB], int buf, int h) {
         TileA::template read<MB>(a, lds + buf * BUF, wm * MB * 16, h, lane);
+    };
+    auto read_b = [&](v8(&b)[NB], int buf, int h) {
+        TileB::template read<NB>(b, lds + buf * BUF + TileA::kBytes, wn * NB * 16, h, lane);
     };
     auto multiply = [&](const v8(&a)[MB], const v8(&b)[NB]) {
 #pragma unroll
@@ -287,8 +300,7 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
             for (int j = 0; j < NB; ++j) acc[i][j] = MmVec<T>::mfma(a[i], b[j], acc[i][j]);
     };
 
-    if (s0 < s1) {
-        const int n = s1 - s0;
+    if (n > 0) {
         issue(0);
         if (n > 1) {
             issue(1);
@@ -297,31 +309,47 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
             __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
         }
         lds_barrier();
-        read(a0, b0, 0, 0);
+        read_b(b0, 0, 0);
+        read_a(a0, 0, 0);
         // The last stage stands by itself: with a way round the barrier inside the loop the compiler would
         // have the second half's products wait for fragments that are read for the next stage.
         int s = 0;
         for (; s + 1 < n; ++s) {
             const int buf = s & 1;
-            read(a1, b1, buf, 1);
+            read_b(b1, buf, 1);
+            read_a(a1, buf, 1);
             multiply(a0, b0);
             // this wave's reads of the buffer are done (lds_barrier waits for them) and the next tile has
             // landed; after the barrier that holds for every wave
             __builtin_amdgcn_s_waitcnt(VH_VMCNT(0));
             lds_barrier();
-            if (s + 2 < n) issue(buf);
-            read(a0, b0, buf ^ 1, 0);
+            if (s + 2 < n) issue(s + 2);
+            if constexpr (MODE == kPairs) {
+                if (g.blo) multiply(a0, b1);
+                read_a(a0, buf ^ 1, 0);
+                if (g.alo) multiply(a1, b0);
+                read_b(b0, buf ^ 1, 0);
+            } else {
+                read_b(b0, buf ^ 1, 0);
+                read_a(a0, buf ^ 1, 0);
+                multiply(a1, b1);
+            }
+        }
+        read_b(b1, s & 1, 1);
+        read_a(a1, s & 1, 1);
+        multiply(a0, b0);
+        if constexpr (MODE == kPairs) {
+            if (g.blo) multiply(a0, b1);
+            if (g.alo) multiply(a1, b0);
+        } else {
             multiply(a1, b1);
         }
-        read(a1, b1, s & 1, 1);
-        multiply(a0, b0);
-        multiply(a1, b1);
     }
     lds_barrier();  // every wave's fragments are read: the buffers are the epilogue's
     epi(acc, m0 + wm * MB * 16, n0 + wn * NB * 16, pl, lds + wave * kEpiBytes);
 }
 
-template <class T, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
+template <class T, MmMode MODE, bool TA, bool TB, int WM, int WN, int MB, int NB, class Epi>
 int mm_launch_tile(MmArgs g, const Epi &epi, hipStream_t s) {
     g.mt = ceil_div(g.M, WM * MB * 16);
     g.nt = ceil_div(g.N, WN * NB * 16);
@@ -329,7 +357,7 @@ int mm_launch_tile(MmArgs g, const Epi &epi, hipStream_t s) {
     const size_t total = tiles * g.ksplit * g.batch;
     if (total > 0x7fffffff || (!TA && g.lda > kMmMaxLd) || (!TB && g.ldb > kMmMaxLd))
         return set_error(VHIP_ERR_INVALID_CONFIG, "a product of the call has too many tiles");
-    k_mm<T, TA, TB, WM, WN, MB, NB, Epi><<<dim3((uint32_t)total), dim3(WM * WN * 64), 0, s>>>(g, epi);
+    k_mm<T, MODE, TA, TB, WM, WN, MB, NB, Epi><<<dim3((uint32_t)total), dim3(WM * WN * 64), 0, s>>>(g, epi);
     return launch_status("product launch");
 }
 
@@ -343,9 +371,9 @@ inline bool mm_big_tiles(size_t M, size_t N, size_t batch, bool upper = false) {
     return ((tiles(256) + 255) / 256) * 4 * 10 <= ((tiles(128) + 511) / 512) * 2 * 14;
 }
 
-template <class T, bool TA, bool TB, class Epi>
+template <class T, MmMode MODE, bool TA, bool TB, class Epi>
 int mm_launch(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
-    return big ? mm_launch_tile<T, TA, TB, 2, 4, 8, 4>(g, epi, s) : mm_launch_tile<T, TA, TB, 2, 2, 4, 4>(g, epi, s);
+    return big ? mm_launch_tile<T, MODE, TA, TB, 2, 4, 8, 4>(g, epi, s) : mm_launch_tile<T, MODE, TA, TB, 2, 2, 4, 4>(g, epi, s);
 }
 
 }  // namespace vh

@@ -5,14 +5,14 @@
 //
 // which drives the singular values towards one while the singular vectors stay.  A direction whose singular
 // value is small grows by `a` a step, and what rounding puts into it grows as much, so X, A and B are held
-// as two float16 planes each (22 bits, mm16.h) and multiplied as three products with 32-bit sums: as exact as
+// in pairs of float16 (22 bits, mm16.h) and multiplied as three products with 32-bit sums: as exact as
 // 32-bit products, at a third of the 16-bit matrix rate.  X is held times 2^10 and A and B times 2^8: the
 // singular values stay below 2 for any useful coefficients, so neither leaves float16's range.
 // The first X is the matrix times the power of two that brings |M|_F to [2^12, 2^13); what is left of the
-// norm goes into the first step's epilogues, so 16-bit matrices are exact in one plane and their first
-// products have no low plane to multiply.  Where the result is rounded to bfloat16 (2^-9), the last step
-// multiplies high planes alone: its rounding of 2^-12 is not amplified by any later step.
-// X's planes reach down to 2^-34: a matrix whose norm is below 2^-34 of eps comes out as zero.
+// norm goes into the first step's epilogues, so 16-bit matrices are exact in the high halves and their
+// first products have no low ones to multiply.  Where the result is rounded to bfloat16 (2^-9), the last step
+// multiplies high halves alone: its rounding of 2^-12 is not amplified by any later step.
+// X's halves reach down to 2^-34: a matrix whose norm is below 2^-34 of eps comes out as zero.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.  a X is part
 // of B's diagonal.
@@ -51,17 +51,18 @@ __global__ __launch_bounds__(256) void k_ns_norm(const T *in, size_t rows, size_
     if (threadIdx.x == 0) part[blockIdx.y * kNormParts + blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-struct Planes2 {
+// A stack of matrices in pairs (mm16.h).
+struct Pairs {
     half_t *p;
-    size_t plane;  // from the high to the low plane
-    size_t ld, stride;
+    size_t cols;        // values of a row, a multiple of 64
+    size_t ld, stride;  // halves
 };
 
 // The matrix times a power of two as x [m][np], zeros past n; BOTH: and its transpose xt [n][mp].
 // gain: what is left to multiply for M / (|M| + eps) times kXScale.
 template <class T, bool BOTH>
 __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int cols, size_t ld, size_t stride, bool tall,
-                                                  const double *part, float eps, Planes2 x, Planes2 xt, float *gain) {
+                                                  const double *part, float eps, Pairs x, Pairs xt, float *gain) {
     __shared__ float tile[64][65];
     __shared__ float s_inv;
     if (threadIdx.x < 64) {
@@ -94,11 +95,11 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int r = m0 + ty + 4 * i, c = n0 + tx;
-        if (r < m && (size_t)c < x.ld) {
+        if (r < m && (size_t)c < x.cols) {
             half_t hi, lo;
             split(tile[ty + 4 * i][tx], hi, lo);
-            o[(size_t)r * x.ld + c] = hi;
-            o[x.plane + (size_t)r * x.ld + c] = lo;
+            o[(size_t)r * x.ld + pair_at(c)] = hi;
+            o[(size_t)r * x.ld + pair_at(c) + 32] = lo;
         }
     }
     if constexpr (BOTH) {
@@ -106,33 +107,33 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int r = n0 + ty + 4 * i, c = m0 + tx;
-            if (r < n && (size_t)c < xt.ld) {
+            if (r < n && (size_t)c < xt.cols) {
                 half_t hi, lo;
                 split(tile[tx][ty + 4 * i], hi, lo);
-                o[(size_t)r * xt.ld + c] = hi;
-                o[xt.plane + (size_t)r * xt.ld + c] = lo;
+                o[(size_t)r * xt.ld + pair_at(c)] = hi;
+                o[(size_t)r * xt.ld + pair_at(c) + 32] = lo;
             }
         }
     }
 }
 
-// A wave's blocks as both planes of rows [r0, rows) and columns [c0, ld).
+// A wave's blocks as pairs of rows [r0, rows) and columns from c0 on.
 template <int MB, int NB>
-__device__ __forceinline__ void store_planes(const floatx4_t (&acc)[MB][NB], char *lds, half_t *p, size_t plane, size_t ld,
-                                             int r0, int rows, int c0) {
-    auto store = [=](half_t *to) {
+__device__ __forceinline__ void store_pairs(const floatx4_t (&acc)[MB][NB], char *lds, half_t *p, const Pairs &to, int r0, int rows, int c0) {
+    auto store = [=](int low) {
         return [=](int r, int c, const Pack<half_t, 8> &v) {
-            if (r0 + r < rows && (size_t)(c0 + c) < ld) *reinterpret_cast<Pack<half_t, 8> *>(to + (size_t)(r0 + r) * ld + c0 + c) = v;
+            if (r0 + r < rows && (size_t)(c0 + c) < to.cols)
+                *reinterpret_cast<Pack<half_t, 8> *>(p + (size_t)(r0 + r) * to.ld + pair_at(c0 + c) + low) = v;
         };
     };
-    rows_through_lds<half_t, MB, NB>(lds, [&](int i, int j, int e) { return (half_t)acc[i][j][e]; }, store(p));
+    rows_through_lds<half_t, MB, NB>(lds, [&](int i, int j, int e) { return (half_t)acc[i][j][e]; }, store(0));
     rows_through_lds<half_t, MB, NB>(
-        lds, [&](int i, int j, int e) { return (half_t)(acc[i][j][e] - (float)(half_t)acc[i][j][e]); }, store(p + plane));
+        lds, [&](int i, int j, int e) { return (half_t)(acc[i][j][e] - (float)(half_t)acc[i][j][e]); }, store(32));
 }
 
 // Epilogue of the symmetric products: out = alpha acc + beta add + diag I, stored at both places.
 struct SymEpi {
-    Planes2 out, add;   // add.p null: none
+    Pairs out, add;   // add.p null: none
     const float *gain;  // null: 1
     float alpha, beta, diag;
     int m;
@@ -150,9 +151,9 @@ struct SymEpi {
             for (int i = 0; i < MB; ++i) {
                 const int r = mw + 16 * i + 4 * q;
                 floatx4_t v = acc[i][j] * al;
-                if (ad && c < m && (size_t)r < add.ld) {
-                    const Pack<half_t, 4> h = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + r);
-                    const Pack<half_t, 4> w = *reinterpret_cast<const Pack<half_t, 4> *>(ad + add.plane + (size_t)c * add.ld + r);
+                if (ad && c < m && (size_t)r < add.cols) {
+                    const Pack<half_t, 4> h = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + pair_at(r));
+                    const Pack<half_t, 4> w = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + pair_at(r) + 32);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = fmaf(beta, (float)h.v[e] + (float)w.v[e], v[e]);
                 }
@@ -161,16 +162,16 @@ struct SymEpi {
                     float x = v[e] + (r + e == c ? diag : 0.f);
                     if (r + e >= m || c >= m) x = 0.f;
                     acc[i][j][e] = x;
-                    if (mirror && r + e < m && (size_t)c < out.ld) {
+                    if (mirror && r + e < m && (size_t)c < out.cols) {
                         half_t hi, lo;
                         split(x, hi, lo);
-                        o[(size_t)(r + e) * out.ld + c] = hi;
-                        o[out.plane + (size_t)(r + e) * out.ld + c] = lo;
+                        o[(size_t)(r + e) * out.ld + pair_at(c)] = hi;
+                        o[(size_t)(r + e) * out.ld + pair_at(c) + 32] = lo;
                     }
                 }
             }
         }
-        store_planes(acc, lds, o, out.plane, out.ld, nw, m, mw);
+        store_pairs(acc, lds, o, out, nw, m, mw);
     }
 };
 
@@ -178,7 +179,7 @@ struct SymEpi {
 // operand's rows have (B where the matrix is tall).
 template <class T>
 struct StepEpi {
-    Planes2 x;
+    Pairs x;
     const float *gain;  // null: 1
     float alpha;
     int cols, rows;  // of what is stored
@@ -196,7 +197,7 @@ struct StepEpi {
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = mw + 16 * i + 4 * q + e < cols ? acc[i][j][e] * al : 0.f;
-            store_planes(acc, lds, x.p + pl.batch * x.stride, x.plane, x.ld, nw, rows, mw);
+            store_pairs(acc, lds, x.p + pl.batch * x.stride, x, nw, rows, mw);
             return;
         }
         constexpr int PER = 16 / (int)sizeof(T);
@@ -222,12 +223,12 @@ struct StepEpi {
 // 8 waves computes a 64 x 64 tile, each wave all of it over every eighth 32 of K, from operands that it loads
 // straight into registers (K contiguous in both: X is kept in both orders); the waves' sums meet in LDS.
 struct SmallArgs {
-    Planes2 a, b;  // tile rows m of a, n of b
+    Pairs a, b;  // tile rows m of a, n of b
     int M, N, K;
-    bool alo, blo;  // whether their low planes count
+    bool alo, blo;  // whether their low halves count
     bool upper;
     // out[n][m..] = alpha acc + beta add[n][m..] + diag I
-    Planes2 out, add, out_t;  // out_t: and the transpose; add.p, out_t.p null: none
+    Pairs out, add, out_t;  // out_t: and the transpose; add.p, out_t.p null: none
     const float *gain;
     int gains;      // powers of the gain in alpha
     float alpha, beta, diag;
@@ -261,16 +262,16 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-    const int steps = (g.K + 31) / 32;  // planes are zero from K to the next multiple of 64
+    const int steps = (g.K + 31) / 32;  // rows are zero from K to the next multiple of 64
 #pragma unroll 2
     for (int s = wave; s < steps; s += 8) {
         v8 ah[4], al[4], bh[4], bl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            ah[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 32);
-            bh[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 32);
-            if (g.alo) al[i] = *reinterpret_cast<const v8 *>(pa + g.a.plane + ra[i] + s * 32);
-            if (g.blo) bl[i] = *reinterpret_cast<const v8 *>(pb + g.b.plane + rb[i] + s * 32);
+            ah[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 64);
+            bh[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 64);
+            if (g.alo) al[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 64 + 32);
+            if (g.blo) bl[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 64 + 32);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -310,8 +311,8 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
         return;
     }
     if (g.add.p && n < g.N && m < g.M) {
-        const half_t *ad = g.add.p + blockIdx.z * g.add.stride + (size_t)n * g.add.ld + m;
-        const v8 h = *reinterpret_cast<const v8 *>(ad), l = *reinterpret_cast<const v8 *>(ad + g.add.plane);
+        const half_t *ad = g.add.p + blockIdx.z * g.add.stride + (size_t)n * g.add.ld + pair_at(m);
+        const v8 h = *reinterpret_cast<const v8 *>(ad), l = *reinterpret_cast<const v8 *>(ad + 32);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(g.beta, (float)h[e] + (float)l[e], v[e]);
     }
@@ -321,21 +322,21 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
         if (m + e == n) v[e] += g.diag;
         split(n < g.N && m + e < g.M ? v[e] : 0.f, hi.v[e], lo.v[e]);
     }
-    if (n < g.N && (size_t)m < g.out.ld) {
-        half_t *o = g.out.p + blockIdx.z * g.out.stride + (size_t)n * g.out.ld + m;
+    if (n < g.N && (size_t)m < g.out.cols) {
+        half_t *o = g.out.p + blockIdx.z * g.out.stride + (size_t)n * g.out.ld + pair_at(m);
         *reinterpret_cast<Pack<half_t, 8> *>(o) = hi;
-        *reinterpret_cast<Pack<half_t, 8> *>(o + g.out.plane) = lo;
+        *reinterpret_cast<Pack<half_t, 8> *>(o + 32) = lo;
     }
     // the other order: X^T, or the mirror image of a symmetric product's tile
-    const Planes2 &t = g.upper ? g.out : g.out_t;
+    const Pairs &t = g.upper ? g.out : g.out_t;
     if ((g.upper && tm != tn) || (!g.upper && t.p)) {
         half_t *o = t.p + blockIdx.z * t.stride;
-        if ((size_t)n < t.ld)
+        if ((size_t)n < t.cols)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (m + e < g.M) {
-                    o[(size_t)(m + e) * t.ld + n] = hi.v[e];
-                    o[t.plane + (size_t)(m + e) * t.ld + n] = lo.v[e];
+                    o[(size_t)(m + e) * t.ld + pair_at(n)] = hi.v[e];
+                    o[(size_t)(m + e) * t.ld + pair_at(n) + 32] = lo.v[e];
                 }
     }
 }
@@ -349,15 +350,15 @@ inline bool ns_small(size_t count, size_t m, size_t n) {
 struct NsParts {
     double *norm;
     float *gain;
-    Planes2 x[2], xt[2], a, b;  // xt for small matrices alone
+    Pairs x[2], xt[2], a, b;  // xt for small matrices alone
 };
 
-inline Planes2 planes(Carver &c, size_t count, size_t rows, size_t ld) {
-    Planes2 p{};
-    p.ld = ld;
-    p.stride = rows * ld;
-    p.plane = count * rows * ld;
-    p.p = c.take<half_t>(2 * p.plane);
+inline Pairs pairs(Carver &c, size_t count, size_t rows, size_t cols) {
+    Pairs p{};
+    p.cols = cols;
+    p.ld = 2 * cols;
+    p.stride = rows * p.ld;
+    p.p = c.take<half_t>(count * p.stride);
     return p;
 }
 
@@ -366,37 +367,35 @@ inline NsParts carve(Carver &c, size_t count, size_t m, size_t n) {
     const size_t mp = round_up(m, kMmK), np = round_up(n, kMmK);
     p.norm = c.take<double>(count * kNormParts);
     p.gain = c.take<float>(count);
-    for (Planes2 &x : p.x) x = planes(c, count, m, np);
+    for (Pairs &x : p.x) x = pairs(c, count, m, np);
     if (ns_small(count, m, n))
-        for (Planes2 &x : p.xt) x = planes(c, count, n, mp);
-    p.a = planes(c, count, m, mp);
-    p.b = planes(c, count, m, mp);
+        for (Pairs &x : p.xt) x = pairs(c, count, n, mp);
+    p.a = pairs(c, count, m, mp);
+    p.b = pairs(c, count, m, mp);
     return p;
 }
 
-inline void operand(const Planes2 &p, const void *(&pl)[2], size_t &ld, size_t &stride) {
-    pl[0] = p.p;
-    pl[1] = p.p + p.plane;
-    ld = p.ld;
-    stride = p.stride;
-}
-
-// nseg: 3 products of planes, 2 without A's low plane, 1 without either.
+// C of stacks a and b; alo, blo: whether their low halves count.
 template <bool TA, bool TB, class Epi>
-int multiply(const Planes2 &a, int M, const Planes2 &b, int N, int K, int nseg, size_t count, bool upper, const Epi &epi,
+int multiply(const Pairs &a, int M, const Pairs &b, int N, int K, bool alo, bool blo, size_t count, bool upper, const Epi &epi,
              hipStream_t s) {
     MmArgs g{};
-    operand(a, g.a, g.lda, g.sa);
-    operand(b, g.b, g.ldb, g.sb);
+    g.a = a.p;
+    g.b = b.p;
+    g.lda = a.ld;
+    g.ldb = b.ld;
+    g.sa = a.stride;
+    g.sb = b.stride;
     g.M = M;
     g.N = N;
-    g.ktiles = ceil_div(K, kMmK);
-    g.ka = g.kb = K;
-    g.nseg = nseg;
+    g.K = K;
+    g.alo = alo;
+    g.blo = blo;
     g.ksplit = 1;
     g.batch = (int)count;
     g.upper = upper;
-    return mm_launch<half_t, TA, TB>(g, mm_big_tiles(M, N, count, upper), epi, s);
+    const bool big = mm_big_tiles(M, N, count, upper);
+    return alo || blo ? mm_launch<half_t, kPairs, TA, TB>(g, big, epi, s) : mm_launch<half_t, kHigh, TA, TB>(g, big, epi, s);
 }
 
 struct NsCall {
@@ -425,10 +424,10 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
     for (int i = 0; i < k.steps; ++i) {
         const bool first = i == 0, last = i + 1 == k.steps;
         const float *gain = first ? p.gain : nullptr;
-        // which low planes count: X's is empty at first where the matrix has 16 bits
+        // which low halves count: X's are empty at first where the matrix has 16 bits
         const bool low = !(last && !first && std::is_same_v<T, bf16_t>);
         const bool xlow = low && !(first && sizeof(T) == 2);
-        const Planes2 &x = p.x[i & 1], &xn = p.x[(i & 1) ^ 1], &xt = p.xt[i & 1], &xtn = p.xt[(i & 1) ^ 1];
+        const Pairs &x = p.x[i & 1], &xn = p.x[(i & 1) ^ 1], &xt = p.xt[i & 1], &xtn = p.xt[(i & 1) ^ 1];
         if (small) {
             SmallArgs g{};
             g.gain = p.gain;
@@ -473,10 +472,10 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }
-        SymEpi ea{p.a, Planes2{}, gain, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
-        VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow ? 3 : 1, k.count, true, ea, s));
+        SymEpi ea{p.a, Pairs{}, gain, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
+        VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow, xlow, k.count, true, ea, s));
         SymEpi eb{p.b, p.a, nullptr, k.c / kAScale, k.b, k.a * kAScale, m};
-        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low ? 3 : 1, k.count, true, eb, s));
+        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low, low, k.count, true, eb, s));
         StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0, false};
         if (last) {
             es.alpha /= kXScale;
@@ -488,9 +487,9 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
         if (last && tall) {
             es.cols = m;
             es.rows = n;
-            VH_CHECK((multiply<false, true>)(p.b, m, x, n, m, low ? 3 : 1, k.count, false, es, s));
+            VH_CHECK((multiply<false, true>)(p.b, m, x, n, m, low, xlow, k.count, false, es, s));
         } else {
-            VH_CHECK((multiply<true, false>)(x, n, p.b, m, m, xlow ? 3 : (low ? 2 : 1), k.count, false, es, s));
+            VH_CHECK((multiply<true, false>)(x, n, p.b, m, m, xlow, low, k.count, false, es, s));
         }
     }
     return VHIP_OK;

@@ -9,7 +9,7 @@
 // with the rows.  Rows are taken in pieces so that G stays below kPieceBytes; from the second piece on the
 // table's gradient is added up in 32 bits.  Every sum has a fixed order: results do not depend on timing.
 //
-// Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as two float16 planes
+// Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
 // plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
 // operands), which is as far as the gradients that are returned are rounded too.  In float16 it is held
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void k_amax(const float *x, size_t rows, int d
     if ((threadIdx.x & 63) == 0) atomicMax(out, m);
 }
 
-// Planes of an operand: T itself, or hi and lo of a float times its scale.
+// An operand's 16-bit form: T itself, or pairs (mm16.h) of a float times its scale.
 template <class T>
 struct Planes {
     typedef T type;
@@ -78,22 +78,24 @@ struct Planes<float> {
     static constexpr int count = 2;
 };
 
-// rows x dim -> planes of rows x kp, zeros past dim and in rows whose bias is -inf.
+// rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              size_t plane, int kp, const uint32_t *amax, const float *bias) {
+                                              int kp, const uint32_t *amax, const float *bias) {
+    typedef typename Planes<T>::type P;
+    constexpr int N = Planes<T>::count;
     const size_t n = rows * (kp / 8);
     float sc = 1.f;
-    if constexpr (Planes<T>::count == 2) sc = unit_scale(*amax);
+    if constexpr (N == 2) sc = unit_scale(*amax);
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
         const size_t r = i / (kp / 8);
         const int c = (int)(i % (kp / 8)) * 8;
         const bool keep = !bias || bias[r] != -INFINITY;
-        Pack<typename Planes<T>::type, 8> hi, lo;
+        Pack<P, 8> hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const T v = keep && c + e < dim ? x[r * ld + c + e] : (T)0.f;
-            if constexpr (Planes<T>::count == 2) {
+            if constexpr (N == 2) {
                 const float f = v * sc;
                 hi.v[e] = (half_t)f;
                 lo.v[e] = (half_t)(f - (float)hi.v[e]);
@@ -101,17 +103,17 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
                 hi.v[e] = v;
             }
         }
-        *reinterpret_cast<Pack<typename Planes<T>::type, 8> *>(out + r * kp + c) = hi;
-        if constexpr (Planes<T>::count == 2)
-            *reinterpret_cast<Pack<typename Planes<T>::type, 8> *>(out + plane + r * kp + c) = lo;
+        P *o = out + r * kp * N + (N == 2 ? pair_at(c) : c);
+        *reinterpret_cast<Pack<P, 8> *>(o) = hi;
+        if constexpr (N == 2) *reinterpret_cast<Pack<P, 8> *>(o + 32) = lo;
     }
 }
 
-// rows x dim -> planes of dim x rp, zeros past rows and for rows with a negative target.
+// rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim, size_t ld,
-                                                typename Planes<T>::type *out, size_t plane, size_t rp,
-                                                const uint32_t *amax, const int64_t *target) {
+                                                typename Planes<T>::type *out, size_t rp, const uint32_t *amax,
+                                                const int64_t *target) {
     __shared__ T tile[64][65];
     const size_t r0 = (size_t)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -135,8 +137,8 @@ __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim
             if constexpr (Planes<T>::count == 2) {
                 const float f = v * sc;
                 const half_t h = (half_t)f;
-                out[c * rp + r] = h;
-                out[plane + c * rp + r] = (half_t)(f - (float)h);
+                out[c * rp * 2 + pair_at(r)] = h;
+                out[c * rp * 2 + pair_at(r) + 32] = (half_t)(f - (float)h);
             } else {
                 out[c * rp + r] = v;
             }
@@ -300,14 +302,14 @@ __global__ __launch_bounds__(256) void k_zero_rows(char *p, size_t rows, size_t 
 }
 
 // Epilogue of the second product: G.
-template <class G>  // element type of G's planes
+template <class G>
 struct GradEpi {
     Logits lg;
     const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
     const float *rowfac;
     const int64_t *target;
-    G *g;  // [tp][vp]
-    size_t plane, vp;
+    G *g;  // [tp][vp] values or pairs
+    size_t vp;
     int rows, tp, table;
     bool split;
     template <int MB, int NB>
@@ -349,15 +351,17 @@ struct GradEpi {
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = c == 0.f ? 0.f : acc[i][j][e];
             }
         }
-        auto store = [&](G *p) {
+        auto store = [&](int low) {
             return [=, *this](int r, int c, const Pack<G, 8> &v) {
-                if (n + r < tp && (size_t)(m + c) < vp) *reinterpret_cast<Pack<G, 8> *>(p + (size_t)(n + r) * vp + m + c) = v;
+                if (n + r >= tp || (size_t)(m + c) >= vp) return;
+                G *o = split ? g + (size_t)(n + r) * vp * 2 + pair_at(m + c) + low : g + (size_t)(n + r) * vp + m + c;
+                *reinterpret_cast<Pack<G, 8> *>(o) = v;
             };
         };
-        rows_through_lds<G, MB, NB>(lds, [&](int i, int j, int e) { return (G)acc[i][j][e]; }, store(g));
+        rows_through_lds<G, MB, NB>(lds, [&](int i, int j, int e) { return (G)acc[i][j][e]; }, store(0));
         if (split)
             rows_through_lds<G, MB, NB>(
-                lds, [&](int i, int j, int e) { return (G)(acc[i][j][e] - (float)(G)acc[i][j][e]); }, store(g + plane));
+                lds, [&](int i, int j, int e) { return (G)(acc[i][j][e] - (float)(G)acc[i][j][e]); }, store(32));
     }
 };
 
@@ -509,7 +513,7 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.pieces = ceil_div(table, z.stat_big ? 128 : 64);
     z.dh_big = dim > 128 && z.piece_rows > 128;
     const size_t bs = z.dh_big ? 256 : 128, tiles = (size_t)ceil_div(dim, bs) * ceil_div(z.piece_rows, bs);
-    const size_t want = z.dh_big ? 256 : 512, ks = z.vp / kMmK;
+    const size_t want = z.dh_big ? 256 : 512, ks = z.vp / kMmK;  // at least 8 stages a part
     size_t k = want / tiles;
     if (k > ks / 8) k = ks / 8;
     z.ksplit = (int)(k < 1 ? 1 : k);
@@ -612,6 +616,7 @@ template <class T>
 int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     typedef typename Planes<T>::type P;
     constexpr bool kSplit = Planes<T>::count == 2;
+    constexpr MmMode kMode = kSplit ? kPairs : kPlain;
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
@@ -623,12 +628,11 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
     if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
-        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, z.table * z.kp, (int)z.kp,
+        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp,
                                                                   &p.sc->amax_w, (const float *)c.bias);
         wp = (const P *)p.wp;
-        ldw = z.kp;
+        ldw = z.kp * Planes<T>::count;
     }
-    const size_t w_plane = kSplit ? z.table * z.kp : 0;
 
     for (size_t r0 = 0; r0 < z.rows; r0 += z.piece_rows) {
         const size_t rows = z.rows - r0 < z.piece_rows ? z.rows - r0 : z.piece_rows;
@@ -637,25 +641,23 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, z.piece_rows * z.kp, (int)z.kp,
+            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp,
                                                                 &p.sc->amax_h, nullptr);
             hp = (const P *)p.hp;
-            ldh = z.kp;
+            ldh = z.kp * Planes<T>::count;
         }
         MmArgs g{};
-        g.a[0] = wp;
-        g.a[1] = wp + w_plane;
-        g.b[0] = hp;
-        g.b[1] = kSplit ? hp + z.piece_rows * z.kp : hp;
+        g.a = wp;
+        g.b = hp;
         g.lda = ldw;
         g.ldb = ldh;
         g.M = table;
         g.N = (int)rows;
-        g.ktiles = (int)(z.kp / kMmK);
-        g.nseg = kSplit ? 3 : 1;
+        g.K = (int)z.kp;
+        g.alo = g.blo = true;
         g.ksplit = g.batch = 1;
         const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
-        VH_CHECK((mm_launch<P, false, false>)(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
+        VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
         join_pieces(p, z, rows, target, c.row_weight ? c.row_weight + r0 : nullptr, c.scale, c.loss ? c.loss + r0 : nullptr,
                     c.lse ? c.lse + r0 : nullptr, s);
         VH_CHECK(launch_status("softmax launch"));
@@ -667,55 +669,48 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         ge.rowfac = p.rowfac;
         ge.target = target;
         ge.g = (P *)p.g;
-        ge.plane = kSplit ? z.tp * z.vp : 0;
         ge.vp = z.vp;
         ge.rows = (int)rows;
         ge.tp = (int)tp;
         ge.table = table;
         ge.split = kSplit;
-        VH_CHECK((mm_launch<P, false, false>)(g, z.stat_big, ge, s));
+        VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, ge, s));
         const P *gg = (const P *)p.g;
         if (c.dh) {
             // columns of the table, K its rows: G's columns past the table are zeros
             MmArgs d = g;
-            d.b[0] = gg;
-            d.b[1] = gg + ge.plane;
-            d.ldb = z.vp;
+            d.b = gg;
+            d.ldb = z.vp * Planes<T>::count;
             d.M = dim;
             d.N = (int)rows;
-            d.ktiles = (int)(z.vp / kMmK);
-            d.ka = table;
+            d.K = table;
             d.ksplit = z.ksplit;
             const OutScale os{p.sc, kSplit, false};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
                          true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
-            VH_CHECK((mm_launch<P, true, false>)(d, z.dh_big, oe, s));
+            VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_big, oe, s));
             if (z.ksplit > 1)
                 join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
         }
         if (c.dtable) {
             // K the rows: those past the last are zeros in both operands, those that do not count in the first
             k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
-                hr, rows, dim, c.ldh, (P *)p.ht, z.dim * z.tp, tp, &p.sc->amax_h, target);
+                hr, rows, dim, c.ldh, (P *)p.ht, tp, &p.sc->amax_h, target);
             MmArgs d{};
-            const P *ht = (const P *)p.ht;
-            d.a[0] = ht;
-            d.a[1] = ht + (kSplit ? z.dim * z.tp : 0);
-            d.b[0] = gg;
-            d.b[1] = gg + ge.plane;
-            d.lda = tp;
-            d.ldb = z.vp;
+            d.a = p.ht;
+            d.b = gg;
+            d.lda = tp * Planes<T>::count;
+            d.ldb = z.vp * Planes<T>::count;
             d.M = dim;
             d.N = table;
-            d.ktiles = (int)(tp / kMmK);
-            d.kb = (int)tp;
-            d.nseg = g.nseg;
+            d.K = (int)tp;
+            d.alo = d.blo = true;
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
             OutEpi<T> oe{OutScale{p.sc, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % (16 / sizeof(T)) == 0 && aligned16(c.dtable)};
-            VH_CHECK((mm_launch<P, false, true>)(d, z.dw_big, oe, s));
+            VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_big, oe, s));
         }
         VH_CHECK(launch_status("gradient launch"));
     }
@@ -725,7 +720,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
 int check_call(int dtype, const Call &c, size_t rows, size_t table, size_t dim, bool grad) {
     if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
     if (dim == 0 || dim > 65536) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 65536]");
-    if (table == 0 || table > kMmMaxLd - kMmK) return set_error(VHIP_ERR_INVALID_CONFIG, "the table must have 1 to 2^23 - 64 rows");
+    if (table == 0 || table > kMmMaxLd / 2 - kMmK) return set_error(VHIP_ERR_INVALID_CONFIG, "the table must have 1 to 2^22 - 64 rows");
     if (rows > 0x3fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows");
     if ((rows && (!c.h || !c.target)) || !c.table) return set_error(VHIP_ERR_INVALID_CONFIG, "an input is null");
     if (c.ldh < dim || c.ldt < dim || (c.dh && c.lddh < dim) || (c.dtable && c.lddt < dim))

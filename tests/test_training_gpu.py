@@ -377,7 +377,7 @@ def ns_tolerance(want, steps, small, unit):
     return 8 * 2.0 ** -22 * (grown + 3.9 ** steps) + unit * float(want.norm())
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 9), (5, 3), (3, 5), (64, 64), (100, 300), (300, 100), (129, 257), (400, 390)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 9), (5, 3), (3, 5), (64, 64), (100, 300), (300, 100), (129, 257), (400, 390), (800, 820), (900, 700)])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("steps", [1, 5])
 def test_orthogonalize(tr, rows, cols, dtype, steps):

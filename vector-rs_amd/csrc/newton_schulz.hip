@@ -32,17 +32,23 @@ __device__ __forceinline__ void split(float x, half_t &hi, half_t &lo) {
     lo = (half_t)(x - (float)hi);
 }
 
-// Partial sums of squares, in 64 bits: values of any magnitude neither overflow nor vanish.
-template <class T>
-__global__ __launch_bounds__(256) void k_ns_norm(const T *in, size_t rows, size_t cols, size_t ld, size_t stride,
-                                                 double *part) {
+// Partial sums of squares, in 64 bits: values of any magnitude neither overflow nor vanish.  2^lanes lanes a
+// row, V values each at a time.
+template <class T, int V>
+__global__ __launch_bounds__(256) void k_ns_norm(const T *in, int rows, int cols, size_t ld, size_t stride, int lanes, double *part) {
     __shared__ double lds[4];
     const T *p = in + blockIdx.y * stride;
+    const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
     double s = 0.0;
-    const size_t n = rows * cols;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)kNormParts * 256) {
-        const double v = (double)(float)p[i / cols * ld + i % cols];
-        s += v * v;
+    for (int r = blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += kNormParts * per) {
+        for (int c = l * V; c < cols; c += V << lanes) {
+            const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(p + (size_t)r * ld + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const double x = (double)(float)v.v[e];
+                s += x * x;
+            }
+        }
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
@@ -220,8 +226,9 @@ struct StepEpi {
 
 // ---- small matrices ------------------------------------------------------------------------------
 // With few tiles a product is bound by how long one workgroup takes for its K loop.  Here a workgroup of
-// 8 waves computes a 64 x 64 tile, each wave all of it over every eighth 32 of K, from operands that it loads
-// straight into registers (K contiguous in both: X is kept in both orders); the waves' sums meet in LDS.
+// 8 waves computes a tile of 64 x 64, or of 32 x 32 where there are few, each wave all of it over every eighth
+// 32 of K, from operands that it loads straight into registers (K contiguous in both: X is kept in both
+// orders); the waves' sums meet in LDS.
 struct SmallArgs {
     Pairs a, b;  // tile rows m of a, n of b
     int M, N, K;
@@ -237,11 +244,11 @@ struct SmallArgs {
     bool result_t;  // result[m][n]
 };
 
-template <class T>
+template <class T, int TB>  // blocks of 16 along a tile's side
 __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
     typedef MmVec<half_t>::v8 v8;
-    constexpr int PITCH = 68;
-    __shared__ __align__(16) float s_part[8][64][PITCH];
+    constexpr int SIDE = 16 * TB, V = SIDE * SIDE / 512;  // values of a lane in the end
+    __shared__ __align__(16) float s_part[8][SIDE][SIDE + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
     int tm = blockIdx.x, tn = blockIdx.y;
     if (g.upper) {
@@ -249,83 +256,82 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
         while ((tn + 1) * (tn + 2) / 2 <= (int)blockIdx.x) ++tn;
         tm = blockIdx.x - tn * (tn + 1) / 2;
     }
-    const int m0 = tm * 64, n0 = tn * 64;
+    const int m0 = tm * SIDE, n0 = tn * SIDE;
     const half_t *pa = g.a.p + blockIdx.z * g.a.stride + q * 8, *pb = g.b.p + blockIdx.z * g.b.stride + q * 8;
-    size_t ra[4], rb[4];
+    size_t ra[TB], rb[TB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < TB; ++i) {
         ra[i] = (size_t)min(m0 + 16 * i + i16, g.M - 1) * g.a.ld;
         rb[i] = (size_t)min(n0 + 16 * i + i16, g.N - 1) * g.b.ld;
     }
-    floatx4_t acc[4][4];
+    floatx4_t acc[TB][TB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < TB; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TB; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
     const int steps = (g.K + 31) / 32;  // rows are zero from K to the next multiple of 64
-#pragma unroll 2
+#pragma unroll (TB == 4 ? 2 : 4)
     for (int s = wave; s < steps; s += 8) {
-        v8 ah[4], al[4], bh[4], bl[4];
+        v8 ah[TB], al[TB], bh[TB], bl[TB];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < TB; ++i) {
             ah[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 64);
             bh[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 64);
             if (g.alo) al[i] = *reinterpret_cast<const v8 *>(pa + ra[i] + s * 64 + 32);
             if (g.blo) bl[i] = *reinterpret_cast<const v8 *>(pb + rb[i] + s * 64 + 32);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < TB; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < TB; ++j) {
                 acc[i][j] = MmVec<half_t>::mfma(ah[i], bh[j], acc[i][j]);
                 if (g.blo) acc[i][j] = MmVec<half_t>::mfma(ah[i], bl[j], acc[i][j]);
                 if (g.alo) acc[i][j] = MmVec<half_t>::mfma(al[i], bh[j], acc[i][j]);
             }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < TB; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<floatx4_t *>(&s_part[wave][16 * j + i16][16 * i + 4 * q]) = acc[i][j];
+        for (int j = 0; j < TB; ++j) *reinterpret_cast<floatx4_t *>(&s_part[wave][16 * j + i16][16 * i + 4 * q]) = acc[i][j];
     __syncthreads();
-    // 8 values of m of one n a lane
-    const int ln = wave * 8 + (lane >> 3), lm = (lane & 7) * 8, n = n0 + ln, m = m0 + lm;
-    float v[8];
+    // V values of m of one n a lane
+    const int ln = threadIdx.x / (SIDE / V), lm = threadIdx.x % (SIDE / V) * V, n = n0 + ln, m = m0 + lm;
+    float v[V];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        floatx4_t x = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < V; ++e) {
+        float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) x += *reinterpret_cast<const floatx4_t *>(&s_part[w][ln][lm + 4 * h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * h + e] = x[e];
+        for (int w = 0; w < 8; ++w) x += s_part[w][ln][lm + e];
+        v[e] = x;
     }
     float alpha = g.alpha;
     for (int k = 0; k < g.gains; ++k) alpha *= g.gain[blockIdx.z];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= alpha;
+    for (int e = 0; e < V; ++e) v[e] *= alpha;
     if (g.result) {
         T *o = (T *)g.result + blockIdx.z * g.sr;
         if (n < g.N)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < V; ++e)
                 if (m + e < g.M) o[g.result_t ? (size_t)(m + e) * g.ldr + n : (size_t)n * g.ldr + m + e] = (T)v[e];
         return;
     }
     if (g.add.p && n < g.N && m < g.M) {
         const half_t *ad = g.add.p + blockIdx.z * g.add.stride + (size_t)n * g.add.ld + pair_at(m);
-        const v8 h = *reinterpret_cast<const v8 *>(ad), l = *reinterpret_cast<const v8 *>(ad + 32);
+        const Pack<half_t, V> h = *reinterpret_cast<const Pack<half_t, V> *>(ad), l = *reinterpret_cast<const Pack<half_t, V> *>(ad + 32);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(g.beta, (float)h[e] + (float)l[e], v[e]);
+        for (int e = 0; e < V; ++e) v[e] = fmaf(g.beta, (float)h.v[e] + (float)l.v[e], v[e]);
     }
-    Pack<half_t, 8> hi, lo;
+    Pack<half_t, V> hi, lo;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < V; ++e) {
         if (m + e == n) v[e] += g.diag;
         split(n < g.N && m + e < g.M ? v[e] : 0.f, hi.v[e], lo.v[e]);
     }
     if (n < g.N && (size_t)m < g.out.cols) {
         half_t *o = g.out.p + blockIdx.z * g.out.stride + (size_t)n * g.out.ld + pair_at(m);
-        *reinterpret_cast<Pack<half_t, 8> *>(o) = hi;
-        *reinterpret_cast<Pack<half_t, 8> *>(o + 32) = lo;
+        *reinterpret_cast<Pack<half_t, V> *>(o) = hi;
+        *reinterpret_cast<Pack<half_t, V> *>(o + 32) = lo;
     }
     // the other order: X^T, or the mirror image of a symmetric product's tile
     const Pairs &t = g.upper ? g.out : g.out_t;
@@ -333,12 +339,25 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
         half_t *o = t.p + blockIdx.z * t.stride;
         if ((size_t)n < t.cols)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < V; ++e)
                 if (m + e < g.M) {
                     o[(size_t)(m + e) * t.ld + pair_at(n)] = hi.v[e];
                     o[(size_t)(m + e) * t.ld + pair_at(n) + 32] = lo.v[e];
                 }
     }
+}
+
+template <class T>
+void ns_small_product(const SmallArgs &g, size_t count, hipStream_t s) {
+    auto grid = [&](int side) {
+        const uint32_t tm = ceil_div(g.M, side), tn = ceil_div(g.N, side);
+        return g.upper ? dim3(tm * (tm + 1) / 2, 1, (uint32_t)count) : dim3(tm, tn, (uint32_t)count);
+    };
+    const dim3 few = grid(32);
+    if ((size_t)few.x * few.y * few.z <= 512)
+        k_ns_small<T, 2><<<few, 512, 0, s>>>(g);
+    else
+        k_ns_small<T, 4><<<grid(64), 512, 0, s>>>(g);
 }
 
 // Where 64 x 64 tiles of the products between all matrices are at most two rounds of workgroups.
@@ -413,14 +432,17 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
     const int m = (int)(tall ? k.cols : k.rows), n = (int)(tall ? k.rows : k.cols);
     const uint32_t count = (uint32_t)k.count;
     const T *in = (const T *)k.in;
-    k_ns_norm<T><<<dim3(kNormParts, count), 256, 0, s>>>(in, k.rows, k.cols, k.ldi, k.si, p.norm);
+    constexpr int V = 16 / (int)sizeof(T);
+    if (k.cols % V == 0 && k.ldi % V == 0 && (k.count == 1 || k.si % V == 0) && aligned16(in))
+        k_ns_norm<T, V><<<dim3(kNormParts, count), 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, lanes_log2(k.cols / V), p.norm);
+    else
+        k_ns_norm<T, 1><<<dim3(kNormParts, count), 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, lanes_log2(k.cols), p.norm);
     const dim3 tiles((uint32_t)ceil_div(k.rows, 64), (uint32_t)ceil_div(k.cols, 64), count);
     if (small)
         k_ns_start<T, true><<<tiles, 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0], p.xt[0], p.gain);
     else
         k_ns_start<T, false><<<tiles, 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0], p.x[0], p.gain);
     VH_CHECK(launch_status("orthogonalize launch"));
-    const int tm = ceil_div(m, 64), tn = ceil_div(n, 64);
     for (int i = 0; i < k.steps; ++i) {
         const bool first = i == 0, last = i + 1 == k.steps;
         const float *gain = first ? p.gain : nullptr;
@@ -439,7 +461,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             g.out = p.a;
             g.alpha = kAScale / (kXScale * kXScale);
             g.gains = first ? 2 : 0;
-            k_ns_small<T><<<dim3(tm * (tm + 1) / 2, 1, count), 512, 0, s>>>(g);
+            ns_small_product<T>(g, count, s);
             g.a = g.b = g.add = p.a;
             g.K = m;
             g.alo = g.blo = low;
@@ -448,7 +470,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             g.beta = k.b;
             g.diag = k.a * kAScale;
             g.gains = 0;
-            k_ns_small<T><<<dim3(tm * (tm + 1) / 2, 1, count), 512, 0, s>>>(g);
+            ns_small_product<T>(g, count, s);
             SmallArgs h{};
             h.gain = p.gain;
             h.a = xt;
@@ -468,7 +490,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
                 h.sr = k.so;
                 h.result_t = tall;
             }
-            k_ns_small<T><<<dim3(tn, tm, count), 512, 0, s>>>(h);
+            ns_small_product<T>(h, count, s);
             VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }

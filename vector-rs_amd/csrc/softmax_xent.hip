@@ -50,12 +50,31 @@ __global__ void k_xent_init(Scalars *s) {
     if (threadIdx.x == 0) *s = Scalars{0, 0, 0};
 }
 
-__global__ __launch_bounds__(256) void k_amax(const float *x, size_t rows, int dim, size_t ld, uint32_t *out) {
+// Largest finite |value| of h (blockIdx.y 0) and of the table (1).
+struct AmaxArgs {
+    const float *x[2];
+    size_t rows[2], ld[2];
+    uint32_t *out[2];
+    int dim, lanes;  // lanes of a row, log2
+    bool vec;
+};
+__global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
+    const int y = blockIdx.y, per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
     uint32_t m = 0;
-    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        for (int c = threadIdx.x; c < dim; c += 256) {
-            const uint32_t u = __builtin_bit_cast(uint32_t, x[r * ld + c]) & 0x7fffffffu;
-            if (u < 0x7f800000u && u > m) m = u;
+    auto see = [&](float v) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+        if (u < 0x7f800000u && u > m) m = u;
+    };
+    for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes); r < a.rows[y]; r += (size_t)gridDim.x * per) {
+        const float *x = a.x[y] + r * a.ld[y];
+        if (a.vec) {
+            for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
+                const floatx4_t v = *reinterpret_cast<const floatx4_t *>(x + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) see(v[e]);
+            }
+        } else {
+            for (int c = l; c < a.dim; c += 1 << a.lanes) see(x[c]);
         }
     }
 #pragma unroll
@@ -63,7 +82,7 @@ __global__ __launch_bounds__(256) void k_amax(const float *x, size_t rows, int d
         const uint32_t v = __shfl_xor(m, o, 64);
         m = v > m ? v : m;
     }
-    if ((threadIdx.x & 63) == 0) atomicMax(out, m);
+    if ((threadIdx.x & 63) == 0 && m) atomicMax(a.out[y], m);
 }
 
 // An operand's 16-bit form: T itself, or pairs (mm16.h) of a float times its scale.
@@ -78,35 +97,55 @@ struct Planes<float> {
     static constexpr int count = 2;
 };
 
-// rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.
-template <class T>
+// rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
+// row, 8 values each at a time.
+template <class T, bool VEC>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              int kp, const uint32_t *amax, const float *bias) {
+                                              int kp, int lanes, const uint32_t *amax, const float *bias) {
     typedef typename Planes<T>::type P;
     constexpr int N = Planes<T>::count;
-    const size_t n = rows * (kp / 8);
+    const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
     float sc = 1.f;
     if constexpr (N == 2) sc = unit_scale(*amax);
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / (kp / 8);
-        const int c = (int)(i % (kp / 8)) * 8;
+    for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
-        Pack<P, 8> hi, lo;
+        for (int c = l * 8; c < kp; c += 8 << lanes) {
+            alignas(16) T v[8];
+            if (VEC && keep && c + 8 <= dim) {
+                constexpr int E = 16 / (int)sizeof(T);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const T v = keep && c + e < dim ? x[r * ld + c + e] : (T)0.f;
-            if constexpr (N == 2) {
-                const float f = v * sc;
-                hi.v[e] = (half_t)f;
-                lo.v[e] = (half_t)(f - (float)hi.v[e]);
+                for (int h = 0; h < 8 / E; ++h) *reinterpret_cast<Pack<T, E> *>(v + h * E) = *reinterpret_cast<const Pack<T, E> *>(x + r * ld + c + h * E);
             } else {
-                hi.v[e] = v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = keep && c + e < dim ? x[r * ld + c + e] : (T)0.f;
             }
+            Pack<P, 8> hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (N == 2) {
+                    const float f = v[e] * sc;
+                    hi.v[e] = (half_t)f;
+                    lo.v[e] = (half_t)(f - (float)hi.v[e]);
+                } else {
+                    hi.v[e] = v[e];
+                }
+            }
+            P *o = out + r * kp * N + (N == 2 ? pair_at(c) : c);
+            *reinterpret_cast<Pack<P, 8> *>(o) = hi;
+            if constexpr (N == 2) *reinterpret_cast<Pack<P, 8> *>(o + 32) = lo;
         }
-        P *o = out + r * kp * N + (N == 2 ? pair_at(c) : c);
-        *reinterpret_cast<Pack<P, 8> *>(o) = hi;
-        if constexpr (N == 2) *reinterpret_cast<Pack<P, 8> *>(o + 32) = lo;
     }
+}
+template <class T>
+void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const uint32_t *amax,
+          const float *bias, hipStream_t s) {
+    const int lanes = lanes_log2(kp / 8);
+    const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
+    const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
+    if (aligned16(x) && ld % (16 / sizeof(T)) == 0)
+        k_pack<T, true><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+    else
+        k_pack<T, false><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
@@ -558,11 +597,6 @@ inline Parts carve(Carver &c, const Sizes &z) {
     return p;
 }
 
-inline uint32_t wide_grid(size_t items) {
-    const size_t b = (items + 255) / 256;
-    return (uint32_t)(b < 4096 ? (b ? b : 1) : 4096);
-}
-
 struct Call {
     const void *h, *table, *bias;
     size_t ldh, ldt;
@@ -622,14 +656,14 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
 
     if (kSplit || z.grad) k_xent_init<<<1, 64, 0, s>>>(p.sc);
     if constexpr (kSplit) {
-        k_amax<<<(uint32_t)(z.rows < 1024 ? z.rows : 1024), 256, 0, s>>>((const float *)c.h, z.rows, dim, c.ldh, &p.sc->amax_h);
-        k_amax<<<(uint32_t)(z.table < 1024 ? z.table : 1024), 256, 0, s>>>((const float *)c.table, z.table, dim, c.ldt, &p.sc->amax_w);
+        const bool vec = dim % 4 == 0 && c.ldh % 4 == 0 && c.ldt % 4 == 0 && aligned16(c.h) && aligned16(c.table);
+        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2(vec ? z.dim / 4 : z.dim), vec};
+        k_amax<<<dim3(2048, 2), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
     if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
-        k_pack<T><<<wide_grid(z.table * (z.kp / 8)), 256, 0, s>>>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp,
-                                                                  &p.sc->amax_w, (const float *)c.bias);
+        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, &p.sc->amax_w, (const float *)c.bias, s);
         wp = (const P *)p.wp;
         ldw = z.kp * Planes<T>::count;
     }
@@ -641,8 +675,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            k_pack<T><<<wide_grid(rows * (z.kp / 8)), 256, 0, s>>>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp,
-                                                                &p.sc->amax_h, nullptr);
+            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, &p.sc->amax_h, nullptr, s);
             hp = (const P *)p.hp;
             ldh = z.kp * Planes<T>::count;
         }

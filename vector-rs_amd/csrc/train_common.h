@@ -36,6 +36,13 @@ struct CallDevice {
     }
 };
 
+// Threads of a 256-lane workgroup over rows of `chunks` items each: 2^log2 lanes a row.
+inline int lanes_log2(size_t chunks) {
+    int l = 0;
+    while (l < 8 && ((size_t)1 << l) < chunks) ++l;
+    return l;
+}
+
 // Status of the launches of a call so far.
 inline int launch_status(const char *what) {
     const hipError_t e = hipGetLastError();

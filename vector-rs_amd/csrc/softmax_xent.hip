@@ -12,7 +12,7 @@
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
 // plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
-// operands), which is as far as the gradients that are returned are rounded too.  In float16 it is held
+// operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) it is held
 // times 2^14 / 2^e, where 2^e is the power of two above the largest weight times scale: |G| is then at most
 // 2^14 and small probabilities keep their bits; the products' epilogues take the factor out again.
 //
@@ -24,6 +24,7 @@
 
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 namespace vh {
 namespace {
@@ -82,7 +83,14 @@ __global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
         const uint32_t v = __shfl_xor(m, o, 64);
         m = v > m ? v : m;
     }
-    if ((threadIdx.x & 63) == 0 && m) atomicMax(a.out[y], m);
+    // one atomic a workgroup: they are taken one after the other (8192 of them: 150 us)
+    __shared__ uint32_t tops[4];
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 4; ++w) m = tops[w] > m ? tops[w] : m;
+        if (m) atomicMax(a.out[y], m);
+    }
 }
 
 // An operand's 16-bit form: T itself, or pairs (mm16.h) of a float times its scale.
@@ -355,7 +363,7 @@ struct GradEpi {
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = to_logits(acc, lg, m, table), unit = unit_scale(lg.sc->cmax);
+        const float f = to_logits(acc, lg, m, table), unit = std::is_same_v<G, bf16_t> ? 1.f : unit_scale(lg.sc->cmax);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
@@ -406,10 +414,11 @@ struct GradEpi {
 
 // Factor that a gradient's product still has to be multiplied with.
 struct OutScale {
-    const Scalars *sc;
+    const Scalars *sc;  // null: none
     bool split;
     bool of_table;  // the product with the rows (the table's gradient), else with the table
     __device__ __forceinline__ float operator()() const {
+        if (!sc) return 1.f;
         float f = 1.f / unit_scale(sc->cmax);
         if (split) f /= unit_scale(of_table ? sc->amax_h : sc->amax_w);
         return f;
@@ -490,7 +499,7 @@ __global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts
     if (g != 0 || at >= n) return;
 #pragma unroll
     for (int p = 1; p < 8; ++p) v += sums[p][l];
-    v *= sc.sc ? sc() : 1.f;
+    v *= sc();
     const int r = (int)(at / (cols4 / 4)), c = (int)(at % (cols4 / 4)) * 4;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -536,7 +545,7 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.small = rows <= (size_t)kSmallRows;
     if (z.small) {
         z.piece_rows = rows;
-        const size_t groups = (table + 15) / 16, tiles = (table + 63) / 64, ny = ceil_div(dim, vh::kSmallCols);
+        const size_t groups = (table + 15) / 16, tiles = (table + kSmallEntries - 1) / kSmallEntries, ny = ceil_div(dim, kSmallCols);
         z.pieces = (int)(groups < 2048 ? groups : 2048);
         size_t gx = 1024 / ny;
         if (gx < 64) gx = 64;
@@ -611,7 +620,7 @@ struct Call {
 // The pieces' join: as many rows a workgroup as still fill the chip.
 inline void join_pieces(const Parts &p, const Sizes &z, size_t rows, const int64_t *target, const float *weight, float scale,
                         float *loss, float *lse, hipStream_t s) {
-    Scalars *sc = z.grad && !z.small ? p.sc : nullptr;
+    Scalars *sc = z.grad && !z.small && z.dtype != VHIP_DTYPE_BF16 ? p.sc : nullptr;
 #define JOIN(R)                                                                                                       \
     k_xent_join<R><<<(uint32_t)ceil_div(rows, R), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table, \
                                                                weight, scale, loss, lse, p.stat, p.rowfac, sc)
@@ -654,11 +663,12 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
-    if (kSplit || z.grad) k_xent_init<<<1, 64, 0, s>>>(p.sc);
+    constexpr bool kUnit = !std::is_same_v<P, bf16_t>;  // G is held in units of the largest weight
+    if (kUnit && (kSplit || z.grad)) k_xent_init<<<1, 64, 0, s>>>(p.sc);
     if constexpr (kSplit) {
         const bool vec = dim % 4 == 0 && c.ldh % 4 == 0 && c.ldt % 4 == 0 && aligned16(c.h) && aligned16(c.table);
         const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2(vec ? z.dim / 4 : z.dim), vec};
-        k_amax<<<dim3(2048, 2), 256, 0, s>>>(m);
+        k_amax<<<dim3(1024, 2), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
@@ -718,7 +728,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.N = (int)rows;
             d.K = table;
             d.ksplit = z.ksplit;
-            const OutScale os{p.sc, kSplit, false};
+            const OutScale os{kUnit ? p.sc : nullptr, kSplit, false};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
                          true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
@@ -741,7 +751,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.alo = d.blo = true;
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
-            OutEpi<T> oe{OutScale{p.sc, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
+            OutEpi<T> oe{OutScale{kUnit ? p.sc : nullptr, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % (16 / sizeof(T)) == 0 && aligned16(c.dtable)};
             VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_big, oe, s));
         }

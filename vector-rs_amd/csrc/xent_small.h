@@ -7,7 +7,7 @@
 //    table of 64 columns).  A workgroup takes 16 entries at a time; its four waves share the K loop, so a CU
 //    has enough loads in flight for short tables too.  32-bit operands are multiplied as they are, in the
 //    32-bit matrix instruction (157 TFLOP/s: above the memory's rate up to 48 rows).
-//  * k_small_grad turns 64 entries' logits into G in LDS, writes these entries' rows of the table's gradient
+//  * k_small_grad turns 32 entries' logits into G in LDS, writes these entries' rows of the table's gradient
 //    and adds the rows' gradient up in registers; the workgroups' sums are joined afterwards.  G is not
 //    rounded here, and 16-bit operands are widened.
 #pragma once
@@ -152,135 +152,152 @@ struct SmallGrad {
     bool vec;  // of dtable
 };
 
-constexpr int kSmallCols = 128;  // columns of a workgroup
+constexpr int kSmallCols = 128;    // columns of a workgroup
+constexpr int kSmallEntries = 32;  // entries of a turn
 
+// Wave w: entries 16 (w & 1) .. of a turn, columns 64 (w >> 1) .. of the workgroup's.
 template <class T, int TB, bool VEC>
 __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
-    constexpr int R = 16 * TB, GP = 68, HP = kSmallCols + 4;
+    constexpr int R = 16 * TB, NV = kSmallEntries, GP = NV + 4, HP = kSmallCols + 4, NZ = R * NV / 256;
     __shared__ __align__(16) float s_g[R * GP], s_h[R * HP];
-    __shared__ float s_cs[R], s_c[R], s_about[R];
-    __shared__ int s_y[R];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
-    const int d0 = blockIdx.y * kSmallCols;
-    for (int t = tid; t < R; t += 256) {
-        const float c = t < a.rows ? a.rowfac[t] : 0.f;
-        const float2 st = t < a.rows ? a.stat[t] : make_float2(0.f, 0.f);
-        const int64_t y = t < a.rows ? a.target[t] : -1;
-        s_c[t] = c;
-        s_cs[t] = c * st.y;
-        s_about[t] = st.x;
-        s_y[t] = y < a.table ? (int)y : -1;
-    }
-    for (int k = tid; k < R * kSmallCols; k += 256) {
-        const int t = k / kSmallCols, c = k % kSmallCols;
-        float v = 0.f;
-        if (t < a.rows && d0 + c < a.dim && a.target[t] >= 0) v = (float)((const T *)a.h)[(size_t)t * a.ldh + d0 + c];
-        s_h[t * HP + c] = v;
-    }
-    floatx4_t dh[2][TB][4];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int j = 0; j < TB; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dh[c][j][e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    const int sub = 16 * (wave & 1), cw = 64 * (wave >> 1), d0 = blockIdx.y * kSmallCols;
 
-    // 64 columns are four MFMA blocks: block e's row r is column 4 r + e, so that operands and results are
-    // four neighbouring columns a lane
-    for (int v0 = blockIdx.x * 64; v0 < a.table; v0 += gridDim.x * 64) {
+    // this thread's logits of a turn: rows tz + 8 k, entry vz
+    const int tz = tid / NV, vz = tid % NV;
+    float zr[NZ], wr[4][4];
+    auto fetch = [&](int v0) {
+#pragma unroll
+        for (int k = 0; k < NZ; ++k) {
+            const int t = tz + 256 / NV * k;
+            zr[k] = t < a.rows && v0 + vz < a.table ? a.z[(size_t)t * a.vp + v0 + vz] : -INFINITY;
+        }
+        if (!a.part) return;
+        const int col = d0 + cw + 4 * i;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int v = v0 + sub + 4 * q + k;
+            const bool on = v < a.table && !(a.bias && a.bias[v] == -INFINITY);
+            const T *w = (const T *)a.w + (size_t)(on ? v : 0) * a.ldw + col;
+            if (VEC) {
+                Pack<T, 4> p{};
+                if (on && col < a.dim) p = *reinterpret_cast<const Pack<T, 4> *>(w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wr[k][e] = (float)p.v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wr[k][e] = on && col + e < a.dim ? (float)w[e] : 0.f;
+            }
+        }
+    };
+    fetch(blockIdx.x * NV);
+    float cs[NZ], cc[NZ], about[NZ];
+    int yy[NZ];
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) {
+        const int t = tz + 256 / NV * k;
+        const bool in = t < a.rows;
+        const float2 st = in ? a.stat[t] : make_float2(0.f, 0.f);
+        const int64_t y = in ? a.target[t] : -1;
+        cc[k] = in ? a.rowfac[t] : 0.f;
+        cs[k] = cc[k] * st.y;
+        about[k] = st.x;
+        yy[k] = y < a.table ? (int)y : -1;
+    }
+    // h of the workgroup's columns, zeros in rows that do not count: every load before the first store
+    constexpr int HV = kSmallCols / 4, NH = R * HV / 256;
+    float hr[NH][4];
+#pragma unroll
+    for (int k = 0; k < NH; ++k) {
+        const int t = tid / HV + 256 / HV * k, col = d0 + tid % HV * 4;
+        const T *h = (const T *)a.h + (size_t)min(t, a.rows - 1) * a.ldh + col;
+        const bool on = t < a.rows && a.target[min(t, a.rows - 1)] >= 0;
+        if (VEC) {
+            Pack<T, 4> p{};
+            if (col < a.dim) p = *reinterpret_cast<const Pack<T, 4> *>(h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hr[k][e] = on ? (float)p.v[e] : 0.f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hr[k][e] = on && col + e < a.dim ? (float)h[e] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NH; ++k)
+        *reinterpret_cast<floatx4_t *>(s_h + (tid / HV + 256 / HV * k) * HP + tid % HV * 4) = floatx4_t{hr[k][0], hr[k][1], hr[k][2], hr[k][3]};
+    floatx4_t dh[TB][4];
+#pragma unroll
+    for (int j = 0; j < TB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dh[j][e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+
+    // A wave's 64 columns are four MFMA blocks: block e's row r is column 4 r + e, so that operands and
+    // results are four neighbouring columns a lane.
+    for (int v0 = blockIdx.x * NV; v0 < a.table; v0 += gridDim.x * NV) {
         __syncthreads();  // s_h (first turn), the last turn's s_g
-#pragma unroll 4
-        for (int k = tid; k < R * 64; k += 256) {
-            const int t = k >> 6, v = v0 + (k & 63);
-            const float c = s_c[t];
+#pragma unroll
+        for (int k = 0; k < NZ; ++k) {
             float g = 0.f;
-            if (c != 0.f && t < a.rows && v < a.table)
-                g = fmaf(s_cs[t], exp_fine(a.z[(size_t)t * a.vp + v] - s_about[t]), v == s_y[t] ? -c : 0.f);
-            s_g[t * GP + (k & 63)] = g;
+            if (cc[k] != 0.f) g = fmaf(cs[k], exp_fine(zr[k] - about[k]), v0 + vz == yy[k] ? -cc[k] : 0.f);
+            if (v0 + vz >= a.table) g = 0.f;
+            s_g[(tz + 256 / NV * k) * GP + vz] = g;
         }
         __syncthreads();
-        const int vw = v0 + 16 * wave;
-        if (vw >= a.table) continue;  // a whole wave; the barriers are at the loop's head
         if (a.part) {
-            floatx4_t g[TB];  // rows 16 j + i, entries vw + 4 q ..
+            floatx4_t g[TB];  // rows 16 j + i, entries sub + 4 q ..
 #pragma unroll
-            for (int j = 0; j < TB; ++j) g[j] = *reinterpret_cast<const floatx4_t *>(s_g + (16 * j + i) * GP + 16 * wave + 4 * q);
+            for (int j = 0; j < TB; ++j) g[j] = *reinterpret_cast<const floatx4_t *>(s_g + (16 * j + i) * GP + sub + 4 * q);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int v = vw + 4 * q + k;
-                const bool on = v < a.table && !(a.bias && a.bias[v] == -INFINITY);
-                const T *wr = (const T *)a.w + (size_t)(on ? v : 0) * a.ldw;
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int col = d0 + 64 * c + 4 * i;
-                    float x[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (VEC) {
-                        if (on && col < a.dim) {
-                            const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4> *>(wr + col);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = (float)p.v[e];
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (on && col + e < a.dim) x[e] = (float)wr[col + e];
-                    }
-#pragma unroll
-                    for (int j = 0; j < TB; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            dh[c][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], g[j][k], dh[c][j][e], 0, 0, 0);
-                }
-            }
-        }
-        if (!a.dtable) continue;
-        const int v = vw + i;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (d0 + 64 * c >= a.dim) break;
-            floatx4_t dw[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dw[e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 4 * TB; ++k) {
-                const floatx4_t x = *reinterpret_cast<const floatx4_t *>(s_h + (4 * k + q) * HP + 64 * c + 4 * i);
-                const float g = s_g[(4 * k + q) * GP + 16 * wave + i];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dw[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], g, dw[e], 0, 0, 0);
-            }
-            if (v >= a.table) continue;
-            T *o = (T *)a.dtable + (size_t)v * a.ldo;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int col = d0 + 64 * c + 16 * q + 4 * x;
-                if (a.vec && col + 4 <= a.dim) {
-                    Pack<T, 4> p;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p.v[e] = (T)dw[e][x];
-                    *reinterpret_cast<Pack<T, 4> *>(o + col) = p;
-                } else {
+                for (int j = 0; j < TB; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (col + e < a.dim) o[col + e] = (T)dw[e][x];
-                }
+                        dh[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(wr[k][e], g[j][k], dh[j][e], 0, 0, 0);
+        }
+        if (v0 + gridDim.x * NV < (size_t)a.table) fetch(v0 + gridDim.x * NV);
+        if (!a.dtable || d0 + cw >= a.dim) continue;
+        floatx4_t dw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dw[e] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4 * TB; ++k) {
+            const floatx4_t x = *reinterpret_cast<const floatx4_t *>(s_h + (4 * k + q) * HP + cw + 4 * i);
+            const float g = s_g[(4 * k + q) * GP + sub + i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dw[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], g, dw[e], 0, 0, 0);
+        }
+        const int v = v0 + sub + i;
+        if (v >= a.table) continue;
+        T *o = (T *)a.dtable + (size_t)v * a.ldo;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int col = d0 + cw + 16 * q + 4 * x;
+            if (a.vec && col + 4 <= a.dim) {
+                Pack<T, 4> p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p.v[e] = (T)dw[e][x];
+                *reinterpret_cast<Pack<T, 4> *>(o + col) = p;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < a.dim) o[col + e] = (T)dw[e][x];
             }
         }
     }
     if (!a.part) return;
-    // the four waves' sums, one wave after the other
-    for (int w = 0; w < 4; ++w) {
+    // the two waves of a column range, one after the other
+    for (int w = 0; w < 2; ++w) {
         __syncthreads();
-        if (wave != w) continue;
+        if ((wave & 1) != w) continue;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int j = 0; j < TB; ++j)
 #pragma unroll
-            for (int j = 0; j < TB; ++j)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    floatx4_t *p = reinterpret_cast<floatx4_t *>(s_h + (16 * j + i) * HP + 64 * c + 16 * q + 4 * x);
-                    const floatx4_t v = {dh[c][j][0][x], dh[c][j][1][x], dh[c][j][2][x], dh[c][j][3][x]};
-                    *p = w == 0 ? v : *p + v;
-                }
+            for (int x = 0; x < 4; ++x) {
+                floatx4_t *p = reinterpret_cast<floatx4_t *>(s_h + (16 * j + i) * HP + cw + 16 * q + 4 * x);
+                const floatx4_t v = {dh[j][0][x], dh[j][1][x], dh[j][2][x], dh[j][3][x]};
+                *p = w == 0 ? v : *p + v;
+            }
     }
     __syncthreads();
     for (int k = tid; k < a.rows * (kSmallCols / 4); k += 256) {
@@ -313,7 +330,7 @@ void small_stat(const SmallStat &a, uint32_t grid, hipStream_t s) {
 template <class T>
 void small_grad(const SmallGrad &a, uint32_t gx, hipStream_t s) {
     const dim3 grid(gx, (uint32_t)ceil_div(a.dim, kSmallCols));
-    const bool vec = a.dim % 4 == 0 && a.ldw % 4 == 0 && ((uintptr_t)a.w & (4 * sizeof(T) - 1)) == 0;
+    const bool vec = a.dim % 4 == 0 && a.ldw % 4 == 0 && a.ldh % 4 == 0 && (((uintptr_t)a.w | (uintptr_t)a.h) & (4 * sizeof(T) - 1)) == 0;
 #define SMALL_GRAD(TB)                                             \
     if (vec)                                                       \
         k_small_grad<T, TB, true><<<grid, 256, 0, s>>>(a);         \

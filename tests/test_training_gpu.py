@@ -179,10 +179,16 @@ def xent_reference(h, w, target, scale, bias=None, weight=None):
         if lse[t] == -math.inf or z[t, y] == -math.inf:
             loss[t] = math.inf
             continue
-        loss[t] = lse[t] - z[t, y]
+        # by the other entries, so that 64 bits hold a loss and a 1 - p far below 2^-53
+        others = torch.exp(z[t] - z[t, y])
+        others[y] = 0.0
+        loss[t] = torch.log1p(others.sum())
+        if not torch.isfinite(loss[t]):
+            loss[t] = lse[t] - z[t, y]
         c = scale * (1.0 if weight is None else float(weight[t]))
         g[t] = c * torch.exp(z[t] - lse[t])
-        g[t, y] -= c
+        g[t, y] = 0.0
+        g[t, y] = -g[t].sum()
     return loss, torch.logsumexp(real, 1), g @ wd, g.t() @ hd, g, z, hd, wd
 
 
@@ -231,7 +237,7 @@ def xent_inputs(rows, table, dim, dtype, seed=0):
 
 XENT_SHAPES = [(1, 1, 1), (1, 5, 3), (2, 1000, 64), (3, 64, 64), (17, 1000, 100), (33, 4099, 256), (129, 300, 65), (256, 257, 128),
                (300, 2049, 320), (130, 70, 768), (700, 1300, 40), (20, 3000, 300), (64, 500, 130), (65, 500, 130),
-               (32, 40_000, 24), (50, 129, 1030)]
+               (32, 40_000, 24), (50, 129, 1030), (70, 70_000, 520), (260, 515, 390)]
 
 
 @pytest.mark.parametrize("rows,table,dim", XENT_SHAPES)
@@ -243,7 +249,7 @@ def test_softmax_xent(tr, rows, table, dim, dtype):
     xent_check(tr.softmax_xent_grad(h, w, y, weight, scale=2.0), h, w, y, 2.0, None, weight)
 
 
-@pytest.mark.parametrize("rows,table,dim", [(5, 90, 64), (40, 1000, 100), (300, 700, 128)])
+@pytest.mark.parametrize("rows,table,dim", [(5, 90, 64), (40, 1000, 100), (300, 700, 128), (90, 300, 520)])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_softmax_xent_left_out(tr, rows, table, dim, dtype):
     """Entries with a bias of -inf, rows with a negative target and NaN in both places; targets that are left
@@ -267,9 +273,9 @@ def test_softmax_xent_left_out(tr, rows, table, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("rows", [4, 100])
-def test_softmax_xent_nothing_left(tr, dtype, rows):
-    h, w, y = xent_inputs(rows, 130, 64, dtype)
+@pytest.mark.parametrize("rows,dim", [(4, 64), (100, 64), (100, 512)])
+def test_softmax_xent_nothing_left(tr, dtype, rows, dim):
+    h, w, y = xent_inputs(rows, 130, dim, dtype)
     bias = torch.full((130,), -math.inf, device="cuda")
     loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, bias=bias)
     assert (loss == math.inf).all() and (lse == -math.inf).all() and not dh.any() and not dw.any()
@@ -277,13 +283,13 @@ def test_softmax_xent_nothing_left(tr, dtype, rows):
     loss, _, dh, dw = tr.softmax_xent_grad(h, w, y)
     assert not loss.any() and not dh.any() and not dw.any()
     loss, lse, dh, dw = tr.softmax_xent_grad(h[:0], w, y[:0])
-    assert loss.shape == (0,) and dh.shape == (0, 64) and not dw.any()
+    assert loss.shape == (0,) and dh.shape == (0, dim) and not dw.any()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows", [5, 100])
-def test_softmax_xent_target_past_the_table(tr, dtype, rows):
-    h, w, y = xent_inputs(rows, 130, 64, dtype)
+@pytest.mark.parametrize("rows,dim", [(5, 64), (100, 64), (100, 512)])
+def test_softmax_xent_target_past_the_table(tr, dtype, rows, dim):
+    h, w, y = xent_inputs(rows, 130, dim, dtype)
     y[3] = 130
     loss, lse, dh, _ = tr.softmax_xent_grad(h, w, y)
     assert torch.isnan(loss[3]) and torch.isnan(dh[3]).all() and torch.isfinite(lse).all()
@@ -293,10 +299,10 @@ def test_softmax_xent_target_past_the_table(tr, dtype, rows):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("size", [1e-25, 1e-6, 1.0, 1e6])
-@pytest.mark.parametrize("rows", [20, 70])
-def test_softmax_xent_weights_of_any_size(tr, dtype, size, rows):
+@pytest.mark.parametrize("rows,dim", [(20, 64), (70, 64), (70, 512)])
+def test_softmax_xent_weights_of_any_size(tr, dtype, size, rows, dim):
     """Row weights far from one, among them a zero and signs, do not cost the gradients their bits."""
-    h, w, y = xent_inputs(rows, 500, 64, dtype)
+    h, w, y = xent_inputs(rows, 500, dim, dtype)
     weight = size * normal(8, rows)
     weight[3] = 0.0
     _, _, dh, dw = tr.softmax_xent_grad(h, w, y, weight)
@@ -325,15 +331,26 @@ def test_softmax_xent_strides_and_values_far_apart(tr, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_softmax_xent_in_pieces(tr, dtype, monkeypatch):
+@pytest.mark.parametrize("dim", [100, 520])
+def test_softmax_xent_in_pieces(tr, dtype, dim, monkeypatch):
     """Rows taken 256 at a time give what one piece gives: the same loss, gradients within their rounding."""
-    h, w, y = xent_inputs(700, 900, 100, dtype)
+    h, w, y = xent_inputs(700, 900, dim, dtype)
     weight = normal(4, 700)
     whole = tr.softmax_xent_grad(h, w, y, weight)
     monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
     parts = tr.softmax_xent_grad(h, w, y, weight)
     xent_check(parts, h, w, y, 1.0, None, weight)
     within(parts[0], whole[0].double(), 2 * E * 128 * (1 + whole[0].double().abs()))
+
+
+def test_softmax_xent_values_that_differ_in_size_by_entry(tr):
+    """Logits of a row spread over hundreds: probabilities down to the smallest that 32 bits hold."""
+    h, w, y = xent_inputs(100, 700, 512, "bf16")
+    w[::5] *= 40.0
+    w[3::64] *= 0.01
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=3.0), h, w, y, 3.0)
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=-3.0), h, w, y, -3.0)
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=0.0), h, w, y, 0.0)
 
 
 def test_softmax_xent_gradient_against_differences(tr):
@@ -440,6 +457,45 @@ def test_orthogonalize_edges(tr):
     got = tr.orthogonalize(two)
     assert torch.isnan(got[0]).all() and torch.equal(got[1], tr.orthogonalize(two[1]))
     assert tr.orthogonalize(m[:0]).shape == (0, 30) and tr.orthogonalize(two[:0]).shape == (0, 20, 30)
+
+
+# ---- buffers past 2^32 bytes ---------------------------------------------------------------------------
+
+def test_rows_far_apart(tr):
+    """Rows whose last lies more than 2^32 bytes, and 2^31 elements, behind the first."""
+    rows, dim, ld = 3000, 64, 1_000_000
+    wide = torch.empty(rows, ld, device="cuda", dtype=torch.bfloat16)
+    x = wide[:, 8:8 + dim]
+    x.copy_(normal(1, rows, dim))
+    near = x.contiguous()
+    y, mean, rstd = tr.layer_norm(x)
+    for a, b in zip((y, mean, rstd), tr.layer_norm(near)):
+        assert torch.equal(a, b)
+    for a, b in zip(tr.layer_norm_backward(x, x, None, mean, rstd), tr.layer_norm_backward(near, near, None, mean, rstd)):
+        assert torch.equal(a, b)
+    t = torch.randint(0, rows, (rows,), device="cuda", generator=gen(2))
+    for n in (20, 300):
+        for a, b in zip(tr.softmax_xent_grad(x[:n], x, t[:n]), tr.softmax_xent_grad(near[:n], near, t[:n])):
+            assert torch.equal(a, b)
+    assert torch.equal(tr.orthogonalize(x), tr.orthogonalize(near))
+    del wide, x
+
+
+def test_a_gradient_of_many_logits(tr):
+    """4.6e9 logits, in pieces of rows: losses by their definition, and a row's gradient as in a small call."""
+    rows, table, dim = 2300, 2_000_000, 16
+    h, w, y = xent_inputs(rows, table, dim, "bf16")
+    weight = torch.ones(rows, device="cuda")
+    loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, weight)
+    for at in (0, 1024, rows - 128):
+        part = slice(at, at + 128)
+        l2, e2, d2, _ = tr.softmax_xent_grad(h[part], w, y[part], weight[part])
+        xent_check((loss[part], lse[part], None, None), h[part], w, y[part], 1.0)
+        xent_check((l2, e2, None, None), h[part], w, y[part], 1.0)
+        within(dh[part], d2.double(), 4 * UNIT[torch.bfloat16] * d2.double().abs() + 1e-4 * d2.double().abs().max())
+    # every row's probabilities sum to one: the table's gradient adds up to (what the rows lose) = 0 over entries
+    total = dw.double().sum(0)
+    assert float(total.abs().max()) <= 2 ** -8 * float(dw.double().abs().sum(0).max())
 
 
 # ---- streams, graphs, refusals -----------------------------------------------------------------------

@@ -45,6 +45,7 @@ struct MmArgs {
     int ksplit;               // parts of the K loop, each a workgroup of its own
     int batch;
     bool upper;               // only tiles on and above the diagonal (square and symmetric products)
+    const uint32_t *only;     // null, or which tiles to compute: [tile of N][tile of M]
 };
 
 constexpr int kMmK = 64;               // k of one stage
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
     const MmPlace pl = mm_place(g, blockIdx.x, gridDim.x);
+    if (g.only && !g.only[(size_t)pl.tn * g.mt + pl.tm]) return;
     const int m0 = pl.tm * BM, n0 = pl.tn * BN;
 
     // this part's stages

@@ -4,17 +4,25 @@
 //   G_tv = c_t scale (exp(z_tv - lse_t) - [v = y_t]),  dh = G W,  dW = G^T h      (c: weights of the rows)
 //
 // The logits are never kept.  A first product (mm16.h) ends each 128-entry piece of a row's logits in its
-// largest value and the sum of exp about it; a small kernel joins the pieces.  For the gradients a second
-// product makes the same logits again and ends in G, which two more products multiply with the table and
-// with the rows.  Rows are taken in pieces so that G stays below kPieceBytes; from the second piece on the
-// table's gradient is added up in 32 bits.  Every sum has a fixed order: results do not depend on timing.
+// largest value and the sum of exp about it; a small kernel joins the pieces.  For the gradients G comes about
+// in one of two ways, and two more products multiply it with the table and with the rows:
+//  * a second product makes the same logits again and ends in G;
+//  * for wide rows (kStoreDim: a product costs more than a walk through memory) the first product also stores
+//    its exps about their piece's largest logit, and a kernel turns them into G where they lie.  In bfloat16
+//    they are float16 for that while (11 bits before G's 8; exp_code), which holds them down to 2^-57 of their
+//    piece's largest; a tile with smaller ones that a float could hold is marked and made the first way.
+// Rows are taken in pieces so that G stays below kPieceBytes; from the second piece on the table's gradient is
+// added up in 32 bits.  Every sum has a fixed order: results do not depend on timing.
 //
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
 // plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
 // operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) it is held
-// times 2^14 / 2^e, where 2^e is the power of two above the largest weight times scale: |G| is then at most
-// 2^14 and small probabilities keep their bits; the products' epilogues take the factor out again.
+// times 2^14 / 2^e, where 2^e is the power of two above the largest |G|, c scale (1 - p) at some row's target:
+// small probabilities keep their bits; the products' epilogues take the factor out again.
+//
+// A row's sum of exps leaves its target out until it is joined: 1 - p at the target, and the loss
+// log(1 + sum of the others / the target's), keep their bits where p is nearly one.
 //
 // What does not count: a row whose target is negative has loss 0 and no part in the gradients, whatever its
 // values (its h is replaced by zeros where sums over rows are made).  An entry whose bias is -inf is out of
@@ -31,11 +39,18 @@ namespace {
 
 constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G
 constexpr int kGBits = 14;
+// Columns from which G is made of stored exps.  A product's way costs 2 (pairs: 6) dim flops a value at 1.2
+// PFLOP/s, the walk's 4 (8) bytes at 4.5 TB/s and a few operations.  float16 always takes the product: its G
+// would be rounded twice to the 11 bits that the gradients have.
+constexpr size_t kStoreDim16 = 512, kStoreDim32 = 384;
+inline bool stores_exps(int dtype, size_t dim) {
+    return dtype == VHIP_DTYPE_F32 ? dim >= kStoreDim32 : (dtype == VHIP_DTYPE_BF16 && dim >= kStoreDim16);
+}
 
 // State of a call on the device.
 struct Scalars {
     uint32_t amax_h, amax_w;  // bits of the largest finite |value|
-    uint32_t cmax;            // bits of the largest |weight x scale| of a row that counts
+    uint32_t gmax;            // bits of the largest |G|: weight x scale x (1 - p) at a row's target
 };
 
 // 2^(14 - e) with 2^e > x >= 2^(e-1), so that x times it is in [2^13, 2^14); 1 for 0.
@@ -47,8 +62,10 @@ __device__ __forceinline__ float unit_scale(uint32_t bits) {
     return ldexpf(1.f, k);
 }
 
-__global__ void k_xent_init(Scalars *s) {
-    if (threadIdx.x == 0) *s = Scalars{0, 0, 0};
+__global__ __launch_bounds__(256) void k_xent_init(Scalars *s, uint32_t *marks, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i == 0) *s = Scalars{0, 0, 0};
+    if (i < n) marks[i] = 0;
 }
 
 // Largest finite |value| of h (blockIdx.y 0) and of the table (1).
@@ -203,6 +220,12 @@ struct Logits {
         return split ? scale / unit_scale(sc->amax_h) / unit_scale(sc->amax_w) : scale;
     }
 };
+// Exps in (0, 1] as float16: times 2^15, or those below 2^-28 negative and times 2^43.
+__device__ __forceinline__ half_t exp_code(float p) { return (half_t)(p * (p < 0x1p-28f ? -0x1p43f : 0x1p15f)); }
+__device__ __forceinline__ float exp_decode(half_t h) { return (float)h * (h < (half_t)0.f ? -0x1p-43f : 0x1p-15f); }
+// Arguments of exps that exp_code would cut short, and that are not nothing in 32 bits either.
+__device__ __forceinline__ bool exp_cut(float x) { return x < -39.f && x > -104.f; }
+
 // A wave's sums to f times them being the logits: where there is a bias, or entries past the table, the
 // logits themselves (-inf where an entry is out) and f = 1.
 template <int MB, int NB>
@@ -227,14 +250,22 @@ __device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logit
 }
 
 // Epilogue of the first product (A: table, B: rows): a wave's 16 MB entries of each row end in one piece.
+// E: the type that the exps are stored in, void: they are not; FINE: of 32-bit operands.
+template <class E, bool FINE>
 struct StatEpi {
     Logits lg;
-    float2 *part;  // [piece][rows]: largest logit, sum of exp about it
+    float2 *part;  // [piece][rows]: largest logit, sum of exp about it without the target's
     float2 *zt;    // the target's logit less its piece's largest, and that
     const int64_t *target;
     int rows, table;
+    E *exps;  // [rows][vp]
+    size_t vp;
+    uint32_t *marks;  // [tile of N][tile of M]: exps that float16 cannot hold
+    int mt;
     template <int MB, int NB>
-    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *) const {
+    __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
+        constexpr bool kHalf = std::is_same_v<E, half_t>;
+        bool cut = false;
         if (m >= table) return;
         const int l = threadIdx.x & 63, q = l >> 4;
         float f = to_logits(acc, lg, m, table);
@@ -259,23 +290,55 @@ struct StatEpi {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64)) * f;
             const float about = top == -INFINITY ? 0.f : top;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum += exp_neg(fmaf(acc[i][j][e], f, -about));
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
+            // the target's place among this lane's values, past them where it is not here
             const int64_t y = in ? target[t] : -1;
-            if (y >= m && y < m + 16 * MB && y < table) {
-                const int d = (int)(y - m) - 4 * q;
+            const int d = y >= m && y < m + 16 * MB && y < table ? (int)(y - m) - 4 * q : -1;
+            float sum = 0.f;
+            auto add = [&](float &v, bool skip) {
+                const float x = fmaf(v, f, -about);
+                const float p = FINE ? exp_fine(x) : exp_neg(x);
+                if constexpr (kHalf) cut |= exp_cut(x);
+                sum += skip ? 0.f : p;
+                if (skip) zt[t] = make_float2(x, about);
+                return p;
+            };
+            if (__any(d >= 0)) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d == 16 * i + e) zt[t] = make_float2(fmaf(acc[i][j][e], f, -about), about);
+                    for (int e = 0; e < 4; ++e) {
+                        float v = acc[i][j][e];
+                        v = add(v, d == 16 * i + e);
+                        if constexpr (!std::is_void_v<E>) acc[i][j][e] = v;
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = acc[i][j][e];
+                        v = add(v, false);
+                        if constexpr (!std::is_void_v<E>) acc[i][j][e] = v;
+                    }
             }
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
+        }
+        if constexpr (!std::is_void_v<E>) {
+            constexpr int PER = 16 / (int)sizeof(E);
+            if (kHalf && __any(cut) && l == 0) marks[(size_t)pl.tn * mt + pl.tm] = 1;
+            rows_through_lds<E, MB, NB>(
+                lds,
+                [&](int i, int j, int e) {
+                    if constexpr (kHalf)
+                        return exp_code(acc[i][j][e]);
+                    else
+                        return acc[i][j][e];
+                },
+                [&](int r, int c, const Pack<E, PER> &v) {
+                    if (n + r < rows && (size_t)(m + c) < vp) *reinterpret_cast<Pack<E, PER> *>(exps + (size_t)(n + r) * vp + m + c) = v;
+                });
         }
     }
 };
@@ -285,7 +348,7 @@ template <int R>
 __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float2 *zt,
                                                    const int64_t *target, int64_t table, const float *weight,
                                                    float scale, float *loss, float *lse, float2 *stat,
-                                                   float *rowfac, Scalars *sc) {
+                                                   float2 *rowfac, Scalars *sc) {
     constexpr int L0 = 256 / R;
     __shared__ float s_top[L0][R + 1], s_sum[L0][R + 1];
     const int k = threadIdx.x % R, g = threadIdx.x / R, t = blockIdx.x * R + k;
@@ -312,34 +375,41 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int piece
     }
     if (g != 0) return;
     const float about = top == -INFINITY ? 0.f : top;
-    const float L = sum == 0.f ? -INFINITY : about + logf(sum);
     const int64_t y = t < rows ? target[t] : -1;
-    float ls = 0.f, fac = 0.f;
+    float total = sum, ls = 0.f, fac = 0.f, rest = 0.f;
     if (y >= table) {
         ls = fac = NAN;
     } else if (y >= 0) {
         const float2 z = zt[t];
-        const bool out = L == -INFINITY || z.x == -INFINITY;
-        ls = out ? INFINITY : (about - z.y) - z.x + logf(sum);  // not lse - z, which cancels where the loss is small
-        if (!out) fac = (weight ? weight[t] : 1.f) * scale;
+        const float d = (about - z.y) - z.x;  // of the target's logit below the largest
+        total += exp_fine(-d);
+        if (total == 0.f || z.x == -INFINITY) {
+            ls = INFINITY;
+        } else {
+            const float u = sum * exp_fine(d);  // the others' share in units of the target's
+            ls = u < 1e30f ? log1pf(u) : d + logf(total);
+            rest = u < 1e30f ? u / (1.f + u) : (u == u ? 1.f : u);
+            fac = (weight ? weight[t] : 1.f) * scale;
+        }
     }
+    const float L = total == 0.f ? -INFINITY : about + logf(total);
     if (t < rows) {
         if (loss) loss[t] = ls;
         if (lse) lse[t] = L;
         if (rowfac) {
-            stat[t] = make_float2(about, 1.f / sum);
-            rowfac[t] = fac;
+            stat[t] = make_float2(about, 1.f / total);
+            rowfac[t] = make_float2(fac, fac * rest);
         }
     }
     if (sc) {
-        uint32_t u = __builtin_bit_cast(uint32_t, fac) & 0x7fffffffu;
+        uint32_t u = __builtin_bit_cast(uint32_t, fac * rest) & 0x7fffffffu;
         if (u >= 0x7f800000u) u = 0;
 #pragma unroll
         for (int o = 1; o < R; o <<= 1) {
             const uint32_t v = __shfl_xor(u, o, 64);
             u = v > u ? v : u;
         }
-        if (k == 0 && u) atomicMax(&sc->cmax, u);
+        if (k == 0 && u) atomicMax(&sc->gmax, u);
     }
 }
 
@@ -353,7 +423,7 @@ template <class G>
 struct GradEpi {
     Logits lg;
     const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
-    const float *rowfac;
+    const float2 *rowfac; // weight x scale, and times 1 - p at the target
     const int64_t *target;
     G *g;  // [tp][vp] values or pairs
     size_t vp;
@@ -363,13 +433,14 @@ struct GradEpi {
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = to_logits(acc, lg, m, table), unit = std::is_same_v<G, bf16_t> ? 1.f : unit_scale(lg.sc->cmax);
+        const float f = to_logits(acc, lg, m, table), unit = std::is_same_v<G, bf16_t> ? 1.f : unit_scale(lg.sc->gmax);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
             const bool in = t < rows;
             const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
-            const float c = in ? rowfac[t] * unit : 0.f, cs = c * st.y;
+            const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
+            const float c = fac.x * unit, cs = c * st.y;
             if (split) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
@@ -389,7 +460,7 @@ struct GradEpi {
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (d == 16 * i + e) acc[i][j][e] -= c;
+                        if (d == 16 * i + e) acc[i][j][e] = -fac.y * unit;
             }
             if (__any(c == 0.f)) {  // whatever such a row's logits are
 #pragma unroll
@@ -412,6 +483,62 @@ struct GradEpi {
     }
 };
 
+// Stored exps (E) into G where they lie: bfloat16 for float16, pairs for float.  A row a workgroup and
+// gridDim.y parts of it; `cols` entries a piece.  Rows from `rows` on become zeros.
+template <class E>
+__global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *part, int cols, const float2 *stat,
+                                                      const float2 *rowfac, const int64_t *target, int rows, int table,
+                                                      size_t vp, const Scalars *sc) {
+    constexpr int N = 16 / (int)sizeof(E);  // values of a lane
+    const int t = blockIdx.x;
+    const bool in = t < rows;
+    const float unit = std::is_same_v<E, half_t> ? 1.f : unit_scale(sc->gmax);
+    const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
+    const float c = fac.x * unit;
+    const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
+    const int64_t y = in ? target[t] : -1;
+    for (size_t v = ((size_t)blockIdx.y * 256 + threadIdx.x) * N; v < vp; v += (size_t)gridDim.y * 256 * N) {
+        E *at = (E *)g + (size_t)t * vp + v;
+        float x[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = 0.f;
+        if (c != 0.f) {
+            const Pack<E, N> p = *reinterpret_cast<const Pack<E, N> *>(at);
+            const float f = c * st.y * exp_fine(part[v / cols * rows + t].x - st.x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if constexpr (std::is_same_v<E, half_t>)
+                    x[e] = exp_decode(p.v[e]) * f;
+                else
+                    x[e] = p.v[e] * f;
+            }
+            if (y >= (int64_t)v && y < (int64_t)v + N && y < table) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (y == (int64_t)v + e) x[e] = -fac.y * unit;
+            }
+        }
+        if constexpr (std::is_same_v<E, half_t>) {
+            Pack<bf16_t, N> o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o.v[e] = (bf16_t)x[e];
+            *reinterpret_cast<Pack<bf16_t, N> *>(at) = o;
+        } else {
+            // 8 lanes hold a block of 32; they are of one wave, so its values are read before any is written
+            Pack<half_t, N> hi, lo;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                hi.v[e] = (half_t)x[e];
+                lo.v[e] = (half_t)(x[e] - (float)hi.v[e]);
+            }
+            half_t *o = (half_t *)g + (size_t)t * vp * 2 + pair_at(v);
+            __builtin_amdgcn_wave_barrier();
+            *reinterpret_cast<Pack<half_t, N> *>(o) = hi;
+            *reinterpret_cast<Pack<half_t, N> *>(o + 32) = lo;
+        }
+    }
+}
+
 // Factor that a gradient's product still has to be multiplied with.
 struct OutScale {
     const Scalars *sc;  // null: none
@@ -419,7 +546,7 @@ struct OutScale {
     bool of_table;  // the product with the rows (the table's gradient), else with the table
     __device__ __forceinline__ float operator()() const {
         if (!sc) return 1.f;
-        float f = 1.f / unit_scale(sc->cmax);
+        float f = 1.f / unit_scale(sc->gmax);
         if (split) f /= unit_scale(of_table ? sc->amax_h : sc->amax_w);
         return f;
     }
@@ -569,12 +696,19 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     return z;
 }
 
+// Tiles of the logits.
+inline size_t mark_count(const Sizes &z) {
+    const size_t b = z.stat_big ? 256 : 128;
+    return ((z.table + b - 1) / b) * ((z.piece_rows + b - 1) / b);
+}
+
 struct Parts {
     Scalars *sc;
     float2 *part;
-    float2 *stat, *zt;
-    float *rowfac, *split, *sum;
+    float2 *stat, *zt, *rowfac;
+    float *split, *sum;
     float *z;  // few rows: the logits
+    uint32_t *marks;
     void *hp, *wp, *ht, *g;
 };
 
@@ -587,7 +721,7 @@ inline Parts carve(Carver &c, const Sizes &z) {
     if (z.small) {
         if (z.grad) {
             p.stat = c.take<float2>(z.rows);
-            p.rowfac = c.take<float>(z.rows);
+            p.rowfac = c.take<float2>(z.rows);
             p.z = c.take<float>(z.rows * z.vp);
             p.split = c.take<float>((size_t)z.ksplit * z.rows * z.cols4);
         }
@@ -597,9 +731,10 @@ inline Parts carve(Carver &c, const Sizes &z) {
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
         p.stat = c.take<float2>(z.piece_rows);
-        p.rowfac = c.take<float>(z.piece_rows);
+        p.rowfac = c.take<float2>(z.piece_rows);
         p.ht = c.take<uint16_t>(planes * z.dim * z.tp);
         p.g = c.take<uint16_t>(planes * z.tp * z.vp);
+        p.marks = c.take<uint32_t>(mark_count(z));
         if (z.ksplit > 1) p.split = c.take<float>((size_t)z.ksplit * z.piece_rows * z.cols4);
         if (z.piece_rows < z.rows) p.sum = c.take<float>(z.table * z.cols4);
     }
@@ -641,7 +776,7 @@ int xent_small(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     join_pieces(p, z, z.rows, c.target, c.row_weight, c.scale, c.loss, c.lse, s);
     if (z.grad) {
         const bool vec = c.lddt % 4 == 0 && ((uintptr_t)c.dtable & (4 * sizeof(T) - 1)) == 0;
-        small_grad<T>(SmallGrad{c.h, c.table, (const float *)c.bias, p.z, p.rowfac, p.stat, c.target, c.dtable, c.dh ? p.split : nullptr,
+        small_grad<T>(SmallGrad{c.h, c.table, (const float *)c.bias, p.z, p.stat, p.rowfac, c.target, c.dtable, c.dh ? p.split : nullptr,
                                 c.ldh, c.ldt, c.lddt, z.vp, rows, table, dim, (int)z.cols4, vec},
                       (uint32_t)z.ksplit, s);
         if (c.dh) join_parts<T>(p.split, z.ksplit, rows, dim, (int)z.cols4, OutScale{}, (T *)c.dh, c.lddh, s);
@@ -664,7 +799,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
     constexpr bool kUnit = !std::is_same_v<P, bf16_t>;  // G is held in units of the largest weight
-    if (kUnit && (kSplit || z.grad)) k_xent_init<<<1, 64, 0, s>>>(p.sc);
+    if (kSplit || (kUnit && z.grad)) k_xent_init<<<1, 256, 0, s>>>(p.sc, nullptr, 0);
     if constexpr (kSplit) {
         const bool vec = dim % 4 == 0 && c.ldh % 4 == 0 && c.ldt % 4 == 0 && aligned16(c.h) && aligned16(c.table);
         const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2(vec ? z.dim / 4 : z.dim), vec};
@@ -700,24 +835,42 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.alo = g.blo = true;
         g.ksplit = g.batch = 1;
         const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
-        VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, StatEpi{lg, p.part, p.zt, target, (int)rows, table}, s));
+        typedef std::conditional_t<kSplit, float, half_t> E;
+        const bool store = z.grad && stores_exps(z.dtype, z.dim);
+        if (store) {
+            const StatEpi<E, kSplit> se{lg, p.part, p.zt, target, (int)rows, table, (E *)p.g, z.vp, p.marks, ceil_div(table, z.stat_big ? 256 : 128)};
+            if (!kSplit) k_xent_init<<<(uint32_t)ceil_div(mark_count(z), 256), 256, 0, s>>>(p.sc, p.marks, (int)mark_count(z));
+            VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, se, s));
+        } else {
+            const StatEpi<void, kSplit> se{lg, p.part, p.zt, target, (int)rows, table, nullptr, 0, nullptr, 0};
+            VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, se, s));
+        }
         join_pieces(p, z, rows, target, c.row_weight ? c.row_weight + r0 : nullptr, c.scale, c.loss ? c.loss + r0 : nullptr,
                     c.lse ? c.lse + r0 : nullptr, s);
         VH_CHECK(launch_status("softmax launch"));
         if (!z.grad) continue;
         const size_t tp = round_up(rows, kMmK);
-        GradEpi<P> ge{};
-        ge.lg = lg;
-        ge.stat = p.stat;
-        ge.rowfac = p.rowfac;
-        ge.target = target;
-        ge.g = (P *)p.g;
-        ge.vp = z.vp;
-        ge.rows = (int)rows;
-        ge.tp = (int)tp;
-        ge.table = table;
-        ge.split = kSplit;
-        VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, ge, s));
+        if (store) {
+            const size_t parts = (z.vp * sizeof(E) / 16 + 1023) / 1024;  // four turns of a workgroup each
+            k_exps_to_grad<E><<<dim3((uint32_t)tp, (uint32_t)(parts < 64 ? parts : 64)), 256, 0, s>>>(
+                p.g, p.part, z.stat_big ? 128 : 64, p.stat, p.rowfac, target, (int)rows, table, z.vp, p.sc);
+        }
+        if (!store || !kSplit) {
+            GradEpi<P> ge{};
+            ge.lg = lg;
+            ge.stat = p.stat;
+            ge.rowfac = p.rowfac;
+            ge.target = target;
+            ge.g = (P *)p.g;
+            ge.vp = z.vp;
+            ge.rows = (int)rows;
+            ge.tp = (int)tp;
+            ge.table = table;
+            ge.split = kSplit;
+            MmArgs gg = g;
+            gg.only = store ? p.marks : nullptr;
+            VH_CHECK((mm_launch<P, kMode, false, false>)(gg, z.stat_big, ge, s));
+        }
         const P *gg = (const P *)p.g;
         if (c.dh) {
             // columns of the table, K its rows: G's columns past the table are zeros

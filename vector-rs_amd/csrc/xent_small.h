@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
         const float about = m == -INFINITY ? 0.f : m;
         sum *= exp_neg(top - about);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += exp_neg(z[e] - about);
+        for (int e = 0; e < 4; ++e) sum += e0 + e == y ? 0.f : exp_neg(z[e] - about);
         top = m;
         if (mine) {
             if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
 
 struct SmallGrad {
     const void *h, *w;
-    const float *bias, *z, *rowfac;
-    const float2 *stat;
+    const float *bias, *z;
+    const float2 *stat, *rowfac;
     const int64_t *target;
     void *dtable;  // null: not wanted
     float *part;   // [gridDim.x][rows][cols4], null: the rows' gradient is not wanted
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
         }
     };
     fetch(blockIdx.x * NV);
-    float cs[NZ], cc[NZ], about[NZ];
+    float cs[NZ], cc[NZ], cy[NZ], about[NZ];
     int yy[NZ];
 #pragma unroll
     for (int k = 0; k < NZ; ++k) {
@@ -199,7 +199,9 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
         const bool in = t < a.rows;
         const float2 st = in ? a.stat[t] : make_float2(0.f, 0.f);
         const int64_t y = in ? a.target[t] : -1;
-        cc[k] = in ? a.rowfac[t] : 0.f;
+        const float2 fac = in ? a.rowfac[t] : make_float2(0.f, 0.f);
+        cc[k] = fac.x;
+        cy[k] = fac.y;
         cs[k] = cc[k] * st.y;
         about[k] = st.x;
         yy[k] = y < a.table ? (int)y : -1;
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
 #pragma unroll
         for (int k = 0; k < NZ; ++k) {
             float g = 0.f;
-            if (cc[k] != 0.f) g = fmaf(cs[k], exp_fine(zr[k] - about[k]), v0 + vz == yy[k] ? -cc[k] : 0.f);
+            if (cc[k] != 0.f) g = v0 + vz == yy[k] ? -cy[k] : cs[k] * exp_fine(zr[k] - about[k]);
             if (v0 + vz >= a.table) g = 0.f;
             s_g[(tz + 256 / NV * k) * GP + vz] = g;
         }

@@ -123,8 +123,8 @@ struct Planes<float> {
 };
 
 // rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
-// row, 8 values each at a time.
-template <class T, bool VEC>
+// row, 8 values each at a time, loaded E together (1: at any alignment).
+template <class T, int E>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
                                               int kp, int lanes, const uint32_t *amax, const float *bias) {
     typedef typename Planes<T>::type P;
@@ -136,8 +136,7 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
         const bool keep = !bias || bias[r] != -INFINITY;
         for (int c = l * 8; c < kp; c += 8 << lanes) {
             alignas(16) T v[8];
-            if (VEC && keep && c + 8 <= dim) {
-                constexpr int E = 16 / (int)sizeof(T);
+            if (E > 1 && keep && c + 8 <= dim) {
 #pragma unroll
                 for (int h = 0; h < 8 / E; ++h) *reinterpret_cast<Pack<T, E> *>(v + h * E) = *reinterpret_cast<const Pack<T, E> *>(x + r * ld + c + h * E);
             } else {
@@ -167,10 +166,14 @@ void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type 
     const int lanes = lanes_log2(kp / 8);
     const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
     const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
-    if (aligned16(x) && ld % (16 / sizeof(T)) == 0)
-        k_pack<T, true><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+    constexpr int E = 16 / (int)sizeof(T);
+    const uintptr_t at = (uintptr_t)x | ld * sizeof(T);
+    if (at % 16 == 0)
+        k_pack<T, E><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+    else if (at % 8 == 0)
+        k_pack<T, E / 2><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
     else
-        k_pack<T, false><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+        k_pack<T, 1><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
@@ -418,8 +421,8 @@ __global__ __launch_bounds__(256) void k_zero_rows(char *p, size_t rows, size_t 
         for (size_t i = threadIdx.x; i < row_bytes; i += 256) p[r * ld_bytes + i] = 0;
 }
 
-// Epilogue of the second product: G.
-template <class G>
+// Epilogue of the second product: G, SPLIT: in pairs.
+template <class G, bool SPLIT>
 struct GradEpi {
     Logits lg;
     const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
@@ -428,7 +431,6 @@ struct GradEpi {
     G *g;  // [tp][vp] values or pairs
     size_t vp;
     int rows, tp, table;
-    bool split;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
@@ -441,7 +443,7 @@ struct GradEpi {
             const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
             const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
             const float c = fac.x * unit, cs = c * st.y;
-            if (split) {
+            if constexpr (SPLIT) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -454,13 +456,13 @@ struct GradEpi {
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = cs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], f2, -a2));
             }
             const int64_t y = in ? target[t] : -1;
-            if (y >= m && y < m + 16 * MB) {
-                const int d = (int)(y - m) - 4 * q;
+            const int d = y >= m && y < m + 16 * MB ? (int)(y - m) - 4 * q : -1;
+            if (__any(d >= 0)) {
+                const float own = -fac.y * unit;
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d == 16 * i + e) acc[i][j][e] = -fac.y * unit;
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = d == 16 * i + e ? own : acc[i][j][e];
             }
             if (__any(c == 0.f)) {  // whatever such a row's logits are
 #pragma unroll
@@ -469,15 +471,18 @@ struct GradEpi {
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = c == 0.f ? 0.f : acc[i][j][e];
             }
         }
-        auto store = [&](int low) {
-            return [=, *this](int r, int c, const Pack<G, 8> &v) {
-                if (n + r >= tp || (size_t)(m + c) >= vp) return;
-                G *o = split ? g + (size_t)(n + r) * vp * 2 + pair_at(m + c) + low : g + (size_t)(n + r) * vp + m + c;
+        G *const to = g;  // nothing of this struct goes through memory
+        const size_t ld = vp;
+        const int last = tp;
+        auto store = [=](int low) {
+            return [=](int r, int c, const Pack<G, 8> &v) {
+                if (n + r >= last || (size_t)(m + c) >= ld) return;
+                G *o = SPLIT ? to + (size_t)(n + r) * ld * 2 + pair_at(m + c) + low : to + (size_t)(n + r) * ld + m + c;
                 *reinterpret_cast<Pack<G, 8> *>(o) = v;
             };
         };
         rows_through_lds<G, MB, NB>(lds, [&](int i, int j, int e) { return (G)acc[i][j][e]; }, store(0));
-        if (split)
+        if constexpr (SPLIT)
             rows_through_lds<G, MB, NB>(
                 lds, [&](int i, int j, int e) { return (G)(acc[i][j][e] - (float)(G)acc[i][j][e]); }, store(32));
     }
@@ -856,7 +861,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
                 p.g, p.part, z.stat_big ? 128 : 64, p.stat, p.rowfac, target, (int)rows, table, z.vp, p.sc);
         }
         if (!store || !kSplit) {
-            GradEpi<P> ge{};
+            GradEpi<P, kSplit> ge{};
             ge.lg = lg;
             ge.stat = p.stat;
             ge.rowfac = p.rowfac;
@@ -866,7 +871,6 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             ge.rows = (int)rows;
             ge.tp = (int)tp;
             ge.table = table;
-            ge.split = kSplit;
             MmArgs gg = g;
             gg.only = store ? p.marks : nullptr;
             VH_CHECK((mm_launch<P, kMode, false, false>)(gg, z.stat_big, ge, s));

@@ -25,6 +25,7 @@
  *   InvertedList/Index    ivf/inverted_list.rs
  *   IvfPqIndex            ivf/mod.rs:63-449 (storage: a flat row-major float array)
  *   IvfPqSerializer       ivf/serializer.rs:16-377 (IVFPQVEC and VRSKMEAN files)
+ * The operators that train vectors (namespace training) have no counterpart there.
  * VectorIndexError::EmptyIndex is CudaError(EmptyIndex); DimensionMismatch and the config's
  * reasons are CudaError(InvalidConfig).
  */
@@ -869,6 +870,80 @@ private:
     DistanceMetric metric_;
     vhip_ivfpq_desc info_{};
 };
+
+/* ---- training operators (no reference counterpart) ------------------------------------------
+ * Functions over the entry points of the same names: device memory, a stream, the caller's workspace; a
+ * refusal is a thrown CudaError. */
+enum class DType : int { F32 = VHIP_DTYPE_F32, F16 = VHIP_DTYPE_F16, BF16 = VHIP_DTYPE_BF16 };
+
+namespace training {
+
+/* Where a call runs and what it works in. */
+struct Place {
+    int ordinal = 0;
+    void *stream = nullptr; /* hipStream_t */
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+};
+/* Rows of one type in device memory, `ld` elements apart. */
+struct Rows {
+    const void *data = nullptr;
+    size_t rows = 0, dim = 0, ld = 0;
+};
+struct MutableRows {
+    void *data = nullptr;
+    size_t ld = 0;
+};
+
+inline void layer_norm(const Place &at, DType type, DType params, const Rows &x, const void *weight, const void *bias,
+                       float eps, const MutableRows &y, float *mean, float *rstd) {
+    detail::check(vhip_layer_norm(at.ordinal, (int)type, (int)params, x.data, x.rows, x.dim, x.ld, weight, bias, eps, y.data,
+                                  y.ld, mean, rstd, at.stream));
+}
+inline size_t layer_norm_backward_workspace(const Rows &x) { return vhip_layer_norm_backward_workspace(x.rows, x.dim); }
+inline void layer_norm_backward(const Place &at, DType type, DType params, const Rows &dy, const Rows &x, const void *weight,
+                                const float *mean, const float *rstd, const MutableRows &dx, void *dweight, void *dbias) {
+    detail::require(dy.rows == x.rows && dy.dim == x.dim, "dy must have the shape of x");
+    detail::check(vhip_layer_norm_backward(at.ordinal, (int)type, (int)params, dy.data, dy.ld, x.data, x.ld, weight, mean,
+                                           rstd, x.rows, x.dim, dx.data, dx.ld, dweight, dbias, at.workspace,
+                                           at.workspace_bytes, at.stream));
+}
+
+inline size_t softmax_xent_workspace(DType type, const Rows &h, const Rows &table, bool gradients) {
+    return vhip_softmax_xent_workspace((int)type, h.rows, table.rows, h.dim, gradients);
+}
+inline void softmax_xent(const Place &at, DType type, const Rows &h, const Rows &table, const int64_t *target,
+                         const float *bias, float scale, float *loss, float *lse) {
+    detail::require(h.dim == table.dim, "dimension mismatch");
+    detail::check(vhip_softmax_xent(at.ordinal, (int)type, h.data, h.rows, h.ld, table.data, table.rows, table.ld, h.dim,
+                                    target, bias, scale, loss, lse, at.workspace, at.workspace_bytes, at.stream));
+}
+inline void softmax_xent_grad(const Place &at, DType type, const Rows &h, const Rows &table, const int64_t *target,
+                              const float *bias, const float *row_weight, float scale, float *loss, float *lse,
+                              const MutableRows &dh, const MutableRows &dtable) {
+    detail::require(h.dim == table.dim, "dimension mismatch");
+    detail::check(vhip_softmax_xent_grad(at.ordinal, (int)type, h.data, h.rows, h.ld, table.data, table.rows, table.ld, h.dim,
+                                         target, bias, row_weight, scale, loss, lse, dh.data, dh.ld, dtable.data, dtable.ld,
+                                         at.workspace, at.workspace_bytes, at.stream));
+}
+
+/* The coefficients and the norm's eps of the Newton-Schulz steps. */
+struct NewtonSchulz {
+    int steps = 5;
+    float a = 3.4445f, b = -4.7750f, c = 2.0315f, eps = 1e-7f;
+};
+inline size_t orthogonalize_workspace(size_t count, size_t rows, size_t cols) {
+    return vhip_orthogonalize_workspace(count, rows, cols);
+}
+/* `count` matrices of m.rows x m.dim, m.rows * m.ld elements apart; out likewise. */
+inline void orthogonalize(const Place &at, DType type, size_t count, const Rows &m, const NewtonSchulz &ns,
+                          const MutableRows &out) {
+    detail::check(vhip_orthogonalize(at.ordinal, (int)type, m.data, count, m.rows, m.dim, m.ld, m.rows * m.ld, ns.steps, ns.a,
+                                     ns.b, ns.c, ns.eps, out.data, out.ld, m.rows * out.ld, at.workspace, at.workspace_bytes,
+                                     at.stream));
+}
+
+}  // namespace training
 
 }  // namespace vector_hip
 

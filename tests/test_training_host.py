@@ -92,12 +92,34 @@ def test_empty_sizes(lib):
 
 
 def test_arrays_on_the_host_are_refused():
-    torch = pytest.importorskip("torch")
+    import numpy as np
+
     import vector_hip as vh
     from vector_hip import training
 
-    x, y = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
-    for call in (lambda: training.layer_norm(x), lambda: training.orthogonalize(x), lambda: training.softmax_xent(x, x, y),
-                 lambda: training.layer_norm_backward(x, x, None, y, y), lambda: training.layer_norm([1.0])):
-        with pytest.raises(vh.InvalidConfig):
-            call()
+    class Host(np.ndarray):
+        is_cuda = False
+
+    for x in (np.zeros((4, 8), np.float32), np.zeros((4, 8), np.float32).view(Host), [1.0], None):
+        for call in (lambda: training.layer_norm(x), lambda: training.orthogonalize(x), lambda: training.softmax_xent(x, x, x),
+                     lambda: training.softmax_xent_grad(x, x, x), lambda: training.layer_norm_backward(x, x, None, x, x)):
+            with pytest.raises(vh.InvalidConfig):
+                call()
+
+
+@pytest.mark.parametrize("order,refused", [("torch, vector_hip", False), ("vector_hip, torch", True)])
+def test_two_hip_runtimes_are_refused(order, refused):
+    """torch brings a HIP runtime of its own: loaded after the library's, it makes a second one."""
+    import os
+    import subprocess
+    import sys
+
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vector-rs_amd")
+    code = (f"import sys; sys.path.insert(0, {pkg!r})\nimport {order}\nfrom vector_hip import training\n"
+            "try:\n    training._one_runtime()\n    print('one')\n"
+            "except vector_hip.DriverError as e:\n    print('two', e)\n")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    if "No module named 'torch'" in out.stderr:
+        pytest.skip("torch is not installed")
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.startswith("two" if refused else "one"), out.stdout

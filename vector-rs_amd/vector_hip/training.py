@@ -11,13 +11,18 @@ are float32, float16 and bfloat16.  The last dimension is contiguous; rows may b
 
 A call enqueues its work on the current stream of its arguments' device and returns without waiting, as
 other operations on such arrays do.  Wrong arguments raise ``InvalidConfig``; there is no CPU fallback.
+
+Load torch before ``vector_hip``: torch brings a HIP runtime of its own, which this package's library then
+uses as well.  In the other order the process holds two, and a stream of the one means nothing to the other;
+calls raise ``DriverError`` then.
 """
 from __future__ import annotations
 
 import ctypes
+import os
 import sys
 
-from . import InvalidConfig, _check, _lib, _sig, _sz
+from . import DriverError, InvalidConfig, _check, _lib, _sig, _sz
 
 __all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize"]
 
@@ -51,11 +56,23 @@ class _Types(dict):
 _code = _Types()
 
 
+def _one_runtime():
+    """Raises where more than one HIP runtime is loaded into this process."""
+    try:
+        with open("/proc/self/maps") as maps:
+            loaded = {os.path.realpath(line.split()[-1]) for line in maps if "/libamdhip64.so" in line}
+    except OSError:
+        return
+    if len(loaded) > 1:
+        raise DriverError(f"two HIP runtimes are loaded ({', '.join(sorted(loaded))}): load torch before vector_hip")
+
+
 class _Library:
     """What calls need of the library that the caller's arrays come from: the types that they make outputs
     of, and the current stream of a device (by the quicker of the two ways where it has both)."""
 
     def __init__(self, lib):
+        _one_runtime()
         self.f32, self.u8, self.i64 = lib.float32, lib.uint8, lib.int64
         current = lib.cuda.current_stream
         self.stream = getattr(lib._C, "_cuda_getCurrentRawStream", lambda index: current(index).cuda_stream)

@@ -418,7 +418,7 @@ def test_orthogonalize_a_stack(tr, dtype):
         assert torch.equal(got[i], tr.orthogonalize(stack[i].contiguous()))
 
 
-@pytest.mark.parametrize("count,rows,cols", [(60, 130, 300), (60, 300, 130), (12, 400, 390), (1, 1500, 1600), (1, 1700, 1410)])
+@pytest.mark.parametrize("count,rows,cols", [(60, 130, 300), (60, 300, 130), (12, 400, 390), (1, 1500, 1600), (1, 1700, 1410), (1, 900, 2500), (1, 2304, 2200)])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("steps", [1, 2, 5])
 def test_orthogonalize_many_tiles(tr, count, rows, cols, dtype, steps):

@@ -349,8 +349,9 @@ __global__ __launch_bounds__(512) void k_ns_small(SmallArgs g) {
 
 template <class T>
 void ns_small_product(const SmallArgs &g, size_t count, hipStream_t s) {
+    // tiles reach to the next multiple of 64, where rows of pairs end: what is past M and N is stored as zeros
     auto grid = [&](int side) {
-        const uint32_t tm = ceil_div(g.M, side), tn = ceil_div(g.N, side);
+        const uint32_t tm = ceil_div(round_up(g.M, kMmK), side), tn = ceil_div(round_up(g.N, kMmK), side);
         return g.upper ? dim3(tm * (tm + 1) / 2, 1, (uint32_t)count) : dim3(tm, tn, (uint32_t)count);
     };
     const dim3 few = grid(32);
@@ -413,7 +414,9 @@ int multiply(const Pairs &a, int M, const Pairs &b, int N, int K, bool alo, bool
     g.ksplit = 1;
     g.batch = (int)count;
     g.upper = upper;
-    const bool big = mm_big_tiles(M, N, count, upper);
+    // 256 x 256 tiles read and store with the whole CU idle; a K loop of 64 stages makes up for it (one
+    // matrix of 4096 x 4096: 3.52 ms, 3.73 with 128 x 128; eight of 4096 x 1024: 1.96 and 1.75).
+    const bool big = K >= 2048 && mm_big_tiles(M, N, count, upper);
     return alo || blo ? mm_launch<half_t, kPairs, TA, TB>(g, big, epi, s) : mm_launch<half_t, kHigh, TA, TB>(g, big, epi, s);
 }
 
@@ -431,6 +434,10 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
     const bool tall = k.rows > k.cols, small = p.xt[0].p != nullptr;
     const int m = (int)(tall ? k.cols : k.rows), n = (int)(tall ? k.rows : k.cols);
     const uint32_t count = (uint32_t)k.count;
+    // symmetric products of few tiles: a workgroup a 32 or 64 tile, its waves sharing K (1 x 1024 x 4096: 691 us
+    // with 36 workgroups of 128 x 128 each, 513 so; at 78 tiles the two are even)
+    const size_t side = (size_t)ceil_div(m, 128);
+    const bool few = small || k.count * side * (side + 1) / 2 <= 48;
     const T *in = (const T *)k.in;
     constexpr int V = 16 / (int)sizeof(T);
     if (k.cols % V == 0 && k.ldi % V == 0 && (k.count == 1 || k.si % V == 0) && aligned16(in))
@@ -450,27 +457,36 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
         const bool low = !(last && !first && std::is_same_v<T, bf16_t>);
         const bool xlow = low && !(first && sizeof(T) == 2);
         const Pairs &x = p.x[i & 1], &xn = p.x[(i & 1) ^ 1], &xt = p.xt[i & 1], &xtn = p.xt[(i & 1) ^ 1];
+        SmallArgs ga{}, gb{};
+        ga.gain = p.gain;
+        ga.a = ga.b = x;
+        ga.M = ga.N = m;
+        ga.K = n;
+        ga.alo = ga.blo = xlow;
+        ga.upper = true;
+        ga.out = p.a;
+        ga.alpha = kAScale / (kXScale * kXScale);
+        ga.gains = first ? 2 : 0;
+        gb = ga;
+        gb.a = gb.b = gb.add = p.a;
+        gb.K = m;
+        gb.alo = gb.blo = low;
+        gb.out = p.b;
+        gb.alpha = k.c / kAScale;
+        gb.beta = k.b;
+        gb.diag = k.a * kAScale;
+        gb.gains = 0;
+        if (few) {
+            ns_small_product<T>(ga, k.count, s);
+            ns_small_product<T>(gb, k.count, s);
+            VH_CHECK(launch_status("orthogonalize launch"));
+        } else {
+            SymEpi ea{p.a, Pairs{}, gain, ga.alpha, 0.f, 0.f, m};
+            VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow, xlow, k.count, true, ea, s));
+            SymEpi eb{p.b, p.a, nullptr, gb.alpha, gb.beta, gb.diag, m};
+            VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low, low, k.count, true, eb, s));
+        }
         if (small) {
-            SmallArgs g{};
-            g.gain = p.gain;
-            g.a = g.b = x;
-            g.M = g.N = m;
-            g.K = n;
-            g.alo = g.blo = xlow;
-            g.upper = true;
-            g.out = p.a;
-            g.alpha = kAScale / (kXScale * kXScale);
-            g.gains = first ? 2 : 0;
-            ns_small_product<T>(g, count, s);
-            g.a = g.b = g.add = p.a;
-            g.K = m;
-            g.alo = g.blo = low;
-            g.out = p.b;
-            g.alpha = k.c / kAScale;
-            g.beta = k.b;
-            g.diag = k.a * kAScale;
-            g.gains = 0;
-            ns_small_product<T>(g, count, s);
             SmallArgs h{};
             h.gain = p.gain;
             h.a = xt;
@@ -490,14 +506,10 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
                 h.sr = k.so;
                 h.result_t = tall;
             }
-            ns_small_product<T>(h, count, s);
+            ns_small_product<T>(h, k.count, s);
             VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }
-        SymEpi ea{p.a, Pairs{}, gain, kAScale / (kXScale * kXScale), 0.f, 0.f, m};
-        VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow, xlow, k.count, true, ea, s));
-        SymEpi eb{p.b, p.a, nullptr, k.c / kAScale, k.b, k.a * kAScale, m};
-        VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low, low, k.count, true, eb, s));
         StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0, false};
         if (last) {
             es.alpha /= kXScale;

@@ -19,7 +19,9 @@
 // plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
 // operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) it is held
 // times 2^14 / 2^e, where 2^e is the power of two above the largest |G|, c scale (1 - p) at some row's target:
-// small probabilities keep their bits; the products' epilogues take the factor out again.
+// small probabilities keep their bits.  In either type G is also divided by the mantissa of c scale: with the
+// same c in every row, as a mean has it, G at a target far from learned is then a power of two, where rounding c
+// would have moved every such row's gradient by the same 2^-9.  The products' epilogues take the factors out.
 //
 // A row's sum of exps leaves its target out until it is joined: 1 - p at the target, and the loss
 // log(1 + sum of the others / the target's), keep their bits where p is nearly one.
@@ -51,6 +53,7 @@ inline bool stores_exps(int dtype, size_t dim) {
 struct Scalars {
     uint32_t amax_h, amax_w;  // bits of the largest finite |value|
     uint32_t gmax;            // bits of the largest |G|: weight x scale x (1 - p) at a row's target
+    float mantissa;           // of weight x scale, in [1, 2)
 };
 
 // 2^(14 - e) with 2^e > x >= 2^(e-1), so that x times it is in [2^13, 2^14); 1 for 0.
@@ -62,10 +65,36 @@ __device__ __forceinline__ float unit_scale(uint32_t bits) {
     return ldexpf(1.f, k);
 }
 
-__global__ __launch_bounds__(256) void k_xent_init(Scalars *s, uint32_t *marks, int n) {
+// What G is multiplied with; `ranged`: of a type with float16's range.
+__device__ __forceinline__ float grad_unit(const Scalars *s, bool ranged) {
+    return (ranged ? unit_scale(s->gmax) : 1.f) / s->mantissa;
+}
+
+// The call's scalars.  The mantissa is that of the largest weight among the first rows: one that most rows have
+// where it matters, and good for any others.
+__global__ __launch_bounds__(256) void k_xent_init(Scalars *s, const float *weight, int rows, float scale) {
+    __shared__ float top[4];
+    float m = weight ? 0.f : 1.f;
+    if (weight)
+        for (int t = threadIdx.x; t < min(rows, 4096); t += 256) {
+            const float w = fabsf(weight[t]);
+            if (w <= 3.4e38f && w > m) m = w;
+        }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    const float c = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fabsf(scale);
+    const uint32_t u = __builtin_bit_cast(uint32_t, c);
+    // 1 where c is zero, denormal or infinite
+    const bool plain = u >= 0x00800000u && u < 0x7f800000u;
+    *s = Scalars{0, 0, 0, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
+}
+
+__global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i == 0) *s = Scalars{0, 0, 0};
-    if (i < n) marks[i] = 0;
+    if (i < n) p[i] = 0;
 }
 
 // Largest finite |value| of h (blockIdx.y 0) and of the table (1).
@@ -435,7 +464,7 @@ struct GradEpi {
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = to_logits(acc, lg, m, table), unit = std::is_same_v<G, bf16_t> ? 1.f : unit_scale(lg.sc->gmax);
+        const float f = to_logits(acc, lg, m, table), unit = grad_unit(lg.sc, !std::is_same_v<G, bf16_t>);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
@@ -497,7 +526,7 @@ __global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *par
     constexpr int N = 16 / (int)sizeof(E);  // values of a lane
     const int t = blockIdx.x;
     const bool in = t < rows;
-    const float unit = std::is_same_v<E, half_t> ? 1.f : unit_scale(sc->gmax);
+    const float unit = grad_unit(sc, std::is_same_v<E, float>);
     const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
     const float c = fac.x * unit;
     const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
@@ -547,11 +576,11 @@ __global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *par
 // Factor that a gradient's product still has to be multiplied with.
 struct OutScale {
     const Scalars *sc;  // null: none
-    bool split;
+    bool ranged, split;
     bool of_table;  // the product with the rows (the table's gradient), else with the table
     __device__ __forceinline__ float operator()() const {
         if (!sc) return 1.f;
-        float f = 1.f / unit_scale(sc->gmax);
+        float f = 1.f / grad_unit(sc, ranged);
         if (split) f /= unit_scale(of_table ? sc->amax_h : sc->amax_w);
         return f;
     }
@@ -803,8 +832,8 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
-    constexpr bool kUnit = !std::is_same_v<P, bf16_t>;  // G is held in units of the largest weight
-    if (kSplit || (kUnit && z.grad)) k_xent_init<<<1, 256, 0, s>>>(p.sc, nullptr, 0);
+    constexpr bool kRanged = !std::is_same_v<P, bf16_t>;
+    if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
     if constexpr (kSplit) {
         const bool vec = dim % 4 == 0 && c.ldh % 4 == 0 && c.ldt % 4 == 0 && aligned16(c.h) && aligned16(c.table);
         const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2(vec ? z.dim / 4 : z.dim), vec};
@@ -844,7 +873,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const bool store = z.grad && stores_exps(z.dtype, z.dim);
         if (store) {
             const StatEpi<E, kSplit> se{lg, p.part, p.zt, target, (int)rows, table, (E *)p.g, z.vp, p.marks, ceil_div(table, z.stat_big ? 256 : 128)};
-            if (!kSplit) k_xent_init<<<(uint32_t)ceil_div(mark_count(z), 256), 256, 0, s>>>(p.sc, p.marks, (int)mark_count(z));
+            if (!kSplit) k_clear<<<(uint32_t)ceil_div(mark_count(z), 256), 256, 0, s>>>(p.marks, (int)mark_count(z));
             VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, se, s));
         } else {
             const StatEpi<void, kSplit> se{lg, p.part, p.zt, target, (int)rows, table, nullptr, 0, nullptr, 0};
@@ -885,7 +914,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.N = (int)rows;
             d.K = table;
             d.ksplit = z.ksplit;
-            const OutScale os{kUnit ? p.sc : nullptr, kSplit, false};
+            const OutScale os{p.sc, kRanged, kSplit, false};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
                          true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
@@ -908,7 +937,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.alo = d.blo = true;
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
-            OutEpi<T> oe{OutScale{kUnit ? p.sc : nullptr, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
+            OutEpi<T> oe{OutScale{p.sc, kRanged, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % (16 / sizeof(T)) == 0 && aligned16(c.dtable)};
             VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_big, oe, s));
         }

@@ -18,22 +18,25 @@
 namespace vh {
 namespace {
 
-// Elements of a lane's vector: 16 bytes of T where rows allow it, else one.
+// Values of a lane's vector: 16 bytes of T, at whatever alignment the rows have.  TAIL: the row ends inside one.
 template <class T>
-constexpr int full_vec() { return 16 / (int)sizeof(T); }
+constexpr int kVec = 16 / (int)sizeof(T);
 
-template <int N, class T>
-__device__ __forceinline__ void load_vec(float (&o)[N], const T *p) {
-    const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(p);
+template <int N, bool TAIL, class T>
+__device__ __forceinline__ void load_vec(float (&o)[N], const T *row, int c, int dim) {
+    const Pack<T, N> v = TAIL ? load_row<N>(row, c, dim) : load_any<N>(row + c);
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = (float)v.v[e];
 }
-template <int N, class T>
-__device__ __forceinline__ void store_vec(T *p, const float (&o)[N]) {
+template <int N, bool TAIL, class T>
+__device__ __forceinline__ void store_vec(T *row, int c, int dim, const float (&o)[N]) {
     Pack<T, N> v;
 #pragma unroll
     for (int e = 0; e < N; ++e) v.v[e] = (T)o[e];
-    *reinterpret_cast<Pack<T, N> *>(p) = v;
+    if (TAIL)
+        store_row<N>(row, c, dim, v);
+    else
+        store_any<N>(row + c, v);
 }
 
 // Sum of one (two) value(s) over the G lanes that hold a row: a wave by itself, or through LDS.  `slot`
@@ -63,9 +66,9 @@ struct FwdArgs {
     float eps;
 };
 
-template <class T, class P, int G, int VEC, int NV>
+template <class T, class P, int G, bool TAIL, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
-    constexpr int B = G > 256 ? G : 256, R = B / G;
+    constexpr int B = G > 256 ? G : 256, R = B / G, VEC = kVec<T>;
     __shared__ float lds[2 * (G / 64)];
     const size_t row = (size_t)blockIdx.x * R + threadIdx.x / G;
     if (row >= a.rows) return;  // G lanes at once: whole waves, and G > 64 has one row a workgroup
@@ -78,7 +81,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
     for (int i = 0; i < NV; ++i) {
         const int c = (i * G + t) * VEC;
         if (c < a.dim) {
-            load_vec<VEC>(v[i], x + c);
+            load_vec<VEC, TAIL>(v[i], x, c, a.dim);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s += v[i][e];
         }
@@ -88,10 +91,11 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if ((i * G + t) * VEC < a.dim) {
+        const int c = (i * G + t) * VEC;
+        if (c < a.dim) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                v[i][e] -= mu;
+                v[i][e] = TAIL && c + e >= a.dim ? 0.f : v[i][e] - mu;
                 s = fmaf(v[i][e], v[i][e], s);
             }
         }
@@ -106,16 +110,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[i][e] *= r;
             if (w) {
-                load_vec<VEC>(p, w + c);
+                load_vec<VEC, TAIL>(p, w, c, a.dim);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] *= p[e];
             }
             if (b) {
-                load_vec<VEC>(p, b + c);
+                load_vec<VEC, TAIL>(p, b, c, a.dim);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] += p[e];
             }
-            store_vec<VEC>(y + c, v[i]);
+            store_vec<VEC, TAIL>(y, c, a.dim, v[i]);
         }
     }
     if (t == 0) {
@@ -163,9 +167,9 @@ struct BwdArgs {
     int dim, parts;
 };
 
-template <class T, class P, int G, int VEC, int NV>
+template <class T, class P, int G, bool TAIL, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_backward(BwdArgs a) {
-    constexpr int B = G > 256 ? G : 256, R = B / G;
+    constexpr int B = G > 256 ? G : 256, R = B / G, VEC = kVec<T>;
     __shared__ float lds[4 * (G / 64)];
     const int t = threadIdx.x % G, sub = threadIdx.x / G;
     const P *w = (const P *)a.weight;
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_backward(BwdArgs a) {
         const int c = (i * G + t) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) g[i][e] = 1.f, dg[i][e] = 0.f, db[i][e] = 0.f;
-        if (w && c < a.dim) load_vec<VEC>(g[i], w + c);
+        if (w && c < a.dim) load_vec<VEC, TAIL>(g[i], w, c, a.dim);
     }
     int turn = 0;
     for (size_t row = (size_t)blockIdx.x * R + sub; row < a.rows; row += (size_t)gridDim.x * R, ++turn) {
@@ -188,8 +192,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_backward(BwdArgs a) {
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + t) * VEC;
             if (c < a.dim) {
-                load_vec<VEC>(xv[i], x + c);
-                load_vec<VEC>(d[i], dy + c);
+                load_vec<VEC, TAIL>(xv[i], x, c, a.dim);
+                load_vec<VEC, TAIL>(d[i], dy, c, a.dim);
             }
         }
 #pragma unroll
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_backward(BwdArgs a) {
             if (c < a.dim) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) d[i][e] = r * (d[i][e] - s1 - xv[i][e] * s2);
-                store_vec<VEC>(dx + c, d[i]);
+                store_vec<VEC, TAIL>(dx, c, a.dim, d[i]);
             }
         }
     }
@@ -245,7 +249,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_backward(BwdArgs a) {
             const int c = (i * G + t) * VEC;
             if (c < a.dim) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) pg[c + e] = dg[i][e], pb[c + e] = db[i][e];
+                for (int e = 0; e < VEC; ++e)
+                    if (!TAIL || c + e < a.dim) pg[c + e] = dg[i][e], pb[c + e] = db[i][e];
             }
         }
     } else {
@@ -368,26 +373,23 @@ inline Shape ln_shape(size_t dim, int vec) {
     return {0, 0};
 }
 
-#define LN_DISPATCH(KERNEL, T, P, VEC)                                       \
+#define LN_DISPATCH(KERNEL, T, P, TAIL)                                      \
     switch (sh.group * 8 + sh.nv) {                                          \
-        case 64 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 64, VEC, 1>), 64); break;   \
-        case 64 * 8 + 2: LN_LAUNCH((KERNEL<T, P, 64, VEC, 2>), 64); break;   \
-        case 64 * 8 + 3: LN_LAUNCH((KERNEL<T, P, 64, VEC, 3>), 64); break;   \
-        case 64 * 8 + 4: LN_LAUNCH((KERNEL<T, P, 64, VEC, 4>), 64); break;   \
-        case 256 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 256, VEC, 1>), 256); break; \
-        case 256 * 8 + 2: LN_LAUNCH((KERNEL<T, P, 256, VEC, 2>), 256); break; \
-        case 256 * 8 + 3: LN_LAUNCH((KERNEL<T, P, 256, VEC, 3>), 256); break; \
-        case 256 * 8 + 4: LN_LAUNCH((KERNEL<T, P, 256, VEC, 4>), 256); break; \
-        case 1024 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 1024, VEC, 1>), 1024); break; \
-        default: LN_LAUNCH((KERNEL<T, P, 1024, VEC, 2>), 1024); break;       \
+        case 64 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 64, TAIL, 1>), 64); break;   \
+        case 64 * 8 + 2: LN_LAUNCH((KERNEL<T, P, 64, TAIL, 2>), 64); break;   \
+        case 64 * 8 + 3: LN_LAUNCH((KERNEL<T, P, 64, TAIL, 3>), 64); break;   \
+        case 64 * 8 + 4: LN_LAUNCH((KERNEL<T, P, 64, TAIL, 4>), 64); break;   \
+        case 256 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 256, TAIL, 1>), 256); break; \
+        case 256 * 8 + 2: LN_LAUNCH((KERNEL<T, P, 256, TAIL, 2>), 256); break; \
+        case 256 * 8 + 3: LN_LAUNCH((KERNEL<T, P, 256, TAIL, 3>), 256); break; \
+        case 256 * 8 + 4: LN_LAUNCH((KERNEL<T, P, 256, TAIL, 4>), 256); break; \
+        case 1024 * 8 + 1: LN_LAUNCH((KERNEL<T, P, 1024, TAIL, 1>), 1024); break; \
+        default: LN_LAUNCH((KERNEL<T, P, 1024, TAIL, 2>), 1024); break;       \
     }
 
 template <class T, class P>
 int forward(const FwdArgs &a, hipStream_t s) {
-    constexpr int F = full_vec<T>();
-    const bool vec = a.dim % F == 0 && a.ldx % F == 0 && a.ldy % F == 0 && aligned16(a.x) && aligned16(a.y) &&
-                     aligned16(a.weight) && aligned16(a.bias);
-    const Shape sh = ln_shape(a.dim, vec ? F : 1);
+    const Shape sh = ln_shape(a.dim, kVec<T>);
     if (!sh.group) {
         if (a.rows > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows");
         k_ln_forward_long<T, P><<<(uint32_t)a.rows, 1024, 0, s>>>(a);
@@ -397,10 +399,10 @@ int forward(const FwdArgs &a, hipStream_t s) {
     const size_t grid = (a.rows + per - 1) / per;
     if (grid > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows");
 #define LN_LAUNCH(K, G) K<<<(uint32_t)grid, G > 256 ? G : 256, 0, s>>>(a)
-    if (vec) {
-        LN_DISPATCH(k_ln_forward, T, P, F)
+    if (a.dim % kVec<T>) {
+        LN_DISPATCH(k_ln_forward, T, P, true)
     } else {
-        LN_DISPATCH(k_ln_forward, T, P, 1)
+        LN_DISPATCH(k_ln_forward, T, P, false)
     }
 #undef LN_LAUNCH
     return launch_status("layer norm launch");
@@ -408,11 +410,8 @@ int forward(const FwdArgs &a, hipStream_t s) {
 
 template <class T, class P>
 int backward(BwdArgs a, P *dweight, P *dbias, float *ws, hipStream_t s) {
-    constexpr int F = full_vec<T>();
-    const bool vec = a.dim % F == 0 && a.lddy % F == 0 && a.ldx % F == 0 && (!a.dx || a.lddx % F == 0) &&
-                     aligned16(a.dy) && aligned16(a.x) && aligned16(a.weight) && aligned16(a.dx);
     const bool sums = dweight || dbias;
-    const Shape sh = ln_shape(a.dim, vec ? F : 1);
+    const Shape sh = ln_shape(a.dim, kVec<T>);
     a.part = sums ? ws : nullptr;
     if (a.rows == 0) {
         a.parts = 0;  // the sums of no rows
@@ -426,10 +425,10 @@ int backward(BwdArgs a, P *dweight, P *dbias, float *ws, hipStream_t s) {
     } else {
         a.parts = ln_parts(a.rows, sh.group == 64 ? 4 : 1);
 #define LN_LAUNCH(K, G) K<<<(uint32_t)a.parts, G > 256 ? G : 256, 0, s>>>(a)
-        if (vec) {
-            LN_DISPATCH(k_ln_backward, T, P, F)
+        if (a.dim % kVec<T>) {
+            LN_DISPATCH(k_ln_backward, T, P, true)
         } else {
-            LN_DISPATCH(k_ln_backward, T, P, 1)
+            LN_DISPATCH(k_ln_backward, T, P, false)
         }
 #undef LN_LAUNCH
     }

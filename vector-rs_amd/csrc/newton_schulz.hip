@@ -10,8 +10,9 @@
 // singular values stay below 2 for any useful coefficients, so neither leaves float16's range.
 // The first X is the matrix times the power of two that brings |M|_F to [2^12, 2^13); what is left of the
 // norm goes into the first step's epilogues, so 16-bit matrices are exact in the high halves and their
-// first products have no low ones to multiply.  Where the result is rounded to bfloat16 (2^-9), the last step
-// multiplies high halves alone: its rounding of 2^-12 is not amplified by any later step.
+// first products have no low ones to multiply.  Where the result is rounded to bfloat16 (2^-9), the last
+// step's B X multiplies high halves alone: no later step amplifies its 2^-12.  (Its A and A A do not: B is a
+// difference of terms several times its size.)
 // X's halves reach down to 2^-34: a matrix whose norm is below 2^-34 of eps comes out as zero.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.  a X is part
@@ -33,16 +34,17 @@ __device__ __forceinline__ void split(float x, half_t &hi, half_t &lo) {
 }
 
 // Partial sums of squares, in 64 bits: values of any magnitude neither overflow nor vanish.  2^lanes lanes a
-// row, V values each at a time.
-template <class T, int V>
+// row, 16 bytes each at a time.
+template <class T>
 __global__ __launch_bounds__(256) void k_ns_norm(const T *in, int rows, int cols, size_t ld, size_t stride, int lanes, double *part) {
+    constexpr int V = 16 / (int)sizeof(T);
     __shared__ double lds[4];
     const T *p = in + blockIdx.y * stride;
     const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
     double s = 0.0;
     for (int r = blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += kNormParts * per) {
         for (int c = l * V; c < cols; c += V << lanes) {
-            const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(p + (size_t)r * ld + c);
+            const Pack<T, V> v = load_row<V>(p + (size_t)r * ld, c, cols);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const double x = (double)(float)v.v[e];
@@ -191,7 +193,6 @@ struct StepEpi {
     int cols, rows;  // of what is stored
     T *out;          // null: not the last step
     size_t ldo, so;
-    bool vec;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int mw, int nw, const MmPlace &pl, char *lds) const {
         const float al = gain ? gain[pl.batch] * alpha : alpha;
@@ -212,14 +213,7 @@ struct StepEpi {
             lds, [&](int i, int j, int e) { return (T)(acc[i][j][e] * al); },
             [&](int r, int c, const Pack<T, PER> &v) {
                 if (nw + r >= rows || mw + c >= cols) return;
-                T *p = o + (size_t)(nw + r) * ldo + mw + c;
-                if (vec && mw + c + PER <= cols) {
-                    *reinterpret_cast<Pack<T, PER> *>(p) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < PER; ++e)
-                        if (mw + c + e < cols) p[e] = v.v[e];
-                }
+                store_row<PER>(o + (size_t)(nw + r) * ldo, mw + c, cols, v);
             });
     }
 };
@@ -439,11 +433,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
     const size_t side = (size_t)ceil_div(m, 128);
     const bool few = small || k.count * side * (side + 1) / 2 <= 48;
     const T *in = (const T *)k.in;
-    constexpr int V = 16 / (int)sizeof(T);
-    if (k.cols % V == 0 && k.ldi % V == 0 && (k.count == 1 || k.si % V == 0) && aligned16(in))
-        k_ns_norm<T, V><<<dim3(kNormParts, count), 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, lanes_log2(k.cols / V), p.norm);
-    else
-        k_ns_norm<T, 1><<<dim3(kNormParts, count), 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, lanes_log2(k.cols), p.norm);
+    k_ns_norm<T><<<dim3(kNormParts, count), 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, lanes_log2((k.cols * sizeof(T) + 15) / 16), p.norm);
     const dim3 tiles((uint32_t)ceil_div(k.rows, 64), (uint32_t)ceil_div(k.cols, 64), count);
     if (small)
         k_ns_start<T, true><<<tiles, 256, 0, s>>>(in, (int)k.rows, (int)k.cols, k.ldi, k.si, tall, p.norm, k.eps, p.x[0], p.xt[0], p.gain);
@@ -454,8 +444,8 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
         const bool first = i == 0, last = i + 1 == k.steps;
         const float *gain = first ? p.gain : nullptr;
         // which low halves count: X's are empty at first where the matrix has 16 bits
-        const bool low = !(last && !first && std::is_same_v<T, bf16_t>);
-        const bool xlow = low && !(first && sizeof(T) == 2);
+        const bool low = !(last && !first && std::is_same_v<T, bf16_t>);  // in B X
+        const bool xlow = !(first && sizeof(T) == 2);
         const Pairs &x = p.x[i & 1], &xn = p.x[(i & 1) ^ 1], &xt = p.xt[i & 1], &xtn = p.xt[(i & 1) ^ 1];
         SmallArgs ga{}, gb{};
         ga.gain = p.gain;
@@ -470,7 +460,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
         gb = ga;
         gb.a = gb.b = gb.add = p.a;
         gb.K = m;
-        gb.alo = gb.blo = low;
+        gb.alo = gb.blo = true;
         gb.out = p.b;
         gb.alpha = k.c / kAScale;
         gb.beta = k.b;
@@ -484,7 +474,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             SymEpi ea{p.a, Pairs{}, gain, ga.alpha, 0.f, 0.f, m};
             VH_CHECK((multiply<false, false>)(x, m, x, m, n, xlow, xlow, k.count, true, ea, s));
             SymEpi eb{p.b, p.a, nullptr, gb.alpha, gb.beta, gb.diag, m};
-            VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, low, low, k.count, true, eb, s));
+            VH_CHECK((multiply<false, false>)(p.a, m, p.a, m, m, true, true, k.count, true, eb, s));
         }
         if (small) {
             SmallArgs h{};
@@ -493,7 +483,7 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             h.b = p.b;
             h.M = n;
             h.N = h.K = m;
-            h.alo = xlow;
+            h.alo = low && xlow;
             h.blo = low;
             h.out = xn;
             h.out_t = xtn;
@@ -510,20 +500,19 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }
-        StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0, false};
+        StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0};
         if (last) {
             es.alpha /= kXScale;
             es.out = (T *)k.out;
             es.ldo = k.ldo;
             es.so = k.so;
-            es.vec = k.ldo % (16 / sizeof(T)) == 0 && (k.count == 1 || k.so % (16 / sizeof(T)) == 0) && aligned16(k.out);
         }
         if (last && tall) {
             es.cols = m;
             es.rows = n;
-            VH_CHECK((multiply<false, true>)(p.b, m, x, n, m, low, xlow, k.count, false, es, s));
+            VH_CHECK((multiply<false, true>)(p.b, m, x, n, m, low, low && xlow, k.count, false, es, s));
         } else {
-            VH_CHECK((multiply<true, false>)(x, n, p.b, m, m, xlow, low, k.count, false, es, s));
+            VH_CHECK((multiply<true, false>)(x, n, p.b, m, m, low && xlow, low, k.count, false, es, s));
         }
     }
     return VHIP_OK;

@@ -103,7 +103,6 @@ struct AmaxArgs {
     size_t rows[2], ld[2];
     uint32_t *out[2];
     int dim, lanes;  // lanes of a row, log2
-    bool vec;
 };
 __global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
     const int y = blockIdx.y, per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
@@ -114,14 +113,10 @@ __global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
     };
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes); r < a.rows[y]; r += (size_t)gridDim.x * per) {
         const float *x = a.x[y] + r * a.ld[y];
-        if (a.vec) {
-            for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
-                const floatx4_t v = *reinterpret_cast<const floatx4_t *>(x + c);
+        for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
+            const Pack<float, 4> v = load_row<4>(x, c, a.dim);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) see(v[e]);
-            }
-        } else {
-            for (int c = l; c < a.dim; c += 1 << a.lanes) see(x[c]);
+            for (int e = 0; e < 4; ++e) see(v.v[e]);
         }
     }
 #pragma unroll
@@ -152,8 +147,8 @@ struct Planes<float> {
 };
 
 // rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
-// row, 8 values each at a time, loaded E together (1: at any alignment).
-template <class T, int E>
+// row, 8 values each at a time.
+template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
                                               int kp, int lanes, const uint32_t *amax, const float *bias) {
     typedef typename Planes<T>::type P;
@@ -164,23 +159,17 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
         for (int c = l * 8; c < kp; c += 8 << lanes) {
-            alignas(16) T v[8];
-            if (E > 1 && keep && c + 8 <= dim) {
-#pragma unroll
-                for (int h = 0; h < 8 / E; ++h) *reinterpret_cast<Pack<T, E> *>(v + h * E) = *reinterpret_cast<const Pack<T, E> *>(x + r * ld + c + h * E);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = keep && c + e < dim ? x[r * ld + c + e] : (T)0.f;
-            }
+            Pack<T, 8> v{};
+            if (keep) v = load_row<8>(x + r * ld, c, dim);
             Pack<P, 8> hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if constexpr (N == 2) {
-                    const float f = v[e] * sc;
+                    const float f = v.v[e] * sc;
                     hi.v[e] = (half_t)f;
                     lo.v[e] = (half_t)(f - (float)hi.v[e]);
                 } else {
-                    hi.v[e] = v[e];
+                    hi.v[e] = v.v[e];
                 }
             }
             P *o = out + r * kp * N + (N == 2 ? pair_at(c) : c);
@@ -195,14 +184,7 @@ void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type 
     const int lanes = lanes_log2(kp / 8);
     const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
     const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
-    constexpr int E = 16 / (int)sizeof(T);
-    const uintptr_t at = (uintptr_t)x | ld * sizeof(T);
-    if (at % 16 == 0)
-        k_pack<T, E><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
-    else if (at % 8 == 0)
-        k_pack<T, E / 2><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
-    else
-        k_pack<T, 1><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
@@ -596,7 +578,7 @@ struct OutEpi {
     float *part;  // [part][rows][cols4], or null
     float *sum;   // [rows][cols4], or null
     int cols, rows, cols4;
-    bool first, last, vec;
+    bool first, last;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
         const float f = sc();
@@ -618,10 +600,10 @@ struct OutEpi {
                         *s = u;
                         return;
                     }
-                    O *o = out + (size_t)(n + r) * ld + m + c;
+                    Pack<O, 4> o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (m + c + e < cols) o[e] = (O)u.v[e];
+                    for (int e = 0; e < 4; ++e) o.v[e] = (O)u.v[e];
+                    store_row<4>(out + (size_t)(n + r) * ld, m + c, cols, o);
                 });
             return;
         }
@@ -630,14 +612,7 @@ struct OutEpi {
             lds, [&](int i, int j, int e) { return (O)(acc[i][j][e] * f); },
             [&](int r, int c, const Pack<O, PER> &v) {
                 if (n + r >= rows || m + c >= cols) return;
-                O *o = out + (size_t)(n + r) * ld + m + c;
-                if (vec && m + c + PER <= cols) {
-                    *reinterpret_cast<Pack<O, PER> *>(o) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < PER; ++e)
-                        if (m + c + e < cols) o[e] = v.v[e];
-                }
+                store_row<PER>(out + (size_t)(n + r) * ld, m + c, cols, v);
             });
     }
 };
@@ -703,7 +678,7 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.kp = round_up(dim, kMmK);
     z.vp = round_up(table, kMmK);
     z.cols4 = round_up(dim, 4);
-    z.small = rows <= (size_t)kSmallRows;
+    z.small = rows <= small_rows(dtype);
     if (z.small) {
         z.piece_rows = rows;
         const size_t groups = (table + 15) / 16, tiles = (table + kSmallEntries - 1) / kSmallEntries, ny = ceil_div(dim, kSmallCols);
@@ -809,9 +784,8 @@ int xent_small(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
                   (uint32_t)z.pieces, s);
     join_pieces(p, z, z.rows, c.target, c.row_weight, c.scale, c.loss, c.lse, s);
     if (z.grad) {
-        const bool vec = c.lddt % 4 == 0 && ((uintptr_t)c.dtable & (4 * sizeof(T) - 1)) == 0;
         small_grad<T>(SmallGrad{c.h, c.table, (const float *)c.bias, p.z, p.stat, p.rowfac, c.target, c.dtable, c.dh ? p.split : nullptr,
-                                c.ldh, c.ldt, c.lddt, z.vp, rows, table, dim, (int)z.cols4, vec},
+                                c.ldh, c.ldt, c.lddt, z.vp, rows, table, dim, (int)z.cols4},
                       (uint32_t)z.ksplit, s);
         if (c.dh) join_parts<T>(p.split, z.ksplit, rows, dim, (int)z.cols4, OutScale{}, (T *)c.dh, c.lddh, s);
     }
@@ -835,8 +809,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     constexpr bool kRanged = !std::is_same_v<P, bf16_t>;
     if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
     if constexpr (kSplit) {
-        const bool vec = dim % 4 == 0 && c.ldh % 4 == 0 && c.ldt % 4 == 0 && aligned16(c.h) && aligned16(c.table);
-        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2(vec ? z.dim / 4 : z.dim), vec};
+        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2((z.dim + 3) / 4)};
         k_amax<<<dim3(1024, 2), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
@@ -917,7 +890,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             const OutScale os{p.sc, kRanged, kSplit, false};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
-                         true, true, c.lddh % (16 / sizeof(T)) == 0 && aligned16(out)};
+                         true, true};
             VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_big, oe, s));
             if (z.ksplit > 1)
                 join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
@@ -938,7 +911,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
             OutEpi<T> oe{OutScale{p.sc, kRanged, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
-                         (int)z.cols4, r0 == 0, r0 + rows >= z.rows, c.lddt % (16 / sizeof(T)) == 0 && aligned16(c.dtable)};
+                         (int)z.cols4, r0 == 0, r0 + rows >= z.rows};
             VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_big, oe, s));
         }
         VH_CHECK(launch_status("gradient launch"));

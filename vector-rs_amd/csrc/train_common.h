@@ -19,6 +19,40 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T v[N];
 };
 
+// N values from or to memory that is aligned to one of them: one access all the same, as global memory takes
+// any alignment.
+template <int N, class T>
+__device__ __forceinline__ Pack<T, N> load_any(const T *p) {
+    Pack<T, N> v;
+    __builtin_memcpy(&v, p, sizeof v);
+    return v;
+}
+template <int N, class T>
+__device__ __forceinline__ void store_any(T *p, const Pack<T, N> &v) {
+    __builtin_memcpy(p, &v, sizeof v);
+}
+// The same of a row's values from column c on, of which those past dim are zeros, or left alone.
+template <int N, class T>
+__device__ __forceinline__ Pack<T, N> load_row(const T *row, int c, int dim) {
+    if (c + N <= dim) return load_any<N>(row + c);
+    asm volatile("" ::: "memory");  // or the compiler makes single loads of both branches
+    Pack<T, N> v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.v[e] = c + e < dim ? row[c + e] : (T)0.f;
+    return v;
+}
+template <int N, class T>
+__device__ __forceinline__ void store_row(T *row, int c, int dim, const Pack<T, N> &v) {
+    if (c + N <= dim) {
+        store_any<N>(row + c, v);
+    } else {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (c + e < dim) row[c + e] = v.v[e];
+    }
+}
+
 template <int W>
 __device__ __forceinline__ float lane_sum(float x) {
 #pragma unroll

@@ -1,4 +1,4 @@
-// xent_small.h -- softmax cross entropy of up to 64 rows (included by softmax_xent.hip).
+// xent_small.h -- softmax cross entropy of few rows (included by softmax_xent.hip).
 //
 // With few rows the table is what costs: the products of softmax_xent.hip would run tiles that are mostly
 // clamped rows, and 32-bit tables would first be turned into planes.  Here the table is read from memory
@@ -11,6 +11,8 @@
 //    and adds the rows' gradient up in registers; the workgroups' sums are joined afterwards.  G is not
 //    rounded here, and 16-bit operands are widened.
 #pragma once
+
+#include <type_traits>
 
 #include "mm16.h"
 
@@ -27,7 +29,8 @@ __device__ __forceinline__ float exp_fine(float x) {
     return t > -150.f && t < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
 }
 
-constexpr int kSmallRows = 64;
+// Rows of a call: 64, and 128 where the alternative would first turn a 32-bit table into pairs.
+inline size_t small_rows(int dtype) { return dtype == VHIP_DTYPE_F32 ? 128 : 64; }
 
 // Values of one lane in a K step of the logits.
 template <class T>
@@ -47,20 +50,11 @@ struct SmallStep<float> {
     }
 };
 
-// E values of a row from column c on, zeros past dim.
-template <class T, bool VEC>
+// E values of a row from column c on; TAIL: zeros past dim.
+template <class T, bool TAIL>
 __device__ __forceinline__ typename SmallStep<T>::vec small_load(const T *row, int c, int dim) {
-    typedef typename SmallStep<T>::vec vec;
-    vec v;
-    if constexpr (VEC) {
-        if (c < dim) return *reinterpret_cast<const vec *>(row + c);
-#pragma unroll
-        for (int e = 0; e < SmallStep<T>::E; ++e) v[e] = (T)0.f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < SmallStep<T>::E; ++e) v[e] = c + e < dim ? row[c + e] : (T)0.f;
-    }
-    return v;
+    constexpr int E = SmallStep<T>::E;
+    return __builtin_bit_cast(typename SmallStep<T>::vec, TAIL ? load_row<E>(row, c, dim) : load_any<E>(row + c));
 }
 
 struct SmallStat {
@@ -74,20 +68,26 @@ struct SmallStat {
     float scale;
 };
 
-template <class T, int NB, bool VEC>
+template <class T, int NB>
 __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
     typedef SmallStep<T> S;
+    constexpr int NJ = (NB + 3) / 4;  // blocks of 16 rows that a wave ends
     __shared__ floatx4_t s_acc[2][4][NB][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const T *hr[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) hr[j] = (const T *)a.h + (size_t)min(16 * j + i, a.rows - 1) * a.ldh;
-    const int steps = (a.dim + S::K - 1) / S::K;
-    // wave w ends rows 16 w .. 16 w + 15
-    const int t = 16 * wave + i;
-    const bool mine = wave < NB && t < a.rows;
-    const int64_t y = mine ? a.target[t] : -1;
-    float top = -INFINITY, sum = 0.f;
+    const int steps = a.dim / S::K;  // whole ones
+    // wave w ends the blocks w, w + 4 of the rows
+    int64_t y[NJ];
+    float top[NJ], sum[NJ];
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) {
+        const int j = wave + 4 * n, t = 16 * j + i;
+        y[n] = j < NB && t < a.rows ? a.target[t] : -1;
+        top[n] = -INFINITY;
+        sum[n] = 0.f;
+    }
     int buf = 0;
     const int groups = (a.table + 15) / 16;
     for (int g = blockIdx.x; g < groups; g += gridDim.x, buf ^= 1) {
@@ -98,46 +98,61 @@ __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
 #pragma unroll 4
         for (int s = wave; s < steps; s += 4) {
             const int c = s * S::K + q * S::E;
-            const typename S::vec x = small_load<T, VEC>(wr, c, a.dim);
+            const typename S::vec x = small_load<T, false>(wr, c, a.dim);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, VEC>(hr[j], c, a.dim), acc[j]);
+            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, false>(hr[j], c, a.dim), acc[j]);
+        }
+        if (steps * S::K < a.dim && wave == (steps & 3)) {
+            const int c = steps * S::K + q * S::E;
+            const typename S::vec x = small_load<T, true>(wr, c, a.dim);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, true>(hr[j], c, a.dim), acc[j]);
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) s_acc[buf][wave][j][lane] = acc[j];
         __syncthreads();  // the other buffer is written next: one barrier a group is enough
-        if (wave >= NB) continue;
-        const floatx4_t v = (s_acc[buf][0][wave][lane] + s_acc[buf][1][wave][lane]) +
-                            (s_acc[buf][2][wave][lane] + s_acc[buf][3][wave][lane]);
         const int e0 = 16 * g + 4 * q;
-        floatx4_t z;
-        float m = top;
+        float b[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float b = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
-            z[e] = b == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b);
-            m = fmaxf(m, z[e]);
-        }
-        const float about = m == -INFINITY ? 0.f : m;
-        sum *= exp_neg(top - about);
+        for (int e = 0; e < 4; ++e) b[e] = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += e0 + e == y ? 0.f : exp_neg(z[e] - about);
-        top = m;
-        if (mine) {
-            if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
+        for (int n = 0; n < NJ; ++n) {
+            const int j = wave + 4 * n, t = 16 * j + i;
+            if (j >= NB) break;
+            const floatx4_t v = (s_acc[buf][0][j][lane] + s_acc[buf][1][j][lane]) + (s_acc[buf][2][j][lane] + s_acc[buf][3][j][lane]);
+            floatx4_t z;
+            float m = top[n];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e0 + e == y && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
+            for (int e = 0; e < 4; ++e) {
+                z[e] = b[e] == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b[e]);
+                m = fmaxf(m, z[e]);
+            }
+            const float about = m == -INFINITY ? 0.f : m;
+            sum[n] *= exp_neg(top[n] - about);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[n] += e0 + e == y[n] ? 0.f : exp_neg(z[e] - about);
+            top[n] = m;
+            if (t < a.rows) {
+                if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e0 + e == y[n] && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
+            }
         }
     }
-    if (wave >= NB) return;
 #pragma unroll
-    for (int o = 16; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(sum, o, 64), m = fmaxf(top, m2);
-        const float about = m == -INFINITY ? 0.f : m;
-        sum = sum * exp_neg(top - about) + s2 * exp_neg(m2 - about);
-        top = m;
+    for (int n = 0; n < NJ; ++n) {
+        const int j = wave + 4 * n, t = 16 * j + i;
+        if (j >= NB) return;
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(top[n], o, 64), s2 = __shfl_xor(sum[n], o, 64), m = fmaxf(top[n], m2);
+            const float about = m == -INFINITY ? 0.f : m;
+            sum[n] = sum[n] * exp_neg(top[n] - about) + s2 * exp_neg(m2 - about);
+            top[n] = m;
+        }
+        if (t < a.rows && q == 0) a.part[(size_t)blockIdx.x * a.rows + t] = make_float2(top[n], sum[n]);
     }
-    if (mine && q == 0) a.part[(size_t)blockIdx.x * a.rows + t] = make_float2(top, sum);
 }
 
 struct SmallGrad {
@@ -149,20 +164,29 @@ struct SmallGrad {
     float *part;   // [gridDim.x][rows][cols4], null: the rows' gradient is not wanted
     size_t ldh, ldw, ldo, vp;
     int rows, table, dim, cols4;
-    bool vec;  // of dtable
 };
 
 constexpr int kSmallCols = 128;    // columns of a workgroup
 constexpr int kSmallEntries = 32;  // entries of a turn
 
 // Wave w: entries 16 (w & 1) .. of a turn, columns 64 (w >> 1) .. of the workgroup's.
-template <class T, int TB, bool VEC>
+template <class T, int TB, bool TAIL>  // TAIL: rows end inside four columns
 __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
     constexpr int R = 16 * TB, NV = kSmallEntries, GP = NV + 4, HP = kSmallCols + 4, NZ = R * NV / 256;
     __shared__ __align__(16) float s_g[R * GP], s_h[R * HP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
     const int sub = 16 * (wave & 1), cw = 64 * (wave >> 1), d0 = blockIdx.y * kSmallCols;
 
+    // four columns of a row, zeros where it does not count
+    auto four = [&](float (&o)[4], const T *row, int col, bool on) {
+        Pack<T, 4> p{};
+        if (TAIL)
+            p = load_row<4>(row, col, a.dim);
+        else if (col < a.dim)
+            p = load_any<4>(row + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = on ? (float)p.v[e] : 0.f;
+    };
     // this thread's logits of a turn: rows tz + 8 k, entry vz
     const int tz = tid / NV, vz = tid % NV;
     float zr[NZ], wr[4][4];
@@ -178,16 +202,7 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
         for (int k = 0; k < 4; ++k) {
             const int v = v0 + sub + 4 * q + k;
             const bool on = v < a.table && !(a.bias && a.bias[v] == -INFINITY);
-            const T *w = (const T *)a.w + (size_t)(on ? v : 0) * a.ldw + col;
-            if (VEC) {
-                Pack<T, 4> p{};
-                if (on && col < a.dim) p = *reinterpret_cast<const Pack<T, 4> *>(w);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wr[k][e] = (float)p.v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wr[k][e] = on && col + e < a.dim ? (float)w[e] : 0.f;
-            }
+            four(wr[k], (const T *)a.w + (size_t)(on ? v : 0) * a.ldw, col, on);
         }
     };
     fetch(blockIdx.x * NV);
@@ -212,17 +227,8 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
 #pragma unroll
     for (int k = 0; k < NH; ++k) {
         const int t = tid / HV + 256 / HV * k, col = d0 + tid % HV * 4;
-        const T *h = (const T *)a.h + (size_t)min(t, a.rows - 1) * a.ldh + col;
-        const bool on = t < a.rows && a.target[min(t, a.rows - 1)] >= 0;
-        if (VEC) {
-            Pack<T, 4> p{};
-            if (col < a.dim) p = *reinterpret_cast<const Pack<T, 4> *>(h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hr[k][e] = on ? (float)p.v[e] : 0.f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hr[k][e] = on && col + e < a.dim ? (float)h[e] : 0.f;
-        }
+        const int in = min(t, a.rows - 1);
+        four(hr[k], (const T *)a.h + (size_t)in * a.ldh, col, t < a.rows && a.target[in] >= 0);
     }
 #pragma unroll
     for (int k = 0; k < NH; ++k)
@@ -275,16 +281,13 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int col = d0 + cw + 16 * q + 4 * x;
-            if (a.vec && col + 4 <= a.dim) {
-                Pack<T, 4> p;
+            Pack<T, 4> p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p.v[e] = (T)dw[e][x];
-                *reinterpret_cast<Pack<T, 4> *>(o + col) = p;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < a.dim) o[col + e] = (T)dw[e][x];
-            }
+            for (int e = 0; e < 4; ++e) p.v[e] = (T)dw[e][x];
+            if (TAIL)
+                store_row<4>(o, col, a.dim, p);
+            else if (col < a.dim)
+                store_any<4>(o + col, p);
         }
     }
     if (!a.part) return;
@@ -312,29 +315,21 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
 
 template <class T>
 void small_stat(const SmallStat &a, uint32_t grid, hipStream_t s) {
-    constexpr int E = SmallStep<T>::E;
-    const bool vec = a.dim % E == 0 && a.ldh % E == 0 && a.ldw % E == 0 && aligned16(a.h) && aligned16(a.w);
-#define SMALL_STAT(NB)                                             \
-    if (vec)                                                       \
-        k_small_stat<T, NB, true><<<grid, 256, 0, s>>>(a);         \
-    else                                                           \
-        k_small_stat<T, NB, false><<<grid, 256, 0, s>>>(a);
-    if (a.rows <= 16) {
-        SMALL_STAT(1)
-    } else if (a.rows <= 32) {
-        SMALL_STAT(2)
-    } else {
-        SMALL_STAT(4)
-    }
-#undef SMALL_STAT
+    if (a.rows <= 16)
+        k_small_stat<T, 1><<<grid, 256, 0, s>>>(a);
+    else if (a.rows <= 32)
+        k_small_stat<T, 2><<<grid, 256, 0, s>>>(a);
+    else if (a.rows <= 64)
+        k_small_stat<T, 4><<<grid, 256, 0, s>>>(a);
+    else if constexpr (std::is_same_v<T, float>)
+        k_small_stat<T, 8><<<grid, 256, 0, s>>>(a);
 }
 
 template <class T>
 void small_grad(const SmallGrad &a, uint32_t gx, hipStream_t s) {
     const dim3 grid(gx, (uint32_t)ceil_div(a.dim, kSmallCols));
-    const bool vec = a.dim % 4 == 0 && a.ldw % 4 == 0 && a.ldh % 4 == 0 && (((uintptr_t)a.w | (uintptr_t)a.h) & (4 * sizeof(T) - 1)) == 0;
 #define SMALL_GRAD(TB)                                             \
-    if (vec)                                                       \
+    if (a.dim % 4)                                                 \
         k_small_grad<T, TB, true><<<grid, 256, 0, s>>>(a);         \
     else                                                           \
         k_small_grad<T, TB, false><<<grid, 256, 0, s>>>(a);
@@ -342,8 +337,10 @@ void small_grad(const SmallGrad &a, uint32_t gx, hipStream_t s) {
         SMALL_GRAD(1)
     } else if (a.rows <= 32) {
         SMALL_GRAD(2)
-    } else {
+    } else if (a.rows <= 64) {
         SMALL_GRAD(4)
+    } else if constexpr (std::is_same_v<T, float>) {
+        SMALL_GRAD(8)
     }
 #undef SMALL_GRAD
 }

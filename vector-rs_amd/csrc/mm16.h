@@ -18,8 +18,9 @@
 //    the 16 rows of a fragment read spread over all banks;
 //  * across: a row of k is BM / 8 slots, chunk s ^ 2 f(k), f from the bits of k that differ between the 16
 //    rows of a read (two 4 x 16 blocks of the transposing LDS read make a lane's 8 values of k).
-// Measured on 8192^3 in bfloat16: 256 x 256 tiles of 8 waves 1,222 TFLOP/s, 128 x 128 of 4 waves 831, the
-// library's product 1,326.
+// Measured on 8192^3 in bfloat16: 256 x 256 tiles of 8 waves 1,260 TFLOP/s (1,120 to 1,280 with operands across),
+// 128 x 128 of 4 waves 1,040, the library's product 1,326.  The matrix units are busy 64% of the time (131072 x
+// 2048 x 4096); the rest is the barrier of each stage, where every wave issues its DMAs.
 #pragma once
 
 #include "train_common.h"
@@ -364,7 +365,9 @@ int mm_launch_tile(MmArgs g, const Epi &epi, hipStream_t s) {
 }
 
 // Whether 256 x 256 tiles (8 waves, one workgroup a CU) beat 128 x 128 ones (4 waves, two a CU): whole rounds
-// of workgroups times a tile's work at the rates above.
+// of workgroups times a tile's work; small tiles are given 1.4 times the time, which also stands for their
+// reading each operand twice as often (4096 x 131072 x 1024: loss 955 us with large tiles, 1230 with small;
+// 100 x 10000 x 128 with gradients: 65 and 46).
 inline bool mm_big_tiles(size_t M, size_t N, size_t batch, bool upper = false) {
     auto tiles = [&](size_t b) {
         const size_t m = (M + b - 1) / b, n = (N + b - 1) / b;

@@ -355,10 +355,12 @@ void ns_small_product(const SmallArgs &g, size_t count, hipStream_t s) {
         k_ns_small<T, 4><<<grid(64), 512, 0, s>>>(g);
 }
 
-// Where 64 x 64 tiles of the products between all matrices are at most two rounds of workgroups.
+// Where the 64 x 64 tiles of all matrices are at most one round of workgroups.  Tiles of mm16.h / this way in us,
+// 32 bits: 1 x 300 x 768 (60 tiles) 154 / 126, 1 x 1024 x 1024 (256) 369 / 328, 4 x 512 x 512 (256) 238 / 228,
+// 2 x 768 x 768 (288) 305 / 352, 8 x 256 x 1024 (512) 223 / 256.
 inline bool ns_small(size_t count, size_t m, size_t n) {
     const size_t tm = (m + 63) / 64, tn = (n + 63) / 64;
-    return count * tm * tn <= 512;
+    return count * tm * tn <= 256;
 }
 
 struct NsParts {

@@ -41,10 +41,11 @@ namespace {
 
 constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G
 constexpr int kGBits = 14;
-// Columns from which G is made of stored exps.  A product's way costs 2 (pairs: 6) dim flops a value at 1.2
-// PFLOP/s, the walk's 4 (8) bytes at 4.5 TB/s and a few operations.  float16 always takes the product: its G
-// would be rounded twice to the 11 bits that the gradients have.
-constexpr size_t kStoreDim16 = 512, kStoreDim32 = 384;
+// Columns from which G is made of stored exps.  A product's way costs 2 (pairs: 6) dim flops a value, the walk's 4
+// (8) bytes and a few operations.  4096 rows x 65536, product / walk in us: bfloat16 dim 384 1097 / 1125, 512
+// 1207 / 1203, 768 1621 / 1514, 1024 2013 / 1787; 32 bits dim 256 1988 / 1784, 512 3128 / 2660, 1024 5517 / 4460.
+// float16 always takes the product: its G would be rounded twice to the 11 bits that the gradients have.
+constexpr size_t kStoreDim16 = 512, kStoreDim32 = 256;
 inline bool stores_exps(int dtype, size_t dim) {
     return dtype == VHIP_DTYPE_F32 ? dim >= kStoreDim32 : (dtype == VHIP_DTYPE_BF16 && dim >= kStoreDim16);
 }
@@ -678,7 +679,7 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.kp = round_up(dim, kMmK);
     z.vp = round_up(table, kMmK);
     z.cols4 = round_up(dim, 4);
-    z.small = rows <= small_rows(dtype);
+    z.small = few_rows(dtype, rows, table, dim);
     if (z.small) {
         z.piece_rows = rows;
         const size_t groups = (table + 15) / 16, tiles = (table + kSmallEntries - 1) / kSmallEntries, ny = ceil_div(dim, kSmallCols);

@@ -12,8 +12,6 @@
 //    rounded here, and 16-bit operands are widened.
 #pragma once
 
-#include <type_traits>
-
 #include "mm16.h"
 
 namespace vh {
@@ -29,8 +27,15 @@ __device__ __forceinline__ float exp_fine(float x) {
     return t > -150.f && t < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
 }
 
-// Rows of a call: 64, and 128 where the alternative would first turn a 32-bit table into pairs.
-inline size_t small_rows(int dtype) { return dtype == VHIP_DTYPE_F32 ? 128 : 64; }
+// Whether a call takes this way.  32-bit rows, tiles / this way in us, loss and with gradients: 16 x 10000 x 128
+// 37, 82 / 15, 27; 64 x 10000 x 768 61, 111 / 30, 82; 64 x 200003 x 300 256, 538 / 124, 451; 64 x 131072 x 1024
+// 469, 804 / 331, 815; 100 x 50000 x 512 93, 201 / 115, 350.  16-bit rows, whose tables the tiles read as they
+// are: 16 x 10000 x 128 16, 43 / 14, 25; 32 x 10000 x 768 19, 59 / 15, 54; 64 x 10000 x 768 19, 61 / 18, 72;
+// 16 x 131072 x 1024 53, 236 / 69, 288: only while launches are what counts.
+constexpr size_t kSmallRows = 64, kSmallWork16 = 250'000'000;
+inline bool few_rows(int dtype, size_t rows, size_t table, size_t dim) {
+    return rows <= kSmallRows && (dtype == VHIP_DTYPE_F32 || rows * table * dim <= kSmallWork16);
+}
 
 // Values of one lane in a K step of the logits.
 template <class T>
@@ -71,23 +76,17 @@ struct SmallStat {
 template <class T, int NB>
 __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
     typedef SmallStep<T> S;
-    constexpr int NJ = (NB + 3) / 4;  // blocks of 16 rows that a wave ends
     __shared__ floatx4_t s_acc[2][4][NB][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const T *hr[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) hr[j] = (const T *)a.h + (size_t)min(16 * j + i, a.rows - 1) * a.ldh;
     const int steps = a.dim / S::K;  // whole ones
-    // wave w ends the blocks w, w + 4 of the rows
-    int64_t y[NJ];
-    float top[NJ], sum[NJ];
-#pragma unroll
-    for (int n = 0; n < NJ; ++n) {
-        const int j = wave + 4 * n, t = 16 * j + i;
-        y[n] = j < NB && t < a.rows ? a.target[t] : -1;
-        top[n] = -INFINITY;
-        sum[n] = 0.f;
-    }
+    // wave w ends rows 16 w .. 16 w + 15
+    const int t = 16 * wave + i;
+    const bool mine = wave < NB && t < a.rows;
+    const int64_t y = mine ? a.target[t] : -1;
+    float top = -INFINITY, sum = 0.f;
     int buf = 0;
     const int groups = (a.table + 15) / 16;
     for (int g = blockIdx.x; g < groups; g += gridDim.x, buf ^= 1) {
@@ -111,48 +110,39 @@ __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) s_acc[buf][wave][j][lane] = acc[j];
         __syncthreads();  // the other buffer is written next: one barrier a group is enough
+        if (wave >= NB) continue;
+        const floatx4_t v = (s_acc[buf][0][wave][lane] + s_acc[buf][1][wave][lane]) +
+                            (s_acc[buf][2][wave][lane] + s_acc[buf][3][wave][lane]);
         const int e0 = 16 * g + 4 * q;
-        float b[4];
+        floatx4_t z;
+        float m = top;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+            const float b = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
+            z[e] = b == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b);
+            m = fmaxf(m, z[e]);
+        }
+        const float about = m == -INFINITY ? 0.f : m;
+        sum *= exp_neg(top - about);
 #pragma unroll
-        for (int n = 0; n < NJ; ++n) {
-            const int j = wave + 4 * n, t = 16 * j + i;
-            if (j >= NB) break;
-            const floatx4_t v = (s_acc[buf][0][j][lane] + s_acc[buf][1][j][lane]) + (s_acc[buf][2][j][lane] + s_acc[buf][3][j][lane]);
-            floatx4_t z;
-            float m = top[n];
+        for (int e = 0; e < 4; ++e) sum += e0 + e == y ? 0.f : exp_neg(z[e] - about);
+        top = m;
+        if (mine) {
+            if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                z[e] = b[e] == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b[e]);
-                m = fmaxf(m, z[e]);
-            }
-            const float about = m == -INFINITY ? 0.f : m;
-            sum[n] *= exp_neg(top[n] - about);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[n] += e0 + e == y[n] ? 0.f : exp_neg(z[e] - about);
-            top[n] = m;
-            if (t < a.rows) {
-                if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e0 + e == y[n] && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
-            }
+            for (int e = 0; e < 4; ++e)
+                if (e0 + e == y && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
         }
     }
+    if (wave >= NB) return;
 #pragma unroll
-    for (int n = 0; n < NJ; ++n) {
-        const int j = wave + 4 * n, t = 16 * j + i;
-        if (j >= NB) return;
-#pragma unroll
-        for (int o = 16; o < 64; o <<= 1) {
-            const float m2 = __shfl_xor(top[n], o, 64), s2 = __shfl_xor(sum[n], o, 64), m = fmaxf(top[n], m2);
-            const float about = m == -INFINITY ? 0.f : m;
-            sum[n] = sum[n] * exp_neg(top[n] - about) + s2 * exp_neg(m2 - about);
-            top[n] = m;
-        }
-        if (t < a.rows && q == 0) a.part[(size_t)blockIdx.x * a.rows + t] = make_float2(top[n], sum[n]);
+    for (int o = 16; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(sum, o, 64), m = fmaxf(top, m2);
+        const float about = m == -INFINITY ? 0.f : m;
+        sum = sum * exp_neg(top - about) + s2 * exp_neg(m2 - about);
+        top = m;
     }
+    if (mine && q == 0) a.part[(size_t)blockIdx.x * a.rows + t] = make_float2(top, sum);
 }
 
 struct SmallGrad {
@@ -319,10 +309,8 @@ void small_stat(const SmallStat &a, uint32_t grid, hipStream_t s) {
         k_small_stat<T, 1><<<grid, 256, 0, s>>>(a);
     else if (a.rows <= 32)
         k_small_stat<T, 2><<<grid, 256, 0, s>>>(a);
-    else if (a.rows <= 64)
+    else
         k_small_stat<T, 4><<<grid, 256, 0, s>>>(a);
-    else if constexpr (std::is_same_v<T, float>)
-        k_small_stat<T, 8><<<grid, 256, 0, s>>>(a);
 }
 
 template <class T>
@@ -337,10 +325,8 @@ void small_grad(const SmallGrad &a, uint32_t gx, hipStream_t s) {
         SMALL_GRAD(1)
     } else if (a.rows <= 32) {
         SMALL_GRAD(2)
-    } else if (a.rows <= 64) {
+    } else {
         SMALL_GRAD(4)
-    } else if constexpr (std::is_same_v<T, float>) {
-        SMALL_GRAD(8)
     }
 #undef SMALL_GRAD
 }

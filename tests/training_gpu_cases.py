@@ -344,6 +344,7 @@ def test_softmax_xent_in_pieces(tr, dtype, dim, monkeypatch):
     parts = tr.softmax_xent_grad(h, w, y, weight)
     xent_check(parts, h, w, y, 1.0, None, weight)
     within(parts[0], whole[0].double(), 2 * E * 128 * (1 + whole[0].double().abs()))
+    xent_check((*tr.softmax_xent(h, w, y), None, None), h, w, y, 1.0)
 
 
 def test_softmax_xent_values_that_differ_in_size_by_entry(tr):

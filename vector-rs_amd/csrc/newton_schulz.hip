@@ -73,6 +73,14 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
                                                   const double *part, float eps, Pairs x, Pairs xt, float *gain) {
     __shared__ float tile[64][65];
     __shared__ float s_inv;
+    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const T *p = in + blockIdx.z * stride;
+    float v[16];  // on their way while the norm is added up
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = r0 + ty + 4 * i, c = c0 + tx;
+        v[i] = r < rows && c < cols ? (float)p[(size_t)r * ld + c] : 0.f;
+    }
     if (threadIdx.x < 64) {
         double s = part[blockIdx.z * kNormParts + threadIdx.x];
 #pragma unroll
@@ -89,14 +97,8 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
     }
     __syncthreads();
     const float inv = s_inv;
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const T *p = in + blockIdx.z * stride;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = r0 + ty + 4 * i, c = c0 + tx;
-        const float v = r < rows && c < cols ? (float)p[(size_t)r * ld + c] * inv : 0.f;
-        tile[tall ? tx : ty + 4 * i][tall ? ty + 4 * i : tx] = v;
-    }
+    for (int i = 0; i < 16; ++i) tile[tall ? tx : ty + 4 * i][tall ? ty + 4 * i : tx] = v[i] * inv;
     __syncthreads();
     const int m0 = tall ? c0 : r0, n0 = tall ? r0 : c0, m = tall ? cols : rows, n = tall ? rows : cols;
     half_t *o = x.p + blockIdx.z * x.stride;

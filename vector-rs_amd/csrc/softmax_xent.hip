@@ -39,7 +39,7 @@
 namespace vh {
 namespace {
 
-constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G
+constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G, or of what the loss alone needs of its rows
 constexpr int kGBits = 14;
 // Columns from which G is made of stored exps.  A product's way costs 2 (pairs: 6) dim flops a value, the walk's 4
 // (8) bytes and a few operations.  4096 rows x 65536, product / walk in us: bfloat16 dim 384 1097 / 1125, 512
@@ -689,10 +689,11 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
         z.ksplit = (int)(tiles < gx ? tiles : gx);
         return z;
     }
-    const size_t per = z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2);
+    // what a row needs in G, or in pieces of its logits
+    const size_t per = grad ? z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2) : (table + 63) / 64 * sizeof(float2);
     size_t fit = piece_bytes() / per / 256 * 256;
     if (fit < 256) fit = 256;
-    z.piece_rows = !grad || rows <= fit ? rows : fit;
+    z.piece_rows = rows <= fit ? rows : fit;
     z.tp = round_up(z.piece_rows, kMmK);
     z.stat_big = mm_big_tiles(table, z.piece_rows, 1);
     z.pieces = ceil_div(table, z.stat_big ? 128 : 64);

@@ -222,7 +222,11 @@ __device__ __forceinline__ void rows_through_lds(char *w, const Value &value, co
     constexpr int BP = MB * 16 * (int)sizeof(O) <= 256 ? MB : 256 / 16 / (int)sizeof(O);  // blocks of a pass
     constexpr int PITCH = BP * 16 * (int)sizeof(O), NC = PITCH / 16;
     static_assert(NB * 16 * PITCH <= kEpiBytes && MB % BP == 0, "fits");
-    const int l = threadIdx.x & 63, q = l >> 4;
+    int l = threadIdx.x & 63;
+    // Large tiles have no registers left: the compiler would keep addresses in scratch from one call to the next
+    // (Newton-Schulz steps of 4096 x 4096: 3740 us, made anew 3450).
+    if constexpr (MB * NB > 16) asm volatile("" : "+v"(l));
+    const int q = l >> 4;
 #pragma unroll
     for (int p = 0; p < MB / BP; ++p) {
 #pragma unroll

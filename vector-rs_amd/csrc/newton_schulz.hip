@@ -157,9 +157,11 @@ struct SymEpi {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int c = nw + 16 * j + (l & 15);
+            int rq = mw + 4 * q;
+            if constexpr (MB * NB > 16) asm volatile("" : "+v"(rq));  // see rows_through_lds
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
-                const int r = mw + 16 * i + 4 * q;
+                const int r = rq + 16 * i;
                 floatx4_t v = acc[i][j] * al;
                 if (ad && c < m && (size_t)r < add.cols) {
                     const Pack<half_t, 4> h = *reinterpret_cast<const Pack<half_t, 4> *>(ad + (size_t)c * add.ld + pair_at(r));

@@ -347,6 +347,16 @@ def test_softmax_xent_in_pieces(tr, dtype, dim, monkeypatch):
     xent_check((*tr.softmax_xent(h, w, y), None, None), h, w, y, 1.0)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,table,dim", [(200, 70_001, 300), (150, 70_000, 137), (300, 45_000, 550), (300, 50_000, 384)])
+def test_softmax_xent_gradients_of_narrow_tables(tr, dtype, rows, table, dim, monkeypatch):
+    """Columns that fill tiles of 192 better than of 256, in one piece and in pieces of 256 rows."""
+    h, w, y = xent_inputs(rows, table, dim, dtype)
+    xent_check(tr.softmax_xent_grad(h, w, y), h, w, y, 1.0)
+    monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
+    xent_check(tr.softmax_xent_grad(h, w, y), h, w, y, 1.0)
+
+
 def test_softmax_xent_values_that_differ_in_size_by_entry(tr):
     """Logits of a row spread over hundreds: probabilities down to the smallest that 32 bits hold."""
     h, w, y = xent_inputs(100, 700, 512, "bf16")

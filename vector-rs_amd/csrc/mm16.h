@@ -120,7 +120,7 @@ struct MmTile {
     static constexpr int CH = BR / 8;               // chunks of a k row where stored across
     static constexpr int kBytes = BR * 128;
     static constexpr int KS = MODE == kPairs ? 32 : 64;  // k of a stage
-    static_assert(I * 8 * NW == BR, "whole DMAs");
+    static_assert(I * 8 * NW == BR && CH % 8 == 0, "whole DMAs, chunks by eights");
     typedef typename MmVec<T>::v4 v4;
     typedef typename MmVec<T>::v8 v8;
     uint32_t off[I];
@@ -131,7 +131,11 @@ struct MmTile {
 
     // byte of a row's chunk of 8 (high) values
     static __device__ __forceinline__ int chunk(int c) { return MODE == kPlain ? c * 16 : (c >> 2) * 128 + (c & 3) * 16; }
+    // A fragment's read takes 32 bytes of each of 16 rows of k: 0..3 and, further on, every eighth.  What is
+    // xored into their chunks puts them in other banks; rows of 384 bytes (24 chunks) alternate between halves
+    // of the banks by themselves, and a chunk has to stay within its 8.
     static __device__ __forceinline__ int swizzle(int k) {
+        if constexpr (CH % 16) return 2 * ((((k >> 1) & 1) << 1) | ((k >> 3) & 1));
         return 2 * ((k & 3) | (((k >> 3) & (CH >= 32 ? 3 : 1)) << 2));
     }
     // DMA i, across: its row of k, and the byte in that row.  In pairs the tile's rows from 32 on are low halves.
@@ -218,9 +222,12 @@ constexpr int kEpiBytes = 16384;
 // of 16 rows goes through LDS, so that rows leave in pieces of up to 256 bytes.
 template <class O, int MB, int NB, class Value, class Emit>
 __device__ __forceinline__ void rows_through_lds(char *w, const Value &value, const Emit &emit) {
-    constexpr int PER = 16 / (int)sizeof(O);                                   // values of a chunk
-    constexpr int BP = MB * 16 * (int)sizeof(O) <= 256 ? MB : 256 / 16 / (int)sizeof(O);  // blocks of a pass
-    constexpr int PITCH = BP * 16 * (int)sizeof(O), NC = PITCH / 16;
+    constexpr int PER = 16 / (int)sizeof(O);  // values of a chunk
+    constexpr int FIT = 16 / (int)sizeof(O);  // blocks in 256 bytes
+    constexpr int BP = MB <= FIT ? MB : MB % FIT == 0 ? FIT : FIT - 1;  // blocks of a pass
+    constexpr int NC = BP * (int)sizeof(O);                             // chunks of a row
+    constexpr int XOR = NC == 12 ? 15 : NC - 1, PITCH = (XOR + 1) * 16;
+    static_assert((NC & (NC - 1)) == 0 || NC == 12, "chunks");
     static_assert(NB * 16 * PITCH <= kEpiBytes && MB % BP == 0, "fits");
     int l = threadIdx.x & 63;
     // Large tiles have no registers left: the compiler would keep addresses in scratch from one call to the next
@@ -238,7 +245,7 @@ __device__ __forceinline__ void rows_through_lds(char *w, const Value &value, co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v.v[e] = value(p * BP + i, j, e);
                 const int at = (16 * i + 4 * q) * (int)sizeof(O);
-                *reinterpret_cast<Pack<O, 4> *>(w + n * PITCH + (((at >> 4) ^ (n & (NC - 1))) << 4) + (at & 15)) = v;
+                *reinterpret_cast<Pack<O, 4> *>(w + n * PITCH + (((at >> 4) ^ (n & XOR)) << 4) + (at & 15)) = v;
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -246,8 +253,8 @@ __device__ __forceinline__ void rows_through_lds(char *w, const Value &value, co
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
         for (int k = 0; k < NB * 16 * NC / 64; ++k) {
-            const int n = k * (64 / NC) + l / NC, c = l % NC;
-            emit(n, p * BP * 16 + c * PER, *reinterpret_cast<const Pack<O, PER> *>(w + n * PITCH + ((c ^ (n & (NC - 1))) << 4)));
+            const int n = NC == 12 ? (k * 64 + l) / NC : k * (64 / NC) + l / NC, c = NC == 12 ? (k * 64 + l) % NC : l % NC;
+            emit(n, p * BP * 16 + c * PER, *reinterpret_cast<const Pack<O, PER> *>(w + n * PITCH + ((c ^ (n & XOR)) << 4)));
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -263,8 +270,7 @@ __global__ __launch_bounds__(WM *WN * 64) void k_mm(MmArgs g, Epi epi) {
     typedef MmTile<T, MODE, TA, BM, NW> TileA;
     typedef MmTile<T, MODE, TB, BN, NW> TileB;
     typedef typename MmVec<T>::v8 v8;
-    static_assert(2 * BUF >= NW * kEpiBytes, "the epilogue's LDS");
-    __shared__ __align__(1024) char lds[2 * BUF];
+    __shared__ __align__(1024) char lds[2 * BUF >= NW * kEpiBytes ? 2 * BUF : NW * kEpiBytes];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -383,6 +389,25 @@ inline bool mm_big_tiles(size_t M, size_t N, size_t batch, bool upper = false) {
 template <class T, MmMode MODE, bool TA, bool TB, class Epi>
 int mm_launch(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
     return big ? mm_launch_tile<T, MODE, TA, TB, 2, 4, 8, 4>(g, epi, s) : mm_launch_tile<T, MODE, TA, TB, 2, 2, 4, 4>(g, epi, s);
+}
+
+// The same for a product whose M may be a few hundred: tiles of 192 x 256 (8 waves) where they hold at least a
+// ninth less padding (gradients of 1000 x 200003 x 300 in bfloat16: 873 us, 909 with 256 x 256).  A round of them counts as 33 against the 28 of small
+// ones (4096 x 30000 x 384: 505 us, 537 with small tiles; 2048 x 40000 x 300: 351 and 341).
+enum MmShape { k128x128, k256x256, k192x256 };
+
+inline bool mm_narrow(size_t M) { return (M + 191) / 192 * 192 * 9 <= (M + 255) / 256 * 256 * 8; }
+
+inline MmShape mm_shape(size_t M, size_t N, size_t batch) {
+    if (!mm_narrow(M)) return mm_big_tiles(M, N, batch) ? k256x256 : k128x128;
+    const size_t narrow = (M + 191) / 192 * ((N + 255) / 256) * batch, small = (M + 127) / 128 * ((N + 127) / 128) * batch;
+    return (narrow + 255) / 256 * 33 <= (small + 511) / 512 * 28 ? k192x256 : k128x128;
+}
+
+template <class T, MmMode MODE, bool TA, bool TB, class Epi>
+int mm_launch(const MmArgs &g, MmShape shape, const Epi &epi, hipStream_t s) {
+    if (shape == k192x256) return mm_launch_tile<T, MODE, TA, TB, 2, 4, 6, 4>(g, epi, s);
+    return mm_launch<T, MODE, TA, TB>(g, shape == k256x256, epi, s);
 }
 
 }  // namespace vh

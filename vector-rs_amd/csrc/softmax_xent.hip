@@ -656,7 +656,7 @@ struct Sizes {
     bool small;       // few rows: xent_small.h
     bool stat_big;
     int pieces;       // of a row's logits
-    bool dh_big, dw_big;
+    MmShape dh_tile, dw_tile;
     int ksplit;
 };
 
@@ -697,13 +697,14 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.tp = round_up(z.piece_rows, kMmK);
     z.stat_big = mm_big_tiles(table, z.piece_rows, 1);
     z.pieces = ceil_div(table, z.stat_big ? 128 : 64);
-    z.dh_big = dim > 128 && z.piece_rows > 128;
-    const size_t bs = z.dh_big ? 256 : 128, tiles = (size_t)ceil_div(dim, bs) * ceil_div(z.piece_rows, bs);
-    const size_t want = z.dh_big ? 256 : 512, ks = z.vp / kMmK;  // at least 8 stages a part
+    const bool large = dim > 128 && z.piece_rows > 128;
+    z.dh_tile = !large ? k128x128 : mm_narrow(dim) ? k192x256 : k256x256;
+    const size_t tiles = (size_t)ceil_div(dim, z.dh_tile == k192x256 ? 192 : large ? 256 : 128) * ceil_div(z.piece_rows, large ? 256 : 128);
+    const size_t want = large ? 256 : 512, ks = z.vp / kMmK;  // at least 8 stages a part
     size_t k = want / tiles;
     if (k > ks / 8) k = ks / 8;
     z.ksplit = (int)(k < 1 ? 1 : k);
-    z.dw_big = mm_big_tiles(dim, table, 1);
+    z.dw_tile = mm_shape(dim, table, 1);
     return z;
 }
 
@@ -893,7 +894,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
                          true, true};
-            VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_big, oe, s));
+            VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_tile, oe, s));
             if (z.ksplit > 1)
                 join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
         }
@@ -914,7 +915,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             const bool many = z.piece_rows < z.rows;
             OutEpi<T> oe{OutScale{p.sc, kRanged, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows};
-            VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_big, oe, s));
+            VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_tile, oe, s));
         }
         VH_CHECK(launch_status("gradient launch"));
     }

@@ -392,8 +392,9 @@ int mm_launch(const MmArgs &g, bool big, const Epi &epi, hipStream_t s) {
 }
 
 // The same for a product whose M may be a few hundred: tiles of 192 x 256 (8 waves) where they hold at least a
-// ninth less padding (gradients of 1000 x 200003 x 300 in bfloat16: 873 us, 909 with 256 x 256).  A round of them counts as 33 against the 28 of small
-// ones (4096 x 30000 x 384: 505 us, 537 with small tiles; 2048 x 40000 x 300: 351 and 341).
+// ninth less padding (gradients of 1000 x 200003 x 300 in bfloat16: 873 us, 909 with 256 x 256).  A round of
+// them counts as 33 against the 28 of small ones (4096 x 30000 x 384: 505 us, 537 with small tiles;
+// 2048 x 40000 x 300: 351 and 341).
 enum MmShape { k128x128, k256x256, k192x256 };
 
 inline bool mm_narrow(size_t M) { return (M + 191) / 192 * 192 * 9 <= (M + 255) / 256 * 256 * 8; }

@@ -682,7 +682,7 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     z.small = few_rows(dtype, rows, table, dim);
     if (z.small) {
         z.piece_rows = rows;
-        const size_t groups = (table + 15) / 16, tiles = (table + kSmallEntries - 1) / kSmallEntries, ny = ceil_div(dim, kSmallCols);
+        const size_t groups = ceil_div(table, small_turn(rows, table)), tiles = (table + kSmallEntries - 1) / kSmallEntries, ny = ceil_div(dim, kSmallCols);
         z.pieces = (int)(groups < 2048 ? groups : 2048);
         size_t gx = 1024 / ny;
         if (gx < 64) gx = 64;

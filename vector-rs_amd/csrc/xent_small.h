@@ -4,7 +4,7 @@
 // clamped rows, and 32-bit tables would first be turned into planes.  Here the table is read from memory
 // straight into matrix operands, twice in all for the gradients:
 //  * k_small_stat makes the logits, and keeps them where gradients follow (64 rows of them are less than a
-//    table of 64 columns).  A workgroup takes 16 entries at a time; its four waves share the K loop, so a CU
+//    table of 64 columns).  A workgroup takes 16 or 32 entries at a time; its four waves share the K loop, so a CU
 //    has enough loads in flight for short tables too.  32-bit operands are multiplied as they are, in the
 //    32-bit matrix instruction (157 TFLOP/s: above the memory's rate up to 48 rows).
 //  * k_small_grad turns 32 entries' logits into G in LDS, writes these entries' rows of the table's gradient
@@ -36,6 +36,12 @@ constexpr size_t kSmallRows = 64, kSmallWork16 = 250'000'000;
 inline bool few_rows(int dtype, size_t rows, size_t table, size_t dim) {
     return rows <= kSmallRows && (dtype == VHIP_DTYPE_F32 || rows * table * dim <= kSmallWork16);
 }
+
+// Entries of a workgroup's turn.  The rows are read from the caches again for each turn: from 17 rows on with
+// more of them than of the table, so a turn takes 32 entries, where enough turns for every CU are left
+// (float32, 16 / 32 entries, us: 32 x 95296 x 731 129, 97; 64 x 95296 x 768 194, 148; 32 x 40000 x 768 52, 39;
+// 64 x 20000 x 256 24, 20; 17 x 10000 x 768 19, 20).
+inline size_t small_turn(size_t rows, size_t table) { return rows > 16 && table >= 8192 ? 32 : 16; }
 
 // Values of one lane in a K step of the logits.
 template <class T>
@@ -73,10 +79,11 @@ struct SmallStat {
     float scale;
 };
 
-template <class T, int NB>
+template <class T, int NB, int GB>  // blocks of 16 rows, of 16 entries of a turn
 __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
     typedef SmallStep<T> S;
-    __shared__ floatx4_t s_acc[2][4][NB][64];
+    constexpr int BUFS = GB == 1 ? 2 : 1;
+    __shared__ floatx4_t s_acc[BUFS][4][NB][GB][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const T *hr[NB];
 #pragma unroll
@@ -88,50 +95,64 @@ __global__ __launch_bounds__(256) void k_small_stat(SmallStat a) {
     const int64_t y = mine ? a.target[t] : -1;
     float top = -INFINITY, sum = 0.f;
     int buf = 0;
-    const int groups = (a.table + 15) / 16;
-    for (int g = blockIdx.x; g < groups; g += gridDim.x, buf ^= 1) {
-        const T *wr = (const T *)a.w + (size_t)min(16 * g + i, a.table - 1) * a.ldw;
-        floatx4_t acc[NB];
+    const int groups = (a.table + 16 * GB - 1) / (16 * GB);
+    for (int g = blockIdx.x; g < groups; g += gridDim.x) {
+        const T *wr[GB];
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < GB; ++b) wr[b] = (const T *)a.w + (size_t)min(16 * (GB * g + b) + i, a.table - 1) * a.ldw;
+        floatx4_t acc[NB][GB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int b = 0; b < GB; ++b) acc[j][b] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+        auto step = [&](int c, auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
+            typename S::vec x[GB];
+#pragma unroll
+            for (int b = 0; b < GB; ++b) x[b] = small_load<T, TAIL>(wr[b], c, a.dim);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const typename S::vec y = small_load<T, TAIL>(hr[j], c, a.dim);
+#pragma unroll
+                for (int b = 0; b < GB; ++b) acc[j][b] = S::mfma(x[b], y, acc[j][b]);
+            }
+        };
 #pragma unroll 4
-        for (int s = wave; s < steps; s += 4) {
-            const int c = s * S::K + q * S::E;
-            const typename S::vec x = small_load<T, false>(wr, c, a.dim);
+        for (int s = wave; s < steps; s += 4) step(s * S::K + q * S::E, std::false_type());
+        if (steps * S::K < a.dim && wave == (steps & 3)) step(steps * S::K + q * S::E, std::true_type());
+        if (BUFS == 1) __syncthreads();  // the last turn's sums are read
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, false>(hr[j], c, a.dim), acc[j]);
-        }
-        if (steps * S::K < a.dim && wave == (steps & 3)) {
-            const int c = steps * S::K + q * S::E;
-            const typename S::vec x = small_load<T, true>(wr, c, a.dim);
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = S::mfma(x, small_load<T, true>(hr[j], c, a.dim), acc[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) s_acc[buf][wave][j][lane] = acc[j];
-        __syncthreads();  // the other buffer is written next: one barrier a group is enough
+            for (int b = 0; b < GB; ++b) s_acc[buf][wave][j][b][lane] = acc[j][b];
+        __syncthreads();  // with two buffers the other one is written next: one barrier a turn is enough
+        const int from = buf;
+        buf = (buf + 1) % BUFS;
         if (wave >= NB) continue;
-        const floatx4_t v = (s_acc[buf][0][wave][lane] + s_acc[buf][1][wave][lane]) +
-                            (s_acc[buf][2][wave][lane] + s_acc[buf][3][wave][lane]);
-        const int e0 = 16 * g + 4 * q;
-        floatx4_t z;
-        float m = top;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float b = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
-            z[e] = b == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, b);
-            m = fmaxf(m, z[e]);
-        }
-        const float about = m == -INFINITY ? 0.f : m;
-        sum *= exp_neg(top - about);
+        for (int b = 0; b < GB; ++b) {
+            const floatx4_t v = (s_acc[from][0][wave][b][lane] + s_acc[from][1][wave][b][lane]) +
+                                (s_acc[from][2][wave][b][lane] + s_acc[from][3][wave][b][lane]);
+            const int e0 = 16 * (GB * g + b) + 4 * q;
+            floatx4_t z;
+            float m = top;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += e0 + e == y ? 0.f : exp_neg(z[e] - about);
-        top = m;
-        if (mine) {
-            if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
+            for (int e = 0; e < 4; ++e) {
+                const float off = e0 + e < a.table ? (a.bias ? a.bias[e0 + e] : 0.f) : -INFINITY;
+                z[e] = off == -INFINITY ? -INFINITY : fmaf(v[e], a.scale, off);
+                m = fmaxf(m, z[e]);
+            }
+            const float about = m == -INFINITY ? 0.f : m;
+            sum *= exp_neg(top - about);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e0 + e == y && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
+            for (int e = 0; e < 4; ++e) sum += e0 + e == y ? 0.f : exp_neg(z[e] - about);
+            top = m;
+            if (mine) {
+                if (a.z) *reinterpret_cast<floatx4_t *>(a.z + (size_t)t * a.vp + e0) = z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e0 + e == y && e0 + e < a.table) a.zt[t] = make_float2(z[e], 0.f);
+            }
         }
     }
     if (wave >= NB) return;
@@ -305,12 +326,15 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
 
 template <class T>
 void small_stat(const SmallStat &a, uint32_t grid, hipStream_t s) {
+    const bool two = small_turn(a.rows, a.table) == 32;
     if (a.rows <= 16)
-        k_small_stat<T, 1><<<grid, 256, 0, s>>>(a);
+        k_small_stat<T, 1, 1><<<grid, 256, 0, s>>>(a);
     else if (a.rows <= 32)
-        k_small_stat<T, 2><<<grid, 256, 0, s>>>(a);
+        two ? k_small_stat<T, 2, 2><<<grid, 256, 0, s>>>(a) : k_small_stat<T, 2, 1><<<grid, 256, 0, s>>>(a);
+    else if (two && a.rows <= 48)
+        k_small_stat<T, 3, 2><<<grid, 256, 0, s>>>(a);
     else
-        k_small_stat<T, 4><<<grid, 256, 0, s>>>(a);
+        two ? k_small_stat<T, 4, 2><<<grid, 256, 0, s>>>(a) : k_small_stat<T, 4, 1><<<grid, 256, 0, s>>>(a);
 }
 
 template <class T>

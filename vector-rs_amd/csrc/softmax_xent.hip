@@ -98,12 +98,13 @@ __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// Largest finite |value| of h (blockIdx.y 0) and of the table (1).
+// Largest finite |value| of h (blockIdx.y 0) and of the table's entries that are not out (1).
 struct AmaxArgs {
     const float *x[2];
     size_t rows[2], ld[2];
     uint32_t *out[2];
-    int dim, lanes;  // lanes of a row, log2
+    const float *bias[2];  // null, or of the rows: -inf leaves one out
+    int dim, lanes;        // lanes of a row, log2
 };
 __global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
     const int y = blockIdx.y, per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
@@ -113,6 +114,7 @@ __global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
         if (u < 0x7f800000u && u > m) m = u;
     };
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes); r < a.rows[y]; r += (size_t)gridDim.x * per) {
+        if (a.bias[y] && a.bias[y][r] == -INFINITY) continue;
         const float *x = a.x[y] + r * a.ld[y];
         for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
             const Pack<float, 4> v = load_row<4>(x, c, a.dim);
@@ -812,7 +814,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     constexpr bool kRanged = !std::is_same_v<P, bf16_t>;
     if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
     if constexpr (kSplit) {
-        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, dim, lanes_log2((z.dim + 3) / 4)};
+        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, {nullptr, (const float *)c.bias}, dim, lanes_log2((z.dim + 3) / 4)};
         k_amax<<<dim3(1024, 2), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;

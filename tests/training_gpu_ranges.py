@@ -23,7 +23,7 @@ def same(got, want):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300)])
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300), (150, 640)])
 @pytest.mark.parametrize("value", [1e30, -1e6, 3e4, math.inf, math.nan])
 def test_values_of_entries_that_are_left_out(tr, dtype, rows, dim, value):
     """A bias of -inf: the call is what it is with zeros there, to the last bit."""
@@ -39,3 +39,41 @@ def test_values_of_entries_that_are_left_out(tr, dtype, rows, dim, value):
     w[out] = value
     same(tr.softmax_xent_grad(h, w, y, scale=2.0, bias=bias), want)
     same(tr.softmax_xent(h, w, y, scale=2.0, bias=bias), want_loss)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300), (150, 640)])
+@pytest.mark.parametrize("value", [1e30, -1e6, 3e4, math.inf, math.nan])
+def test_values_of_rows_without_a_target(tr, dtype, rows, dim, value):
+    """A negative target: everything but that row's lse is what it is with zeros there, to the last bit, and the
+    lse is that of the row's values."""
+    h, w, y = xent_inputs(rows, 700, dim, dtype)
+    y[2::7] = -1
+    rest = y >= 0
+    h[~rest] = 0.0
+    loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, scale=2.0)
+    xent_check((loss, lse, dh, dw), h, w, y, 2.0)
+    h[~rest] = value * (1 + 0.1 * normal(8, int((~rest).sum()), dim)).to(h.dtype)
+    loss2, lse2, dh2, dw2 = tr.softmax_xent_grad(h, w, y, scale=2.0)
+    same((loss2, lse2[rest], dh2, dw2), (loss, lse[rest], dh, dw))
+    if torch.isfinite(h).all() and abs(value) < 1e8:
+        hd, wd = h[~rest].double(), w.double()
+        z = hd @ wd.t() * 2.0
+        want = torch.logsumexp(z, 1)
+        # a logit's sum of dim products and its roundings (32-bit values to 2^-22 each), as in xent_check
+        zerr = ((dim + 24) * E * 2.0 * (hd.abs() @ wd.abs().t()) + 4 * E * z.abs()).max(1).values
+        within(lse2[~rest], want, zerr + 64 * E + 4 * E * want.abs())
+
+
+# ---- rows of sizes far apart ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300)])
+@pytest.mark.parametrize("power", [-60, 12, 20, 30])
+def test_one_row_far_larger_than_the_others(tr, rows, dim, power):
+    """In 32 bits each row's loss has the accuracy of its own values."""
+    h, w, y = xent_inputs(rows, 700, dim, "f32")
+    h[rows // 2] *= 2.0 ** power
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=2.0), h, w, y, 2.0)
+    xent_check((*tr.softmax_xent(h, w, y, scale=2.0), None, None), h, w, y, 2.0)
+    h *= 2.0 ** -100
+    xent_check((*tr.softmax_xent(h, w * 2.0 ** 100, y, scale=2.0), None, None), h, w * 2.0 ** 100, y, 2.0)

@@ -16,7 +16,8 @@
 //
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
-// plane cannot hold is 2^-39 of that value.  G is rounded to the operands' type (to two planes for 32-bit
+// plane cannot hold is 2^-39 of that value: for the logits a power for each row of h, and one for the entries
+// of the table that are not out; for the table's gradient one for the rows of h that have a target.  G is rounded to the operands' type (to two planes for 32-bit
 // operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) it is held
 // times 2^14 / 2^e, where 2^e is the power of two above the largest |G|, c scale (1 - p) at some row's target:
 // small probabilities keep their bits.  In either type G is also divided by the mantissa of c scale: with the
@@ -52,19 +53,19 @@ inline bool stores_exps(int dtype, size_t dim) {
 
 // State of a call on the device.
 struct Scalars {
-    uint32_t amax_h, amax_w;  // bits of the largest finite |value|
+    uint32_t amax_h, amax_w;  // bits of the largest finite |value| of rows with a target, of entries that are not out
     uint32_t gmax;            // bits of the largest |G|: weight x scale x (1 - p) at a row's target
     float mantissa;           // of weight x scale, in [1, 2)
 };
 
-// 2^(14 - e) with 2^e > x >= 2^(e-1), so that x times it is in [2^13, 2^14); 1 for 0.
-__device__ __forceinline__ float unit_scale(uint32_t bits) {
+// 14 - e with 2^e > x >= 2^(e-1), so that x times two to it is in [2^13, 2^14); 0 for 0.
+__device__ __forceinline__ int unit_power(uint32_t bits) {
     const int e = (int)(bits >> 23) - 126;  // x < 2^e
-    if (bits == 0) return 1.f;
-    int k = kGBits - e;
-    k = k > 120 ? 120 : (k < -120 ? -120 : k);
-    return ldexpf(1.f, k);
+    if (bits == 0) return 0;
+    const int k = kGBits - e;
+    return k > 120 ? 120 : (k < -120 ? -120 : k);
 }
+__device__ __forceinline__ float unit_scale(uint32_t bits) { return ldexpf(1.f, unit_power(bits)); }
 
 // What G is multiplied with; `ranged`: of a type with float16's range.
 __device__ __forceinline__ float grad_unit(const Scalars *s, bool ranged) {
@@ -98,29 +99,41 @@ __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// Largest finite |value| of h (blockIdx.y 0) and of the table's entries that are not out (1).
-struct AmaxArgs {
+// Largest finite |value| of h's rows that have a target (blockIdx.y 0), with the power of two of each row; and of
+// the table's entries that are not out (1).
+struct RangeArgs {
     const float *x[2];
     size_t rows[2], ld[2];
     uint32_t *out[2];
-    const float *bias[2];  // null, or of the rows: -inf leaves one out
-    int dim, lanes;        // lanes of a row, log2
+    const int64_t *target;
+    int *power;         // unit_power of each row of h
+    const float *bias;  // or null
+    int dim, lanes;     // lanes of a row, log2, 6 at most
 };
-__global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
+__global__ __launch_bounds__(256) void k_ranges(RangeArgs a) {
     const int y = blockIdx.y, per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
     uint32_t m = 0;
-    auto see = [&](float v) {
-        const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
-        if (u < 0x7f800000u && u > m) m = u;
-    };
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes); r < a.rows[y]; r += (size_t)gridDim.x * per) {
-        if (a.bias[y] && a.bias[y][r] == -INFINITY) continue;
+        if (y == 1 && a.bias && a.bias[r] == -INFINITY) continue;
         const float *x = a.x[y] + r * a.ld[y];
+        uint32_t own = 0;
         for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
             const Pack<float, 4> v = load_row<4>(x, c, a.dim);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) see(v.v[e]);
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t u = __builtin_bit_cast(uint32_t, v.v[e]) & 0x7fffffffu;
+                if (u < 0x7f800000u && u > own) own = u;
+            }
         }
+        if (y == 0) {
+            for (int o = 1; o < 1 << a.lanes; o <<= 1) {
+                const uint32_t v = __shfl_xor(own, o, 64);
+                own = v > own ? v : own;
+            }
+            if (l == 0) a.power[r] = unit_power(own);
+            if (a.target[r] < 0) continue;
+        }
+        m = own > m ? own : m;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -150,17 +163,20 @@ struct Planes<float> {
 };
 
 // rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
-// row, 8 values each at a time.
+// row, 8 values each at a time.  Pairs are scaled by two to `power` of the row, or by one scale where that is null.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              int kp, int lanes, const uint32_t *amax, const float *bias) {
+                                              int kp, int lanes, const uint32_t *amax, const int *power, const float *bias) {
     typedef typename Planes<T>::type P;
     constexpr int N = Planes<T>::count;
     const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
     float sc = 1.f;
-    if constexpr (N == 2) sc = unit_scale(*amax);
+    if constexpr (N == 2)
+        if (!power) sc = unit_scale(*amax);
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
+        if constexpr (N == 2)
+            if (power) sc = ldexpf(1.f, power[r]);
         for (int c = l * 8; c < kp; c += 8 << lanes) {
             Pack<T, 8> v{};
             if (keep) v = load_row<8>(x + r * ld, c, dim);
@@ -183,11 +199,11 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
 }
 template <class T>
 void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const uint32_t *amax,
-          const float *bias, hipStream_t s) {
+          const int *power, const float *bias, hipStream_t s) {
     const int lanes = lanes_log2(kp / 8);
     const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
     const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
-    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, bias);
+    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, power, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
@@ -227,15 +243,21 @@ __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim
     }
 }
 
-// What turns a product's sum into a logit.
+// What turns a product's sum into a logit.  SPLIT: of pairs.
+template <bool SPLIT>
 struct Logits {
     const float *bias;
     const Scalars *sc;
+    const int *power;  // of the rows
     float scale;
-    bool split;
-    __device__ __forceinline__ float factor() const {
-        return split ? scale / unit_scale(sc->amax_h) / unit_scale(sc->amax_w) : scale;
+    __device__ __forceinline__ float factor() const { return SPLIT ? scale / unit_scale(sc->amax_w) : scale; }
+    // the factor f of row t, if that is one
+    __device__ __forceinline__ float of_row(float f, int t, int rows) const {
+        if constexpr (SPLIT) return ldexpf(f, t < rows ? -power[t] : 0);
+        return f;
     }
+    // whether to_logits makes the wave's logits
+    __device__ __forceinline__ bool made(int last, int table) const { return bias || last > table; }
 };
 // Exps in (0, 1] as float16: times 2^15, or those below 2^-28 negative and times 2^43.
 __device__ __forceinline__ half_t exp_code(float p) { return (half_t)(p * (p < 0x1p-28f ? -0x1p43f : 0x1p15f)); }
@@ -243,13 +265,16 @@ __device__ __forceinline__ float exp_decode(half_t h) { return (float)h * (h < (
 // Arguments of exps that exp_code would cut short, and that are not nothing in 32 bits either.
 __device__ __forceinline__ bool exp_cut(float x) { return x < -39.f && x > -104.f; }
 
-// A wave's sums to f times them being the logits: where there is a bias, or entries past the table, the
-// logits themselves (-inf where an entry is out) and f = 1.
-template <int MB, int NB>
-__device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logits &lg, int m, int table) {
+// A wave's sums to f (of the row) times them being the logits: where there is a bias, or entries past the
+// table, the logits themselves (-inf where an entry is out) and f = 1 for every row.
+template <int MB, int NB, bool SPLIT>
+__device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logits<SPLIT> &lg, int m, int n, int rows, int table) {
     const float f = lg.factor();
-    if (!lg.bias && m + 16 * MB <= table) return f;
-    const int q = (threadIdx.x & 63) >> 4;
+    if (!lg.made(m + 16 * MB, table)) return f;
+    const int l = threadIdx.x & 63, q = l >> 4;
+    float fs[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) fs[j] = lg.of_row(f, n + 16 * j + (l & 15), rows);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         float b[4];
@@ -261,7 +286,7 @@ __device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logit
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = b[e] == -INFINITY ? -INFINITY : fmaf(acc[i][j][e], f, b[e]);
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = b[e] == -INFINITY ? -INFINITY : fmaf(acc[i][j][e], fs[j], b[e]);
     }
     return 1.f;
 }
@@ -270,14 +295,14 @@ __device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logit
 // E: the type that the exps are stored in, void: they are not; FINE: of 32-bit operands.
 template <class E, bool FINE>
 struct StatEpi {
-    Logits lg;
+    Logits<FINE> lg;
     float2 *part;  // [piece][rows]: largest logit, sum of exp about it without the target's
     float2 *zt;    // the target's logit less its piece's largest, and that
     const int64_t *target;
     int rows, table;
     E *exps;  // [rows][vp]
     size_t vp;
-    uint32_t *marks;  // [tile of N][tile of M]: exps that float16 cannot hold
+    uint32_t *marks;  // [tile of N][tile of M]: exps of rows with a target that float16 cannot hold
     int mt;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
@@ -285,9 +310,10 @@ struct StatEpi {
         bool cut = false;
         if (m >= table) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        float f = to_logits(acc, lg, m, table);
-        if (f < 0.f) {
-            f = -f;
+        const bool made = lg.made(m + 16 * MB, table);
+        float fw = to_logits(acc, lg, m, n, rows, table);
+        if (fw < 0.f) {
+            fw = -fw;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -298,6 +324,7 @@ struct StatEpi {
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
             const bool in = t < rows;
+            const float f = made ? 1.f : lg.of_row(fw, t, rows);
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
@@ -311,10 +338,11 @@ struct StatEpi {
             const int64_t y = in ? target[t] : -1;
             const int d = y >= m && y < m + 16 * MB && y < table ? (int)(y - m) - 4 * q : -1;
             float sum = 0.f;
+            bool wide = false;
             auto add = [&](float &v, bool skip) {
                 const float x = fmaf(v, f, -about);
                 const float p = FINE ? exp_fine(x) : exp_neg(x);
-                if constexpr (kHalf) cut |= exp_cut(x);
+                if constexpr (kHalf) wide |= exp_cut(x);
                 sum += skip ? 0.f : p;
                 if (skip) zt[t] = make_float2(x, about);
                 return p;
@@ -338,6 +366,7 @@ struct StatEpi {
                         if constexpr (!std::is_void_v<E>) acc[i][j][e] = v;
                     }
             }
+            if constexpr (kHalf) cut |= wide && y >= 0;
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
@@ -438,7 +467,7 @@ __global__ __launch_bounds__(256) void k_zero_rows(char *p, size_t rows, size_t 
 // Epilogue of the second product: G, SPLIT: in pairs.
 template <class G, bool SPLIT>
 struct GradEpi {
-    Logits lg;
+    Logits<SPLIT> lg;
     const float2 *stat;   // the row's largest logit, 1 / sum of exp about it
     const float2 *rowfac; // weight x scale, and times 1 - p at the target
     const int64_t *target;
@@ -449,11 +478,14 @@ struct GradEpi {
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float f = to_logits(acc, lg, m, table), unit = grad_unit(lg.sc, !std::is_same_v<G, bf16_t>);
+        const float unit = grad_unit(lg.sc, !std::is_same_v<G, bf16_t>);
+        const bool made = lg.made(m + 16 * MB, table);
+        const float fw = to_logits(acc, lg, m, n, rows, table);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int t = n + 16 * j + (l & 15);
             const bool in = t < rows;
+            const float f = made ? 1.f : lg.of_row(fw, t, rows);
             const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
             const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
             const float c = fac.x * unit, cs = c * st.y;
@@ -723,6 +755,7 @@ struct Parts {
     float *split, *sum;
     float *z;  // few rows: the logits
     uint32_t *marks;
+    int *power;  // 32 bits: of the rows of h (Logits)
     void *hp, *wp, *ht, *g;
 };
 
@@ -741,6 +774,7 @@ inline Parts carve(Carver &c, const Sizes &z) {
         }
         return p;
     }
+    if (planes == 2) p.power = c.take<int>(z.rows);
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
@@ -814,13 +848,15 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     constexpr bool kRanged = !std::is_same_v<P, bf16_t>;
     if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
     if constexpr (kSplit) {
-        const AmaxArgs m{{h, w}, {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w}, {nullptr, (const float *)c.bias}, dim, lanes_log2((z.dim + 3) / 4)};
-        k_amax<<<dim3(1024, 2), 256, 0, s>>>(m);
+        const int lanes = lanes_log2((z.dim + 3) / 4);
+        const RangeArgs m{{h, w},   {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w},
+                          c.target, p.power,           (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
+        k_ranges<<<dim3(1024, 2), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
     if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
-        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, &p.sc->amax_w, (const float *)c.bias, s);
+        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, &p.sc->amax_w, nullptr, (const float *)c.bias, s);
         wp = (const P *)p.wp;
         ldw = z.kp * Planes<T>::count;
     }
@@ -832,7 +868,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, &p.sc->amax_h, nullptr, s);
+            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, nullptr, p.power ? p.power + r0 : nullptr, nullptr, s);
             hp = (const P *)p.hp;
             ldh = z.kp * Planes<T>::count;
         }
@@ -846,7 +882,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.K = (int)z.kp;
         g.alo = g.blo = true;
         g.ksplit = g.batch = 1;
-        const Logits lg{(const float *)c.bias, p.sc, c.scale, kSplit};
+        const Logits<kSplit> lg{(const float *)c.bias, p.sc, p.power ? p.power + r0 : nullptr, c.scale};
         typedef std::conditional_t<kSplit, float, half_t> E;
         const bool store = z.grad && stores_exps(z.dtype, z.dim);
         if (store) {

@@ -77,3 +77,57 @@ def test_one_row_far_larger_than_the_others(tr, rows, dim, power):
     xent_check((*tr.softmax_xent(h, w, y, scale=2.0), None, None), h, w, y, 2.0)
     h *= 2.0 ** -100
     xent_check((*tr.softmax_xent(h, w * 2.0 ** 100, y, scale=2.0), None, None), h, w * 2.0 ** 100, y, 2.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300), (90, 640)])
+def test_row_weights_far_apart(tr, dtype, rows, dim, monkeypatch):
+    """Each row's gradient has the accuracy of its own weight: here over 2^26 (2^60 in 32 bits and bfloat16)."""
+    h, w, y = xent_inputs(rows, 500, dim, dtype)
+    h, w = h / 32, w * 32
+    low, high = (-16, 10) if dtype == "f16" else (-40, 20)
+    weight = torch.exp2(torch.linspace(low, high, rows, device="cuda"))[torch.randperm(rows, device="cuda", generator=base.gen(3))]
+    _, _, rdh, rdw, g, z, hd, wd = xent_reference(h, w, y, 1.0, None, weight)
+    t = h.dtype
+    # the relative error of p and of 1 - p: that of the logits and the sum; then G's rounding (two planes in 32
+    # bits), the sum's chain and the planes of the table.  What G's smallest step leaves out is below
+    # 2^-24 / 2^13 of the row's largest value a value of the row, in float16; a plane more in 32 bits.
+    per = (dim + 8 if t != torch.float32 else dim + 24) * E
+    zerr = (per * (hd.abs() @ wd.abs().t()) + 4 * E * z.abs()).max(1).values
+    unit = UNIT[t] if t != torch.float32 else 2.0 ** -22
+    rel = 4 * (zerr + 128 * E) + unit + (500 + 32) * E + 2.0 ** -22
+    least = 2.0 ** -37 * g.abs().max(1, keepdim=True).values * wd.abs().sum(0) if t != torch.bfloat16 else 0.0
+    aw = wd.abs()
+    tol = UNIT[t] * rdh.abs() + TINY[t] + rel[:, None] * (g.abs() @ aw) + least + 2.0 ** -38 * aw.max() * g.abs().sum(1, keepdim=True)
+    within(tr.softmax_xent_grad(h, w, y, weight)[2], rdh, tol)
+    xent_check(tr.softmax_xent_grad(h, w, y, weight), h, w, y, 1.0, None, weight)
+    monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
+    within(tr.softmax_xent_grad(h, w, y, weight)[2], rdh, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_row_weights_that_grow_from_piece_to_piece(tr, dtype, monkeypatch):
+    """Pieces of 256 rows whose weights differ by 2^12 from one to the next, and a last piece without any."""
+    h, w, y = xent_inputs(900, 500, 96, dtype)
+    weight = torch.exp2(12.0 * (torch.arange(900, device="cuda") // 256) - 24)
+    y[768:] = -1
+    monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
+    xent_check(tr.softmax_xent_grad(h, w, y, weight), h, w, y, 1.0, None, weight)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (90, 640)])
+def test_rows_of_zeros_and_rows_without_a_loss(tr, dtype, rows, dim):
+    """Rows of zeros, beside them rows whose loss is nothing, and rows of both sizes that have no weight."""
+    h, w, y = xent_inputs(rows, 500, dim, dtype)
+    weight = torch.rand(rows, device="cuda", generator=base.gen(9)) / rows
+    h[3::5] = 0.0
+    h[4::5] = 30 * w[y[4::5]]
+    weight[::9] = 0.0
+    xent_check(tr.softmax_xent_grad(h, w, y, weight, scale=2.0), h, w, y, 2.0, None, weight)
+    h[:] = 0.0
+    xent_check(tr.softmax_xent_grad(h, w, y, weight, scale=2.0), h, w, y, 2.0, None, weight)
+    h[:] = 30 * w[y]
+    got = tr.softmax_xent_grad(h, w, y, weight, scale=2.0)
+    xent_check(got, h, w, y, 2.0, None, weight)
+    assert not got[0].any() and not got[2].any() and not got[3].any()

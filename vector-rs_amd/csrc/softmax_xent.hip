@@ -17,10 +17,12 @@
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
 // plane cannot hold is 2^-39 of that value: for the logits a power for each row of h, and one for the entries
-// of the table that are not out; for the table's gradient one for the rows of h that have a target.  G is rounded to the operands' type (to two planes for 32-bit
-// operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) it is held
-// times 2^14 / 2^e, where 2^e is the power of two above the largest |G|, c scale (1 - p) at some row's target:
-// small probabilities keep their bits.  In either type G is also divided by the mantissa of c scale: with the
+// of the table that are not out.  G is rounded to the operands' type (to two planes for 32-bit
+// operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) each row
+// of G is held times 2^14 / 2^e, where 2^e is the power of two above its largest value, c scale (1 - p) at the
+// target: neither small probabilities nor rows of small weight lose their bits.  For the table's gradient the rows
+// of h take 2^e back, times the power of two that brings the largest of all 2^e h to [2^13, 2^14).
+// In any type G is also divided by the mantissa of c scale: with the
 // same c in every row, as a mean has it, G at a target far from learned is then a power of two, where rounding c
 // would have moved every such row's gradient by the same 2^-9.  The products' epilogues take the factors out.
 //
@@ -53,9 +55,9 @@ inline bool stores_exps(int dtype, size_t dim) {
 
 // State of a call on the device.
 struct Scalars {
-    uint32_t amax_h, amax_w;  // bits of the largest finite |value| of rows with a target, of entries that are not out
-    uint32_t gmax;            // bits of the largest |G|: weight x scale x (1 - p) at a row's target
-    float mantissa;           // of weight x scale, in [1, 2)
+    uint32_t amax_w;  // bits of the largest finite |value| of entries that are not out
+    int least;        // least sum of a row's power (k_ranges) and of its row_power
+    float mantissa;   // of weight x scale, in [1, 2)
 };
 
 // 14 - e with 2^e > x >= 2^(e-1), so that x times two to it is in [2^13, 2^14); 0 for 0.
@@ -67,10 +69,17 @@ __device__ __forceinline__ int unit_power(uint32_t bits) {
 }
 __device__ __forceinline__ float unit_scale(uint32_t bits) { return ldexpf(1.f, unit_power(bits)); }
 
-// What G is multiplied with; `ranged`: of a type with float16's range.
-__device__ __forceinline__ float grad_unit(const Scalars *s, bool ranged) {
-    return (ranged ? unit_scale(s->gmax) : 1.f) / s->mantissa;
+// What a row of G is multiplied with is two to this (float16 and pairs: by its value at the target, rowfac's
+// second) over the mantissa.  Held so that the row's weight x scale, rowfac's first, does not leave 32 bits.
+__device__ __forceinline__ int row_power(float2 fac) {
+    const int k = unit_power(__builtin_bit_cast(uint32_t, fac.y) & 0x7fffffffu);
+    return min(k, 86 + unit_power(__builtin_bit_cast(uint32_t, fac.x) & 0x7fffffffu));
 }
+template <bool RANGED>
+__device__ __forceinline__ float grad_unit(float2 fac, const Scalars *s) {
+    return ldexpf(1.f / s->mantissa, RANGED ? row_power(fac) : 0);
+}
+constexpr int kNoPower = 1 << 16;  // of a row of zeros
 
 // The call's scalars.  The mantissa is that of the largest weight among the first rows: one that most rows have
 // where it matters, and good for any others.
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(256) void k_xent_init(Scalars *s, const float *weig
     const uint32_t u = __builtin_bit_cast(uint32_t, c);
     // 1 where c is zero, denormal or infinite
     const bool plain = u >= 0x00800000u && u < 0x7f800000u;
-    *s = Scalars{0, 0, 0, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
+    *s = Scalars{0, 2 * kNoPower, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
 }
 
 __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
@@ -99,41 +108,50 @@ __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// Largest finite |value| of h's rows that have a target (blockIdx.y 0), with the power of two of each row; and of
-// the table's entries that are not out (1).
+// The power of two of each row of h, unit_power of its largest finite |value| (blockIdx.y 0), and the largest
+// finite |value| of the table's entries that are not out (1).
+template <class T>
 struct RangeArgs {
-    const float *x[2];
-    size_t rows[2], ld[2];
-    uint32_t *out[2];
-    const int64_t *target;
-    int *power;         // unit_power of each row of h
+    const T *h, *table;
+    size_t rows, entries, ldh, ldt;
+    int *power;
+    uint32_t *amax_w;
     const float *bias;  // or null
     int dim, lanes;     // lanes of a row, log2, 6 at most
 };
-__global__ __launch_bounds__(256) void k_ranges(RangeArgs a) {
-    const int y = blockIdx.y, per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
+template <class T>
+__device__ __forceinline__ uint32_t largest(const T *x, int dim, int l, int lanes) {
     uint32_t m = 0;
-    for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes); r < a.rows[y]; r += (size_t)gridDim.x * per) {
-        if (y == 1 && a.bias && a.bias[r] == -INFINITY) continue;
-        const float *x = a.x[y] + r * a.ld[y];
-        uint32_t own = 0;
-        for (int c = l * 4; c < a.dim; c += 4 << a.lanes) {
-            const Pack<float, 4> v = load_row<4>(x, c, a.dim);
+    for (int c = l * 4; c < dim; c += 4 << lanes) {
+        const Pack<T, 4> v = load_row<4>(x, c, dim);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t u = __builtin_bit_cast(uint32_t, v.v[e]) & 0x7fffffffu;
-                if (u < 0x7f800000u && u > own) own = u;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, (float)v.v[e]) & 0x7fffffffu;
+            if (u < 0x7f800000u && u > m) m = u;
         }
-        if (y == 0) {
+    }
+    return m;
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_ranges(RangeArgs<T> a) {
+    const int per = 256 >> a.lanes, l = threadIdx.x & ((1 << a.lanes) - 1);
+    const size_t first = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes), step = (size_t)gridDim.x * per;
+    if (blockIdx.y == 0) {
+        for (size_t r = first; r < a.rows; r += step) {
+            uint32_t m = largest(a.h + r * a.ldh, a.dim, l, a.lanes);
             for (int o = 1; o < 1 << a.lanes; o <<= 1) {
-                const uint32_t v = __shfl_xor(own, o, 64);
-                own = v > own ? v : own;
+                const uint32_t v = __shfl_xor(m, o, 64);
+                m = v > m ? v : m;
             }
-            if (l == 0) a.power[r] = unit_power(own);
-            if (a.target[r] < 0) continue;
+            if (l == 0) a.power[r] = m ? unit_power(m) : kNoPower;
         }
-        m = own > m ? own : m;
+        return;
+    }
+    uint32_t m = 0;
+    for (size_t r = first; r < a.entries; r += step) {
+        if (a.bias && a.bias[r] == -INFINITY) continue;
+        const uint32_t v = largest(a.table + r * a.ldt, a.dim, l, a.lanes);
+        m = v > m ? v : m;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -146,7 +164,7 @@ __global__ __launch_bounds__(256) void k_ranges(RangeArgs a) {
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 4; ++w) m = tops[w] > m ? tops[w] : m;
-        if (m) atomicMax(a.out[y], m);
+        if (m) atomicMax(a.amax_w, m);
     }
 }
 
@@ -176,7 +194,7 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
         if constexpr (N == 2)
-            if (power) sc = ldexpf(1.f, power[r]);
+            if (power) sc = ldexpf(1.f, min(power[r], 120));
         for (int c = l * 8; c < kp; c += 8 << lanes) {
             Pack<T, 8> v{};
             if (keep) v = load_row<8>(x + r * ld, c, dim);
@@ -206,11 +224,13 @@ void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type 
     k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, power, bias);
 }
 
-// rows x dim -> dim rows of rp values (or pairs), zeros past rows and for rows with a negative target.
+// rows x dim -> dim rows of rp values (or pairs), zeros past rows, for rows with a negative target and where G's
+// row is zeros.  What G's row was multiplied with is taken back (see the top).
 template <class T>
 __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim, size_t ld,
-                                                typename Planes<T>::type *out, size_t rp, const uint32_t *amax,
-                                                const int64_t *target) {
+                                                typename Planes<T>::type *out, size_t rp, const Scalars *sc,
+                                                const float2 *rowfac, const int64_t *target) {
+    constexpr bool kRanged = !std::is_same_v<T, bf16_t>;
     __shared__ T tile[64][65];
     const size_t r0 = (size_t)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -223,16 +243,22 @@ __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim
         tile[ty + 4 * i][tx] = v;
     }
     __syncthreads();
-    float sc = 1.f;
-    if constexpr (Planes<T>::count == 2) sc = unit_scale(*amax);
+    const size_t r = r0 + tx;
+    int power = 0;
+    bool on = true;
+    if constexpr (kRanged) {
+        const float2 fac = r < rows ? rowfac[r] : make_float2(0.f, 0.f);
+        power = sc->least - row_power(fac);
+        on = fac.y != 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int c = c0 + ty + 4 * i;
-        const size_t r = r0 + tx;
         if (c < dim && r < rp) {
-            const T v = tile[tx][ty + 4 * i];
+            T v = tile[tx][ty + 4 * i];
+            if constexpr (kRanged) v = on ? (T)ldexpf((float)v, power) : (T)0.f;
             if constexpr (Planes<T>::count == 2) {
-                const float f = v * sc;
+                const float f = v;
                 const half_t h = (half_t)f;
                 out[c * rp * 2 + pair_at(r)] = h;
                 out[c * rp * 2 + pair_at(r) + 32] = (half_t)(f - (float)h);
@@ -394,7 +420,7 @@ template <int R>
 __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int pieces, int rows, const float2 *zt,
                                                    const int64_t *target, int64_t table, const float *weight,
                                                    float scale, float *loss, float *lse, float2 *stat,
-                                                   float2 *rowfac, Scalars *sc) {
+                                                   float2 *rowfac, const int *power, Scalars *sc) {
     constexpr int L0 = 256 / R;
     __shared__ float s_top[L0][R + 1], s_sum[L0][R + 1];
     const int k = threadIdx.x % R, g = threadIdx.x / R, t = blockIdx.x * R + k;
@@ -448,14 +474,12 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2 *part, int piece
         }
     }
     if (sc) {
-        uint32_t u = __builtin_bit_cast(uint32_t, fac * rest) & 0x7fffffffu;
-        if (u >= 0x7f800000u) u = 0;
+        const float2 f = make_float2(fac, fac * rest);
+        const uint32_t u = __builtin_bit_cast(uint32_t, f.y) & 0x7fffffffu;
+        int least = u && u < 0x7f800000u ? power[t] + row_power(f) : 2 * kNoPower;
 #pragma unroll
-        for (int o = 1; o < R; o <<= 1) {
-            const uint32_t v = __shfl_xor(u, o, 64);
-            u = v > u ? v : u;
-        }
-        if (k == 0 && u) atomicMax(&sc->gmax, u);
+        for (int o = 1; o < R; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
+        if (k == 0 && least < kNoPower) atomicMin(&sc->least, least);
     }
 }
 
@@ -478,7 +502,6 @@ struct GradEpi {
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &, char *lds) const {
         if ((size_t)m >= vp) return;
         const int l = threadIdx.x & 63, q = l >> 4;
-        const float unit = grad_unit(lg.sc, !std::is_same_v<G, bf16_t>);
         const bool made = lg.made(m + 16 * MB, table);
         const float fw = to_logits(acc, lg, m, n, rows, table);
 #pragma unroll
@@ -488,6 +511,7 @@ struct GradEpi {
             const float f = made ? 1.f : lg.of_row(fw, t, rows);
             const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
             const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
+            const float unit = grad_unit<!std::is_same_v<G, bf16_t>>(fac, lg.sc);
             const float c = fac.x * unit, cs = c * st.y;
             if constexpr (SPLIT) {
 #pragma unroll
@@ -543,8 +567,8 @@ __global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *par
     constexpr int N = 16 / (int)sizeof(E);  // values of a lane
     const int t = blockIdx.x;
     const bool in = t < rows;
-    const float unit = grad_unit(sc, std::is_same_v<E, float>);
     const float2 fac = in ? rowfac[t] : make_float2(0.f, 0.f);
+    const float unit = grad_unit<std::is_same_v<E, float>>(fac, sc);
     const float c = fac.x * unit;
     const float2 st = in ? stat[t] : make_float2(0.f, 0.f);
     const int64_t y = in ? target[t] : -1;
@@ -590,16 +614,20 @@ __global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *par
     }
 }
 
-// Factor that a gradient's product still has to be multiplied with.
+// What a gradient's product still has to be multiplied with: factor() and two to power() of the row of the result.
+template <class O>
 struct OutScale {
-    const Scalars *sc;  // null: none
-    bool ranged, split;
-    bool of_table;  // the product with the rows (the table's gradient), else with the table
-    __device__ __forceinline__ float operator()() const {
-        if (!sc) return 1.f;
-        float f = 1.f / grad_unit(sc, ranged);
-        if (split) f /= unit_scale(of_table ? sc->amax_h : sc->amax_w);
-        return f;
+    const Scalars *sc;     // null: nothing
+    const float2 *rowfac;  // null: the table's gradient
+    __device__ __forceinline__ float factor() const { return sc ? sc->mantissa : 1.f; }
+    __device__ __forceinline__ int power(int r, int rows) const {
+        if (std::is_same_v<O, bf16_t> || !sc) return 0;
+        if (!rowfac) return -sc->least;
+        return (r < rows ? -row_power(rowfac[r]) : 0) - (std::is_same_v<O, float> ? unit_power(sc->amax_w) : 0);
+    }
+    static __device__ __forceinline__ float apply(float v, float f, int k) {
+        if constexpr (std::is_same_v<O, bf16_t>) return v * f;
+        return ldexpf(v * f, k);
     }
 };
 
@@ -607,7 +635,7 @@ struct OutScale {
 // or the 32-bit sum over pieces.
 template <class O>
 struct OutEpi {
-    OutScale sc;
+    OutScale<O> sc;
     O *out;
     size_t ld;
     float *part;  // [part][rows][cols4], or null
@@ -616,11 +644,14 @@ struct OutEpi {
     bool first, last;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
-        const float f = sc();
+        const float f = sc.factor();
+        int k[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) k[j] = sc.power(n + 16 * j + ((int)threadIdx.x & 15), rows);
         if (part || sum) {
             float *to = part ? part + (size_t)pl.part * rows * cols4 : sum;
             rows_through_lds<float, MB, NB>(
-                lds, [&](int i, int j, int e) { return part ? acc[i][j][e] : acc[i][j][e] * f; },
+                lds, [&](int i, int j, int e) { return part ? acc[i][j][e] : sc.apply(acc[i][j][e], f, k[j]); },
                 [&](int r, int c, const Pack<float, 4> &v) {
                     if (n + r >= rows || m + c >= cols) return;
                     Pack<float, 4> *s = reinterpret_cast<Pack<float, 4> *>(to + (size_t)(n + r) * cols4 + m + c);
@@ -644,7 +675,7 @@ struct OutEpi {
         }
         constexpr int PER = 16 / (int)sizeof(O);
         rows_through_lds<O, MB, NB>(
-            lds, [&](int i, int j, int e) { return (O)(acc[i][j][e] * f); },
+            lds, [&](int i, int j, int e) { return (O)sc.apply(acc[i][j][e], f, k[j]); },
             [&](int r, int c, const Pack<O, PER> &v) {
                 if (n + r >= rows || m + c >= cols) return;
                 store_row<PER>(out + (size_t)(n + r) * ld, m + c, cols, v);
@@ -656,7 +687,7 @@ struct OutEpi {
 // eighth part.
 template <class O>
 __global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts, int rows, int cols, int cols4,
-                                                    OutScale sc, O *out, size_t ld) {
+                                                    OutScale<O> sc, O *out, size_t ld) {
     __shared__ floatx4_t sums[8][32];
     const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
     const size_t at = (size_t)blockIdx.x * 32 + l, n = (size_t)rows * (cols4 / 4);
@@ -670,14 +701,15 @@ __global__ __launch_bounds__(256) void k_join_parts(const float *part, int parts
     if (g != 0 || at >= n) return;
 #pragma unroll
     for (int p = 1; p < 8; ++p) v += sums[p][l];
-    v *= sc();
     const int r = (int)(at / (cols4 / 4)), c = (int)(at % (cols4 / 4)) * 4;
+    const float f = sc.factor();
+    const int power = sc.power(r, rows);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (c + e < cols) out[(size_t)r * ld + c + e] = (O)v[e];
+        if (c + e < cols) out[(size_t)r * ld + c + e] = (O)sc.apply(v[e], f, power);
 }
 template <class O>
-void join_parts(const float *part, int parts, int rows, int cols, int cols4, OutScale sc, O *out, size_t ld, hipStream_t s) {
+void join_parts(const float *part, int parts, int rows, int cols, int cols4, OutScale<O> sc, O *out, size_t ld, hipStream_t s) {
     const size_t n = (size_t)rows * (cols4 / 4);
     k_join_parts<O><<<(uint32_t)((n + 31) / 32), 256, 0, s>>>(part, parts, rows, cols, cols4, sc, out, ld);
 }
@@ -755,7 +787,7 @@ struct Parts {
     float *split, *sum;
     float *z;  // few rows: the logits
     uint32_t *marks;
-    int *power;  // 32 bits: of the rows of h (Logits)
+    int *power;  // of the rows of h (k_ranges)
     void *hp, *wp, *ht, *g;
 };
 
@@ -774,7 +806,7 @@ inline Parts carve(Carver &c, const Sizes &z) {
         }
         return p;
     }
-    if (planes == 2) p.power = c.take<int>(z.rows);
+    if (planes == 2 || (z.grad && z.dtype == VHIP_DTYPE_F16)) p.power = c.take<int>(z.rows);
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
@@ -802,11 +834,11 @@ struct Call {
 
 // The pieces' join: as many rows a workgroup as still fill the chip.
 inline void join_pieces(const Parts &p, const Sizes &z, size_t rows, const int64_t *target, const float *weight, float scale,
-                        float *loss, float *lse, hipStream_t s) {
+                        float *loss, float *lse, const int *power, hipStream_t s) {
     Scalars *sc = z.grad && !z.small && z.dtype != VHIP_DTYPE_BF16 ? p.sc : nullptr;
 #define JOIN(R)                                                                                                       \
     k_xent_join<R><<<(uint32_t)ceil_div(rows, R), 256, 0, s>>>(p.part, z.pieces, (int)rows, p.zt, target, (int64_t)z.table, \
-                                                               weight, scale, loss, lse, p.stat, p.rowfac, sc)
+                                                               weight, scale, loss, lse, p.stat, p.rowfac, power, sc)
     if (rows <= 512)
         JOIN(1);
     else if (rows <= 8192)
@@ -821,12 +853,12 @@ int xent_small(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table, rows = (int)z.rows;
     small_stat<T>(SmallStat{c.h, c.table, (const float *)c.bias, c.target, p.part, p.zt, p.z, c.ldh, c.ldt, z.vp, rows, table, dim, c.scale},
                   (uint32_t)z.pieces, s);
-    join_pieces(p, z, z.rows, c.target, c.row_weight, c.scale, c.loss, c.lse, s);
+    join_pieces(p, z, z.rows, c.target, c.row_weight, c.scale, c.loss, c.lse, nullptr, s);
     if (z.grad) {
         small_grad<T>(SmallGrad{c.h, c.table, (const float *)c.bias, p.z, p.stat, p.rowfac, c.target, c.dtable, c.dh ? p.split : nullptr,
                                 c.ldh, c.ldt, c.lddt, z.vp, rows, table, dim, (int)z.cols4},
                       (uint32_t)z.ksplit, s);
-        if (c.dh) join_parts<T>(p.split, z.ksplit, rows, dim, (int)z.cols4, OutScale{}, (T *)c.dh, c.lddh, s);
+        if (c.dh) join_parts<T>(p.split, z.ksplit, rows, dim, (int)z.cols4, OutScale<T>{}, (T *)c.dh, c.lddh, s);
     }
     return launch_status("softmax launch");
 }
@@ -845,13 +877,11 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
-    constexpr bool kRanged = !std::is_same_v<P, bf16_t>;
     if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
-    if constexpr (kSplit) {
+    if (p.power) {
         const int lanes = lanes_log2((z.dim + 3) / 4);
-        const RangeArgs m{{h, w},   {z.rows, z.table}, {c.ldh, c.ldt}, {&p.sc->amax_h, &p.sc->amax_w},
-                          c.target, p.power,           (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
-        k_ranges<<<dim3(1024, 2), 256, 0, s>>>(m);
+        const RangeArgs<T> m{h, w, z.rows, z.table, c.ldh, c.ldt, p.power, &p.sc->amax_w, (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
+        k_ranges<T><<<dim3(1024, kSplit ? 2 : 1), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
@@ -865,10 +895,11 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const size_t rows = z.rows - r0 < z.piece_rows ? z.rows - r0 : z.piece_rows;
         const T *hr = h + r0 * c.ldh;
         const int64_t *target = c.target + r0;
+        const int *power = p.power ? p.power + r0 : nullptr;
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, nullptr, p.power ? p.power + r0 : nullptr, nullptr, s);
+            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, nullptr, power, nullptr, s);
             hp = (const P *)p.hp;
             ldh = z.kp * Planes<T>::count;
         }
@@ -882,7 +913,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.K = (int)z.kp;
         g.alo = g.blo = true;
         g.ksplit = g.batch = 1;
-        const Logits<kSplit> lg{(const float *)c.bias, p.sc, p.power ? p.power + r0 : nullptr, c.scale};
+        const Logits<kSplit> lg{(const float *)c.bias, p.sc, power, c.scale};
         typedef std::conditional_t<kSplit, float, half_t> E;
         const bool store = z.grad && stores_exps(z.dtype, z.dim);
         if (store) {
@@ -894,7 +925,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             VH_CHECK((mm_launch<P, kMode, false, false>)(g, z.stat_big, se, s));
         }
         join_pieces(p, z, rows, target, c.row_weight ? c.row_weight + r0 : nullptr, c.scale, c.loss ? c.loss + r0 : nullptr,
-                    c.lse ? c.lse + r0 : nullptr, s);
+                    c.lse ? c.lse + r0 : nullptr, power, s);
         VH_CHECK(launch_status("softmax launch"));
         if (!z.grad) continue;
         const size_t tp = round_up(rows, kMmK);
@@ -928,7 +959,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.N = (int)rows;
             d.K = table;
             d.ksplit = z.ksplit;
-            const OutScale os{p.sc, kRanged, kSplit, false};
+            const OutScale<T> os{p.sc, p.rowfac};
             T *out = (T *)c.dh + r0 * c.lddh;
             OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
                          true, true};
@@ -939,7 +970,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         if (c.dtable) {
             // K the rows: those past the last are zeros in both operands, those that do not count in the first
             k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
-                hr, rows, dim, c.ldh, (P *)p.ht, tp, &p.sc->amax_h, target);
+                hr, rows, dim, c.ldh, (P *)p.ht, tp, p.sc, p.rowfac, target);
             MmArgs d{};
             d.a = p.ht;
             d.b = gg;
@@ -951,7 +982,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.alo = d.blo = true;
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
-            OutEpi<T> oe{OutScale{p.sc, kRanged, kSplit, true}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
+            OutEpi<T> oe{OutScale<T>{p.sc, nullptr}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows};
             VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_tile, oe, s));
         }

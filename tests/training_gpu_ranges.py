@@ -131,3 +131,22 @@ def test_rows_of_zeros_and_rows_without_a_loss(tr, dtype, rows, dim):
     got = tr.softmax_xent_grad(h, w, y, weight, scale=2.0)
     xent_check(got, h, w, y, 2.0, None, weight)
     assert not got[0].any() and not got[2].any() and not got[3].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 640)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, 6e4])
+def test_values_of_rows_whose_target_is_left_out(tr, dtype, rows, dim, value):
+    """Loss +inf and no part in the gradients, whatever the row holds."""
+    h, w, y = xent_inputs(rows, 700, dim, dtype)
+    bias = torch.zeros(700, device="cuda")
+    y[:] = y % 699
+    y[3::9] = 699
+    bias[699] = -math.inf
+    gone = y == 699
+    want = tr.softmax_xent_grad(h, w, y, bias=bias)
+    xent_check(want, h, w, y, 1.0, bias)
+    assert (want[0][gone] == math.inf).all() and not want[2][gone].any()
+    h[gone] = value
+    loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, bias=bias)
+    same((loss, lse[~gone], dh, dw), (want[0], want[1][~gone], want[2], want[3]))

@@ -30,9 +30,10 @@
 // log(1 + sum of the others / the target's), keep their bits where p is nearly one.
 //
 // What does not count: a row whose target is negative has loss 0 and no part in the gradients, whatever its
-// values (its h is replaced by zeros where sums over rows are made).  An entry whose bias is -inf is out of
-// the softmax whatever its values.  A row whose target is out, or that has nothing left in, has loss +inf
-// and no part in the gradients.  A target past the table gives NaN.
+// values.  An entry whose bias is -inf is out of the softmax whatever its values.  A row whose target is out, or
+// that has nothing left in, has loss +inf and no part in the gradients, whatever its values.  (Where sums over rows
+// are made, h is replaced by zeros in rows whose G is zeros.)  A target past the table makes its row's loss and
+// gradient NaN, and so the table's gradient, which is a sum over rows.
 #include "xent_small.h"
 
 #include <cmath>
@@ -224,12 +225,12 @@ void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type 
     k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, power, bias);
 }
 
-// rows x dim -> dim rows of rp values (or pairs), zeros past rows, for rows with a negative target and where G's
-// row is zeros.  What G's row was multiplied with is taken back (see the top).
+// rows x dim -> dim rows of rp values (or pairs), zeros past rows and where G's row is zeros.  What G's row was
+// multiplied with is taken back (see the top).
 template <class T>
 __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim, size_t ld,
                                                 typename Planes<T>::type *out, size_t rp, const Scalars *sc,
-                                                const float2 *rowfac, const int64_t *target) {
+                                                const float2 *rowfac) {
     constexpr bool kRanged = !std::is_same_v<T, bf16_t>;
     __shared__ T tile[64][65];
     const size_t r0 = (size_t)blockIdx.x * 64;
@@ -239,24 +240,21 @@ __global__ __launch_bounds__(256) void k_pack_t(const T *x, size_t rows, int dim
         const size_t r = r0 + ty + 4 * i;
         const int c = c0 + tx;
         T v = (T)0.f;
-        if (r < rows && c < dim && target[r] >= 0) v = x[r * ld + c];
+        if (r < rows && c < dim) v = x[r * ld + c];
         tile[ty + 4 * i][tx] = v;
     }
     __syncthreads();
     const size_t r = r0 + tx;
+    const float2 fac = r < rows ? rowfac[r] : make_float2(0.f, 0.f);
+    const bool on = fac.y != 0.f;
     int power = 0;
-    bool on = true;
-    if constexpr (kRanged) {
-        const float2 fac = r < rows ? rowfac[r] : make_float2(0.f, 0.f);
-        power = sc->least - row_power(fac);
-        on = fac.y != 0.f;
-    }
+    if constexpr (kRanged) power = sc->least - row_power(fac);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int c = c0 + ty + 4 * i;
         if (c < dim && r < rp) {
-            T v = tile[tx][ty + 4 * i];
-            if constexpr (kRanged) v = on ? (T)ldexpf((float)v, power) : (T)0.f;
+            T v = on ? tile[tx][ty + 4 * i] : (T)0.f;
+            if constexpr (kRanged) v = (T)ldexpf((float)v, power);
             if constexpr (Planes<T>::count == 2) {
                 const float f = v;
                 const half_t h = (half_t)f;
@@ -328,7 +326,7 @@ struct StatEpi {
     int rows, table;
     E *exps;  // [rows][vp]
     size_t vp;
-    uint32_t *marks;  // [tile of N][tile of M]: exps of rows with a target that float16 cannot hold
+    uint32_t *marks;  // [tile of N][tile of M]: exps of rows that count and that float16 cannot hold
     int mt;
     template <int MB, int NB>
     __device__ void operator()(floatx4_t (&acc)[MB][NB], int m, int n, const MmPlace &pl, char *lds) const {
@@ -392,7 +390,7 @@ struct StatEpi {
                         if constexpr (!std::is_void_v<E>) acc[i][j][e] = v;
                     }
             }
-            if constexpr (kHalf) cut |= wide && y >= 0;
+            if constexpr (kHalf) cut |= wide && y >= 0 && !(lg.bias && y < table && lg.bias[y] == -INFINITY);
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (in && q == 0) part[(size_t)piece * rows + t] = make_float2(top, sum);
@@ -970,7 +968,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         if (c.dtable) {
             // K the rows: those past the last are zeros in both operands, those that do not count in the first
             k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
-                hr, rows, dim, c.ldh, (P *)p.ht, tp, p.sc, p.rowfac, target);
+                hr, rows, dim, c.ldh, (P *)p.ht, tp, p.sc, p.rowfac);
             MmArgs d{};
             d.a = p.ht;
             d.b = gg;

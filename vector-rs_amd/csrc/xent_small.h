@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void k_small_grad(SmallGrad a) {
     for (int k = 0; k < NH; ++k) {
         const int t = tid / HV + 256 / HV * k, col = d0 + tid % HV * 4;
         const int in = min(t, a.rows - 1);
-        four(hr[k], (const T *)a.h + (size_t)in * a.ldh, col, t < a.rows && a.target[in] >= 0);
+        four(hr[k], (const T *)a.h + (size_t)in * a.ldh, col, t < a.rows && a.rowfac[in].y != 0.f);
     }
 #pragma unroll
     for (int k = 0; k < NH; ++k)

@@ -150,3 +150,29 @@ def test_values_of_rows_whose_target_is_left_out(tr, dtype, rows, dim, value):
     h[gone] = value
     loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, bias=bias)
     same((loss, lse[~gone], dh, dw), (want[0], want[1][~gone], want[2], want[3]))
+
+
+# ---- limits ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_rows_than_an_operand_of_a_product_may_have(tr, dtype):
+    """Past 2^22 (16 bits: 2^23) rows the products' limit on K and not the size of G makes the pieces."""
+    rows, table, dim = (1 << 22) + 1000 if dtype == "f32" else (1 << 23) + 1000, 90, 8
+    h, w, y = xent_inputs(rows, table, dim, dtype)
+    loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, scale=2.0)
+    for part in (slice(0, 128), slice(rows - 128, rows)):
+        xent_check((loss[part], lse[part], None, None), h[part], w, y[part], 2.0)
+    step, total, size = 1 << 20, torch.zeros(table, dim, dtype=torch.float64, device="cuda"), 0.0
+    for i in range(0, rows, step):
+        z = (h[i:i + step].double() @ w.double().t()) * 2
+        p = torch.softmax(z, 1)
+        p[torch.arange(len(z), device="cuda"), y[i:i + step]] -= 1
+        p *= 2
+        total += p.t() @ h[i:i + step].double()
+        size = size + p.abs().t() @ h[i:i + step].double().abs()
+        unit = UNIT[h.dtype]
+        a = p.abs() @ w.double().abs()
+        within(dh[i:i + step], p @ w.double(), 2 * unit * a + (table + 128) * E * a + 2.0 ** -36)
+    # G's rounding is at random: over millions of rows it is far below a unit of the absolute sum, as are
+    # 32-bit sums in chains of a million
+    within(dw, total, 2 * UNIT[h.dtype] * total.abs() + 2.0 ** -10 * size)

@@ -756,6 +756,9 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
     // what a row needs in G, or in pieces of its logits
     const size_t per = grad ? z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2) : (table + 63) / 64 * sizeof(float2);
     size_t fit = piece_bytes() / per / 256 * 256;
+    // the rows are K of the table's gradient, which a product reads as rows of kMmMaxLd at most
+    const size_t longest = kMmMaxLd / (dtype == VHIP_DTYPE_F32 ? 2 : 1);
+    if (grad && fit > longest) fit = longest;
     if (fit < 256) fit = 256;
     z.piece_rows = rows <= fit ? rows : fit;
     z.tp = round_up(z.piece_rows, kMmK);

@@ -19,3 +19,15 @@ def test_gradients_take_rows_in_pieces_that_a_product_can_read(lib, dtype, longe
     size = lib.vhip_softmax_xent_workspace
     at, past = size(dtype, longest, table, 16, 1), size(dtype, 4 * longest, table, 16, 1)
     assert past - at <= 4 * 3 * longest + 4 * table * 16 + 4096
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("gradients", [0, 1])
+@pytest.mark.parametrize("rows,table,dim", [(1 << 25, 1000, 1024), (1 << 22, 100, 65_536), (1 << 20, 1, 65_536), (1 << 29, 300, 64)])
+def test_packed_rows_count_in_a_piece(lib, dtype, gradients, rows, table, dim):
+    """Rows are packed a piece at a time: 4 GiB hold what a piece needs, beside the table's operands, the parts of
+    one product (at most 512 of them), the sum over pieces and a power of two a row."""
+    got = lib.vhip_softmax_xent_workspace(dtype, rows, table, dim, gradients)
+    size = 4 if dtype == F32 else 2
+    beside = table * (dim + 64) * (size + 4) + 512 * 256 * (dim + 4) * 4 + 4 * rows
+    assert got <= (4 << 30) + (1 << 28) + beside

@@ -11,7 +11,7 @@
 //    its exps about their piece's largest logit, and a kernel turns them into G where they lie.  In bfloat16
 //    they are float16 for that while (11 bits before G's 8; exp_code), which holds them down to 2^-57 of their
 //    piece's largest; a tile with smaller ones that a float could hold is marked and made the first way.
-// Rows are taken in pieces so that G stays below kPieceBytes; from the second piece on the table's gradient is
+// Rows are taken in pieces so that G and the rows' packed copies stay below kPieceBytes; from the second piece on the table's gradient is
 // added up in 32 bits.  Every sum has a fixed order: results do not depend on timing.
 //
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
@@ -43,7 +43,7 @@
 namespace vh {
 namespace {
 
-constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G, or of what the loss alone needs of its rows
+constexpr size_t kPieceBytes = (size_t)4 << 30;  // of G, or of what the loss alone keeps, and of packed rows
 constexpr int kGBits = 14;
 // Columns from which G is made of stored exps.  A product's way costs 2 (pairs: 6) dim flops a value, the walk's 4
 // (8) bytes and a few operations.  4096 rows x 65536, product / walk in us: bfloat16 dim 384 1097 / 1125, 512
@@ -753,8 +753,9 @@ inline Sizes sizes_of(int dtype, size_t rows, size_t table, size_t dim, bool gra
         z.ksplit = (int)(tiles < gx ? tiles : gx);
         return z;
     }
-    // what a row needs in G, or in pieces of its logits
-    const size_t per = grad ? z.vp * (dtype == VHIP_DTYPE_F32 ? 4 : 2) : (table + 63) / 64 * sizeof(float2);
+    // what a row needs: G, or the pieces of its logits, and its packed copies
+    const size_t operand = dtype == VHIP_DTYPE_F32 ? 4 : 2;
+    const size_t per = (grad ? (z.vp + dim) * operand : (table + 63) / 64 * sizeof(float2)) + z.kp * operand;
     size_t fit = piece_bytes() / per / 256 * 256;
     // the rows are K of the table's gradient, which a product reads as rows of kMmMaxLd at most
     const size_t longest = kMmMaxLd / (dtype == VHIP_DTYPE_F32 ? 2 : 1);

@@ -443,8 +443,8 @@ int vhip_softmax_xent_grad(int ordinal, int dtype, const void *h, size_t rows, s
 
 /* `steps` Newton-Schulz steps on each of `count` matrices (stride elements apart):
  *   X = M / (|M|_F + eps);  A = X X^T, X <- a X + (b A + c A A) X   (on M^T where rows > cols),
- * which moves the singular values towards one.  The coefficients have to keep X bounded (singular values
- * below 32). */
+ * which moves the singular values towards one.  They start at 1 at most; coefficients that could let one, or a
+ * value of a I + b A + c A A, pass 2^30 in one of the steps are refused. */
 size_t vhip_orthogonalize_workspace(size_t count, size_t rows, size_t cols);
 int vhip_orthogonalize(int ordinal, int dtype, const void *in, size_t count, size_t rows, size_t cols, size_t ld_in,
                        size_t stride_in, int steps, float a, float b, float c, float eps, void *out, size_t ld_out,

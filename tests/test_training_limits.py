@@ -31,3 +31,15 @@ def test_packed_rows_count_in_a_piece(lib, dtype, gradients, rows, table, dim):
     size = 4 if dtype == F32 else 2
     beside = table * (dim + 64) * (size + 4) + 512 * 256 * (dim + 4) * 4 + 4 * rows
     assert got <= (4 << 30) + (1 << 28) + beside
+
+
+@pytest.mark.parametrize("a,b,c,steps,refused", [
+    (3.4445, -4.7750, 2.0315, 100, False), (25.0, -0.04, 0.0, 2, False), (25.0, -0.04, 0.0, 3, False), (25.0, -0.04, 0.0, 4, True), (2.0, 0.0, 0.0, 30, False),
+    (2.0, 0.0, 0.0, 31, True), (25.0, 0.0, 0.0, 7, True), (1e20, 0.0, 0.0, 1, True), (3.0, 40.0, 0.0, 5, True),
+    (0.0, 0.0, 1.5e9, 1, True), (1.0, -4e9, 3e9, 1, True), (-2.0, 1.5, -0.5, 50, False), (0.0, 0.0, 0.0, 3, False),
+])
+def test_coefficients_without_a_bound_are_refused(lib, a, b, c, steps, refused):
+    """All other checks are passed: what is not refused gets as far as looking for its GPU."""
+    missing = lib.vhip_device_count() + 100
+    got = lib.vhip_orthogonalize(missing, F32, 4096, 1, 4, 8, 8, 32, steps, a, b, c, 1e-7, 4096, 8, 32, 4096, 1 << 30, None)
+    assert got != 0 and (got == -5) == refused

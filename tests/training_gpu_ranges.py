@@ -176,3 +176,55 @@ def test_more_rows_than_an_operand_of_a_product_may_have(tr, dtype):
     # G's rounding is at random: over millions of rows it is far below a unit of the absolute sum, as are
     # 32-bit sums in chains of a million
     within(dw, total, 2 * UNIT[h.dtype] * total.abs() + 2.0 ** -10 * size)
+
+
+# ---- Newton-Schulz --------------------------------------------------------------------------------------
+
+def ns_steps(m, steps, coefficients, eps=1e-7):
+    """The definition in 64 bits, with the largest norms that it passes through."""
+    a, b, c = coefficients
+    x = m.double()
+    x = x / (x.norm() + eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    for _ in range(steps):
+        p = x @ x.t()
+        x = a * x + (b * p + c * p @ p) @ x
+    return x.t() if tall else x
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 40), (40, 90), (200, 90), (900, 1000)])
+@pytest.mark.parametrize("coefficients,steps", [
+    ((25.0, -0.04, 0.0), 2),      # singular values to 25, and back
+    ((2.0, -1.5, 0.5), 5),
+    ((1.5, -0.5, 0.0), 8),
+    ((300.0, 0.0, 0.0), 1),       # B past 255
+    ((300.0, -299.0, 0.0), 1),
+    ((3000.0, 0.0, 0.0), 2),
+    ((10.0, -200.0, 191.0), 1),   # large terms that cancel at one
+    ((0.01, 0.0, 0.0), 1),
+    ((-2.0, 1.5, -0.5), 3),
+])
+def test_orthogonalize_with_other_coefficients(tr, shape, coefficients, steps):
+    """Steps that take the singular values far from one on their way."""
+    m = normal(sum(shape), *shape)
+    got, want = tr.orthogonalize(m, steps=steps, coefficients=coefficients).double(), ns_steps(m, steps, coefficients)
+    # a step's error is 2^-20 of the sum of its terms' sizes times X, and what was there grows by its largest slope;
+    # both bounded over the interval that the singular values can reach
+    a, b, c = (abs(v) for v in coefficients)
+    s, err = 1.0, 2.0 ** -20
+    for _ in range(steps):
+        size = a + b * s * s + c * s ** 4
+        err = err * (a + 3 * b * s * s + 5 * c * s ** 4) + 2.0 ** -20 * size * s
+        s = max(abs(coefficients[0] * v + coefficients[1] * v ** 3 + coefficients[2] * v ** 5) for v in (s * i / 1000 for i in range(1001)))
+    assert torch.isfinite(got).all()
+    assert float((got - want).norm()) <= err * math.sqrt(min(shape)) + 2.0 ** -23 * float(want.norm())
+
+
+def test_orthogonalize_refuses_steps_without_a_bound(tr):
+    import vector_hip as vh
+
+    m = normal(1, 20, 30)
+    for coefficients, steps in (((25.0, 0.0, 0.0), 100), ((1e20, 0.0, 0.0), 1), ((3.0, 40.0, 0.0), 5)):
+        with pytest.raises(vh.InvalidConfig):
+            tr.orthogonalize(m, steps=steps, coefficients=coefficients)

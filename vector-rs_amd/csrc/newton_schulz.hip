@@ -6,8 +6,8 @@
 // which drives the singular values towards one while the singular vectors stay.  A direction whose singular
 // value is small grows by `a` a step, and what rounding puts into it grows as much, so X, A and B are held
 // in pairs of float16 (22 bits, mm16.h) and multiplied as three products with 32-bit sums: as exact as
-// 32-bit products, at a third of the 16-bit matrix rate.  X is held times 2^10 and A and B times 2^8: the
-// singular values stay below 2 for any useful coefficients, so neither leaves float16's range.
+// 32-bit products, at a third of the 16-bit matrix rate.  X is held times 2^10 and A and B times 2^8, or by smaller
+// powers of two where the coefficients let them leave float16's range (ns_scales).
 // The first X is the matrix times the power of two that brings |M|_F to [2^12, 2^13); what is left of the
 // norm goes into the first step's epilogues, so 16-bit matrices are exact in the high halves and their
 // first products have no low ones to multiply.  Where the result is rounded to bfloat16 (2^-9), the last
@@ -25,7 +25,7 @@
 namespace vh {
 namespace {
 
-constexpr float kXScale = 1024.f, kAScale = 256.f;
+constexpr float kXScale = 1024.f;  // of the first X
 constexpr int kNormParts = 64;
 
 __device__ __forceinline__ void split(float x, half_t &hi, half_t &lo) {
@@ -367,6 +367,51 @@ inline bool ns_small(size_t count, size_t m, size_t n) {
     return count * tm * tn <= 256;
 }
 
+// What X, A and B of a step are held times.
+struct NsScale {
+    double x, a, b;
+};
+constexpr int kMaxSteps = 100;
+// The scales of `steps` steps and of the X after them.  The singular values of X start at 1 at most, and a step takes
+// s to |a s + b s^3 + c s^5|: the largest of that over [0, s] bounds the next ones, and the values of each matrix
+// are at most its norm.  False where they may pass 2^30.
+inline bool ns_scales(double a, double b, double c, int steps, NsScale *out) {
+    auto held = [](double bound, double usual) {
+        while (usual * bound > 0x1p15) usual /= 2;
+        return usual;
+    };
+    // largest |p0 + p1 u + p2 u^2| over [0, top], times sqrt(u) where ROOT
+    auto largest = [&](double top, bool root) {
+        auto at = [&](double u) { return std::fabs(a + b * u + c * u * u) * (root ? std::sqrt(u) : 1.0); };
+        double m = std::fmax(at(0.0), at(top));
+        auto see = [&](double u) {
+            if (u > 0.0 && u < top) m = std::fmax(m, at(u));
+        };
+        // where the derivative is zero: q0 + q1 u + q2 u^2
+        const double q0 = root ? a : b, q1 = root ? 3 * b : 2 * c, q2 = root ? 5 * c : 0.0;
+        if (q2 != 0.0) {
+            const double d = q1 * q1 - 4 * q0 * q2;
+            if (d >= 0.0) {
+                // the root of larger size without cancellation, the other by the product of both
+                const double big = -0.5 * (q1 + std::copysign(std::sqrt(d), q1));
+                see(big / q2);
+                if (big != 0.0) see(q0 / big);
+            }
+        } else if (q1 != 0.0) {
+            see(-q0 / q1);
+        }
+        return m;
+    };
+    double s = 1.0;
+    for (int i = 0; i <= steps; ++i) {
+        const double bound = largest(s * s, false);
+        if (!(s <= 0x1p30 && (i == steps || bound <= 0x1p30))) return false;
+        out[i] = {held(s, kXScale), held(s * s, 256.0), held(bound, 256.0)};
+        s = largest(s * s, true);
+    }
+    return true;
+}
+
 struct NsParts {
     double *norm;
     float *gain;
@@ -426,6 +471,7 @@ struct NsCall {
     size_t count, rows, cols, ldi, si;
     int steps;
     float a, b, c, eps;
+    const NsScale *scale;
     void *out;
     size_t ldo, so;
 };
@@ -462,16 +508,18 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
         ga.alo = ga.blo = xlow;
         ga.upper = true;
         ga.out = p.a;
-        ga.alpha = kAScale / (kXScale * kXScale);
+        const NsScale &sc = k.scale[i];
+        ga.alpha = (float)(sc.a / (sc.x * sc.x));
         ga.gains = first ? 2 : 0;
         gb = ga;
         gb.a = gb.b = gb.add = p.a;
         gb.K = m;
         gb.alo = gb.blo = true;
         gb.out = p.b;
-        gb.alpha = k.c / kAScale;
-        gb.beta = k.b;
-        gb.diag = k.a * kAScale;
+        gb.alpha = (float)(k.c * sc.b / (sc.a * sc.a));
+        gb.beta = (float)(k.b * sc.b / sc.a);
+        gb.diag = (float)(k.a * sc.b);
+        const float alpha = (float)((last ? 1.0 : k.scale[i + 1].x) / (sc.b * sc.x));  // of B X
         gb.gains = 0;
         if (few) {
             ns_small_product<T>(ga, k.count, s);
@@ -494,10 +542,9 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             h.blo = low;
             h.out = xn;
             h.out_t = xtn;
-            h.alpha = 1.f / kAScale;
+            h.alpha = alpha;
             h.gains = first ? 1 : 0;
             if (last) {
-                h.alpha /= kXScale;
                 h.result = k.out;
                 h.ldr = k.ldo;
                 h.sr = k.so;
@@ -507,9 +554,8 @@ int newton_schulz(const NsCall &k, const NsParts &p, hipStream_t s) {
             VH_CHECK(launch_status("orthogonalize launch"));
             continue;
         }
-        StepEpi<T> es{xn, gain, 1.f / kAScale, n, m, nullptr, 0, 0};
+        StepEpi<T> es{xn, gain, alpha, n, m, nullptr, 0, 0};
         if (last) {
-            es.alpha /= kXScale;
             es.out = (T *)k.out;
             es.ldo = k.ldo;
             es.so = k.so;
@@ -545,8 +591,11 @@ int vhip_orthogonalize(int ordinal, int dtype, const void *in, size_t count, siz
     if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
     if (rows > 65536 || cols > 65536 || count > 65535)
         return set_error(VHIP_ERR_INVALID_CONFIG, "at most 65535 matrices of 65536 rows and columns");
-    if (steps < 1 || steps > 100) return set_error(VHIP_ERR_INVALID_CONFIG, "steps must be in [1, 100]");
+    if (steps < 1 || steps > kMaxSteps) return set_error(VHIP_ERR_INVALID_CONFIG, "steps must be in [1, 100]");
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return set_error(VHIP_ERR_INVALID_CONFIG, "coefficients must be finite");
+    NsScale scale[kMaxSteps + 1];
+    if (!ns_scales(a, b, c, steps, scale))
+        return set_error(VHIP_ERR_INVALID_CONFIG, "the coefficients let singular values grow past 2^30");
     if (!(eps >= 0.f)) return set_error(VHIP_ERR_INVALID_CONFIG, "eps must be >= 0");
     const bool empty = count == 0 || rows == 0 || cols == 0;
     if (!empty) {
@@ -564,7 +613,7 @@ int vhip_orthogonalize(int ordinal, int dtype, const void *in, size_t count, siz
     CallDevice dev;
     VH_CHECK(dev.enter(ordinal));
     if (empty) return VHIP_OK;
-    const NsCall k{in, count, rows, cols, ld_in, stride_in, steps, a, b, c, eps, out, ld_out, stride_out};
+    const NsCall k{in, count, rows, cols, ld_in, stride_in, steps, a, b, c, eps, scale, out, ld_out, stride_out};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case VHIP_DTYPE_F32: return newton_schulz<float>(k, p, s);

@@ -228,3 +228,13 @@ def test_orthogonalize_refuses_steps_without_a_bound(tr):
     for coefficients, steps in (((25.0, 0.0, 0.0), 100), ((1e20, 0.0, 0.0), 1), ((3.0, 40.0, 0.0), 5)):
         with pytest.raises(vh.InvalidConfig):
             tr.orthogonalize(m, steps=steps, coefficients=coefficients)
+
+
+@pytest.mark.parametrize("eps", [1e-7, 1e-20, 1e-30, 1e-44])
+@pytest.mark.parametrize("shape", [(20, 30), (30, 20), (900, 1000)])
+def test_orthogonalize_a_zero_matrix(tr, eps, shape):
+    """0 / (0 + eps) is 0 for every eps but 0, in a stack beside another matrix too."""
+    z = torch.zeros(2, *shape, device="cuda")
+    z[1] = normal(3, *shape)
+    got = tr.orthogonalize(z, eps=eps)
+    assert not got[0].any() and torch.isfinite(got[1]).all() and got[1].any()

@@ -92,7 +92,9 @@ __global__ __launch_bounds__(256) void k_ns_start(const T *in, int rows, int col
             const double up = norm > 0.0 && norm <= 1e300 ? ldexp(1.0, 13 - e) : 1.0;
             // a power of two that a float holds: what is past its range goes into the gain as well
             s_inv = (float)fmin(fmax(up, 0x1p-126), 0x1p126);
-            if (blockIdx.x == 0 && blockIdx.y == 0) gain[blockIdx.z] = (float)((double)kXScale / ((norm + (double)eps) * (double)s_inv));
+            // zeros over a small eps are zeros, though the gain's square may leave 32 bits
+            const double left = norm == 0.0 && eps > 0.f ? 0.0 : (double)kXScale / ((norm + (double)eps) * (double)s_inv);
+            if (blockIdx.x == 0 && blockIdx.y == 0) gain[blockIdx.z] = (float)left;
         }
     }
     __syncthreads();

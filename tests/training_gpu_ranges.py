@@ -238,3 +238,29 @@ def test_orthogonalize_a_zero_matrix(tr, eps, shape):
     z[1] = normal(3, *shape)
     got = tr.orthogonalize(z, eps=eps)
     assert not got[0].any() and torch.isfinite(got[1]).all() and got[1].any()
+
+
+# ---- arguments that torch differentiates --------------------------------------------------------------------
+
+def test_arguments_that_require_a_gradient(tr):
+    """Outputs have no graph: the forward calls refuse such arguments where a graph is being recorded."""
+    import vector_hip as vh
+
+    x, w = normal(1, 6, 32), normal(2, 32)
+    h, table, y = xent_inputs(6, 50, 32, "f32")
+    for make in (lambda r: tr.layer_norm(r(x), w, w), lambda r: tr.layer_norm(x, r(w), w), lambda r: tr.layer_norm(x, w, r(w)),
+                 lambda r: tr.softmax_xent(r(h), table, y), lambda r: tr.softmax_xent(h, r(table), y),
+                 lambda r: tr.softmax_xent(h, table, y, bias=r(normal(4, 50))), lambda r: tr.orthogonalize(r(x))):
+        leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+        with pytest.raises(vh.InvalidConfig):
+            make(leaf)
+        want = make(lambda t: t.clone())
+        with torch.no_grad():
+            got = make(leaf)
+        same([got] if torch.is_tensor(got) else got, [want] if torch.is_tensor(want) else want)
+        got = make(lambda t: leaf(t).detach())
+        same([got] if torch.is_tensor(got) else got, [want] if torch.is_tensor(want) else want)
+    # the gradients' calls give what a backward pass wants of them, parameters or not
+    grads = tr.softmax_xent_grad(h.clone().requires_grad_(), torch.nn.Parameter(table.clone()), y)
+    same(grads, tr.softmax_xent_grad(h, table, y))
+    assert not any(t.requires_grad for t in grads)

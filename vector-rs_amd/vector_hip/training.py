@@ -12,6 +12,11 @@ are float32, float16 and bfloat16.  The last dimension is contiguous; rows may b
 A call enqueues its work on the current stream of its arguments' device and returns without waiting, as
 other operations on such arrays do.  Wrong arguments raise ``InvalidConfig``; there is no CPU fallback.
 
+Outputs belong to no graph of automatic differentiation: gradients come from ``layer_norm_backward`` and
+``softmax_xent_grad``, which give them for any arguments and are themselves not differentiated.  The other calls
+refuse arguments that require a gradient where torch records a graph; call them under ``torch.no_grad()``, or
+with ``detach()``.  Tangents of forward-mode differentiation are not carried on either.
+
 Load torch before ``vector_hip``: torch brings a HIP runtime of its own, which this package's library then
 uses as well.  In the other order the process holds two, and a stream of the one means nothing to the other;
 calls raise ``DriverError`` then.
@@ -74,6 +79,7 @@ class _Library:
     def __init__(self, lib):
         _one_runtime()
         self.f32, self.u8, self.i64 = lib.float32, lib.uint8, lib.int64
+        self.records = getattr(lib, "is_grad_enabled", lambda: False)
         current = lib.cuda.current_stream
         self.stream = getattr(lib._C, "_cuda_getCurrentRawStream", lambda index: current(index).cuda_stream)
 
@@ -92,6 +98,14 @@ _library = _Libraries()
 def _on_gpu(name, a):
     if not getattr(a, "is_cuda", False):
         raise InvalidConfig(f"{name} is not an array in GPU memory")
+
+
+def _no_graph(lib, *arrays):
+    """Refuses arrays whose gradient would be lost with the outputs' graph."""
+    for a in arrays:
+        if getattr(a, "requires_grad", False) and lib.records():
+            raise InvalidConfig("an argument requires a gradient, and the outputs would have none: "
+                                "call this under torch.no_grad() or with detach()")
 
 
 def _rows2(name, a, like=None) -> int:
@@ -146,6 +160,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
         b, params = _vector("bias", bias, dim, device), _param_code(bias.dtype, code)
         if weight is not None and bias.dtype != weight.dtype:
             raise InvalidConfig("weight and bias must have the same type")
+    _no_graph(lib, x, weight, bias)
     y = x.new_empty((rows, dim))
     mean, rstd = x.new_empty((2, rows), dtype=lib.f32).unbind()
     _check(_lib.vhip_layer_norm(device, code, params, x.data_ptr(), rows, dim, ldx, w, b, eps, y.data_ptr(), dim,
@@ -197,6 +212,7 @@ def softmax_xent(h, table, target, scale: float = 1.0, bias=None):
     z = scale h table^T + bias, lse = log sum exp z, loss = lse - z[target].  target is int64; a negative one
     has loss 0.  bias (float32, constant) may hold -inf, which leaves an entry out."""
     rows, n, dim, ldh, ldt, device, code, lib, y, b = _xent_args(h, table, target, bias)
+    _no_graph(lib, h, table, bias)
     loss, lse = h.new_empty((2, rows), dtype=lib.f32).unbind()
     need = _lib.vhip_softmax_xent_workspace(code, rows, n, dim, 0)
     ws = h.new_empty(need, dtype=lib.u8)
@@ -236,6 +252,7 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
         raise InvalidConfig("rows of update overlap")
     a, b, c = coefficients
     device, code, lib = update.get_device(), _code[update.dtype], _library[type(update.dtype)]
+    _no_graph(lib, update)
     out = update.new_empty(update.shape)
     need = _lib.vhip_orthogonalize_workspace(count, rows, cols)
     ws = update.new_empty(need, dtype=lib.u8)

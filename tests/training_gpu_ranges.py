@@ -264,3 +264,74 @@ def test_arguments_that_require_a_gradient(tr):
     grads = tr.softmax_xent_grad(h.clone().requires_grad_(), torch.nn.Parameter(table.clone()), y)
     same(grads, tr.softmax_xent_grad(h, table, y))
     assert not any(t.requires_grad for t in grads)
+
+
+# ---- kernels that only larger calls reach --------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,dim", [(1500, 4096), (1100, 2300), (1100, 8192), (530, 16_384), (1300, 1025), (200, 20_000)])
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+def test_layer_norm_backward_of_many_long_rows(tr, rows, dim, dtype, params):
+    """Rows held by 4 and 16 waves, more of them than workgroups, and rows past that."""
+    base.test_layer_norm_backward(tr, rows, dim, 0, dtype, params)
+
+
+@pytest.mark.parametrize("rows,dim,pad", base.LN_SHAPES)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_layer_norm_scale(tr, rows, dim, pad, dtype):
+    """rstd: 64 additions in a chain put the mean off by 64 e mean|x| and the variance by 64 e of itself."""
+    x = (normal(1, rows, dim + pad) * 2 + 0.5).to(TYPES[dtype])[:, :dim]
+    _, _, rstd = tr.layer_norm(x)
+    _, _, rr, _ = base.ln_reference(x, None, None, 1e-5)
+    off = 64 * E * 2 * x.double().abs().mean(1) * rr
+    within(rstd, rr, rr * (off + off * off + 40 * E))
+
+
+@pytest.mark.parametrize("rows,table,dim", [(20, 9000, 330), (33, 8192, 100), (40, 9001, 264), (48, 20_000, 65), (49, 8500, 200), (64, 9000, 331),
+                                            (17, 8191, 90), (64, 8191, 90)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_softmax_xent_of_few_rows_over_longer_tables(tr, rows, table, dim, dtype):
+    """Turns of 16 and of 32 entries, one to four blocks of rows."""
+    h, w, y = xent_inputs(rows, table, dim, dtype)
+    bias = 0.3 * normal(5, table)
+    out = int(y[0]) - 1
+    bias[out] = -math.inf
+    y = torch.where(y == out % table, int(y[0]), y)
+    xent_check((*tr.softmax_xent(h, w, y, scale=2.0), None, None), h, w, y, 2.0)
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=2.0, bias=bias), h, w, y, 2.0, bias)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_softmax_xent_of_more_rows_than_a_join_takes_by_fours(tr, dtype):
+    h, w, y = xent_inputs(9001, 300, 40, dtype)
+    weight = torch.rand(9001, device="cuda", generator=base.gen(9)) / 9001
+    xent_check(tr.softmax_xent_grad(h, w, y, weight, scale=2.0), h, w, y, 2.0, None, weight)
+
+
+def pairs_model(m, steps, eps=1e-7):
+    """The steps with X, A and B rounded to pairs of float16 (22 bits) where they are held so, in 64 bits else:
+    how far that alone takes the result from the definition."""
+    def pair(x, scale):
+        hi = (x * scale).half().double()
+        return (hi + (x * scale - hi).half().double()) / scale
+
+    a, b, c = base.NS
+    x = m.double()
+    x = x / (x.norm() + eps)
+    x = x.t() if x.shape[0] > x.shape[1] else x
+    x = pair(x, 1024.0)
+    for i in range(steps):
+        p = pair(x @ x.t(), 256.0)
+        q = pair(a * torch.eye(len(p), dtype=p.dtype, device=p.device) + b * p + c * p @ p, 256.0)
+        x = q @ x
+        x = x if i + 1 == steps else pair(x, 1024.0)
+    return x if m.shape[0] <= m.shape[1] else x.t()
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 64), (100, 300), (300, 100), (129, 257), (400, 390), (900, 700), (1500, 1600), (2304, 2200)])
+def test_orthogonalize_is_as_near_as_its_pairs(tr, rows, cols):
+    """32 bits, 5 steps: no further from the definition than 20 times what holding pairs costs (products drop the
+    low halves' product and add in 32 bits, each of about the size of a pair's rounding, over three products a step)."""
+    m = 0.01 * normal(rows + cols, rows, cols)
+    want = base.ns_reference(m, 5, 1e-7)
+    limit = 20 * float((pairs_model(m, 5) - want).norm()) + 4 * E * float(want.norm())
+    assert float((tr.orthogonalize(m).double() - want).norm()) <= limit

@@ -133,6 +133,48 @@ def test_rows_of_zeros_and_rows_without_a_loss(tr, dtype, rows, dim):
     assert not got[0].any() and not got[2].any() and not got[3].any()
 
 
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300), (300, 640)])
+@pytest.mark.parametrize("power", [12, 20, 30, 60])
+@pytest.mark.parametrize("pieces", [False, True])
+def test_one_entry_far_larger_than_the_others(tr, rows, dim, power, pieces, monkeypatch):
+    """An entry that no row comes near (its logits are below -2^power): everything is as without it."""
+    if pieces:
+        monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
+    h, w, y = xent_inputs(rows, 700, dim, "f32")
+    y = torch.where(y == 5, 6, y)
+    h[:, 0], w[5] = 1.0, 0.0
+    w[5, 0] = -2.0 ** power
+    w[9:300:7] *= 2.0 ** -14
+    bias = 0.3 * normal(5, 700)
+    keep = torch.arange(700, device="cuda") != 5
+    at = y - (y > 5).long()
+    loss, lse, dh, dw = tr.softmax_xent_grad(h, w, y, scale=2.0, bias=bias)
+    few = w[keep].contiguous()
+    off = bias[keep].contiguous()
+    _, _, rdh, _, g, *_ = xent_reference(h, few, at, 2.0, off)
+    want = tr.softmax_xent_grad(h, few, at, scale=2.0, bias=off)
+    xent_check((loss, lse, want[2], dw[keep].contiguous()), h, few, at, 2.0, off)
+    assert not dw[5].any()
+    xent_check((loss, lse, dh, want[3]), h, few, at, 2.0, off)
+    # 32-bit operands' G and sums as in xent_check, for logits below 32, and G's smallest step in every entry
+    a = few.double().abs()
+    within(dh, rdh, 2.0 ** -16 * (g.abs() @ a) + 2.0 ** -36 * g.abs().max(1, keepdim=True).values * a.sum(0) + 2.0 ** -40)
+    xent_check((*tr.softmax_xent(h, w, y, scale=2.0, bias=bias), None, None), h, few, at, 2.0, off)
+
+
+@pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 300), (300, 640)])
+@pytest.mark.parametrize("pieces", [False, True])
+def test_entries_of_sizes_far_apart(tr, rows, dim, pieces, monkeypatch):
+    """Entries from 2^-60 of the largest to the largest, zeros among them."""
+    if pieces:
+        monkeypatch.setenv("VHIP_XENT_PIECE_BYTES", "1")
+    h, w, y = xent_inputs(rows, 700, dim, "f32")
+    w *= torch.exp2(-60.0 * torch.rand(700, 1, device="cuda", generator=base.gen(4)) ** 2)
+    w[::11] = 0.0
+    xent_check(tr.softmax_xent_grad(h, w, y, scale=2.0), h, w, y, 2.0)
+    xent_check((*tr.softmax_xent(h, w, y, scale=2.0), None, None), h, w, y, 2.0)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,dim", [(20, 96), (100, 96), (150, 640)])
 @pytest.mark.parametrize("value", [math.nan, math.inf, 6e4])

@@ -16,8 +16,9 @@
 //
 // Types.  float16 and bfloat16 operands are multiplied as they are; 32-bit ones as pairs of float16
 // (mm16.h), scaled by a power of two that brings the largest finite value to [2^13, 2^14), so that what a
-// plane cannot hold is 2^-39 of that value: for the logits a power for each row of h, and one for the entries
-// of the table that are not out.  G is rounded to the operands' type (to two planes for 32-bit
+// plane cannot hold is 2^-39 of that value: for the logits a power for each row of h, one for the entries
+// of the table that are not out, and their own for those that are far smaller than the largest (kWide; where there
+// are such entries G takes their powers before it multiplies the table, k_fold_powers).  G is rounded to the operands' type (to two planes for 32-bit
 // operands), which is as far as the gradients that are returned are rounded too.  In float16 (and pairs) each row
 // of G is held times 2^14 / 2^e, where 2^e is the power of two above its largest value, c scale (1 - p) at the
 // target: neither small probabilities nor rows of small weight lose their bits.  For the table's gradient the rows
@@ -57,6 +58,7 @@ inline bool stores_exps(int dtype, size_t dim) {
 // State of a call on the device.
 struct Scalars {
     uint32_t amax_w;  // bits of the largest finite |value| of entries that are not out
+    uint32_t wide;    // whether entries have powers of their own
     int least;        // least sum of a row's power (k_ranges) and of its row_power
     float mantissa;   // of weight x scale, in [1, 2)
 };
@@ -80,7 +82,11 @@ template <bool RANGED>
 __device__ __forceinline__ float grad_unit(float2 fac, const Scalars *s) {
     return ldexpf(1.f / s->mantissa, RANGED ? row_power(fac) : 0);
 }
-constexpr int kNoPower = 1 << 16;  // of a row of zeros
+constexpr int kNoPower = 1 << 16;  // of a row of zeros, or one that is out
+// An entry has a power of its own where its largest value is less than 2^-8 of the table's: values down to 2^-15
+// of it keep the 22 bits of a pair.
+constexpr int kWide = 8;
+__device__ __forceinline__ bool own_power(int own, int common) { return own < kNoPower && own - common > kWide; }
 
 // The call's scalars.  The mantissa is that of the largest weight among the first rows: one that most rows have
 // where it matters, and good for any others.
@@ -101,7 +107,7 @@ __global__ __launch_bounds__(256) void k_xent_init(Scalars *s, const float *weig
     const uint32_t u = __builtin_bit_cast(uint32_t, c);
     // 1 where c is zero, denormal or infinite
     const bool plain = u >= 0x00800000u && u < 0x7f800000u;
-    *s = Scalars{0, 2 * kNoPower, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
+    *s = Scalars{0, 0, 2 * kNoPower, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
 }
 
 __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
@@ -109,17 +115,18 @@ __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// The power of two of each row of h, unit_power of its largest finite |value| (blockIdx.y 0), and the largest
-// finite |value| of the table's entries that are not out (1).
+// The power of two of each row of h, unit_power of its largest finite |value| (blockIdx.y 0), and that of the
+// table's entries that are not out, with the largest |value| of all (1).
 template <class T>
 struct RangeArgs {
     const T *h, *table;
     size_t rows, entries, ldh, ldt;
-    int *power;
+    int *power, *entry_power;
     uint32_t *amax_w;
     const float *bias;  // or null
     int dim, lanes;     // lanes of a row, log2, 6 at most
 };
+// of a row, in each of its lanes
 template <class T>
 __device__ __forceinline__ uint32_t largest(const T *x, int dim, int l, int lanes) {
     uint32_t m = 0;
@@ -131,6 +138,10 @@ __device__ __forceinline__ uint32_t largest(const T *x, int dim, int l, int lane
             if (u < 0x7f800000u && u > m) m = u;
         }
     }
+    for (int o = 1; o < 1 << lanes; o <<= 1) {
+        const uint32_t v = __shfl_xor(m, o, 64);
+        m = v > m ? v : m;
+    }
     return m;
 }
 template <class T>
@@ -139,19 +150,16 @@ __global__ __launch_bounds__(256) void k_ranges(RangeArgs<T> a) {
     const size_t first = (size_t)blockIdx.x * per + (threadIdx.x >> a.lanes), step = (size_t)gridDim.x * per;
     if (blockIdx.y == 0) {
         for (size_t r = first; r < a.rows; r += step) {
-            uint32_t m = largest(a.h + r * a.ldh, a.dim, l, a.lanes);
-            for (int o = 1; o < 1 << a.lanes; o <<= 1) {
-                const uint32_t v = __shfl_xor(m, o, 64);
-                m = v > m ? v : m;
-            }
+            const uint32_t m = largest(a.h + r * a.ldh, a.dim, l, a.lanes);
             if (l == 0) a.power[r] = m ? unit_power(m) : kNoPower;
         }
         return;
     }
     uint32_t m = 0;
     for (size_t r = first; r < a.entries; r += step) {
-        if (a.bias && a.bias[r] == -INFINITY) continue;
-        const uint32_t v = largest(a.table + r * a.ldt, a.dim, l, a.lanes);
+        const bool out = a.bias && a.bias[r] == -INFINITY;
+        const uint32_t v = out ? 0 : largest(a.table + r * a.ldt, a.dim, l, a.lanes);
+        if (l == 0) a.entry_power[r] = v ? unit_power(v) : kNoPower;
         m = v > m ? v : m;
     }
 #pragma unroll
@@ -182,20 +190,28 @@ struct Planes<float> {
 };
 
 // rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
-// row, 8 values each at a time.  Pairs are scaled by two to `power` of the row, or by one scale where that is null.
+// row, 8 values each at a time.  Pairs are scaled by two to their row's power; `entries`: by that of the table's
+// largest value, or the entry's own.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              int kp, int lanes, const uint32_t *amax, const int *power, const float *bias) {
+                                              int kp, int lanes, const int *power, Scalars *entries, const float *bias) {
     typedef typename Planes<T>::type P;
     constexpr int N = Planes<T>::count;
     const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
-    float sc = 1.f;
+    int common = 0;
     if constexpr (N == 2)
-        if (!power) sc = unit_scale(*amax);
+        if (entries) common = unit_power(entries->amax_w);
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
-        if constexpr (N == 2)
-            if (power) sc = ldexpf(1.f, min(power[r], 120));
+        float sc = 1.f;
+        if constexpr (N == 2) {
+            int k = min(power[r], 120);
+            if (entries && !own_power(power[r], common))
+                k = common;
+            else if (entries && l == 0)
+                entries->wide = 1;
+            sc = ldexpf(1.f, k);
+        }
         for (int c = l * 8; c < kp; c += 8 << lanes) {
             Pack<T, 8> v{};
             if (keep) v = load_row<8>(x + r * ld, c, dim);
@@ -217,12 +233,12 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
     }
 }
 template <class T>
-void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const uint32_t *amax,
-          const int *power, const float *bias, hipStream_t s) {
+void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const int *power, Scalars *entries,
+          const float *bias, hipStream_t s) {
     const int lanes = lanes_log2(kp / 8);
     const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
     const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
-    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, amax, power, bias);
+    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, power, entries, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and where G's row is zeros.  What G's row was
@@ -272,7 +288,7 @@ template <bool SPLIT>
 struct Logits {
     const float *bias;
     const Scalars *sc;
-    const int *power;  // of the rows
+    const int *power, *entry_power;  // of the rows, of the entries
     float scale;
     __device__ __forceinline__ float factor() const { return SPLIT ? scale / unit_scale(sc->amax_w) : scale; }
     // the factor f of row t, if that is one
@@ -294,8 +310,22 @@ __device__ __forceinline__ bool exp_cut(float x) { return x < -39.f && x > -104.
 template <int MB, int NB, bool SPLIT>
 __device__ __forceinline__ float to_logits(floatx4_t (&acc)[MB][NB], const Logits<SPLIT> &lg, int m, int n, int rows, int table) {
     const float f = lg.factor();
-    if (!lg.made(m + 16 * MB, table)) return f;
     const int l = threadIdx.x & 63, q = l >> 4;
+    if constexpr (SPLIT) {
+        if (lg.sc->wide) {
+            const int common = unit_power(lg.sc->amax_w);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = m + 16 * i + 4 * q + e, own = v < table ? lg.entry_power[v] : kNoPower;
+                    const int k = own_power(own, common) ? common - own : 0;
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) acc[i][j][e] = ldexpf(acc[i][j][e], k);
+                }
+        }
+    }
+    if (!lg.made(m + 16 * MB, table)) return f;
     float fs[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) fs[j] = lg.of_row(f, n + 16 * j + (l & 15), rows);
@@ -612,16 +642,64 @@ __global__ __launch_bounds__(256) void k_exps_to_grad(void *g, const float2 *par
     }
 }
 
+// Where entries have powers of their own: a row of G (pairs) takes them back before it multiplies the table, and
+// then the power of two that brings the largest of what is left to [2^13, 2^14).  A row a workgroup.
+__global__ __launch_bounds__(256) void k_fold_powers(half_t *g, size_t vp, int table, const int *entry_power, const Scalars *sc, int *boost) {
+    if (!sc->wide) return;
+    __shared__ uint32_t tops[4];
+    half_t *row = g + (size_t)blockIdx.x * vp * 2;
+    const int common = unit_power(sc->amax_w);
+    // calls f(value, power to take back, hi, lo) for this lane's values
+    auto walk = [&](auto &&f) {
+        for (size_t v = (size_t)threadIdx.x * 8; v < vp; v += 256 * 8) {
+            half_t *at = row + pair_at(v);
+            Pack<half_t, 8> hi = *reinterpret_cast<Pack<half_t, 8> *>(at), lo = *reinterpret_cast<Pack<half_t, 8> *>(at + 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int own = (int)v + e < table ? entry_power[v + e] : kNoPower;
+                f((float)hi.v[e] + (float)lo.v[e], own_power(own, common) ? common - own : 0, hi.v[e], lo.v[e]);
+            }
+            *reinterpret_cast<Pack<half_t, 8> *>(at) = hi;
+            *reinterpret_cast<Pack<half_t, 8> *>(at + 32) = lo;
+        }
+    };
+    uint32_t m = 0;
+    walk([&](float x, int k, half_t &, half_t &) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, ldexpf(x, k)) & 0x7fffffffu;
+        if (u < 0x7f800000u && u > m) m = u;
+    });
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_xor(m, o, 64);
+        m = v > m ? v : m;
+    }
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = tops[w] > m ? tops[w] : m;
+    const int up = unit_power(m);
+    walk([&](float x, int k, half_t &hi, half_t &lo) {
+        x = ldexpf(x, k + up);
+        hi = (half_t)x;
+        lo = (half_t)(x - (float)hi);
+    });
+    if (threadIdx.x == 0) boost[blockIdx.x] = up;
+}
+
 // What a gradient's product still has to be multiplied with: factor() and two to power() of the row of the result.
 template <class O>
 struct OutScale {
     const Scalars *sc;     // null: nothing
     const float2 *rowfac;  // null: the table's gradient
+    const int *boost;      // of k_fold_powers
     __device__ __forceinline__ float factor() const { return sc ? sc->mantissa : 1.f; }
     __device__ __forceinline__ int power(int r, int rows) const {
         if (std::is_same_v<O, bf16_t> || !sc) return 0;
         if (!rowfac) return -sc->least;
-        return (r < rows ? -row_power(rowfac[r]) : 0) - (std::is_same_v<O, float> ? unit_power(sc->amax_w) : 0);
+        if (r >= rows) return 0;
+        int k = row_power(rowfac[r]);
+        if constexpr (std::is_same_v<O, float>) k += unit_power(sc->amax_w) + (sc->wide ? boost[r] : 0);
+        return -k;
     }
     static __device__ __forceinline__ float apply(float v, float f, int k) {
         if constexpr (std::is_same_v<O, bf16_t>) return v * f;
@@ -789,7 +867,8 @@ struct Parts {
     float *split, *sum;
     float *z;  // few rows: the logits
     uint32_t *marks;
-    int *power;  // of the rows of h (k_ranges)
+    int *power, *entry_power;  // of the rows of h, of the table's (k_ranges)
+    int *boost;
     void *hp, *wp, *ht, *g;
 };
 
@@ -809,9 +888,11 @@ inline Parts carve(Carver &c, const Sizes &z) {
         return p;
     }
     if (planes == 2 || (z.grad && z.dtype == VHIP_DTYPE_F16)) p.power = c.take<int>(z.rows);
+    if (planes == 2) p.entry_power = c.take<int>(z.table);
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
+        if (planes == 2) p.boost = c.take<int>(z.tp);
         p.stat = c.take<float2>(z.piece_rows);
         p.rowfac = c.take<float2>(z.piece_rows);
         p.ht = c.take<uint16_t>(planes * z.dim * z.tp);
@@ -882,13 +963,13 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
     if (p.power) {
         const int lanes = lanes_log2((z.dim + 3) / 4);
-        const RangeArgs<T> m{h, w, z.rows, z.table, c.ldh, c.ldt, p.power, &p.sc->amax_w, (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
+        const RangeArgs<T> m{h, w, z.rows, z.table, c.ldh, c.ldt, p.power, p.entry_power, &p.sc->amax_w, (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
         k_ranges<T><<<dim3(1024, kSplit ? 2 : 1), 256, 0, s>>>(m);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
     if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
-        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, &p.sc->amax_w, nullptr, (const float *)c.bias, s);
+        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, p.entry_power, p.sc, (const float *)c.bias, s);
         wp = (const P *)p.wp;
         ldw = z.kp * Planes<T>::count;
     }
@@ -901,7 +982,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, nullptr, power, nullptr, s);
+            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, power, nullptr, nullptr, s);
             hp = (const P *)p.hp;
             ldh = z.kp * Planes<T>::count;
         }
@@ -915,7 +996,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         g.K = (int)z.kp;
         g.alo = g.blo = true;
         g.ksplit = g.batch = 1;
-        const Logits<kSplit> lg{(const float *)c.bias, p.sc, power, c.scale};
+        const Logits<kSplit> lg{(const float *)c.bias, p.sc, power, p.entry_power, c.scale};
         typedef std::conditional_t<kSplit, float, half_t> E;
         const bool store = z.grad && stores_exps(z.dtype, z.dim);
         if (store) {
@@ -952,23 +1033,6 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             VH_CHECK((mm_launch<P, kMode, false, false>)(gg, z.stat_big, ge, s));
         }
         const P *gg = (const P *)p.g;
-        if (c.dh) {
-            // columns of the table, K its rows: G's columns past the table are zeros
-            MmArgs d = g;
-            d.b = gg;
-            d.ldb = z.vp * Planes<T>::count;
-            d.M = dim;
-            d.N = (int)rows;
-            d.K = table;
-            d.ksplit = z.ksplit;
-            const OutScale<T> os{p.sc, p.rowfac};
-            T *out = (T *)c.dh + r0 * c.lddh;
-            OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
-                         true, true};
-            VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_tile, oe, s));
-            if (z.ksplit > 1)
-                join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
-        }
         if (c.dtable) {
             // K the rows: those past the last are zeros in both operands, those that do not count in the first
             k_pack_t<T><<<dim3((uint32_t)(tp / 64), (uint32_t)ceil_div(dim, 64)), 256, 0, s>>>(
@@ -984,9 +1048,27 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
             d.alo = d.blo = true;
             d.ksplit = d.batch = 1;
             const bool many = z.piece_rows < z.rows;
-            OutEpi<T> oe{OutScale<T>{p.sc, nullptr}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
+            OutEpi<T> oe{OutScale<T>{p.sc, nullptr, nullptr}, (T *)c.dtable, c.lddt, nullptr, many ? p.sum : nullptr, dim, table,
                          (int)z.cols4, r0 == 0, r0 + rows >= z.rows};
             VH_CHECK((mm_launch<P, kMode, false, true>)(d, z.dw_tile, oe, s));
+        }
+        if (c.dh) {
+            if constexpr (kSplit) k_fold_powers<<<(uint32_t)rows, 256, 0, s>>>((half_t *)p.g, z.vp, table, p.entry_power, p.sc, p.boost);
+            // columns of the table, K its rows: G's columns past the table are zeros
+            MmArgs d = g;
+            d.b = gg;
+            d.ldb = z.vp * Planes<T>::count;
+            d.M = dim;
+            d.N = (int)rows;
+            d.K = table;
+            d.ksplit = z.ksplit;
+            const OutScale<T> os{p.sc, p.rowfac, p.boost};
+            T *out = (T *)c.dh + r0 * c.lddh;
+            OutEpi<T> oe{os, out, c.lddh, z.ksplit > 1 ? p.split : nullptr, nullptr, dim, (int)rows, (int)z.cols4,
+                         true, true};
+            VH_CHECK((mm_launch<P, kMode, true, false>)(d, z.dh_tile, oe, s));
+            if (z.ksplit > 1)
+                join_parts<T>(p.split, z.ksplit, (int)rows, dim, (int)z.cols4, os, out, c.lddh, s);
         }
         VH_CHECK(launch_status("gradient launch"));
     }

@@ -90,12 +90,18 @@ __device__ __forceinline__ bool own_power(int own, int common) { return own < kN
 
 // The call's scalars.  The mantissa is that of the largest weight among the first rows: one that most rows have
 // where it matters, and good for any others.
-__global__ __launch_bounds__(256) void k_xent_init(Scalars *s, const float *weight, int rows, float scale) {
+struct InitArgs {
+    Scalars *sc;
+    const float *weight;
+    int rows;
+    float scale;
+};
+__device__ void init_scalars(const InitArgs &a) {
     __shared__ float top[4];
-    float m = weight ? 0.f : 1.f;
-    if (weight)
-        for (int t = threadIdx.x; t < min(rows, 4096); t += 256) {
-            const float w = fabsf(weight[t]);
+    float m = a.weight ? 0.f : 1.f;
+    if (a.weight)
+        for (int t = threadIdx.x; t < min(a.rows, 4096); t += 256) {
+            const float w = fabsf(a.weight[t]);
             if (w <= 3.4e38f && w > m) m = w;
         }
 #pragma unroll
@@ -103,12 +109,13 @@ __global__ __launch_bounds__(256) void k_xent_init(Scalars *s, const float *weig
     if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    const float c = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fabsf(scale);
+    const float c = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fabsf(a.scale);
     const uint32_t u = __builtin_bit_cast(uint32_t, c);
     // 1 where c is zero, denormal or infinite
     const bool plain = u >= 0x00800000u && u < 0x7f800000u;
-    *s = Scalars{0, 0, 2 * kNoPower, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
+    *a.sc = Scalars{0, 0, 2 * kNoPower, plain ? __builtin_bit_cast(float, (u & 0x007fffffu) | 0x3f800000u) : 1.f};
 }
+__global__ __launch_bounds__(256) void k_xent_init(InitArgs a) { init_scalars(a); }
 
 __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
     const int i = blockIdx.x * 256 + threadIdx.x;
@@ -116,15 +123,18 @@ __global__ __launch_bounds__(256) void k_clear(uint32_t *p, int n) {
 }
 
 // The power of two of each row of h, unit_power of its largest finite |value| (blockIdx.y 0), and that of the
-// table's entries that are not out, with the largest |value| of all (1).
+// table's entries that are not out, with the largest |value| of all that a workgroup sees (1).  One workgroup also
+// makes the call's scalars.
+constexpr int kRangeGroups = 1024;
 template <class T>
 struct RangeArgs {
     const T *h, *table;
     size_t rows, entries, ldh, ldt;
     int *power, *entry_power;
-    uint32_t *amax_w;
+    uint32_t *tops;     // [kRangeGroups]
     const float *bias;  // or null
     int dim, lanes;     // lanes of a row, log2, 6 at most
+    InitArgs init;
 };
 // of a row, in each of its lanes
 template <class T>
@@ -153,6 +163,7 @@ __global__ __launch_bounds__(256) void k_ranges(RangeArgs<T> a) {
             const uint32_t m = largest(a.h + r * a.ldh, a.dim, l, a.lanes);
             if (l == 0) a.power[r] = m ? unit_power(m) : kNoPower;
         }
+        if (blockIdx.x == kRangeGroups - 1) init_scalars(a.init);
         return;
     }
     uint32_t m = 0;
@@ -167,14 +178,25 @@ __global__ __launch_bounds__(256) void k_ranges(RangeArgs<T> a) {
         const uint32_t v = __shfl_xor(m, o, 64);
         m = v > m ? v : m;
     }
-    // one atomic a workgroup: they are taken one after the other (8192 of them: 150 us)
     __shared__ uint32_t tops[4];
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 4; ++w) m = tops[w] > m ? tops[w] : m;
-        if (m) atomicMax(a.amax_w, m);
+        a.tops[blockIdx.x] = m;
     }
+}
+// The largest of k_ranges' workgroups, in each lane of a workgroup.
+__device__ __forceinline__ uint32_t largest_of(const uint32_t *tops) {
+    __shared__ uint32_t waves[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < kRangeGroups; k += 256) m = max(m, tops[k + threadIdx.x]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return max(max(waves[0], waves[1]), max(waves[2], waves[3]));
 }
 
 // An operand's 16-bit form: T itself, or pairs (mm16.h) of a float times its scale.
@@ -190,26 +212,31 @@ struct Planes<float> {
 };
 
 // rows x dim -> rows of kp values (or pairs), zeros past dim and in rows whose bias is -inf.  2^lanes lanes a
-// row, 8 values each at a time.  Pairs are scaled by two to their row's power; `entries`: by that of the table's
-// largest value, or the entry's own.
+// row, 8 values each at a time.  Pairs are scaled by two to their row's power; `tops` (of k_ranges): by that of the
+// table's largest value, or the entry's own, of which the call's scalars are told.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out,
-                                              int kp, int lanes, const int *power, Scalars *entries, const float *bias) {
+                                              int kp, int lanes, const int *power, const uint32_t *tops, Scalars *call,
+                                              const float *bias) {
     typedef typename Planes<T>::type P;
     constexpr int N = Planes<T>::count;
     const int per = 256 >> lanes, l = threadIdx.x & ((1 << lanes) - 1);
     int common = 0;
     if constexpr (N == 2)
-        if (entries) common = unit_power(entries->amax_w);
+        if (tops) {
+            const uint32_t m = largest_of(tops);
+            common = unit_power(m);
+            if (blockIdx.x == 0 && threadIdx.x == 0) call->amax_w = m;
+        }
     for (size_t r = (size_t)blockIdx.x * per + (threadIdx.x >> lanes); r < rows; r += (size_t)gridDim.x * per) {
         const bool keep = !bias || bias[r] != -INFINITY;
         float sc = 1.f;
         if constexpr (N == 2) {
             int k = min(power[r], 120);
-            if (entries && !own_power(power[r], common))
+            if (tops && !own_power(power[r], common))
                 k = common;
-            else if (entries && l == 0)
-                entries->wide = 1;
+            else if (tops && l == 0)
+                call->wide = 1;
             sc = ldexpf(1.f, k);
         }
         for (int c = l * 8; c < kp; c += 8 << lanes) {
@@ -233,12 +260,12 @@ __global__ __launch_bounds__(256) void k_pack(const T *x, size_t rows, int dim, 
     }
 }
 template <class T>
-void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const int *power, Scalars *entries,
-          const float *bias, hipStream_t s) {
+void pack(const T *x, size_t rows, int dim, size_t ld, typename Planes<T>::type *out, int kp, const int *power, const uint32_t *tops,
+          Scalars *call, const float *bias, hipStream_t s) {
     const int lanes = lanes_log2(kp / 8);
     const size_t wgs = (rows + (256 >> lanes) - 1) >> (8 - lanes);
     const uint32_t grid = (uint32_t)(wgs < 8192 ? wgs : 8192);
-    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, power, entries, bias);
+    k_pack<T><<<grid, 256, 0, s>>>(x, rows, dim, ld, out, kp, lanes, power, tops, call, bias);
 }
 
 // rows x dim -> dim rows of rp values (or pairs), zeros past rows and where G's row is zeros.  What G's row was
@@ -869,6 +896,7 @@ struct Parts {
     uint32_t *marks;
     int *power, *entry_power;  // of the rows of h, of the table's (k_ranges)
     int *boost;
+    uint32_t *tops;
     void *hp, *wp, *ht, *g;
 };
 
@@ -888,7 +916,10 @@ inline Parts carve(Carver &c, const Sizes &z) {
         return p;
     }
     if (planes == 2 || (z.grad && z.dtype == VHIP_DTYPE_F16)) p.power = c.take<int>(z.rows);
-    if (planes == 2) p.entry_power = c.take<int>(z.table);
+    if (planes == 2) {
+        p.entry_power = c.take<int>(z.table);
+        p.tops = c.take<uint32_t>(kRangeGroups);
+    }
     p.hp = c.take<uint16_t>(planes * z.piece_rows * z.kp);
     p.wp = c.take<uint16_t>(planes * z.table * z.kp);
     if (z.grad) {
@@ -960,16 +991,19 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
     const int dim = (int)z.dim, table = (int)z.table;
     const T *h = (const T *)c.h, *w = (const T *)c.table;
 
-    if (kSplit || z.grad) k_xent_init<<<1, 256, 0, s>>>(p.sc, c.row_weight, (int)z.rows, c.scale);
+    const InitArgs init{p.sc, c.row_weight, (int)z.rows, c.scale};
     if (p.power) {
         const int lanes = lanes_log2((z.dim + 3) / 4);
-        const RangeArgs<T> m{h, w, z.rows, z.table, c.ldh, c.ldt, p.power, p.entry_power, &p.sc->amax_w, (const float *)c.bias, dim, lanes < 6 ? lanes : 6};
-        k_ranges<T><<<dim3(1024, kSplit ? 2 : 1), 256, 0, s>>>(m);
+        const RangeArgs<T> m{h, w, z.rows, z.table, c.ldh, c.ldt, p.power, p.entry_power, p.tops, (const float *)c.bias, dim,
+                             lanes < 6 ? lanes : 6, init};
+        k_ranges<T><<<dim3(kRangeGroups, kSplit ? 2 : 1), 256, 0, s>>>(m);
+    } else if (z.grad) {
+        k_xent_init<<<1, 256, 0, s>>>(init);
     }
     const P *wp = (const P *)c.table;
     size_t ldw = c.ldt;
     if (!direct<T>(c.table, c.ldt, z.dim) || (z.grad && c.bias)) {
-        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, p.entry_power, p.sc, (const float *)c.bias, s);
+        pack<T>(w, z.table, dim, c.ldt, (P *)p.wp, (int)z.kp, p.entry_power, p.tops, p.sc, (const float *)c.bias, s);
         wp = (const P *)p.wp;
         ldw = z.kp * Planes<T>::count;
     }
@@ -982,7 +1016,7 @@ int xent(const Call &c, const Sizes &z, const Parts &p, hipStream_t s) {
         const P *hp = (const P *)(const void *)hr;
         size_t ldh = c.ldh;
         if (!direct<T>(hr, c.ldh, z.dim)) {
-            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, power, nullptr, nullptr, s);
+            pack<T>(hr, rows, dim, c.ldh, (P *)p.hp, (int)z.kp, power, nullptr, nullptr, nullptr, s);
             hp = (const P *)p.hp;
             ldh = z.kp * Planes<T>::count;
         }

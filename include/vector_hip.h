@@ -433,7 +433,8 @@ int vhip_softmax_xent(int ordinal, int dtype, const void *h, size_t rows, size_t
                       float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* The same with the gradients of sum_t row_weight_t loss_t (row_weight NULL: all 1) for h and for the table
  * (either may be NULL).  A row with a negative target has no part in them, whatever h holds there, and
- * neither has one whose loss is +inf as above.  Rows are taken in pieces that keep the working memory for the
+ * neither has one whose loss is +inf as above; a target past the table makes its row's gradient and the whole
+ * table's NaN.  Rows are taken in pieces that keep the working memory for the
  * logits' gradient, or for what the loss alone keeps of its rows, and for copies of the rows below 4 GiB; the
  * environment variable VHIP_XENT_PIECE_BYTES sets another limit. */
 int vhip_softmax_xent_grad(int ordinal, int dtype, const void *h, size_t rows, size_t ldh, const void *table,

@@ -28,10 +28,10 @@ __device__ __forceinline__ float exp_fine(float x) {
 }
 
 // Whether a call takes this way.  32-bit rows, tiles / this way in us, loss and with gradients: 16 x 10000 x 128
-// 37, 82 / 15, 27; 64 x 10000 x 768 61, 111 / 30, 82; 64 x 200003 x 300 256, 538 / 124, 451; 64 x 131072 x 1024
-// 469, 804 / 331, 815; 100 x 50000 x 512 93, 201 / 115, 350.  16-bit rows, whose tables the tiles read as they
-// are: 16 x 10000 x 128 16, 43 / 14, 25; 32 x 10000 x 768 19, 59 / 15, 54; 64 x 10000 x 768 19, 61 / 18, 72;
-// 16 x 131072 x 1024 53, 236 / 69, 288: only while launches are what counts.
+// 26, 72 / 15, 25; 64 x 10000 x 768 50, 101 / 27, 78; 64 x 200003 x 300 272, 536 / 119, 423; 64 x 131072 x 1024
+// 475, 817 / 263, 738; 100 x 50000 x 512 90, 208 / 115, 350.  16-bit rows, whose tables the tiles read as they
+// are: 16 x 10000 x 128 15, 42 / 14, 24; 32 x 10000 x 768 17, 56 / 15, 50; 64 x 10000 x 768 18, 58 / 17, 68;
+// 16 x 131072 x 1024 55, 230 / 69, 286: only while launches are what counts.
 constexpr size_t kSmallRows = 64, kSmallWork16 = 250'000'000;
 inline bool few_rows(int dtype, size_t rows, size_t table, size_t dim) {
     return rows <= kSmallRows && (dtype == VHIP_DTYPE_F32 || rows * table * dim <= kSmallWork16);
@@ -40,7 +40,8 @@ inline bool few_rows(int dtype, size_t rows, size_t table, size_t dim) {
 // Entries of a workgroup's turn.  The rows are read from the caches again for each turn: from 17 rows on with
 // more of them than of the table, so a turn takes 32 entries, where enough turns for every CU are left
 // (float32, 16 / 32 entries, us: 32 x 95296 x 731 129, 97; 64 x 95296 x 768 194, 148; 32 x 40000 x 768 52, 39;
-// 64 x 20000 x 256 24, 20; 17 x 10000 x 768 19, 20).
+// 64 x 20000 x 256 24, 20; 17 x 10000 x 768 19, 20; bfloat16: 40 x 30000 x 200 16.0, 14.7; 17 x 200000 x 64 20.7, 19.7;
+// 32 x 100000 x 64 15.8, 14.9; up to 20,000 entries both are the time of the call).
 inline size_t small_turn(size_t rows, size_t table) { return rows > 16 && table >= 8192 ? 32 : 16; }
 
 // Values of one lane in a K step of the logits.

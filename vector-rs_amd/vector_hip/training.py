@@ -210,7 +210,8 @@ def _xent_args(h, table, target, bias):
 def softmax_xent(h, table, target, scale: float = 1.0, bias=None):
     """(loss, lse) of the rows of h [rows, dim] against every row of table [n, dim], float32 each:
     z = scale h table^T + bias, lse = log sum exp z, loss = lse - z[target].  target is int64; a negative one
-    has loss 0.  bias (float32, constant) may hold -inf, which leaves an entry out."""
+    has loss 0, one past the table NaN.  bias (float32, constant) may hold -inf, which leaves an entry out; a row
+    whose target is left out has loss +inf."""
     rows, n, dim, ldh, ldt, device, code, lib, y, b = _xent_args(h, table, target, bias)
     _no_graph(lib, h, table, bias)
     loss, lse = h.new_empty((2, rows), dtype=lib.f32).unbind()
@@ -223,7 +224,9 @@ def softmax_xent(h, table, target, scale: float = 1.0, bias=None):
 
 def softmax_xent_grad(h, table, target, row_weight=None, scale: float = 1.0, bias=None):
     """(loss, lse, dh, dtable): softmax_xent with the gradients of sum(row_weight * loss) for h and the table,
-    in their type.  row_weight (float32) is 1 everywhere by default; 1 / (number of targets) gives the mean."""
+    in their type.  row_weight (float32) is 1 everywhere by default; 1 / (number of targets) gives the mean.
+    Rows with a negative target, and those with loss +inf, have no part in the gradients, whatever they hold; a
+    target past the table makes its row's gradient and the table's NaN."""
     rows, n, dim, ldh, ldt, device, code, lib, y, b = _xent_args(h, table, target, bias)
     c = None if row_weight is None else _vector("row_weight", row_weight, rows, device, lib.f32)
     loss, lse = h.new_empty((2, rows), dtype=lib.f32).unbind()
@@ -238,7 +241,8 @@ def softmax_xent_grad(h, table, target, row_weight=None, scale: float = 1.0, bia
 
 def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
     """`steps` Newton-Schulz steps on update [rows, cols], or on each matrix of a stack [count, rows, cols]:
-    X = M / (|M| + eps); A = X X^T; X <- a X + (b A + c A A) X.  The result has the update's type."""
+    X = M / (|M| + eps); A = X X^T; X <- a X + (b A + c A A) X.  The result has the update's type.  Coefficients
+    that could take a singular value past 2^30 are refused."""
     _on_gpu("update", update)
     if update.dim() not in (2, 3):
         raise InvalidConfig("update must be a matrix or a stack of matrices")

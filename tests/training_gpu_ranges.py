@@ -377,3 +377,40 @@ def test_orthogonalize_is_as_near_as_its_pairs(tr, rows, cols):
     want = base.ns_reference(m, 5, 1e-7)
     limit = 20 * float((pairs_model(m, 5) - want).norm()) + 4 * E * float(want.norm())
     assert float((tr.orthogonalize(m).double() - want).norm()) <= limit
+
+
+# ---- rows far from the origin ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [2, 3, 49, 300, 769, 1500, 4097, 9001, 20_001])
+@pytest.mark.parametrize("value", [1.9, 7.0, 1000.1, 1e4, -12345.67])
+def test_layer_norm_of_constant_rows(tr, dim, value):
+    """A mean that is off by d makes every deviation d; their own mean takes it out again, to 66 roundings."""
+    x = torch.full((5, dim), value, device="cuda")
+    y, mean, rstd = tr.layer_norm(x)
+    assert float(y.abs().max()) <= 66 * E * 64 * E * abs(value) * 317
+    assert float((mean.double() - x[0, 0].double()).abs().max()) <= 2 * E * abs(value)
+    assert float((rstd.double() * 1e-5 ** 0.5 - 1).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("dim", [49, 300, 1500, 4097, 9001, 20_001])
+@pytest.mark.parametrize("offset", [100.0, 1e4, -1e5])
+def test_layer_norm_of_rows_with_a_large_mean(tr, dim, offset):
+    """Deviations from a mean nearby are exact; what is left of the mean's error is 66 roundings of 64 of it."""
+    x = normal(1, 40, dim) + offset
+    y, mean, rstd = tr.layer_norm(x)
+    ry, rm, rr, _ = base.ln_reference(x, None, None, 1e-5)
+    left = (66 * E * 64 * E * abs(offset) + 2 * E) * rr
+    within(y, ry, left[:, None] + 70 * E * ry.abs() + 2 * E)
+    within(mean, rm, 2 * E * rm.abs())
+    within(rstd, rr, 70 * E * rr)
+
+
+@pytest.mark.parametrize("dim", [5, 300, 1500, 9001, 20_001])
+def test_layer_norm_of_rows_that_are_not_finite(tr, dim):
+    """NaN and infinity reach y and the scale (and the mean), and no other row."""
+    x = normal(2, 5, dim)
+    x[1, dim // 2] = math.nan
+    x[3, dim - 1] = math.inf
+    y, mean, rstd = tr.layer_norm(x)
+    assert y[1::2].isnan().all() and rstd[1::2].isnan().all() and not mean[1::2].isfinite().any()
+    same(tr.layer_norm(x[::2].contiguous()), (y[::2], mean[::2], rstd[::2]))

@@ -6,7 +6,9 @@
 //
 // Both passes are bound by memory.  A row is held in the registers of the lanes that own it, so x (and dy)
 // are read once: the variance is the mean of squares about the mean, not a difference of two sums, at no
-// further read.  Rows of up to 4 vectors a lane belong to one wave (no barrier, four rows a workgroup),
+// further read.  The mean is rounded (values near 10^4: by 10^-3, a third of y where all are equal and eps is 10^-5), so
+// the deviations from it are summed beside their squares, and their own mean, d, comes off:
+// mu + d, sum (x - mu)^2 / D - d^2, y = (x - mu - d) r g + b.  Rows of up to 4 vectors a lane belong to one wave (no barrier, four rows a workgroup),
 // longer ones to a workgroup of 4 or 16 waves; rows past that are walked in three passes.  All sums are
 // in 32 bits.
 //
@@ -39,9 +41,9 @@ __device__ __forceinline__ void store_vec(T *row, int c, int dim, const float (&
         store_any<N>(row + c, v);
 }
 
-// Sum of one (two) value(s) over the G lanes that hold a row: a wave by itself, or through LDS.  `slot`
-// alternates between two buffers, so one barrier a sum is enough: a buffer is written again only after the
-// barrier of the sum between.
+// Sum of a value over the G lanes that hold a row: a wave by itself, or through LDS.  `slot` alternates between
+// two buffers, so one barrier a sum is enough: a buffer is written again only after the barrier of the sum
+// between.  row_sums: of two values, in a buffer of their own.
 template <int G>
 __device__ __forceinline__ float row_sum(float x, float *lds, int slot) {
     x = lane_sum<64>(x);
@@ -57,6 +59,30 @@ __device__ __forceinline__ float row_sum(float x, float *lds, int slot) {
     return x;
 }
 
+template <int G>
+__device__ __forceinline__ float2 row_sums(float x, float y, float2 *lds) {
+    x = lane_sum<64>(x);
+    y = lane_sum<64>(y);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(x, y);
+        __syncthreads();
+        x = y = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            x += lds[w].x;
+            y += lds[w].y;
+        }
+    }
+    return make_float2(x, y);
+}
+
+// The mean's correction d and 1 / std from the sums of deviations and of their squares.
+__device__ __forceinline__ float2 row_scale(float2 s, float n, float eps) {
+    const float d = s.x * n, v = fmaf(-d, d, s.y * n);
+    return make_float2(d, 1.f / sqrtf((v < 0.f ? 0.f : v) + eps));  // NaN stays
+}
+
 struct FwdArgs {
     const void *x, *weight, *bias;
     void *y;
@@ -69,7 +95,8 @@ struct FwdArgs {
 template <class T, class P, int G, bool TAIL, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
     constexpr int B = G > 256 ? G : 256, R = B / G, VEC = kVec<T>;
-    __shared__ float lds[2 * (G / 64)];
+    __shared__ float lds[G / 64];
+    __shared__ float2 lds2[G / 64];
     const size_t row = (size_t)blockIdx.x * R + threadIdx.x / G;
     if (row >= a.rows) return;  // G lanes at once: whole waves, and G > 64 has one row a workgroup
     const int t = threadIdx.x % G;
@@ -88,6 +115,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
     }
     const float n = 1.f / (float)a.dim;
     const float mu = row_sum<G>(s, lds, 0) * n;
+    float s2 = 0.f;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -96,11 +124,13 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 v[i][e] = TAIL && c + e >= a.dim ? 0.f : v[i][e] - mu;
-                s = fmaf(v[i][e], v[i][e], s);
+                s += v[i][e];
+                s2 = fmaf(v[i][e], v[i][e], s2);
             }
         }
     }
-    const float r = 1.f / sqrtf(row_sum<G>(s, lds, 1) * n + a.eps);
+    const float2 sc = row_scale(row_sums<G>(s, s2, lds2), n, a.eps);
+    const float d = sc.x, r = sc.y;
     T *y = (T *)a.y + row * a.ldy;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -108,7 +138,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
         if (c < a.dim) {
             float p[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[i][e] *= r;
+            for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - d) * r;
             if (w) {
                 load_vec<VEC, TAIL>(p, w, c, a.dim);
 #pragma unroll
@@ -123,7 +153,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
         }
     }
     if (t == 0) {
-        if (a.mean) a.mean[row] = mu;
+        if (a.mean) a.mean[row] = mu + d;
         if (a.rstd) a.rstd[row] = r;
     }
 }
@@ -131,7 +161,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_ln_forward(FwdArgs a) {
 // Rows of any length, one workgroup of 1024 each: the second and third walk find the row in the L2.
 template <class T, class P>
 __global__ __launch_bounds__(1024) void k_ln_forward_long(FwdArgs a) {
-    __shared__ float lds[2 * 16];
+    __shared__ float lds[16];
+    __shared__ float2 lds2[16];
     const size_t row = blockIdx.x;
     const T *x = (const T *)a.x + row * a.ldx;
     const P *w = (const P *)a.weight, *b = (const P *)a.bias;
@@ -140,20 +171,23 @@ __global__ __launch_bounds__(1024) void k_ln_forward_long(FwdArgs a) {
     float s = 0.f;
     for (int c = threadIdx.x; c < a.dim; c += 1024) s += (float)x[c];
     const float mu = row_sum<1024>(s, lds, 0) * n;
+    float s2 = 0.f;
     s = 0.f;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        const float d = (float)x[c] - mu;
-        s = fmaf(d, d, s);
+        const float v = (float)x[c] - mu;
+        s += v;
+        s2 = fmaf(v, v, s2);
     }
-    const float r = 1.f / sqrtf(row_sum<1024>(s, lds, 1) * n + a.eps);
+    const float2 sc = row_scale(row_sums<1024>(s, s2, lds2), n, a.eps);
+    const float d = sc.x, r = sc.y;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        float v = ((float)x[c] - mu) * r;
+        float v = ((float)x[c] - mu - d) * r;
         if (w) v *= (float)w[c];
         if (b) v += (float)b[c];
         y[c] = (T)v;
     }
     if (threadIdx.x == 0) {
-        if (a.mean) a.mean[row] = mu;
+        if (a.mean) a.mean[row] = mu + d;
         if (a.rstd) a.rstd[row] = r;
     }
 }

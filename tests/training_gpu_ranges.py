@@ -414,3 +414,53 @@ def test_layer_norm_of_rows_that_are_not_finite(tr, dim):
     y, mean, rstd = tr.layer_norm(x)
     assert y[1::2].isnan().all() and rstd[1::2].isnan().all() and not mean[1::2].isfinite().any()
     same(tr.layer_norm(x[::2].contiguous()), (y[::2], mean[::2], rstd[::2]))
+
+
+# ---- the largest and the narrowest sizes -------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,table,dim,dtype", [(70, 100, 65_536, "f32"), (70, 100, 65_536, "bf16"), (9, 40, 65_536, "f32"), (3, 40, 65_535, "f16"),
+                                                  (65, (1 << 22) - 64, 3, "f32"), (65, (1 << 22) - 64, 8, "f16"), (2, (1 << 22) - 65, 5, "bf16")])
+def test_softmax_xent_at_the_limits(tr, rows, table, dim, dtype):
+    h, w, y = xent_inputs(rows, table, dim, dtype)
+    if dim > 1000:
+        h = h / 8  # + 0.1 w of the target is a logit of thousands
+    xent_check(tr.softmax_xent_grad(h, w, y), h, w, y, 1.0)
+    xent_check((*tr.softmax_xent(h, w, y), None, None), h, w, y, 1.0)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 65_536), (65_536, 1), (2, 40_000), (65_535, 3), (65_536, 40)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_orthogonalize_at_the_limits(tr, rows, cols, dtype):
+    m = (0.01 * normal(5, rows, cols)).to(TYPES[dtype])
+    got, want = tr.orthogonalize(m), base.ns_reference(m, 5, 1e-7)
+    assert float((got.double() - want).norm()) <= base.ns_tolerance(want, 5, min(rows, cols), 2 * UNIT[m.dtype])
+
+
+def test_orthogonalize_many_small_matrices(tr):
+    m = normal(6, 65_535, 3, 5)
+    got = tr.orthogonalize(m)
+    for i in (0, 1, 32_768, 65_534):
+        want = base.ns_reference(m[i], 5, 1e-7)
+        assert float((got[i].double() - want).norm()) <= base.ns_tolerance(want, 5, 3, 2 * E)
+
+
+@pytest.mark.parametrize("rows,dim", [(3, (1 << 20) + 1), (1, 5_000_000), (300_000, 3), (1_000_000, 1)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_layer_norm_at_the_limits(tr, rows, dim, dtype):
+    """Chains of a thousandth of a long row, and of a 512th of many rows."""
+    x = (normal(1, rows, dim) + 0.25).to(TYPES[dtype])
+    w, b = 1 + 0.1 * normal(2, dim), 0.1 * normal(3, dim)
+    y, mean, rstd = tr.layer_norm(x, w, b)
+    ry, rm, rr, xh = base.ln_reference(x, w, b, 1e-5)
+    chain = (64 + dim / 1024) * E
+    within(rstd, rr, rr * 2 * chain)
+    within(y, ry, UNIT[x.dtype] * ry.abs() + TINY[x.dtype] + 4 * chain * (1 + ry.abs()))
+    dy = normal(4, rows, dim).to(x.dtype)
+    dx, dw, db = tr.layer_norm_backward(dy, x, w, mean, rstd)
+    a = dy.double() * w.double()
+    size = a.abs() + a.abs().mean(1, keepdim=True) + xh.abs() * (a * xh).abs().mean(1, keepdim=True)
+    want = rr[:, None] * (a - a.mean(1, keepdim=True) - xh * (a * xh).mean(1, keepdim=True))
+    within(dx, want, UNIT[x.dtype] * want.abs() + TINY[x.dtype] + 8 * chain * rr[:, None] * (1 + xh.abs()) * size)
+    rowchain = (rows / 512 + 160) * E
+    within(db, dy.double().sum(0), E * dy.double().sum(0).abs() + rowchain * dy.double().abs().sum(0))
+    within(dw, (dy.double() * xh).sum(0), E * (dy.double() * xh).sum(0).abs() + 2 * rowchain * (dy.double().abs() * (0.3 * rr[:, None] + xh.abs())).sum(0))

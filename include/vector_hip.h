@@ -451,6 +451,30 @@ int vhip_orthogonalize(int ordinal, int dtype, const void *in, size_t count, siz
                        size_t stride_in, int steps, float a, float b, float c, float eps, void *out, size_t ld_out,
                        size_t stride_out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- attention and what a training step adds (no reference counterpart) -----------------
+ * The operators of an encoder between its projections, in the manner of the training operators above.
+ * Rows of heads: element (token t, head h, column c) is at data + t * token + h * head + c elements, the
+ * columns contiguous; no two rows overlap, tokens are at most 2^23 elements apart. */
+typedef struct vhip_heads {
+    void *data; /* an input is only read */
+    size_t token, head;
+} vhip_heads;
+
+/* Softmax attention over `sequences` packed sequences: sequence s has the queries offsets[s] .. offsets[s + 1] and
+ * the keys and values key_offsets[s] .. key_offsets[s + 1] (key_offsets NULL: the queries' own).  Offsets are
+ * device memory, sequences + 1 values that do not fall.  heads is a multiple of kv_heads: query head h reads
+ * key head h / (heads / kv_heads).  With `causal` the last query of a sequence sees all its keys and each query before it
+ * one fewer, so queries may be the last tokens of a longer text.
+ *   s_rj = scale <q_r, k_j>,  lse_r = log sum_j exp s_rj,  out_r = sum_j exp(s_rj - lse_r) v_j
+ * A row that sees no key has out 0 and lse -inf, and so has one of no sequence.  lse ([tokens, heads], may be
+ * NULL).  dim <= 128, tokens * heads <= 2^30. */
+size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
+                                size_t sequences);
+int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads *k, const vhip_heads *v, size_t tokens,
+                   size_t key_tokens, size_t heads, size_t kv_heads, size_t dim, const int64_t *offsets,
+                   const int64_t *key_offsets, size_t sequences, int causal, float scale, const vhip_heads *out, float *lse,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -1,0 +1,20 @@
+"""Runs encoder_gpu_cases.py in one process in which torch comes before the library (the two have to share one HIP
+runtime), apart from the process that runs the other GPU tests."""
+import os
+import re
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+pytestmark = pytest.mark.gpu
+
+
+def test_encoder_operators():
+    args = ["-m", "pytest", os.path.join("tests", "encoder_gpu_cases.py"), "-m", "gpu", "-x", "-q", "--tb=short", "-p", "no:cacheprovider"]
+    p = subprocess.run([sys.executable, "-u"] + args, cwd=ROOT, capture_output=True, text=True, timeout=600)
+    print(p.stdout[-20000:], flush=True)
+    assert p.returncode == 0, p.stdout[-4000:] + p.stderr[-4000:]
+    assert re.search(r"\d+ passed", p.stdout) and "skipped" not in p.stdout

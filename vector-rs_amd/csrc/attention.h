@@ -1,0 +1,267 @@
+// attention.h -- what the passes of attention over packed sequences share: which rows a workgroup has, tiles of
+// rows in LDS, and products of them on the matrix cores.
+//
+// Rows.  A query row is a (token, head).  The heads of a group read the same keys and values, so a tile holds
+// consecutive packed rows of one sequence and one key head, packed row r being token r / group, head r % group of the
+// group: keys are read once for the whole group, and a single token of many heads still fills a tile.
+//
+// Products.  All are 32 x 32 blocks (32x32x16 of 16-bit values, 32x32x2 of 32-bit ones), whose result has column l % 32
+// in lane l and, in its register i, row 8 (i / 4) + 4 (l / 32) + i % 4.  Scores are made transposed to what multiplies
+// them next: with S^T = K Q^T a lane has one query row and 16 of a block's keys, so a softmax needs one exchange between
+// the lanes' halves, its statistics are a lane's own scalars, and the values that a lane holds are the ones that it
+// has to give as operand of O^T = V^T P^T: the order of keys in that product is free as long as both operands have
+// the same, so the operand from LDS is read in the order in which registers hold the other (no data moves between
+// lanes).
+//
+// Tiles in LDS are rows of DP values as chunks of 16 bytes, chunk c of row r at slot c ^ swz(r): both the reads of a
+// chunk of 32 rows and the transposing reads (4 rows x 32 bytes to 16 lanes) then spread over all banks.
+#pragma once
+
+#include <climits>
+
+#include "mm16.h"
+
+namespace vh {
+namespace attn {
+
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// ---- which rows --------------------------------------------------------------------------------
+
+// Sequences in one array of `tokens` rows.  The rows before the first and after the last one count as two more
+// sequences without a counterpart on the other side.  Offsets are device data: each is clamped to the array, so wrong
+// ones give wrong rows and no access out of bounds.
+struct Packed {
+    const int64_t *offsets;
+    int64_t tokens;
+    int count;  // sequences
+};
+
+struct Span {
+    int64_t begin;
+    int len;
+};
+
+__device__ __forceinline__ int64_t packed_bound(const Packed &p, int s) {
+    if (s <= 0) return 0;
+    if (s > p.count + 1) return p.tokens;
+    const int64_t v = p.offsets[s - 1];
+    return v < 0 ? 0 : v > p.tokens ? p.tokens : v;
+}
+__device__ __forceinline__ Span packed_span(const Packed &p, int s) {
+    const int64_t b = packed_bound(p, s), e = packed_bound(p, s + 1);
+    return {b, e > b ? (int)(e - b) : 0};
+}
+
+// Workgroup `slot` of ceil-sized tiles of R rows (times `mult` for each token) without a list of them: sequence s has
+// the slots from floor(begin_s mult / R) + s on, which are as many as it has tiles or one more.  Each wave finds its
+// s by itself, 64 candidates a round.
+template <int R>
+__device__ __forceinline__ int64_t first_slot(const Packed &p, int s, int mult) {
+    return packed_bound(p, s) * mult / R + s;
+}
+inline int64_t slot_count(int64_t tokens, int64_t sequences, int64_t mult, int64_t R) { return tokens * mult / R + sequences + 2; }
+
+struct Place {
+    int seq;   // 0 and count + 1: rows of no sequence
+    int tile;  // of that sequence; may be past its last
+};
+template <int R>
+__device__ __forceinline__ Place find_tile(const Packed &p, int mult, int64_t slot) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = p.count + 2;
+    for (int step = (hi + 63) / 64;; step = (step + 63) / 64) {
+        const int s = lo + lane * step;
+        const uint64_t in = __ballot(s < hi && first_slot<R>(p, s, mult) <= slot);
+        const int n = in ? __popcll(in) : 1;
+        lo += (n - 1) * step;
+        hi = hi < lo + step ? hi : lo + step;
+        if (step == 1) break;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int64_t t = slot - first_slot<R>(p, lo, mult);
+    return {lo, __builtin_amdgcn_readfirstlane((int)(t < 0 ? INT_MAX : t > INT_MAX ? INT_MAX : t))};
+}
+
+// r / group, quickly where group is a power of two.
+struct Group {
+    int size, shift;  // shift < 0: not a power of two
+    __device__ __forceinline__ int token(int r) const { return shift >= 0 ? r >> shift : (int)((unsigned)r / (unsigned)size); }
+};
+
+// Rows of one array: element (t, h, c) at t * token + h * head + c.
+struct Heads {
+    char *data;
+    size_t token, head;  // bytes
+};
+
+// ---- tiles in LDS ------------------------------------------------------------------------------
+
+constexpr int swz_of(int row_bytes, int r) {
+    return row_bytes % 256 == 0 ? ((r & 7) << 1) | ((r >> 3) & 1)
+           : row_bytes % 128 == 0 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1)
+                                  : (r >> 2) & 3;
+}
+
+// A tile of ROWS rows of DP values that NW waves load.
+template <class T, int DP, int ROWS, int NW, bool DMA>
+struct Tile {
+    static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, N = ROWS * CH / (NW * 64);
+    static constexpr int kBytes = ROWS * RB;
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    static_assert(N * NW * 64 == ROWS * CH, "whole loads");
+    static constexpr int swz(int r) { return swz_of(RB, r); }
+
+    static __device__ __forceinline__ void spot(int i, int &row, int &chunk) {
+        const int n = (i * NW + (int)(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63);
+        row = n / CH;
+        chunk = (n % CH) ^ swz(row);
+    }
+    // Loads the tile to `to`: row r is at base + at(r) bytes (uniform base), of `dim` values.  By DMA rows are
+    // whole chunks at 16-byte addresses, and chunks past the last are copies of it (the other operand has zeros
+    // there, or the result is not used); otherwise values come one vector at a time, zeros past dim.
+    template <class At>
+    static __device__ __forceinline__ void load(const char *base, const At &at, int dim, char *to) {
+        if constexpr (DMA) {
+            const int last = dim * (int)sizeof(T) / 16 - 1;
+            const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)to +
+                                                                (threadIdx.x >> 6) * 1024);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int r, c;
+                spot(i, r, c);
+                dma_lds16_at(base, (uint32_t)at(r) + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int r, c;
+                spot(i, r, c);
+                const auto v = load_row<VEC>((const T *)(base + (uint32_t)at(r)), c * VEC, dim);
+                *(Pack<T, VEC> *)(to + ((i * NW + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) * 16) = v;
+            }
+        }
+    }
+};
+
+// ---- fragments and products --------------------------------------------------------------------
+
+template <class T>
+struct Frag;  // 16 bytes of a row: operand of a step of 32 bytes of k, half a step from each half of the lanes
+template <>
+struct Frag<half_t> {
+    typedef MmVec<half_t>::v8 type;
+};
+template <>
+struct Frag<bf16_t> {
+    typedef MmVec<bf16_t>::v8 type;
+};
+template <>
+struct Frag<float> {
+    typedef floatx4_t type;
+};
+
+__device__ __forceinline__ floatx16_t mma(MmVec<half_t>::v8 a, MmVec<half_t>::v8 b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16_t mma(MmVec<bf16_t>::v8 a, MmVec<bf16_t>::v8 b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16_t mma(floatx4_t a, floatx4_t b, floatx16_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ constexpr int row_of(int i) { return 8 * (i / 4) + i % 4; }  // plus 4 (lane / 32)
+
+// Chunk 2 ks + lane / 32 of row r0 + lane % 32 (r0 a multiple of 32).
+template <class T, int RB>
+__device__ __forceinline__ typename Frag<T>::type rows_frag(const char *tile, int r0, int ks, int lane) {
+    const int r = lane & 31, x = swz_of(RB, r) ^ (lane >> 5);
+    return *(const typename Frag<T>::type *)(tile + r * RB + ((2 * ks) ^ x) * 16 + r0 * RB);
+}
+
+// c += A^T B, where A's rows r0 .. r0 + 31 are the tile's, its columns 32 dt .. 32 dt + 31, and B is in the lanes'
+// registers as a product left it.
+template <class T, int RB, class V>
+__device__ __forceinline__ floatx16_t mma_cols(const char *tile, int r0, int dt, const V *b, floatx16_t c, int lane) {
+    if constexpr (sizeof(T) == 2) {
+        typedef typename MmVec<T>::v4 v4;
+        typedef typename MmVec<T>::v8 v8;
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const int g = lane >> 4, i = lane & 15, r = 4 * (g >> 1) + (i >> 2);
+        const int x = (2 * (g & 1) + ((i & 3) >> 1)) ^ swz_of(RB, r);
+        const char *p = tile + r * RB + (i & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const char *q = p + (r0 + 16 * k) * RB;
+            const v4 lo = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q + ((4 * dt) ^ x) * 16)));
+            const v4 hi = __builtin_bit_cast(
+                v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q + 8 * RB + ((4 * dt) ^ x ^ swz_of(RB, 8)) * 16)));
+            c = mma(v8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), b[k], c);
+        }
+    } else {
+        const int h = lane >> 5, x = ((lane & 31) >> 2) ^ swz_of(RB, 4 * h);
+        const char *p = tile + (r0 + 4 * h) * RB + (lane & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float a = *(const float *)(p + row_of(i) * RB + ((8 * dt) ^ x ^ swz_of(RB, row_of(i))) * 16);
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b[i / 4][i % 4], c, 0, 0, 0);
+        }
+    }
+    return c;
+}
+
+// The 16 values of a block as that operand: two of 8 in 16 bits, four of 4 in 32.
+template <class T>
+constexpr int kOps = sizeof(T) == 2 ? 2 : 4;
+template <class T>
+__device__ __forceinline__ void to_operand(const floatx16_t &v, typename Frag<T>::type (&o)[kOps<T>]) {
+    constexpr int E = 16 / kOps<T>;
+#pragma unroll
+    for (int k = 0; k < kOps<T>; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[k][e] = (T)v[k * E + e];
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// Writes a lane's part of a transposed result: its row's values 32 dt + 8 (i / 4) + 4 (lane / 32) + i % 4.
+template <class T, int DT, class F>
+__device__ __forceinline__ void store_cols(T *row, const floatx16_t (&acc)[DT], int dim, int lane, const F &f) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int c = 32 * dt + 8 * b + 4 * (lane >> 5);
+            Pack<T, 4> v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v.v[e] = (T)f(acc[dt][4 * b + e]);
+            if (c < dim) store_row<4>(row, c, dim, v);
+        }
+}
+
+// All DMAs of this wave have landed, and everyone is past what it read before.
+__device__ __forceinline__ void tiles_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+// Arguments that all passes check alike.
+struct Shape {
+    size_t tokens, key_tokens, heads, kv_heads, dim, sequences;
+};
+int check_shape(int dtype, const Shape &s, const int64_t *offsets, const int64_t *key_offsets, float scale);
+int check_heads(const char *name, const vhip_heads *a, int dtype, size_t tokens, size_t heads, size_t dim);
+// Whether rows can be loaded by 16-byte chunks.
+bool whole_chunks(const vhip_heads *a, int dtype, size_t dim);
+Heads to_heads(const vhip_heads *a, int dtype);
+
+}  // namespace attn
+}  // namespace vh

@@ -1,0 +1,321 @@
+// attention_forward.hip -- softmax attention of packed sequences with grouped heads.
+//
+//   s_rj = scale <q_r, k_j> over the keys j that row r sees,  lse_r = log sum_j exp s_rj,
+//   o_r = sum_j exp(s_rj - lse_r) v_j;  a row that sees no key has o = 0 and lse = -inf
+//
+// One pass over the keys: a workgroup has 128 packed rows (attention.h) of one sequence and key head, 32 to a wave,
+// and walks tiles of keys and values that come by DMA into the other of two buffers while one is multiplied. A
+// row's largest score m and sum l run along, in the scores' base-2 logarithms; the output and l are only scaled anew
+// once a row's m has grown by more than 2^8, so most tiles take no pass over the accumulators.
+#include <type_traits>
+
+#include "attention.h"
+
+namespace vh {
+namespace attn {
+namespace {
+
+struct FwdArgs {
+    Heads q, k, v, out;
+    float *lse;
+    Packed rows, keys;
+    Group group;
+    int heads, kv_heads, dim;
+    bool causal;
+    float scale;
+    int splits;     // parts of the keys, each a workgroup; more than one leave `part`, which k_attn_join adds up
+    float *part;    // [split][token][head][DP]: outputs over their row's own m
+    float2 *stats;  // [split][token][head]: m, l
+};
+
+constexpr int kBM = 128;
+
+// Keys of a tile: 64, or 32 where they have 32 bits (two buffers of K and V of 128 columns in 64 KB, two workgroups a CU).
+template <class T>
+constexpr int kBN = sizeof(T) == 2 ? 64 : 32;
+
+// Added to the exponents of float16's p, so that weights of 2^-20 of the largest still have all their bits: p <= 2^8
+// (see above) times this stays below 2^15.
+template <class T>
+constexpr float kShift = std::is_same<T, half_t>::value ? 6.f : 0.f;
+
+template <class T, int DP, bool DMA>
+__global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
+    constexpr int BN = kBN<T>, NS = BN / 32, RB = DP * (int)sizeof(T), KS = RB / 32, DT = DP / 32, VEC = 16 / (int)sizeof(T);
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, DP, BN, 4, DMA> KV;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][KV::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    const uint32_t id = blockIdx.x;
+    const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
+    const Place at = find_tile<kBM>(a.rows, a.group.size, id / a.kv_heads / a.splits);
+    const Span rows = packed_span(a.rows, at.seq);
+    const int n = rows.len * a.group.size;
+    if (at.tile >= (n + kBM - 1) / kBM) return;
+    const bool real = at.seq >= 1 && at.seq <= a.rows.count;
+    const Span keys = real ? packed_span(a.keys, at.seq) : Span{0, 0};
+    // the last tile of a sequence first: it sees the most keys
+    const int row0 = ((n + kBM - 1) / kBM - 1 - at.tile) * kBM;
+
+    // this lane's row, and how many keys it sees
+    const int r = row0 + wave * 32 + (lane & 31), rc = min(r, n - 1);
+    const int token = a.group.token(rc), head = kh * a.group.size + rc - token * a.group.size;
+    const int64_t row = rows.begin + token;
+    const int shift = keys.len - rows.len + 1;
+    const int sees = a.causal ? min(keys.len, max(0, token + shift)) : keys.len;
+    // how many the workgroup sees, and its part of them; what all rows of the wave see, and any of them
+    const int most = a.causal ? min(keys.len, max(0, a.group.token(min(row0 + kBM, n) - 1) + shift)) : keys.len;
+    const int tiles = (most + BN - 1) / BN, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
+    const int w0 = row0 + wave * 32, w1 = min(w0 + 32, n) - 1;
+    const int all = a.causal ? min(keys.len, max(0, a.group.token(min(w0, n - 1)) + shift)) : keys.len;
+    const int any = w0 >= n ? 0 : a.causal ? min(keys.len, max(0, a.group.token(w1) + shift)) : keys.len;
+
+    const char *kb = a.k.data + keys.begin * a.k.token + kh * a.k.head, *vb = a.v.data + keys.begin * a.v.token + kh * a.v.head;
+    auto load = [&](int t, int buf) {
+        const int last = keys.len - 1 - t * BN;
+        const uint32_t ks = (uint32_t)a.k.token, vs = (uint32_t)a.v.token;
+        KV::load(kb + (int64_t)t * BN * a.k.token, [&](int i) { return (uint32_t)min(i, last) * ks; }, a.dim, lds[buf][0]);
+        KV::load(vb + (int64_t)t * BN * a.v.token, [&](int i) { return (uint32_t)min(i, last) * vs; }, a.dim, lds[buf][1]);
+    };
+    if (t0 < t1) load(t0, 0);
+
+    frag q[KS];
+    {
+        const T *p = (const T *)(a.q.data + row * (int64_t)a.q.token + (int64_t)head * a.q.head);
+        const bool neg = a.scale < 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const auto x = load_row<VEC>(p, (2 * ks + half) * VEC, a.dim);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) q[ks][e] = neg ? -x.v[e] : x.v[e];
+        }
+    }
+    const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // s = 0 of a zero scale, and -inf of what is not seen
+
+    floatx16_t o[DT] = {};
+    float m = -INFINITY, l = 0.f;
+    for (int t = t0; t < t1; ++t) {
+        tiles_ready();
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
+        const int key0 = t * BN;
+        if (key0 >= any) continue;
+
+        floatx16_t s[NS] = {};
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[j] = mma(rows_frag<T, RB>(lds[buf][0], 32 * j, ks, lane), q[ks], s[j]);
+        if (key0 + BN > all) {
+            const int left = sees - key0 - 4 * half;
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * j + row_of(i) >= left) s[j][i] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
+        top = fmaxf(top, other_half(top)) * c;
+        if (__any(top > m + 8.f)) {
+            const float next = fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        const float base = kShift<T> - (m == -INFINITY ? 0.f : m);
+        float sum[4] = {};
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, base));
+                sum[i % 4] += s[j][i];
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            frag p[kOps<T>];
+            to_operand<T>(s[j], p);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = mma_cols<T, RB>(lds[buf][1], 32 * j, d, p, o[d], lane);
+        }
+    }
+    if (r >= n) return;
+    l += other_half(l);
+    const int64_t at_row = row * a.heads + head;
+    if (a.splits > 1) {
+        const int64_t i = ((int64_t)split * a.rows.tokens * a.heads) + at_row;
+        if (half == 0) a.stats[i] = make_float2(m, l);
+        if (m != -INFINITY) store_cols<float, DT>(a.part + i * DP, o, DP, lane, [](float x) { return x; });
+        return;
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (a.lse && half == 0) a.lse[at_row] = (m - kShift<T> + __builtin_amdgcn_logf(l)) * kLn2;
+    store_cols<T, DT>((T *)(a.out.data + row * (int64_t)a.out.token + (int64_t)head * a.out.head), o, a.dim, lane,
+                      [&](float x) { return x * f; });
+}
+
+// A row's parts: its largest m, and their outputs and sums over it.  A row of DP values has DP / 4 lanes.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
+    constexpr int L = DP / 4, R = 256 / L;  // 96 columns: 10 rows of 24 lanes, and 16 lanes without one
+    const int64_t all = a.rows.tokens * a.heads;
+    const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    if (threadIdx.x >= R * L || i >= all) return;
+    const int e = threadIdx.x % L * 4;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stats[s * all + i].x);
+    float l = 0.f, o[4] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 st = a.stats[s * all + i];
+        if (st.x == -INFINITY) continue;  // nothing is written there
+        const float f = __builtin_amdgcn_exp2f(st.x - m);
+        l = fmaf(st.y, f, l);
+        const Pack<float, 4> p = load_any<4>(a.part + (s * all + i) * DP + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(p.v[k], f, o[k]);
+    }
+    const int64_t token = i / a.heads, head = i % a.heads;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (a.lse && e == 0) a.lse[i] = (m - kShift<T> + __builtin_amdgcn_logf(l)) * kLn2;
+    Pack<T, 4> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v.v[k] = (T)(o[k] * f);
+    if (e < a.dim) store_row<4>((T *)(a.out.data + token * (int64_t)a.out.token + head * (int64_t)a.out.head), e, a.dim, v);
+}
+
+// Parts of the keys: enough workgroups for two rounds of the GPU where rows are few, none shorter than 256 keys of
+// an average sequence.  Lengths are on the device, so it goes by the sizes alone.
+int split_count(const Shape &s) {
+    const int64_t base = slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads;
+    const int64_t keys = (int64_t)(s.key_tokens / (s.sequences ? s.sequences : 1));
+    int64_t n = 1024 / (base ? base : 1);
+    if (n > keys / 256) n = keys / 256;
+    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+
+inline size_t padded(size_t dim) { return round_up(dim, 32); }
+
+template <class T, int DP>
+int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
+    if (dma)
+        k_attn_forward<T, DP, true><<<grid, 256, 0, s>>>(a);
+    else
+        k_attn_forward<T, DP, false><<<grid, 256, 0, s>>>(a);
+    if (a.splits > 1) {
+        constexpr int R = 256 / (DP / 4);
+        k_attn_join<T, DP><<<(uint32_t)ceil_div((size_t)a.rows.tokens * a.heads, R), 256, 0, s>>>(a);
+    }
+    return launch_status("attention launch");
+}
+template <class T>
+int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
+    switch (padded(a.dim)) {
+        case 32: return launch<T, 32>(a, dma, grid, s);
+        case 64: return launch<T, 64>(a, dma, grid, s);
+        case 96: return launch<T, 96>(a, dma, grid, s);
+        default: return launch<T, 128>(a, dma, grid, s);
+    }
+}
+
+}  // namespace
+
+int check_shape(int dtype, const Shape &s, const int64_t *offsets, const int64_t *key_offsets, float scale) {
+    if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
+    if (s.dim == 0 || s.dim > 128) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 128]");
+    if (s.heads == 0 || s.kv_heads == 0 || s.heads > 65536 || s.heads % s.kv_heads)
+        return set_error(VHIP_ERR_INVALID_CONFIG, "heads must be a multiple of kv_heads, in [1, 65536]");
+    if (!offsets) return set_error(VHIP_ERR_INVALID_CONFIG, "offsets are null");
+    if (!key_offsets && s.key_tokens != s.tokens)
+        return set_error(VHIP_ERR_INVALID_CONFIG, "without key_offsets there are as many keys as queries");
+    if (!(fabsf(scale) <= 3.4e38f)) return set_error(VHIP_ERR_INVALID_CONFIG, "scale must be finite");
+    if (s.tokens > (1u << 30) || s.key_tokens > (1u << 30) || s.sequences > (1u << 28) || s.tokens * s.heads > (1u << 30))
+        return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
+    return VHIP_OK;
+}
+
+int check_heads(const char *name, const vhip_heads *a, int dtype, size_t tokens, size_t heads, size_t dim) {
+    const std::string who(name);
+    if (!a || (tokens && !a->data)) return set_error(VHIP_ERR_INVALID_CONFIG, who + " is null");
+    if ((uintptr_t)a->data % dtype_size(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, who + " is not aligned to its type");
+    if ((tokens > 1 && a->token > kMmMaxLd) || (heads > 1 && a->head > ((size_t)1 << 40)))
+        return set_error(VHIP_ERR_INVALID_CONFIG, who + ": tokens are more than 2^23 elements apart, or heads 2^40");
+    if ((tokens > 1 && a->token < dim) || (heads > 1 && a->head < dim) ||
+        (tokens > 1 && heads > 1 && a->token < (heads - 1) * a->head + dim && a->head < (tokens - 1) * a->token + dim))
+        return set_error(VHIP_ERR_INVALID_CONFIG, who + ": rows overlap");
+    return VHIP_OK;
+}
+
+bool whole_chunks(const vhip_heads *a, int dtype, size_t dim) {
+    const size_t s = dtype_size(dtype);
+    return aligned16(a->data) && a->token * s % 16 == 0 && a->head * s % 16 == 0 && dim * s % 16 == 0;
+}
+
+Heads to_heads(const vhip_heads *a, int dtype) {
+    const size_t s = dtype_size(dtype);
+    return {(char *)a->data, a->token * s, a->head * s};
+}
+
+}  // namespace attn
+}  // namespace vh
+
+using namespace vh;
+using namespace vh::attn;
+
+extern "C" {
+
+size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
+                                size_t sequences) {
+    (void)dtype;
+    if (!kv_heads || !heads) return 0;
+    const int n = split_count({tokens, key_tokens, heads, kv_heads, dim, sequences});
+    return n > 1 ? n * tokens * heads * (padded(dim) * sizeof(float) + sizeof(float2)) : 0;
+}
+
+int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads *k, const vhip_heads *v, size_t tokens,
+                   size_t key_tokens, size_t heads, size_t kv_heads, size_t dim, const int64_t *offsets,
+                   const int64_t *key_offsets, size_t sequences, int causal, float scale, const vhip_heads *out, float *lse,
+                   void *workspace, size_t workspace_bytes, void *stream) {
+    clear_error();
+    const Shape sh{tokens, key_tokens, heads, kv_heads, dim, sequences};
+    VH_CHECK(check_shape(dtype, sh, offsets, key_offsets, scale));
+    VH_CHECK(check_heads("q", q, dtype, tokens, heads, dim));
+    VH_CHECK(check_heads("k", k, dtype, key_tokens, kv_heads, dim));
+    VH_CHECK(check_heads("v", v, dtype, key_tokens, kv_heads, dim));
+    VH_CHECK(check_heads("out", out, dtype, tokens, heads, dim));
+    const int splits = split_count(sh);
+    if (splits > 1 && (!workspace || workspace_bytes < vhip_attention_workspace(dtype, tokens, key_tokens, heads, kv_heads, dim, sequences) ||
+                       !aligned16(workspace)))
+        return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_attention_workspace() or not aligned");
+    const int group = (int)(heads / kv_heads);
+    const int64_t grid = slot_count(tokens, sequences, group, kBM) * (int64_t)kv_heads * splits;
+    if (grid > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
+    CallDevice dev;
+    VH_CHECK(dev.enter(ordinal));
+    if (tokens == 0) return VHIP_OK;
+    const int shift = (group & (group - 1)) ? -1 : __builtin_ctz(group);
+    FwdArgs a{to_heads(q, dtype), to_heads(k, dtype), to_heads(v, dtype), to_heads(out, dtype), lse,
+              {offsets, (int64_t)tokens, (int)sequences},
+              {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
+              {group, shift}, (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, splits, (float *)workspace,
+              (float2 *)((float *)workspace + (size_t)splits * tokens * heads * padded(dim))};
+    const bool dma = whole_chunks(k, dtype, dim) && whole_chunks(v, dtype, dim);
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+        case VHIP_DTYPE_F32: return launch<float>(a, dma, (uint32_t)grid, s);
+        case VHIP_DTYPE_F16: return launch<half_t>(a, dma, (uint32_t)grid, s);
+        default: return launch<bf16_t>(a, dma, (uint32_t)grid, s);
+    }
+}
+
+}  // extern "C"

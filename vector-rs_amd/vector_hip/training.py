@@ -29,7 +29,7 @@ import sys
 
 from . import DriverError, InvalidConfig, _check, _lib, _sig, _sz
 
-__all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize"]
+__all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize", "attention"]
 
 F32, F16, BF16 = 0, 1, 2
 _NAMES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
@@ -46,6 +46,17 @@ _sig("vhip_softmax_xent_grad", _int, _int, _int, _p, _sz, _sz, _p, _sz, _sz, _sz
 _sig("vhip_orthogonalize_workspace", _sz, _sz, _sz, _sz)
 _sig("vhip_orthogonalize", _int, _int, _int, _p, _sz, _sz, _sz, _sz, _sz, _int, _f, _f, _f, _f, _p, _sz, _sz, _p, _sz,
      _p)
+
+
+class _Heads(ctypes.Structure):
+    _fields_ = [("data", _p), ("token", _sz), ("head", _sz)]
+
+
+_h = ctypes.POINTER(_Heads)
+_shape = [_sz] * 6  # tokens, key_tokens, heads, kv_heads, dim, sequences
+_sig("vhip_attention_workspace", _sz, _int, *_shape)
+_sig("vhip_attention", _int, _int, _int, _h, _h, _h, _sz, _sz, _sz, _sz, _sz, _p, _p, _sz, _int, _f, _h, _p, _p, _sz, _p)
+
 
 class _Types(dict):
     """dtype object -> code"""
@@ -264,3 +275,64 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
                                    st[0] if update.dim() == 3 else 0, steps, a, b, c, eps, out.data_ptr(), cols,
                                    rows * cols, ws.data_ptr(), need, lib.stream(device)))
     return out
+
+
+def _heads(name, a, like=None) -> _Heads:
+    """Checks rows of heads [tokens, heads, dim]."""
+    if not getattr(a, "is_cuda", False):
+        _on_gpu(name, a)
+    st = a.stride()
+    if len(st) != 3:
+        raise InvalidConfig(f"{name} must have three dimensions: tokens, heads, dim")
+    if like is not None and (a.dtype != like.dtype or a.get_device() != like.get_device()):
+        raise InvalidConfig(f"{name} must have the type and the device of the other rows")
+    n, h, d = a.shape
+    if st[2] != 1 and d > 1:
+        raise InvalidConfig(f"the values of a row of {name} must be contiguous")
+    return _Heads(a.data_ptr(), st[0] if n > 1 else h * d, st[1] if h > 1 else d)
+
+
+def _offsets(name, a, device, lib, count=None):
+    """Checks the offsets of packed sequences; their address and the number of sequences."""
+    _on_gpu(name, a)
+    n = a.numel() - 1
+    if n < 0 or (count is not None and n != count):
+        raise InvalidConfig(f"{name} must hold one value more than there are sequences")
+    return _vector(name, a, n + 1, device, lib.i64), n
+
+
+def _attention_args(q, k, v, offsets, key_offsets, scale):
+    hq, hk, hv = _heads("q", q), _heads("k", k, q), _heads("v", v, q)
+    tokens, heads, dim = q.shape
+    keys, kv_heads, d = k.shape
+    if v.shape != k.shape or d != dim:
+        raise InvalidConfig("k and v must have the same shape, and rows as long as those of q")
+    if kv_heads == 0 or heads % kv_heads:
+        raise InvalidConfig(f"{heads} heads are no multiple of {kv_heads}")
+    device, lib = q.get_device(), _library[type(q.dtype)]
+    at, n = _offsets("offsets", offsets, device, lib)
+    kat = None if key_offsets is None else _offsets("key_offsets", key_offsets, device, lib, n)[0]
+    if kat is None and keys != tokens:
+        raise InvalidConfig("without key_offsets there are as many keys as queries")
+    if scale is None:
+        scale = dim ** -0.5 if dim else 1.0
+    return hq, hk, hv, (tokens, keys, heads, kv_heads, dim), device, _code[q.dtype], lib, at, kat, n, scale
+
+
+def attention(q, k, v, offsets, key_offsets=None, causal: bool = True, scale=None):
+    """(out, lse) of softmax attention over packed sequences: q [tokens, heads, dim], k and v [tokens, kv_heads,
+    dim], heads a multiple of kv_heads (query head h reads key head h // (heads // kv_heads)).  offsets (int64,
+    sequences + 1 values that do not fall) bound the sequences; with key_offsets k and v have bounds of their own.
+    With `causal` the last query of a sequence sees all its keys and each query before it one fewer.  scale is 1 / sqrt(dim)
+    by default.  out has q's type and shape, lse is float32 [tokens, heads]; a row that sees no key, or is in no
+    sequence, has out 0 and lse -inf."""
+    hq, hk, hv, shape, device, code, lib, at, kat, n, scale = _attention_args(q, k, v, offsets, key_offsets, scale)
+    _no_graph(lib, q, k, v)
+    tokens, _, heads, _, dim = shape
+    out, lse = q.new_empty((tokens, heads, dim)), q.new_empty((tokens, heads), dtype=lib.f32)
+    need = _lib.vhip_attention_workspace(code, *shape, n)
+    ws = q.new_empty(need, dtype=lib.u8) if need else None
+    _check(_lib.vhip_attention(device, code, hq, hk, hv, *shape, at, kat, n, causal, scale,
+                               _Heads(out.data_ptr(), heads * dim, dim), lse.data_ptr(),
+                               None if ws is None else ws.data_ptr(), need, lib.stream(device)))
+    return out, lse

@@ -474,6 +474,15 @@ int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads
                    size_t key_tokens, size_t heads, size_t kv_heads, size_t dim, const int64_t *offsets,
                    const int64_t *key_offsets, size_t sequences, int causal, float scale, const vhip_heads *out, float *lse,
                    void *workspace, size_t workspace_bytes, void *stream);
+/* The gradients of sum <dout, out> for q, k and v from the forward call's out and lse; the heads of a group add up in
+ * the gradients of their key head.  Rows of no sequence have gradient 0. */
+size_t vhip_attention_backward_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
+                                         size_t sequences);
+int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, const vhip_heads *q, const vhip_heads *k,
+                            const vhip_heads *v, const vhip_heads *out, const float *lse, size_t tokens, size_t key_tokens,
+                            size_t heads, size_t kv_heads, size_t dim, const int64_t *offsets, const int64_t *key_offsets,
+                            size_t sequences, int causal, float scale, const vhip_heads *dq, const vhip_heads *dk,
+                            const vhip_heads *dv, void *workspace, size_t workspace_bytes, void *stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -72,17 +72,21 @@ def attention_case(lq, lk, heads, kv, dim, dtype, seed=0, tail=0, size=1.0):
     return q, k, v, do
 
 
-def attention_reference(q, k, v, lq, lk, causal, scale, do=None, dtype=None):
+def attention_reference(q, k, v, lq, lk, causal, scale, do=None):
     """out, lse, their tolerances, and with do the gradients of q, k, v with theirs, all in 64 bits.
 
-    A score of |q|.|k| scale = a is off by (dim + 4) e a from its sum, and by 4 e a where it is scaled and the largest
-    one taken off; a weight p then by twice that (its own and its row's sum) and the 8 e of exp, sum and quotient, and
-    by u where it is rounded for the product.  ds = p (dp - delta) has p's error and that of dp and of delta, which
-    takes the rounded out; it is rounded itself, then multiplied."""
-    t = q.dtype if dtype is None else dtype
-    u, tiny = UNIT[t], TINY[t]
-    heads, kv, dim = q.shape[1], k.shape[1], q.shape[2]
-    per = heads // kv
+    A score of a = scale |q|.|k| is off by (dim + 8) e a: its sum's chain, the scale, the largest one taken off.
+    lse is off by the scores' mean of that, by the row's sum (m e), by exp's and log's own 8 e and by 4 e |lse|; a
+    weight by its score and that, and by u where it is rounded to be multiplied.  The backward pass makes p from the
+    rounded lse: twice lse's error.  ds = p (dp - delta) has the errors of p, of dp and of delta, which takes the
+    rounded out, and is rounded to be multiplied; in float16 it loses 2^-39 of its row's or key's largest one, and p 2^-39.
+    Sums of m keys, or of all rows of a key, have that many e more."""
+    t = q.dtype
+    u, tiny, wide = UNIT[t], TINY[t], t == torch.float32
+    up = 0.0 if wide else u  # of p and ds as operands
+    lost = 2.0 ** -39 if t == torch.float16 else 0.0
+    heads, dim = q.shape[1], q.shape[2]
+    per = heads // k.shape[1]
     z = lambda x: torch.zeros(x.shape, dtype=torch.float64, device="cuda")  # noqa: E731
     r = {"out": z(q), "lse": torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")}
     tol = {"out": z(q) + tiny, "lse": z(r["lse"])}
@@ -91,45 +95,42 @@ def attention_reference(q, k, v, lq, lk, causal, scale, do=None, dtype=None):
             r[n], tol[n] = z(x), z(x) + tiny
     qb = kb = 0
     for n, m in zip(lq, lk):
+        rows, keys = slice(qb, qb + n), slice(kb, kb + m)
         for h in range(heads if n and m else 0):
-            Q, K, V = q[qb:qb + n, h].double(), k[kb:kb + m, h // per].double(), v[kb:kb + m, h // per].double()
+            Q, K, V = q[rows, h].double(), k[keys, h // per].double(), v[keys, h // per].double()
             seen = torch.ones(n, m, device="cuda", dtype=torch.bool)
             if causal:
                 seen = seen.tril(m - n)
             s = (Q @ K.t() * scale).masked_fill(~seen, -math.inf)
-            a = (Q.abs() @ K.abs().t() * abs(scale)).masked_fill(~seen, 0.0)
-            some = seen.any(1)
+            off = ((dim + 8) * E * abs(scale) * (Q.abs() @ K.abs().t())).masked_fill(~seen, 0.0)
             lse = torch.logsumexp(s, 1)
-            p = torch.where(seen, torch.exp(s - torch.where(some, lse, torch.zeros_like(lse))[:, None]), 0.0)
-            o = p @ V
-            off = (dim + 8) * E * a  # of a score
-            offl = (p * off).sum(1) + 8 * E + 4 * E * torch.where(some, lse, torch.zeros_like(lse)).abs() + m * E
-            rp = off + offl[:, None]  # of a weight, relative
-            up = rp + (0 if t == torch.float32 else u)
-            r["out"][qb:qb + n, h], r["lse"][qb:qb + n, h] = o, lse
-            osize = p @ V.abs()
-            tol["out"][qb:qb + n, h] += (p * up) @ V.abs() + (m + 8) * E * osize + u * o.abs() + 2.0 ** -28 * V.abs().sum(0)
-            tol["lse"][qb:qb + n, h] = torch.where(some, offl, torch.zeros_like(offl))
-            if do is not None:
-                G = do[qb:qb + n, h].double()
-                dp = G @ V.t()
-                delta = (G * o).sum(1, keepdim=True)
-                ds = p * (dp - delta)
-                r["dq"][qb:qb + n, h] = scale * ds @ K
-                r["dk"][kb:kb + m, h // per] += scale * ds.t() @ Q
-                r["dv"][kb:kb + m, h // per] += p.t() @ G
-                ea = (dim + 4) * E * (G.abs() @ V.abs().t() + (G.abs() * osize).sum(1, keepdim=True))
-                ed = (G.abs() * (tol["out"][qb:qb + n, h])).sum(1, keepdim=True)
-                eds = p * (ea + ed) + up * ds.abs() + 4 * E * ds.abs() + p * up * 0 + rp * p * (dp.abs() + delta.abs())
-                floor = 0.0 if t != torch.float16 else 2.0 ** -24  # of what shares a power of two with a value
-                rowmax, colmax = ds.abs().amax(1, keepdim=True), ds.abs().amax(0, keepdim=True)
-                s1 = abs(scale)
-                tol["dq"][qb:qb + n, h] += s1 * ((eds + floor * rowmax) @ K.abs() + (m + 8) * E * ds.abs() @ K.abs()) + u * r["dq"][qb:qb + n, h].abs()
-                tol["dk"][kb:kb + m, h // per] += s1 * ((eds + floor * colmax).t() @ Q.abs() + (per * n + 8) * E * ds.abs().t() @ Q.abs())
-                tol["dv"][kb:kb + m, h // per] += (p * up + (2.0 ** -38 if floor else 0.0)).t() @ G.abs() + (per * n + 8) * E * p.t() @ G.abs()
-        if do is not None:
-            for x in ("dk", "dv"):
-                tol[x][kb:kb + m] += u * r[x][kb:kb + m].abs()
+            safe = torch.where(seen.any(1), lse, torch.zeros_like(lse))
+            p = torch.where(seen, torch.exp(s - safe[:, None]), 0.0)
+            o, osize = p @ V, p @ V.abs()
+            elses = (p * off).sum(1) + (m + 8) * E + 4 * E * safe.abs()
+            rel = off + elses[:, None]
+            r["out"][rows, h], r["lse"][rows, h] = o, lse
+            tol["out"][rows, h] += (p * (rel + up)) @ V.abs() + (m + 8) * E * osize + u * o.abs() + lost * V.abs().sum(0)
+            tol["lse"][rows, h] = torch.where(seen.any(1), elses, torch.zeros_like(elses))
+            if do is None:
+                continue
+            G, rel = do[rows, h].double(), off + 2 * elses[:, None]
+            dp, delta = G @ V.t(), (G * o).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            edp = (dim + 4) * E * (G.abs() @ V.abs().t() + (G.abs() * osize).sum(1, keepdim=True))
+            edelta = (G.abs() * tol["out"][rows, h]).sum(1, keepdim=True)
+            eds = p * (edp + edelta) + (rel + up + 4 * E) * ds.abs()
+            top = lambda x, d: lost * x.abs().amax(d, keepdim=True)  # noqa: E731
+            a = abs(scale)
+            r["dq"][rows, h] = scale * ds @ K
+            tol["dq"][rows, h] += a * (eds + top(ds, 1) + (m + 8) * E * ds.abs()) @ K.abs() + u * r["dq"][rows, h].abs()
+            more = (per * n + 8) * E
+            r["dk"][keys, h // per] += scale * ds.t() @ Q
+            tol["dk"][keys, h // per] += a * (eds + top(ds, 0) + more * ds.abs()).t() @ Q.abs()
+            r["dv"][keys, h // per] += p.t() @ G
+            tol["dv"][keys, h // per] += (p * (rel + up) + lost + more * p).t() @ G.abs()
+        for x in ("dk", "dv") if do is not None else ():
+            tol[x][keys] += u * r[x][keys].abs()
         qb, kb = qb + n, kb + m
     return r, tol
 
@@ -155,3 +156,18 @@ def test_attention(tr, lq, lk, heads, kv, dim, causal, dtype):
     assert out.dtype == q.dtype and lse.dtype == torch.float32
     within(out, want["out"], tol["out"])
     within(lse, want["lse"], tol["lse"])
+
+
+@pytest.mark.parametrize("lq,lk,heads,kv,dim", ATTENTION)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_backward(tr, lq, lk, heads, kv, dim, causal, dtype):
+    print("attention_backward", lq[:4], lk[:4], heads, kv, dim, causal, dtype, flush=True)
+    q, k, v, do = attention_case(lq, lk, heads, kv, dim, dtype, tail=3)
+    scale = 1 / math.sqrt(dim)
+    at, kat = bounds(lq), None if lq == lk else bounds(lk)
+    out, lse = tr.attention(q, k, v, at, kat, causal=causal)
+    want, tol = attention_reference(q, k, v, lq, lk, causal, scale, do)
+    for name, got in zip(("dq", "dk", "dv"), tr.attention_backward(do, q, k, v, out, lse, at, kat, causal=causal)):
+        assert got.dtype == q.dtype
+        within(got, want[name], tol[name])

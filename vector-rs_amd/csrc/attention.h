@@ -18,6 +18,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "mm16.h"
 
@@ -105,6 +106,15 @@ constexpr int swz_of(int row_bytes, int r) {
                                   : (r >> 2) & 3;
 }
 
+// dma_lds16_at with a lane's whole address: heads may be further apart than 32 bits count.
+__device__ __forceinline__ void dma_lds16_far(const void *p, uint32_t m0_base) {
+    uint32_t sv;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(sv)
+                 : "v"(p), "s"(m0_base)
+                 : "memory");
+}
+
 // A tile of ROWS rows of DP values that NW waves load.
 template <class T, int DP, int ROWS, int NW, bool DMA>
 struct Tile {
@@ -119,7 +129,7 @@ struct Tile {
         row = n / CH;
         chunk = (n % CH) ^ swz(row);
     }
-    // Loads the tile to `to`: row r is at base + at(r) bytes (uniform base), of `dim` values.  By DMA rows are
+    // Loads the tile to `to`: row r is at base + at(r) bytes (uniform base; 32 or 64 bits), of `dim` values.  By DMA rows are
     // whole chunks at 16-byte addresses, and chunks past the last are copies of it (the other operand has zeros
     // there, or the result is not used); otherwise values come one vector at a time, zeros past dim.
     template <class At>
@@ -132,14 +142,17 @@ struct Tile {
             for (int i = 0; i < N; ++i) {
                 int r, c;
                 spot(i, r, c);
-                dma_lds16_at(base, (uint32_t)at(r) + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
+                if constexpr (sizeof(at(0)) == 4)
+                    dma_lds16_at(base, at(r) + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
+                else
+                    dma_lds16_far(base + at(r) + min(c, last) * 16, lds + i * NW * 1024);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int r, c;
                 spot(i, r, c);
-                const auto v = load_row<VEC>((const T *)(base + (uint32_t)at(r)), c * VEC, dim);
+                const auto v = load_row<VEC>((const T *)(base + at(r)), c * VEC, dim);
                 *(Pack<T, VEC> *)(to + ((i * NW + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) * 16) = v;
             }
         }
@@ -245,11 +258,49 @@ __device__ __forceinline__ void store_cols(T *row, const floatx16_t (&acc)[DT], 
         }
 }
 
+// Float16 has too few powers of two for a row's ds = p (dp - delta): what a lane's row or key adds up is held in
+// units of 2^-e, e as large as lets its largest |ds| so far stay below 2^15.  A value then loses what falls below
+// 2^-39 of that largest one.  Other types need none of it.
+template <class T>
+struct Units {
+    static constexpr bool kOn = std::is_same<T, half_t>::value;
+    int e = 100;
+    // ds (a lane's 16 values and those of its other half) in units, sums scaled anew where those got coarser
+    template <int DT>
+    __device__ __forceinline__ void to_units(floatx16_t &ds, floatx16_t (&sum)[DT]) {
+        if constexpr (kOn) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t = fmaxf(t, fabsf(ds[i]));
+            t = fmaxf(t, other_half(t));
+            const int next = t > 0.f ? min(e, 15 - __builtin_amdgcn_frexp_expf(t)) : e;
+            if (__any(next != e)) {
+                const float f = ldexpf(1.f, next - e);
+                e = next;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[d][i] *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[i] = ldexpf(ds[i], e);
+        }
+    }
+    __device__ __forceinline__ float back(float x) const {
+        if constexpr (kOn) return ldexpf(x, -e);
+        return x;
+    }
+};
+
 // All DMAs of this wave have landed, and everyone is past what it read before.
 __device__ __forceinline__ void tiles_ready() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
+
+// The DP values of a row as DP / 4 threads' vectors of 4 (96 columns: 10 rows of 24 threads, and 16 idle ones).
+template <int DP>
+constexpr int kRowsOf256 = 256 / (DP / 4);
 
 // ---- host --------------------------------------------------------------------------------------
 
@@ -257,6 +308,19 @@ __device__ __forceinline__ void tiles_ready() {
 struct Shape {
     size_t tokens, key_tokens, heads, kv_heads, dim, sequences;
 };
+inline size_t padded(size_t dim) { return round_up(dim, 32); }
+// Parts of the keys that a row sees, or of the rows that see a key: enough workgroups for some rounds of the GPU where
+// there are few, none shorter than `shortest` of an average sequence.  Lengths are on the device, so it goes by sizes.
+inline int split_count(int64_t workgroups, size_t along, size_t sequences, int shortest) {
+    const int64_t each = (int64_t)(along / (sequences ? sequences : 1)) / shortest;
+    int64_t n = 1024 / (workgroups ? workgroups : 1);
+    n = n < each ? n : each;
+    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+inline Group to_group(size_t heads, size_t kv_heads) {
+    const int n = (int)(heads / kv_heads);
+    return {n, (n & (n - 1)) ? -1 : __builtin_ctz(n)};
+}
 int check_shape(int dtype, const Shape &s, const int64_t *offsets, const int64_t *key_offsets, float scale);
 int check_heads(const char *name, const vhip_heads *a, int dtype, size_t tokens, size_t heads, size_t dim);
 // Whether rows can be loaded by 16-byte chunks.

@@ -1,0 +1,416 @@
+// attention_backward.hip -- gradients of softmax attention of packed sequences with grouped heads.
+//
+//   p_rj = exp(s_rj - lse_r),  delta_r = <do_r, o_r>,  dp_rj = <do_r, v_j>,  ds_rj = p_rj (dp_rj - delta_r)
+//   dq_r = scale sum_j ds_rj k_j,  dk_j = scale sum_r ds_rj q_r,  dv_j = sum_r p_rj do_r
+// with the sums over r running over all heads of the group that read key head of j.
+//
+// Two kernels, each of which owns what it adds up in registers, so no result is made by atomics and none depends on
+// timing: one by rows (dq, and delta on its way), one by keys (dk and dv).  Scores and dp are made twice, seven products
+// in all where five would do, for which no gradient is written and read again as partial sums.
+//  * by rows: 128 packed rows a workgroup, 32 a wave, q and do in registers; tiles of keys and values.
+//    S^T and dP^T leave a lane with its own row's scores, so lse and delta are its own scalars.
+//  * by keys: 128 keys a workgroup, 32 a wave, k and v in registers; tiles of packed rows of q and do, whose lse and
+//    delta come from LDS.  S and dP leave a lane with its own key's column.
+// p and ds are rounded to the operands' type for the last products, which is half a unit of each; in float16 they are held
+// in powers of two of their own (p times 2^14, ds see Units).
+#include "attention.h"
+
+namespace vh {
+namespace attn {
+namespace {
+
+struct BwdArgs {
+    Heads q, k, v, o, go, dq, dk, dv;
+    const float *lse;
+    float *delta;
+    Packed rows, keys;
+    Group group;
+    int heads, kv_heads, dim;
+    bool causal;
+    float scale;
+    int splits;   // parts of what is summed over, each a workgroup; more than one leave `part`, which k_attn_sum adds up
+    float *part;  // dq: [split][token][head][DP]; dk, dv: [split][2][token][head][DP]
+};
+
+constexpr int kBM = 128, kBK = 128;  // rows and keys of a workgroup
+template <class T>
+constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // keys, or rows, of a tile
+
+// Workgroups of a CU whose waves' registers hold all that they own: two have 256 a lane, one has 512.
+template <class T, int DP>
+struct RegsFor {
+    static constexpr int dq = sizeof(T) == 4 && DP > 96 ? 1 : 2, dkv = DP > 64 ? 1 : 2;
+};
+
+// Power of two of p where it is an operand
+template <class T>
+constexpr float kShift = std::is_same<T, half_t>::value ? 14.f : 0.f;
+
+template <class T, int KS>
+__device__ __forceinline__ void load_operand(typename Frag<T>::type (&f)[KS], const char *row, int dim, int half, bool neg) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const auto x = load_row<VEC>((const T *)row, (2 * ks + half) * VEC, dim);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[ks][e] = neg ? -x.v[e] : x.v[e];
+    }
+}
+
+template <class T, int DP, bool DMA>
+__global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a) {
+    constexpr int BN = kBN<T>, NS = BN / 32, RB = DP * (int)sizeof(T), KS = RB / 32, DT = DP / 32, VEC = 16 / (int)sizeof(T);
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, DP, BN, 4, DMA> KV;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][KV::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    const uint32_t id = blockIdx.x;
+    const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
+    const Place at = find_tile<kBM>(a.rows, a.group.size, id / a.kv_heads / a.splits);
+    const Span rows = packed_span(a.rows, at.seq);
+    const int n = rows.len * a.group.size;
+    if (at.tile >= (n + kBM - 1) / kBM) return;
+    const bool real = at.seq >= 1 && at.seq <= a.rows.count;
+    const Span keys = real ? packed_span(a.keys, at.seq) : Span{0, 0};
+    const int row0 = ((n + kBM - 1) / kBM - 1 - at.tile) * kBM;
+
+    const int r = row0 + wave * 32 + (lane & 31), rc = min(r, n - 1);
+    const int token = a.group.token(rc), head = kh * a.group.size + rc - token * a.group.size;
+    const int64_t row = rows.begin + token;
+    const int shift = keys.len - rows.len + 1;
+    const int sees = a.causal ? min(keys.len, max(0, token + shift)) : keys.len;
+    const int most = a.causal ? min(keys.len, max(0, a.group.token(min(row0 + kBM, n) - 1) + shift)) : keys.len;
+    const int tiles = (most + BN - 1) / BN, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
+    const int w0 = row0 + wave * 32, w1 = min(w0 + 32, n) - 1;
+    const int all = a.causal ? min(keys.len, max(0, a.group.token(min(w0, n - 1)) + shift)) : keys.len;
+    const int any = w0 >= n ? 0 : a.causal ? min(keys.len, max(0, a.group.token(w1) + shift)) : keys.len;
+
+    const char *kb = a.k.data + keys.begin * a.k.token + kh * a.k.head, *vb = a.v.data + keys.begin * a.v.token + kh * a.v.head;
+    auto load = [&](int t, int buf) {
+        const int last = keys.len - 1 - t * BN;
+        const uint32_t ks = (uint32_t)a.k.token, vs = (uint32_t)a.v.token;
+        KV::load(kb + (int64_t)t * BN * a.k.token, [&](int i) { return (uint32_t)min(i, last) * ks; }, a.dim, lds[buf][0]);
+        KV::load(vb + (int64_t)t * BN * a.v.token, [&](int i) { return (uint32_t)min(i, last) * vs; }, a.dim, lds[buf][1]);
+    };
+    if (t0 < t1) load(t0, 0);
+
+    const int64_t at_row = row * a.heads + head;
+    frag q[KS], go[KS];
+    load_operand<T>(q, a.q.data + row * (int64_t)a.q.token + (int64_t)head * a.q.head, a.dim, half, a.scale < 0.f);
+    load_operand<T>(go, a.go.data + row * (int64_t)a.go.token + (int64_t)head * a.go.head, a.dim, half, false);
+    float delta = 0.f;
+    {
+        const T *p = (const T *)(a.o.data + row * (int64_t)a.o.token + (int64_t)head * a.o.head);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const auto x = load_row<VEC>(p, (2 * ks + half) * VEC, a.dim);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) delta = fmaf((float)go[ks][e], (float)x.v[e], delta);
+        }
+        delta += other_half(delta);
+        if (split == 0 && half == 0 && r < n) a.delta[at_row] = delta;
+    }
+    const float lse = a.lse[at_row], c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
+    const float base = lse == -INFINITY ? 0.f : -lse * kLog2e;
+
+    floatx16_t dq[DT] = {};
+    Units<T> units;
+    for (int t = t0; t < t1; ++t) {
+        tiles_ready();
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int key0 = t * BN + 32 * j;
+            if (key0 >= any) break;
+            floatx16_t s = {}, dp = {};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s = mma(rows_frag<T, RB>(lds[buf][0], 32 * j, ks, lane), q[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dp = mma(rows_frag<T, RB>(lds[buf][1], 32 * j, ks, lane), go[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, base)) * (dp[i] - delta);
+            if (key0 + 32 > all) {
+                const int left = sees - key0 - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (row_of(i) >= left) s[i] = 0.f;
+            }
+            units.to_units(s, dq);
+            frag ds[kOps<T>];
+            to_operand<T>(s, ds);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dq[d] = mma_cols<T, RB>(lds[buf][0], 32 * j, d, ds, dq[d], lane);
+        }
+    }
+    if (r >= n) return;
+    auto value = [&](float x) { return units.back(x) * a.scale; };
+    if (a.splits > 1)
+        store_cols<float, DT>(a.part + ((int64_t)split * a.rows.tokens * a.heads + at_row) * DP, dq, DP, lane, value);
+    else
+        store_cols<T, DT>((T *)(a.dq.data + row * (int64_t)a.dq.token + (int64_t)head * a.dq.head), dq, a.dim, lane, value);
+}
+
+template <class T, int DP, bool DMA>
+__global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs a) {
+    constexpr int BR = kBN<T>, NS = BR / 32, RB = DP * (int)sizeof(T), KS = RB / 32, DT = DP / 32;
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, DP, BR, 4, DMA> QG;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][QG::kBytes];
+    __shared__ __attribute__((aligned(16))) float stats[2][2][BR];  // -lse in base 2, delta
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    const uint32_t id = blockIdx.x;
+    const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
+    const Place at = find_tile<kBK>(a.keys, 1, id / a.kv_heads / a.splits);
+    const Span keys = packed_span(a.keys, at.seq);
+    if (at.tile >= (keys.len + kBK - 1) / kBK) return;
+    const bool real = at.seq >= 1 && at.seq <= a.keys.count;
+    const Span rows = real ? packed_span(a.rows, at.seq) : Span{0, 0};
+    const int n = rows.len * a.group.size, g = a.group.size;
+    // the first keys of a sequence are seen by the most rows
+    const int key0 = at.tile * kBK, w0 = key0 + wave * 32;
+
+    // this lane's key, and the first row that sees it: of the lane, of the wave's first and last key, of the workgroup
+    const int j = w0 + (lane & 31), back = rows.len - keys.len;
+    auto first_row = [&](int key) { return a.causal ? min(n, max(0, key + back) * g) : 0; };
+    const int first = first_row(j), wave_first = first_row(w0), wave_last = first_row(w0 + 31);
+    const int b0 = first_row(key0) / BR, blocks = (n + BR - 1) / BR - b0, per = (blocks + a.splits - 1) / a.splits;
+    const int t0 = b0 + split * per, t1 = min(b0 + blocks, t0 + per);
+
+    const char *qb = a.q.data + rows.begin * a.q.token + (int64_t)kh * g * a.q.head;
+    const char *gb = a.go.data + rows.begin * a.go.token + (int64_t)kh * g * a.go.head;
+    float next_lse = 0.f, next_delta = 0.f;
+    auto load = [&](int t, int buf) {
+        const int r0 = t * BR, tok0 = a.group.token(r0);
+        if (threadIdx.x < BR) {
+            const int r = min(r0 + (int)threadIdx.x, n - 1), token = a.group.token(r);
+            const int64_t i = (rows.begin + token) * a.heads + kh * g + r - token * g;
+            next_lse = a.lse[i];
+            next_delta = a.delta[i];
+        }
+        auto far = [&](int i, const Heads &x) {
+            const int r = min(r0 + i, n - 1), token = a.group.token(r);
+            return (int64_t)(token - tok0) * (int64_t)x.token + (int64_t)(r - token * g) * (int64_t)x.head;
+        };
+        QG::load(qb + tok0 * (int64_t)a.q.token, [&](int i) { return far(i, a.q); }, a.dim, lds[buf][0]);
+        QG::load(gb + tok0 * (int64_t)a.go.token, [&](int i) { return far(i, a.go); }, a.dim, lds[buf][1]);
+    };
+    auto put_stats = [&](int buf) {
+        if (threadIdx.x < BR) {
+            stats[buf][0][threadIdx.x] = next_lse == -INFINITY ? 0.f : fmaf(-next_lse, kLog2e, kShift<T>);
+            stats[buf][1][threadIdx.x] = next_delta;
+        }
+    };
+    if (t0 < t1) {
+        load(t0, 0);
+        put_stats(0);
+    }
+
+    const int jc = min(j, keys.len - 1);
+    frag k[KS], v[KS];
+    load_operand<T>(k, a.k.data + (keys.begin + jc) * (int64_t)a.k.token + (int64_t)kh * a.k.head, a.dim, half, a.scale < 0.f);
+    load_operand<T>(v, a.v.data + (keys.begin + jc) * (int64_t)a.v.token + (int64_t)kh * a.v.head, a.dim, half, false);
+    const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
+
+    floatx16_t dk[DT] = {}, dv[DT] = {};
+    Units<T> units;
+    for (int t = t0; t < t1; ++t) {
+        tiles_ready();
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
+#pragma unroll
+        for (int b = 0; b < NS; ++b) {
+            const int r0 = t * BR + 32 * b;
+            if (r0 + 32 <= wave_first || r0 >= n) continue;
+            floatx16_t s = {}, dp = {};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s = mma(rows_frag<T, RB>(lds[buf][0], 32 * b, ks, lane), k[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dp = mma(rows_frag<T, RB>(lds[buf][1], 32 * b, ks, lane), v[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const Pack<float, 4> l = *(const Pack<float, 4> *)&stats[buf][0][32 * b + row_of(i) + 4 * half];
+                const Pack<float, 4> d = *(const Pack<float, 4> *)&stats[buf][1][32 * b + row_of(i) + 4 * half];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i + e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], c, l.v[e]));
+                    dp[i + e] = s[i + e] * (dp[i + e] - d.v[e]);
+                }
+            }
+            if (r0 < wave_last || r0 + 32 > n) {
+                const int from = first - r0 - 4 * half, to = n - r0 - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (row_of(i) < from || row_of(i) >= to) s[i] = dp[i] = 0.f;
+            }
+            frag p[kOps<T>];
+            to_operand<T>(s, p);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dv[d] = mma_cols<T, RB>(lds[buf][1], 32 * b, d, p, dv[d], lane);
+            units.to_units(dp, dk);
+            frag ds[kOps<T>];
+            to_operand<T>(dp, ds);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dk[d] = mma_cols<T, RB>(lds[buf][0], 32 * b, d, ds, dk[d], lane);
+        }
+        if (t + 1 < t1) put_stats(buf ^ 1);
+    }
+    if (j >= keys.len) return;
+    const float shrink = kShift<T> > 0.f ? 1.f / 16384.f : 1.f;
+    auto kvalue = [&](float x) { return units.back(x) * (a.scale * shrink); };
+    auto vvalue = [&](float x) { return x * shrink; };
+    const int64_t row = keys.begin + j;
+    if (a.splits > 1) {
+        const int64_t all = a.keys.tokens * a.kv_heads, i = row * a.kv_heads + kh;
+        store_cols<float, DT>(a.part + ((2 * split) * all + i) * DP, dk, DP, lane, kvalue);
+        store_cols<float, DT>(a.part + ((2 * split + 1) * all + i) * DP, dv, DP, lane, vvalue);
+    } else {
+        store_cols<T, DT>((T *)(a.dk.data + row * (int64_t)a.dk.token + (int64_t)kh * a.dk.head), dk, a.dim, lane, kvalue);
+        store_cols<T, DT>((T *)(a.dv.data + row * (int64_t)a.dv.token + (int64_t)kh * a.dv.head), dv, a.dim, lane, vvalue);
+    }
+}
+
+// Adds up parts: of dq (KEYS false), or of dk and dv (blockIdx.y), in the order of the parts.
+template <class T, int DP, bool KEYS>
+__global__ __launch_bounds__(256) void k_attn_sum(BwdArgs a) {
+    constexpr int L = DP / 4, R = kRowsOf256<DP>;
+    const int heads = KEYS ? a.kv_heads : a.heads;
+    const int64_t all = (KEYS ? a.keys.tokens : a.rows.tokens) * heads;
+    const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    const int e = threadIdx.x % L * 4;
+    if (threadIdx.x >= R * L || i >= all || e >= a.dim) return;
+    const int which = KEYS ? blockIdx.y : 0;
+    float sum[4] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const Pack<float, 4> p = load_any<4>(a.part + ((KEYS ? 2 * s + which : s) * all + i) * DP + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += p.v[k];
+    }
+    Pack<T, 4> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v.v[k] = (T)sum[k];
+    const Heads &o = !KEYS ? a.dq : which ? a.dv : a.dk;
+    store_row<4>((T *)(o.data + i / heads * (int64_t)o.token + i % heads * (int64_t)o.head), e, a.dim, v);
+}
+
+// What a call works in: delta, then the parts of dq and afterwards, in the same place, those of dk and dv.
+struct Work {
+    int qsplits, ksplits;
+    float *delta, *part;
+    size_t bytes;
+};
+Work work_of(const Shape &s, void *base) {
+    Work w;
+    w.qsplits = split_count(slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads, s.key_tokens, s.sequences, 256);
+    w.ksplits = split_count(slot_count(s.key_tokens, s.sequences, 1, kBK) * s.kv_heads, s.tokens * (s.heads / s.kv_heads), s.sequences, 256);
+    const size_t dp = padded(s.dim);
+    const size_t q = w.qsplits > 1 ? w.qsplits * s.tokens * s.heads * dp : 0;
+    const size_t k = w.ksplits > 1 ? 2 * w.ksplits * s.key_tokens * s.kv_heads * dp : 0;
+    Carver c{(char *)base};
+    w.delta = c.take<float>(s.tokens * s.heads);
+    w.part = c.take<float>(q > k ? q : k);
+    w.bytes = c.used;
+    return w;
+}
+
+struct Run {
+    Work w;
+    bool dq, dkv, dma_kv, dma_q;
+    uint32_t qgrid, kgrid;
+    hipStream_t s;
+};
+
+template <class T, int DP>
+int launch(BwdArgs a, const Run &r) {
+    if (r.qgrid) {
+        a.splits = r.w.qsplits;
+        if (r.dma_kv)
+            k_attn_dq<T, DP, true><<<r.qgrid, 256, 0, r.s>>>(a);
+        else
+            k_attn_dq<T, DP, false><<<r.qgrid, 256, 0, r.s>>>(a);
+        if (a.splits > 1) k_attn_sum<T, DP, false><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, r.s>>>(a);
+    }
+    if (r.kgrid) {
+        a.splits = r.w.ksplits;
+        if (r.dma_q)
+            k_attn_dkv<T, DP, true><<<r.kgrid, 256, 0, r.s>>>(a);
+        else
+            k_attn_dkv<T, DP, false><<<r.kgrid, 256, 0, r.s>>>(a);
+        if (a.splits > 1)
+            k_attn_sum<T, DP, true><<<dim3((uint32_t)ceil_div(a.keys.tokens * a.kv_heads, kRowsOf256<DP>), 2), 256, 0, r.s>>>(a);
+    }
+    return launch_status("attention launch");
+}
+template <class T>
+int launch(const BwdArgs &a, const Run &r) {
+    switch (padded(a.dim)) {
+        case 32: return launch<T, 32>(a, r);
+        case 64: return launch<T, 64>(a, r);
+        case 96: return launch<T, 96>(a, r);
+        default: return launch<T, 128>(a, r);
+    }
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace vh
+
+using namespace vh;
+using namespace vh::attn;
+
+extern "C" {
+
+size_t vhip_attention_backward_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
+                                         size_t sequences) {
+    (void)dtype;
+    if (!kv_heads || !heads) return 0;
+    return work_of({tokens, key_tokens, heads, kv_heads, dim, sequences}, nullptr).bytes;
+}
+
+int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, const vhip_heads *q, const vhip_heads *k,
+                            const vhip_heads *v, const vhip_heads *out, const float *lse, size_t tokens, size_t key_tokens,
+                            size_t heads, size_t kv_heads, size_t dim, const int64_t *offsets, const int64_t *key_offsets,
+                            size_t sequences, int causal, float scale, const vhip_heads *dq, const vhip_heads *dk,
+                            const vhip_heads *dv, void *workspace, size_t workspace_bytes, void *stream) {
+    clear_error();
+    const Shape sh{tokens, key_tokens, heads, kv_heads, dim, sequences};
+    VH_CHECK(check_shape(dtype, sh, offsets, key_offsets, scale));
+    VH_CHECK(check_heads("dout", dout, dtype, tokens, heads, dim));
+    VH_CHECK(check_heads("q", q, dtype, tokens, heads, dim));
+    VH_CHECK(check_heads("k", k, dtype, key_tokens, kv_heads, dim));
+    VH_CHECK(check_heads("v", v, dtype, key_tokens, kv_heads, dim));
+    VH_CHECK(check_heads("out", out, dtype, tokens, heads, dim));
+    if (tokens && !lse) return set_error(VHIP_ERR_INVALID_CONFIG, "lse is null");
+    VH_CHECK(check_heads("dq", dq, dtype, tokens, heads, dim));
+    VH_CHECK(check_heads("dk", dk, dtype, key_tokens, kv_heads, dim));
+    VH_CHECK(check_heads("dv", dv, dtype, key_tokens, kv_heads, dim));
+    Run r;
+    r.w = work_of(sh, workspace);
+    if (r.w.bytes && (!workspace || workspace_bytes < r.w.bytes || !aligned16(workspace)))
+        return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_attention_backward_workspace() or not aligned");
+    const int64_t qgrid = slot_count(tokens, sequences, heads / kv_heads, kBM) * (int64_t)kv_heads * r.w.qsplits;
+    const int64_t kgrid = slot_count(key_tokens, sequences, 1, kBK) * (int64_t)kv_heads * r.w.ksplits;
+    if (qgrid > 0x7fffffff || kgrid > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
+    CallDevice dev;
+    VH_CHECK(dev.enter(ordinal));
+    r.qgrid = tokens ? (uint32_t)qgrid : 0;
+    r.kgrid = key_tokens ? (uint32_t)kgrid : 0;
+    r.dma_kv = whole_chunks(k, dtype, dim) && whole_chunks(v, dtype, dim);
+    r.dma_q = whole_chunks(q, dtype, dim) && whole_chunks(dout, dtype, dim);
+    r.s = (hipStream_t)stream;
+    const BwdArgs a{to_heads(q, dtype), to_heads(k, dtype), to_heads(v, dtype), to_heads(out, dtype), to_heads(dout, dtype),
+                    to_heads(dq, dtype), to_heads(dk, dtype), to_heads(dv, dtype), lse, r.w.delta,
+                    {offsets, (int64_t)tokens, (int)sequences},
+                    {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
+                    to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, 1, r.w.part};
+    switch (dtype) {
+        case VHIP_DTYPE_F32: return launch<float>(a, r);
+        case VHIP_DTYPE_F16: return launch<half_t>(a, r);
+        default: return launch<bf16_t>(a, r);
+    }
+}
+
+}  // extern "C"

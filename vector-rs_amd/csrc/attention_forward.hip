@@ -7,8 +7,6 @@
 // and walks tiles of keys and values that come by DMA into the other of two buffers while one is multiplied. A
 // row's largest score m and sum l run along, in the scores' base-2 logarithms; the output and l are only scaled anew
 // once a row's m has grown by more than 2^8, so most tiles take no pass over the accumulators.
-#include <type_traits>
-
 #include "attention.h"
 
 namespace vh {
@@ -168,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
 // A row's parts: its largest m, and their outputs and sums over it.  A row of DP values has DP / 4 lanes.
 template <class T, int DP>
 __global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
-    constexpr int L = DP / 4, R = 256 / L;  // 96 columns: 10 rows of 24 lanes, and 16 lanes without one
+    constexpr int L = DP / 4, R = kRowsOf256<DP>;
     const int64_t all = a.rows.tokens * a.heads;
     const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
     if (threadIdx.x >= R * L || i >= all) return;
@@ -194,17 +192,9 @@ __global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
     if (e < a.dim) store_row<4>((T *)(a.out.data + token * (int64_t)a.out.token + head * (int64_t)a.out.head), e, a.dim, v);
 }
 
-// Parts of the keys: enough workgroups for two rounds of the GPU where rows are few, none shorter than 256 keys of
-// an average sequence.  Lengths are on the device, so it goes by the sizes alone.
-int split_count(const Shape &s) {
-    const int64_t base = slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads;
-    const int64_t keys = (int64_t)(s.key_tokens / (s.sequences ? s.sequences : 1));
-    int64_t n = 1024 / (base ? base : 1);
-    if (n > keys / 256) n = keys / 256;
-    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+int splits_of(const Shape &s) {
+    return split_count(slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads, s.key_tokens, s.sequences, 256);
 }
-
-inline size_t padded(size_t dim) { return round_up(dim, 32); }
 
 template <class T, int DP>
 int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
@@ -213,8 +203,7 @@ int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
     else
         k_attn_forward<T, DP, false><<<grid, 256, 0, s>>>(a);
     if (a.splits > 1) {
-        constexpr int R = 256 / (DP / 4);
-        k_attn_join<T, DP><<<(uint32_t)ceil_div((size_t)a.rows.tokens * a.heads, R), 256, 0, s>>>(a);
+        k_attn_join<T, DP><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, s>>>(a);
     }
     return launch_status("attention launch");
 }
@@ -278,7 +267,7 @@ size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, siz
                                 size_t sequences) {
     (void)dtype;
     if (!kv_heads || !heads) return 0;
-    const int n = split_count({tokens, key_tokens, heads, kv_heads, dim, sequences});
+    const int n = splits_of({tokens, key_tokens, heads, kv_heads, dim, sequences});
     return n > 1 ? n * tokens * heads * (padded(dim) * sizeof(float) + sizeof(float2)) : 0;
 }
 
@@ -293,21 +282,19 @@ int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads
     VH_CHECK(check_heads("k", k, dtype, key_tokens, kv_heads, dim));
     VH_CHECK(check_heads("v", v, dtype, key_tokens, kv_heads, dim));
     VH_CHECK(check_heads("out", out, dtype, tokens, heads, dim));
-    const int splits = split_count(sh);
+    const int splits = splits_of(sh);
     if (splits > 1 && (!workspace || workspace_bytes < vhip_attention_workspace(dtype, tokens, key_tokens, heads, kv_heads, dim, sequences) ||
                        !aligned16(workspace)))
         return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_attention_workspace() or not aligned");
-    const int group = (int)(heads / kv_heads);
-    const int64_t grid = slot_count(tokens, sequences, group, kBM) * (int64_t)kv_heads * splits;
+    const int64_t grid = slot_count(tokens, sequences, heads / kv_heads, kBM) * (int64_t)kv_heads * splits;
     if (grid > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
     CallDevice dev;
     VH_CHECK(dev.enter(ordinal));
     if (tokens == 0) return VHIP_OK;
-    const int shift = (group & (group - 1)) ? -1 : __builtin_ctz(group);
     FwdArgs a{to_heads(q, dtype), to_heads(k, dtype), to_heads(v, dtype), to_heads(out, dtype), lse,
               {offsets, (int64_t)tokens, (int)sequences},
               {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
-              {group, shift}, (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, splits, (float *)workspace,
+              to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, splits, (float *)workspace,
               (float2 *)((float *)workspace + (size_t)splits * tokens * heads * padded(dim))};
     const bool dma = whole_chunks(k, dtype, dim) && whole_chunks(v, dtype, dim);
     hipStream_t s = (hipStream_t)stream;

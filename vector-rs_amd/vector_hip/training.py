@@ -29,7 +29,8 @@ import sys
 
 from . import DriverError, InvalidConfig, _check, _lib, _sig, _sz
 
-__all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize", "attention"]
+__all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize", "attention",
+           "attention_backward"]
 
 F32, F16, BF16 = 0, 1, 2
 _NAMES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
@@ -56,6 +57,9 @@ _h = ctypes.POINTER(_Heads)
 _shape = [_sz] * 6  # tokens, key_tokens, heads, kv_heads, dim, sequences
 _sig("vhip_attention_workspace", _sz, _int, *_shape)
 _sig("vhip_attention", _int, _int, _int, _h, _h, _h, _sz, _sz, _sz, _sz, _sz, _p, _p, _sz, _int, _f, _h, _p, _p, _sz, _p)
+_sig("vhip_attention_backward_workspace", _sz, _int, *_shape)
+_sig("vhip_attention_backward", _int, _int, _int, _h, _h, _h, _h, _h, _p, _sz, _sz, _sz, _sz, _sz, _p, _p, _sz, _int, _f, _h, _h,
+     _h, _p, _sz, _p)
 
 
 class _Types(dict):
@@ -336,3 +340,24 @@ def attention(q, k, v, offsets, key_offsets=None, causal: bool = True, scale=Non
                                _Heads(out.data_ptr(), heads * dim, dim), lse.data_ptr(),
                                None if ws is None else ws.data_ptr(), need, lib.stream(device)))
     return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, offsets, key_offsets=None, causal: bool = True, scale=None):
+    """(dq, dk, dv), in the type of q, k and v, from the gradient of attention's out, its arguments and what it
+    returned.  Heads that share a key head add up in its gradients; rows of no sequence have gradient 0."""
+    hq, hk, hv, shape, device, code, lib, at, kat, n, scale = _attention_args(q, k, v, offsets, key_offsets, scale)
+    hg, ho = _heads("dout", dout, q), _heads("out", out, q)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise InvalidConfig("dout and out must have the shape of q")
+    tokens, keys, heads, kv_heads, dim = shape
+    if lse.shape != (tokens, heads):
+        raise InvalidConfig("lse must hold a value for each token and head")
+    ls = _vector("lse", lse.view(-1) if lse.is_contiguous() else lse, tokens * heads, device, lib.f32)
+    dq, dk, dv = q.new_empty((tokens, heads, dim)), k.new_empty((keys, kv_heads, dim)), k.new_empty((keys, kv_heads, dim))
+    need = _lib.vhip_attention_backward_workspace(code, *shape, n)
+    ws = q.new_empty(need, dtype=lib.u8)
+    rows = lambda a, h: _Heads(a.data_ptr(), h * dim, dim)  # noqa: E731
+    _check(_lib.vhip_attention_backward(device, code, hg, hq, hk, hv, ho, ls, *shape, at, kat, n, causal, scale,
+                                        rows(dq, heads), rows(dk, kv_heads), rows(dv, kv_heads), ws.data_ptr(), need,
+                                        lib.stream(device)))
+    return dq, dk, dv

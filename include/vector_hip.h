@@ -484,6 +484,44 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
                             size_t sequences, int causal, float scale, const vhip_heads *dq, const vhip_heads *dk,
                             const vhip_heads *dv, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Norms of queries and keys for each head and the rotation by their tokens' positions, in one pass:
+ *   r = 1 / sqrt(mean x^2 + eps),  n = x r weight,
+ * then pair i of the first `rotary` columns (an even number; i and i + rotary / 2, or with `interleaved` 2 i and
+ * 2 i + 1) turns by positions[t] * frequencies[i] radians, a product in 64 bits (exact positions up to 2^53).
+ * Weights (dim values of param_dtype, which is dtype or f32) may be NULL, and either side may have no heads.
+ * dim <= 512. */
+int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_heads *q, const vhip_heads *k, size_t tokens,
+                        size_t heads, size_t kv_heads, size_t dim, const void *q_weight, const void *k_weight,
+                        const int64_t *positions, const float *frequencies, size_t rotary, int interleaved, float eps,
+                        const vhip_heads *q_out, const vhip_heads *k_out, void *stream);
+/* Gradients from those of the outputs (dq, dk) and the forward call's inputs: of q, k (dq_out, dk_out) and of the
+ * weights (param_dtype; each may be NULL, and without both so may the workspace). */
+size_t vhip_qk_norm_rotary_backward_workspace(size_t tokens, size_t dim);
+int vhip_qk_norm_rotary_backward(int ordinal, int dtype, int param_dtype, const vhip_heads *dq, const vhip_heads *dk,
+                                 const vhip_heads *q, const vhip_heads *k, size_t tokens, size_t heads, size_t kv_heads,
+                                 size_t dim, const void *q_weight, const void *k_weight, const int64_t *positions,
+                                 const float *frequencies, size_t rotary, int interleaved, float eps, const vhip_heads *dq_out,
+                                 const vhip_heads *dk_out, void *dq_weight, void *dk_weight, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/* The norm of all values of `count` arrays together, and clipping to a largest norm:
+ *   norm = sqrt(sum g^2),  out = g min(1, max_norm / (norm + eps)),
+ * squares and their sum in 64 bits.  The list of arrays is host memory that is read before the call returns; norm (a
+ * float of device memory; for vhip_clip_gradients it may be NULL) and the arrays are device memory.  out is data
+ * itself, of the same type, or an array of any of the types that overlaps no other.  A norm of infinity gives zeros
+ * (and NaN for the infinite values), one of NaN gives NaN. */
+typedef struct vhip_array {
+    const void *data;
+    void *out; /* not used by vhip_gradient_norm */
+    size_t count;
+    int dtype, out_dtype;
+} vhip_array;
+size_t vhip_clip_gradients_workspace(size_t count);
+int vhip_gradient_norm(int ordinal, const vhip_array *arrays, size_t count, float *norm, void *workspace, size_t workspace_bytes,
+                       void *stream);
+int vhip_clip_gradients(int ordinal, const vhip_array *arrays, size_t count, float max_norm, float eps, float *norm, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

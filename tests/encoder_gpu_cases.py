@@ -171,3 +171,136 @@ def test_attention_backward(tr, lq, lk, heads, kv, dim, causal, dtype):
     for name, got in zip(("dq", "dk", "dv"), tr.attention_backward(do, q, k, v, out, lse, at, kat, causal=causal)):
         assert got.dtype == q.dtype
         within(got, want[name], tol[name])
+
+
+# ---- head norms with rotation -----------------------------------------------------------------------
+
+def turn(x, angle, interleaved, back=False):
+    """Rows [tokens, heads, dim] with their first pairs turned, in 64 bits."""
+    rot = 2 * angle.shape[1]
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :rot // 2], x[..., rot // 2:rot])
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None] * (-1 if back else 1)
+    y = x.clone()
+    ya, yb = a * c - b * s, a * s + b * c
+    if interleaved:
+        y[..., 0:rot:2], y[..., 1:rot:2] = ya, yb
+    else:
+        y[..., :rot // 2], y[..., rot // 2:rot] = ya, yb
+    return y
+
+
+def both_of_a_pair(x, pairs, interleaved):
+    """For each column what its pair holds together."""
+    rot = 2 * pairs
+    y = x.clone()
+    for a, b in ([(slice(0, rot, 2), slice(1, rot, 2))] if interleaved else [(slice(0, pairs), slice(pairs, rot))]):
+        y[..., a] = y[..., b] = x[..., a] + x[..., b]
+    return y
+
+
+def head_norm_reference(x, w, angle, interleaved, eps, dy=None):
+    """y or (dx, dw) in 64 bits with bounds: the sum of dim squares and the scale are off by (dim / 2 + 6) e, sine and
+    cosine by 4 e of a whole, products and their sum by 4 e more; dx and dw likewise by their terms' sizes."""
+    dim, pairs = x.shape[2], angle.shape[1]
+    x, w = x.double(), torch.ones(dim, device="cuda", dtype=torch.float64) if w is None else w.double()
+    r = 1 / torch.sqrt((x * x).mean(2, keepdim=True) + eps)
+    rel = (dim / 2 + 6) * E
+    if dy is None:
+        n = x * r * w
+        return turn(n, angle, interleaved), (rel + 8 * E) * both_of_a_pair(n.abs(), pairs, interleaved)
+    dn = turn(dy.double(), angle, interleaved, back=True)
+    size = both_of_a_pair(dy.double().abs(), pairs, interleaved)
+    xh, u = x * r, dn * w
+    usize = size * w.abs()
+    m = (u * xh).mean(2, keepdim=True)
+    msize = (usize * xh.abs()).mean(2, keepdim=True)
+    dx = r * (u - xh * m)
+    tol = r * (rel + 16 * E + dim * E) * (usize + xh.abs() * msize)
+    chain = x.shape[0] * x.shape[1]
+    return dx, tol, (dn * xh).sum((0, 1)), (chain * E + rel + 16 * E) * (size * xh.abs()).sum((0, 1))
+
+
+# tokens, heads, key heads, dim, rotated columns, neighbouring pairs, padding between rows
+HEAD_NORMS = [
+    (1, 12, 12, 64, 64, False, 0), (5, 32, 8, 128, 128, False, 8), (17, 4, 2, 80, 40, True, 0), (9, 3, 1, 33, 32, False, 1),
+    (3, 2, 2, 256, 64, False, 0), (2, 1, 1, 512, 512, True, 0), (130, 6, 2, 72, 72, True, 0), (40, 5, 5, 1, 0, False, 0),
+    (7, 2, 1, 7, 6, False, 0), (300, 2, 2, 20, 6, True, 3), (3000, 3, 1, 96, 96, False, 0), (0, 4, 2, 64, 64, False, 0),
+    (4, 4, 2, 64, 0, False, 0), (9000, 1, 1, 16, 16, True, 0), (2, 3, 0, 64, 64, False, 0), (3, 2, 1, 509, 300, False, 5),
+]
+
+
+def head_norm_case(tokens, heads, kv, dim, rot, pad, dtype, params, far=40_000):
+    t = TYPES[dtype]
+    x = (2 * normal(1, tokens, heads + kv, dim + pad)).to(t)[..., :dim]
+    w = [(1 + 0.3 * normal(2 + i, dim)).to(TYPES[params]) for i in range(2)]
+    pos = torch.randint(-far, far, (tokens,), device="cuda", generator=gen(5))
+    freq = 10000.0 ** (-torch.arange(0, rot, 2, device="cuda", dtype=torch.float32) / max(rot, 1))
+    return x[:, :heads], x[:, heads:], w, pos, freq
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,near,pad", HEAD_NORMS)
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+def test_head_norm(tr, tokens, heads, kv, dim, rot, near, pad, dtype, params):
+    print("qk_norm_rotary", tokens, heads, kv, dim, rot, near, pad, dtype, params, flush=True)
+    q, k, w, pos, freq = head_norm_case(tokens, heads, kv, dim, rot, pad, dtype, params)
+    got = tr.qk_norm_rotary(q, k, w[0], w[1], pos, freq, eps=1e-5, interleaved=near)
+    angle = pos.double()[:, None] * freq.double()
+    u, tiny = UNIT[q.dtype], TINY[q.dtype]
+    for x, y, wt in zip((q, k), got, w):
+        want, tol = head_norm_reference(x, wt, angle, near, 1e-5)
+        assert y.dtype == x.dtype and y.shape == x.shape
+        within(y, want, tol + u * want.abs() + tiny)
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,near,pad", HEAD_NORMS)
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+def test_head_norm_backward(tr, tokens, heads, kv, dim, rot, near, pad, dtype, params):
+    print("qk_norm_rotary_backward", tokens, heads, kv, dim, rot, near, pad, dtype, params, flush=True)
+    q, k, w, pos, freq = head_norm_case(tokens, heads, kv, dim, rot, pad, dtype, params)
+    dq, dk = normal(8, *q.shape).to(q.dtype), normal(9, *k.shape).to(q.dtype)
+    got = tr.qk_norm_rotary_backward(dq, dk, q, k, w[0], w[1], pos, freq, eps=1e-5, interleaved=near)
+    angle = pos.double()[:, None] * freq.double()
+    for x, g, wt, dx, dw in zip((q, k), (dq, dk), w, got[:2], got[2:]):
+        want, tol, wantw, tolw = head_norm_reference(x, wt, angle, near, 1e-5, g)
+        assert dx.dtype == x.dtype and dw.dtype == wt.dtype
+        within(dx, want, tol + UNIT[x.dtype] * want.abs() + TINY[x.dtype])
+        within(dw, wantw, tolw + UNIT[wt.dtype] * wantw.abs() + TINY[wt.dtype])
+
+
+# ---- clipping ---------------------------------------------------------------------------------------
+
+def clip_arrays(sizes, dtypes, scale=1.0):
+    return [(scale * normal(i, *((n,) if isinstance(n, int) else n))).to(TYPES[dtypes[i % len(dtypes)]]) for i, n in enumerate(sizes)]
+
+
+def clip_reference(arrays, max_norm, eps):
+    total = sum(((a.double() ** 2).sum() for a in arrays), torch.zeros((), device="cuda", dtype=torch.float64))
+    norm = total.sqrt()
+    return norm, torch.clamp(max_norm / (norm + eps), max=1.0)
+
+
+CLIPS = [[1], [3, 5], [2047, 2048, 2049, 1], [(96, 128), (128,), (128,), (2000, 128)], [0, 7, 0], [1] * 300, [17, 4096] * 130,
+         [3_000_001], [8193, (33, 65), 100_003, 2], [0]]
+
+
+@pytest.mark.parametrize("sizes", CLIPS)
+@pytest.mark.parametrize("dtypes", [("f32",), ("f16",), ("bf16",), ("bf16", "f32", "f16")])
+@pytest.mark.parametrize("out", [None, "f32", "bf16"])
+@pytest.mark.parametrize("max_norm", [0.5, 1e6])
+def test_clip(tr, sizes, dtypes, out, max_norm):
+    print("clip", sizes[:4], len(sizes), dtypes, out, max_norm, flush=True)
+    arrays = clip_arrays(sizes, dtypes)
+    norm, c = clip_reference(arrays, max_norm, 1e-6)
+    before = [a.clone() for a in arrays]
+    outs = None if out is None else [torch.full(a.shape, math.nan, device="cuda", dtype=TYPES[out]) for a in arrays]
+    within(tr.gradient_norm(arrays), norm, 2 * E * norm)
+    got = tr.clip_gradients(arrays, max_norm, out=outs)
+    assert got.dtype == torch.float32 and got.shape == ()
+    within(got, norm, 2 * E * norm)
+    for a, b, o in zip(arrays, before, arrays if outs is None else outs):
+        if outs is not None:
+            assert torch.equal(a, b)
+        want = b.double() * c
+        within(o, want, (2 * E + UNIT[o.dtype]) * want.abs() + TINY[o.dtype])
+        if float(c) == 1.0 and o.dtype == b.dtype:
+            assert torch.equal(o, b)

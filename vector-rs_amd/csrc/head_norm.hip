@@ -1,0 +1,411 @@
+// head_norm.hip -- norms of queries and keys for each head with the rotation by position, and their gradients.
+//
+//   r = 1 / sqrt(mean x^2 + eps),  n = x r w;  pair i of a row (a, b) turns by t_i = position frequency_i:
+//   a' = a cos t - b sin t,  b' = a sin t + b cos t  (columns past the pairs stay as they are)
+//   backward: dn = dy turned back,  xh = x r,  u = dn w:  dx = r (u - xh mean(u xh)),  dw = sum over rows of dn xh
+//
+// Both passes are bound by memory: a row is read once into the registers of L lanes, which hold both columns of
+// each of their pairs (pairs of halves: a vector of the first half and its counterpart of the second; neighbouring pairs:
+// two vectors one after the other), so nothing is exchanged but the row's sums. L is a power of two of at least dim / 2
+// vectors. A workgroup takes a few tokens at a time and makes their cosines and sines once in LDS, for all heads.
+//
+// Angles are products in 64 bits, taken modulo a quarter turn there: at position 10^6 a 32-bit product is off by 0.03.
+// What is left, at most pi / 4, goes into the Taylor polynomials of sine and cosine in 32 bits, whose remainders
+// (pi / 4)^11 / 11! and (pi / 4)^12 / 12! are below half a unit of them.
+//
+// The weights' gradients are sums over all rows: a workgroup keeps its columns' sums in registers over its tokens,
+// leaves them in a row of the workspace, and a second kernel adds those rows in a fixed order.
+#include "train_common.h"
+
+namespace vh {
+namespace {
+
+constexpr int kTok = 8;                // tokens a workgroup has at a time, at most
+constexpr int kMaxPairs = 256;         // of a row
+constexpr int kMaxDim = 2 * kMaxPairs;
+constexpr size_t kMaxParts = 1024;     // workgroups of the backward pass: rows of partial sums
+
+struct Side {
+    const char *x, *dy;  // dy: backward
+    char *out;           // y, or dx
+    size_t x_token, x_head, dy_token, dy_head, out_token, out_head;  // bytes
+    const void *weight;
+    int heads;
+};
+
+struct HeadArgs {
+    Side side[2];  // queries, keys
+    const int64_t *positions;
+    const float *frequencies;
+    float *part;  // backward: [workgroup][2][dim]
+    int64_t tokens;
+    int dim, pairs, lanes_log2, at_once;  // at_once: tokens of a turn
+    bool f32_params;
+    float eps;
+};
+
+// A lane's columns of a row: the first and the second vectors of its pairs, and two of what is not turned.
+template <class T, bool NEAR>
+struct Columns {
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    int c[4], end[4];
+    __device__ __forceinline__ Columns(int t, int lanes, int dim, int pairs) {
+        const int v = t * VEC;
+        c[0] = NEAR ? 2 * v : v;
+        c[1] = NEAR ? 2 * v + VEC : pairs + v;
+        end[0] = NEAR ? 2 * pairs : pairs;
+        end[1] = 2 * pairs;
+        c[2] = 2 * pairs + v;
+        c[3] = c[2] + lanes * VEC;
+        end[2] = end[3] = dim;
+    }
+    template <class U>
+    __device__ __forceinline__ void load(float (&v)[4][VEC], const U *row) const {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (c[s] < end[s]) {
+                const Pack<U, VEC> p = load_row<VEC>(row, c[s], end[s]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[s][e] = (float)p.v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[s][e] = 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const float (&v)[4][VEC]) const {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (c[s] < end[s]) {
+                Pack<T, VEC> p;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) p.v[e] = (T)v[s][e];
+                store_row<VEC>(row, c[s], end[s], p);
+            }
+    }
+    // Pair e of the lane: both its values
+    static __device__ __forceinline__ float &first(float (&v)[4][VEC], int e) { return NEAR ? v[2 * e / VEC][2 * e % VEC] : v[0][e]; }
+    static __device__ __forceinline__ float &second(float (&v)[4][VEC], int e) {
+        return NEAR ? v[2 * e / VEC][2 * e % VEC + 1] : v[1][e];
+    }
+    // Turns the lane's pairs by cs (cosines, sines of the row's token), or back.
+    __device__ __forceinline__ void turn(float (&v)[4][VEC], const float2 *cs, int t, int pairs, bool back) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if (t * VEC + e >= pairs) continue;
+            const float2 p = cs[t * VEC + e];
+            const float s = back ? -p.y : p.y;
+            const float a = first(v, e), b = second(v, e);
+            first(v, e) = a * p.x - b * s;
+            second(v, e) = a * s + b * p.x;
+        }
+    }
+};
+
+__device__ __forceinline__ float2 cos_sin(int64_t position, float frequency) {
+    const double a = (double)position * (double)frequency;
+    const double k = rint(a * 0.63661977236758134308);  // quarter turns
+    const float r = (float)fma(-k, 6.123233995736766036e-17, fma(-k, 1.57079632679489661923, a));
+    const int q = (int)((long long)k & 3);
+    const float z = r * r;
+    const float s = r + r * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
+    const float c = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+    const float x = q & 1 ? s : c, y = q & 1 ? c : s;
+    return make_float2(q == 1 || q == 2 ? -x : x, q >= 2 ? -y : y);
+}
+
+__device__ __forceinline__ void make_turns(const HeadArgs &a, int64_t tok0, int count, float2 (*cs)[kMaxPairs]) {
+    for (int i = threadIdx.x; i < count * a.pairs; i += 256) {
+        const int t = i / a.pairs, p = i - t * a.pairs;
+        cs[t][p] = cos_sin(a.positions[tok0 + t], a.frequencies[p]);
+    }
+}
+
+__device__ __forceinline__ float row_lanes_sum(float x, int lanes_log2) {
+    for (int l = 0; l < lanes_log2; ++l) x += __shfl_xor(x, 1 << l, 64);
+    return x;
+}
+
+template <class T, bool NEAR>
+__device__ __forceinline__ void load_weight(float (&w)[4][16 / (int)sizeof(T)], const Columns<T, NEAR> &cols, const HeadArgs &a,
+                                            const void *weight) {
+    if (!weight) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e) w[s][e] = 1.f;
+    } else if (a.f32_params) {
+        cols.load(w, (const float *)weight);
+    } else {
+        cols.load(w, (const T *)weight);
+    }
+}
+
+template <class T, bool NEAR>
+__global__ __launch_bounds__(256) void k_head_forward(HeadArgs a) {
+    typedef Columns<T, NEAR> Cols;
+    constexpr int VEC = Cols::VEC;
+    __shared__ float2 cs[kTok][kMaxPairs];
+    const int lanes = 1 << a.lanes_log2, t = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2, slots = 256 >> a.lanes_log2;
+    const Cols cols(t, lanes, a.dim, a.pairs);
+    const int64_t tok0 = (int64_t)blockIdx.x * a.at_once;
+    const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
+    make_turns(a, tok0, count, cs);
+    __syncthreads();
+    const float inv = 1.f / (float)a.dim;
+    for (int s = 0; s < 2; ++s) {
+        const Side &side = a.side[s];
+        float w[4][VEC];
+        load_weight<T, NEAR>(w, cols, a, side.weight);
+        for (int i = slot; i < count * side.heads; i += slots) {
+            const int k = i / side.heads, h = i - k * side.heads;
+            float x[4][VEC];
+            cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
+            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum = fmaf(x[v][e], x[v][e], sum);
+            const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[v][e] *= r * w[v][e];
+            cols.turn(x, cs[k], t, a.pairs, false);
+            cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
+        }
+    }
+}
+
+template <class T, bool NEAR>
+__global__ __launch_bounds__(256) void k_head_backward(HeadArgs a) {
+    typedef Columns<T, NEAR> Cols;
+    constexpr int VEC = Cols::VEC;
+    __shared__ float2 cs[kTok][kMaxPairs];
+    __shared__ float sums[kMaxDim];
+    const int lanes = 1 << a.lanes_log2, t = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2, slots = 256 >> a.lanes_log2;
+    const Cols cols(t, lanes, a.dim, a.pairs);
+    const float inv = 1.f / (float)a.dim;
+    for (int s = 0; s < 2; ++s) {
+        const Side &side = a.side[s];
+        float w[4][VEC], dw[4][VEC] = {};
+        load_weight<T, NEAR>(w, cols, a, side.weight);
+        for (int64_t tok0 = (int64_t)blockIdx.x * a.at_once; tok0 < a.tokens; tok0 += (int64_t)gridDim.x * a.at_once) {
+            const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
+            __syncthreads();
+            make_turns(a, tok0, count, cs);
+            __syncthreads();
+            for (int i = slot; i < count * side.heads; i += slots) {
+                const int k = i / side.heads, h = i - k * side.heads;
+                float x[4][VEC], g[4][VEC];
+                cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
+                cols.load(g, (const T *)(side.dy + (tok0 + k) * side.dy_token + h * side.dy_head));
+                cols.turn(g, cs[k], t, a.pairs, true);
+                float sum = 0.f, dot = 0.f;
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        sum = fmaf(x[v][e], x[v][e], sum);
+                        dot = fmaf(x[v][e], g[v][e] * w[v][e], dot);
+                    }
+                const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
+                const float m = row_lanes_sum(dot, a.lanes_log2) * r * inv;  // mean of u xh
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float xh = x[v][e] * r;
+                        dw[v][e] = fmaf(g[v][e], xh, dw[v][e]);
+                        x[v][e] = r * (g[v][e] * w[v][e] - xh * m);
+                    }
+                cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
+            }
+        }
+        if (!a.part) continue;
+        // the sums of the workgroup's rows: the slots' one after the other
+        for (int q = 0; q < slots; ++q) {
+            __syncthreads();
+            if (slot == q)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int c = cols.c[v] + e;
+                        if (c < cols.end[v]) sums[c] = (q ? sums[c] : 0.f) + dw[v][e];
+                    }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.dim; c += 256) a.part[((size_t)blockIdx.x * 2 + s) * a.dim + c] = sums[c];
+    }
+}
+
+// Adds the workgroups' rows in a fixed order: 32 columns and one side a workgroup, 8 rows at a time.
+template <class P>
+__global__ __launch_bounds__(256) void k_head_sums(const float *part, int parts, int dim, P *dq, P *dk) {
+    __shared__ float sums[8][33];
+    P *out = blockIdx.y ? dk : dq;
+    if (!out) return;
+    const int g = threadIdx.x >> 5, l = threadIdx.x & 31, c = blockIdx.x * 32 + l;
+    float s = 0.f;
+    if (c < dim)
+        for (int p = g; p < parts; p += 8) s += part[((size_t)p * 2 + blockIdx.y) * dim + c];
+    sums[g][l] = s;
+    __syncthreads();
+    if (g == 0 && c < dim) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += sums[k][l];
+        out[c] = (P)s;
+    }
+}
+
+// Lanes of a row: a power of two of at least half its vectors.
+inline int row_lanes_log2(size_t dim, int dtype) {
+    const size_t per = 2 * 16 / dtype_size(dtype);
+    return lanes_log2((dim + per - 1) / per);
+}
+// Tokens of a turn: as many as the workgroup's rows at once, so that all are busy, but no more than leave enough workgroups.
+inline int tokens_at_once(size_t tokens, size_t heads, int lanes_log2) {
+    size_t n = (256u >> lanes_log2) / heads;
+    const size_t enough = tokens / 1024;
+    n = n < 4 ? 4 : n;
+    n = n < enough ? n : enough;
+    return n < 1 ? 1 : n > kTok ? kTok : (int)n;
+}
+inline size_t part_count(size_t tokens, int at_once) {
+    const size_t n = (tokens + at_once - 1) / at_once;
+    return n < kMaxParts ? n : kMaxParts;
+}
+
+int check_side(const char *name, const vhip_heads *a, int dtype, size_t tokens, size_t heads, size_t dim) {
+    const std::string who(name);
+    if (!a || (tokens && heads && !a->data)) return set_error(VHIP_ERR_INVALID_CONFIG, who + " is null");
+    if (!tokens || !heads) return VHIP_OK;
+    if ((uintptr_t)a->data % dtype_size(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, who + " is not aligned to its type");
+    if (a->token > ((size_t)1 << 40) || a->head > ((size_t)1 << 40))
+        return set_error(VHIP_ERR_INVALID_CONFIG, who + ": rows are more than 2^40 elements apart");
+    if ((tokens > 1 && a->token < dim) || (heads > 1 && a->head < dim) ||
+        (tokens > 1 && heads > 1 && a->token < (heads - 1) * a->head + dim && a->head < (tokens - 1) * a->token + dim))
+        return set_error(VHIP_ERR_INVALID_CONFIG, who + ": rows overlap");
+    return VHIP_OK;
+}
+
+int check_common(int dtype, int param_dtype, size_t tokens, size_t heads, size_t kv_heads, size_t dim, size_t rotary,
+                 const int64_t *positions, const float *frequencies, float eps) {
+    if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
+    if (param_dtype != dtype && param_dtype != VHIP_DTYPE_F32)
+        return set_error(VHIP_ERR_INVALID_CONFIG, "parameters are of the rows' type or f32");
+    if (dim == 0 || dim > kMaxDim) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 512]");
+    if (rotary > dim || rotary % 2) return set_error(VHIP_ERR_INVALID_CONFIG, "rotary must be even and at most dim");
+    if (heads + kv_heads == 0 || heads > 65536 || kv_heads > 65536)
+        return set_error(VHIP_ERR_INVALID_CONFIG, "heads must be in [1, 65536]");
+    if (tokens > (1u << 30)) return set_error(VHIP_ERR_INVALID_CONFIG, "too many tokens");
+    if (rotary && ((tokens && !positions) || !frequencies)) return set_error(VHIP_ERR_INVALID_CONFIG, "positions or frequencies are null");
+    if (!(eps >= 0.f)) return set_error(VHIP_ERR_INVALID_CONFIG, "eps must be >= 0");
+    return VHIP_OK;
+}
+
+Side to_side(int dtype, const vhip_heads *x, const vhip_heads *dy, const vhip_heads *out, const void *weight, size_t heads) {
+    const size_t s = dtype_size(dtype);
+    return {(const char *)x->data, dy ? (const char *)dy->data : nullptr, (char *)out->data,
+            x->token * s, x->head * s, dy ? dy->token * s : 0, dy ? dy->head * s : 0, out->token * s, out->head * s, weight, (int)heads};
+}
+
+template <class T>
+int forward(const HeadArgs &a, bool near, hipStream_t s) {
+    const uint32_t grid = (uint32_t)((a.tokens + a.at_once - 1) / a.at_once);
+    if (near)
+        k_head_forward<T, true><<<grid, 256, 0, s>>>(a);
+    else
+        k_head_forward<T, false><<<grid, 256, 0, s>>>(a);
+    return launch_status("head norm launch");
+}
+
+template <class T>
+int backward(const HeadArgs &a, bool near, void *dqw, void *dkw, hipStream_t s) {
+    const int parts = (int)part_count(a.tokens, a.at_once);
+    if (parts) {
+        if (near)
+            k_head_backward<T, true><<<parts, 256, 0, s>>>(a);
+        else
+            k_head_backward<T, false><<<parts, 256, 0, s>>>(a);
+    }
+    if (dqw || dkw) {
+        const dim3 grid((uint32_t)ceil_div(a.dim, 32), 2);
+        if (a.f32_params)
+            k_head_sums<float><<<grid, 256, 0, s>>>(a.part, parts, a.dim, (float *)dqw, (float *)dkw);
+        else
+            k_head_sums<T><<<grid, 256, 0, s>>>(a.part, parts, a.dim, (T *)dqw, (T *)dkw);
+    }
+    return launch_status("head norm launch");
+}
+
+}  // namespace
+}  // namespace vh
+
+using namespace vh;
+
+extern "C" {
+
+int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_heads *q, const vhip_heads *k, size_t tokens,
+                        size_t heads, size_t kv_heads, size_t dim, const void *q_weight, const void *k_weight,
+                        const int64_t *positions, const float *frequencies, size_t rotary, int interleaved, float eps,
+                        const vhip_heads *q_out, const vhip_heads *k_out, void *stream) {
+    clear_error();
+    VH_CHECK(check_common(dtype, param_dtype, tokens, heads, kv_heads, dim, rotary, positions, frequencies, eps));
+    VH_CHECK(check_side("q", q, dtype, tokens, heads, dim));
+    VH_CHECK(check_side("k", k, dtype, tokens, kv_heads, dim));
+    VH_CHECK(check_side("q_out", q_out, dtype, tokens, heads, dim));
+    VH_CHECK(check_side("k_out", k_out, dtype, tokens, kv_heads, dim));
+    CallDevice dev;
+    VH_CHECK(dev.enter(ordinal));
+    if (tokens == 0) return VHIP_OK;
+    const int l = row_lanes_log2(dim, dtype);
+    const HeadArgs a{{to_side(dtype, q, nullptr, q_out, q_weight, heads), to_side(dtype, k, nullptr, k_out, k_weight, kv_heads)},
+                     positions, frequencies, nullptr, (int64_t)tokens, (int)dim, (int)rotary / 2, l,
+                     tokens_at_once(tokens, heads + kv_heads, l), param_dtype == VHIP_DTYPE_F32, eps};
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+        case VHIP_DTYPE_F32: return forward<float>(a, interleaved, s);
+        case VHIP_DTYPE_F16: return forward<half_t>(a, interleaved, s);
+        default: return forward<bf16_t>(a, interleaved, s);
+    }
+}
+
+size_t vhip_qk_norm_rotary_backward_workspace(size_t tokens, size_t dim) {
+    return 2 * sizeof(float) * dim * part_count(tokens, 1);
+}
+
+int vhip_qk_norm_rotary_backward(int ordinal, int dtype, int param_dtype, const vhip_heads *dq, const vhip_heads *dk,
+                                 const vhip_heads *q, const vhip_heads *k, size_t tokens, size_t heads, size_t kv_heads,
+                                 size_t dim, const void *q_weight, const void *k_weight, const int64_t *positions,
+                                 const float *frequencies, size_t rotary, int interleaved, float eps, const vhip_heads *dq_out,
+                                 const vhip_heads *dk_out, void *dq_weight, void *dk_weight, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    clear_error();
+    VH_CHECK(check_common(dtype, param_dtype, tokens, heads, kv_heads, dim, rotary, positions, frequencies, eps));
+    VH_CHECK(check_side("dq", dq, dtype, tokens, heads, dim));
+    VH_CHECK(check_side("dk", dk, dtype, tokens, kv_heads, dim));
+    VH_CHECK(check_side("q", q, dtype, tokens, heads, dim));
+    VH_CHECK(check_side("k", k, dtype, tokens, kv_heads, dim));
+    VH_CHECK(check_side("dq_out", dq_out, dtype, tokens, heads, dim));
+    VH_CHECK(check_side("dk_out", dk_out, dtype, tokens, kv_heads, dim));
+    if ((dq_weight || dk_weight) && tokens &&
+        (!workspace || workspace_bytes < vhip_qk_norm_rotary_backward_workspace(tokens, dim) || ((uintptr_t)workspace & 3)))
+        return set_error(VHIP_ERR_INVALID_CONFIG,
+                         "the workspace is smaller than vhip_qk_norm_rotary_backward_workspace() or not aligned");
+    CallDevice dev;
+    VH_CHECK(dev.enter(ordinal));
+    const int l = row_lanes_log2(dim, dtype);
+    const HeadArgs a{{to_side(dtype, q, dq, dq_out, q_weight, heads), to_side(dtype, k, dk, dk_out, k_weight, kv_heads)},
+                     positions, frequencies, dq_weight || dk_weight ? (float *)workspace : nullptr, (int64_t)tokens, (int)dim,
+                     (int)rotary / 2, l, tokens_at_once(tokens, heads + kv_heads, l), param_dtype == VHIP_DTYPE_F32, eps};
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+        case VHIP_DTYPE_F32: return backward<float>(a, interleaved, dq_weight, dk_weight, s);
+        case VHIP_DTYPE_F16: return backward<half_t>(a, interleaved, dq_weight, dk_weight, s);
+        default: return backward<bf16_t>(a, interleaved, dq_weight, dk_weight, s);
+    }
+}
+
+}  // extern "C"

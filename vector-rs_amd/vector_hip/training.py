@@ -30,7 +30,7 @@ import sys
 from . import DriverError, InvalidConfig, _check, _lib, _sig, _sz
 
 __all__ = ["layer_norm", "layer_norm_backward", "softmax_xent", "softmax_xent_grad", "orthogonalize", "attention",
-           "attention_backward"]
+           "attention_backward", "qk_norm_rotary", "qk_norm_rotary_backward", "gradient_norm", "clip_gradients"]
 
 F32, F16, BF16 = 0, 1, 2
 _NAMES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
@@ -60,6 +60,20 @@ _sig("vhip_attention", _int, _int, _int, _h, _h, _h, _sz, _sz, _sz, _sz, _sz, _p
 _sig("vhip_attention_backward_workspace", _sz, _int, *_shape)
 _sig("vhip_attention_backward", _int, _int, _int, _h, _h, _h, _h, _h, _p, _sz, _sz, _sz, _sz, _sz, _p, _p, _sz, _int, _f, _h, _h,
      _h, _p, _sz, _p)
+
+
+class _Array(ctypes.Structure):
+    _fields_ = [("data", _p), ("out", _p), ("count", _sz), ("dtype", _int), ("out_dtype", _int)]
+
+
+_a = ctypes.POINTER(_Array)
+_sig("vhip_qk_norm_rotary", _int, _int, _int, _int, _h, _h, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _sz, _int, _f, _h, _h, _p)
+_sig("vhip_qk_norm_rotary_backward_workspace", _sz, _sz, _sz)
+_sig("vhip_qk_norm_rotary_backward", _int, _int, _int, _int, _h, _h, _h, _h, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _sz, _int,
+     _f, _h, _h, _p, _p, _p, _sz, _p)
+_sig("vhip_clip_gradients_workspace", _sz, _sz)
+_sig("vhip_gradient_norm", _int, _int, _a, _sz, _p, _p, _sz, _p)
+_sig("vhip_clip_gradients", _int, _int, _a, _sz, _f, _f, _p, _p, _sz, _p)
 
 
 class _Types(dict):
@@ -361,3 +375,130 @@ def attention_backward(dout, q, k, v, out, lse, offsets, key_offsets=None, causa
                                         rows(dq, heads), rows(dk, kv_heads), rows(dv, kv_heads), ws.data_ptr(), need,
                                         lib.stream(device)))
     return dq, dk, dv
+
+
+def _head_args(q, k, q_weight, k_weight, positions, frequencies):
+    hq, hk = _heads("q", q), _heads("k", k, q)
+    tokens, heads, dim = q.shape
+    if k.shape[0] != tokens or k.shape[2] != dim:
+        raise InvalidConfig("q and k must have the same tokens, and rows of the same length")
+    device, code, lib = q.get_device(), _code[q.dtype], _library[type(q.dtype)]
+    wq = wk = None
+    params = code
+    if (q_weight is None) != (k_weight is None):
+        raise InvalidConfig("q_weight and k_weight are given together or not at all")
+    if q_weight is not None:
+        wq, wk = _vector("q_weight", q_weight, dim, device), _vector("k_weight", k_weight, dim, device)
+        if q_weight.dtype != k_weight.dtype:
+            raise InvalidConfig("q_weight and k_weight must have the same type")
+        params = _param_code(q_weight.dtype, code)
+    at = _vector("positions", positions, tokens, device, lib.i64)
+    _on_gpu("frequencies", frequencies)
+    pairs = frequencies.numel()
+    fr = _vector("frequencies", frequencies, pairs, device, lib.f32)
+    return hq, hk, (tokens, heads, k.shape[1], dim), device, code, params, lib, wq, wk, at, fr, 2 * pairs
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, eps: float = 1e-6, interleaved: bool = False):
+    """(q', k') of queries [tokens, heads, dim] and keys [tokens, kv_heads, dim]: each row over its root mean square,
+    x / sqrt(mean x^2 + eps), times the weight (dim values; both None: 1), its first 2 len(frequencies) columns
+    turned by their token's position (int64): pair i by positions[t] * frequencies[i] radians (float32, their product in
+    64 bits).  Pairs are columns i and i + len(frequencies), or with `interleaved` 2 i and 2 i + 1."""
+    hq, hk, shape, device, code, params, lib, wq, wk, at, fr, rotary = _head_args(q, k, q_weight, k_weight, positions, frequencies)
+    _no_graph(lib, q, k, q_weight, k_weight, frequencies)
+    tokens, heads, kv_heads, dim = shape
+    qo, ko = q.new_empty((tokens, heads, dim)), k.new_empty((tokens, kv_heads, dim))
+    _check(_lib.vhip_qk_norm_rotary(device, code, params, hq, hk, *shape, wq, wk, at, fr, rotary, interleaved, eps,
+                                    _Heads(qo.data_ptr(), heads * dim, dim), _Heads(ko.data_ptr(), kv_heads * dim, dim),
+                                    lib.stream(device)))
+    return qo, ko
+
+
+def qk_norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, positions, frequencies, eps: float = 1e-6,
+                            interleaved: bool = False):
+    """(dq, dk, dq_weight, dk_weight) from the gradients of qk_norm_rotary's outputs and its arguments.  The weights'
+    gradients have their type; without weights they are None."""
+    hq, hk, shape, device, code, params, lib, wq, wk, at, fr, rotary = _head_args(q, k, q_weight, k_weight, positions, frequencies)
+    gq, gk = _heads("dq", dq, q), _heads("dk", dk, q)
+    if dq.shape != q.shape or dk.shape != k.shape:
+        raise InvalidConfig("dq and dk must have the shapes of q and k")
+    tokens, heads, kv_heads, dim = shape
+    qo, ko = q.new_empty((tokens, heads, dim)), k.new_empty((tokens, kv_heads, dim))
+    dqw = dkw = ws = None
+    need = 0
+    if wq is not None:
+        dqw, dkw = q_weight.new_empty((2, dim)).unbind()
+        need = _lib.vhip_qk_norm_rotary_backward_workspace(tokens, dim)
+        ws = q.new_empty(need, dtype=lib.u8)
+    at_of = lambda a: None if a is None else a.data_ptr()  # noqa: E731
+    _check(_lib.vhip_qk_norm_rotary_backward(device, code, params, gq, gk, hq, hk, *shape, wq, wk, at, fr, rotary, interleaved,
+                                             eps, _Heads(qo.data_ptr(), heads * dim, dim),
+                                             _Heads(ko.data_ptr(), kv_heads * dim, dim), at_of(dqw), at_of(dkw), at_of(ws),
+                                             need, lib.stream(device)))
+    return qo, ko, dqw, dkw
+
+
+def _dense(a) -> bool:
+    """Whether an array's values fill a block of memory, in whatever order of its dimensions."""
+    if a.is_contiguous():
+        return True
+    size = 1
+    for stride, n in sorted((st, n) for st, n in zip(a.stride(), a.shape) if n != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+def _arrays(gradients, out):
+    gradients = list(gradients)
+    if not gradients:
+        raise InvalidConfig("there is no array")
+    _on_gpu("a gradient", gradients[0])
+    device = gradients[0].get_device()
+    table = (_Array * len(gradients))()
+    for i, g in enumerate(gradients):
+        _on_gpu("a gradient", g)
+        if g.get_device() != device:
+            raise InvalidConfig("the gradients are on more than one device")
+        if not _dense(g):
+            raise InvalidConfig("the values of a gradient must fill a block of memory")
+        code = _code[g.dtype]
+        at = g.data_ptr()
+        table[i] = (at, at, g.numel(), code, code)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(gradients):
+            raise InvalidConfig("out must hold an array for each gradient")
+        for row, g, o in zip(table, gradients, out):
+            _on_gpu("an output", o)
+            if o.shape != g.shape or o.get_device() != device:
+                raise InvalidConfig("an output must have the shape and the device of its gradient")
+            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                raise InvalidConfig("an output must have the strides of its gradient")
+            row.out, row.out_dtype = o.data_ptr(), _code[o.dtype]
+    first = gradients[0]
+    lib = _library[type(first.dtype)]
+    need = _lib.vhip_clip_gradients_workspace(len(gradients))
+    return table, len(gradients), first.new_empty((), dtype=lib.f32), first.new_empty(need, dtype=lib.u8), need, device, lib
+
+
+def gradient_norm(gradients):
+    """The norm (float32, no dimensions) of all values of a list of arrays together: sqrt(sum g^2), in 64 bits until it
+    is rounded.  The arrays are of any of the types, each filling a block of memory."""
+    gradients = list(gradients)
+    table, n, norm, ws, need, device, lib = _arrays(gradients, None)
+    _no_graph(lib, *gradients)
+    _check(_lib.vhip_gradient_norm(device, table, n, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
+    return norm
+
+
+def clip_gradients(gradients, max_norm: float, out=None, eps: float = 1e-6):
+    """gradient_norm of the arrays; each is scaled by min(1, max_norm / (norm + eps)), in place or into the arrays `out`
+    (the same shapes, any of the types), which overlap nothing else.  A norm that is infinite or NaN is no error: it
+    leaves zeros and NaN."""
+    gradients = list(gradients)
+    table, n, norm, ws, need, device, lib = _arrays(gradients, out)
+    _no_graph(lib, *gradients)
+    _check(_lib.vhip_clip_gradients(device, table, n, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
+    return norm

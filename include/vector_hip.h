@@ -489,7 +489,7 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
  * then pair i of the first `rotary` columns (an even number; i and i + rotary / 2, or with `interleaved` 2 i and
  * 2 i + 1) turns by positions[t] * frequencies[i] radians, a product in 64 bits (exact positions up to 2^53).
  * Weights (dim values of param_dtype, which is dtype or f32) may be NULL, and either side may have no heads.
- * dim <= 512. */
+ * dim <= 256. */
 int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_heads *q, const vhip_heads *k, size_t tokens,
                         size_t heads, size_t kv_heads, size_t dim, const void *q_weight, const void *k_weight,
                         const int64_t *positions, const float *frequencies, size_t rotary, int interleaved, float eps,

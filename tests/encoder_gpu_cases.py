@@ -223,9 +223,9 @@ def head_norm_reference(x, w, angle, interleaved, eps, dy=None):
 # tokens, heads, key heads, dim, rotated columns, neighbouring pairs, padding between rows
 HEAD_NORMS = [
     (1, 12, 12, 64, 64, False, 0), (5, 32, 8, 128, 128, False, 8), (17, 4, 2, 80, 40, True, 0), (9, 3, 1, 33, 32, False, 1),
-    (3, 2, 2, 256, 64, False, 0), (2, 1, 1, 512, 512, True, 0), (130, 6, 2, 72, 72, True, 0), (40, 5, 5, 1, 0, False, 0),
+    (3, 2, 2, 256, 64, False, 0), (2, 1, 1, 256, 256, True, 0), (130, 6, 2, 72, 72, True, 0), (40, 5, 5, 1, 0, False, 0),
     (7, 2, 1, 7, 6, False, 0), (300, 2, 2, 20, 6, True, 3), (3000, 3, 1, 96, 96, False, 0), (0, 4, 2, 64, 64, False, 0),
-    (4, 4, 2, 64, 0, False, 0), (9000, 1, 1, 16, 16, True, 0), (2, 3, 0, 64, 64, False, 0), (3, 2, 1, 509, 300, False, 5),
+    (4, 4, 2, 64, 0, False, 0), (9000, 1, 1, 16, 16, True, 0), (2, 3, 0, 64, 64, False, 0), (3, 2, 1, 253, 150, False, 5), (3, 1, 2, 256, 2, True, 0),
 ]
 
 

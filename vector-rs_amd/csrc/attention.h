@@ -100,9 +100,11 @@ struct Heads {
 
 // ---- tiles in LDS ------------------------------------------------------------------------------
 
+// A cycle serves 256 bytes: 16 rows' same chunk, or the 64 bytes of each of 4 rows from 4 a on that half a wave reads by
+// transposing. Rows of 256 bytes give the 4 rows other quarters of the banks, and the 16 rows all sixteen chunks.
 constexpr int swz_of(int row_bytes, int r) {
-    return row_bytes % 256 == 0 ? ((r & 7) << 1) | ((r >> 3) & 1)
-           : row_bytes % 128 == 0 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1)
+    return row_bytes % 256 == 0 ? ((r & 3) << 2) | ((r >> 2) & 3)
+           : row_bytes % 128 == 0 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3)
                                   : (r >> 2) & 3;
 }
 
@@ -115,17 +117,28 @@ __device__ __forceinline__ void dma_lds16_far(const void *p, uint32_t m0_base) {
                  : "memory");
 }
 
+// A lane's number that the compiler takes for new: what is computed from it stays inside the loop that asks for it, where
+// it costs an instruction or two a tile and no register from one tile to the next.
+__device__ __forceinline__ int anew(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A tile of ROWS rows of DP values that NW waves load.
 template <class T, int DP, int ROWS, int NW, bool DMA>
 struct Tile {
-    static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, N = ROWS * CH / (NW * 64);
+    static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, N = (ROWS * CH + NW * 64 - 1) / (NW * 64);
     static constexpr int kBytes = ROWS * RB;
     static constexpr int VEC = 16 / (int)sizeof(T);
-    static_assert(N * NW * 64 == ROWS * CH, "whole loads");
+    // Where a row's chunks are a power of two, the rows of a thread's loads are STEP apart and its chunk is the same.
+    static constexpr int STEP = NW * 64 / CH;
+    static constexpr bool kWhole = N * NW * 64 == ROWS * CH;  // or the last load is some waves' only
+    static constexpr bool kEven = kWhole && (CH & (CH - 1)) == 0 && STEP % 16 == 0;  // 16: the rows' swizzle
+    static_assert(ROWS * CH % 64 == 0, "whole waves");
     static constexpr int swz(int r) { return swz_of(RB, r); }
 
-    static __device__ __forceinline__ void spot(int i, int &row, int &chunk) {
-        const int n = (i * NW + (int)(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63);
+    static __device__ __forceinline__ void spot(int i, int thread, int &row, int &chunk) {
+        const int n = i * NW * 64 + thread;
         row = n / CH;
         chunk = (n % CH) ^ swz(row);
     }
@@ -134,30 +147,76 @@ struct Tile {
     // there, or the result is not used); otherwise values come one vector at a time, zeros past dim.
     template <class At>
     static __device__ __forceinline__ void load(const char *base, const At &at, int dim, char *to) {
+        const int thread = anew(threadIdx.x);
+        const uint32_t lds = place(to);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int r, c;
+            spot(i, thread, r, c);
+            one(base, at(r), c, dim, to, lds, i, thread);
+        }
+    }
+    // The same where row r + STEP i is i `step` bytes after row r (kEven): one lane's offset for all loads.
+    template <class At>
+    static __device__ __forceinline__ void load_even(const char *base, const At &at, int64_t step, int dim, char *to) {
+        const int thread = anew(threadIdx.x);
+        const uint32_t lds = place(to);
+        int r, c;
+        spot(0, thread, r, c);
+        const auto off = at(r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) one(base + i * step, off, c, dim, to, lds, i, thread);
+    }
+
+   private:
+    static __device__ __forceinline__ uint32_t place(char *to) {
+        return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)to + (threadIdx.x >> 6) * 1024);
+    }
+    template <class Off>
+    static __device__ __forceinline__ void one(const char *base, Off off, int c, int dim, char *to, uint32_t lds, int i, int thread) {
+        if (!kWhole && i == N - 1 && (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= ROWS * CH / 64 - i * NW) return;
         if constexpr (DMA) {
             const int last = dim * (int)sizeof(T) / 16 - 1;
-            const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)to +
-                                                                (threadIdx.x >> 6) * 1024);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                int r, c;
-                spot(i, r, c);
-                if constexpr (sizeof(at(0)) == 4)
-                    dma_lds16_at(base, at(r) + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
-                else
-                    dma_lds16_far(base + at(r) + min(c, last) * 16, lds + i * NW * 1024);
-            }
+            if constexpr (sizeof(Off) == 4)
+                dma_lds16_at(base, off + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
+            else
+                dma_lds16_far(base + off + min(c, last) * 16, lds + i * NW * 1024);
         } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                int r, c;
-                spot(i, r, c);
-                const auto v = load_row<VEC>((const T *)(base + at(r)), c * VEC, dim);
-                *(Pack<T, VEC> *)(to + ((i * NW + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) * 16) = v;
-            }
+            const auto v = load_row<VEC>((const T *)(base + off), c * VEC, dim);
+            *(Pack<T, VEC> *)(to + (i * NW * 64 + thread) * 16) = v;
         }
     }
 };
+
+// A tile of consecutive rows from row0 on, of which those past `last` are copies of it; rows `stride` bytes apart, less
+// than 2^25.
+template <class TILE, int ROWS>
+__device__ __forceinline__ void load_rows(const char *base, int64_t stride, int row0, int last, int dim, char *to) {
+    const char *p = base + row0 * stride;
+    const uint32_t s = (uint32_t)stride;
+    last -= row0;
+    if (TILE::kEven && last >= ROWS - 1)
+        TILE::load_even(p, [&](int r) { return (uint32_t)r * s; }, TILE::STEP * stride, dim, to);
+    else
+        TILE::load(p, [&](int r) { return (uint32_t)min(r, last) * s; }, dim, to);
+}
+
+// A tile of packed rows from row0 on, those past `last` copies of it; base is token 0 of the group's first head.
+template <class TILE, int ROWS>
+__device__ __forceinline__ void load_packed(const char *base, const Heads &x, const Group &g, int row0, int last, int dim, char *to) {
+    const int tok0 = g.token(row0);
+    const char *p = base + tok0 * (int64_t)x.token;
+    if (TILE::kEven && last >= row0 + ROWS - 1 && g.shift >= 0 && TILE::STEP % g.size == 0) {
+        // the group divides STEP and so row0, a multiple of ROWS: the tile begins with the group's first head
+        TILE::load_even(p, [&](int r) { return (int64_t)(r >> g.shift) * (int64_t)x.token + (int64_t)(r & (g.size - 1)) * (int64_t)x.head; },
+                        (int64_t)(TILE::STEP >> g.shift) * (int64_t)x.token, dim, to);
+    } else {
+        TILE::load(p, [&](int i) {
+            const int r = min(row0 + i, last), token = g.token(r);
+            return (int64_t)(token - tok0) * (int64_t)x.token + (int64_t)(r - token * g.size) * (int64_t)x.head;
+        }, dim, to);
+    }
+}
 
 // ---- fragments and products --------------------------------------------------------------------
 
@@ -197,41 +256,51 @@ __device__ __forceinline__ typename Frag<T>::type rows_frag(const char *tile, in
     return *(const typename Frag<T>::type *)(tile + r * RB + ((2 * ks) ^ x) * 16 + r0 * RB);
 }
 
-// c += A^T B, where A's rows r0 .. r0 + 31 are the tile's, its columns 32 dt .. 32 dt + 31, and B is in the lanes'
-// registers as a product left it.
-template <class T, int RB, class V>
-__device__ __forceinline__ floatx16_t mma_cols(const char *tile, int r0, int dt, const V *b, floatx16_t c, int lane) {
+// Operand k (of kOps) of columns 32 dt .. 32 dt + 31 of the tile's rows r0 .. r0 + 31, the rows in the order in which a
+// product's registers hold its rows (see to_operand).
+template <class T>
+constexpr int kOps = sizeof(T) == 2 ? 2 : 4;
+template <class T, int RB>
+__device__ __forceinline__ typename Frag<T>::type cols_frag(const char *tile, int r0, int dt, int k, int lane) {
     if constexpr (sizeof(T) == 2) {
         typedef typename MmVec<T>::v4 v4;
-        typedef typename MmVec<T>::v8 v8;
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4 lds_s4;
         const int g = lane >> 4, i = lane & 15, r = 4 * (g >> 1) + (i >> 2);
         const int x = (2 * (g & 1) + ((i & 3) >> 1)) ^ swz_of(RB, r);
-        const char *p = tile + r * RB + (i & 1) * 8;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const char *q = p + (r0 + 16 * k) * RB;
-            const v4 lo = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q + ((4 * dt) ^ x) * 16)));
-            const v4 hi = __builtin_bit_cast(
-                v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q + 8 * RB + ((4 * dt) ^ x ^ swz_of(RB, 8)) * 16)));
-            c = mma(v8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), b[k], c);
-        }
+        const char *p = tile + r * RB + (i & 1) * 8 + (r0 + 16 * k) * RB;
+        const v4 lo = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + ((4 * dt) ^ x) * 16)));
+        const v4 hi = __builtin_bit_cast(
+            v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 8 * RB + ((4 * dt) ^ x ^ swz_of(RB, 8)) * 16)));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
         const int h = lane >> 5, x = ((lane & 31) >> 2) ^ swz_of(RB, 4 * h);
         const char *p = tile + (r0 + 4 * h) * RB + (lane & 3) * 4;
+        floatx4_t f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float a = *(const float *)(p + row_of(i) * RB + ((8 * dt) ^ x ^ swz_of(RB, row_of(i))) * 16);
-            c = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b[i / 4][i % 4], c, 0, 0, 0);
-        }
+        for (int e = 0; e < 4; ++e) f[e] = *(const float *)(p + row_of(4 * k + e) * RB + ((8 * dt) ^ x ^ swz_of(RB, row_of(4 * k + e))) * 16);
+        return f;
     }
-    return c;
+}
+
+// sum[d] += A^T B for the DT blocks of columns of A, the tile's rows r0 .. r0 + 31; B as to_operand gives it.
+template <class T, int RB, int DT>
+__device__ __forceinline__ void mma_cols(const char *tile, int r0, const typename Frag<T>::type (&b)[kOps<T>], floatx16_t (&sum)[DT], int lane) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int k = 0; k < kOps<T>; ++k) sum[d] = mma(cols_frag<T, RB>(tile, r0, d, k, lane), b[k], sum[d]);
+}
+// A B over KS steps, A the tile's rows r0 .. r0 + 31.
+template <class T, int RB, int KS>
+__device__ __forceinline__ floatx16_t mma_rows(const char *tile, int r0, const typename Frag<T>::type (&b)[KS], int lane) {
+    floatx16_t sum = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sum = mma(rows_frag<T, RB>(tile, r0, ks, lane), b[ks], sum);
+    return sum;
 }
 
 // The 16 values of a block as that operand: two of 8 in 16 bits, four of 4 in 32.
-template <class T>
-constexpr int kOps = sizeof(T) == 2 ? 2 : 4;
 template <class T>
 __device__ __forceinline__ void to_operand(const floatx16_t &v, typename Frag<T>::type (&o)[kOps<T>]) {
     constexpr int E = 16 / kOps<T>;
@@ -240,8 +309,6 @@ __device__ __forceinline__ void to_operand(const floatx16_t &v, typename Frag<T>
 #pragma unroll
         for (int e = 0; e < E; ++e) o[k][e] = (T)v[k * E + e];
 }
-
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 // Writes a lane's part of a transposed result: its row's values 32 dt + 8 (i / 4) + 4 (lane / 32) + i % 4.
 template <class T, int DT, class F>
@@ -258,6 +325,19 @@ __device__ __forceinline__ void store_cols(T *row, const floatx16_t (&acc)[DT], 
         }
 }
 
+// Both halves' values together, in every lane.
+template <class F>
+__device__ __forceinline__ float both_halves(float x, const F &f) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float half_max(float x) {
+    return both_halves(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float half_sum(float x) {
+    return both_halves(x, [](float a, float b) { return a + b; });
+}
+
 // Float16 has too few powers of two for a row's ds = p (dp - delta): what a lane's row or key adds up is held in
 // units of 2^-e, e as large as lets its largest |ds| so far stay below 2^15.  A value then loses what falls below
 // 2^-39 of that largest one.  Other types need none of it.
@@ -272,7 +352,7 @@ struct Units {
             float t = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) t = fmaxf(t, fabsf(ds[i]));
-            t = fmaxf(t, other_half(t));
+            t = half_max(t);
             const int next = t > 0.f ? min(e, 15 - __builtin_amdgcn_frexp_expf(t)) : e;
             if (__any(next != e)) {
                 const float f = ldexpf(1.f, next - e);
@@ -298,7 +378,8 @@ __device__ __forceinline__ void tiles_ready() {
     __syncthreads();
 }
 
-// The DP values of a row as DP / 4 threads' vectors of 4 (96 columns: 10 rows of 24 threads, and 16 idle ones).
+// The DP values of a row as DP / 4 threads' vectors of 4; a workgroup has as many rows, or parts of one, as fit (96 columns:
+// 10 of 24 threads, and 16 idle ones).
 template <int DP>
 constexpr int kRowsOf256 = 256 / (DP / 4);
 
@@ -309,13 +390,25 @@ struct Shape {
     size_t tokens, key_tokens, heads, kv_heads, dim, sequences;
 };
 inline size_t padded(size_t dim) { return round_up(dim, 32); }
-// Parts of the keys that a row sees, or of the rows that see a key: enough workgroups for some rounds of the GPU where
-// there are few, none shorter than `shortest` of an average sequence.  Lengths are on the device, so it goes by sizes.
-inline int split_count(int64_t workgroups, size_t along, size_t sequences, int shortest) {
+// Parts of what a workgroup walks along (the keys that rows see, the rows that see keys), each a workgroup of its own, where there
+// are fewer than `enough` workgroups; none is shorter than `shortest` of an average sequence.  Lengths are on the device, so
+// it goes by the sizes alone.
+constexpr int kMaxSplits = 64;
+inline int split_count(int64_t workgroups, size_t along, size_t sequences, int enough, int shortest) {
     const int64_t each = (int64_t)(along / (sequences ? sequences : 1)) / shortest;
-    int64_t n = 1024 / (workgroups ? workgroups : 1);
+    int64_t n = enough / (workgroups ? workgroups : 1);
     n = n < each ? n : each;
-    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : (int)n;
+}
+// Of the keys, for workgroups of `rows` rows: enough for two on each CU, and more, since sequences differ in length, as long as the parts'
+// sums (32 bits, written and read) stay below a quarter of the keys and values that are read: with few rows they do.
+inline int key_splits(int dtype, const Shape &s, int rows) {
+    const int64_t wgs = slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, rows) * s.kv_heads;
+    const int fill = split_count(wgs, s.key_tokens, s.sequences, 512, 256);
+    const int even = split_count(wgs, s.key_tokens, s.sequences, 4096, 256);
+    const size_t cheap = s.tokens ? s.key_tokens * s.kv_heads * dtype_size(dtype) / (s.tokens * s.heads * 16) : 0;
+    const int more = cheap < (size_t)even ? (int)cheap : even;
+    return fill > more ? fill : more;
 }
 inline Group to_group(size_t heads, size_t kv_heads) {
     const int n = (int)(heads / kv_heads);

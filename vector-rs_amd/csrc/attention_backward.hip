@@ -39,7 +39,16 @@ constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // keys, or rows, of a tile
 // Workgroups of a CU whose waves' registers hold all that they own: two have 256 a lane, one has 512.
 template <class T, int DP>
 struct RegsFor {
-    static constexpr int dq = sizeof(T) == 4 && DP > 96 ? 1 : 2, dkv = DP > 64 ? 1 : 2;
+    static constexpr int dq = sizeof(T) == 4 && DP > 96 ? 1 : 2;
+};
+
+// The kernel by keys: 4 waves of 32 keys each, where registers allow it twice: both halves of the waves have the same
+// keys, and every second block of 32 rows. The longest workgroup, not their sum, is what few long sequences wait for.
+template <class T, int DP>
+struct ByKeys {
+    static constexpr bool wide = sizeof(T) == 4 && DP > 64;
+    static constexpr int halves = wide ? 1 : 2, waves = 4 * halves;
+    static constexpr int rows = wide ? 32 : sizeof(T) == 4 ? 64 : 128;  // of a tile
 };
 
 // Power of two of p where it is an operand
@@ -89,10 +98,8 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
 
     const char *kb = a.k.data + keys.begin * a.k.token + kh * a.k.head, *vb = a.v.data + keys.begin * a.v.token + kh * a.v.head;
     auto load = [&](int t, int buf) {
-        const int last = keys.len - 1 - t * BN;
-        const uint32_t ks = (uint32_t)a.k.token, vs = (uint32_t)a.v.token;
-        KV::load(kb + (int64_t)t * BN * a.k.token, [&](int i) { return (uint32_t)min(i, last) * ks; }, a.dim, lds[buf][0]);
-        KV::load(vb + (int64_t)t * BN * a.v.token, [&](int i) { return (uint32_t)min(i, last) * vs; }, a.dim, lds[buf][1]);
+        load_rows<KV, BN>(kb, a.k.token, t * BN, keys.len - 1, a.dim, lds[buf][0]);
+        load_rows<KV, BN>(vb, a.v.token, t * BN, keys.len - 1, a.dim, lds[buf][1]);
     };
     if (t0 < t1) load(t0, 0);
 
@@ -109,7 +116,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
 #pragma unroll
             for (int e = 0; e < VEC; ++e) delta = fmaf((float)go[ks][e], (float)x.v[e], delta);
         }
-        delta += other_half(delta);
+        delta = half_sum(delta);
         if (split == 0 && half == 0 && r < n) a.delta[at_row] = delta;
     }
     const float lse = a.lse[at_row], c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
@@ -125,11 +132,8 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
         for (int j = 0; j < NS; ++j) {
             const int key0 = t * BN + 32 * j;
             if (key0 >= any) break;
-            floatx16_t s = {}, dp = {};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mma(rows_frag<T, RB>(lds[buf][0], 32 * j, ks, lane), q[ks], s);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) dp = mma(rows_frag<T, RB>(lds[buf][1], 32 * j, ks, lane), go[ks], dp);
+            floatx16_t s = mma_rows<T, RB>(lds[buf][0], 32 * j, q, lane);
+            floatx16_t dp = mma_rows<T, RB>(lds[buf][1], 32 * j, go, lane);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, base)) * (dp[i] - delta);
             if (key0 + 32 > all) {
@@ -141,8 +145,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
             units.to_units(s, dq);
             frag ds[kOps<T>];
             to_operand<T>(s, ds);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dq[d] = mma_cols<T, RB>(lds[buf][0], 32 * j, d, ds, dq[d], lane);
+            mma_cols<T, RB>(lds[buf][0], 32 * j, ds, dq, lane);
         }
     }
     if (r >= n) return;
@@ -154,11 +157,12 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
 }
 
 template <class T, int DP, bool DMA>
-__global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs a) {
-    constexpr int BR = kBN<T>, NS = BR / 32, RB = DP * (int)sizeof(T), KS = RB / 32, DT = DP / 32;
+__global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves)) void k_attn_dkv(BwdArgs a) {
+    constexpr int NW = ByKeys<T, DP>::waves, HALVES = ByKeys<T, DP>::halves, BR = ByKeys<T, DP>::rows, NS = BR / 32, RB = DP * (int)sizeof(T), KS = RB / 32, DT = DP / 32;
     typedef typename Frag<T>::type frag;
-    typedef Tile<T, DP, BR, 4, DMA> QG;
+    typedef Tile<T, DP, BR, NW, DMA> QG;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][QG::kBytes];
+    static_assert(HALVES == 1 || 4 * QG::kBytes >= 4 * DT * 4096, "room for one half's sums");
     __shared__ __attribute__((aligned(16))) float stats[2][2][BR];  // -lse in base 2, delta
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
@@ -171,7 +175,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs
     const Span rows = real ? packed_span(a.rows, at.seq) : Span{0, 0};
     const int n = rows.len * a.group.size, g = a.group.size;
     // the first keys of a sequence are seen by the most rows
-    const int key0 = at.tile * kBK, w0 = key0 + wave * 32;
+    const int key0 = at.tile * kBK, w0 = key0 + (wave & 3) * 32, row_half = wave >> 2;
 
     // this lane's key, and the first row that sees it: of the lane, of the wave's first and last key, of the workgroup
     const int j = w0 + (lane & 31), back = rows.len - keys.len;
@@ -184,19 +188,15 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs
     const char *gb = a.go.data + rows.begin * a.go.token + (int64_t)kh * g * a.go.head;
     float next_lse = 0.f, next_delta = 0.f;
     auto load = [&](int t, int buf) {
-        const int r0 = t * BR, tok0 = a.group.token(r0);
+        const int r0 = t * BR;
         if (threadIdx.x < BR) {
             const int r = min(r0 + (int)threadIdx.x, n - 1), token = a.group.token(r);
             const int64_t i = (rows.begin + token) * a.heads + kh * g + r - token * g;
             next_lse = a.lse[i];
             next_delta = a.delta[i];
         }
-        auto far = [&](int i, const Heads &x) {
-            const int r = min(r0 + i, n - 1), token = a.group.token(r);
-            return (int64_t)(token - tok0) * (int64_t)x.token + (int64_t)(r - token * g) * (int64_t)x.head;
-        };
-        QG::load(qb + tok0 * (int64_t)a.q.token, [&](int i) { return far(i, a.q); }, a.dim, lds[buf][0]);
-        QG::load(gb + tok0 * (int64_t)a.go.token, [&](int i) { return far(i, a.go); }, a.dim, lds[buf][1]);
+        load_packed<QG, BR>(qb, a.q, a.group, r0, n - 1, a.dim, lds[buf][0]);
+        load_packed<QG, BR>(gb, a.go, a.group, r0, n - 1, a.dim, lds[buf][1]);
     };
     auto put_stats = [&](int buf) {
         if (threadIdx.x < BR) {
@@ -221,15 +221,13 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs
         tiles_ready();
         const int buf = (t - t0) & 1;
         if (t + 1 < t1) load(t + 1, buf ^ 1);
-#pragma unroll
-        for (int b = 0; b < NS; ++b) {
+#pragma unroll 1
+        for (int h = 0; h < NS / HALVES; ++h) {
+            const int b = h * HALVES + row_half, ln = anew(lane);
             const int r0 = t * BR + 32 * b;
             if (r0 + 32 <= wave_first || r0 >= n) continue;
-            floatx16_t s = {}, dp = {};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mma(rows_frag<T, RB>(lds[buf][0], 32 * b, ks, lane), k[ks], s);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) dp = mma(rows_frag<T, RB>(lds[buf][1], 32 * b, ks, lane), v[ks], dp);
+            floatx16_t s = mma_rows<T, RB>(lds[buf][0], 32 * b, k, ln);
+            floatx16_t dp = mma_rows<T, RB>(lds[buf][1], 32 * b, v, ln);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const Pack<float, 4> l = *(const Pack<float, 4> *)&stats[buf][0][32 * b + row_of(i) + 4 * half];
@@ -248,28 +246,53 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dkv)) void k_attn_dkv(BwdArgs
             }
             frag p[kOps<T>];
             to_operand<T>(s, p);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dv[d] = mma_cols<T, RB>(lds[buf][1], 32 * b, d, p, dv[d], lane);
+            __builtin_amdgcn_sched_barrier(0);  // operands read ahead of these would not fit the registers
+            mma_cols<T, RB>(lds[buf][1], 32 * b, p, dv, ln);
+            __builtin_amdgcn_sched_barrier(0);
             units.to_units(dp, dk);
             frag ds[kOps<T>];
             to_operand<T>(dp, ds);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dk[d] = mma_cols<T, RB>(lds[buf][0], 32 * b, d, ds, dk[d], lane);
+            mma_cols<T, RB>(lds[buf][0], 32 * b, ds, dk, ln);
         }
         if (t + 1 < t1) put_stats(buf ^ 1);
     }
-    if (j >= keys.len) return;
     const float shrink = kShift<T> > 0.f ? 1.f / 16384.f : 1.f;
-    auto kvalue = [&](float x) { return units.back(x) * (a.scale * shrink); };
-    auto vvalue = [&](float x) { return x * shrink; };
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            dk[d][i] = units.back(dk[d][i]) * (a.scale * shrink);
+            dv[d][i] *= shrink;
+        }
+    if constexpr (HALVES == 2) {  // the second half's sums go through LDS
+        float *sums = (float *)&lds[0][0][0] + (wave & 3) * DT * 1024 + lane;
+        auto join = [&](floatx16_t (&x)[DT]) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (row_half) sums[(d * 16 + i) * 64] = x[d][i];
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!row_half) x[d][i] += sums[(d * 16 + i) * 64];
+        };
+        join(dk);
+        join(dv);
+    }
+    if (row_half || j >= keys.len) return;
+    auto same = [](float x) { return x; };
     const int64_t row = keys.begin + j;
     if (a.splits > 1) {
         const int64_t all = a.keys.tokens * a.kv_heads, i = row * a.kv_heads + kh;
-        store_cols<float, DT>(a.part + ((2 * split) * all + i) * DP, dk, DP, lane, kvalue);
-        store_cols<float, DT>(a.part + ((2 * split + 1) * all + i) * DP, dv, DP, lane, vvalue);
+        store_cols<float, DT>(a.part + ((2 * split) * all + i) * DP, dk, DP, lane, same);
+        store_cols<float, DT>(a.part + ((2 * split + 1) * all + i) * DP, dv, DP, lane, same);
     } else {
-        store_cols<T, DT>((T *)(a.dk.data + row * (int64_t)a.dk.token + (int64_t)kh * a.dk.head), dk, a.dim, lane, kvalue);
-        store_cols<T, DT>((T *)(a.dv.data + row * (int64_t)a.dv.token + (int64_t)kh * a.dv.head), dv, a.dim, lane, vvalue);
+        store_cols<T, DT>((T *)(a.dk.data + row * (int64_t)a.dk.token + (int64_t)kh * a.dk.head), dk, a.dim, lane, same);
+        store_cols<T, DT>((T *)(a.dv.data + row * (int64_t)a.dv.token + (int64_t)kh * a.dv.head), dv, a.dim, lane, same);
     }
 }
 
@@ -284,6 +307,7 @@ __global__ __launch_bounds__(256) void k_attn_sum(BwdArgs a) {
     if (threadIdx.x >= R * L || i >= all || e >= a.dim) return;
     const int which = KEYS ? blockIdx.y : 0;
     float sum[4] = {};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const Pack<float, 4> p = load_any<4>(a.part + ((KEYS ? 2 * s + which : s) * all + i) * DP + e);
 #pragma unroll
@@ -302,10 +326,15 @@ struct Work {
     float *delta, *part;
     size_t bytes;
 };
-Work work_of(const Shape &s, void *base) {
+Work work_of(int dtype, const Shape &s, void *base) {
     Work w;
-    w.qsplits = split_count(slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads, s.key_tokens, s.sequences, 256);
-    w.ksplits = split_count(slot_count(s.key_tokens, s.sequences, 1, kBK) * s.kv_heads, s.tokens * (s.heads / s.kv_heads), s.sequences, 256);
+    w.qsplits = key_splits(dtype, s, kBM);
+    // By keys a workgroup walks all rows of a group, so the longest sequence's decide. Parts cost a pass over sums of 32 bits:
+    // 2048 rows at least where it is to even workgroups out, fewer where there are too few of them.
+    const int64_t wgs = slot_count(s.key_tokens, s.sequences, 1, kBK) * s.kv_heads;
+    const size_t along = s.tokens * (s.heads / s.kv_heads);
+    const int fill = split_count(wgs, along, s.sequences, 512, 256), even = split_count(wgs, along, s.sequences, 2048, 2048);
+    w.ksplits = fill > even ? fill : even;
     const size_t dp = padded(s.dim);
     const size_t q = w.qsplits > 1 ? w.qsplits * s.tokens * s.heads * dp : 0;
     const size_t k = w.ksplits > 1 ? 2 * w.ksplits * s.key_tokens * s.kv_heads * dp : 0;
@@ -336,9 +365,9 @@ int launch(BwdArgs a, const Run &r) {
     if (r.kgrid) {
         a.splits = r.w.ksplits;
         if (r.dma_q)
-            k_attn_dkv<T, DP, true><<<r.kgrid, 256, 0, r.s>>>(a);
+            k_attn_dkv<T, DP, true><<<r.kgrid, 64 * ByKeys<T, DP>::waves, 0, r.s>>>(a);
         else
-            k_attn_dkv<T, DP, false><<<r.kgrid, 256, 0, r.s>>>(a);
+            k_attn_dkv<T, DP, false><<<r.kgrid, 64 * ByKeys<T, DP>::waves, 0, r.s>>>(a);
         if (a.splits > 1)
             k_attn_sum<T, DP, true><<<dim3((uint32_t)ceil_div(a.keys.tokens * a.kv_heads, kRowsOf256<DP>), 2), 256, 0, r.s>>>(a);
     }
@@ -365,9 +394,8 @@ extern "C" {
 
 size_t vhip_attention_backward_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                          size_t sequences) {
-    (void)dtype;
-    if (!kv_heads || !heads) return 0;
-    return work_of({tokens, key_tokens, heads, kv_heads, dim, sequences}, nullptr).bytes;
+    if (!kv_heads || !heads || !dtype_known(dtype)) return 0;
+    return work_of(dtype, {tokens, key_tokens, heads, kv_heads, dim, sequences}, nullptr).bytes;
 }
 
 int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, const vhip_heads *q, const vhip_heads *k,
@@ -388,7 +416,7 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
     VH_CHECK(check_heads("dk", dk, dtype, key_tokens, kv_heads, dim));
     VH_CHECK(check_heads("dv", dv, dtype, key_tokens, kv_heads, dim));
     Run r;
-    r.w = work_of(sh, workspace);
+    r.w = work_of(dtype, sh, workspace);
     if (r.w.bytes && (!workspace || workspace_bytes < r.w.bytes || !aligned16(workspace)))
         return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_attention_backward_workspace() or not aligned");
     const int64_t qgrid = slot_count(tokens, sequences, heads / kv_heads, kBM) * (int64_t)kv_heads * r.w.qsplits;

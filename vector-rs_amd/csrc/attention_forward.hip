@@ -27,6 +27,7 @@ struct FwdArgs {
 };
 
 constexpr int kBM = 128;
+constexpr int kFew = 8;  // parts
 
 // Keys of a tile: 64, or 32 where they have 32 bits (two buffers of K and V of 128 columns in 64 KB, two workgroups a CU).
 template <class T>
@@ -72,10 +73,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
 
     const char *kb = a.k.data + keys.begin * a.k.token + kh * a.k.head, *vb = a.v.data + keys.begin * a.v.token + kh * a.v.head;
     auto load = [&](int t, int buf) {
-        const int last = keys.len - 1 - t * BN;
-        const uint32_t ks = (uint32_t)a.k.token, vs = (uint32_t)a.v.token;
-        KV::load(kb + (int64_t)t * BN * a.k.token, [&](int i) { return (uint32_t)min(i, last) * ks; }, a.dim, lds[buf][0]);
-        KV::load(vb + (int64_t)t * BN * a.v.token, [&](int i) { return (uint32_t)min(i, last) * vs; }, a.dim, lds[buf][1]);
+        load_rows<KV, BN>(kb, a.k.token, t * BN, keys.len - 1, a.dim, lds[buf][0]);
+        load_rows<KV, BN>(vb, a.v.token, t * BN, keys.len - 1, a.dim, lds[buf][1]);
     };
     if (t0 < t1) load(t0, 0);
 
@@ -101,11 +100,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
         const int key0 = t * BN;
         if (key0 >= any) continue;
 
-        floatx16_t s[NS] = {};
+        floatx16_t s[NS];
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[j] = mma(rows_frag<T, RB>(lds[buf][0], 32 * j, ks, lane), q[ks], s[j]);
+        for (int j = 0; j < NS; ++j) s[j] = mma_rows<T, RB>(lds[buf][0], 32 * j, q, lane);
         if (key0 + BN > all) {
             const int left = sees - key0 - 4 * half;
 #pragma unroll
@@ -119,7 +116,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
         for (int j = 0; j < NS; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
-        top = fmaxf(top, other_half(top)) * c;
+        top = half_max(top) * c;
         if (__any(top > m + 8.f)) {
             const float next = fmaxf(m, top);
             const float f = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
@@ -144,17 +141,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
         for (int j = 0; j < NS; ++j) {
             frag p[kOps<T>];
             to_operand<T>(s[j], p);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = mma_cols<T, RB>(lds[buf][1], 32 * j, d, p, o[d], lane);
+            mma_cols<T, RB>(lds[buf][1], 32 * j, p, o, lane);
         }
     }
     if (r >= n) return;
-    l += other_half(l);
+    l = half_sum(l);
     const int64_t at_row = row * a.heads + head;
     if (a.splits > 1) {
         const int64_t i = ((int64_t)split * a.rows.tokens * a.heads) + at_row;
         if (half == 0) a.stats[i] = make_float2(m, l);
-        if (m != -INFINITY) store_cols<float, DT>(a.part + i * DP, o, DP, lane, [](float x) { return x; });
+        if (l != 0.f) store_cols<float, DT>(a.part + i * DP, o, DP, lane, [](float x) { return x; });
         return;
     }
     const float f = l == 0.f ? 0.f : 1.f / l;
@@ -163,25 +159,30 @@ __global__ __launch_bounds__(256, 2) void k_attn_forward(FwdArgs a) {
                       [&](float x) { return x * f; });
 }
 
-// A row's parts: its largest m, and their outputs and sums over it.  A row of DP values has DP / 4 lanes.
+// A row's parts: its largest m, and their outputs and sums over it.  For few parts; DP / 4 threads a row.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
-    constexpr int L = DP / 4, R = kRowsOf256<DP>;
-    const int64_t all = a.rows.tokens * a.heads;
-    const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
-    if (threadIdx.x >= R * L || i >= all) return;
+__global__ __launch_bounds__(256) void k_attn_join_few(FwdArgs a) {
+    constexpr int L = DP / 4, G = kRowsOf256<DP>;
+    const int64_t all = a.rows.tokens * a.heads, i = (int64_t)blockIdx.x * G + threadIdx.x / L;
+    if (threadIdx.x >= G * L || i >= all) return;
     const int e = threadIdx.x % L * 4;
+    float2 st[kFew];
+    Pack<float, 4> p[kFew];
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stats[s * all + i].x);
-    float l = 0.f, o[4] = {};
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 st = a.stats[s * all + i];
-        if (st.x == -INFINITY) continue;  // nothing is written there
-        const float f = __builtin_amdgcn_exp2f(st.x - m);
-        l = fmaf(st.y, f, l);
-        const Pack<float, 4> p = load_any<4>(a.part + (s * all + i) * DP + e);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = fmaf(p.v[k], f, o[k]);
+    for (int s = 0; s < kFew; ++s) {
+        st[s] = s < a.splits ? a.stats[s * all + i] : make_float2(-INFINITY, 0.f);
+        if (s < a.splits) p[s] = load_any<4>(a.part + (s * all + i) * DP + e);  // of no meaning where the part saw no key
+        m = fmaxf(m, st[s].x);
+    }
+    float l = 0.f, o[4] = {};
+#pragma unroll
+    for (int s = 0; s < kFew; ++s) {
+        if (st[s].y == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(st[s].x - m);
+        l = fmaf(st[s].y, f, l);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(p[s].v[k], f, o[k]);
     }
     const int64_t token = i / a.heads, head = i % a.heads;
     const float f = l == 0.f ? 0.f : 1.f / l;
@@ -192,8 +193,53 @@ __global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
     if (e < a.dim) store_row<4>((T *)(a.out.data + token * (int64_t)a.out.token + head * (int64_t)a.out.head), e, a.dim, v);
 }
 
-int splits_of(const Shape &s) {
-    return split_count(slot_count(s.tokens, s.sequences, s.heads / s.kv_heads, kBM) * s.kv_heads, s.key_tokens, s.sequences, 256);
+// The same for many parts, a workgroup a row: its largest m, and the parts' outputs and sums over it.  Lanes hold the parts' weights, and
+// every G-th part goes to another group of threads.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
+    constexpr int L = DP / 4, G = kRowsOf256<DP>;
+    __shared__ float weight[kMaxSplits];
+    __shared__ bool seen[kMaxSplits];
+    __shared__ __attribute__((aligned(16))) float sums[G][DP];
+    const int64_t all = a.rows.tokens * a.heads, i = blockIdx.x;
+    const int lane = threadIdx.x & 63, g = threadIdx.x / L, e = threadIdx.x % L * 4;
+    const float2 st = lane < a.splits ? a.stats[lane * all + i] : make_float2(-INFINITY, 0.f);
+    float m = st.x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float w = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - m);  // 0: a part that saw no key
+    const float l = lane_sum<64>(st.y * w);
+    if (threadIdx.x < a.splits) {
+        weight[threadIdx.x] = w;
+        seen[threadIdx.x] = st.y != 0.f;
+    }
+    __syncthreads();
+    float o[4] = {};
+    if (g < G) {
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += G) {
+            const float f = weight[s];
+            if (!seen[s]) continue;  // nothing is written there
+            const Pack<float, 4> p = load_any<4>(a.part + (s * all + i) * DP + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = fmaf(p.v[k], f, o[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[g][e + k] = o[k];
+    }
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int q = 1; q < G; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] += sums[q][e + k];
+    const int64_t token = i / a.heads, head = i % a.heads;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (a.lse && e == 0) a.lse[i] = (m - kShift<T> + __builtin_amdgcn_logf(l)) * kLn2;
+    Pack<T, 4> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v.v[k] = (T)(o[k] * f);
+    if (e < a.dim) store_row<4>((T *)(a.out.data + token * (int64_t)a.out.token + head * (int64_t)a.out.head), e, a.dim, v);
 }
 
 template <class T, int DP>
@@ -202,9 +248,10 @@ int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
         k_attn_forward<T, DP, true><<<grid, 256, 0, s>>>(a);
     else
         k_attn_forward<T, DP, false><<<grid, 256, 0, s>>>(a);
-    if (a.splits > 1) {
-        k_attn_join<T, DP><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, s>>>(a);
-    }
+    if (a.splits > kFew)
+        k_attn_join<T, DP><<<(uint32_t)(a.rows.tokens * a.heads), 256, 0, s>>>(a);
+    else if (a.splits > 1)
+        k_attn_join_few<T, DP><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, s>>>(a);
     return launch_status("attention launch");
 }
 template <class T>
@@ -265,9 +312,8 @@ extern "C" {
 
 size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                 size_t sequences) {
-    (void)dtype;
-    if (!kv_heads || !heads) return 0;
-    const int n = splits_of({tokens, key_tokens, heads, kv_heads, dim, sequences});
+    if (!kv_heads || !heads || !dtype_known(dtype)) return 0;
+    const int n = key_splits(dtype, {tokens, key_tokens, heads, kv_heads, dim, sequences}, kBM);
     return n > 1 ? n * tokens * heads * (padded(dim) * sizeof(float) + sizeof(float2)) : 0;
 }
 
@@ -282,7 +328,7 @@ int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads
     VH_CHECK(check_heads("k", k, dtype, key_tokens, kv_heads, dim));
     VH_CHECK(check_heads("v", v, dtype, key_tokens, kv_heads, dim));
     VH_CHECK(check_heads("out", out, dtype, tokens, heads, dim));
-    const int splits = splits_of(sh);
+    const int splits = key_splits(dtype, sh, kBM);
     if (splits > 1 && (!workspace || workspace_bytes < vhip_attention_workspace(dtype, tokens, key_tokens, heads, kv_heads, dim, sequences) ||
                        !aligned16(workspace)))
         return set_error(VHIP_ERR_INVALID_CONFIG, "the workspace is smaller than vhip_attention_workspace() or not aligned");

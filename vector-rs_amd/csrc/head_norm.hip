@@ -4,26 +4,26 @@
 //   a' = a cos t - b sin t,  b' = a sin t + b cos t  (columns past the pairs stay as they are)
 //   backward: dn = dy turned back,  xh = x r,  u = dn w:  dx = r (u - xh mean(u xh)),  dw = sum over rows of dn xh
 //
-// Both passes are bound by memory: a row is read once into the registers of L lanes, which hold both columns of
-// each of their pairs (pairs of halves: a vector of the first half and its counterpart of the second; neighbouring pairs:
-// two vectors one after the other), so nothing is exchanged but the row's sums. L is a power of two of at least dim / 2
-// vectors. A workgroup takes a few tokens at a time and makes their cosines and sines once in LDS, for all heads.
+// Both passes are bound by memory: a row is read once into the registers of a few lanes, two vectors each. A lane that turns
+// pairs holds both columns of them (pairs of halves: a vector of the first half and its counterpart of the second; neighbouring
+// pairs: two vectors one after the other), so nothing is exchanged but the row's sums; the columns behind the pairs have lanes of
+// their own. A workgroup takes a few tokens and makes their cosines and sines once in LDS, for all heads; some of its
+// waves have the queries, the others the keys, in proportion to their heads.
 //
 // Angles are products in 64 bits, taken modulo a quarter turn there: at position 10^6 a 32-bit product is off by 0.03.
 // What is left, at most pi / 4, goes into the Taylor polynomials of sine and cosine in 32 bits, whose remainders
 // (pi / 4)^11 / 11! and (pi / 4)^12 / 12! are below half a unit of them.
 //
-// The weights' gradients are sums over all rows: a workgroup keeps its columns' sums in registers over its tokens,
-// leaves them in a row of the workspace, and a second kernel adds those rows in a fixed order.
+// The weights' gradients are sums over all rows: a lane keeps its columns' sums in registers over its rows, a workgroup leaves
+// those of its waves in a row of the workspace, and a second kernel adds the rows in a fixed order.
 #include "train_common.h"
 
 namespace vh {
 namespace {
 
-constexpr int kTok = 8;                // tokens a workgroup has at a time, at most
-constexpr int kMaxPairs = 256;         // of a row
-constexpr int kMaxDim = 2 * kMaxPairs;
-constexpr size_t kMaxParts = 1024;     // workgroups of the backward pass: rows of partial sums
+constexpr int kTok = 8;            // tokens of a turn, at most
+constexpr int kMaxDim = 256, kMaxPairs = kMaxDim / 2;  // 34 lanes of 32-bit values at most: a row is a wave's
+constexpr size_t kMaxParts = 1024;  // workgroups of the backward pass: rows of partial sums
 
 struct Side {
     const char *x, *dy;  // dy: backward
@@ -39,43 +39,50 @@ struct HeadArgs {
     const float *frequencies;
     float *part;  // backward: [workgroup][2][dim]
     int64_t tokens;
-    int dim, pairs, lanes_log2, at_once;  // at_once: tokens of a turn
+    int dim, pairs, lanes_log2, at_once;  // lanes of a row; tokens of a turn
+    int key_waves;                        // of 4
     bool f32_params;
     float eps;
 };
 
-// A lane's columns of a row: the first and the second vectors of its pairs, and two of what is not turned.
+// A lane's columns of a row, two vectors: of pairs (lanes below ceil(pairs / VEC)), or of what is not turned.
 template <class T, bool NEAR>
 struct Columns {
     static constexpr int VEC = 16 / (int)sizeof(T);
-    int c[4], end[4];
-    __device__ __forceinline__ Columns(int t, int lanes, int dim, int pairs) {
-        const int v = t * VEC;
-        c[0] = NEAR ? 2 * v : v;
-        c[1] = NEAR ? 2 * v + VEC : pairs + v;
-        end[0] = NEAR ? 2 * pairs : pairs;
-        end[1] = 2 * pairs;
-        c[2] = 2 * pairs + v;
-        c[3] = c[2] + lanes * VEC;
-        end[2] = end[3] = dim;
-    }
-    template <class U>
-    __device__ __forceinline__ void load(float (&v)[4][VEC], const U *row) const {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (c[s] < end[s]) {
-                const Pack<U, VEC> p = load_row<VEC>(row, c[s], end[s]);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[s][e] = (float)p.v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[s][e] = 0.f;
-            }
+    typedef float Values[2][VEC];
+    int c[2], end[2];
+    int first_pair, count;  // of the lane's pairs
+    __device__ __forceinline__ Columns(int t, int dim, int pairs) {
+        const int turning = (pairs + VEC - 1) / VEC, v = t * VEC;
+        if (t < turning) {
+            c[0] = NEAR ? 2 * v : v;
+            c[1] = NEAR ? 2 * v + VEC : pairs + v;
+            end[0] = NEAR ? 2 * pairs : pairs;
+            end[1] = 2 * pairs;
+            first_pair = v;
+            count = min(VEC, pairs - v);
+        } else {
+            c[0] = 2 * pairs + 2 * (t - turning) * VEC;
+            c[1] = c[0] + VEC;
+            end[0] = end[1] = dim;
+            first_pair = count = 0;
         }
     }
-    __device__ __forceinline__ void store(T *row, const float (&v)[4][VEC]) const {
+    template <class U>
+    __device__ __forceinline__ void load(Values &v, const U *row) const {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 2; ++s) {
+            Pack<U, VEC> p;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p.v[e] = (U)0.f;
+            if (c[s] < end[s]) p = load_row<VEC>(row, c[s], end[s]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[s][e] = (float)p.v[e];
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const Values &v) const {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
             if (c[s] < end[s]) {
                 Pack<T, VEC> p;
 #pragma unroll
@@ -83,21 +90,18 @@ struct Columns {
                 store_row<VEC>(row, c[s], end[s], p);
             }
     }
-    // Pair e of the lane: both its values
-    static __device__ __forceinline__ float &first(float (&v)[4][VEC], int e) { return NEAR ? v[2 * e / VEC][2 * e % VEC] : v[0][e]; }
-    static __device__ __forceinline__ float &second(float (&v)[4][VEC], int e) {
-        return NEAR ? v[2 * e / VEC][2 * e % VEC + 1] : v[1][e];
-    }
-    // Turns the lane's pairs by cs (cosines, sines of the row's token), or back.
-    __device__ __forceinline__ void turn(float (&v)[4][VEC], const float2 *cs, int t, int pairs, bool back) const {
+    // Turns the lane's pairs by cs (cosines and sines of the row's token), or back.
+    template <bool BACK>
+    __device__ __forceinline__ void turn(Values &v, const float2 *cs) const {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            if (t * VEC + e >= pairs) continue;
-            const float2 p = cs[t * VEC + e];
-            const float s = back ? -p.y : p.y;
-            const float a = first(v, e), b = second(v, e);
-            first(v, e) = a * p.x - b * s;
-            second(v, e) = a * s + b * p.x;
+            if (e >= count) break;
+            const float2 p = cs[first_pair + e];
+            const float s = BACK ? -p.y : p.y;
+            float &x = NEAR ? v[2 * e / VEC][2 * e % VEC] : v[0][e], &y = NEAR ? v[2 * e / VEC][2 * e % VEC + 1] : v[1][e];
+            const float a = x, b = y;
+            x = a * p.x - b * s;
+            y = a * s + b * p.x;
         }
     }
 };
@@ -126,14 +130,26 @@ __device__ __forceinline__ float row_lanes_sum(float x, int lanes_log2) {
     return x;
 }
 
+// Which side a wave has, and its place among that side's.
+struct Waves {
+    int side, slot, slots, t;
+    __device__ __forceinline__ explicit Waves(const HeadArgs &a) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, rows = 64 >> a.lanes_log2;
+        side = wave >= 4 - a.key_waves;
+        slot = (side ? wave - (4 - a.key_waves) : wave) * rows + (lane >> a.lanes_log2);
+        slots = (side ? a.key_waves : 4 - a.key_waves) * rows;
+        t = lane & ((1 << a.lanes_log2) - 1);
+    }
+};
+
 template <class T, bool NEAR>
-__device__ __forceinline__ void load_weight(float (&w)[4][16 / (int)sizeof(T)], const Columns<T, NEAR> &cols, const HeadArgs &a,
+__device__ __forceinline__ void load_weight(typename Columns<T, NEAR>::Values &w, const Columns<T, NEAR> &cols, const HeadArgs &a,
                                             const void *weight) {
     if (!weight) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int e = 0; e < 16 / (int)sizeof(T); ++e) w[s][e] = 1.f;
+            for (int e = 0; e < Columns<T, NEAR>::VEC; ++e) w[s][e] = 1.f;
     } else if (a.f32_params) {
         cols.load(w, (const float *)weight);
     } else {
@@ -146,34 +162,32 @@ __global__ __launch_bounds__(256) void k_head_forward(HeadArgs a) {
     typedef Columns<T, NEAR> Cols;
     constexpr int VEC = Cols::VEC;
     __shared__ float2 cs[kTok][kMaxPairs];
-    const int lanes = 1 << a.lanes_log2, t = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2, slots = 256 >> a.lanes_log2;
-    const Cols cols(t, lanes, a.dim, a.pairs);
+    const Waves at(a);
+    const Cols cols(at.t, a.dim, a.pairs);
+    const Side &side = a.side[at.side];
     const int64_t tok0 = (int64_t)blockIdx.x * a.at_once;
     const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
+    typename Cols::Values w;
+    load_weight<T, NEAR>(w, cols, a, side.weight);
     make_turns(a, tok0, count, cs);
     __syncthreads();
     const float inv = 1.f / (float)a.dim;
-    for (int s = 0; s < 2; ++s) {
-        const Side &side = a.side[s];
-        float w[4][VEC];
-        load_weight<T, NEAR>(w, cols, a, side.weight);
-        for (int i = slot; i < count * side.heads; i += slots) {
-            const int k = i / side.heads, h = i - k * side.heads;
-            float x[4][VEC];
-            cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
-            float sum = 0.f;
+    for (int i = at.slot; i < count * side.heads; i += at.slots) {
+        const int k = i / side.heads, h = i - k * side.heads;
+        typename Cols::Values x;
+        cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
+        float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) sum = fmaf(x[v][e], x[v][e], sum);
-            const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
+            for (int e = 0; e < VEC; ++e) sum = fmaf(x[v][e], x[v][e], sum);
+        const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) x[v][e] *= r * w[v][e];
-            cols.turn(x, cs[k], t, a.pairs, false);
-            cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
-        }
+            for (int e = 0; e < VEC; ++e) x[v][e] *= r * w[v][e];
+        cols.template turn<false>(x, cs[k]);
+        cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
     }
 }
 
@@ -182,95 +196,106 @@ __global__ __launch_bounds__(256) void k_head_backward(HeadArgs a) {
     typedef Columns<T, NEAR> Cols;
     constexpr int VEC = Cols::VEC;
     __shared__ float2 cs[kTok][kMaxPairs];
-    __shared__ float sums[kMaxDim];
-    const int lanes = 1 << a.lanes_log2, t = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2, slots = 256 >> a.lanes_log2;
-    const Cols cols(t, lanes, a.dim, a.pairs);
+    __shared__ float sums[4][kMaxDim];
+    const Waves at(a);
+    const Cols cols(at.t, a.dim, a.pairs);
+    const Side &side = a.side[at.side];
     const float inv = 1.f / (float)a.dim;
-    for (int s = 0; s < 2; ++s) {
-        const Side &side = a.side[s];
-        float w[4][VEC], dw[4][VEC] = {};
-        load_weight<T, NEAR>(w, cols, a, side.weight);
-        for (int64_t tok0 = (int64_t)blockIdx.x * a.at_once; tok0 < a.tokens; tok0 += (int64_t)gridDim.x * a.at_once) {
-            const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
-            __syncthreads();
-            make_turns(a, tok0, count, cs);
-            __syncthreads();
-            for (int i = slot; i < count * side.heads; i += slots) {
-                const int k = i / side.heads, h = i - k * side.heads;
-                float x[4][VEC], g[4][VEC];
-                cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
-                cols.load(g, (const T *)(side.dy + (tok0 + k) * side.dy_token + h * side.dy_head));
-                cols.turn(g, cs[k], t, a.pairs, true);
-                float sum = 0.f, dot = 0.f;
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        sum = fmaf(x[v][e], x[v][e], sum);
-                        dot = fmaf(x[v][e], g[v][e] * w[v][e], dot);
-                    }
-                const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
-                const float m = row_lanes_sum(dot, a.lanes_log2) * r * inv;  // mean of u xh
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float xh = x[v][e] * r;
-                        dw[v][e] = fmaf(g[v][e], xh, dw[v][e]);
-                        x[v][e] = r * (g[v][e] * w[v][e] - xh * m);
-                    }
-                cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
-            }
-        }
-        if (!a.part) continue;
-        // the sums of the workgroup's rows: the slots' one after the other
-        for (int q = 0; q < slots; ++q) {
-            __syncthreads();
-            if (slot == q)
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int c = cols.c[v] + e;
-                        if (c < cols.end[v]) sums[c] = (q ? sums[c] : 0.f) + dw[v][e];
-                    }
-        }
+    typename Cols::Values w, dw = {};
+    load_weight<T, NEAR>(w, cols, a, side.weight);
+    for (int64_t tok0 = (int64_t)blockIdx.x * a.at_once; tok0 < a.tokens; tok0 += (int64_t)gridDim.x * a.at_once) {
+        const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
         __syncthreads();
-        for (int c = threadIdx.x; c < a.dim; c += 256) a.part[((size_t)blockIdx.x * 2 + s) * a.dim + c] = sums[c];
+        make_turns(a, tok0, count, cs);
+        __syncthreads();
+        for (int i = at.slot; i < count * side.heads; i += at.slots) {
+            const int k = i / side.heads, h = i - k * side.heads;
+            typename Cols::Values x, g;
+            cols.load(x, (const T *)(side.x + (tok0 + k) * side.x_token + h * side.x_head));
+            cols.load(g, (const T *)(side.dy + (tok0 + k) * side.dy_token + h * side.dy_head));
+            cols.template turn<true>(g, cs[k]);
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    sum = fmaf(x[v][e], x[v][e], sum);
+                    dot = fmaf(x[v][e], g[v][e] * w[v][e], dot);
+                }
+            const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
+            const float m = row_lanes_sum(dot, a.lanes_log2) * r * inv;  // mean of u xh
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float xh = x[v][e] * r;
+                    dw[v][e] = fmaf(g[v][e], xh, dw[v][e]);
+                    x[v][e] = r * (g[v][e] * w[v][e] - xh * m);
+                }
+            cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
+        }
+    }
+    if (!a.part) return;
+    // the sums of the workgroup's rows: over a wave's rows by exchange, then over the waves of a side
+    const int lanes = 1 << a.lanes_log2;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            for (int o = lanes; o < 64; o <<= 1) dw[v][e] += __shfl_xor(dw[v][e], o, 64);
+    if ((threadIdx.x & 63) < lanes)
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (cols.c[v] + e < cols.end[v]) sums[threadIdx.x >> 6][cols.c[v] + e] = dw[v][e];
+    __syncthreads();
+    float *part = a.part + (size_t)blockIdx.x * 2 * a.dim;
+    for (int c = threadIdx.x; c < 2 * a.dim; c += 256) {
+        const int s = c >= a.dim, col = c - s * a.dim;
+        float x = 0.f;
+        for (int w = s ? 4 - a.key_waves : 0; w < (s ? 4 : 4 - a.key_waves); ++w) x += sums[w][col];
+        part[c] = x;
     }
 }
 
-// Adds the workgroups' rows in a fixed order: 32 columns and one side a workgroup, 8 rows at a time.
+// Adds the workgroups' rows in a fixed order: 32 of the 2 dim columns a workgroup, every 32nd row a group of threads.
 template <class P>
-__global__ __launch_bounds__(256) void k_head_sums(const float *part, int parts, int dim, P *dq, P *dk) {
-    __shared__ float sums[8][33];
-    P *out = blockIdx.y ? dk : dq;
-    if (!out) return;
+__global__ __launch_bounds__(1024) void k_head_sums(const float *part, int parts, int dim, P *dq, P *dk) {
+    __shared__ float sums[32][33];
     const int g = threadIdx.x >> 5, l = threadIdx.x & 31, c = blockIdx.x * 32 + l;
     float s = 0.f;
-    if (c < dim)
-        for (int p = g; p < parts; p += 8) s += part[((size_t)p * 2 + blockIdx.y) * dim + c];
+    if (c < 2 * dim) {
+#pragma unroll 4
+        for (int p = g; p < parts; p += 32) s += part[(size_t)p * 2 * dim + c];
+    }
     sums[g][l] = s;
     __syncthreads();
-    if (g == 0 && c < dim) {
+    s = sums[l][g];  // group g adds column g's
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += sums[k][l];
-        out[c] = (P)s;
-    }
+    for (int o = 1; o < 32; o <<= 1) s += __shfl_xor(s, o, 32);
+    const int at = blockIdx.x * 32 + g;
+    P *out = at < dim ? dq : dk;
+    if (l == 0 && at < 2 * dim && out) out[at < dim ? at : at - dim] = (P)s;
 }
 
-// Lanes of a row: a power of two of at least half its vectors.
-inline int row_lanes_log2(size_t dim, int dtype) {
-    const size_t per = 2 * 16 / dtype_size(dtype);
-    return lanes_log2((dim + per - 1) / per);
+// Lanes of a row: a power of two of those that its pairs and its other columns take.
+inline int row_lanes_log2(size_t dim, size_t rotary, int dtype) {
+    const size_t vec = 16 / dtype_size(dtype);
+    const size_t lanes = (rotary / 2 + vec - 1) / vec + (dim - rotary + 2 * vec - 1) / (2 * vec);
+    static_assert(kMaxDim / 8 + 2 <= 64, "a row's lanes are of one wave");
+    return lanes_log2(lanes);
 }
-// Tokens of a turn: as many as the workgroup's rows at once, so that all are busy, but no more than leave enough workgroups.
-inline int tokens_at_once(size_t tokens, size_t heads, int lanes_log2) {
-    size_t n = (256u >> lanes_log2) / heads;
-    const size_t enough = tokens / 1024;
-    n = n < 4 ? 4 : n;
-    n = n < enough ? n : enough;
+// Tokens of a turn: 8, fewer where there are not enough for a turn on every CU.
+inline int tokens_at_once(size_t tokens) {
+    const size_t n = tokens / 512;
     return n < 1 ? 1 : n > kTok ? kTok : (int)n;
+}
+// Waves of 4 that have the keys: their share of the heads, but one at least for either side that has any.
+inline int key_waves(size_t heads, size_t kv_heads) {
+    if (!kv_heads || !heads) return kv_heads ? 4 : 0;
+    const size_t n = (4 * kv_heads + (heads + kv_heads) / 2) / (heads + kv_heads);
+    return n < 1 ? 1 : n > 3 ? 3 : (int)n;
 }
 inline size_t part_count(size_t tokens, int at_once) {
     const size_t n = (tokens + at_once - 1) / at_once;
@@ -295,7 +320,7 @@ int check_common(int dtype, int param_dtype, size_t tokens, size_t heads, size_t
     if (!dtype_known(dtype)) return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type " + std::to_string(dtype));
     if (param_dtype != dtype && param_dtype != VHIP_DTYPE_F32)
         return set_error(VHIP_ERR_INVALID_CONFIG, "parameters are of the rows' type or f32");
-    if (dim == 0 || dim > kMaxDim) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 512]");
+    if (dim == 0 || dim > kMaxDim) return set_error(VHIP_ERR_INVALID_CONFIG, "dim must be in [1, 256]");
     if (rotary > dim || rotary % 2) return set_error(VHIP_ERR_INVALID_CONFIG, "rotary must be even and at most dim");
     if (heads + kv_heads == 0 || heads > 65536 || kv_heads > 65536)
         return set_error(VHIP_ERR_INVALID_CONFIG, "heads must be in [1, 65536]");
@@ -331,11 +356,11 @@ int backward(const HeadArgs &a, bool near, void *dqw, void *dkw, hipStream_t s) 
             k_head_backward<T, false><<<parts, 256, 0, s>>>(a);
     }
     if (dqw || dkw) {
-        const dim3 grid((uint32_t)ceil_div(a.dim, 32), 2);
+        const uint32_t grid = (uint32_t)ceil_div(2 * a.dim, 32);
         if (a.f32_params)
-            k_head_sums<float><<<grid, 256, 0, s>>>(a.part, parts, a.dim, (float *)dqw, (float *)dkw);
+            k_head_sums<float><<<grid, 1024, 0, s>>>(a.part, parts, a.dim, (float *)dqw, (float *)dkw);
         else
-            k_head_sums<T><<<grid, 256, 0, s>>>(a.part, parts, a.dim, (T *)dqw, (T *)dkw);
+            k_head_sums<T><<<grid, 1024, 0, s>>>(a.part, parts, a.dim, (T *)dqw, (T *)dkw);
     }
     return launch_status("head norm launch");
 }
@@ -360,10 +385,10 @@ int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_head
     CallDevice dev;
     VH_CHECK(dev.enter(ordinal));
     if (tokens == 0) return VHIP_OK;
-    const int l = row_lanes_log2(dim, dtype);
+    const int l = row_lanes_log2(dim, rotary, dtype);
     const HeadArgs a{{to_side(dtype, q, nullptr, q_out, q_weight, heads), to_side(dtype, k, nullptr, k_out, k_weight, kv_heads)},
                      positions, frequencies, nullptr, (int64_t)tokens, (int)dim, (int)rotary / 2, l,
-                     tokens_at_once(tokens, heads + kv_heads, l), param_dtype == VHIP_DTYPE_F32, eps};
+                     tokens_at_once(tokens), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case VHIP_DTYPE_F32: return forward<float>(a, interleaved, s);
@@ -396,10 +421,10 @@ int vhip_qk_norm_rotary_backward(int ordinal, int dtype, int param_dtype, const 
                          "the workspace is smaller than vhip_qk_norm_rotary_backward_workspace() or not aligned");
     CallDevice dev;
     VH_CHECK(dev.enter(ordinal));
-    const int l = row_lanes_log2(dim, dtype);
+    const int l = row_lanes_log2(dim, rotary, dtype);
     const HeadArgs a{{to_side(dtype, q, dq, dq_out, q_weight, heads), to_side(dtype, k, dk, dk_out, k_weight, kv_heads)},
                      positions, frequencies, dq_weight || dk_weight ? (float *)workspace : nullptr, (int64_t)tokens, (int)dim,
-                     (int)rotary / 2, l, tokens_at_once(tokens, heads + kv_heads, l), param_dtype == VHIP_DTYPE_F32, eps};
+                     (int)rotary / 2, l, tokens_at_once(tokens), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case VHIP_DTYPE_F32: return backward<float>(a, interleaved, dq_weight, dk_weight, s);

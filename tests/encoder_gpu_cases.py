@@ -304,3 +304,353 @@ def test_clip(tr, sizes, dtypes, out, max_norm):
         within(o, want, (2 * E + UNIT[o.dtype]) * want.abs() + TINY[o.dtype])
         if float(c) == 1.0 and o.dtype == b.dtype:
             assert torch.equal(o, b)
+
+
+# ---- what else a call may be given -------------------------------------------------------------------
+
+def attention_both(tr, q, k, v, do, at, kat, causal, scale=None):
+    out, lse = tr.attention(q, k, v, at, kat, causal=causal, scale=scale)
+    return (out, lse) + tuple(tr.attention_backward(do, q, k, v, out, lse, at, kat, causal=causal, scale=scale))
+
+
+def check_attention(got, want, tol, names=("out", "lse", "dq", "dk", "dv")):
+    for name, x in zip(names, got):
+        within(x, want[name], tol[name])
+
+
+@pytest.mark.parametrize("layout", ["heads first", "padded", "odd addresses", "one buffer"])
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("bf16", 64), ("f16", 40), ("bf16", 33)])
+def test_attention_layouts(tr, layout, dtype, dim):
+    """The same values in other places, bit by bit."""
+    lq, heads, kv = [70, 3, 130], 6, 2
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, dtype)
+
+    def place(x):
+        n, h, d = x.shape
+        if layout == "heads first":
+            return x.transpose(0, 1).contiguous().transpose(0, 1)
+        if layout == "padded":
+            y = torch.full((n, h + 1, d + 24), math.nan, device="cuda", dtype=x.dtype)[:, :h, :d]
+        elif layout == "odd addresses":
+            y = torch.full((n * h * (d + 1) + 1,), math.nan, device="cuda", dtype=x.dtype)[1:].view(n, h, d + 1)[..., :d]
+        else:
+            y = torch.full((n, 3 * h, d), math.nan, device="cuda", dtype=x.dtype)[:, h:2 * h]
+        y.copy_(x)
+        return y
+
+    at = bounds(lq)
+    want = attention_both(tr, q, k, v, do, at, None, True)
+    got = attention_both(tr, place(q), place(k), place(v), place(do), at, None, True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_attention_scales(tr, dtype, scale):
+    lq, heads, kv, dim = [40, 100], 4, 2, 48
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, dtype)
+    want, tol = attention_reference(q, k, v, lq, lq, True, scale, do)
+    check_attention(attention_both(tr, q, k, v, do, bounds(lq), None, True, scale), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-3, 8.0])
+def test_attention_flat_and_peaked_rows(tr, dtype, size):
+    lq, heads, kv, dim = [300], 2, 1, 64
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, dtype, size=size)
+    scale = 1 / math.sqrt(dim)
+    want, tol = attention_reference(q, k, v, lq, lq, False, scale, do)
+    check_attention(attention_both(tr, q, k, v, do, bounds(lq), None, False), want, tol)
+
+
+@pytest.mark.parametrize("power", [-14, -20, 12])
+def test_attention_gradients_of_any_size_in_float16(tr, power):
+    """ds has powers of two of its own: gradients of small out gradients keep their bits."""
+    lq, heads, kv, dim = [90, 260], 2, 1, 64
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, "f16")
+    do = (do.float() * 2.0 ** power).half()
+    v = (v.float() * 2.0 ** -4).half()
+    scale = 1 / math.sqrt(dim)
+    want, tol = attention_reference(q, k, v, lq, lq, True, scale, do)
+    check_attention(attention_both(tr, q, k, v, do, bounds(lq), None, True), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_sequences_do_not_meet(tr, dtype, causal):
+    """What other sequences hold, and rows of none, changes nothing: not a bit."""
+    lq, heads, kv, dim = [50, 33, 77], 4, 2, 64
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, dtype, tail=20)
+    at = bounds(lq)
+    want = attention_both(tr, q, k, v, do, at, None, causal)
+    for bad in (math.nan, math.inf):
+        x = [y.clone() for y in (q, k, v, do)]
+        for y in x:
+            y[50:83] = bad
+            y[160:] = bad
+        got = attention_both(tr, *x, at, None, causal)
+        for a, b in zip(got, want):
+            assert torch.equal(a[:50], b[:50]) and torch.equal(a[83:160], b[83:160])
+            assert torch.equal(a[160:], torch.full_like(a[160:], -math.inf) if a.dim() == 2 else torch.zeros_like(a[160:]))
+
+
+def test_offsets_that_skip_rows_or_fall(tr):
+    """Rows before the first and behind the last sequence come out empty; offsets out of the arrays reach nothing."""
+    q, k, v, do = attention_case([100], [100], 2, 1, 32, "bf16")
+    at = torch.tensor([10, 40, 90], device="cuda")
+    out, lse, dq, dk, dv = attention_both(tr, q, k, v, do, at, None, True)
+    inner = attention_both(tr, *(x[10:90].clone() for x in (q, k, v, do)), at - 10, None, True)
+    for a, b in zip((out, lse, dq, dk, dv), inner):
+        assert torch.equal(a[10:90], b)
+        assert torch.equal(a[:10], torch.full_like(a[:10], -math.inf) if a.dim() == 2 else torch.zeros_like(a[:10]))
+    for wild in ([-5, 40, 1 << 40], [100, 0, 100], [50, 20, 10], [-(1 << 62), 7, 3]):
+        attention_both(tr, q, k, v, do, torch.tensor(wild, device="cuda"), None, True)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_parts_of_the_keys_and_rows(tr, dtype):
+    """Few rows against many keys, and many rows against few keys: sums over parts."""
+    for lq, lk, heads, kv, causal in (([3, 1], [9000, 40], 8, 2, True), ([5000], [30], 2, 1, False), ([2, 700], [6000, 700], 4, 4, True)):
+        print("parts", lq, lk, dtype, flush=True)
+        q, k, v, do = attention_case(lq, lk, heads, kv, 64, dtype, tail=2)
+        want, tol = attention_reference(q, k, v, lq, lk, causal, 0.125, do)
+        check_attention(attention_both(tr, q, k, v, do, bounds(lq), bounds(lk), causal), want, tol)
+
+
+def test_attention_gradient_against_differences(tr):
+    """A step along a direction changes sum(do out) by what the gradients say."""
+    lq, h = [30, 45], 1e-3
+    q, k, v, do = attention_case(lq, lq, 4, 2, 32, "f32")
+    at = bounds(lq)
+    out, lse, dq, dk, dv = attention_both(tr, q, k, v, do, at, None, True)
+    for x, g in ((q, dq), (k, dk), (v, dv)):
+        u = normal(50, *x.shape)
+        said = float((g.double() * u.double()).sum())
+        found = 0.0
+        for s in (1, -1):
+            moved = [y if y is not x else (x + s * h * u) for y in (q, k, v)]
+            want, _ = attention_reference(*moved, lq, lq, True, 1 / math.sqrt(32))
+            found += s * float((want["out"] * do.double()).sum()) / (2 * h)
+        # third derivatives: h^2 of the size of the sum's terms; 32-bit rounding of moved inputs over 2 h
+        size = float((g.double().abs() * u.double().abs()).sum()) + float((do.double().abs() * out.double().abs()).sum())
+        assert abs(said - found) <= (10 * h * h + 64 * E / h) * size
+
+
+def test_keys_past_32_bits(tr):
+    """A cache of more than 4 GiB; the sequence at its end."""
+    tokens, kv, dim, n = 4_500_000, 8, 64, 700
+    k = torch.zeros(tokens, kv, dim, device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    q, ks, vs, do = attention_case([n], [n], 16, kv, dim, "bf16")
+    k[-n:], v[-n:] = ks, vs
+    at, kat = bounds([n]), torch.tensor([tokens - n, tokens], device="cuda")
+    want = attention_both(tr, q, ks, vs, do, at, None, True)
+    got = attention_both(tr, q, k, v, do, at, kat, True)
+    ref, tol = attention_reference(q, ks, vs, [n], [n], True, 0.125, do)
+    # both are within tol of the same value (a larger cache is read in other parts), so within 2 tol of each other
+    within(got[0], want[0], 2 * tol["out"])
+    check_attention((got[0], got[1], got[2], got[3][-n:], got[4][-n:]), ref, tol)
+    assert not got[3][:-n].any() and not got[4][:-n].any()
+
+
+def test_everything_is_repeatable(tr):
+    lq = [513, 20, 77]
+    q, k, v, do = attention_case(lq, lq, 6, 2, 64, "bf16")
+    first = attention_both(tr, q, k, v, do, bounds(lq), None, True)
+    x, y, w, pos, freq = head_norm_case(3000, 4, 2, 64, 64, 0, "bf16", "f32")
+    heads = tr.qk_norm_rotary_backward(x.contiguous(), y.contiguous(), x, y, w[0], w[1], pos, freq)
+    arrays = clip_arrays([3_000_001, 77, (33, 65)], ["f32", "bf16"])
+    norm = tr.gradient_norm(arrays)
+    for _ in range(5):
+        for a, b in zip(first, attention_both(tr, q, k, v, do, bounds(lq), None, True)):
+            assert torch.equal(a, b)
+        for a, b in zip(heads, tr.qk_norm_rotary_backward(x.contiguous(), y.contiguous(), x, y, w[0], w[1], pos, freq)):
+            assert torch.equal(a, b)
+        assert torch.equal(norm, tr.gradient_norm(arrays))
+
+
+# ---- head norms and clipping at their edges ----------------------------------------------------------
+
+def test_head_norm_without_weights_and_far_positions(tr):
+    q, k, _, _, _ = head_norm_case(50, 3, 1, 64, 64, 0, "f32", "f32")
+    freq = torch.ones(32, device="cuda")
+    pos = torch.tensor([0, 1, -1, 10**6, -10**9, 2**40, 2**52], device="cuda").repeat(8)[:50]
+    got = tr.qk_norm_rotary(q, k, None, None, pos, freq)
+    angle = pos.double()[:, None] * freq.double()
+    for x, y in zip((q, k), got):
+        want, tol = head_norm_reference(x, None, angle, False, 1e-6)
+        # 2^52 radians: the reference's own reduction and this one's are exact to 2^52 2^-107
+        within(y, want, tol + UNIT[y.dtype] * want.abs())
+    dq, dk, dqw, dkw = tr.qk_norm_rotary_backward(got[0], got[1], q, k, None, None, pos, freq)
+    assert dqw is None and dkw is None
+    # the gradient of half the squared norm of rows whose norm is fixed: only eps moves it
+    assert float(dq.abs().max()) <= 1e-4 and float(dk.abs().max()) <= 1e-4
+
+
+def test_head_norm_rows_of_zeros_and_one_bad_row(tr):
+    q, k, w, pos, freq = head_norm_case(20, 2, 2, 48, 32, 0, "bf16", "f32")
+    q, k = q.clone(), k.clone()
+    want = tr.qk_norm_rotary(q, k, w[0], w[1], pos, freq)
+    q[3], q[5], k[7] = 0, math.nan, math.inf
+    got = tr.qk_norm_rotary(q, k, w[0], w[1], pos, freq)
+    assert not got[0][3].any() and torch.isnan(got[0][5]).all() and torch.isnan(got[1][7]).all()
+    keep = torch.ones(20, dtype=torch.bool, device="cuda")
+    keep[[3, 5]] = False
+    assert torch.equal(got[0][keep], want[0][keep])
+    keep[:], keep[7] = True, False
+    assert torch.equal(got[1][keep], want[1][keep])
+
+
+def test_head_norm_gradient_against_differences(tr):
+    q, k, w, pos, freq = head_norm_case(9, 3, 2, 40, 24, 0, "f32", "f32")
+    dq, dk = normal(8, *q.shape), normal(9, *k.shape)
+    got = tr.qk_norm_rotary_backward(dq, dk, q, k, w[0], w[1], pos, freq, eps=1e-3)
+    angle, h = pos.double()[:, None] * freq.double(), 1e-4
+    for x, wt, g, dx, dw in zip((q, k), w, (dq, dk), got[:2], got[2:]):
+        u, uw = normal(20, *x.shape).double(), normal(21, *wt.shape).double()
+        f = lambda s: float((head_norm_reference(x.double() + s * h * u, wt.double() + s * h * uw, angle, False, 1e-3)[0] * g.double()).sum())  # noqa: E731,B023
+        said = float((dx.double() * u).sum() + (dw.double() * uw).sum())
+        size = float((dx.double().abs() * u.abs()).sum() + (dw.double().abs() * uw.abs()).sum())
+        assert abs(said - (f(1) - f(-1)) / (2 * h)) <= (1e3 * h * h + 64 * E) * (size + float(g.abs().sum()))
+
+
+@pytest.mark.parametrize("dtype,value", [("f32", 3e38), ("f32", 1e-40), ("f32", 1e25), ("bf16", 1e38), ("bf16", 1e-38), ("f16", 65504.0), ("f16", 6e-8)])
+def test_clip_values_of_any_size(tr, dtype, value):
+    a = torch.full((1000,), value, device="cuda").to(TYPES[dtype])
+    norm, c = clip_reference([a], 1.0, 0.0)
+    got = tr.gradient_norm([a])
+    if float(norm) < 3.4e38:
+        within(got, norm, 2 * E * norm + 2.0 ** -149)
+    else:
+        assert math.isinf(float(got))
+    b = a.clone()
+    tr.clip_gradients([b], 1.0, eps=0.0)
+    want = a.double() * float(c)
+    # c itself is rounded to 32 bits, where it may have lost bits below 2^-126
+    within(b, want, (2 * E + UNIT[b.dtype] + 2.0 ** -149 / max(float(c), 1e-300)) * want.abs() + TINY[b.dtype] + (2.0 ** -126 if dtype == "f32" else 0))
+
+
+def test_clip_norms_that_are_not_finite(tr):
+    for bad in (math.inf, -math.inf, math.nan):
+        a, b = torch.ones(3000, device="cuda"), torch.ones(5, device="cuda", dtype=torch.bfloat16)
+        a[7] = bad
+        norm = tr.clip_gradients([a, b], 1.0)
+        if math.isnan(bad):
+            assert math.isnan(float(norm)) and torch.isnan(a).all() and torch.isnan(b).all()
+        else:
+            assert math.isinf(float(norm)) and torch.isnan(a[7]) and not b.any() and int((a == 0).sum()) == 2999
+
+
+def test_clip_dense_arrays_in_other_orders(tr):
+    a = normal(1, 40, 50).t()
+    o = torch.empty(40, 50, device="cuda").t()
+    want = a.double() * min(1.0, 1.0 / float(a.double().norm()))
+    tr.clip_gradients([a, a[:0]], 1.0, out=[o, a[:0]], eps=0.0)
+    within(o, want, 4 * E * want.abs())
+
+
+# ---- streams, graphs, refusals ----------------------------------------------------------------------
+
+def encoder_calls(tr, dtype="bf16"):
+    """All operators as a step has them one after the other, as a function without arguments."""
+    lq = [60, 133, 5]
+    at = bounds(lq)
+    q, k, v, do = attention_case(lq, lq, 4, 2, 64, dtype)
+    _, _, w, pos, freq = head_norm_case(sum(lq), 4, 2, 64, 64, 0, dtype, dtype)
+    few_q, few_k = bounds([1, 2]), bounds([5000, 100])
+    fq, fk, fv, fdo = attention_case([1, 2], [5000, 100], 4, 2, 64, dtype)
+
+    def run():
+        a, b = tr.qk_norm_rotary(q, k, w[0], w[1], pos, freq)
+        out, lse = tr.attention(a, b, v, at)
+        da, db, dv = tr.attention_backward(do, a, b, v, out, lse, at)
+        dq, dk, dqw, dkw = tr.qk_norm_rotary_backward(da, db, q, k, w[0], w[1], pos, freq)
+        clipped = [torch.empty_like(x) for x in (dq, dk, dv, dqw, dkw)]
+        norm = tr.clip_gradients([dq, dk, dv, dqw, dkw], 0.5, out=clipped)
+        few = attention_both(tr, fq, fk, fv, fdo, few_q, few_k, True)
+        return [out, lse, norm, *clipped, *few]
+
+    return run
+
+
+def test_calls_on_another_stream(tr):
+    run = encoder_calls(tr)
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run()
+    other = run()  # at the same time
+    torch.cuda.synchronize()
+    for a, b, c in zip(got, want, other):
+        assert torch.equal(a, b) and torch.equal(c, b)
+
+
+def test_calls_in_graphs(tr):
+    """Two captured graphs, replayed in turn and with eager work between."""
+    runs = [encoder_calls(tr, "bf16"), encoder_calls(tr, "f16")]
+    want = [run() for run in runs]
+    graphs, got = [], []
+    for run in runs:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(run())
+        graphs.append(g)
+    for _ in range(4):
+        for g, outs, w, run in zip(graphs, got, want, runs):
+            for x in outs:
+                x.zero_()
+            g.replay()
+            eager = run()
+            torch.cuda.synchronize()
+            for a, b, c in zip(outs, w, eager):
+                assert torch.equal(a, b) and torch.equal(c, b)
+
+
+def test_refusals(tr):
+    import vector_hip as vh
+
+    q, k, v, do = attention_case([9], [9], 4, 2, 32, "bf16")
+    at = bounds([9])
+    out, lse = tr.attention(q, k, v, at)
+    w, pos, freq = torch.ones(32, device="cuda", dtype=torch.bfloat16), torch.arange(9, device="cuda"), torch.ones(16, device="cuda")
+    norm = lambda *a, **o: tr.qk_norm_rotary(*a, **o)  # noqa: E731
+    big = torch.zeros(2, 1, 129, device="cuda")
+    wrong = [
+        lambda: tr.attention(q, k, v, at.int()), lambda: tr.attention(q, k, v, at.cpu()), lambda: tr.attention(q, k, v, at[:0]),
+        lambda: tr.attention(q[0], k, v, at), lambda: tr.attention(q, k.float(), v, at), lambda: tr.attention(q, k, v[:, :1], at),
+        lambda: tr.attention(q[:, :3], k, v, at), lambda: tr.attention(q, k[..., :16], v[..., :16], at), lambda: tr.attention(q, k[:5], v[:5], at),
+        lambda: tr.attention(q, k, v, at, at[:1]), lambda: tr.attention(q, k, v, at, scale=math.inf), lambda: tr.attention(q, k, v, at, scale=math.nan),
+        lambda: tr.attention(q.long(), k.long(), v.long(), at), lambda: tr.attention(big, big, big, bounds([2])),
+        lambda: tr.attention(q[..., ::2], k[..., ::2], v[..., ::2], at), lambda: tr.attention(q, k[:1].expand(9, 2, 32), v, at),
+        lambda: tr.attention(q.requires_grad_(), k, v, at), lambda: tr.attention(q.cpu(), k.cpu(), v.cpu(), at.cpu()),
+        lambda: tr.attention_backward(do[:5], q, k, v, out, lse, at), lambda: tr.attention_backward(do, q, k, v, out[:, :2], lse, at),
+        lambda: tr.attention_backward(do, q, k, v, out, lse.t(), at), lambda: tr.attention_backward(do, q, k, v, out, lse.double(), at),
+        lambda: norm(q, k, w, None, pos, freq), lambda: norm(q, k, w, w.float(), pos, freq), lambda: norm(q, k, w.half(), w.half(), pos, freq),
+        lambda: norm(q, k, w[:5], w[:5], pos, freq), lambda: norm(q, k, w, w, pos[:5], freq), lambda: norm(q, k, w, w, pos.int(), freq),
+        lambda: norm(q, k, w, w, pos, freq.double()), lambda: norm(q, k, w, w, pos, torch.ones(17, device="cuda")), lambda: norm(q, k[:4], w, w, pos, freq),
+        lambda: norm(q, k, w, w, pos, freq, eps=-1.0), lambda: norm(q, k.half(), w, w, pos, freq),
+        lambda: norm(torch.zeros(9, 2, 257, device="cuda"), torch.zeros(9, 2, 257, device="cuda"), None, None, pos, freq),
+        lambda: tr.qk_norm_rotary_backward(do[:4], k, q, k, w, w, pos, freq),
+        lambda: tr.clip_gradients([], 1.0), lambda: tr.clip_gradients([q, q], 1.0), lambda: tr.clip_gradients([q.detach(), q.detach()[3:]], 1.0),
+        lambda: tr.clip_gradients([do], -1.0), lambda: tr.clip_gradients([do], math.nan), lambda: tr.clip_gradients([do], 1.0, eps=-1.0),
+        lambda: tr.clip_gradients([do[:, ::2]], 1.0), lambda: tr.clip_gradients([do, at], 1.0), lambda: tr.clip_gradients([do], 1.0, out=[]),
+        lambda: tr.clip_gradients([do], 1.0, out=[do[:4]]), lambda: tr.clip_gradients([do, k], 1.0, out=[k, do.float()]),
+        lambda: tr.clip_gradients([do, k], 1.0, out=[k[:0].new_empty(do.shape), do.view(-1)[:k.numel()].view(k.shape)]),
+        lambda: tr.clip_gradients([do.cpu()], 1.0), lambda: tr.gradient_norm([do, do.cpu()]),
+    ]
+    for i, call in enumerate(wrong):
+        with pytest.raises(vh.InvalidConfig):
+            call()
+            pytest.fail(f"call {i} was not refused")
+        q = q.detach()
+    with torch.no_grad():
+        tr.attention(q.requires_grad_(), k, v, at)

@@ -291,6 +291,19 @@ __device__ __forceinline__ void mma_cols(const char *tile, int r0, const typenam
 #pragma unroll
         for (int k = 0; k < kOps<T>; ++k) sum[d] = mma(cols_frag<T, RB>(tile, r0, d, k, lane), b[k], sum[d]);
 }
+// The same of two operands, by the same reads.
+template <class T, int RB, int DT>
+__device__ __forceinline__ void mma_cols2(const char *tile, int r0, const typename Frag<T>::type (&b)[kOps<T>], floatx16_t (&sum)[DT],
+                                          const typename Frag<T>::type (&b2)[kOps<T>], floatx16_t (&sum2)[DT], int lane) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int k = 0; k < kOps<T>; ++k) {
+            const auto f = cols_frag<T, RB>(tile, r0, d, k, lane);
+            sum[d] = mma(f, b[k], sum[d]);
+            sum2[d] = mma(f, b2[k], sum2[d]);
+        }
+}
 // A B over KS steps, A the tile's rows r0 .. r0 + 31.
 template <class T, int RB, int KS>
 __device__ __forceinline__ floatx16_t mma_rows(const char *tile, int r0, const typename Frag<T>::type (&b)[KS], int lane) {

@@ -11,6 +11,11 @@
 //    S^T and dP^T leave a lane with its own row's scores, so lse and delta are its own scalars.
 //  * by keys: 128 keys a workgroup, 32 a wave, k and v in registers; tiles of packed rows of q and do, whose lse and
 //    delta come from LDS.  S and dP leave a lane with its own key's column.
+// delta comes from out, whose rounding and whose weights' rounding would go into every ds of the row: an error of 2.2e-3 of dq and
+// dk in bfloat16, more than rounding ds (1.8e-3) or the results (1.7e-3). But sum_j ds_rj is 0, so what the kernel by rows finds
+// for it, e_r, is delta's error times one: it hands delta + e to the kernel by keys, and takes e_r sum_j p_rj k_j off dq, an
+// eighth product, by operands that are in registers already (not in 32 bits).
+//
 // p and ds are rounded to the operands' type for the last products, which is half a unit of each; in float16 they are held
 // in powers of two of their own (p times 2^14, ds see Units).
 #include "attention.h"
@@ -28,8 +33,9 @@ struct BwdArgs {
     int heads, kv_heads, dim;
     bool causal;
     float scale;
-    int splits;   // parts of what is summed over, each a workgroup; more than one leave `part`, which k_attn_sum adds up
-    float *part;  // dq: [split][token][head][DP]; dk, dv: [split][2][token][head][DP]
+    int splits;   // parts of what is summed over, each a workgroup; more than one leave `part`, which other kernels add up
+    float *part;  // [split][2][token][head][DP]: dq and sum p k, or dk and dv
+    float *off;   // [split][token][head]: sum ds
 };
 
 constexpr int kBM = 128, kBK = 128;  // rows and keys of a workgroup
@@ -117,43 +123,72 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
             for (int e = 0; e < VEC; ++e) delta = fmaf((float)go[ks][e], (float)x.v[e], delta);
         }
         delta = half_sum(delta);
-        if (split == 0 && half == 0 && r < n) a.delta[at_row] = delta;
     }
     const float lse = a.lse[at_row], c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
     const float base = lse == -INFINITY ? 0.f : -lse * kLog2e;
 
-    floatx16_t dq[DT] = {};
+    constexpr bool EXACT = sizeof(T) == 2;  // see above
+    floatx16_t dq[DT] = {}, pk[EXACT ? DT : 1] = {};
+    float off = 0.f;
     Units<T> units;
     for (int t = t0; t < t1; ++t) {
         tiles_ready();
         const int buf = (t - t0) & 1;
         if (t + 1 < t1) load(t + 1, buf ^ 1);
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < NS; ++j) {
-            const int key0 = t * BN + 32 * j;
+            const int key0 = t * BN + 32 * j, ln = anew(lane);
             if (key0 >= any) break;
-            floatx16_t s = mma_rows<T, RB>(lds[buf][0], 32 * j, q, lane);
-            floatx16_t dp = mma_rows<T, RB>(lds[buf][1], 32 * j, go, lane);
+            floatx16_t s = mma_rows<T, RB>(lds[buf][0], 32 * j, q, ln);
+            floatx16_t dp = mma_rows<T, RB>(lds[buf][1], 32 * j, go, ln);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, base)) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, base));
+                dp[i] = s[i] * (dp[i] - delta);
+            }
             if (key0 + 32 > all) {
                 const int left = sees - key0 - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (row_of(i) >= left) s[i] = 0.f;
+                    if (row_of(i) >= left) s[i] = dp[i] = 0.f;
             }
-            units.to_units(s, dq);
-            frag ds[kOps<T>];
-            to_operand<T>(s, ds);
-            mma_cols<T, RB>(lds[buf][0], 32 * j, ds, dq, lane);
+            frag ds[kOps<T>], p[kOps<T>];
+            if constexpr (EXACT) {
+                float sum[2] = {};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[i % 2] += dp[i];
+                off += sum[0] + sum[1];
+                to_operand<T>(s, p);
+            }
+            units.to_units(dp, dq);
+            to_operand<T>(dp, ds);
+            __builtin_amdgcn_sched_barrier(0);  // operands read ahead of these would not fit the registers
+            if constexpr (EXACT)
+                mma_cols2<T, RB>(lds[buf][0], 32 * j, ds, dq, p, pk, ln);
+            else
+                mma_cols<T, RB>(lds[buf][0], 32 * j, ds, dq, ln);
         }
     }
     if (r >= n) return;
-    auto value = [&](float x) { return units.back(x) * a.scale; };
-    if (a.splits > 1)
-        store_cols<float, DT>(a.part + ((int64_t)split * a.rows.tokens * a.heads + at_row) * DP, dq, DP, lane, value);
-    else
-        store_cols<T, DT>((T *)(a.dq.data + row * (int64_t)a.dq.token + (int64_t)head * a.dq.head), dq, a.dim, lane, value);
+    off = half_sum(off);
+    if (split == 0 && half == 0) a.delta[at_row] = a.splits > 1 ? delta : delta + off;
+    if (a.splits > 1) {  // k_attn_sum_rows does the rest
+        const int64_t all = a.rows.tokens * a.heads;
+        if (EXACT && half == 0) a.off[split * all + at_row] = off;
+        store_cols<float, DT>(a.part + (2 * split * all + at_row) * DP, dq, DP, lane, [&](float x) { return units.back(x); });
+        if constexpr (EXACT)
+            store_cols<float, DT>(a.part + ((2 * split + 1) * all + at_row) * DP, pk, DP, lane, [](float x) { return x; });
+        return;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            dq[d][i] = units.back(dq[d][i]);
+            if constexpr (EXACT) dq[d][i] = fmaf(-off, pk[d][i], dq[d][i]);
+        }
+    store_cols<T, DT>((T *)(a.dq.data + row * (int64_t)a.dq.token + (int64_t)head * a.dq.head), dq, a.dim, lane,
+                      [&](float x) { return x * a.scale; });
 }
 
 template <class T, int DP, bool DMA>
@@ -296,34 +331,61 @@ __global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves
     }
 }
 
-// Adds up parts: of dq (KEYS false), or of dk and dv (blockIdx.y), in the order of the parts.
-template <class T, int DP, bool KEYS>
-__global__ __launch_bounds__(256) void k_attn_sum(BwdArgs a) {
+// Adds up the parts of dq, in their order, and what they found for delta.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void k_attn_sum_rows(BwdArgs a) {
     constexpr int L = DP / 4, R = kRowsOf256<DP>;
-    const int heads = KEYS ? a.kv_heads : a.heads;
-    const int64_t all = (KEYS ? a.keys.tokens : a.rows.tokens) * heads;
+    constexpr bool EXACT = sizeof(T) == 2;
+    const int64_t all = a.rows.tokens * a.heads;
     const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
     const int e = threadIdx.x % L * 4;
     if (threadIdx.x >= R * L || i >= all || e >= a.dim) return;
-    const int which = KEYS ? blockIdx.y : 0;
+    float sum[4] = {}, pk[4] = {}, off = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const Pack<float, 4> p = load_any<4>(a.part + (2 * s * all + i) * DP + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += p.v[k];
+        if constexpr (EXACT) {
+            const Pack<float, 4> w = load_any<4>(a.part + ((2 * s + 1) * all + i) * DP + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pk[k] += w.v[k];
+            off += a.off[s * all + i];
+        }
+    }
+    if (EXACT && e == 0) a.delta[i] += off;
+    Pack<T, 4> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v.v[k] = (T)(fmaf(-off, pk[k], sum[k]) * a.scale);
+    store_row<4>((T *)(a.dq.data + i / a.heads * (int64_t)a.dq.token + i % a.heads * (int64_t)a.dq.head), e, a.dim, v);
+}
+
+// Adds up the parts of dk or dv (blockIdx.y).
+template <class T, int DP>
+__global__ __launch_bounds__(256) void k_attn_sum_keys(BwdArgs a) {
+    constexpr int L = DP / 4, R = kRowsOf256<DP>;
+    const int64_t all = a.keys.tokens * a.kv_heads;
+    const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    const int e = threadIdx.x % L * 4;
+    if (threadIdx.x >= R * L || i >= all || e >= a.dim) return;
     float sum[4] = {};
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-        const Pack<float, 4> p = load_any<4>(a.part + ((KEYS ? 2 * s + which : s) * all + i) * DP + e);
+        const Pack<float, 4> p = load_any<4>(a.part + ((2 * s + blockIdx.y) * all + i) * DP + e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] += p.v[k];
     }
     Pack<T, 4> v;
 #pragma unroll
     for (int k = 0; k < 4; ++k) v.v[k] = (T)sum[k];
-    const Heads &o = !KEYS ? a.dq : which ? a.dv : a.dk;
-    store_row<4>((T *)(o.data + i / heads * (int64_t)o.token + i % heads * (int64_t)o.head), e, a.dim, v);
+    const Heads &o = blockIdx.y ? a.dv : a.dk;
+    store_row<4>((T *)(o.data + i / a.kv_heads * (int64_t)o.token + i % a.kv_heads * (int64_t)o.head), e, a.dim, v);
 }
 
 // What a call works in: delta, then the parts of dq and afterwards, in the same place, those of dk and dv.
 struct Work {
     int qsplits, ksplits;
-    float *delta, *part;
+    float *delta, *off, *part;
     size_t bytes;
 };
 Work work_of(int dtype, const Shape &s, void *base) {
@@ -336,10 +398,11 @@ Work work_of(int dtype, const Shape &s, void *base) {
     const int fill = split_count(wgs, along, s.sequences, 512, 256), even = split_count(wgs, along, s.sequences, 2048, 2048);
     w.ksplits = fill > even ? fill : even;
     const size_t dp = padded(s.dim);
-    const size_t q = w.qsplits > 1 ? w.qsplits * s.tokens * s.heads * dp : 0;
+    const size_t q = w.qsplits > 1 ? 2 * w.qsplits * s.tokens * s.heads * dp : 0;
     const size_t k = w.ksplits > 1 ? 2 * w.ksplits * s.key_tokens * s.kv_heads * dp : 0;
     Carver c{(char *)base};
     w.delta = c.take<float>(s.tokens * s.heads);
+    w.off = c.take<float>(w.qsplits > 1 ? w.qsplits * s.tokens * s.heads : 0);
     w.part = c.take<float>(q > k ? q : k);
     w.bytes = c.used;
     return w;
@@ -360,7 +423,7 @@ int launch(BwdArgs a, const Run &r) {
             k_attn_dq<T, DP, true><<<r.qgrid, 256, 0, r.s>>>(a);
         else
             k_attn_dq<T, DP, false><<<r.qgrid, 256, 0, r.s>>>(a);
-        if (a.splits > 1) k_attn_sum<T, DP, false><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, r.s>>>(a);
+        if (a.splits > 1) k_attn_sum_rows<T, DP><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, r.s>>>(a);
     }
     if (r.kgrid) {
         a.splits = r.w.ksplits;
@@ -369,7 +432,7 @@ int launch(BwdArgs a, const Run &r) {
         else
             k_attn_dkv<T, DP, false><<<r.kgrid, 64 * ByKeys<T, DP>::waves, 0, r.s>>>(a);
         if (a.splits > 1)
-            k_attn_sum<T, DP, true><<<dim3((uint32_t)ceil_div(a.keys.tokens * a.kv_heads, kRowsOf256<DP>), 2), 256, 0, r.s>>>(a);
+            k_attn_sum_keys<T, DP><<<dim3((uint32_t)ceil_div(a.keys.tokens * a.kv_heads, kRowsOf256<DP>), 2), 256, 0, r.s>>>(a);
     }
     return launch_status("attention launch");
 }
@@ -433,7 +496,7 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
                     to_heads(dq, dtype), to_heads(dk, dtype), to_heads(dv, dtype), lse, r.w.delta,
                     {offsets, (int64_t)tokens, (int)sequences},
                     {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
-                    to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, 1, r.w.part};
+                    to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, 1, r.w.part, r.w.off};
     switch (dtype) {
         case VHIP_DTYPE_F32: return launch<float>(a, r);
         case VHIP_DTYPE_F16: return launch<half_t>(a, r);

@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import os
 import sys
+from array import array
 
 from . import DriverError, InvalidConfig, _check, _lib, _sig, _sz
 
@@ -62,18 +63,13 @@ _sig("vhip_attention_backward", _int, _int, _int, _h, _h, _h, _h, _h, _p, _sz, _
      _h, _p, _sz, _p)
 
 
-class _Array(ctypes.Structure):
-    _fields_ = [("data", _p), ("out", _p), ("count", _sz), ("dtype", _int), ("out_dtype", _int)]
-
-
-_a = ctypes.POINTER(_Array)
 _sig("vhip_qk_norm_rotary", _int, _int, _int, _int, _h, _h, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _sz, _int, _f, _h, _h, _p)
 _sig("vhip_qk_norm_rotary_backward_workspace", _sz, _sz, _sz)
 _sig("vhip_qk_norm_rotary_backward", _int, _int, _int, _int, _h, _h, _h, _h, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _sz, _int,
      _f, _h, _h, _p, _p, _p, _sz, _p)
 _sig("vhip_clip_gradients_workspace", _sz, _sz)
-_sig("vhip_gradient_norm", _int, _int, _a, _sz, _p, _p, _sz, _p)
-_sig("vhip_clip_gradients", _int, _int, _a, _sz, _f, _f, _p, _p, _sz, _p)
+_sig("vhip_gradient_norm", _int, _int, _p, _sz, _p, _p, _sz, _p)
+_sig("vhip_clip_gradients", _int, _int, _p, _sz, _f, _f, _p, _p, _sz, _p)
 
 
 class _Types(dict):
@@ -451,34 +447,32 @@ def _dense(a) -> bool:
 
 
 def _arrays(gradients, out):
-    gradients = list(gradients)
     if not gradients:
         raise InvalidConfig("there is no array")
-    _on_gpu("a gradient", gradients[0])
-    device = gradients[0].get_device()
-    table = (_Array * len(gradients))()
-    for i, g in enumerate(gradients):
-        _on_gpu("a gradient", g)
-        if g.get_device() != device:
-            raise InvalidConfig("the gradients are on more than one device")
-        if not _dense(g):
-            raise InvalidConfig("the values of a gradient must fill a block of memory")
-        code = _code[g.dtype]
-        at = g.data_ptr()
-        table[i] = (at, at, g.numel(), code, code)
-    if out is not None:
+    first = gradients[0]
+    _on_gpu("a gradient", first)
+    device, lib = first.get_device(), _library[type(first.dtype)]
+    table = array("Q")  # of vhip_array: data, out, count, and the two types in one
+    if out is None:
+        for g in gradients:
+            if not (getattr(g, "is_cuda", False) and g.get_device() == device):
+                raise InvalidConfig("the gradients are not all on one GPU")
+            if not (g.is_contiguous() or _dense(g)):
+                raise InvalidConfig("the values of a gradient must fill a block of memory")
+            at, code = g.data_ptr(), _code[g.dtype]
+            table.extend((at, at, g.numel(), code | code << 32))
+    else:
         out = list(out)
         if len(out) != len(gradients):
             raise InvalidConfig("out must hold an array for each gradient")
-        for row, g, o in zip(table, gradients, out):
-            _on_gpu("an output", o)
-            if o.shape != g.shape or o.get_device() != device:
-                raise InvalidConfig("an output must have the shape and the device of its gradient")
-            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise InvalidConfig("an output must have the strides of its gradient")
-            row.out, row.out_dtype = o.data_ptr(), _code[o.dtype]
-    first = gradients[0]
-    lib = _library[type(first.dtype)]
+        for g, o in zip(gradients, out):
+            if not (getattr(g, "is_cuda", False) and getattr(o, "is_cuda", False) and g.get_device() == o.get_device() == device):
+                raise InvalidConfig("the gradients and the outputs are not all on one GPU")
+            if o.shape != g.shape:
+                raise InvalidConfig("an output must have the shape of its gradient")
+            if not (g.is_contiguous() and o.is_contiguous()) and not (_dense(g) and g.stride() == o.stride()):
+                raise InvalidConfig("a gradient and its output must fill blocks of memory in the same order")
+            table.extend((g.data_ptr(), o.data_ptr(), g.numel(), _code[g.dtype] | _code[o.dtype] << 32))
     need = _lib.vhip_clip_gradients_workspace(len(gradients))
     return table, len(gradients), first.new_empty((), dtype=lib.f32), first.new_empty(need, dtype=lib.u8), need, device, lib
 
@@ -489,7 +483,7 @@ def gradient_norm(gradients):
     gradients = list(gradients)
     table, n, norm, ws, need, device, lib = _arrays(gradients, None)
     _no_graph(lib, *gradients)
-    _check(_lib.vhip_gradient_norm(device, table, n, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
+    _check(_lib.vhip_gradient_norm(device, table.buffer_info()[0], n, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
     return norm
 
 
@@ -500,5 +494,5 @@ def clip_gradients(gradients, max_norm: float, out=None, eps: float = 1e-6):
     gradients = list(gradients)
     table, n, norm, ws, need, device, lib = _arrays(gradients, out)
     _no_graph(lib, *gradients)
-    _check(_lib.vhip_clip_gradients(device, table, n, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
+    _check(_lib.vhip_clip_gradients(device, table.buffer_info()[0], n, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
     return norm

@@ -943,6 +943,68 @@ inline void orthogonalize(const Place &at, DType type, size_t count, const Rows 
                                      at.stream));
 }
 
+/* Packed sequences: their number, and device memory of sequences + 1 offsets (key_offsets null: the queries' own). */
+struct Sequences {
+    size_t count = 0;
+    const int64_t *offsets = nullptr, *key_offsets = nullptr;
+};
+/* Queries [tokens, heads, dim] and keys and values [key_tokens, kv_heads, dim] of one type. */
+struct Attended {
+    vhip_heads q, k, v;
+    size_t tokens = 0, key_tokens = 0, heads = 0, kv_heads = 0, dim = 0;
+};
+
+inline size_t attention_workspace(DType type, const Attended &x, const Sequences &s) {
+    return vhip_attention_workspace((int)type, x.tokens, x.key_tokens, x.heads, x.kv_heads, x.dim, s.count);
+}
+inline void attention(const Place &at, DType type, const Attended &x, const Sequences &s, bool causal, float scale, const vhip_heads &out,
+                      float *lse) {
+    detail::check(vhip_attention(at.ordinal, (int)type, &x.q, &x.k, &x.v, x.tokens, x.key_tokens, x.heads, x.kv_heads, x.dim, s.offsets,
+                                 s.key_offsets, s.count, causal, scale, &out, lse, at.workspace, at.workspace_bytes, at.stream));
+}
+inline size_t attention_backward_workspace(DType type, const Attended &x, const Sequences &s) {
+    return vhip_attention_backward_workspace((int)type, x.tokens, x.key_tokens, x.heads, x.kv_heads, x.dim, s.count);
+}
+inline void attention_backward(const Place &at, DType type, const vhip_heads &dout, const Attended &x, const vhip_heads &out,
+                               const float *lse, const Sequences &s, bool causal, float scale, const vhip_heads &dq, const vhip_heads &dk,
+                               const vhip_heads &dv) {
+    detail::check(vhip_attention_backward(at.ordinal, (int)type, &dout, &x.q, &x.k, &x.v, &out, lse, x.tokens, x.key_tokens, x.heads,
+                                          x.kv_heads, x.dim, s.offsets, s.key_offsets, s.count, causal, scale, &dq, &dk, &dv,
+                                          at.workspace, at.workspace_bytes, at.stream));
+}
+
+/* Queries and keys of the same tokens, their weights (null: 1), and how rows are turned. */
+struct HeadNorm {
+    vhip_heads q, k;
+    size_t tokens = 0, heads = 0, kv_heads = 0, dim = 0;
+    const void *q_weight = nullptr, *k_weight = nullptr;
+    const int64_t *positions = nullptr;
+    const float *frequencies = nullptr;
+    size_t rotary = 0;
+    bool interleaved = false;
+    float eps = 1e-6f;
+};
+inline void qk_norm_rotary(const Place &at, DType type, DType params, const HeadNorm &x, const vhip_heads &q_out, const vhip_heads &k_out) {
+    detail::check(vhip_qk_norm_rotary(at.ordinal, (int)type, (int)params, &x.q, &x.k, x.tokens, x.heads, x.kv_heads, x.dim, x.q_weight,
+                                      x.k_weight, x.positions, x.frequencies, x.rotary, x.interleaved, x.eps, &q_out, &k_out, at.stream));
+}
+inline size_t qk_norm_rotary_backward_workspace(const HeadNorm &x) { return vhip_qk_norm_rotary_backward_workspace(x.tokens, x.dim); }
+inline void qk_norm_rotary_backward(const Place &at, DType type, DType params, const vhip_heads &dq, const vhip_heads &dk, const HeadNorm &x,
+                                    const vhip_heads &dq_out, const vhip_heads &dk_out, void *dq_weight, void *dk_weight) {
+    detail::check(vhip_qk_norm_rotary_backward(at.ordinal, (int)type, (int)params, &dq, &dk, &x.q, &x.k, x.tokens, x.heads, x.kv_heads,
+                                               x.dim, x.q_weight, x.k_weight, x.positions, x.frequencies, x.rotary, x.interleaved, x.eps,
+                                               &dq_out, &dk_out, dq_weight, dk_weight, at.workspace, at.workspace_bytes, at.stream));
+}
+
+inline size_t clip_gradients_workspace(size_t arrays) { return vhip_clip_gradients_workspace(arrays); }
+inline void gradient_norm(const Place &at, const std::vector<vhip_array> &arrays, float *norm) {
+    detail::check(vhip_gradient_norm(at.ordinal, arrays.data(), arrays.size(), norm, at.workspace, at.workspace_bytes, at.stream));
+}
+inline void clip_gradients(const Place &at, const std::vector<vhip_array> &arrays, float max_norm, float eps, float *norm) {
+    detail::check(vhip_clip_gradients(at.ordinal, arrays.data(), arrays.size(), max_norm, eps, norm, at.workspace, at.workspace_bytes,
+                                      at.stream));
+}
+
 }  // namespace training
 
 }  // namespace vector_hip

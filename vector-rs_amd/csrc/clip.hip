@@ -184,7 +184,7 @@ int check_ranges(const vhip_array *arrays, size_t count) {
     // the furthest end so far, of outputs and of inputs, and whose it is
     const Range *out = nullptr, *in = nullptr, *in2 = nullptr;  // in2: the furthest of another array than in
     for (const Range &x : r) {
-        auto meets = [&](const Range *y) { return y && y->end > x.begin && !(y->of == x.of && y->out != x.out); };
+        auto meets = [&](const Range *y) { return y && y->end > x.begin && !(y->of == x.of && y->begin == x.begin); };
         if (meets(out) || (x.out && (meets(in) || meets(in2))))
             return set_error(VHIP_ERR_INVALID_CONFIG, "an output overlaps another array");
         const Range *&far = x.out ? out : in;

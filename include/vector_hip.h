@@ -466,8 +466,8 @@ typedef struct vhip_heads {
  * key head h / (heads / kv_heads).  With `causal` the last query of a sequence sees all its keys and each query before it
  * one fewer, so queries may be the last tokens of a longer text.
  *   s_rj = scale <q_r, k_j>,  lse_r = log sum_j exp s_rj,  out_r = sum_j exp(s_rj - lse_r) v_j
- * A row that sees no key has out 0 and lse -inf, and so has one of no sequence.  lse ([tokens, heads], may be
- * NULL).  dim <= 128, tokens * heads <= 2^30. */
+ * A row that sees no key has out 0 and lse -inf, and so has one of no sequence; keys and values that a row does not see
+ * have no part in it, whatever they hold.  lse ([tokens, heads], may be NULL).  dim <= 128, tokens * heads <= 2^30. */
 size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                 size_t sequences);
 int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads *k, const vhip_heads *v, size_t tokens,
@@ -475,7 +475,8 @@ int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads
                    const int64_t *key_offsets, size_t sequences, int causal, float scale, const vhip_heads *out, float *lse,
                    void *workspace, size_t workspace_bytes, void *stream);
 /* The gradients of sum <dout, out> for q, k and v from the forward call's out and lse; the heads of a group add up in
- * the gradients of their key head.  Rows of no sequence have gradient 0. */
+ * the gradients of their key head.  Rows of no sequence have gradient 0.  Infinities and NaN stay within their
+ * sequence, but there may reach gradients of rows and keys that do not see one another. */
 size_t vhip_attention_backward_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                          size_t sequences);
 int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, const vhip_heads *q, const vhip_heads *k,

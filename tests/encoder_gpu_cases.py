@@ -654,3 +654,42 @@ def test_refusals(tr):
         q = q.detach()
     with torch.no_grad():
         tr.attention(q.requires_grad_(), k, v, at)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (6, 2, 128), (3, 1, 40)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_not_seen_counts_for_nothing(tr, dtype, heads, kv, dim, bad):
+    """Causal: keys and values behind a row may hold anything; the row keeps its bits."""
+    print("not seen", dtype, heads, kv, dim, bad, flush=True)
+    lq, cut = [150, 300], 83
+    q, k, v, _ = attention_case(lq, lq, heads, kv, dim, dtype)
+    out, lse = tr.attention(q, k, v, bounds(lq))
+    for which in ("kv", "k", "v"):
+        x, y = k.clone(), v.clone()
+        if "k" in which:
+            x[cut:150] = bad
+        if "v" in which:
+            y[cut:150] = bad
+        got, gl = tr.attention(q, x, y, bounds(lq))
+        keep = torch.ones(450, dtype=torch.bool, device="cuda")
+        keep[cut:150] = False
+        assert torch.equal(got[keep], out[keep]) and torch.equal(gl[keep], lse[keep])
+        assert which == "k" or not torch.isfinite(got[cut:150]).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_infinities_that_are_seen(tr, dtype):
+    """An infinite value comes out in the rows that see it, in its column; both signs together are NaN."""
+    n = 100
+    q, k, v, do = attention_case([n], [n], 2, 2, 64, dtype)
+    v[40, 0, 5], v[60, 1, 9], v[70, 1, 9] = math.inf, -math.inf, math.inf
+    for causal in (True, False):
+        out, _ = tr.attention(q, k, v, bounds([n]), causal=causal)
+        want = torch.zeros(n, 2, 64, device="cuda")
+        want[(40 if causal else 0):, 0, 5] = math.inf
+        want[(60 if causal else 0):, 1, 9] = -math.inf
+        want[(70 if causal else 0):, 1, 9] = math.nan
+        bad = ~torch.isfinite(want)
+        assert torch.equal(~torch.isfinite(out), bad)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[torch.isinf(want)].float(), want[torch.isinf(want)])

@@ -304,6 +304,56 @@ __device__ __forceinline__ void mma_cols2(const char *tile, int r0, const typena
             sum2[d] = mma(f, b2[k], sum2[d]);
         }
 }
+// What is not seen has weight 0, which an infinity or NaN still turns into NaN. The forward pass multiplies without a thought
+// for that; only where its sums are not finite in the end, it does its work once more with this form of mma_cols for tiles
+// that are not seen as a whole (seen(i): what register i of B belongs to): zeros in place of A's values that are not finite,
+// and then infinities and NaN where one that is seen has them. What is finite keeps its bits.
+template <class T, int RB, int DT, class Seen>
+__device__ __forceinline__ void mma_cols_masked(const char *tile, int r0, const typename Frag<T>::type (&b)[kOps<T>], floatx16_t (&sum)[DT],
+                                                int lane, const Seen &seen) {
+    typedef typename Frag<T>::type frag;
+    constexpr int E = 16 / kOps<T>;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int k = 0; k < kOps<T>; ++k) {
+            frag f = cols_frag<T, RB>(tile, r0, d, k, lane);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (!(fabsf((float)f[e]) < INFINITY)) f[e] = (T)0.f;
+            sum[d] = mma(f, b[k], sum[d]);
+        }
+#pragma unroll 1
+        for (int c = 0; c < 3; ++c) {
+            floatx16_t count = {};
+#pragma unroll
+            for (int k = 0; k < kOps<T>; ++k) {
+                frag f = cols_frag<T, RB>(tile, r0, d, k, lane), m;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = (float)f[e];
+                    f[e] = (T)((c == 0 ? x == INFINITY : c == 1 ? x == -INFINITY : x != x) ? 1.f : 0.f);
+                    m[e] = (T)(seen(k * E + e) ? 1.f : 0.f);
+                }
+                count = mma(f, m, count);
+            }
+            const float value = c == 0 ? INFINITY : c == 1 ? -INFINITY : NAN;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (count[i] > 0.f) sum[d][i] += value;
+        }
+    }
+}
+// NaN where a sum is not finite, 0 otherwise.
+template <int DT>
+__device__ __forceinline__ float not_finite(const floatx16_t (&sum)[DT]) {
+    float bad = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad = fmaf(sum[d][i], 0.f, bad);
+    return bad;
+}
 // A B over KS steps, A the tile's rows r0 .. r0 + 31.
 template <class T, int RB, int KS>
 __device__ __forceinline__ floatx16_t mma_rows(const char *tile, int r0, const typename Frag<T>::type (&b)[KS], int lane) {

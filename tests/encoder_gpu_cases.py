@@ -693,3 +693,49 @@ def test_infinities_that_are_seen(tr, dtype):
         bad = ~torch.isfinite(want)
         assert torch.equal(~torch.isfinite(out), bad)
         assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[torch.isinf(want)].float(), want[torch.isinf(want)])
+
+
+# ---- the operators together --------------------------------------------------------------------------
+
+def test_an_encoder_with_its_gradients(tr):
+    """A step of examples/train_text_encoder.py against automatic differentiation of the same encoder in 64 bits."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_text_encoder.py")
+    spec = importlib.util.spec_from_file_location("train_text_encoder", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    encoder = ex.TextEncoder(300, 20, seed=3)
+    text, topic = ex.texts(40, 20, 300, gen(9))
+    loss, found = encoder.gradients(text, topic)
+
+    tokens, offsets, positions = text
+    w = {name: x.double().requires_grad_() for name, x in encoder.weights.items()}
+    h, g, d = encoder.heads, encoder.kv_heads, encoder.size
+    x = w["words"][tokens]
+    qkv = (x @ w["qkv"]).view(len(tokens), h + 2 * g, d)
+    angle = positions.double()[:, None] * encoder.frequencies.double()
+    z = []
+    rows = [(int(b), int(e)) for b, e in zip(offsets, offsets[1:])]
+    for b, e in rows:
+        sides = []
+        for part, weight in ((qkv[b:e, :h], w["q"]), (qkv[b:e, h:h + g], w["k"])):
+            n = part / torch.sqrt((part * part).mean(2, keepdim=True) + 1e-6) * weight
+            c, s = torch.cos(angle[b:e])[:, None], torch.sin(angle[b:e])[:, None]
+            lo, hi = n[..., :d // 2], n[..., d // 2:]
+            sides.append(torch.cat((lo * c - hi * s, lo * s + hi * c), 2))
+        q, k = sides
+        k, v = (y.repeat_interleave(h // g, 1) for y in (k, qkv[b:e, h + g:]))
+        p = torch.softmax((k * q[-1]).sum(2) / d ** 0.5, 0)  # the last word sees all
+        z.append(x[e - 1] + (p[..., None] * v).sum(0).flatten() @ w["out"])
+    z = torch.stack(z)
+    y = torch.nn.functional.layer_norm(z, (z.shape[1],), w["scale"], w["shift"], 1e-5)
+    want = torch.nn.functional.cross_entropy(y @ w["topics"].t(), topic)
+    assert abs(float(loss) - float(want.detach())) <= 1e-5 * float(want.detach())
+    # a chain of ten operators in 32 bits, sums of up to 2000 terms: 2000 e of the gradient's largest values
+    for name, got in zip(found, torch.autograd.grad(want, [w[n] for n in found])):
+        within(found[name], got, 2000 * E * (got.abs() + got.abs().max()))
+    before = [x.clone() for x in found.values()]
+    norm, _ = clip_reference(before, 0.5, 1e-6)
+    within(encoder.step(text, topic)[1], norm, 4 * E * norm)

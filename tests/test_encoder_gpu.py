@@ -18,3 +18,12 @@ def test_encoder_operators():
     print(p.stdout[-20000:], flush=True)
     assert p.returncode == 0, p.stdout[-4000:] + p.stderr[-4000:]
     assert re.search(r"\d+ passed", p.stdout) and "skipped" not in p.stdout
+
+
+def test_the_example_runs():
+    """examples/train_text_encoder.py: the operators together, and a search over what they made."""
+    args = [os.path.join("examples", "train_text_encoder.py"), "--topics", "50", "--words", "1000", "--steps", "30"]
+    p = subprocess.run([sys.executable, "-u"] + args, cwd=ROOT, capture_output=True, text=True, timeout=120)
+    print(p.stdout, flush=True)
+    assert p.returncode == 0, p.stderr[-4000:]
+    assert re.search(r"[0-9.]+ before, [0-9.]+ after", p.stdout) and "nan" not in p.stdout

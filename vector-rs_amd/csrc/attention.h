@@ -373,6 +373,22 @@ __device__ __forceinline__ void to_operand(const floatx16_t &v, typename Frag<T>
         for (int e = 0; e < E; ++e) o[k][e] = (T)v[k * E + e];
 }
 
+// c plus the sum of an operand's values.
+__device__ __forceinline__ float operand_sum(const MmVec<bf16_t>::v8 &v, float c) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    const v2 one = {(bf16_t)1.f, (bf16_t)1.f};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) c = __builtin_amdgcn_fdot2_f32_bf16(v2{v[e], v[e + 1]}, one, c, false);
+    return c;
+}
+__device__ __forceinline__ float operand_sum(const MmVec<half_t>::v8 &v, float c) {
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    const v2 one = {(half_t)1.f, (half_t)1.f};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) c = __builtin_amdgcn_fdot2(v2{v[e], v[e + 1]}, one, c, false);
+    return c;
+}
+
 // Writes a lane's part of a transposed result: its row's values 32 dt + 8 (i / 4) + 4 (lane / 32) + i % 4.
 template <class T, int DT, class F>
 __device__ __forceinline__ void store_cols(T *row, const floatx16_t (&acc)[DT], int dim, int lane, const F &f) {
@@ -410,7 +426,7 @@ struct Units {
     int e = 100;
     // ds (a lane's 16 values and those of its other half) in units, sums scaled anew where those got coarser
     template <int DT>
-    __device__ __forceinline__ void to_units(floatx16_t &ds, floatx16_t (&sum)[DT]) {
+    __device__ __forceinline__ void to_units(floatx16_t &ds, floatx16_t (&sum)[DT], float &sum2) {
         if constexpr (kOn) {
             float t = 0.f;
 #pragma unroll
@@ -420,6 +436,7 @@ struct Units {
             if (__any(next != e)) {
                 const float f = ldexpf(1.f, next - e);
                 e = next;
+                sum2 *= f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll

@@ -13,8 +13,9 @@
 //    delta come from LDS.  S and dP leave a lane with its own key's column.
 // delta comes from out, whose rounding and whose weights' rounding would go into every ds of the row: an error of 2.2e-3 of dq and
 // dk in bfloat16, more than rounding ds (1.8e-3) or the results (1.7e-3). But sum_j ds_rj is 0, so what the kernel by rows finds
-// for it, e_r, is delta's error times one: it hands delta + e to the kernel by keys, and takes e_r sum_j p_rj k_j off dq, an
-// eighth product, by operands that are in registers already (not in 32 bits).
+// for it is delta's error: it hands the exact one to the kernel by keys.  For dq it sums ds as rounded, and takes that sum
+// times sum_j p_rj k_j off: an eighth product, by operands that are in registers already, after which what is
+// multiplied sums to 0 again, so that neither delta's error nor what rounding adds to all keys alike is left (not in 32 bits).
 //
 // p and ds are rounded to the operands' type for the last products, which is half a unit of each; in float16 they are held
 // in powers of two of their own (p times 2^14, ds see Units).
@@ -35,7 +36,7 @@ struct BwdArgs {
     float scale;
     int splits;   // parts of what is summed over, each a workgroup; more than one leave `part`, which other kernels add up
     float *part;  // [split][2][token][head][DP]: dq and sum p k, or dk and dv
-    float *off;   // [split][token][head]: sum ds
+    float2 *off;  // [split][token][head]: sum ds, and of ds as rounded
 };
 
 constexpr int kBM = 128, kBK = 128;  // rows and keys of a workgroup
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
 
     constexpr bool EXACT = sizeof(T) == 2;  // see above
     floatx16_t dq[DT] = {}, pk[EXACT ? DT : 1] = {};
-    float off = 0.f;
+    float off = 0.f, rounded = 0.f;  // sum ds, and as rounded, in units
     Units<T> units;
     for (int t = t0; t < t1; ++t) {
         tiles_ready();
@@ -160,8 +161,9 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
                 off += sum[0] + sum[1];
                 to_operand<T>(s, p);
             }
-            units.to_units(dp, dq);
+            units.to_units(dp, dq, rounded);
             to_operand<T>(dp, ds);
+            if constexpr (EXACT) rounded = operand_sum(ds[1], operand_sum(ds[0], rounded));
             __builtin_amdgcn_sched_barrier(0);  // operands read ahead of these would not fit the registers
             if constexpr (EXACT)
                 mma_cols2<T, RB>(lds[buf][0], 32 * j, ds, dq, p, pk, ln);
@@ -171,10 +173,11 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
     }
     if (r >= n) return;
     off = half_sum(off);
+    rounded = units.back(half_sum(rounded));
     if (split == 0 && half == 0) a.delta[at_row] = a.splits > 1 ? delta : delta + off;
     if (a.splits > 1) {  // k_attn_sum_rows does the rest
         const int64_t all = a.rows.tokens * a.heads;
-        if (EXACT && half == 0) a.off[split * all + at_row] = off;
+        if (EXACT && half == 0) a.off[split * all + at_row] = make_float2(off, rounded);
         store_cols<float, DT>(a.part + (2 * split * all + at_row) * DP, dq, DP, lane, [&](float x) { return units.back(x); });
         if constexpr (EXACT)
             store_cols<float, DT>(a.part + ((2 * split + 1) * all + at_row) * DP, pk, DP, lane, [](float x) { return x; });
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             dq[d][i] = units.back(dq[d][i]);
-            if constexpr (EXACT) dq[d][i] = fmaf(-off, pk[d][i], dq[d][i]);
+            if constexpr (EXACT) dq[d][i] = fmaf(-rounded, pk[d][i], dq[d][i]);
         }
     store_cols<T, DT>((T *)(a.dq.data + row * (int64_t)a.dq.token + (int64_t)head * a.dq.head), dq, a.dim, lane,
                       [&](float x) { return x * a.scale; });
@@ -251,6 +254,7 @@ __global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves
     const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
 
     floatx16_t dk[DT] = {}, dv[DT] = {};
+    float none = 0.f;
     Units<T> units;
     for (int t = t0; t < t1; ++t) {
         tiles_ready();
@@ -284,7 +288,7 @@ __global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves
             __builtin_amdgcn_sched_barrier(0);  // operands read ahead of these would not fit the registers
             mma_cols<T, RB>(lds[buf][1], 32 * b, p, dv, ln);
             __builtin_amdgcn_sched_barrier(0);
-            units.to_units(dp, dk);
+            units.to_units(dp, dk, none);
             frag ds[kOps<T>];
             to_operand<T>(dp, ds);
             mma_cols<T, RB>(lds[buf][0], 32 * b, ds, dk, ln);
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(256) void k_attn_sum_rows(BwdArgs a) {
     const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x / L;
     const int e = threadIdx.x % L * 4;
     if (threadIdx.x >= R * L || i >= all || e >= a.dim) return;
-    float sum[4] = {}, pk[4] = {}, off = 0.f;
+    float sum[4] = {}, pk[4] = {}, off = 0.f, rounded = 0.f;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const Pack<float, 4> p = load_any<4>(a.part + (2 * s * all + i) * DP + e);
@@ -350,13 +354,15 @@ __global__ __launch_bounds__(256) void k_attn_sum_rows(BwdArgs a) {
             const Pack<float, 4> w = load_any<4>(a.part + ((2 * s + 1) * all + i) * DP + e);
 #pragma unroll
             for (int k = 0; k < 4; ++k) pk[k] += w.v[k];
-            off += a.off[s * all + i];
+            const float2 o = a.off[s * all + i];
+            off += o.x;
+            rounded += o.y;
         }
     }
     if (EXACT && e == 0) a.delta[i] += off;
     Pack<T, 4> v;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v.v[k] = (T)(fmaf(-off, pk[k], sum[k]) * a.scale);
+    for (int k = 0; k < 4; ++k) v.v[k] = (T)(fmaf(-rounded, pk[k], sum[k]) * a.scale);
     store_row<4>((T *)(a.dq.data + i / a.heads * (int64_t)a.dq.token + i % a.heads * (int64_t)a.dq.head), e, a.dim, v);
 }
 
@@ -385,7 +391,8 @@ __global__ __launch_bounds__(256) void k_attn_sum_keys(BwdArgs a) {
 // What a call works in: delta, then the parts of dq and afterwards, in the same place, those of dk and dv.
 struct Work {
     int qsplits, ksplits;
-    float *delta, *off, *part;
+    float *delta, *part;
+    float2 *off;
     size_t bytes;
 };
 Work work_of(int dtype, const Shape &s, void *base) {
@@ -402,7 +409,7 @@ Work work_of(int dtype, const Shape &s, void *base) {
     const size_t k = w.ksplits > 1 ? 2 * w.ksplits * s.key_tokens * s.kv_heads * dp : 0;
     Carver c{(char *)base};
     w.delta = c.take<float>(s.tokens * s.heads);
-    w.off = c.take<float>(w.qsplits > 1 ? w.qsplits * s.tokens * s.heads : 0);
+    w.off = c.take<float2>(w.qsplits > 1 ? w.qsplits * s.tokens * s.heads : 0);
     w.part = c.take<float>(q > k ? q : k);
     w.bytes = c.used;
     return w;

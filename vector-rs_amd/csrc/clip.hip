@@ -10,7 +10,9 @@
 //
 // The arrays' places go with the launch as kernel arguments, so nothing is copied to the device or kept there; more arrays
 // than fit take more launches. A launch's values are cut into chunks of one vector a thread, an array beginning with
-// a chunk of its own, and every workgroup takes a contiguous run of chunks.
+// a chunk of its own, and every workgroup takes a contiguous run of chunks, four vectors of a thread in flight.
+//
+// 456M values in bfloat16 (0.9 GB read twice, 0.9 written): 555 us, 4.9 TB/s; 594 with one vector in flight in the second kernel.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -120,7 +122,20 @@ __global__ __launch_bounds__(256) void k_squares(Batch b, double *part) {
 
 template <class T, class O>
 __device__ __forceinline__ void scale(const T *p, O *o, uint64_t n, float c) {
-    for (uint64_t i = threadIdx.x * 8; i < n; i += 2048) {
+    uint64_t i = threadIdx.x * 8;
+    for (; i + 3 * 2048 + 8 <= n; i += 4 * 2048) {
+        float v[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load8(v[k], p + i + k * 2048);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            Pack<O, 8> x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x.v[e] = (O)(v[k][e] * c);
+            store_any<8>(o + i + k * 2048, x);
+        }
+    }
+    for (; i < n; i += 2048) {
         if (i + 8 <= n) {
             float v[8];
             load8(v, p + i);

@@ -17,6 +17,10 @@
 // times sum_j p_rj k_j off: an eighth product, by operands that are in registers already, after which what is
 // multiplied sums to 0 again, so that neither delta's error nor what rounding adds to all keys alike is left (not in 32 bits).
 //
+// 1 x 32768 tokens, causal, 16 / 4 heads of 128 in bfloat16: by rows 7.2 ms (four products, 1.2 PFLOP/s), by keys 8.6 (1.02),
+// bound by power as the forward pass is.  8 sequences of 512 to 8192 tokens: 0.73 and 0.84 ms, and 0.04 to add up the parts of
+// dk and dv into which the longest sequences' rows are cut (without: 1.04).
+//
 // p and ds are rounded to the operands' type for the last products, which is half a unit of each; in float16 they are held
 // in powers of two of their own (p times 2^14, ds see Units).
 #include "attention.h"

@@ -3,6 +3,9 @@
 * ``layer_norm`` / ``layer_norm_backward``       the last layer before an embedding
 * ``softmax_xent`` / ``softmax_xent_grad``       cross entropy against every row of a table, and its gradients
 * ``orthogonalize``                              Newton-Schulz steps on update matrices
+* ``attention`` / ``attention_backward``         softmax attention over packed sequences with grouped heads
+* ``qk_norm_rotary`` / ``..._backward``          norms of queries and keys for each head, turned by position
+* ``gradient_norm`` / ``clip_gradients``         the norm of many arrays together, and clipping to a largest one
 
 They have no counterpart in the reference.  Arguments are arrays in the memory of one GPU: objects with the
 tensor interface of torch (``data_ptr()``, ``stride()``, ``new_empty()`` and so on), which this module does not
@@ -12,8 +15,8 @@ are float32, float16 and bfloat16.  The last dimension is contiguous; rows may b
 A call enqueues its work on the current stream of its arguments' device and returns without waiting, as
 other operations on such arrays do.  Wrong arguments raise ``InvalidConfig``; there is no CPU fallback.
 
-Outputs belong to no graph of automatic differentiation: gradients come from ``layer_norm_backward`` and
-``softmax_xent_grad``, which give them for any arguments and are themselves not differentiated.  The other calls
+Outputs belong to no graph of automatic differentiation: gradients come from ``softmax_xent_grad`` and the calls
+named ``..._backward``, which give them for any arguments and are themselves not differentiated.  The other calls
 refuse arguments that require a gradient where torch records a graph; call them under ``torch.no_grad()``, or
 with ``detach()``.  Tangents of forward-mode differentiation are not carried on either.
 

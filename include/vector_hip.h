@@ -467,7 +467,8 @@ typedef struct vhip_heads {
  * one fewer, so queries may be the last tokens of a longer text.
  *   s_rj = scale <q_r, k_j>,  lse_r = log sum_j exp s_rj,  out_r = sum_j exp(s_rj - lse_r) v_j
  * A row that sees no key has out 0 and lse -inf, and so has one of no sequence; keys and values that a row does not see
- * have no part in it, whatever they hold.  lse ([tokens, heads], may be NULL).  dim <= 128, tokens * heads <= 2^30. */
+ * have no part in it, whatever they hold.  lse ([tokens, heads], may be NULL).  dim <= 128, tokens * heads <= 2^30,
+ * |scale| <= 1e30. */
 size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                 size_t sequences);
 int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads *k, const vhip_heads *v, size_t tokens,
@@ -488,7 +489,7 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
 /* Norms of queries and keys for each head and the rotation by their tokens' positions, in one pass:
  *   r = 1 / sqrt(mean x^2 + eps),  n = x r weight,
  * then pair i of the first `rotary` columns (an even number; i and i + rotary / 2, or with `interleaved` 2 i and
- * 2 i + 1) turns by positions[t] * frequencies[i] radians, a product in 64 bits (exact positions up to 2^53).
+ * 2 i + 1) turns by positions[t] * frequencies[i] radians, a product in 64 bits (one past 2^52 gives NaN).
  * Weights (dim values of param_dtype, which is dtype or f32) may be NULL, and either side may have no heads.
  * dim <= 256. */
 int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_heads *q, const vhip_heads *k, size_t tokens,

@@ -695,6 +695,42 @@ def test_infinities_that_are_seen(tr, dtype):
         assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[torch.isinf(want)].float(), want[torch.isinf(want)])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(160, 1, 16), (128, 1, 64), (192, 2, 24), (7, 7, 128), (65, 13, 8)])
+def test_groups_of_any_size(tr, dtype, heads, kv, dim):
+    """Groups wider than a tile of rows, and of sizes that divide nothing."""
+    print("groups", heads, kv, dim, dtype, flush=True)
+    lq = [5, 0, 41, 1]
+    q, k, v, do = attention_case(lq, lq, heads, kv, dim, dtype)
+    for causal in (True, False):
+        want, tol = attention_reference(q, k, v, lq, lq, causal, 1 / math.sqrt(dim), do)
+        check_attention(attention_both(tr, q, k, v, do, bounds(lq), None, causal), want, tol)
+
+
+def test_no_sequences_and_no_rows(tr):
+    q, k, v, do = attention_case([6], [6], 4, 2, 32, "bf16")
+    none = torch.zeros(1, device="cuda", dtype=torch.int64)
+    out, lse, dq, dk, dv = attention_both(tr, q, k, v, do, none, None, True)
+    assert not out.any() and torch.isinf(lse).all() and not dq.any() and not dk.any() and not dv.any()
+    at, kat = bounds([0, 0]), bounds([4, 2])
+    out, lse, dq, dk, dv = attention_both(tr, q[:0], k, v, do[:0], at, kat, False)
+    assert out.shape == (0, 4, 32) and not dk.any() and not dv.any()
+    out, lse, dq, dk, dv = attention_both(tr, q, k[:0], v[:0], do, kat, at, False)
+    assert not out.any() and torch.isinf(lse).all() and not dq.any() and dk.shape == (0, 2, 32)
+    out, lse, dq, dk, dv = attention_both(tr, q[:0], k[:0], v[:0], do[:0], none, None, True)
+    assert dv.shape == (0, 2, 32)
+
+
+def test_angles_that_are_none(tr):
+    """A product of position and frequency past 2^52 has no angle: NaN in the pairs, and nowhere else."""
+    q, k, _, _, _ = head_norm_case(3, 2, 1, 16, 8, 0, "f32", "f32")
+    pos = torch.tensor([5, 2**53, 2**62], device="cuda")
+    a, b = tr.qk_norm_rotary(q, k, None, None, pos, torch.tensor([1.0, 2.0, 1e3, 1e30], device="cuda"))
+    for y in (a, b):
+        bad = torch.isnan(y)
+        assert not bad[..., 8:].any() and not bad[0, :, :3].any() and bad[0, :, 3].all() and bad[1:, :, :8].all()
+
+
 # ---- the operators together --------------------------------------------------------------------------
 
 def test_an_encoder_with_its_gradients(tr):

@@ -69,7 +69,7 @@ def clip(tr, rows=((P, P, 10, F32, F32),), count=None, **wrong):
 @pytest.mark.parametrize("what,wrong", [
     (attn, dict(dtype=3)), (attn, dict(dtype=-1)), (attn, dict(dim=0)), (attn, dict(dim=129, q=dict(token=258, head=129))), (attn, dict(heads=0)),
     (attn, dict(kv_heads=0)), (attn, dict(heads=3)), (attn, dict(offsets=None)), (attn, dict(key_tokens=7)), (attn, dict(scale=NAN)),
-    (attn, dict(scale=INF)), (attn, dict(q=dict(data=None))), (attn, dict(k=dict(data=None))), (attn, dict(v=dict(data=None))), (attn, dict(out=dict(data=None))),
+    (attn, dict(scale=INF)), (attn, dict(scale=-1e31)), (attn, dict(q=dict(data=None))), (attn, dict(k=dict(data=None))), (attn, dict(v=dict(data=None))), (attn, dict(out=dict(data=None))),
     (attn, dict(q=None)), (attn, dict(q=dict(token=31))), (attn, dict(k=dict(token=63))), (attn, dict(v=dict(head=31))), (attn, dict(out=dict(token=33, head=32))),
     (attn, dict(q=dict(data=P + 2))), (attn, dict(k=dict(token=(1 << 23) + 1))), (attn, dict(v=dict(token=32, head=(1 << 40) + 1))), (attn, dict(tokens=1 << 31)),
     (attn, dict(tokens=1 << 30, key_tokens=1 << 30)), (attn, dict(sequences=1 << 29)), (attn, dict(key_offsets=P, key_tokens=100_000, ws=None)),

@@ -306,7 +306,7 @@ int check_shape(int dtype, const Shape &s, const int64_t *offsets, const int64_t
     if (!offsets) return set_error(VHIP_ERR_INVALID_CONFIG, "offsets are null");
     if (!key_offsets && s.key_tokens != s.tokens)
         return set_error(VHIP_ERR_INVALID_CONFIG, "without key_offsets there are as many keys as queries");
-    if (!(fabsf(scale) <= 3.4e38f)) return set_error(VHIP_ERR_INVALID_CONFIG, "scale must be finite");
+    if (!(fabsf(scale) <= 1e30f)) return set_error(VHIP_ERR_INVALID_CONFIG, "scale must be finite, of 1e30 at most");
     if (s.tokens > (1u << 30) || s.key_tokens > (1u << 30) || s.sequences > (1u << 28) || s.tokens * s.heads > (1u << 30))
         return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
     return VHIP_OK;

@@ -114,7 +114,8 @@ struct Columns {
 __device__ __forceinline__ float2 cos_sin(int64_t position, float frequency) {
     const double a = (double)position * (double)frequency;
     const double k = rint(a * 0.63661977236758134308);  // quarter turns
-    const float r = (float)fma(-k, 6.123233995736766036e-17, fma(-k, 1.57079632679489661923, a));
+    // past 2^52 a product has no angle left
+    const float r = fabs(a) <= 4503599627370496. ? (float)fma(-k, 6.123233995736766036e-17, fma(-k, 1.57079632679489661923, a)) : NAN;
     const int q = (int)((long long)k & 3);
     const float z = r * r;
     const float s = r + r * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));

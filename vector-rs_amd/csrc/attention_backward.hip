@@ -45,9 +45,9 @@ struct BwdArgs {
 
 constexpr int kBM = 128, kBK = 128;  // rows and keys of a workgroup
 template <class T>
-constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // keys, or rows, of a tile
+constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 
-// Workgroups of a CU whose waves' registers hold all that they own: two have 256 a lane, one has 512.
+// Waves of a SIMD whose registers hold all that they own: two have 256 a lane, one has 512.
 template <class T, int DP>
 struct RegsFor {
     static constexpr int dq = sizeof(T) == 4 && DP > 96 ? 1 : 2;

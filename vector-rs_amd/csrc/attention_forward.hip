@@ -31,13 +31,15 @@ struct FwdArgs {
     int heads, kv_heads, dim;
     bool causal;
     float scale;
-    int splits;     // parts of the keys, each a workgroup; more than one leave `part`, which k_attn_join adds up
+    int splits;     // parts of the keys, each a workgroup; more than one leave `part`, which k_attn_join or k_attn_join_few adds up
     float *part;    // [split][token][head][DP]: outputs over their row's own m
     float2 *stats;  // [split][token][head]: m, l
 };
 
 constexpr int kBM = 128;
-constexpr int kFew = 8;  // parts
+// Parts of a row that its own few threads join, all loaded at once; more of them take a workgroup a row (18 parts of 160 rows:
+// 15.7 us by a loop of the row's threads, 5 by a workgroup; 2 parts of 98304 rows: 103 by a workgroup each).
+constexpr int kFew = 8;
 
 // Keys of a tile: 64, or 32 where they have 32 bits (two buffers of K and V of 128 columns in 64 KB, two workgroups a CU).
 template <class T>

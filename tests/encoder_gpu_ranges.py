@@ -1,0 +1,70 @@
+"""Attention, head norms and clipping where values, sizes and layouts are at their limits.  Definitions and tolerances are those
+of encoder_gpu_cases.py; what is new is derived where it stands.
+
+test_encoder_ranges_gpu.py runs this file in a process of its own, where torch is imported before the library."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from encoder_gpu_cases import (E, TINY, TYPES, UNIT, attention_both, attention_case, attention_reference, bounds, clip_arrays,  # noqa: E402,F401
+                               gen, head_norm_case, head_norm_reference, normal, tr, within)
+
+pytestmark = pytest.mark.gpu
+
+
+def odd_address(x):
+    """The same values one element off a vector's alignment."""
+    n, h, d = x.shape
+    y = torch.full((n * h * (d + 1) + 1,), math.nan, device=x.device, dtype=x.dtype)[1:].view(n, h, d + 1)[..., :d]
+    y.copy_(x)
+    return y
+
+
+# ---- infinities that are seen ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("dtype,dim", [("f32", 36), ("f32", 72), ("f32", 64), ("f16", 40), ("f16", 80), ("bf16", 72), ("bf16", 104), ("bf16", 128)])
+def test_keys_of_weight_zero_by_an_infinite_score(tr, dtype, dim, odd):
+    """A key whose last column is -inf where queries are positive has score -inf: the rows come out as without it.  Its own
+    gradients are 0, and the queries' are 0 * inf in that column alone."""
+    print("infinite keys", dtype, dim, odd, flush=True)
+    n, heads, kv = 150, 4, 2
+    q, k, v, do = attention_case([n], [n], heads, kv, dim, dtype)
+    q[..., -1] = q[..., -1].abs() + 0.5
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[[3, 40, 89, 149]] = False
+    k[~keep, :, -1] = -math.inf
+    want, tol = attention_reference(q, k[keep], v[keep], [n], [n - 4], False, 1 / math.sqrt(dim), do)
+    if odd:
+        q, k, v, do = (odd_address(x) for x in (q, k, v, do))
+    out, lse, dq, dk, dv = attention_both(tr, q, k, v, do, bounds([n]), None, False)
+    within(out, want["out"], tol["out"])
+    within(lse, want["lse"], tol["lse"])
+    within(dq[..., :-1], want["dq"][..., :-1], tol["dq"][..., :-1])
+    within(dk[keep], want["dk"], tol["dk"])
+    within(dv[keep], want["dv"], tol["dv"])
+    assert not dk[~keep].any() and not dv[~keep].any()
+
+
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("dtype,dim", [("f32", 36), ("f32", 72), ("f16", 40), ("bf16", 72), ("bf16", 104), ("bf16", 128)])
+def test_rows_whose_scores_are_all_minus_infinity(tr, dtype, dim, odd):
+    """Such a row counts as one that sees no key, and the keys' gradients come from the others (its own column times 0 aside)."""
+    print("rows of infinite scores", dtype, dim, odd, flush=True)
+    n, heads, kv = 150, 2, 2
+    q, k, v, do = attention_case([n], [n], heads, kv, dim, dtype)
+    k[..., -1] = k[..., -1].abs() + 0.5
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[[5, 70, 149]] = False
+    q[~keep, :, -1] = -math.inf
+    want, tol = attention_reference(q[keep], k, v, [n - 3], [n], False, 1 / math.sqrt(dim), do[keep])
+    if odd:
+        q, k, v, do = (odd_address(x) for x in (q, k, v, do))
+    out, lse, dq, dk, dv = attention_both(tr, q, k, v, do, bounds([n]), None, False)
+    for name, x in (("out", out), ("lse", lse), ("dq", dq)):
+        within(x[keep], want[name], tol[name])
+    assert not out[~keep].any() and not dq[~keep].any() and (lse[~keep] == -math.inf).all()
+    within(dk[..., :-1], want["dk"][..., :-1], tol["dk"][..., :-1])
+    within(dv, want["dv"], tol["dv"])

@@ -143,8 +143,9 @@ struct Tile {
         chunk = (n % CH) ^ swz(row);
     }
     // Loads the tile to `to`: row r is at base + at(r) bytes (uniform base; 32 or 64 bits), of `dim` values.  By DMA rows are
-    // whole chunks at 16-byte addresses, and chunks past the last are copies of it (the other operand has zeros
-    // there, or the result is not used); otherwise values come one vector at a time, zeros past dim.
+    // whole chunks at 16-byte addresses, and lanes whose chunk is past the last stay out of it: what is there are the zeros
+    // of clear_past, as infinities or NaN times the other operand's zeros would be NaN.  Otherwise values come one vector at a
+    // time, zeros past dim.
     template <class At>
     static __device__ __forceinline__ void load(const char *base, const At &at, int dim, char *to) {
         const int thread = anew(threadIdx.x);
@@ -156,7 +157,16 @@ struct Tile {
             one(base, at(r), c, dim, to, lds, i, thread);
         }
     }
-    // The same where row r + STEP i is i `step` bytes after row r (kEven): one lane's offset for all loads.
+    // Zeros in the chunks past the last of `rows` rows, tiles one behind the other.
+    static __device__ __forceinline__ void clear_past(int dim, int rows, char *to) {
+        if constexpr (DMA) {
+            const int first = dim * (int)sizeof(T) / 16;
+            if (first == CH) return;
+            for (int r = threadIdx.x; r < rows; r += NW * 64)
+                for (int c = first; c < CH; ++c) *(Pack<float, 4> *)(to + r * RB + (c ^ swz(r)) * 16) = Pack<float, 4>{};
+        }
+    }
+    // load() where row r + STEP i is i `step` bytes after row r (kEven): one lane's offset for all loads.
     template <class At>
     static __device__ __forceinline__ void load_even(const char *base, const At &at, int64_t step, int dim, char *to) {
         const int thread = anew(threadIdx.x);
@@ -176,11 +186,11 @@ struct Tile {
     static __device__ __forceinline__ void one(const char *base, Off off, int c, int dim, char *to, uint32_t lds, int i, int thread) {
         if (!kWhole && i == N - 1 && (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= ROWS * CH / 64 - i * NW) return;
         if constexpr (DMA) {
-            const int last = dim * (int)sizeof(T) / 16 - 1;
+            if (c >= dim * (int)sizeof(T) / 16) return;
             if constexpr (sizeof(Off) == 4)
-                dma_lds16_at(base, off + (uint32_t)min(c, last) * 16, lds + i * NW * 1024);
+                dma_lds16_at(base, off + (uint32_t)c * 16, lds + i * NW * 1024);
             else
-                dma_lds16_far(base + off + min(c, last) * 16, lds + i * NW * 1024);
+                dma_lds16_far(base + off + c * 16, lds + i * NW * 1024);
         } else {
             const auto v = load_row<VEC>((const T *)(base + off), c * VEC, dim);
             *(Pack<T, VEC> *)(to + (i * NW * 64 + thread) * 16) = v;

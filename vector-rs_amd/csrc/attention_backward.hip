@@ -113,6 +113,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
         load_rows<KV, BN>(vb, a.v.token, t * BN, keys.len - 1, a.dim, lds[buf][1]);
     };
     if (t0 < t1) load(t0, 0);
+    KV::clear_past(a.dim, 4 * BN, lds[0][0]);
 
     const int64_t at_row = row * a.heads + head;
     frag q[KS], go[KS];
@@ -250,6 +251,7 @@ __global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves
         load(t0, 0);
         put_stats(0);
     }
+    QG::clear_past(a.dim, 4 * BR, lds[0][0]);
 
     const int jc = min(j, keys.len - 1);
     frag k[KS], v[KS];

@@ -94,6 +94,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void k_attn_forward(FwdArgs a
         load_rows<KV, BN>(vb, a.v.token, t * BN, keys.len - 1, a.dim, lds[buf][1]);
     };
     if (t0 < t1) load(t0, 0);
+    KV::clear_past(a.dim, 4 * BN, lds[0][0]);
 
     frag q[KS];
     {

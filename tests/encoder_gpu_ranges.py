@@ -68,3 +68,22 @@ def test_rows_whose_scores_are_all_minus_infinity(tr, dtype, dim, odd):
     assert not out[~keep].any() and not dq[~keep].any() and (lse[~keep] == -math.inf).all()
     within(dk[..., :-1], want["dk"][..., :-1], tol["dk"][..., :-1])
     within(dv, want["dv"], tol["dv"])
+
+
+# ---- bits that do not depend on other rows -----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (6, 2, 128), (3, 1, 40)])
+@pytest.mark.parametrize("size", [8.0, 100.0, 1000.0])
+def test_keys_that_are_not_seen_move_no_bit(tr, dtype, heads, kv, dim, size):
+    """Causal: rows before keys of far larger scores keep their bits, though rows of the same tile see them."""
+    print("larger keys", dtype, heads, kv, dim, size, flush=True)
+    lq, cut = [150, 300], 83
+    q, k, v, _ = attention_case(lq, lq, heads, kv, dim, dtype)
+    out, lse = tr.attention(q, k, v, bounds(lq))
+    k[cut:150] = (k[cut:150].float() * size).to(k.dtype)
+    got, gl = tr.attention(q, k, v, bounds(lq))
+    keep = torch.ones(450, dtype=torch.bool, device="cuda")
+    keep[cut:150] = False
+    assert torch.equal(got[keep], out[keep]) and torch.equal(gl[keep], lse[keep])
+    assert not torch.equal(got[cut:150], out[cut:150])

@@ -136,8 +136,9 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void k_attn_forward(FwdArgs a
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
         top = half_max(top) * c;
-        if (__any(top > m + 8.f)) {
-            const float next = fmaxf(m, top);
+        const bool grown = top > m + 8.f;  // a row's own matter: others of its wave may see keys that it does not
+        if (__any(grown)) {
+            const float next = grown ? top : m;
             const float f = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
             m = next;
             l *= f;

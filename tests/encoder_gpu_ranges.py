@@ -87,3 +87,47 @@ def test_keys_that_are_not_seen_move_no_bit(tr, dtype, heads, kv, dim, size):
     keep[cut:150] = False
     assert torch.equal(got[keep], out[keep]) and torch.equal(gl[keep], lse[keep])
     assert not torch.equal(got[cut:150], out[cut:150])
+
+
+# ---- head norms of rows of any size ------------------------------------------------------------------------
+
+ROWS = [(40, 4, 2, 128, 128, False), (33, 3, 1, 80, 40, True), (70, 2, 2, 20, 12, False), (9, 1, 1, 256, 64, True)]
+
+
+def rows_of_sizes(tokens, heads, kv, dim, rot, dtype, size):
+    """Every second row `size` times as large."""
+    q, k, w, pos, freq = head_norm_case(tokens, heads, kv, dim, rot, 0, "f32", "f32")
+    q, k = (x.double() for x in (q, k))
+    q[::2], k[1::2] = q[::2] * size, k[1::2] * size
+    return q.float().to(TYPES[dtype]), k.float().to(TYPES[dtype]), w, pos, freq
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,near", ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,eps", [(1e17, 1e-6), (3e18, 0.0), (1e19, 1e-6), (1e25, 1e-6), (2e37, 1e-6), (2e37, 1e30), (1e-18, 0.0), (1e-21, 0.0), (1e-18, 1e-36),
+                                      (1e-30, 0.0), (1e-30, 1e-6), (1e-39, 0.0)])
+def test_head_norm_of_rows_of_any_size(tr, tokens, heads, kv, dim, rot, near, dtype, size, eps):
+    """Rows whose squares are past the range of 32 bits, beside ordinary ones."""
+    print("rows of size", size, eps, tokens, heads, kv, dim, rot, near, dtype, flush=True)
+    q, k, w, pos, freq = rows_of_sizes(tokens, heads, kv, dim, rot, dtype, size)
+    angle = pos.double()[:, None] * freq.double()
+    got = tr.qk_norm_rotary(q, k, w[0], w[1], pos, freq, eps=eps, interleaved=near)
+    for x, y, wt in zip((q, k), got, w):
+        want, tol = head_norm_reference(x, wt, angle, near, eps)
+        within(y, want, tol + UNIT[y.dtype] * want.abs() + TINY[y.dtype])
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,near", ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,eps,dsize", [(1e17, 1e-6, 1.0), (1e19, 1e-6, 1.0), (1e25, 1e-6, 1.0), (2e37, 1e-6, 1.0), (2e37, 1e30, 1.0), (1e-18, 0.0, 1.0),
+                                            (1e-21, 0.0, 1.0), (1e-18, 1e-36, 1.0), (1e-30, 0.0, 1.0), (1e15, 1e-6, 1e28), (2e37, 1e-6, 1e30), (1e-12, 0.0, 1e-32)])
+def test_head_norm_backward_of_rows_of_any_size(tr, tokens, heads, kv, dim, rot, near, dtype, size, eps, dsize):
+    print("gradients of rows of size", size, eps, dsize, tokens, heads, kv, dim, rot, near, dtype, flush=True)
+    q, k, w, pos, freq = rows_of_sizes(tokens, heads, kv, dim, rot, dtype, size)
+    dq, dk = ((dsize * normal(8 + i, *x.shape).double()).float().to(x.dtype) for i, x in enumerate((q, k)))
+    angle = pos.double()[:, None] * freq.double()
+    got = tr.qk_norm_rotary_backward(dq, dk, q, k, w[0], w[1], pos, freq, eps=eps, interleaved=near)
+    for x, g, wt, dx, dw in zip((q, k), (dq, dk), w, got[:2], got[2:]):
+        want, tol, wantw, tolw = head_norm_reference(x, wt, angle, near, eps, g)
+        within(dx, want, tol + UNIT[x.dtype] * want.abs() + TINY[x.dtype])
+        within(dw, wantw, tolw + UNIT[wt.dtype] * wantw.abs() + TINY[wt.dtype])

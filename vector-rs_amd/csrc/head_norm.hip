@@ -136,6 +136,33 @@ __device__ __forceinline__ float row_lanes_sum(float x, int lanes_log2) {
     return x;
 }
 
+// A row's squares fit 32 bits where their mean is far from both ends of these.  Other rows (values from about 1e18 on; below
+// 3e-14 where eps is as small as their squares) are taken in units of 2^k, with which the larger of their largest value and
+// sqrt(eps) is near 1: x and the row's mean are replaced by theirs in these units, and the scale that comes of it is 2^k too large.
+__device__ __forceinline__ bool ordinary(float mean) { return mean > 0x1p-90f && mean < 0x1p120f; }
+template <int VEC>
+__device__ __forceinline__ int to_units(float (&x)[2][VEC], float &mean, const HeadArgs &a, float inv) {
+    float top = 0.f, sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = fmaxf(top, fabsf(x[v][e]));
+    for (int l = 0; l < a.lanes_log2; ++l) top = fmaxf(top, __shfl_xor(top, 1 << l, 64));
+    int k = top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -200;
+    if (a.eps > 0.f) k = max(k, __builtin_amdgcn_frexp_expf(a.eps) >> 1);
+    if (ordinary(mean)) k = 0;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            x[v][e] = ldexpf(x[v][e], -k);
+            sum = fmaf(x[v][e], x[v][e], sum);
+        }
+    sum = row_lanes_sum(sum, a.lanes_log2);
+    if (!ordinary(mean)) mean = fmaf(sum, inv, ldexpf(a.eps, -2 * k));
+    return k;
+}
+
 // Which side a wave has, and its place among that side's.
 struct Waves {
     int side, slot, slots, t;
@@ -187,7 +214,9 @@ __global__ __launch_bounds__(256) void k_head_forward(HeadArgs a) {
         for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) sum = fmaf(x[v][e], x[v][e], sum);
-        const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
+        float mean = fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps);
+        if (__any(!ordinary(mean))) to_units<VEC>(x, mean, a, inv);
+        const float r = 1.f / sqrtf(mean);
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -224,20 +253,30 @@ __global__ __launch_bounds__(256) void k_head_backward(HeadArgs a) {
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    sum = fmaf(x[v][e], x[v][e], sum);
-                    dot = fmaf(x[v][e], g[v][e] * w[v][e], dot);
-                }
-            const float r = 1.f / sqrtf(fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps));
-            const float m = row_lanes_sum(dot, a.lanes_log2) * r * inv;  // mean of u xh
+                for (int e = 0; e < VEC; ++e) sum = fmaf(x[v][e], x[v][e], sum);
+            float mean = fmaf(row_lanes_sum(sum, a.lanes_log2), inv, a.eps);
+            int units = 0;
+            if (__any(!ordinary(mean))) units = to_units<VEC>(x, mean, a, inv);
+            const float r = 1.f / sqrtf(mean);
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float xh = x[v][e] * r;
-                    dw[v][e] = fmaf(g[v][e], xh, dw[v][e]);
-                    x[v][e] = r * (g[v][e] * w[v][e] - xh * m);
+                    x[v][e] *= r;
+                    dw[v][e] = fmaf(g[v][e], x[v][e], dw[v][e]);
+                    g[v][e] *= w[v][e];
+                    dot = fmaf(x[v][e], g[v][e], dot);  // of values near 1, so that it is as large as u
                 }
+            const float m = row_lanes_sum(dot, a.lanes_log2) * inv;  // mean of u xh
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[v][e] = r * (g[v][e] - x[v][e] * m);
+            if (__any(units))
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) x[v][e] = ldexpf(x[v][e], -units);
             cols.store((T *)(side.out + (tok0 + k) * side.out_token + h * side.out_head), x);
         }
     }

@@ -131,3 +131,44 @@ def test_head_norm_backward_of_rows_of_any_size(tr, tokens, heads, kv, dim, rot,
         want, tol, wantw, tolw = head_norm_reference(x, wt, angle, near, eps, g)
         within(dx, want, tol + UNIT[x.dtype] * want.abs() + TINY[x.dtype])
         within(dw, wantw, tolw + UNIT[wt.dtype] * wantw.abs() + TINY[wt.dtype])
+
+
+# ---- clipping and graphs of automatic differentiation ------------------------------------------------------
+
+def test_arrays_that_are_clipped_count_as_changed(tr):
+    """A graph that saved an array raises once the array was clipped or written to, as after torch's own operations."""
+    import vector_hip as vh
+
+    w, g, o = torch.ones(50, device="cuda", requires_grad=True), 10 * normal(1, 50), normal(2, 50)
+    for call, saved in ((lambda: tr.clip_gradients([g], 1.0), g), (lambda: tr.clip_gradients([g], 1.0, out=[o]), o),
+                        (lambda: tr.clip_gradients([g[:20], g[20:]], 1.0), g)):
+        loss = (w * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # what is only read stays valid, and so does what a refused call was given
+    loss, want = (w * g).sum(), g.clone()
+    tr.gradient_norm([g])
+    tr.clip_gradients([g], 1.0, out=[o])
+    with pytest.raises(vh.InvalidConfig):
+        tr.clip_gradients([g], -1.0)
+    loss.backward()
+    assert torch.equal(w.grad, want)
+
+
+def test_outputs_that_require_a_gradient_are_refused(tr):
+    import vector_hip as vh
+
+    g, leaf = normal(1, 50), torch.zeros(50, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(vh.InvalidConfig):
+            tr.clip_gradients([g], 1.0, out=[out])
+        assert not out.any()
+    with torch.no_grad():
+        tr.clip_gradients([g], 1e6, out=[leaf])
+    assert torch.equal(leaf.detach(), g)
+    with torch.inference_mode():  # arrays without a version
+        a, b = g + 1, g + 1
+        tr.clip_gradients([a], 1e6, out=[b])
+        tr.clip_gradients([a], 1e6)
+        assert torch.equal(a, b)

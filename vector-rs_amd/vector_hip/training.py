@@ -17,7 +17,7 @@ other operations on such arrays do.  Wrong arguments raise ``InvalidConfig``; th
 
 Outputs belong to no graph of automatic differentiation: gradients come from ``softmax_xent_grad`` and the calls
 named ``..._backward``, which give them for any arguments and are themselves not differentiated.  The other calls
-refuse arguments that require a gradient where torch records a graph; call them under ``torch.no_grad()``, or
+refuse arguments (``out`` among them) that require a gradient where torch records a graph; call them under ``torch.no_grad()``, or
 with ``detach()``.  Tangents of forward-mode differentiation are not carried on either.
 
 Load torch before ``vector_hip``: torch brings a HIP runtime of its own, which this package's library then
@@ -108,6 +108,8 @@ class _Library:
         _one_runtime()
         self.f32, self.u8, self.i64 = lib.float32, lib.uint8, lib.int64
         self.records = getattr(lib, "is_grad_enabled", lambda: False)
+        # counts arrays as changed, so that a graph that saved one raises where its gradient would come of other values
+        self.changed = lib.autograd.graph.increment_version if hasattr(lib, "autograd") else lambda arrays: None
         current = lib.cuda.current_stream
         self.stream = getattr(lib._C, "_cuda_getCurrentRawStream", lambda index: current(index).cuda_stream)
 
@@ -465,7 +467,6 @@ def _arrays(gradients, out):
             at, code = g.data_ptr(), _code[g.dtype]
             table.extend((at, at, g.numel(), code | code << 32))
     else:
-        out = list(out)
         if len(out) != len(gradients):
             raise InvalidConfig("out must hold an array for each gradient")
         for g, o in zip(gradients, out):
@@ -493,9 +494,11 @@ def gradient_norm(gradients):
 def clip_gradients(gradients, max_norm: float, out=None, eps: float = 1e-6):
     """gradient_norm of the arrays; each is scaled by min(1, max_norm / (norm + eps)), in place or into the arrays `out`
     (the same shapes, any of the types), which overlap nothing else.  A norm that is infinite or NaN is no error: it
-    leaves zeros and NaN."""
+    leaves zeros and NaN.  What is written counts as changed: a graph of torch that saved it raises."""
     gradients = list(gradients)
+    out = None if out is None else list(out)
     table, n, norm, ws, need, device, lib = _arrays(gradients, out)
-    _no_graph(lib, *gradients)
+    _no_graph(lib, *gradients, *(out or ()))
     _check(_lib.vhip_clip_gradients(device, table.buffer_info()[0], n, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need, lib.stream(device)))
+    lib.changed(gradients if out is None else out)
     return norm

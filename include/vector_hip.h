@@ -468,7 +468,8 @@ typedef struct vhip_heads {
  *   s_rj = scale <q_r, k_j>,  lse_r = log sum_j exp s_rj,  out_r = sum_j exp(s_rj - lse_r) v_j
  * A row that sees no key has out 0 and lse -inf, and so has one of no sequence; keys and values that a row does not see
  * have no part in it, whatever they hold.  lse ([tokens, heads], may be NULL).  dim <= 128, tokens * heads <= 2^30,
- * |scale| <= 1e30. */
+ * |scale| <= 1e30; kv_heads * (sequences + 2), and a tile more for each 128 rows of a key head (backward: or keys), stay
+ * below 2^31. */
 size_t vhip_attention_workspace(int dtype, size_t tokens, size_t key_tokens, size_t heads, size_t kv_heads, size_t dim,
                                 size_t sequences);
 int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads *k, const vhip_heads *v, size_t tokens,

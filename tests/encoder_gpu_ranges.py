@@ -172,3 +172,33 @@ def test_outputs_that_require_a_gradient_are_refused(tr):
         tr.clip_gradients([a], 1e6, out=[b])
         tr.clip_gradients([a], 1e6)
         assert torch.equal(a, b)
+
+
+# ---- more workgroups than one launch has -------------------------------------------------------------------
+
+def test_attention_over_more_sequences_than_a_launch_has_workgroups(tr):
+    """A launch has fewer than 2^32 threads: 2^24 workgroups of 256.  1.1 million sequences of 16 key heads take more, most of
+    them empty here; those that are not come out as in a call of their own."""
+    count, heads, dim = 1_100_000, 16, 16
+    at = torch.zeros(count + 1, device="cuda", dtype=torch.int64)
+    lengths = {0: 5, 400_000: 3, 700_001: 7, count - 1: 4}
+    for s, n in lengths.items():
+        at[s + 1:] += n
+    n = sum(lengths.values())
+    q, k, v, do = attention_case([n], [n], heads, heads, dim, "bf16")
+    want = attention_both(tr, q, k, v, do, bounds(list(lengths.values())), None, True)
+    got = attention_both(tr, q, k, v, do, at, None, True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_head_norms_of_more_tokens_than_a_launch_has(tr):
+    """2 tokens are a workgroup's: 2^25 tokens are more than a launch has."""
+    tokens, dim = (1 << 25) + 5, 2
+    q = normal(1, tokens, 1, dim).half()
+    k = q.new_empty(tokens, 0, dim)
+    pos, freq = torch.arange(tokens, device="cuda"), torch.ones(1, device="cuda")
+    got = tr.qk_norm_rotary(q, k, None, None, pos, freq)[0]
+    for b, e in ((0, 1 << 24), (1 << 24, 1 << 25), ((1 << 25) - 1001, tokens)):
+        part = tr.qk_norm_rotary(q[b:e], k[b:e], None, None, pos[b:e], freq)[0]
+        assert torch.equal(got[b:e], part)

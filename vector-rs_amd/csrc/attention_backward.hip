@@ -41,6 +41,7 @@ struct BwdArgs {
     int splits;   // parts of what is summed over, each a workgroup; more than one leave `part`, which other kernels add up
     float *part;  // [split][2][token][head][DP]: dq and sum p k, or dk and dv
     float2 *off;  // [split][token][head]: sum ds, and of ds as rounded
+    uint32_t first;  // workgroup of this launch
 };
 
 constexpr int kBM = 128, kBK = 128;  // rows and keys of a workgroup
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(256, (RegsFor<T, DP>::dq)) void k_attn_dq(BwdArgs a
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KV::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
-    const uint32_t id = blockIdx.x;
+    const uint32_t id = a.first + blockIdx.x;
     const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
     const Place at = find_tile<kBM>(a.rows, a.group.size, id / a.kv_heads / a.splits);
     const Span rows = packed_span(a.rows, at.seq);
@@ -209,7 +210,7 @@ __global__ __launch_bounds__((64 * ByKeys<T, DP>::waves), (ByKeys<T, DP>::halves
     __shared__ __attribute__((aligned(16))) float stats[2][2][BR];  // -lse in base 2, delta
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
-    const uint32_t id = blockIdx.x;
+    const uint32_t id = a.first + blockIdx.x;
     const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
     const Place at = find_tile<kBK>(a.keys, 1, id / a.kv_heads / a.splits);
     const Span keys = packed_span(a.keys, at.seq);
@@ -424,7 +425,7 @@ Work work_of(int dtype, const Shape &s, void *base) {
 struct Run {
     Work w;
     bool dq, dkv, dma_kv, dma_q;
-    uint32_t qgrid, kgrid;
+    int64_t qgrid, kgrid;
     hipStream_t s;
 };
 
@@ -432,18 +433,25 @@ template <class T, int DP>
 int launch(BwdArgs a, const Run &r) {
     if (r.qgrid) {
         a.splits = r.w.qsplits;
-        if (r.dma_kv)
-            k_attn_dq<T, DP, true><<<r.qgrid, 256, 0, r.s>>>(a);
-        else
-            k_attn_dq<T, DP, false><<<r.qgrid, 256, 0, r.s>>>(a);
+        each_launch(r.qgrid, 256, [&](int64_t first, uint32_t n) {
+            a.first = (uint32_t)first;
+            if (r.dma_kv)
+                k_attn_dq<T, DP, true><<<n, 256, 0, r.s>>>(a);
+            else
+                k_attn_dq<T, DP, false><<<n, 256, 0, r.s>>>(a);
+        });
         if (a.splits > 1) k_attn_sum_rows<T, DP><<<(uint32_t)ceil_div(a.rows.tokens * a.heads, kRowsOf256<DP>), 256, 0, r.s>>>(a);
     }
     if (r.kgrid) {
         a.splits = r.w.ksplits;
-        if (r.dma_q)
-            k_attn_dkv<T, DP, true><<<r.kgrid, 64 * ByKeys<T, DP>::waves, 0, r.s>>>(a);
-        else
-            k_attn_dkv<T, DP, false><<<r.kgrid, 64 * ByKeys<T, DP>::waves, 0, r.s>>>(a);
+        constexpr int threads = 64 * ByKeys<T, DP>::waves;
+        each_launch(r.kgrid, threads, [&](int64_t first, uint32_t n) {
+            a.first = (uint32_t)first;
+            if (r.dma_q)
+                k_attn_dkv<T, DP, true><<<n, threads, 0, r.s>>>(a);
+            else
+                k_attn_dkv<T, DP, false><<<n, threads, 0, r.s>>>(a);
+        });
         if (a.splits > 1)
             k_attn_sum_keys<T, DP><<<dim3((uint32_t)ceil_div(a.keys.tokens * a.kv_heads, kRowsOf256<DP>), 2), 256, 0, r.s>>>(a);
     }
@@ -500,8 +508,8 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
     if (qgrid > 0x7fffffff || kgrid > 0x7fffffff) return set_error(VHIP_ERR_INVALID_CONFIG, "too many rows or sequences");
     CallDevice dev;
     VH_CHECK(dev.enter(ordinal));
-    r.qgrid = tokens ? (uint32_t)qgrid : 0;
-    r.kgrid = key_tokens ? (uint32_t)kgrid : 0;
+    r.qgrid = tokens ? qgrid : 0;
+    r.kgrid = key_tokens ? kgrid : 0;
     r.dma_kv = whole_chunks(k, dtype, dim) && whole_chunks(v, dtype, dim);
     r.dma_q = whole_chunks(q, dtype, dim) && whole_chunks(dout, dtype, dim);
     r.s = (hipStream_t)stream;
@@ -509,7 +517,7 @@ int vhip_attention_backward(int ordinal, int dtype, const vhip_heads *dout, cons
                     to_heads(dq, dtype), to_heads(dk, dtype), to_heads(dv, dtype), lse, r.w.delta,
                     {offsets, (int64_t)tokens, (int)sequences},
                     {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
-                    to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, 1, r.w.part, r.w.off};
+                    to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, 1, r.w.part, r.w.off, 0};
     switch (dtype) {
         case VHIP_DTYPE_F32: return launch<float>(a, r);
         case VHIP_DTYPE_F16: return launch<half_t>(a, r);

@@ -34,6 +34,7 @@ struct FwdArgs {
     int splits;     // parts of the keys, each a workgroup; more than one leave `part`, which k_attn_join or k_attn_join_few adds up
     float *part;    // [split][token][head][DP]: outputs over their row's own m
     float2 *stats;  // [split][token][head]: m, l
+    uint32_t first;  // workgroup of this launch
 };
 
 constexpr int kBM = 128;
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void k_attn_forward(FwdArgs a
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KV::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
-    const uint32_t id = blockIdx.x;
+    const uint32_t id = a.first + blockIdx.x;
     const int kh = id % a.kv_heads, split = (id / a.kv_heads) % a.splits;
     const Place at = find_tile<kBM>(a.rows, a.group.size, id / a.kv_heads / a.splits);
     const Span rows = packed_span(a.rows, at.seq);
@@ -279,11 +280,14 @@ __global__ __launch_bounds__(256) void k_attn_join(FwdArgs a) {
 }
 
 template <class T, int DP>
-int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
-    if (dma)
-        k_attn_forward<T, DP, true><<<grid, 256, 0, s>>>(a);
-    else
-        k_attn_forward<T, DP, false><<<grid, 256, 0, s>>>(a);
+int launch(FwdArgs a, bool dma, int64_t grid, hipStream_t s) {
+    each_launch(grid, 256, [&](int64_t first, uint32_t n) {
+        a.first = (uint32_t)first;
+        if (dma)
+            k_attn_forward<T, DP, true><<<n, 256, 0, s>>>(a);
+        else
+            k_attn_forward<T, DP, false><<<n, 256, 0, s>>>(a);
+    });
     if (a.splits > kFew)
         k_attn_join<T, DP><<<(uint32_t)(a.rows.tokens * a.heads), 256, 0, s>>>(a);
     else if (a.splits > 1)
@@ -291,7 +295,7 @@ int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
     return launch_status("attention launch");
 }
 template <class T>
-int launch(const FwdArgs &a, bool dma, uint32_t grid, hipStream_t s) {
+int launch(const FwdArgs &a, bool dma, int64_t grid, hipStream_t s) {
     switch (padded(a.dim)) {
         case 32: return launch<T, 32>(a, dma, grid, s);
         case 64: return launch<T, 64>(a, dma, grid, s);
@@ -377,13 +381,13 @@ int vhip_attention(int ordinal, int dtype, const vhip_heads *q, const vhip_heads
               {offsets, (int64_t)tokens, (int)sequences},
               {key_offsets ? key_offsets : offsets, (int64_t)key_tokens, (int)sequences},
               to_group(heads, kv_heads), (int)heads, (int)kv_heads, (int)dim, causal != 0, scale, splits, (float *)workspace,
-              (float2 *)((float *)workspace + (size_t)splits * tokens * heads * padded(dim))};
+              (float2 *)((float *)workspace + (size_t)splits * tokens * heads * padded(dim)), 0};
     const bool dma = whole_chunks(k, dtype, dim) && whole_chunks(v, dtype, dim);
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
-        case VHIP_DTYPE_F32: return launch<float>(a, dma, (uint32_t)grid, s);
-        case VHIP_DTYPE_F16: return launch<half_t>(a, dma, (uint32_t)grid, s);
-        default: return launch<bf16_t>(a, dma, (uint32_t)grid, s);
+        case VHIP_DTYPE_F32: return launch<float>(a, dma, grid, s);
+        case VHIP_DTYPE_F16: return launch<half_t>(a, dma, grid, s);
+        default: return launch<bf16_t>(a, dma, grid, s);
     }
 }
 

@@ -48,6 +48,7 @@ struct HeadArgs {
     int key_waves;                        // of 4
     bool f32_params;
     float eps;
+    int64_t first;  // token of this launch, forward
 };
 
 // A lane's columns of a row, two vectors: of pairs (lanes below ceil(pairs / VEC)), or of what is not turned.
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(256) void k_head_forward(HeadArgs a) {
     const Waves at(a);
     const Cols cols(at.t, a.dim, a.pairs);
     const Side &side = a.side[at.side];
-    const int64_t tok0 = (int64_t)blockIdx.x * a.at_once;
+    const int64_t tok0 = a.first + (int64_t)blockIdx.x * a.at_once;
     const int count = (int)min((int64_t)a.at_once, a.tokens - tok0);
     typename Cols::Values w;
     load_weight<T, NEAR>(w, cols, a, side.weight);
@@ -382,12 +383,14 @@ Side to_side(int dtype, const vhip_heads *x, const vhip_heads *dy, const vhip_he
 }
 
 template <class T>
-int forward(const HeadArgs &a, bool near, hipStream_t s) {
-    const uint32_t grid = (uint32_t)((a.tokens + a.at_once - 1) / a.at_once);
-    if (near)
-        k_head_forward<T, true><<<grid, 256, 0, s>>>(a);
-    else
-        k_head_forward<T, false><<<grid, 256, 0, s>>>(a);
+int forward(HeadArgs a, bool near, hipStream_t s) {
+    each_launch((a.tokens + a.at_once - 1) / a.at_once, 256, [&](int64_t first, uint32_t n) {
+        a.first = first * a.at_once;
+        if (near)
+            k_head_forward<T, true><<<n, 256, 0, s>>>(a);
+        else
+            k_head_forward<T, false><<<n, 256, 0, s>>>(a);
+    });
     return launch_status("head norm launch");
 }
 
@@ -433,7 +436,7 @@ int vhip_qk_norm_rotary(int ordinal, int dtype, int param_dtype, const vhip_head
     const int l = row_lanes_log2(dim, rotary, dtype);
     const HeadArgs a{{to_side(dtype, q, nullptr, q_out, q_weight, heads), to_side(dtype, k, nullptr, k_out, k_weight, kv_heads)},
                      positions, frequencies, nullptr, (int64_t)tokens, (int)dim, (int)rotary / 2, l,
-                     tokens_at_once(tokens, kTokForward), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps};
+                     tokens_at_once(tokens, kTokForward), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps, 0};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case VHIP_DTYPE_F32: return forward<float>(a, interleaved, s);
@@ -469,7 +472,7 @@ int vhip_qk_norm_rotary_backward(int ordinal, int dtype, int param_dtype, const 
     const int l = row_lanes_log2(dim, rotary, dtype);
     const HeadArgs a{{to_side(dtype, q, dq, dq_out, q_weight, heads), to_side(dtype, k, dk, dk_out, k_weight, kv_heads)},
                      positions, frequencies, dq_weight || dk_weight ? (float *)workspace : nullptr, (int64_t)tokens, (int)dim,
-                     (int)rotary / 2, l, tokens_at_once(tokens, kTokBackward), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps};
+                     (int)rotary / 2, l, tokens_at_once(tokens, kTokBackward), key_waves(heads, kv_heads), param_dtype == VHIP_DTYPE_F32, eps, 0};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case VHIP_DTYPE_F32: return backward<float>(a, interleaved, dq_weight, dk_weight, s);

@@ -77,6 +77,13 @@ inline int lanes_log2(size_t chunks) {
     return l;
 }
 
+// Calls f(first workgroup, workgroups) for the launches that `groups` workgroups of `threads` take: one has fewer than 2^32 threads.
+template <class F>
+inline void each_launch(int64_t groups, int threads, const F &f) {
+    const int64_t most = 0xffffffffll / threads;
+    for (int64_t first = 0; first < groups; first += most) f(first, (uint32_t)(groups - first < most ? groups - first : most));
+}
+
 // Status of the launches of a call so far.
 inline int launch_status(const char *what) {
     const hipError_t e = hipGetLastError();

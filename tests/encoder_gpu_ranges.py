@@ -202,3 +202,30 @@ def test_head_norms_of_more_tokens_than_a_launch_has(tr):
     for b, e in ((0, 1 << 24), (1 << 24, 1 << 25), ((1 << 25) - 1001, tokens)):
         part = tr.qk_norm_rotary(q[b:e], k[b:e], None, None, pos[b:e], freq)[0]
         assert torch.equal(got[b:e], part)
+
+
+# ---- clipping: limits and norms whose quotient is none -----------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("out", [False, True])
+def test_clip_limits_of_zero_and_infinity(tr, dtype, out):
+    def clipped(values, max_norm, eps):
+        arrays = [torch.tensor(x, device="cuda").to(TYPES[dtype]) for x in values]
+        outs = [torch.full_like(a, 7.0) for a in arrays] if out else None
+        norm = tr.clip_gradients(arrays, max_norm, out=outs, eps=eps)
+        return float(norm), [a.tolist() for a in (outs or arrays)]
+
+    nan, inf = math.nan, math.inf
+    zeros, ordinary = [[0.0, 0.0, 0.0], [0.0]], [[3.0, 0.0], [4.0]]
+    # zeros have norm 0, which a limit of 0 allows
+    assert clipped(zeros, 0.0, 0.0) == (0.0, zeros)
+    assert clipped(zeros, 0.0, 1e-6) == (0.0, zeros)
+    assert clipped(ordinary, 0.0, 0.0) == (5.0, [[0.0, 0.0], [0.0]])
+    assert clipped(ordinary, 5.0, 0.0) == (5.0, ordinary)
+    assert clipped(ordinary, inf, 0.0) == (5.0, ordinary)
+    # an infinite norm gives zeros, and NaN for the infinite values, whatever the limit
+    for limit in (0.0, 1.0, inf):
+        norm, ((a, b), (c,)) = clipped([[inf, 2.0], [3.0]], limit, 0.0)
+        assert norm == inf and math.isnan(a) and b == 0.0 and c == 0.0
+        norm, got = clipped([[nan, 2.0], [3.0]], limit, 0.0)
+        assert math.isnan(norm) and all(math.isnan(x) for part in got for x in part)

@@ -165,8 +165,9 @@ __global__ __launch_bounds__(256) void k_scale(Batch b, const double *part, int 
     for (int i = threadIdx.x; i < parts; i += 256) s += part[i];
     const double n = sqrt(group_sum(s, lds));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    const double ratio = (double)max_norm / (n + (double)eps);
-    const float c = ratio >= 1. ? 1.f : (float)ratio;  // NaN stays
+    // without the quotients that are none: 0 / 0 is within the limit, and an infinite norm gives zeros whatever the limit
+    const double over = n + (double)eps;
+    const float c = n != n ? NAN : n == INFINITY ? 0.f : over <= max_norm ? 1.f : (float)(max_norm / over);
     each_run(b, [&](const Array &a, uint64_t from, uint64_t count) {
         if (!a.out || (c == 1.f && a.out == a.in)) return;
         if (a.type == VHIP_DTYPE_F32)

@@ -219,13 +219,14 @@ int check_arrays(const vhip_array *arrays, size_t count, bool outputs) {
     uint64_t chunks = 0;
     for (size_t i = 0; i < count; ++i) {
         const vhip_array &a = arrays[i];
-        if (!dtype_known(a.dtype) || (a.out && !dtype_known(a.out_dtype)))
+        const void *out = outputs ? a.out : nullptr;  // the norm alone does not look at them
+        if (!dtype_known(a.dtype) || (out && !dtype_known(a.out_dtype)))
             return set_error(VHIP_ERR_INVALID_CONFIG, "unknown element type of array " + std::to_string(i));
         if (a.count > ((size_t)1 << 40)) return set_error(VHIP_ERR_INVALID_CONFIG, "an array of more than 2^40 values");
-        if (a.count && (!a.data || (outputs && !a.out))) return set_error(VHIP_ERR_INVALID_CONFIG, "array " + std::to_string(i) + " is null");
-        if ((uintptr_t)a.data % dtype_size(a.dtype) || (a.out && (uintptr_t)a.out % dtype_size(a.out_dtype)))
+        if (a.count && (!a.data || (outputs && !out))) return set_error(VHIP_ERR_INVALID_CONFIG, "array " + std::to_string(i) + " is null");
+        if ((uintptr_t)a.data % dtype_size(a.dtype) || (out && (uintptr_t)out % dtype_size(a.out_dtype)))
             return set_error(VHIP_ERR_INVALID_CONFIG, "array " + std::to_string(i) + " is not aligned to its type");
-        if (a.out == a.data && a.out && a.out_dtype != a.dtype)
+        if (out == a.data && out && a.out_dtype != a.dtype)
             return set_error(VHIP_ERR_INVALID_CONFIG, "an array that is scaled in place keeps its type");
         chunks += (a.count + kChunk - 1) / kChunk;
     }

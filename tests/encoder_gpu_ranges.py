@@ -229,3 +229,79 @@ def test_clip_limits_of_zero_and_infinity(tr, dtype, out):
         assert norm == inf and math.isnan(a) and b == 0.0 and c == 0.0
         norm, got = clipped([[nan, 2.0], [3.0]], limit, 0.0)
         assert math.isnan(norm) and all(math.isnan(x) for part in got for x in part)
+
+
+# ---- what out's rounding does to the gradients -------------------------------------------------------------
+
+def offset_case(dtype, lq, lk, heads, dim):
+    """Values and keys far from zero, so that out's rounding is large beside what its gradients are made of: values differ
+    by 1 around 64.2, and keys by 1 around 32, which a row's weights do not see.  Queries and out's gradients do not cancel over rows."""
+    t = TYPES[dtype]
+    q = (0.25 + 0.1 * normal(1, lq, heads, dim)).to(t)
+    k, v = (32 + normal(2, lk, 1, dim)).to(t), (64.2 + normal(3, lk, 1, dim)).to(t)
+    return q, k, v, (normal(4, 1, heads, dim) + 0.05 * normal(5, lq, heads, dim)).to(t)
+
+
+def offset_reference(q, k, v, do, scale):
+    """dq, dk in 64 bits for one sequence both ways, their tolerances where delta's error has been taken off, and what it would leave
+    per unit of it.
+
+    ds~ = (ds - p d) (1 + u), d the error of delta by the rounded out and its rounded weights (2 u of their sizes).  By rows
+    sum ds~ is taken off times sum p~ k: what is left of d is multiplied by what p~ and its sum are off by (u and 32-bit errors),
+    and roundings act on k's distance from its weighted mean.  By keys d is replaced by the 32-bit errors of the sum that finds it."""
+    u, (n, heads, dim), m = UNIT[q.dtype], q.shape, k.shape[0]
+    K, V, a = k[:, 0].double(), v[:, 0].double(), abs(scale)
+    r = {x: torch.zeros(y.shape, dtype=torch.float64, device=q.device) for x, y in (("dq", q), ("dk", k), ("left_q", q), ("left_k", k))}
+    tol = {"dq": r["dq"].clone(), "dk": r["dk"].clone()}
+    for h in range(heads):
+        Q, G = q[:, h].double(), do[:, h].double()
+        s = scale * Q @ K.t()
+        off = (dim + 8) * E * a * (Q.abs() @ K.abs().t())
+        lse = torch.logsumexp(s, 1, keepdim=True)
+        p = torch.exp(s - lse)
+        rel = off + 2 * ((p * off).sum(1, keepdim=True) + (m + 8) * E + 4 * E * lse.abs())
+        o, osize = p @ V, p @ V.abs()
+        d = (2 * u + (p * rel).sum(1, keepdim=True)) * (G.abs() * osize).sum(1, keepdim=True)
+        dp, delta = G @ V.t(), (G * o).sum(1, keepdim=True)
+        ds = p * (dp - delta)
+        big = ds.abs() + p * d
+        edp = (dim + 4) * E * (G.abs() @ V.abs().t() + (G.abs() * osize).sum(1, keepdim=True))
+        each = big * (u + rel + 4 * E) + p * edp
+        sums = d + each.sum(1, keepdim=True) + (m + 8) * E * big.sum(1, keepdim=True)
+        mean = p @ K
+        for j in range(dim):
+            far = (K[:, j][None] - mean[:, j:j + 1]).abs()
+            tol["dq"][:, h, j] = a * ((each * far).sum(1) + (sums * p * (u + rel) * K[:, j].abs()[None]).sum(1)
+                                      + 2 * (m + 8) * E * ((big + sums * p) * K[:, j].abs()[None]).sum(1))
+        r["dq"][:, h] = scale * ds @ K
+        r["left_q"][:, h] = scale * mean
+        found = (p * edp + big * (rel + 4 * E)).sum(1, keepdim=True) + (m + 8) * E * big.sum(1, keepdim=True) + 4 * E * delta.abs()
+        r["dk"][:, 0] += scale * ds.t() @ Q
+        r["left_k"][:, 0] += scale * p.t() @ Q
+        more = (n * heads + 8) * E
+        tol["dk"][:, 0] += a * (ds.abs() * (u + rel + 4 * E + more) + p * (edp + found)).t() @ Q.abs()
+        if q.dtype == torch.float16:  # what its powers of two lose of a row's or key's largest one
+            tol["dq"][:, h] += 2.0 ** -39 * a * big.amax(1, keepdim=True) * K.abs().sum(0)
+            tol["dk"][:, 0] += 2.0 ** -39 * a * big.amax(0)[:, None] * Q.abs().sum(0)
+    tol["dq"] += u * r["dq"].abs() + TINY[q.dtype]
+    tol["dk"] += u * r["dk"].abs() + TINY[q.dtype]
+    return r, tol
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lq,lk", [(64, 64), (20, 1500), (300, 100)])
+def test_the_rounding_of_out_is_taken_off_the_gradients(tr, dtype, lq, lk):
+    """In one workgroup's pass over the keys, and in parts of them (20 rows of 1500 keys)."""
+    print("rounding of out", dtype, lq, lk, flush=True)
+    heads, dim, scale = 2, 64, 0.125
+    q, k, v, do = offset_case(dtype, lq, lk, heads, dim)
+    out, _, dq, dk, _ = attention_both(tr, q, k, v, do, bounds([lq]), bounds([lk]), False, scale)
+    want, tol = offset_reference(q, k, v, do, scale)
+    within(dq, want["dq"], tol["dq"])
+    within(dk, want["dk"], tol["dk"])
+    # left in, or taken off twice or the wrong way, it would pass the tolerance somewhere
+    exact = torch.stack([torch.softmax(scale * q[:, h].double() @ k[:, 0].double().t(), 1) @ v[:, 0].double() for h in range(heads)], 1)
+    delta = (do.double() * (out.double() - exact)).sum(2, keepdim=True)
+    assert ((delta * want["left_q"]).abs() > 2 * tol["dq"]).any()
+    if dtype == "bf16":
+        assert (float(delta.abs().median()) * want["left_k"].abs() > 2 * tol["dk"]).any()

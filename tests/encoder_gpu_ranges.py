@@ -305,3 +305,16 @@ def test_the_rounding_of_out_is_taken_off_the_gradients(tr, dtype, lq, lk):
     assert ((delta * want["left_q"]).abs() > 2 * tol["dq"]).any()
     if dtype == "bf16":
         assert (float(delta.abs().median()) * want["left_k"].abs() > 2 * tol["dk"]).any()
+
+
+def test_arrays_of_other_kinds_among_gradients_are_refused(tr):
+    import numpy as np
+
+    import vector_hip as vh
+
+    g, o = normal(1, 50), normal(2, 50)
+    for other in (g.cpu(), g.to("meta"), np.zeros(50, np.float32), [1.0], None):
+        for call in (lambda: tr.gradient_norm([g, other]), lambda: tr.clip_gradients([g, other], 1.0), lambda: tr.clip_gradients([g, other], 1.0, out=[o, o]),  # noqa: B023
+                     lambda: tr.clip_gradients([g], 1.0, out=[other])):  # noqa: B023
+            with pytest.raises(vh.InvalidConfig):
+                call()

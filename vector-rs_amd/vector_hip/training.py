@@ -458,25 +458,29 @@ def _arrays(gradients, out):
     _on_gpu("a gradient", first)
     device, lib = first.get_device(), _library[type(first.dtype)]
     table = array("Q")  # of vhip_array: data, out, count, and the two types in one
-    if out is None:
-        for g in gradients:
-            if not (getattr(g, "is_cuda", False) and g.get_device() == device):
-                raise InvalidConfig("the gradients are not all on one GPU")
-            if not (g.is_contiguous() or _dense(g)):
-                raise InvalidConfig("the values of a gradient must fill a block of memory")
-            at, code = g.data_ptr(), _code[g.dtype]
-            table.extend((at, at, g.numel(), code | code << 32))
-    else:
-        if len(out) != len(gradients):
-            raise InvalidConfig("out must hold an array for each gradient")
-        for g, o in zip(gradients, out):
-            if not (getattr(g, "is_cuda", False) and getattr(o, "is_cuda", False) and g.get_device() == o.get_device() == device):
-                raise InvalidConfig("the gradients and the outputs are not all on one GPU")
-            if o.shape != g.shape:
-                raise InvalidConfig("an output must have the shape of its gradient")
-            if not (g.is_contiguous() and o.is_contiguous()) and not (_dense(g) and g.stride() == o.stride()):
-                raise InvalidConfig("a gradient and its output must fill blocks of memory in the same order")
-            table.extend((g.data_ptr(), o.data_ptr(), g.numel(), _code[g.dtype] | _code[o.dtype] << 32))
+    # the other arrays are of the first one's kind: an array in host memory has no device number, or -1
+    try:
+        if out is None:
+            for g in gradients:
+                if g.get_device() != device:
+                    raise InvalidConfig("the gradients are not all on one GPU")
+                if not (g.is_contiguous() or _dense(g)):
+                    raise InvalidConfig("the values of a gradient must fill a block of memory")
+                at, code = g.data_ptr(), _code[g.dtype]
+                table.extend((at, at, g.numel(), code | code << 32))
+        else:
+            if len(out) != len(gradients):
+                raise InvalidConfig("out must hold an array for each gradient")
+            for g, o in zip(gradients, out):
+                if not g.get_device() == o.get_device() == device:
+                    raise InvalidConfig("the gradients and the outputs are not all on one GPU")
+                if o.shape != g.shape:
+                    raise InvalidConfig("an output must have the shape of its gradient")
+                if not (g.is_contiguous() and o.is_contiguous()) and not (_dense(g) and g.stride() == o.stride()):
+                    raise InvalidConfig("a gradient and its output must fill blocks of memory in the same order")
+                table.extend((g.data_ptr(), o.data_ptr(), g.numel(), _code[g.dtype] | _code[o.dtype] << 32))
+    except AttributeError:
+        raise InvalidConfig("the gradients and the outputs are not all arrays in GPU memory") from None
     need = _lib.vhip_clip_gradients_workspace(len(gradients))
     return table, len(gradients), first.new_empty((), dtype=lib.f32), first.new_empty(need, dtype=lib.u8), need, device, lib
 

@@ -511,8 +511,9 @@ int vhip_qk_norm_rotary_backward(int ordinal, int dtype, int param_dtype, const 
  *   norm = sqrt(sum g^2),  out = g min(1, max_norm / (norm + eps)),
  * squares and their sum in 64 bits.  The list of arrays is host memory that is read before the call returns; norm (a
  * float of device memory; for vhip_clip_gradients it may be NULL) and the arrays are device memory.  out is data
- * itself, of the same type, or an array of any of the types that overlaps no other.  A norm of infinity gives zeros
- * (and NaN for the infinite values), one of NaN gives NaN. */
+ * itself, of the same type, or an array of any of the types that overlaps no other.  The factor is rounded to 32 bits.  A
+ * norm of infinity gives zeros (and NaN for the infinite values) whatever max_norm is, one of NaN gives NaN; a max_norm of 0
+ * leaves zeros. */
 typedef struct vhip_array {
     const void *data;
     void *out; /* not used by vhip_gradient_norm */

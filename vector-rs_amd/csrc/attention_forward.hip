@@ -10,13 +10,13 @@
 // values' type to be multiplied (half a unit of each); their sum takes them as they were.
 //
 // A causal sequence of 32768 tokens, 32 / 8 heads of 128 in bfloat16: 8.5 ms, 1.03 PFLOP/s, where the library's product of
-// 8192^3 reaches 1.11 to 1.33.  What bounds it is power: the clock is at 1.85 GHz of 2.4, and inputs of zeros take 6.8 ms.  Two
+// 8192^3 reaches 1.11 to 1.33.  What bounds it is power: the clock is at 1.83 GHz of 2.4, and inputs of zeros take 6.8 ms.  Two
 // other arrangements (8 waves in turns, one half multiplying while the other weighs; scores a tile ahead, weights made
 // between products) kept the matrix units busier per cycle or not, at a lower clock: 8.5 to 8.9 ms.  64 columns
 // multiply half as much for the same exponentials: 8 x 4096 tokens, 16 heads, both ways: 0.69 ms, 800 TFLOP/s.
 //
 // Few rows (a single token of each text) take parts of the keys, a workgroup each, and a second kernel joins them: five
-// texts of 67177 keys together 59 us, 4.7 TB/s, and 5 to join.
+// texts of 67177 keys together 56 us, 4.9 TB/s, and 5 to join.
 #include "attention.h"
 
 namespace vh {
